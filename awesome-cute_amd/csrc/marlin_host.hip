@@ -14,6 +14,7 @@
 #include <mutex>
 #include <vector>
 
+#include "../../include/feedforward_amd.h"
 #include "../../include/marlin_amd.h"
 #include "../../include/marlin_amd_tools.h"
 #include "scratch_pool.hpp"
@@ -889,7 +890,7 @@ Planned plans_off_lines(Planned p, PlanCtx cx) {
 // Enqueue the launches of plan pl with the scratch of `view` (null pointers
 // when the plan exchanges nothing through scratch).
 int enqueue(const Plan& pl, const ScratchView& view, const void* A, const void* B, void* C,
-            const void* s, int m, int n, int k, void* workspace, int groupsize, int max_par,
+            const void* s, int m, int n, int k, void* workspace, int groupsize, int max_par, int act,
             hipStream_t stream) {
   // the caller's workspace holds at least n/128 * max_par zero ints
   // (reference marlin_gemm.cpp:29-31, marlin_cute_kernel.cu:68); one counter
@@ -897,6 +898,7 @@ int enqueue(const Plan& pl, const ScratchView& view, const void* A, const void* 
   // only does that when max_par >= 2), and the counters are spread max_par
   // ints apart (64 bytes at the launcher's default of 16)
   const int lock_stride = max_par > 16 ? 16 : max_par;
+  const size_t c_row = (size_t)(act ? n / 2 : n) * 2;  // bytes
   (void)hipGetLastError();  // an earlier call's error is not this launch's
   int rc = MARLIN_OK;
   if (pl.kernel == 3) {
@@ -906,7 +908,7 @@ int enqueue(const Plan& pl, const ScratchView& view, const void* A, const void* 
       GemmArgs a = {};
       a.A = (const char*)A + (size_t)m0 * k * 2;
       a.B = B;
-      a.C = (char*)C + (size_t)m0 * n * 2;
+      a.C = (char*)C + m0 * c_row;
       a.S = s;
       a.M = m - m0 < rows_per_launch ? m - m0 : rows_per_launch;
       a.N = n;
@@ -914,6 +916,7 @@ int enqueue(const Plan& pl, const ScratchView& view, const void* A, const void* 
       a.lock_stride = 1;
       a.row_parts = pl.row_parts;
       a.part_rows = pl.row_parts > 1 ? 16 : 0;
+      a.act = act;
       rc = launch_strip(a, groupsize != -1, pl.strips, stream);
     }
   } else if (pl.kernel == 2) {
@@ -932,6 +935,7 @@ int enqueue(const Plan& pl, const ScratchView& view, const void* A, const void* 
     a.wpt = 0;
     a.row_parts = 1;
     a.part_rows = 0;
+    a.act = act;
     a.finish_polls = t_force.finish_polls < 0 ? kFinishPolls : t_force.finish_polls;
     // tiles of 80 to 128 rows: four waves with accumulators of all rows x 128 columns; 64-row tiles: eight
     // waves with 64 x 64
@@ -944,7 +948,7 @@ int enqueue(const Plan& pl, const ScratchView& view, const void* A, const void* 
       GemmArgs a;
       a.A = (const char*)A + (size_t)m0 * k * 2;
       a.B = B;
-      a.C = (char*)C + (size_t)m0 * n * 2;
+      a.C = (char*)C + m0 * c_row;
       a.S = s;
       a.M = m - m0 < rows_per_launch ? m - m0 : rows_per_launch;
       a.N = n;
@@ -956,6 +960,7 @@ int enqueue(const Plan& pl, const ScratchView& view, const void* A, const void* 
       a.wpt = pl.sp.wpt;
       a.row_parts = pl.row_parts;
       a.part_rows = pl.part_rows;
+      a.act = act;
       rc = launch_stream(a, groupsize != -1, pl.grid, stream);
     }
   }
@@ -964,7 +969,7 @@ int enqueue(const Plan& pl, const ScratchView& view, const void* A, const void* 
 }
 
 int enqueue_rows(const RowsPlan& rows, const void* A, const void* B, void* C, const void* s, int m,
-                 int n, int k, int groupsize, hipStream_t stream) {
+                 int n, int k, int groupsize, int act, hipStream_t stream) {
   (void)hipGetLastError();  // an earlier call's error is not this launch's
   GemmArgs a = {};
   a.A = A;
@@ -974,6 +979,7 @@ int enqueue_rows(const RowsPlan& rows, const void* A, const void* B, void* C, co
   a.M = m;
   a.N = n;
   a.K = k;
+  a.act = act;
   const int rc = launch_rows(a, groupsize != -1, rows.strips, rows.blocks, stream);
   if (rc == MARLIN_ERR_RUNTIME) set_error(w4a16::last_launch_error(), "kernel launch");
   return rc;
@@ -998,10 +1004,11 @@ unsigned char* static_scratch_for(int dev) {
 }
 
 // use_static: marlin_gemm_static -- the fixed array instead of the pool, a
-// plan made for its size, and no allocation on any path.
+// plan made for its size, and no allocation on any path.  act: the product's columns
+// are pairs of a gated projection, and C holds n / 2 of them.
 int run(const void* A, const void* B, void* C, const void* s, int m, int n, int k,
         void* workspace, int groupsize, int dev, hipStream_t stream, int thread_k, int thread_n,
-        int sms, int max_par, bool use_static) {
+        int sms, int max_par, bool use_static, int act = kActNone) {
   int rc = check_shape(m, n, k, groupsize, thread_k, thread_n);
   if (rc != MARLIN_OK || m == 0 || n == 0 || k == 0) return rc;
   if (max_par < 1) {
@@ -1080,9 +1087,9 @@ int run(const void* A, const void* B, void* C, const void* s, int m, int n, int 
     // (with the plan's scratch in hand: what a stream must have seen before it can be
     // captured does not depend on a choice that is a matter of speed)
     if (ok && planned.rows.strips > 0)
-      rc = enqueue_rows(planned.rows, A, B, C, s, m, n, k, groupsize, stream);
+      rc = enqueue_rows(planned.rows, A, B, C, s, m, n, k, groupsize, act, stream);
     else if (ok)
-      rc = enqueue(pl, view, A, B, C, s, m, n, k, workspace, groupsize, max_par, stream);
+      rc = enqueue(pl, view, A, B, C, s, m, n, k, workspace, groupsize, max_par, act, stream);
   }
   if (prev != dev) (void)hipSetDevice(prev);
   return rc;
@@ -1152,6 +1159,37 @@ int marlin_mul(const void* A, const void* B, void* C, const void* s, int prob_m,
                 thread_k, thread_n, groupsize);
   if (rc == MARLIN_ERR_RUNTIME) return fail(rc, "HIP runtime error: %s", g_last_error);
   if (rc != MARLIN_OK) return fail(rc, "%s", g_last_error);
+  return rc;
+}
+
+int feedforward_gated_w4(const void* A, const void* B, void* C, const void* s, int prob_m, int prob_n,
+                 int prob_k, int s_rows, void* workspace, long long workspace_numel, int activation,
+                 int dev, void* stream, int max_par, char* err, int err_len) {
+  auto fail = [&](int code, const char* fmt, auto... args) {
+    if (err && err_len > 0) snprintf(err, (size_t)err_len, fmt, args...);
+    return code;
+  };
+  if (err && err_len > 0) err[0] = 0;
+  if (!act_known(activation)) return fail(MARLIN_ERR_KERN_SHAPE, "unknown activation %d.", activation);
+  // (the product has twice C's columns)
+  if (prob_m < 0 || prob_n < 0 || prob_k < 0 || prob_n > 0x3fffffff || prob_n % 128 != 0 || prob_k % 128 != 0)
+    return fail(MARLIN_ERR_PROB_SHAPE, "Gated problem (m=%d, n=%d, k=%d): n and k must be multiples of 128.",
+                prob_m, prob_n, prob_k);
+  if (s_rows <= 0) return fail(MARLIN_ERR_GROUPS, "k=%d not compatible with %d groups.", prob_k, s_rows);
+  const int groupsize = s_rows == 1 ? -1 : prob_k / s_rows;
+  if (groupsize != -1 && groupsize * s_rows != prob_k)
+    return fail(MARLIN_ERR_GROUPS, "k=%d not compatible with %d groups.", prob_k, s_rows);
+  if (groupsize != -1 && groupsize != 128)
+    return fail(MARLIN_ERR_KERN_SHAPE, "No kernel implementation for groupsize=%d.", groupsize);
+  if (max_par < 1 || workspace_numel < (long long)(2 * prob_n / 128) * max_par)
+    return fail(MARLIN_ERR_WORKSPACE, "workspace must be of size at least %lld.",
+                (long long)(2 * prob_n / 128) * (max_par < 1 ? 1 : max_par));
+  if (prob_k == 0 && prob_m > 0 && prob_n > 0)
+    return fail(MARLIN_ERR_PROB_SHAPE, "Gated problem (m=%d, n=%d, k=0): an empty sum.", prob_m, prob_n);
+  const int rc = run(A, B, C, s, prob_m, 2 * prob_n, prob_k, workspace, groupsize, dev,
+                     (hipStream_t)stream, -1, -1, -1, max_par, false, activation);
+  if (rc == MARLIN_ERR_RUNTIME) return fail(rc, "HIP runtime error: %s", g_last_error);
+  if (rc != MARLIN_OK) return fail(rc, "Gated problem (m=%d, n=%d, k=%d) is not supported.", prob_m, prob_n, prob_k);
   return rc;
 }
 

@@ -21,6 +21,7 @@
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 
+#include "../../include/feedforward_amd.h"
 #include "../../include/marlin_amd.h"
 #include "../../include/marlin_amd_convert.h"
 #include "../../include/streamk_amd.h"
@@ -146,6 +147,97 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const at::Tensor* const t[kMulTensors] = {A, B, &C, s, workspace};
   if (!check_mul(t)) return nullptr;
   if (!enqueue_mul(*A, *B, C, *s, *workspace, A->numel() / k, n, k, h)) return nullptr;
+  return THPVariable_Wrap(std::move(C));
+  END_HANDLE_TH_ERRORS
+}
+
+// The operands of a gated projection with 4-bit weights: A (rows, k), B (k/16, 4n), C (rows, n),
+// s (groups, 2n); false with an exception set.
+bool enqueue_gated(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, const at::Tensor& s,
+                   const at::Tensor& workspace, int act, int max_par) {
+  const at::Tensor* const t[kMulTensors] = {&A, &B, &C, &s, &workspace};
+  if (!check_mul(t)) return false;
+  for (int i = 0; i < kMulTensors; i++) {
+    const bool whole = i == 1 || i == 4;
+    if (t[i]->scalar_type() != (whole ? at::kInt : at::kHalf)) {
+      PyErr_Format(PyExc_ValueError, "%s must be of type torch.%s", kMulNames[i], whole ? "int32" : "half");
+      return false;
+    }
+    if (t[i]->device() != A.device()) {
+      PyErr_Format(PyExc_ValueError, "%s must be on A's device", kMulNames[i]);
+      return false;
+    }
+  }
+  constexpr int64_t most = 0x7fffffff;
+  if (A.dim() != 2 || B.dim() != 2 || C.dim() != 2 || s.dim() != 2 || A.size(0) != C.size(0) ||
+      A.size(0) > most || A.size(1) > most || C.size(1) > most / 2 || s.size(0) > most ||
+      B.size(0) != A.size(1) / 16 || B.size(1) != 4 * C.size(1) || s.size(1) != 2 * C.size(1)) {
+    PyErr_SetString(PyExc_ValueError,
+                    "a gated product takes A (m, k), B (k/16, 4n), C (m, n) and s (groups, 2n)");
+    return false;
+  }
+  const int dev = A.get_device();
+  char err[512];
+  int rc;
+  void* const st = current_stream(dev);
+  const void *pa = A.data_ptr(), *pb = B.data_ptr(), *ps = s.data_ptr();
+  void *pc = C.data_ptr(), *pw = workspace.data_ptr();
+  const int m = (int)A.size(0), n = (int)C.size(1), k = (int)A.size(1), groups = (int)s.size(0);
+  const long long ws = workspace.numel();
+  Py_BEGIN_ALLOW_THREADS
+  rc = feedforward_gated_w4(pa, pb, pc, ps, m, n, k, groups, pw, ws, act, dev, st, max_par, err, sizeof(err));
+  Py_END_ALLOW_THREADS
+  if (rc == 0) return true;
+  PyErr_SetString(PyExc_RuntimeError, err);
+  return false;
+}
+
+// gated_mul(A, B, C, s, workspace, activation, max_par)
+PyObject* py_gated_mul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7) {
+    PyErr_SetString(PyExc_TypeError, "gated_mul takes 7 arguments");
+    return nullptr;
+  }
+  const at::Tensor* t[kMulTensors];
+  for (int i = 0; i < kMulTensors; i++)
+    if (!(t[i] = tensor(args[i], kMulNames[i]))) return nullptr;
+  int act, max_par;
+  if (!to_int(args[5], &act) || !to_int(args[6], &max_par)) return nullptr;
+  if (!enqueue_gated(*t[0], *t[1], *t[2], *t[3], *t[4], act, max_par)) return nullptr;
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_linear(A, B, s, workspace, activation) -> C, rows of any shape
+PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5) {
+    PyErr_SetString(PyExc_TypeError, "gated_linear takes 5 arguments");
+    return nullptr;
+  }
+  const at::Tensor *A = tensor(args[0], "A"), *B = tensor(args[1], "B"), *s = tensor(args[2], "s"),
+                   *workspace = tensor(args[3], "workspace");
+  if (!A || !B || !s || !workspace) return nullptr;
+  int act;
+  if (!to_int(args[4], &act)) return nullptr;
+  if (A->dim() < 1 || s->dim() != 2 || s->size(1) % 2 != 0 || A->size(-1) == 0) {
+    PyErr_SetString(PyExc_ValueError, "A needs a last dimension, s two and an even number of columns");
+    return nullptr;
+  }
+  const int64_t n = s->size(1) / 2, k = A->size(-1);
+  c10::SmallVector<int64_t, 6> shape(A->sizes().begin(), A->sizes().end());
+  shape.back() = n;
+  at::Tensor C, rows, out;
+  {
+    pybind11::gil_scoped_release unlocked;
+    C = at::empty(shape, A->options().requires_grad(false).memory_format(c10::nullopt));
+    // (a copy where the leading dimensions do not fold into one)
+    rows = A->reshape({-1, k});
+    if (!rows.is_contiguous()) rows = rows.contiguous();
+    out = C.view({rows.size(0), n});
+  }
+  if (!enqueue_gated(rows, *B, out, *s, *workspace, act, 16)) return nullptr;
   return THPVariable_Wrap(std::move(C));
   END_HANDLE_TH_ERRORS
 }
@@ -341,6 +433,8 @@ PyObject* py_pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {
     {"mul", (PyCFunction)(void (*)(void))py_mul, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void (*)(void))py_linear, METH_FASTCALL, nullptr},
+    {"gated_mul", (PyCFunction)(void (*)(void))py_gated_mul, METH_FASTCALL, nullptr},
+    {"gated_linear", (PyCFunction)(void (*)(void))py_gated_linear, METH_FASTCALL, nullptr},
     {"quantize", (PyCFunction)(void (*)(void))py_quantize, METH_FASTCALL, nullptr},
     {"pack", (PyCFunction)(void (*)(void))py_pack, METH_FASTCALL, nullptr},
     {"dense", (PyCFunction)(void (*)(void))py_dense, METH_FASTCALL, nullptr},

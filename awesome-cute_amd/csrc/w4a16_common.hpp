@@ -22,6 +22,8 @@
 
 #include <type_traits>
 
+#include "gated_act.hpp"
+
 namespace w4a16 {
 
 typedef _Float16 half_t;
@@ -183,7 +185,17 @@ struct GemmArgs {
                     // (launch_rows sets it)
   int part_rows;    // rows of a part: 16 or 32 (streaming and column-strip kernels)
   int finish_polls; // prefill kernels: looks at a tile's other slices before leaving them a share
+  // kActNone, or the activation of a gated projection: of every 16 columns of the product the
+  // first eight are gates and the others, eight further on, their partners, so that a lane of
+  // any kernel here holds both, and C is (M, N/2): act(gate) partner, in fp32, rounded once.
+  // Every kernel that ends in C has a form for it (GATED), since the two sums are in hand
+  // there: the product written out, and read again by a kernel for the activation, would cost
+  // a launch of few rows 3 us and more, a prompt a tenth.
+  int act = kActNone;
 };
+
+// the column of C that column `col` of the product, a gate, becomes part of
+__host__ __device__ __forceinline__ int gated_col(int col) { return ((col >> 4) << 3) + (col & 7); }
 
 // bytes of fp32 partial sums of mb row blocks of 16 (one slot)
 constexpr size_t stream_slot_bytes(int mb) { return (size_t)mb * 4 * 2 * 64 * 16; }

@@ -59,7 +59,7 @@ struct PfShape {
 
 }  // namespace
 
-template <bool GROUP, int RB>
+template <bool GROUP, int RB, bool GATED>
 __global__ __launch_bounds__(512) void prefill_kernel(GemmArgs p, int tiles_m, int tiles_n,
                                                       int ksplit) {
   extern __shared__ __attribute__((aligned(16))) char smem_all[];  // PfShape<RB>::kLdsBytes
@@ -511,6 +511,50 @@ __global__ __launch_bounds__(512) void prefill_kernel(GemmArgs p, int tiles_m, i
   // consecutive columns.
   constexpr int kPitch = kPfTileN * 2 + 16;  // bytes per tile row in LDS
   const int q = lane >> 4;
+  if constexpr (GATED) {
+    // half as many columns: (j2, h = 0), gates, and (j2, h = 1) become four columns of C
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const int nloc = 128 * pr + 64 * (q >> 1) + 16 * (2 * jp + (j >> 1)) + 4 * (q & 1);
+      f4 sg, su;
+      if constexpr (!GROUP) {
+        const half_t* S = (const half_t*)p.S;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          sg[r] = (float)S[scale_index_single(kPfTileN * tn + nloc + r)];
+          su[r] = (float)S[scale_index_single(kPfTileN * tn + nloc + 8 + r)];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < HB; i++) {
+        const int m = 16 * row_block(own + i) + nu;
+        h4 o;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          float gate = fin[i][j][r], up = fin[i][j + 1][r];
+          if constexpr (!GROUP) {
+            gate *= sg[r];
+            up *= su[r];
+          }
+          o[r] = (half_t)act_mul(gate, up, p.act);
+        }
+        *(h4*)(smem_all + m * kPitch + gated_col(nloc) * 2) = o;
+      }
+    }
+    __syncthreads();
+    half_t* C = (half_t*)p.C;
+#pragma unroll
+    for (int it = 0; it < kPfTileM / 32; it++) {
+      const int piece = it * 512 + (int)threadIdx.x;
+      const int m = piece >> 4;
+      const int c16 = piece & 15;
+      if (m < rows) {
+        const i4 v = *(const i4*)(smem_all + m * kPitch + c16 * 16);
+        __builtin_nontemporal_store(v, (i4*)(C + (size_t)(m0 + m) * (p.N >> 1) + kPfTileN / 2 * tn + c16 * 8));
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     const int nloc = 128 * pr + 64 * (q >> 1) + 16 * (2 * jp + (j >> 1)) + 8 * (j & 1) + 4 * (q & 1);
@@ -548,12 +592,13 @@ template <int RB>
 static int configure_rb() {
   // more LDS than the default per-workgroup limit: opt in per kernel and device
   constexpr int lds = PfShape<RB>::kLdsBytes;
-  if (hipFuncSetAttribute((const void*)prefill_kernel<true, RB>,
-                          hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess ||
-      hipFuncSetAttribute((const void*)prefill_kernel<false, RB>,
-                          hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
-    return 3;
-  return 0;
+  const auto raise = [](auto kernel) {
+    return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
+  };
+  return raise(prefill_kernel<true, RB, false>) && raise(prefill_kernel<false, RB, false>) &&
+                 raise(prefill_kernel<true, RB, true>) && raise(prefill_kernel<false, RB, true>)
+             ? 0
+             : 3;
 }
 
 int configure_prefill_kernels() { return configure_rb<4>() ? 3 : 0; }
@@ -563,8 +608,10 @@ static void launch_rb(const GemmArgs& a, int ksplit, hipStream_t stream) {
   const int tiles_m = ceil_div(a.M, PfShape<RB>::kTileM);
   const int tiles_n = a.N / kPfTileN;
   constexpr int lds = PfShape<RB>::kLdsBytes;
-  hipLaunchKernelGGL((prefill_kernel<GROUP, RB>), dim3(tiles_m * tiles_n * ksplit), dim3(512), lds,
-                     stream, a, tiles_m, tiles_n, ksplit);
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(tiles_m * tiles_n * ksplit), dim3(512), lds, stream, a, tiles_m, tiles_n, ksplit);
+  };
+  a.act ? launch(prefill_kernel<GROUP, RB, true>) : launch(prefill_kernel<GROUP, RB, false>);
 }
 
 int launch_prefill(const GemmArgs& a, bool group, int ksplit, hipStream_t stream) {

@@ -75,7 +75,7 @@ struct WdShape {
 // tiles: in one kernel for both, the sums of a whole tile took moves and tests
 // on the way out (M = 3614, N = 6656, K = 1280 with one scale per column 58.0
 // -> 59.3 us).
-template <bool GROUP, int RB, bool SLICED>
+template <bool GROUP, int RB, bool SLICED, bool GATED>
 __global__ __launch_bounds__(256) void prefill_wide_kernel(GemmArgs p, int tiles_m, int tiles_n,
                                                            int ksplit) {
   extern __shared__ __attribute__((aligned(16))) char smem_all[];  // Shape::kLdsBytes
@@ -295,6 +295,53 @@ __global__ __launch_bounds__(256) void prefill_wide_kernel(GemmArgs p, int tiles
   // (j, h), the four consecutive columns 64(q/2) + 16j + 8h + 4(q%2) + r of its
   // wave's 128, q = lane/16.
   const int q = lane >> 4;
+  if constexpr (GATED) {
+    // half as many columns: operands 2j (gates) and 2j + 1 become four columns of C
+#pragma unroll
+    for (int o = 0; o < 8; o += 2) {
+      const int nloc = 128 * nw + 64 * (q >> 1) + 16 * (o >> 1) + 4 * (q & 1);
+      f4 sg, su;
+      if constexpr (!GROUP) {
+        const half_t* S = (const half_t*)p.S;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          sg[r] = (float)S[scale_index_single(kWdTileN * tn + nloc + r)];
+          su[r] = (float)S[scale_index_single(kWdTileN * tn + nloc + 8 + r)];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < HB; i++) {
+        if ((RB & 1) && own + i >= RB) continue;
+        if (SLICED && !(pieces >> (2 * i + (o >> 2)) & 1)) continue;
+        h4 v;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          float gate = fin[i][o][r], up = fin[i][o + 1][r];
+          if constexpr (!GROUP) {
+            gate *= sg[r];
+            up *= su[r];
+          }
+          v[r] = (half_t)act_mul(gate, up, p.act);
+        }
+        *(h4*)(smem_all + (16 * (own + i) + nu) * kWdPitch + gated_col(nloc) * 2) = v;
+      }
+    }
+    __syncthreads();
+    half_t* C = (half_t*)p.C;
+#pragma unroll
+    for (int it = 0; it < kWdTileM / 16; it++) {
+      const int piece = it * 256 + (int)threadIdx.x;
+      const int m = piece >> 4;
+      const int c16 = piece & 15;
+      const int i = m >= 16 * HB ? (m >> 4) - HB : m >> 4;
+      if (m < rows && (!SLICED || (pieces >> (2 * i + ((c16 >> 1) & 1)) & 1))) {
+        const i4 v = *(const i4*)(smem_all + m * kWdPitch + c16 * 16);
+        __builtin_nontemporal_store(v, (i4*)(C + (size_t)(m0 + m) * (p.N >> 1) + kWdTileN / 2 * tn + c16 * 8));
+      }
+    }
+    if (SLICED && threadIdx.x == 0) finish_leave(&p.locks[tile * p.lock_stride], ksplit);
+    return;
+  }
 #pragma unroll
   for (int o = 0; o < 8; o++) {
     const int nloc = 128 * nw + 64 * (q >> 1) + 16 * (o >> 1) + 8 * (o & 1) + 4 * (q & 1);
@@ -336,10 +383,11 @@ __global__ __launch_bounds__(256) void prefill_wide_kernel(GemmArgs p, int tiles
 template <bool GROUP, int RB>
 static int configure_wide() {
   constexpr int lds = WdShape<RB>::kLdsBytes;
-  return hipFuncSetAttribute((const void*)prefill_wide_kernel<GROUP, RB, false>,
-                             hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess ||
-         hipFuncSetAttribute((const void*)prefill_wide_kernel<GROUP, RB, true>,
-                             hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess;
+  const auto raise = [](auto kernel) {
+    return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess;
+  };
+  return raise(prefill_wide_kernel<GROUP, RB, false, false>) || raise(prefill_wide_kernel<GROUP, RB, true, false>) ||
+         raise(prefill_wide_kernel<GROUP, RB, false, true>) || raise(prefill_wide_kernel<GROUP, RB, true, true>);
 }
 int configure_prefill_wide_kernels() {
   return configure_wide<false, 5>() | configure_wide<false, 6>() | configure_wide<false, 7>() |
@@ -355,12 +403,13 @@ static int launch_wide(const GemmArgs& a, int ksplit, hipStream_t stream) {
   const int tiles_m = ceil_div(a.M, 16 * RB);
   const int tiles_n = a.N / kWdTileN;
   const dim3 grid(tiles_m * tiles_n * ksplit);
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, a, tiles_m, tiles_n, ksplit > 1 ? ksplit : 1);
+  };
   if (ksplit > 1)
-    hipLaunchKernelGGL((prefill_wide_kernel<GROUP, RB, true>), grid, dim3(256), lds, stream, a,
-                       tiles_m, tiles_n, ksplit);
+    a.act ? launch(prefill_wide_kernel<GROUP, RB, true, true>) : launch(prefill_wide_kernel<GROUP, RB, true, false>);
   else
-    hipLaunchKernelGGL((prefill_wide_kernel<GROUP, RB, false>), grid, dim3(256), lds, stream, a,
-                       tiles_m, tiles_n, 1);
+    a.act ? launch(prefill_wide_kernel<GROUP, RB, false, true>) : launch(prefill_wide_kernel<GROUP, RB, false, false>);
   return launch_status();
 }
 

@@ -80,7 +80,7 @@ struct RowsShape {
 };
 
 // ONCE: the weights are requested as read once, where one workgroup reads them (launch_rows)
-template <int CS, int MB, bool GROUP, int DEPTH, int UNITS, bool ONCE>
+template <int CS, int MB, bool GROUP, int DEPTH, int UNITS, bool ONCE, bool GATED>
 __global__ __launch_bounds__(64 * kRowsWaves) void rows_kernel(GemmArgs p) {
   using Sh = RowsShape<CS, MB, DEPTH, UNITS>;
   constexpr int NA = Sh::kALoads, NB = Sh::kBLoads, NS = GROUP ? CS : 0;
@@ -329,6 +329,23 @@ __global__ __launch_bounds__(64 * kRowsWaves) void rows_kernel(GemmArgs p) {
       // The lanes of both e, 32 apart, exchange halves and store two columns at a time.
       const int col = 64 * (strip >> 2) + 2 * (strip & 3) + 32 * (kg & 1);
       const int e = kg >> 1;
+      if constexpr (GATED) {
+        unsigned o[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float gate = v[2 * h], up = v[2 * h + 1];
+          if constexpr (!GROUP) {
+            gate *= (float)__builtin_bit_cast(half_t, chan[ps][i][2 * h]);
+            up *= (float)__builtin_bit_cast(half_t, chan[ps][i][2 * h + 1]);
+          }
+          o[h] = __builtin_bit_cast(unsigned short, (half_t)act_mul(gate, up, p.act));
+        }
+        const unsigned got = __shfl_xor((int)(e ? o[0] : o[1]), 32);
+        if (row < p.M)
+          *(unsigned*)((half_t*)p.C + (size_t)row * (p.N >> 1) + gated_col(col) + 8 * e) =
+              e ? got | (o[1] << 16) : o[0] | (got << 16);
+        continue;
+      }
       unsigned o[4];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
@@ -350,15 +367,17 @@ namespace {
 
 // calls f(kernel, LDS bytes) for a set of strips and rows that exists
 template <class F>
-bool with_rows_kernel(int strips, int blocks, bool group, bool once, F f) {
+bool with_rows_kernel(int strips, int blocks, bool group, bool once, bool gated, F f) {
 #define ROWS(CS, MB, DEPTH, UNITS, GROUP)                                               \
   if (strips == CS && blocks == MB && group == GROUP) {                               \
     using Sh = RowsShape<CS, MB, DEPTH, UNITS>;                                       \
     static_assert(Sh::kLds <= 160 * 1024, "LDS of a compute unit");                   \
     if (once)                                                                         \
-      f(rows_kernel<CS, MB, GROUP, DEPTH, UNITS, true>, Sh::kLds);                    \
+      f(gated ? rows_kernel<CS, MB, GROUP, DEPTH, UNITS, true, true>                  \
+              : rows_kernel<CS, MB, GROUP, DEPTH, UNITS, true, false>, Sh::kLds);     \
     else                                                                              \
-      f(rows_kernel<CS, MB, GROUP, DEPTH, UNITS, false>, Sh::kLds);                   \
+      f(gated ? rows_kernel<CS, MB, GROUP, DEPTH, UNITS, false, true>                 \
+              : rows_kernel<CS, MB, GROUP, DEPTH, UNITS, false, false>, Sh::kLds);    \
     return true;                                                                      \
   }
 #define ROWS_OF_BOTH(CS, MB, DEPTH, UNITS) ROWS(CS, MB, DEPTH, UNITS, true) ROWS(CS, MB, DEPTH, UNITS, false)
@@ -386,7 +405,7 @@ bool with_rows_kernel(int strips, int blocks, bool group, bool once, F f) {
 }  // namespace
 
 bool rows_exist(int strips, int blocks, bool group) {
-  return strips == 8 ? rows_wide_exist(blocks) : with_rows_kernel(strips, blocks, group, true, [](auto, int) {});
+  return strips == 8 ? rows_wide_exist(blocks) : with_rows_kernel(strips, blocks, group, true, false, [](auto, int) {});
 }
 
 int configure_rows_kernels() {
@@ -395,10 +414,11 @@ int configure_rows_kernels() {
     for (int blocks = 1; blocks <= kRowsMaxBlocks; blocks++)
       for (const bool group : {false, true})
         for (const bool once : {false, true})
-          with_rows_kernel(strips, blocks, group, once, [&](auto kernel, int lds) {
-            ok = ok && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           lds) == hipSuccess;
-          });
+          for (const bool gated : {false, true})
+            with_rows_kernel(strips, blocks, group, once, gated, [&](auto kernel, int lds) {
+              ok = ok && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             lds) == hipSuccess;
+            });
   return ok ? 0 : 3;
 }
 
@@ -407,7 +427,7 @@ int launch_rows(const GemmArgs& a, bool group, int strips, int blocks, hipStream
   GemmArgs b = a;
   b.row_parts = ceil_div(a.M, 16 * blocks);
   b.gpb = ceil_div(a.N / 16, strips) * b.row_parts;
-  const bool found = with_rows_kernel(strips, blocks, group, b.row_parts == 1, [&](auto kernel, int lds) {
+  const bool found = with_rows_kernel(strips, blocks, group, b.row_parts == 1, b.act != kActNone, [&](auto kernel, int lds) {
     hipLaunchKernelGGL(kernel, dim3(b.gpb), dim3(64 * kRowsWaves), lds, stream, b);
   });
   return found ? launch_status() : 2;

@@ -42,12 +42,63 @@ struct WideShape {
 };
 
 // the waves' sums meet, a block of 16 slots x 16 rows to a wave, and C is written
-template <int MB, bool GROUP>
+template <int MB, bool GROUP, bool GATED>
 __device__ __forceinline__ void wide_finish(const GemmArgs& p, char* smem, const f4 (&acc)[8][MB],
                                             const __amdgpu_buffer_rsrc_t rS, int set, int row0, int wave, int lane) {
   using Sh = WideShape<MB>;
   const int kg = lane >> 4, nu = lane & 15;
   f4* const red = (f4*)smem;
+  if constexpr (GATED) {
+    // the same in pairs, a gate's block 2j and its partner's 2j + 1 of the same rows to a
+    // wave: a pass is whole pairs, eight at most
+    constexpr int kPairs = Sh::kPass / 2;
+    static_assert(kPairs <= kWaves && Sh::kPass % (2 * MB) == 0, "");
+#pragma unroll
+    for (int ps = 0; ps < Sh::kPasses; ps++) {
+      const int b0 = ps * Sh::kPass;
+      const int j = ps * (kPairs / MB) + wave / MB, m = wave % MB;
+      const int col = 128 * set + 64 * (kg >> 1) + 4 * (kg & 1) + 16 * j;  // of the gates
+      const bool mine = wave < kPairs;
+      h4 chan[2] = {};
+      if constexpr (!GROUP) {
+        if (mine) {
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              chan[h][r] = __builtin_bit_cast(half_t, __builtin_amdgcn_raw_buffer_load_b16(
+                                                          rS, 2 * scale_index_single(col + 8 * h + r), 0, 0));
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int b = b0; b < b0 + Sh::kPass; b++) red[(rows_run(wave) * Sh::kPass + b - b0) * 64 + lane] = acc[b / MB][b % MB];
+      __syncthreads();
+      if (mine) {
+        f4 v[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int b = (2 * j + h) * MB + m - b0;
+          v[h] = red[b * 64 + lane];
+#pragma unroll
+          for (int w = 1; w < kWaves; w++) v[h] += red[(w * Sh::kPass + b) * 64 + lane];
+        }
+        h4 o;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          float gate = v[0][r], up = v[1][r];
+          if constexpr (!GROUP) {
+            gate *= (float)chan[0][r];
+            up *= (float)chan[1][r];
+          }
+          o[r] = (half_t)act_mul(gate, up, p.act);
+        }
+        const int row = row0 + 16 * m + nu;
+        if (row < p.M) *(h4*)((half_t*)p.C + (size_t)row * (p.N >> 1) + gated_col(col)) = o;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int ps = 0; ps < Sh::kPasses; ps++) {
     const int b0 = ps * Sh::kPass;
@@ -129,7 +180,7 @@ struct WideLane {
 
 }  // namespace
 
-template <int MB, bool GROUP>
+template <int MB, bool GROUP, bool GATED>
 __global__ __launch_bounds__(64 * kWaves) void rows_wide_kernel(GemmArgs p) {
   using Sh = WideShape<MB>;
   constexpr int NA = 2 * MB;
@@ -231,12 +282,12 @@ __global__ __launch_bounds__(64 * kWaves) void rows_wide_kernel(GemmArgs p) {
   // nothing may still be on its way into LDS when it is reused
   __builtin_amdgcn_s_waitcnt(0);
 
-  wide_finish<MB, GROUP>(p, smem, acc, rS, me.set, me.row0, me.wave, me.lane);
+  wide_finish<MB, GROUP, GATED>(p, smem, acc, rS, me.set, me.row0, me.wave, me.lane);
 }
 
 // The same over a deep k range, with the loop that gen_rows_wide.py writes: weights requested
 // three chunks ahead, activations two.
-template <int MB, bool GROUP>
+template <int MB, bool GROUP, bool GATED>
 __global__ __launch_bounds__(64 * kWaves) void rows_deep_kernel(GemmArgs p) {
   constexpr int kSlot = 8192;  // activations of a chunk, slots swapped by an exclusive or
   extern __shared__ __attribute__((aligned(16))) char smem[];  // kDeepLds
@@ -274,24 +325,24 @@ __global__ __launch_bounds__(64 * kWaves) void rows_deep_kernel(GemmArgs p) {
   __amdgpu_buffer_rsrc_t rS = make_rsrc(p.S, (unsigned)(GROUP ? p.K / 128 : 1) * (unsigned)p.N * 2u);
   // (the lane once more, so that no register is held through the statement, which leaves six)
   const int again = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
-  wide_finish<MB, GROUP>(p, smem, acc, rS, me.set, me.row0, me.wave, again);
+  wide_finish<MB, GROUP, GATED>(p, smem, acc, rS, me.set, me.row0, me.wave, again);
 }
 
 namespace {
 
 template <class F>
-bool with_wide_kernel(int blocks, bool group, bool deep, F f) {
+bool with_wide_kernel(int blocks, bool group, bool deep, bool gated, F f) {
   switch ((deep ? 100 : 0) + 2 * blocks + (group ? 1 : 0)) {
-    case 106: f(rows_deep_kernel<3, false>, kDeepLds); return true;
-    case 107: f(rows_deep_kernel<3, true>, kDeepLds); return true;
-    case 108: f(rows_deep_kernel<4, false>, kDeepLds); return true;
-    case 109: f(rows_deep_kernel<4, true>, kDeepLds); return true;
-    case 4: f(rows_wide_kernel<2, false>, WideShape<2>::kLds); return true;
-    case 5: f(rows_wide_kernel<2, true>, WideShape<2>::kLds); return true;
-    case 6: f(rows_wide_kernel<3, false>, WideShape<3>::kLds); return true;
-    case 7: f(rows_wide_kernel<3, true>, WideShape<3>::kLds); return true;
-    case 8: f(rows_wide_kernel<4, false>, WideShape<4>::kLds); return true;
-    case 9: f(rows_wide_kernel<4, true>, WideShape<4>::kLds); return true;
+    case 106: f(gated ? rows_deep_kernel<3, false, true> : rows_deep_kernel<3, false, false>, kDeepLds); return true;
+    case 107: f(gated ? rows_deep_kernel<3, true, true> : rows_deep_kernel<3, true, false>, kDeepLds); return true;
+    case 108: f(gated ? rows_deep_kernel<4, false, true> : rows_deep_kernel<4, false, false>, kDeepLds); return true;
+    case 109: f(gated ? rows_deep_kernel<4, true, true> : rows_deep_kernel<4, true, false>, kDeepLds); return true;
+    case 4: f(gated ? rows_wide_kernel<2, false, true> : rows_wide_kernel<2, false, false>, WideShape<2>::kLds); return true;
+    case 5: f(gated ? rows_wide_kernel<2, true, true> : rows_wide_kernel<2, true, false>, WideShape<2>::kLds); return true;
+    case 6: f(gated ? rows_wide_kernel<3, false, true> : rows_wide_kernel<3, false, false>, WideShape<3>::kLds); return true;
+    case 7: f(gated ? rows_wide_kernel<3, true, true> : rows_wide_kernel<3, true, false>, WideShape<3>::kLds); return true;
+    case 8: f(gated ? rows_wide_kernel<4, false, true> : rows_wide_kernel<4, false, false>, WideShape<4>::kLds); return true;
+    case 9: f(gated ? rows_wide_kernel<4, true, true> : rows_wide_kernel<4, true, false>, WideShape<4>::kLds); return true;
   }
   return false;
 }
@@ -299,7 +350,7 @@ bool with_wide_kernel(int blocks, bool group, bool deep, F f) {
 }  // namespace
 
 bool rows_wide_exist(int blocks) {
-  return with_wide_kernel(blocks, true, false, [](auto, int) {});
+  return with_wide_kernel(blocks, true, false, false, [](auto, int) {});
 }
 
 int configure_rows_wide_kernels() {
@@ -307,10 +358,11 @@ int configure_rows_wide_kernels() {
   for (int blocks = 1; blocks <= kRowsMaxBlocks; blocks++)
     for (const bool group : {false, true})
       for (const bool deep : {false, true})
-        with_wide_kernel(blocks, group, deep, [&](auto kernel, int lds) {
-          ok = ok && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                         lds) == hipSuccess;
-        });
+        for (const bool gated : {false, true})
+          with_wide_kernel(blocks, group, deep, gated, [&](auto kernel, int lds) {
+            ok = ok && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                           lds) == hipSuccess;
+          });
   return ok ? 0 : 3;
 }
 
@@ -321,7 +373,7 @@ int launch_rows_wide(const GemmArgs& a, bool group, int blocks, hipStream_t stre
   b.gpb = a.N / 128 * b.row_parts;
   // (from where it is a hundredth faster with four row blocks, half that with three)
   const bool deep = (blocks == 4 && a.K >= 3072) || (blocks == 3 && a.K >= 5120);
-  const bool found = with_wide_kernel(blocks, group, deep, [&](auto kernel, int lds) {
+  const bool found = with_wide_kernel(blocks, group, deep, b.act != kActNone, [&](auto kernel, int lds) {
     hipLaunchKernelGGL(kernel, dim3(b.gpb), dim3(64 * kWaves), lds, stream, b);
   });
   return found ? launch_status() : 2;

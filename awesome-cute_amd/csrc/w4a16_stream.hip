@@ -113,7 +113,7 @@ constexpr int wait_vmcnt_imm(int n) { return (n & 15) | (7 << 4) | (15 << 8) | (
 // which a workgroup never leaves its tile: no tile bookkeeping in the main
 // loop and exactly one finish at the end.  Otherwise the first form (equal
 // runs of the tile-major sequence), where a run may cross tile boundaries.
-template <int MB, bool GROUP, int DEPTH, bool ONE_TILE, bool PARTS>
+template <int MB, bool GROUP, int DEPTH, bool ONE_TILE, bool PARTS, bool GATED>
 __global__ __launch_bounds__(256) void stream_kernel(GemmArgs p) {
   static_assert(!PARTS || (ONE_TILE && MB <= 2), "rows are only cut in the one-tile form, into parts of 16 or 32");
   extern __shared__ __attribute__((aligned(16))) char smem[];  // StreamLds<MB, DEPTH, ONE_TILE>::kBytes
@@ -455,6 +455,36 @@ __global__ __launch_bounds__(256) void stream_kernel(GemmArgs p) {
     if (writer) {
       half_t* C = (half_t*)p.C;
       const int q = lane >> 4;
+      if constexpr (GATED) {
+        const int n0 = kTileN * t + 64 * (q >> 1) + 4 * (q & 1) + 16 * wave;  // of the gates
+        f4 sg, su;
+        if constexpr (!GROUP) {
+          const half_t* S = (const half_t*)p.S;
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            sg[r] = (float)S[scale_index_single(n0 + r)];
+            su[r] = (float)S[scale_index_single(n0 + 8 + r)];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
+          const int m = 16 * i + nu;
+          if (m < rows_m) {
+            h4 o;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              float gate = res[i][0][r], up = res[i][1][r];
+              if constexpr (!GROUP) {
+                gate *= sg[r];
+                up *= su[r];
+              }
+              o[r] = (half_t)act_mul(gate, up, p.act);
+            }
+            *(h4*)(C + (size_t)(row0 + m) * (p.N >> 1) + gated_col(n0)) = o;
+          }
+        }
+        return;
+      }
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const int n0 = kTileN * t + 64 * (q >> 1) + 4 * (q & 1) + 16 * wave + 8 * h;
@@ -595,12 +625,15 @@ template <int MB, bool GROUP, int DEPTH, bool ONE_TILE>
 static int configure_variant() {
   constexpr int lds = StreamLds<MB, DEPTH, ONE_TILE>::kBytes;
   if (lds <= 65536) return 0;  // within the default limit of dynamic LDS
-  if (hipFuncSetAttribute((const void*)stream_kernel<MB, GROUP, DEPTH, ONE_TILE, false>,
-                          hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+  const auto raise = [](auto kernel) {
+    return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
+  };
+  if (!raise(stream_kernel<MB, GROUP, DEPTH, ONE_TILE, false, false>) ||
+      !raise(stream_kernel<MB, GROUP, DEPTH, ONE_TILE, false, true>))
     return 3;
   if constexpr (ONE_TILE && MB <= 2) {
-    if (hipFuncSetAttribute((const void*)stream_kernel<MB, GROUP, DEPTH, ONE_TILE, true>,
-                            hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+    if (!raise(stream_kernel<MB, GROUP, DEPTH, ONE_TILE, true, false>) ||
+        !raise(stream_kernel<MB, GROUP, DEPTH, ONE_TILE, true, true>))
       return 3;
   }
   return 0;
@@ -628,16 +661,17 @@ static int launch_variant(const GemmArgs& a, int grid, hipStream_t stream) {
   constexpr int lds = StreamLds<MB, DEPTH, ONE_TILE>::kBytes;
   // (the instance with the rows cut in two is a kernel of its own, so that
   // launches that do not cut them carry none of its bookkeeping)
+  const auto launch = [&](auto plain, auto gated) {
+    hipLaunchKernelGGL(a.act ? gated : plain, dim3(grid), dim3(256), lds, stream, a);
+    return launch_status();
+  };
   if constexpr (ONE_TILE && MB <= 2) {
-    if (a.row_parts > 1) {
-      hipLaunchKernelGGL((stream_kernel<MB, GROUP, DEPTH, ONE_TILE, true>), dim3(grid), dim3(256),
-                         lds, stream, a);
-      return launch_status();
-    }
+    if (a.row_parts > 1)
+      return launch(stream_kernel<MB, GROUP, DEPTH, ONE_TILE, true, false>,
+                    stream_kernel<MB, GROUP, DEPTH, ONE_TILE, true, true>);
   }
-  hipLaunchKernelGGL((stream_kernel<MB, GROUP, DEPTH, ONE_TILE, false>), dim3(grid), dim3(256),
-                     lds, stream, a);
-  return launch_status();
+  return launch(stream_kernel<MB, GROUP, DEPTH, ONE_TILE, false, false>,
+                stream_kernel<MB, GROUP, DEPTH, ONE_TILE, false, true>);
 }
 
 template <int MB, bool GROUP, bool ONE_TILE>

@@ -67,7 +67,7 @@ struct StripShape {
   static constexpr int kBytes = kReduceBase + kStripWaves * CS * 1024;
 };
 
-template <int CS, int MR, bool GROUP, int DEPTH>
+template <int CS, int MR, bool GROUP, int DEPTH, bool GATED>
 __global__ __launch_bounds__(64 * kStripWaves) void strip_kernel(GemmArgs p) {
   using Sh = StripShape<CS, MR>;
   constexpr int KC = Sh::kSteps;
@@ -302,7 +302,18 @@ __global__ __launch_bounds__(64 * kStripWaves) void strip_kernel(GemmArgs p) {
 #pragma unroll
     for (int w = 1; w < kStripWaves; w++) v += red[(w * CS + s) * 64 + lane];
     const int m = nu;
-    if (m < p.M) {
+    if (GATED && m < p.M) {
+      half_t* crow = (half_t*)p.C + (size_t)m * (p.N >> 1) + gated_col(res_col);
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float gate = v[2 * h], up = v[2 * h + 1];
+        if constexpr (!GROUP) {
+          gate *= (float)__builtin_bit_cast(half_t, chan[2 * h]);
+          up *= (float)__builtin_bit_cast(half_t, chan[2 * h + 1]);
+        }
+        crow[8 * h] = (half_t)act_mul(gate, up, p.act);
+      }
+    } else if (m < p.M) {
       half_t* crow = (half_t*)p.C + (size_t)m * p.N + res_col;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
@@ -318,12 +329,13 @@ template <int CS, int MR, bool GROUP>
 static int configure_strip_variant() {
   constexpr int lds = StripShape<CS, MR>::kBytes;
   if (lds <= 65536) return 0;
-  if (hipFuncSetAttribute((const void*)strip_kernel<CS, MR, GROUP, 1>,
-                          hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess ||
-      hipFuncSetAttribute((const void*)strip_kernel<CS, MR, GROUP, 2>,
-                          hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
-    return 3;
-  return 0;
+  const auto raise = [](auto kernel) {
+    return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
+  };
+  return raise(strip_kernel<CS, MR, GROUP, 1, false>) && raise(strip_kernel<CS, MR, GROUP, 2, false>) &&
+                 raise(strip_kernel<CS, MR, GROUP, 1, true>) && raise(strip_kernel<CS, MR, GROUP, 2, true>)
+             ? 0
+             : 3;
 }
 template <int CS>
 static int configure_strip_width() {
@@ -352,10 +364,11 @@ static int launch_strip_variant(const GemmArgs& a, hipStream_t stream) {
   // N = 4096, K = 11008 (five to six chunks per wave) 8.6 us with one chunk
   // in flight, 7.8 with two, 8.5 with three, 9.2 with four, 9.6 with six.
   const int per_wave = ceil_div(ceil_div(a.K, StripShape<CS, MR>::kChunkK), kStripWaves);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, lds, stream, b); };
   if (per_wave <= 2)
-    hipLaunchKernelGGL((strip_kernel<CS, MR, GROUP, 1>), grid, block, lds, stream, b);
+    b.act ? launch(strip_kernel<CS, MR, GROUP, 1, true>) : launch(strip_kernel<CS, MR, GROUP, 1, false>);
   else
-    hipLaunchKernelGGL((strip_kernel<CS, MR, GROUP, 2>), grid, block, lds, stream, b);
+    b.act ? launch(strip_kernel<CS, MR, GROUP, 2, true>) : launch(strip_kernel<CS, MR, GROUP, 2, false>);
   return launch_status();
 }
 template <int CS, bool GROUP>

@@ -22,6 +22,9 @@ _lib.marlin_mul.argtypes = [_P, _P, _P, _P, _I, _I, _I, _I, _P, ctypes.c_longlon
 for _name in ("marlin_gemm", "marlin_cute", "marlin_official", "marlin_gemm_static"):
     getattr(_lib, _name).restype = _I
     getattr(_lib, _name).argtypes = [_P, _P, _P, _P, _I, _I, _I, _P, _I, _I, _P, _I, _I, _I, _I]
+_lib.feedforward_gated_w4.restype = _I
+_lib.feedforward_gated_w4.argtypes = [_P, _P, _P, _P, _I, _I, _I, _I, _P, ctypes.c_longlong, _I, _I, _P, _I,
+                              ctypes.c_char_p, _I]
 _lib.marlin_gemm_static_capacity.restype = ctypes.c_longlong
 _lib.marlin_amd_scratch_bytes.restype = ctypes.c_longlong
 _lib.marlin_amd_scratch_bytes.argtypes = [_I, _P]
@@ -97,6 +100,41 @@ def _mul_op(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, s: torch.Tensor,
 
 @_mul_op.register_fake
 def _mul_fake(A, B, C, s, workspace, thread_k, thread_n, sms, max_par, cute_version):
+    return None
+
+
+ACTIVATIONS = {"silu": 1, "gelu": 2}  # (gelu in its tanh form)
+
+
+def _activation(name):
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}") from None
+
+
+def gated_mul(A, B, C, s, workspace, activation="silu", max_par=16):
+    """Both projections of a gated feed-forward block, the activation and the product of the two in
+    one launch: C = act(A @ G) * (A @ U), rounded once; no reference counterpart.
+
+    A: (m, k) half.  B: (k/16, 4n) int32, s: (groups, 2n) or (1, 2n) half: G and U as
+    `GatedLayer.pack` leaves them.  C: (m, n) half, overwritten.  workspace: at least n/64*max_par
+    zero int32 entries; zero again afterwards.  activation: "silu" or "gelu" (its tanh form).
+    n and k are multiples of 128.  Asynchronous on the current stream of A's device."""
+    act = _activation(activation)
+    if torch.compiler.is_compiling():
+        return torch.ops.marlin_amd.gated_mul(A, B, C, s, workspace, act, max_par)
+    _torch_binding.gated_mul(A, B, C, s, workspace, act, max_par)
+
+
+@torch.library.custom_op("marlin_amd::gated_mul", mutates_args=("C", "workspace"))
+def _gated_mul_op(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, s: torch.Tensor,
+                  workspace: torch.Tensor, activation: int, max_par: int) -> None:
+    _torch_binding.gated_mul(A, B, C, s, workspace, activation, max_par)
+
+
+@_gated_mul_op.register_fake
+def _gated_mul_fake(A, B, C, s, workspace, activation, max_par):
     return None
 
 
@@ -293,6 +331,54 @@ class Layer(nn.Module):
         q = torch.clamp(torch.round(w / s_full).int() + 8, 0, 15)
         self.B[:, :] = pack_weights(q).to(self.B.device)
         self.s[:, :] = pack_scales(s, groupwise).to(self.s.device)
+
+
+def _interleave(gate, up):
+    """(n, ...) twice -> (2n, ...): eight rows of the one, eight of the other."""
+    n = gate.shape[0]
+    rest = gate.shape[1:]
+    return torch.stack([gate.reshape(n // 8, 8, *rest), up.reshape(n // 8, 8, *rest)], dim=1).reshape(2 * n, *rest)
+
+
+class _Weight:
+    def __init__(self, weight):
+        self.weight = weight
+
+
+class GatedLayer(Layer):
+    """The gate and up projections of a feed-forward block in 4 bits, with the activation and the
+    product: (..., infeatures) -> (..., outfeatures) half, act(x Wg^T) * (x Wu^T) in one launch.
+    Buffers as a `Layer` of 2 * outfeatures columns, gate and up in turns of eight."""
+
+    def __init__(self, infeatures, outfeatures, groupsize=-1, activation="silu"):
+        self_act = _activation(activation)
+        if outfeatures % 128 != 0:
+            raise ValueError('`outfeatures` of a gated layer must be divisible by 128.')
+        super().__init__(infeatures, 2 * outfeatures, groupsize)
+        self.outfeatures = outfeatures
+        self.activation = activation
+        self._act = self_act
+
+    def forward(self, A):
+        if not torch.compiler.is_compiling():
+            return _torch_binding.gated_linear(A, self.B, self.s, self.workspace, self._act)
+        C = torch.empty(A.shape[:-1] + (self.outfeatures,), dtype=A.dtype, device=A.device)
+        gated_mul(A.reshape((-1, A.shape[-1])), self.B, C.view((-1, self.outfeatures)), self.s,
+                  self.workspace, self.activation)
+        return C
+
+    def pack(self, gate, up, gate_scales, up_scales):
+        """Fill B and s from two fake-quantised `torch.nn.Linear` (half weights) of (outfeatures,
+        infeatures) and their scales of shape (outfeatures, groups)."""
+        shape = (self.outfeatures, self.k)
+        groups = (self.outfeatures, self.k // self.groupsize)
+        for linear, scales in ((gate, gate_scales), (up, up_scales)):
+            if linear.weight.dtype != torch.half:
+                raise ValueError('Only `torch.half` weights are supported.')
+            if tuple(linear.weight.shape) != shape or tuple(scales.shape) != groups:
+                raise ValueError(f'weights must be {shape} and scales {groups}.')
+        super().pack(_Weight(_interleave(gate.weight.data, up.weight.data)),
+                     _interleave(gate_scales, up_scales))
 
 
 def replace_linear(module, name_filter=lambda n: True, groupsize=-1, name=''):
