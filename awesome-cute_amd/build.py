@@ -28,6 +28,10 @@ SOURCES = {
     "w4a16_convert.hip": [],
     "f16_streamk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "f16_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "ff_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "ff_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "ff_grads.hip": [],
+    "ff_host.hip": [],
 }
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

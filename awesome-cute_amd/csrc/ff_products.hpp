@@ -1,0 +1,73 @@
+// What the dense products of the feed-forward block share: their arguments, the two 16-bit
+// types, and the gated column order.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "buffer_loads.hpp"
+#include "f16_dense.hpp"
+#include "gated_act.hpp"
+#include "w4a16_common.hpp"
+
+namespace w4a16 {
+
+// C (M x N) = A (M x K) B^T, B given as N rows of K, rows `lda`, `ldb`, `ldc` elements apart;
+// or, gated, C (M x n) = act(A G^T) * (A U^T), B given as the n rows of G and then the n of U.
+struct ProductArgs {
+  const void* A;
+  const void* B;
+  void* C;
+  void* pre;  // gated: null, or (M x 2n), both sums in 16 bits for the backward pass
+  int M, N, K;  // N: columns of C
+  int lda, ldb, ldc, ldpre;
+  int act;  // kActNone: not gated
+  int tiles_m, tiles_n;
+};
+
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+template <bool BF>
+__device__ __forceinline__ f4 product_mfma(i4 a, i4 b, f4 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// four sums rounded to nearest
+template <bool BF>
+__device__ __forceinline__ i2 product_round(f4 v) {
+  if constexpr (BF)
+    return __builtin_bit_cast(i2, (b4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]});
+  else
+    return __builtin_bit_cast(i2, (h4){(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]});
+}
+
+__device__ __forceinline__ f4 act_mul4(f4 g, f4 u, int act) {
+  return (f4){act_mul(g[0], u[0], act), act_mul(g[1], u[1], act), act_mul(g[2], u[2], act), act_mul(g[3], u[3], act)};
+}
+
+// Gated, the product's columns are gates and ups in turns of sixteen, an MFMA operand each, so
+// that neighbouring operands of a wave hold a gate's sum and its partner's in the same lane and
+// register: nothing is exchanged.  The order exists in the addresses of B's rows alone.  Column
+// `col`, counted from `first` (a multiple of 32): its row of B as an offset in elements from
+// row first / 2 of G.  Rows past the last repeat it (their columns are not stored).
+__device__ __forceinline__ int gated_row(int first, int col, int n, int ldb) {
+  const int at = first + col;
+  int row = ((at >> 5) << 4) + (at & 15);
+  if (row >= n) row = n - 1;
+  return (row - (first >> 1)) * ldb + (at & 16 ? n * ldb : 0);
+}
+
+// Tiles of ff_tiles.hip: rows x columns of the product, 256 x 256 the big kernel's
+struct FfTile {
+  int rows, cols;
+};
+hipError_t configure_product_tiles();
+hipError_t configure_product_rows();
+// launches of either kind; bf: bfloat16 operands
+void launch_product_tiles(ProductArgs a, const FfTile& t, bool bf, hipStream_t stream);
+void launch_product_rows(const ProductArgs& a, bool bf, hipStream_t stream);
+constexpr int kProductRows = 64;  // rows of A that launch_product_rows takes at most
+
+}  // namespace w4a16

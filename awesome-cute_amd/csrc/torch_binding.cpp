@@ -13,12 +13,15 @@
 // the stream's queue, a stream's first call allocates, and an allocation may
 // wait for another thread's.
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <pybind11/pybind11.h>
 
 #include "../../include/feedforward_amd.h"
@@ -303,6 +306,295 @@ PyObject* py_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- dense feed-forward products (feedforward_amd.h) with fp16 or bfloat16 tensors.  A pass that
+// takes several launches makes all of them here, its temporaries among them: they come from torch's
+// allocator on the current stream and go back to it in that stream's order.
+
+// a matrix as the kernels address it: rows that start on 16 bytes
+struct Matrix {
+  at::Tensor t;
+  long long ld = 0;
+  Matrix() = default;
+  explicit Matrix(const at::Tensor& x) : t(x) {
+    const bool one = x.size(0) <= 1;
+    if (x.numel() != 0 && ((x.size(1) > 1 && x.stride(1) != 1) || (!one && (x.stride(0) % 8 != 0 || x.stride(0) < x.size(1))) ||
+                           (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) != 0)) {
+      t = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+      t.copy_(x);
+    }
+    ld = t.size(0) <= 1 || t.numel() == 0 ? (t.size(1) + 7) / 8 * 8 : t.stride(0);
+  }
+  void* at() const { return t.data_ptr(); }
+};
+
+long long up64(long long x) { return (x + 63) / 64 * 64; }
+
+// set by a pass that failed, raised once the interpreter lock is held again
+struct Failed {
+  int rc = 0;
+  bool operator()(int code) {
+    rc = code;
+    return code != FEEDFORWARD_OK;
+  }
+  bool raise() const {
+    if (rc == FEEDFORWARD_OK) return false;
+    PyErr_SetString(rc == FEEDFORWARD_ERR_SHAPE ? PyExc_ValueError : PyExc_RuntimeError, feedforward_last_error());
+    return true;
+  }
+};
+
+// x (..., k) and w (rows, k); false with an exception set
+bool check_dense(const at::Tensor& x, const at::Tensor& w, const char* x_name) {
+  for (const at::Tensor* t : {&x, &w}) {
+    const char* const name = t == &x ? x_name : "weight";
+    if (!t->is_cuda() || (t->scalar_type() != at::kHalf && t->scalar_type() != at::kBFloat16)) {
+      PyErr_Format(PyExc_ValueError, "%s must be a torch.half or torch.bfloat16 tensor on the GPU", name);
+      return false;
+    }
+    if (t->layout() != at::kStrided || t->is_neg() || t->is_conj()) {
+      PyErr_Format(PyExc_ValueError, "%s must be a plain tensor", name);
+      return false;
+    }
+  }
+  if (x.scalar_type() != w.scalar_type() || x.device() != w.device()) {
+    PyErr_Format(PyExc_ValueError, "%s and weight must have one type and one device", x_name);
+    return false;
+  }
+  if (x.dim() < 1 || w.dim() != 2 || x.size(-1) != w.size(1) || w.size(1) == 0) {
+    PyErr_Format(PyExc_ValueError, "weight must have two dimensions, the second one %s's last, not 0", x_name);
+    return false;
+  }
+  if (w.size(0) > 0x7fffffff || w.size(1) > 0x7fffffff || x.numel() / w.size(1) > 0x7fffffff) {
+    PyErr_SetString(PyExc_ValueError, "a size does not fit into a C int");
+    return false;
+  }
+  return true;
+}
+
+int type_code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? FEEDFORWARD_BF16 : FEEDFORWARD_FP16; }
+
+at::Tensor empty_as(const at::Tensor& like, at::IntArrayRef shape) {
+  return at::empty(shape, like.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+}
+
+// A backward pass that is captured into a graph while an eager graph of the same leaves is alive:
+// a leaf's accumulator lives as long as any graph that ends in it and belongs to the stream that was
+// current when it was made.  The engine would make that stream wait for the captured one, which draws
+// it into the capture without a way back, and the capture's end takes the process with it.  Refused
+// here, before the engine gets there; false with an exception set.
+bool check_capture(std::initializer_list<const at::Tensor*> inputs, int dev) {
+  const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return true;
+  for (const at::Tensor* t : inputs) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = accumulator ? accumulator->stream() : std::nullopt;
+    // (by number: torch names the device of one of them CUDA, of the other HIP)
+    if (!stream || (stream->id() == now.id() && stream->device_index() == dev)) continue;
+    PyErr_SetString(PyExc_RuntimeError,
+                    "the stream is being captured, and an eager graph of the same leaf, made on another stream, is "
+                    "alive: free what was computed from it before the capture, or compute it on this stream");
+    return false;
+  }
+  return true;
+}
+
+PyObject* pair_of(at::Tensor&& a, at::Tensor&& b) {
+  PyObject* const tuple = PyTuple_New(2);
+  if (!tuple) return nullptr;
+  PyTuple_SET_ITEM(tuple, 0, THPVariable_Wrap(std::move(a)));  // (None where undefined)
+  PyTuple_SET_ITEM(tuple, 1, THPVariable_Wrap(std::move(b)));
+  return tuple;
+}
+
+// gated_dense(x, weight, activation, keep) -> (h, both sums or None)
+PyObject* py_gated_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 4) {
+    PyErr_SetString(PyExc_TypeError, "gated_dense takes 4 arguments");
+    return nullptr;
+  }
+  const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
+  int act;
+  if (!x || !w || !to_int(args[2], &act) || !check_dense(*x, *w, "x")) return nullptr;
+  const int keep = PyObject_IsTrue(args[3]);
+  if (keep < 0) return nullptr;
+  if (w->size(0) % 2 != 0) {
+    PyErr_SetString(PyExc_ValueError, "weight must hold the rows of gate and, behind them, as many of up");
+    return nullptr;
+  }
+  const int64_t n = w->size(0) / 2, k = w->size(1), m = x->numel() / k;
+  const int dev = x->get_device();
+  void* const st = current_stream(dev);
+  at::Tensor h, pre;
+  Failed failed;
+  {
+    pybind11::gil_scoped_release unlocked;
+    c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = n;
+    h = empty_as(*x, shape);
+    if (keep) pre = empty_as(*x, {m, 2 * n});
+    const Matrix a(x->reshape({m, k})), b(*w);
+    failed(feedforward_gated(a.at(), b.at(), h.data_ptr(), keep ? pre.data_ptr() : nullptr, (int)m, (int)n, (int)k,
+                             a.ld, b.ld, n, 2 * n, type_code(*x), act, dev, st));
+  }
+  if (failed.raise()) return nullptr;
+  return pair_of(std::move(h), std::move(pre));
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_dense(x, weight) -> x weight^T
+PyObject* py_linear_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 2) {
+    PyErr_SetString(PyExc_TypeError, "linear_dense takes 2 arguments");
+    return nullptr;
+  }
+  const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
+  if (!x || !w || !check_dense(*x, *w, "x")) return nullptr;
+  const int64_t n = w->size(0), k = w->size(1), m = x->numel() / k;
+  const int dev = x->get_device();
+  void* const st = current_stream(dev);
+  at::Tensor y;
+  Failed failed;
+  {
+    pybind11::gil_scoped_release unlocked;
+    c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = n;
+    y = empty_as(*x, shape);
+    const Matrix a(x->reshape({m, k})), b(*w);
+    failed(feedforward_product(a.at(), b.at(), y.data_ptr(), (int)m, (int)n, (int)k, a.ld, b.ld, n, type_code(*x),
+                               dev, st));
+  }
+  if (failed.raise()) return nullptr;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// The gradients of rows x (m, k) and weights w (r, k) of a product, from its gradient as rows
+// (d, m x r, zeros behind it up to a multiple of 64 columns unless `depth` is r) and turned over
+// (d_t, r x m, zeros likewise).  dx = d w and dw = d_t x are products over r and m, of the
+// transposes of w and x.
+bool product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, int64_t depth, const at::Tensor& d_t,
+                   at::Tensor* dx, at::Tensor* dw, int dev, void* st, Failed& failed) {
+  const int64_t m = x.size(0), k = x.size(1), r = w.size(0);
+  const int type = type_code(x);
+  if (dx) {
+    const Matrix b(w);
+    const at::Tensor turned = empty_as(x, {k, up64(r)});
+    if (failed(feedforward_transpose(b.at(), turned.data_ptr(), (int)r, (int)k, b.ld, up64(r), dev, st))) return false;
+    if (failed(feedforward_product(d.at(), turned.data_ptr(), dx->data_ptr(), (int)m, (int)k, (int)depth, d.ld,
+                                   up64(r), k, type, dev, st)))
+      return false;
+  }
+  if (dw) {
+    const Matrix a(x);
+    const at::Tensor turned = empty_as(x, {k, up64(m)});
+    if (failed(feedforward_transpose(a.at(), turned.data_ptr(), (int)m, (int)k, a.ld, up64(m), dev, st))) return false;
+    if (failed(feedforward_product(d_t.data_ptr(), turned.data_ptr(), dw->data_ptr(), (int)r, (int)k, (int)up64(m),
+                                   up64(m), up64(m), k, type, dev, st)))
+      return false;
+  }
+  return true;
+}
+
+// gated_grads(dh, sums, x, weight, activation, whether dx, whether dweight) -> (dx, dweight)
+PyObject* py_gated_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7) {
+    PyErr_SetString(PyExc_TypeError, "gated_grads takes 7 arguments");
+    return nullptr;
+  }
+  const at::Tensor *dh = tensor(args[0], "dh"), *pre = tensor(args[1], "sums"), *x = tensor(args[2], "x"),
+                   *w = tensor(args[3], "weight");
+  int act;
+  if (!dh || !pre || !x || !w || !to_int(args[4], &act) || !check_dense(*x, *w, "x")) return nullptr;
+  const int want_x = PyObject_IsTrue(args[5]), want_w = PyObject_IsTrue(args[6]);
+  if (want_x < 0 || want_w < 0) return nullptr;
+  const int64_t n = w->size(0) / 2, k = w->size(1), m = x->numel() / k;
+  const auto fits = [&](const at::Tensor& t, int64_t columns) {
+    return t.scalar_type() == x->scalar_type() && t.device() == x->device() && t.dim() >= 1 &&
+           t.size(-1) == columns && t.numel() == m * columns;
+  };
+  if (!fits(*dh, n) || !fits(*pre, 2 * n) || !pre->is_contiguous()) {
+    PyErr_SetString(PyExc_ValueError, "dh and the sums must be those of x and weight");
+    return nullptr;
+  }
+  const int dev = x->get_device();
+  if (!check_capture({x, w}, dev)) return nullptr;
+  void* const st = current_stream(dev);
+  at::Tensor dx, dw;
+  Failed failed;
+  {
+    pybind11::gil_scoped_release unlocked;
+    if (want_x) dx = empty_as(*x, x->sizes());
+    if (want_w) dw = empty_as(*w, w->sizes());
+    if (m == 0) {
+      if (want_w) dw.zero_();
+    } else if (want_x || want_w) {
+      const Matrix d(dh->reshape({m, n}));
+      Matrix dgu;
+      at::Tensor turned;
+      if (want_x) dgu = Matrix(empty_as(*x, {m, up64(2 * n)}));
+      if (want_w) turned = empty_as(*x, {2 * n, up64(m)});
+      at::Tensor flat_dx = want_x ? dx.view({m, k}) : dx;
+      if (!failed(feedforward_gated_grad(d.at(), pre->data_ptr(), want_x ? dgu.at() : nullptr,
+                                         want_w ? turned.data_ptr() : nullptr, (int)m, (int)n, d.ld, 2 * n,
+                                         up64(2 * n), up64(m), type_code(*x), act, dev, st)))
+        product_grads(x->reshape({m, k}), *w, dgu, up64(2 * n), turned, want_x ? &flat_dx : nullptr,
+                      want_w ? &dw : nullptr, dev, st, failed);
+    }
+  }
+  if (failed.raise()) return nullptr;
+  return pair_of(std::move(dx), std::move(dw));
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_grads(dy, x, weight, whether dx, whether dweight) -> (dx, dweight)
+PyObject* py_linear_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5) {
+    PyErr_SetString(PyExc_TypeError, "linear_grads takes 5 arguments");
+    return nullptr;
+  }
+  const at::Tensor *dy = tensor(args[0], "dy"), *x = tensor(args[1], "x"), *w = tensor(args[2], "weight");
+  if (!dy || !x || !w || !check_dense(*x, *w, "x")) return nullptr;
+  const int want_x = PyObject_IsTrue(args[3]), want_w = PyObject_IsTrue(args[4]);
+  if (want_x < 0 || want_w < 0) return nullptr;
+  const int64_t n = w->size(0), k = w->size(1), m = x->numel() / k;
+  if (dy->scalar_type() != x->scalar_type() || dy->device() != x->device() || dy->dim() < 1 || dy->size(-1) != n ||
+      dy->numel() != m * n) {
+    PyErr_SetString(PyExc_ValueError, "dy must be that of x and weight");
+    return nullptr;
+  }
+  const int dev = x->get_device();
+  if (!check_capture({x, w}, dev)) return nullptr;
+  void* const st = current_stream(dev);
+  at::Tensor dx, dw;
+  Failed failed;
+  {
+    pybind11::gil_scoped_release unlocked;
+    if (want_x) dx = empty_as(*x, x->sizes());
+    if (want_w) dw = empty_as(*w, w->sizes());
+    if (m == 0 || n == 0) {
+      if (want_x) dx.zero_();
+      if (want_w) dw.zero_();
+    } else if (want_x || want_w) {
+      const Matrix d(dy->reshape({m, n}));
+      at::Tensor turned;
+      if (want_w) turned = empty_as(*x, {n, up64(m)});
+      at::Tensor flat_dx = want_x ? dx.view({m, k}) : dx;
+      if (!want_w || !failed(feedforward_transpose(d.at(), turned.data_ptr(), (int)m, (int)n, d.ld, up64(m), dev, st)))
+        product_grads(x->reshape({m, k}), *w, d, n, turned, want_x ? &flat_dx : nullptr, want_w ? &dw : nullptr, dev,
+                      st, failed);
+    }
+  }
+  if (failed.raise()) return nullptr;
+  return pair_of(std::move(dx), std::move(dw));
+  END_HANDLE_TH_ERRORS
+}
+
 // What the conversion kernels may take: plain tensors on one GPU, 16-byte aligned,
 // without gradients.  (That nothing looks on is the caller's to know.)
 //
@@ -433,6 +725,10 @@ PyObject* py_pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {
     {"mul", (PyCFunction)(void (*)(void))py_mul, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void (*)(void))py_linear, METH_FASTCALL, nullptr},
+    {"gated_dense", (PyCFunction)(void (*)(void))py_gated_dense, METH_FASTCALL, nullptr},
+    {"gated_grads", (PyCFunction)(void (*)(void))py_gated_grads, METH_FASTCALL, nullptr},
+    {"linear_dense", (PyCFunction)(void (*)(void))py_linear_dense, METH_FASTCALL, nullptr},
+    {"linear_grads", (PyCFunction)(void (*)(void))py_linear_grads, METH_FASTCALL, nullptr},
     {"gated_mul", (PyCFunction)(void (*)(void))py_gated_mul, METH_FASTCALL, nullptr},
     {"gated_linear", (PyCFunction)(void (*)(void))py_gated_linear, METH_FASTCALL, nullptr},
     {"quantize", (PyCFunction)(void (*)(void))py_quantize, METH_FASTCALL, nullptr},

@@ -1,8 +1,14 @@
 """Dense fp16 GEMM with a stream-K tail (the reference's gemm/streamk_gemm) over
 the C ABI of libmarlin_amd.so: C = A @ B.T with A (m, k) and B (n, k) in fp16,
 fp32 accumulation.  The GEMM always runs in the HIP library; a missing library
-is an import-time error."""
+is an import-time error.
+
+Beside it the dense products of a feed-forward block that is trained, in fp16 or
+bfloat16, with their gradients: `gated` and `linear` (include/feedforward_amd.h;
+no reference counterpart)."""
 import ctypes
+
+import torch
 
 from native import lib as _lib, torch_binding as _torch_binding
 
@@ -85,3 +91,162 @@ def force_finish_polls(polls):
 def gemm(A, B, C=None):
     """C (m, n) = A (m, k) @ B (n, k).T on the current stream; returns C."""
     return _torch_binding.dense(A, B, C)
+
+
+# ---------------------------------------------------------------------------
+# Products with gradients.  Under a compiler each is one operator of torch's dispatcher, which
+# costs more host time than a product of a few rows takes; else an autograd function, or the call
+# itself where nothing is to be differentiated.
+
+ACTIVATIONS = {"silu": 1, "gelu": 2}  # (gelu in its tanh form)
+_lib.feedforward_tile.restype = _I
+_lib.feedforward_tile.argtypes = [_I, _I, _I, _I, _I, _P]
+_lib.feedforward_force_tile.restype = None
+_lib.feedforward_force_tile.argtypes = [_I, _I]
+_lib.feedforward_last_error.restype = ctypes.c_char_p
+
+
+def _activation(name):
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}") from None
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, act):
+        h, sums = _torch_binding.gated_dense(x, weight, act, True)
+        ctx.save_for_backward(x, weight, sums)
+        ctx.act = act
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, weight, sums = ctx.saved_tensors
+        dx, dw = _torch_binding.gated_grads(dh, sums, x, weight, ctx.act, *ctx.needs_input_grad[:2])
+        return dx, dw, None
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight):
+        ctx.save_for_backward(x, weight)
+        return _torch_binding.linear_dense(x, weight)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight = ctx.saved_tensors
+        return _torch_binding.linear_grads(dy, x, weight, *ctx.needs_input_grad)
+
+
+def _differentiated(*tensors):
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
+def gated(x, weight, activation="silu"):
+    """Both projections of a gated feed-forward block, the activation and the product of the two in
+    one launch: act(x @ G.T) * (x @ U.T), rounded once, for x (..., k) and weight (2n, k), the rows
+    of G and behind them those of U; returns (..., n).
+
+    torch.half or torch.bfloat16, n and k multiples of 8, weight at most 2 GiB; activation "silu"
+    or "gelu" (its tanh form).  Where gradients are wanted the two sums are kept in that type as
+    well, 4n bytes a row.  Rows that do not start on 16 bytes are copied.  Differentiable once, on
+    the current stream of x's device."""
+    act = _activation(activation)
+    if torch.compiler.is_compiling():
+        return torch.ops.marlin_amd.gated_dense(x, weight, act)[0]
+    if _differentiated(x, weight):
+        return _Gated.apply(x, weight, act)
+    return _torch_binding.gated_dense(x, weight, act, False)[0]
+
+
+def linear(x, weight):
+    """x @ weight.T for x (..., k) and weight (n, k), torch.half or torch.bfloat16, n and k multiples
+    of 8; returns (..., n).  Differentiable once; streams and alignment as `gated`."""
+    if torch.compiler.is_compiling():
+        return torch.ops.marlin_amd.linear_dense(x, weight)
+    if _differentiated(x, weight):
+        return _Linear.apply(x, weight)
+    return _torch_binding.linear_dense(x, weight)
+
+
+@torch.library.custom_op("marlin_amd::gated_dense", mutates_args=())
+def _gated_op(x: torch.Tensor, weight: torch.Tensor, act: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return _torch_binding.gated_dense(x, weight, act, True)
+
+
+@_gated_op.register_fake
+def _gated_fake(x, weight, act):
+    n = weight.shape[0] // 2
+    return x.new_empty(x.shape[:-1] + (n,)), x.new_empty((x.numel() // x.shape[-1], 2 * n))
+
+
+@torch.library.custom_op("marlin_amd::gated_grads", mutates_args=())
+def _gated_grads_op(dh: torch.Tensor, sums: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+                    act: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return _torch_binding.gated_grads(dh, sums, x, weight, act, True, True)
+
+
+@_gated_grads_op.register_fake
+def _gated_grads_fake(dh, sums, x, weight, act):
+    return x.new_empty(x.shape), weight.new_empty(weight.shape)
+
+
+@torch.library.custom_op("marlin_amd::linear_dense", mutates_args=())
+def _linear_op(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    return _torch_binding.linear_dense(x, weight)
+
+
+@_linear_op.register_fake
+def _linear_fake(x, weight):
+    return x.new_empty(x.shape[:-1] + (weight.shape[0],))
+
+
+@torch.library.custom_op("marlin_amd::linear_grads", mutates_args=())
+def _linear_grads_op(dy: torch.Tensor, x: torch.Tensor,
+                     weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return _torch_binding.linear_grads(dy, x, weight, True, True)
+
+
+@_linear_grads_op.register_fake
+def _linear_grads_fake(dy, x, weight):
+    return x.new_empty(x.shape), weight.new_empty(weight.shape)
+
+
+def _keep_gated(ctx, inputs, output):
+    ctx.save_for_backward(inputs[0], inputs[1], output[1])
+    ctx.act = inputs[2]
+
+
+def _gated_backward(ctx, dh, _):
+    x, weight, sums = ctx.saved_tensors
+    dx, dw = torch.ops.marlin_amd.gated_grads(dh, sums, x, weight, ctx.act)
+    return dx, dw, None
+
+
+def _keep_linear(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _linear_backward(ctx, dy):
+    return torch.ops.marlin_amd.linear_grads(dy, *ctx.saved_tensors)
+
+
+_gated_op.register_autograd(_gated_backward, setup_context=_keep_gated)
+_linear_op.register_autograd(_linear_backward, setup_context=_keep_linear)
+
+
+def product_tile(m, n, k, gated=False, cus=256):
+    """(rows, columns) of the tiles that compute `linear` or `gated`, or None for few rows."""
+    out = (ctypes.c_int * 2)()
+    if _lib.feedforward_tile(m, n, k, int(gated), cus, out) != 0:
+        raise ValueError(_lib.feedforward_last_error().decode())
+    return tuple(out) if out[0] > 0 else None
+
+
+def force_product_tile(rows, cols=0):
+    """Tiles for every product of the calling thread; 0 = by cost."""
+    _lib.feedforward_force_tile(int(rows), int(cols))

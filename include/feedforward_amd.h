@@ -38,6 +38,53 @@ int feedforward_gated_w4(const void *A, const void *B, void *C, const void *s, i
                  int prob_k, int s_rows, void *workspace, long long workspace_numel, int activation,
                  int dev, void *stream, int max_par, char *err, int err_len);
 
+/* codes of the entries below, text in feedforward_last_error() */
+#define FEEDFORWARD_OK 0
+#define FEEDFORWARD_ERR_SHAPE 1   /* a size, a stride, an address, a type that no kernel takes */
+#define FEEDFORWARD_ERR_RUNTIME 3 /* the HIP runtime reported an error */
+
+/* types of matrices */
+#define FEEDFORWARD_FP16 0
+#define FEEDFORWARD_BF16 1
+
+/*
+ * Matrices below are row-major in fp16 or bfloat16 (`type`), `ld...` elements from one row to
+ * the next; rows start on 16 bytes (addresses, and ld a multiple of 8), are at most 4 MiB
+ * apart, and n and k are multiples of 8.  Sums are fp32, results rounded once.  Entries may
+ * be called from any thread, on any stream, and captured.
+ */
+
+/* C (m x n) = A (m x k) B^T, B n rows of k; k > 0 */
+int feedforward_product(const void *A, const void *B, void *C, int m, int n, int k, long long lda,
+                        long long ldb, long long ldc, int type, int dev, void *stream);
+
+/* h (m x n) = act(x G^T) * (x U^T), element by element, x (m x k), w the n rows of G and behind
+ * them the n rows of U; pre, if not null, (m x 2n): both sums in 16 bits, x G^T and beside it
+ * x U^T.  w holds at most 2 GiB; k > 0. */
+int feedforward_gated(const void *x, const void *w, void *h, void *pre, int m, int n, int k,
+                      long long ldx, long long ldw, long long ldh, long long ldpre, int type,
+                      int activation, int dev, void *stream);
+
+/* The gradients of both sums from that of h: [dg | du] as rows (dgu, m x 2n) and turned over
+ * (dgu_t, 2n x m), either of which may be null.  Behind a row of 2n or m columns there are
+ * zeros up to the next multiple of 64, which ld has room for. */
+int feedforward_gated_grad(const void *dh, const void *pre, void *dgu, void *dgu_t, int m, int n,
+                           long long lddh, long long ldpre, long long lddgu, long long lddgu_t,
+                           int type, int activation, int dev, void *stream);
+
+/* out (cols x rows) = in^T, in (rows x cols) of either type; zeros behind a row of out up to the
+ * next multiple of 64 columns, which ld_out has room for */
+int feedforward_transpose(const void *in, void *out, int rows, int cols, long long ld_in,
+                          long long ld_out, int dev, void *stream);
+
+/* out[0..1] = rows and columns of the product's tiles for a device of `cus` compute units, zeros
+ * where up to 64 rows are computed by blocks of columns; no GPU touched */
+int feedforward_tile(int m, int n, int k, int gated, int cus, int *out);
+/* such tiles for every product of the calling thread (0 = by cost); for tests and tools */
+void feedforward_force_tile(int rows, int cols);
+
+const char *feedforward_last_error(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,459 @@
+"""Dense products of the feed-forward block and their gradients: streamk.gated, streamk.linear.
+
+The oracle is the definition in 64 bits on the rounded inputs.  Bounds, element by element, with e
+half a step of the type (2^-11 fp16, 2^-8 bf16), S the sum of a product's magnitudes:
+  a sum of k products in fp32 is off by at most k 2^-24 S, a result rounded to the type by e of it;
+  the activations' slopes stay below 1.13, their second derivatives below 1, and in fp32 they are
+  off by less than 2^-18 of their size (an exponential whose argument is good to 2^-24 of itself);
+  for the gradients g and u are kept in the type, and dg and du rounded to it.
+"""
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "awesome-cute_amd"))
+import streamk  # noqa: E402
+
+gpu = pytest.mark.gpu
+TYPES = [torch.float16, torch.bfloat16]
+FP32 = 2.0 ** -24
+ACT = 2.0 ** -18
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def least(t):  # half the smallest step of all
+    return 2.0 ** -25 if t == torch.float16 else 2.0 ** -134
+
+
+def act64(g, name):
+    """value and slope"""
+    if name == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s + g * s * (1 - s)
+    z = np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3)
+    t = torch.tanh(z)
+    return g / 2 * (1 + t), (1 + t) / 2 + g / 2 * (1 - t * t) * np.sqrt(2 / np.pi) * (1 + 3 * 0.044715 * g * g)
+
+
+def make(m, n, k, type, seed, dev="cuda", rows=None):
+    gen = torch.Generator(device=dev).manual_seed(seed)
+
+    def randn(*shape, std=1.0):
+        return (torch.randn(shape, device=dev, generator=gen) * std).to(type)
+
+    return randn(m, k), randn(rows or 2 * n, k, std=k ** -0.5), randn(m, n)
+
+
+def within(got, want, bound, type, parts=3.0):
+    bound = bound * (1 + 2.0 ** -6) + least(type)  # (roundings of what is off already)
+    err = (got.double() - want).abs()
+    assert got.dtype == type and got.shape == want.shape and torch.isfinite(got).all()
+    assert (err <= bound).all(), float((err / bound).max())
+    # roundings are independent of each other: together they stay near one of them
+    assert err.norm() <= parts * half_step(type) * want.norm() + least(type) * want.numel() ** 0.5
+
+
+class Gated64:
+    def __init__(self, x, w, act):
+        n, self.k = w.shape[0] // 2, w.shape[1]
+        self.x, self.wg, self.wu = x.double(), w[:n].double(), w[n:].double()
+        self.g, self.u = self.x @ self.wg.t(), self.x @ self.wu.t()
+        self.sg, self.su = self.x.abs() @ self.wg.abs().t(), self.x.abs() @ self.wu.abs().t()
+        self.value, self.slope = act64(self.g, act)
+
+    def check_forward(self, h, type):
+        dg, du = self.k * FP32 * self.sg, self.k * FP32 * self.su
+        want = self.value * self.u
+        bound = 1.13 * dg * (self.u.abs() + du) + self.value.abs() * du + (half_step(type) + 2 * ACT) * want.abs()
+        within(h, want, bound, type, 1.01)
+
+    def check_grads(self, dh, dx, dw, type):
+        e, d = half_step(type), dh.double()
+        eg = e * self.g.abs() + self.k * FP32 * self.sg + least(type)
+        eu = e * self.u.abs() + self.k * FP32 * self.su + least(type)
+        g, u = d * self.u * self.slope, d * self.value
+        off_g = d.abs() * ((self.u.abs() + eu) * (eg + ACT) + 1.13 * eu) + e * g.abs() + least(type)
+        off_u = d.abs() * (1.13 * eg + ACT * self.value.abs()) + e * u.abs() + least(type)
+        n2, m = 2 * self.g.shape[1], self.x.shape[0]
+        if dx is not None:
+            want = g @ self.wg + u @ self.wu
+            size = g.abs() @ self.wg.abs() + u.abs() @ self.wu.abs()
+            bound = off_g @ self.wg.abs() + off_u @ self.wu.abs() + n2 * FP32 * size + e * want.abs()
+            within(dx, want, bound, type)
+        if dw is not None:
+            want = torch.cat([g.t() @ self.x, u.t() @ self.x])
+            ax = self.x.abs()
+            size = torch.cat([g.abs().t() @ ax, u.abs().t() @ ax])
+            bound = torch.cat([off_g.t() @ ax, off_u.t() @ ax]) + m * FP32 * size + e * want.abs()
+            within(dw, want, bound, type)
+
+
+def check_product(got, a, b, type):
+    """got = a @ b.T"""
+    a, b = a.double(), b.double()
+    want = a @ b.t()
+    bound = a.shape[1] * FP32 * (a.abs() @ b.abs().t()) + half_step(type) * want.abs()
+    within(got, want, bound, type, 1.01)
+
+
+# --- without a GPU -------------------------------------------------------------------------
+
+def test_refuses_host_tensors_and_unknown_activations():
+    x, w = torch.zeros(2, 16).half(), torch.zeros(32, 16).half()
+    with pytest.raises(ValueError, match="on the GPU"):
+        streamk.gated(x, w)
+    with pytest.raises(ValueError, match="on the GPU"):
+        streamk.linear(x, w)
+    with pytest.raises(ValueError, match="activation"):
+        streamk.gated(x, w, "relu")
+    with pytest.raises(TypeError, match="Tensor"):
+        streamk.linear(None, w)
+
+
+@pytest.mark.parametrize("m,n,k,lda,ldb,ldc,type,code", [
+    (-1, 8, 8, 8, 8, 8, 0, 1), (4, 12, 8, 8, 8, 16, 0, 1), (4, 8, 12, 16, 16, 8, 0, 1), (4, 8, 8, 8, 8, 8, 2, 1),
+    (4, 8, 16, 8, 16, 8, 0, 1), (4, 8, 16, 20, 16, 8, 0, 1), (4, 8, 16, 16, 16, 4, 0, 1), (4, 8, 0, 8, 8, 8, 0, 1),
+    (4, 8, 16, 1 << 22, 16, 8, 0, 1), (0, 8, 16, 16, 16, 8, 0, 0), (4, 0, 16, 16, 16, 8, 1, 0)])
+def test_codes_of_the_entries(m, n, k, lda, ldb, ldc, type, code):
+    import ctypes
+    lib, L = streamk._lib, ctypes.c_longlong
+    rc = lib.feedforward_product(None, None, None, m, n, k, L(lda), L(ldb), L(ldc), type, 0, None)
+    assert rc == code
+    rc = lib.feedforward_gated(None, None, None, None, m, n, k, L(lda), L(ldb), L(ldc), L(2 * ldc), type, 1, 0, None)
+    assert rc == code
+    assert (len(lib.feedforward_last_error()) > 0) or code == 0
+
+
+def test_codes_of_the_gradients_and_transposes():
+    import ctypes
+    lib, L = streamk._lib, ctypes.c_longlong
+
+    def grad(m, n, lddh, ldpre, lddgu, ldt, type=0, act=1, dgu=16, dgu_t=16):
+        return lib.feedforward_gated_grad(None, None, ctypes.c_void_p(dgu), ctypes.c_void_p(dgu_t), m, n, L(lddh),
+                                          L(ldpre), L(lddgu), L(ldt), type, act, 0, None)
+
+    assert grad(0, 40, 40, 80, 128, 64) == 0
+    assert grad(0, 40, 40, 80, 80, 64) == 1       # no room for the zeros behind 2n columns
+    assert grad(70, 0, 8, 8, 64, 64) == 1         # ... behind m columns
+    assert grad(0, 40, 32, 80, 128, 64) == 1
+    assert grad(0, 40, 40, 72, 128, 64) == 1
+    assert grad(0, 40, 40, 80, 128, 64, act=0) == 1
+    assert grad(0, 40, 40, 80, 128, 64, type=5) == 1
+    assert grad(0, 40, 40, 80, 128, 64, dgu=8) == 1  # off 16 bytes
+    turn = lib.feedforward_transpose
+    assert turn(None, None, 0, 8, L(8), L(64), 0, None) == 0
+    assert turn(None, None, 4, 12, L(16), L(64), 0, None) == 1
+    assert turn(None, None, 65, 8, L(8), L(64), 0, None) == 1
+    assert turn(None, None, -1, 8, L(8), L(64), 0, None) == 1
+    # more than 2 GiB of a gated product's weights
+    rc = lib.feedforward_gated(None, None, None, None, 1, 1 << 20, 1024, L(1024), L(1024), L(1 << 20), L(1 << 21), 0, 1,
+                               0, None)
+    assert rc == 1 and b"2 GiB" in lib.feedforward_last_error()
+
+
+def test_tiles_cover_what_they_are_asked():
+    seen = set()
+    rng = np.random.default_rng(0)
+    for _ in range(4000):
+        m, n, k = (int(2 ** rng.uniform(*r)) for r in ((0, 14), (3, 14), (3, 14)))
+        n, k = 8 * max(1, n // 8), 8 * max(1, k // 8)
+        for gated in (False, True):
+            t = streamk.product_tile(m, n, k, gated)
+            assert (t is None) == (m <= 64)
+            if t:
+                assert k % 64 == 0 or t != (256, 256)
+                seen.add(t)
+    assert seen == {(64, 64), (64, 128), (96, 128), (128, 128), (96, 256), (128, 256), (256, 256)}
+
+
+# --- on the GPU ----------------------------------------------------------------------------
+
+# up to 64 rows by blocks of columns; the tiles; depths and widths that nothing divides
+FORWARD = [(1, 8, 8), (1, 10752, 4096), (2, 40, 72), (7, 1032, 520), (16, 5208, 4160), (17, 2744, 1032), (33, 24, 8),
+           (40, 8200, 1096), (48, 16, 4096), (64, 4104, 968), (65, 8, 8), (65, 72, 136), (100, 1000, 1000),
+           (300, 520, 4160), (777, 5208, 4160), (1025, 264, 64), (2100, 1544, 192)]
+
+
+@gpu
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("m,n,k", FORWARD)
+def test_forward(m, n, k, type):
+    x, w, _ = make(m, n, k, type, m + n + k)
+    for act in ("silu", "gelu"):
+        Gated64(x, w, act).check_forward(streamk.gated(x, w, act), type)
+    check_product(streamk.linear(x, w), x, w, type)
+
+
+TILES = [(64, 64), (64, 128), (96, 128), (128, 128), (96, 256), (128, 256), (256, 256)]
+
+
+@gpu
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("m,n,k", [(1, 8, 64), (300, 520, 192), (257, 136, 1096), (130, 264, 128)])
+def test_every_tile(tile, m, n, k):
+    try:
+        streamk.force_product_tile(*tile)
+        for type in TYPES:
+            x, w, dh = make(m, n, k, type, 5)
+            x.requires_grad_()
+            w.requires_grad_()
+            ref = Gated64(x.detach(), w.detach(), "gelu")
+            ref.check_forward(streamk.gated(x.detach(), w.detach(), "gelu"), type)
+            h = streamk.gated(x, w, "gelu")
+            ref.check_forward(h.detach(), type)
+            ref.check_grads(dh, *torch.autograd.grad(h, (x, w), dh), type)
+            check_product(streamk.linear(x.detach(), w.detach()), x.detach(), w.detach(), type)
+    finally:
+        streamk.force_product_tile(0)
+
+
+GRADS = [(1, 8, 8), (3, 40, 72), (65, 64, 64), (64, 520, 136), (200, 1032, 264), (777, 200, 1000), (1237, 2744, 1032),
+         (2048, 512, 512)]
+
+
+@gpu
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("m,n,k", GRADS)
+def test_gradients(m, n, k, type):
+    x, w, dh = make(m, n, k, type, m * n + k)
+    x.requires_grad_()
+    w.requires_grad_()
+    for act in ("silu", "gelu"):
+        h = streamk.gated(x, w, act)
+        ref = Gated64(x.detach(), w.detach(), act)
+        ref.check_forward(h.detach(), type)
+        dx, dw = torch.autograd.grad(h, (x, w), dh)
+        ref.check_grads(dh, dx, dw, type)
+    y = streamk.linear(x, w[:n])
+    dx, dw = torch.autograd.grad(y, (x, w), dh)
+    check_product(y.detach(), x.detach(), w[:n].detach(), type)
+    check_product(dx, dh, w[:n].detach().t(), type)
+    check_product(dw[:n], dh.t(), x.detach().t(), type)
+    assert not dw[n:].any()
+
+
+@gpu
+def test_gradients_against_differences():
+    """The loss sum(h c) along a direction, by differences of the definition in 64 bits: the step t
+    leaves a relative t^2 of the third derivative and 2^-52 / t of cancellation."""
+    m, n, k = 24, 40, 48
+    for act in ("silu", "gelu"):
+        x, w, c = make(m, n, k, torch.float16, 3)
+        x.requires_grad_()
+        w.requires_grad_()
+        dx, dw = torch.autograd.grad(streamk.gated(x, w, act), (x, w), c)
+        gen = torch.Generator(device="cuda").manual_seed(4)
+        vx = torch.randn(x.shape, device="cuda", generator=gen, dtype=torch.float64)
+        vw = torch.randn(w.shape, device="cuda", generator=gen, dtype=torch.float64) * k ** -0.5
+
+        def loss(t):
+            xd, wd = x.detach().double() + t * vx, w.detach().double() + t * vw
+            return (act64(xd @ wd[:n].t(), act)[0] * (xd @ wd[n:].t()) * c.double()).sum()
+
+        t = 1e-4
+        slope = (loss(t) - loss(-t)) / (2 * t)
+        terms = torch.cat([(dx.double() * vx).flatten(), (dw.double() * vw).flatten()])
+        # every term of the inner product is off by some half steps: 6 of them, as independent errors
+        assert (terms.sum() - slope).abs() <= 6 * 2.0 ** -11 * 3 * terms.norm() + 1e-5 * terms.abs().sum()
+
+
+@gpu
+def test_only_the_gradients_that_are_wanted():
+    x, w, dh = make(70, 72, 136, torch.bfloat16, 1)
+    both = [t.clone().requires_grad_() for t in (x, w)]
+    dx, dw = torch.autograd.grad(streamk.gated(*both), both, dh)
+    xg = x.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(streamk.gated(xg, w), xg, dh)[0], dx)
+    wg = w.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(streamk.gated(x, wg), wg, dh)[0], dw)
+    with torch.no_grad():
+        assert not streamk.gated(xg, wg).requires_grad
+    assert torch.equal(streamk.gated(x, w), streamk.gated(xg, wg).detach())
+
+
+@gpu
+@pytest.mark.parametrize("m", [5, 200])
+def test_strides_alignment_and_shapes(m):
+    n, k = 72, 136
+    x, w, dh = make(m, n, k, torch.float16, 2)
+    want, want_y = streamk.gated(x, w), streamk.linear(x, w)
+    wide = torch.full((m, k + 24), float("nan"), dtype=torch.float16, device="cuda")
+    wide[:, 8:8 + k] = x
+    deep = torch.full((2 * n, k + 8), float("nan"), dtype=torch.float16, device="cuda")
+    deep[:, :k] = w
+    room = torch.empty(x.numel() + 1, dtype=torch.float16, device="cuda")[1:].view(x.shape).copy_(x)
+    for a in (x, wide[:, 8:8 + k], x.t().contiguous().t(), room):
+        for b in (w, deep[:, :k], w.t().contiguous().t()):
+            assert torch.equal(streamk.gated(a, b), want)
+            assert torch.equal(streamk.linear(a, b), want_y)
+            a_, b_ = a.detach().requires_grad_(), b.detach().requires_grad_()
+            for got, ref in zip(torch.autograd.grad(streamk.gated(a_, b_), (a_, b_), dh),
+                                torch.autograd.grad(streamk.gated(x.requires_grad_(), w.requires_grad_()), (x, w), dh)):
+                assert torch.equal(got, ref)
+            x, w = x.detach(), w.detach()
+    assert torch.equal(streamk.gated(x.view(1, m, k), w), want.view(1, m, n))
+    assert streamk.gated(x[0], w).shape == (n,)
+    # a gradient that is one value everywhere has no strides
+    x.requires_grad_()
+    w.requires_grad_()
+    one = torch.autograd.grad(streamk.gated(x, w).float().sum(), (x, w))
+    ones = torch.autograd.grad(streamk.gated(x, w), (x, w), torch.ones((m, n), dtype=torch.float16, device="cuda"))
+    assert all(torch.equal(a, b) for a, b in zip(one, ones))
+
+
+@gpu
+def test_empty():
+    x, w, _ = make(0, 72, 136, torch.float16, 2)
+    x.requires_grad_()
+    w.requires_grad_()
+    for y in (streamk.gated(x, w), streamk.linear(x, w)):
+        dx, dw = torch.autograd.grad(y.sum(), (x, w))
+        assert dx.shape == (0, 136) and not dw.any()
+    assert streamk.linear(torch.zeros(3, 16, device="cuda").half(), torch.zeros(0, 16, device="cuda").half()).shape == (3, 0)
+
+
+@gpu
+def test_refusals_on_the_gpu():
+    x, w, _ = make(4, 16, 32, torch.float16, 0)
+    with pytest.raises(ValueError, match="GPU"):
+        streamk.gated(x.float(), w.float())
+    with pytest.raises(ValueError, match="one type"):
+        streamk.linear(x.bfloat16(), w)
+    with pytest.raises(ValueError, match="two dimensions"):
+        streamk.linear(x, w[:, :16])
+    with pytest.raises(ValueError, match="multiples of 8"):
+        streamk.linear(x[:, :12], w[:, :12])
+    with pytest.raises(ValueError, match="multiples of 8"):
+        streamk.linear(x, w[:4])
+    with pytest.raises(ValueError, match="as many of up"):
+        streamk.gated(x, w[:31])
+    with pytest.raises(ValueError, match="not 0"):
+        streamk.linear(x[:, :0], w[:, :0])
+    x.requires_grad_()
+    with pytest.raises(RuntimeError, match="does not require grad"):
+        g, = torch.autograd.grad(streamk.gated(x, w).float().sum(), x, create_graph=True)
+        g.float().sum().backward()
+
+
+@gpu
+def test_infinities_and_nan_stay_in_their_rows():
+    for m in (20, 300):
+        x, w, _ = make(m, 72, 200, torch.bfloat16, 8)
+        want = streamk.gated(x, w)
+        bad = x.clone()
+        bad[3] = float("nan")
+        bad[9, 7] = float("inf")
+        got = streamk.gated(bad, w)
+        keep = [i for i in range(m) if i not in (3, 9)]
+        assert torch.equal(got[keep], want[keep]) and got[3].isnan().all()
+    # far out the activations are g and 0 and their slopes 1 and 0, without NaN
+    x = torch.full((70, 8), 100.0, dtype=torch.bfloat16, device="cuda")
+    w = torch.eye(8, device="cuda").repeat(2, 1).bfloat16()
+    w[1, 1] = -1
+    x.requires_grad_()
+    w.requires_grad_()
+    for act in ("silu", "gelu"):
+        h = streamk.gated(x, w, act)
+        assert (h[:, 0] == 9984).all() and (h[:, 1] == 0).all()
+        dx, dw = torch.autograd.grad(h.float().sum(), (x, w))
+        assert torch.isfinite(dx).all() and torch.isfinite(dw).all()
+
+
+@gpu
+def test_streams_and_two_at_once():
+    problems = [make(m, 264, 520, torch.bfloat16, m) for m in (30, 90, 700)]
+    want = [streamk.gated(x, w) for x, w, _ in problems]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in problems]
+    out = []
+    for _ in range(4):
+        for (x, w, dh), stream in zip(problems, streams):
+            with torch.cuda.stream(stream):
+                a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+                h = streamk.gated(a, b)
+                out.append((h.detach(), torch.autograd.grad(h, (a, b), dh)))
+    torch.cuda.synchronize()
+    for i, (h, grads) in enumerate(out):
+        assert torch.equal(h, want[i % 3])
+        assert all(torch.equal(a, b) for a, b in zip(grads, out[i % 3][1]))
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 64, 200])
+def test_captured_and_replayed(m):
+    n, k = 136, 264
+    x, w, dh = make(m, n, k, torch.float16, 6)
+    x.requires_grad_()
+    w.requires_grad_()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.autograd.grad(streamk.gated(x, w), (x, w), dh)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        h = streamk.gated(x, w)
+        y = streamk.linear(x, w)
+        dx, dw = torch.autograd.grad(h, (x, w), dh)
+    for seed in range(3):
+        nx, nw, ndh = make(m, n, k, torch.float16, 20 + seed)
+        with torch.no_grad():
+            x.copy_(nx), w.copy_(nw), dh.copy_(ndh)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        a, b = nx.requires_grad_(), nw.requires_grad_()
+        ref = streamk.gated(a, b)
+        assert torch.equal(h, ref) and torch.equal(y, streamk.linear(nx, nw))
+        assert all(torch.equal(p, q) for p, q in zip((dx, dw), torch.autograd.grad(ref, (a, b), ndh)))
+
+
+@gpu
+def test_a_captured_backward_pass_beside_an_eager_graph_of_its_leaves():
+    # made on the capture's own stream the eager graph is no hindrance, on another it is refused
+    # before the engine draws that stream into the capture
+    x, w, dh = make(70, 72, 136, torch.float16, 6)
+    x.requires_grad_()
+    w.requires_grad_()
+    side = torch.cuda.Stream()
+    for forward in (lambda: streamk.gated(x, w), lambda: streamk.linear(x, w[:72])):
+        with torch.cuda.stream(side):
+            want = torch.autograd.grad(forward(), (x, w), dh)
+            alive = forward()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = torch.autograd.grad(forward(), (x, w), dh)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del alive, got, graph
+    alive = streamk.gated(x, w)
+    with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            torch.autograd.grad(streamk.gated(x, w), (x, w), dh)
+    torch.cuda.synchronize()
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(alive, (x, w), dh))
+
+
+@gpu
+def test_under_a_compiler():
+    x, w, dh = make(70, 72, 136, torch.bfloat16, 1)
+    leaves = [t.requires_grad_() for t in (x, w)]
+
+    def loss(a, b):
+        return (streamk.gated(a, b, "gelu") * 2, streamk.linear(a, b))
+
+    compiled = torch.compile(loss, backend="aot_eager", fullgraph=True)
+    for got, want in zip(compiled(*leaves), loss(*leaves)):
+        assert torch.equal(got, want)
+    got = torch.autograd.grad(compiled(*leaves)[0], leaves, dh)
+    want = torch.autograd.grad(loss(*leaves)[0], leaves, dh)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
