@@ -31,6 +31,7 @@ SOURCES = {
     "ff_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ff_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ff_grads.hip": [],
+    "ff_norm.hip": [],
     "ff_host.hip": [],
 }
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

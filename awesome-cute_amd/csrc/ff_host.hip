@@ -9,6 +9,7 @@
 
 #include "../../include/feedforward_amd.h"
 #include "ff_grads.hpp"
+#include "ff_norm.hpp"
 #include "ff_products.hpp"
 
 namespace {
@@ -132,6 +133,25 @@ int run_product(ProductArgs a, bool bf, int dev, hipStream_t stream) {
   });
 }
 
+int type_bytes(int type) { return type == FEEDFORWARD_FP32 ? 4 : 2; }
+NormType norm_type(int type) {
+  return type == FEEDFORWARD_FP32 ? kNormFp32 : type == FEEDFORWARD_BF16 ? kNormBf16 : kNormFp16;
+}
+
+int check_norm(long long rows, int d, int rows_per_gate, int type) {
+  if (rows < 0 || d < 1 || d > kNormMax)
+    return fail(FEEDFORWARD_ERR_SHAPE, "%lld rows of %d: rows must hold 1 to %d elements", rows, d, kNormMax);
+  if (rows_per_gate < 1 || rows % rows_per_gate != 0)
+    return fail(FEEDFORWARD_ERR_SHAPE, "%lld rows are no multiple of the %d of a gate", rows, rows_per_gate);
+  if (type != FEEDFORWARD_FP16 && type != FEEDFORWARD_BF16 && type != FEEDFORWARD_FP32)
+    return fail(FEEDFORWARD_ERR_SHAPE, "unknown type %d", type);
+  return FEEDFORWARD_OK;
+}
+int check_rows(const char* name, const void* p, long long ld, int d) {
+  if (p && ld < d) return fail(FEEDFORWARD_ERR_SHAPE, "%s: rows of %d elements lie %lld apart", name, d, ld);
+  return FEEDFORWARD_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -196,6 +216,68 @@ int feedforward_transpose(const void* in, void* out, int rows, int cols, long lo
   if (rc == FEEDFORWARD_OK && rows > 64 * 65535) rc = fail(FEEDFORWARD_ERR_SHAPE, "%d rows: too many", rows);
   if (rc != FEEDFORWARD_OK || rows == 0 || cols == 0) return rc;
   return on_device(dev, [&](int) { launch_transpose(in, ld_in, out, ld_out, rows, cols, (hipStream_t)stream); });
+}
+
+int feedforward_norm(const void* residual, long long ld_residual, const void* block, long long ld_block,
+                     const void* post, const void* gate, long long ld_gate, int rows_per_gate, const void* pre,
+                     float scale, float eps, void* r, void* y, float* stats, long long rows, int d, int type,
+                     int dev, void* stream) {
+  int rc = check_norm(rows, d, rows_per_gate, type);
+  if (rc == FEEDFORWARD_OK) rc = check_rows("residual", residual, ld_residual, d);
+  if (rc == FEEDFORWARD_OK) rc = check_rows("block", block, ld_block, d);
+  if (rc == FEEDFORWARD_OK) rc = check_rows("gate", rows > rows_per_gate ? gate : nullptr, ld_gate, d);
+  if (rc == FEEDFORWARD_OK && !(eps >= 0.f)) rc = fail(FEEDFORWARD_ERR_SHAPE, "eps must not be negative");
+  if (rc != FEEDFORWARD_OK || rows == 0) return rc;
+  if (!residual || (block ? !r : (post || gate || !pre)) || (pre && !y))
+    return fail(FEEDFORWARD_ERR_SHAPE, "a block needs its output r, a norm its output y, and one of them must be there");
+  NormArgs a = {};
+  a.residual = residual, a.block = block, a.post = post, a.gate = gate, a.pre = pre;
+  a.r = block ? r : nullptr, a.y = pre ? y : nullptr, a.stats = stats;
+  a.ld_residual = ld_residual, a.ld_block = ld_block, a.ld_gate = ld_gate;
+  a.rows = rows, a.rows_per_gate = rows_per_gate, a.d = d;
+  a.scale = scale, a.eps = eps;
+  return on_device(dev, [&](int cus) { launch_norm(a, norm_type(type), cus, (hipStream_t)stream); });
+}
+
+long long feedforward_norm_grad_bytes(long long rows, int d, int rows_per_gate, int type) {
+  if (check_norm(rows, d, rows_per_gate, type) != FEEDFORWARD_OK) return -1;
+  // (whichever loads the addresses allow)
+  const size_t a = norm_parts(rows, rows_per_gate, d, type_bytes(type), true).bytes;
+  const size_t b = norm_parts(rows, rows_per_gate, d, type_bytes(type), false).bytes;
+  return (long long)(a > b ? a : b);
+}
+
+int feedforward_norm_grad(const void* dy, long long ld_dy, const void* dr, long long ld_dr, const void* r,
+                          long long ld_r, const void* block, long long ld_block, const void* post, const void* gate,
+                          long long ld_gate, int rows_per_gate, const void* pre, float scale, const float* stats,
+                          void* dresidual, void* dblock, void* dpost, void* dgate, void* dpre, void* partials,
+                          long long partial_bytes, long long rows, int d, int type, int dev, void* stream) {
+  int rc = check_norm(rows, d, rows_per_gate, type);
+  const struct {
+    const char* name;
+    const void* at;
+    long long ld;
+  } matrices[] = {{"dy", dy, ld_dy}, {"dr", dr, ld_dr}, {"r", r, ld_r}, {"block", block, ld_block},
+                  {"gate", rows > rows_per_gate ? gate : nullptr, ld_gate}};
+  for (const auto& m : matrices)
+    if (rc == FEEDFORWARD_OK) rc = check_rows(m.name, m.at, m.ld, d);
+  if (rc != FEEDFORWARD_OK || rows == 0) return rc;
+  if ((pre && (!dy || !r)) || ((pre || post) && !stats) || (!block && (post || gate || dblock || dpost || dgate)) ||
+      (!post && dpost) || (!gate && dgate) || (!pre && dpre) || (!pre && !dr))
+    return fail(FEEDFORWARD_ERR_SHAPE, "an input that a gradient is made from is missing");
+  const bool sums = dpost || dgate || dpre;
+  if (sums && (!partials || partial_bytes < feedforward_norm_grad_bytes(rows, d, rows_per_gate, type)))
+    return fail(FEEDFORWARD_ERR_SHAPE, "the sums over rows need %lld bytes of scratch",
+                feedforward_norm_grad_bytes(rows, d, rows_per_gate, type));
+  NormGradArgs a = {};
+  a.dy = pre ? dy : nullptr, a.dr = dr, a.r = r, a.block = block, a.post = post, a.gate = gate, a.pre = pre;
+  a.stats = stats;
+  a.dresidual = dresidual, a.dblock = dblock, a.dpost = dpost, a.dgate = dgate, a.dpre = dpre;
+  a.partials = sums ? (float*)partials : nullptr;
+  a.ld_dy = ld_dy, a.ld_dr = ld_dr, a.ld_r = ld_r, a.ld_block = ld_block, a.ld_gate = ld_gate;
+  a.rows = rows, a.rows_per_gate = rows_per_gate, a.d = d;
+  a.scale = scale;
+  return on_device(dev, [&](int) { launch_norm_grad(a, norm_type(type), (hipStream_t)stream); });
 }
 
 int feedforward_tile(int m, int n, int k, int gated, int cus, int* out) {

@@ -595,6 +595,234 @@ PyObject* py_linear_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the norms around a block, fp16, bfloat16 or fp32
+
+// rows of d neighbouring elements, any distance apart that is not less
+struct Rows {
+  at::Tensor t;
+  long long ld = 0;
+  Rows() = default;
+  Rows(const at::Tensor& x, int64_t rows, int64_t d) : t(x.reshape({rows, d})) {
+    if (t.numel() != 0 && ((d > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < d)))
+      t = t.contiguous();
+    ld = rows > 1 && t.numel() != 0 ? t.stride(0) : d;
+  }
+  void* at() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+
+int norm_code(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat ? FEEDFORWARD_FP32 : type_code(t);
+}
+
+// an argument that may be None; false with an exception set
+bool optional(PyObject* o, const char* name, at::Tensor* out) {
+  if (o == Py_None) return true;
+  const at::Tensor* const t = tensor(o, name);
+  if (!t) return false;
+  *out = *t;
+  return true;
+}
+
+struct NormInputs {
+  at::Tensor residual, block, post, gate, pre;
+  int64_t rows = 0, d = 0, gates = 1, rows_per_gate = 1;
+
+  // false with an exception set
+  bool check() {
+    const struct {
+      const char* name;
+      const at::Tensor* t;
+    } all[] = {{"residual", &residual}, {"block", &block}, {"post_weight", &post}, {"gate", &gate}, {"pre_weight", &pre}};
+    for (const auto& x : all) {
+      if (!x.t->defined()) continue;
+      const auto type = x.t->scalar_type();
+      if (!x.t->is_cuda() || (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat)) {
+        PyErr_Format(PyExc_ValueError, "%s must be a torch.half, torch.bfloat16 or torch.float tensor on the GPU", x.name);
+        return false;
+      }
+      if (x.t->layout() != at::kStrided || x.t->is_neg()) {
+        PyErr_Format(PyExc_ValueError, "%s must be a plain tensor", x.name);
+        return false;
+      }
+      if (type != residual.scalar_type() || x.t->device() != residual.device()) {
+        PyErr_Format(PyExc_ValueError, "%s must have the residual's type and device", x.name);
+        return false;
+      }
+    }
+    const int64_t dims = residual.dim();
+    if (dims < 1 || residual.size(-1) == 0) {
+      PyErr_SetString(PyExc_ValueError, "residual needs a last dimension, not 0");
+      return false;
+    }
+    d = residual.size(-1);
+    rows = residual.numel() / d;
+    if (rows > 0x7fffffff || d > 0x7fffffff) {
+      PyErr_SetString(PyExc_ValueError, "a size does not fit into a C int");
+      return false;
+    }
+    if (block.defined() && block.sizes() != residual.sizes()) {
+      PyErr_SetString(PyExc_ValueError, "block must have the residual's shape");
+      return false;
+    }
+    for (const at::Tensor* w : {&post, &pre})
+      if (w->defined() && (w->dim() != 1 || w->size(0) != d)) {
+        PyErr_Format(PyExc_ValueError, "%s must have one dimension, the residual's last", w == &post ? "post_weight" : "pre_weight");
+        return false;
+      }
+    if (!block.defined() && (post.defined() || gate.defined() || !pre.defined())) {
+      PyErr_SetString(PyExc_ValueError,
+                      block.defined() || pre.defined() ? "post_weight and gate belong to a block" : "there is neither a block nor a pre_weight");
+      return false;
+    }
+    rows_per_gate = rows > 0 ? rows : 1;
+    if (gate.defined()) {
+      // (d), or the residual's leading dimensions, ones for the others, and d
+      bool fits = gate.dim() >= 1 && gate.size(-1) == d && (gate.dim() == 1 || gate.dim() == dims);
+      if (fits && gate.dim() > 1) {
+        int64_t ones = dims - 1, shared = 1;
+        while (ones > 0 && gate.size(ones - 1) == 1) shared *= residual.size(--ones);
+        for (int64_t i = 0; i < ones; i++) fits = fits && gate.size(i) == residual.size(i);
+        rows_per_gate = shared > 0 ? shared : 1;
+      }
+      if (!fits) {
+        PyErr_SetString(PyExc_ValueError,
+                        "gate must have the shape (d,), or the residual's with ones for its last dimensions but d");
+        return false;
+      }
+    }
+    gates = rows > 0 ? rows / rows_per_gate : gate.defined() ? gate.numel() / d : 1;
+    return true;
+  }
+  int dev() const { return residual.get_device(); }
+  Rows gate_rows() const { return gate.defined() ? Rows(gate, gate.numel() / d, d) : Rows(); }
+};
+
+at::Tensor weight_of(const at::Tensor& w) { return w.defined() ? w.contiguous() : w; }
+void* at_of(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// residual_norm(residual, block, post, gate, pre, scale, eps, keep) -> (y, r, lengths); block, post,
+// gate and pre may be None, and so are then r (without a block) and y (without pre)
+PyObject* py_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8) {
+    PyErr_SetString(PyExc_TypeError, "residual_norm takes 8 arguments");
+    return nullptr;
+  }
+  NormInputs in;
+  const at::Tensor* const residual = tensor(args[0], "residual");
+  if (!residual || !optional(args[1], "block", &in.block) || !optional(args[2], "post_weight", &in.post) ||
+      !optional(args[3], "gate", &in.gate) || !optional(args[4], "pre_weight", &in.pre))
+    return nullptr;
+  in.residual = *residual;
+  const double scale = PyFloat_AsDouble(args[5]), eps = PyFloat_AsDouble(args[6]);
+  if (PyErr_Occurred()) return nullptr;
+  const int keep = PyObject_IsTrue(args[7]);
+  if (keep < 0 || !in.check()) return nullptr;
+  const int dev = in.dev();
+  void* const st = current_stream(dev);
+  at::Tensor y, r, stats;
+  Failed failed;
+  {
+    pybind11::gil_scoped_release unlocked;
+    if (in.pre.defined()) y = empty_as(in.residual, in.residual.sizes());
+    if (in.block.defined()) r = empty_as(in.residual, in.residual.sizes());
+    if (keep) stats = at::empty({in.rows, 2}, in.residual.options().requires_grad(false).dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+    const Rows res(in.residual, in.rows, in.d), gate = in.gate_rows();
+    const Rows block = in.block.defined() ? Rows(in.block, in.rows, in.d) : Rows();
+    const at::Tensor post = weight_of(in.post), pre = weight_of(in.pre);
+    failed(feedforward_norm(res.at(), res.ld, block.at(), block.ld, at_of(post), gate.at(), gate.ld,
+                            (int)in.rows_per_gate, at_of(pre), (float)scale, (float)eps, at_of(r), at_of(y),
+                            (float*)at_of(stats), in.rows, (int)in.d, norm_code(in.residual), dev, st));
+  }
+  if (failed.raise()) return nullptr;
+  PyObject* const tuple = PyTuple_New(3);
+  if (!tuple) return nullptr;
+  PyTuple_SET_ITEM(tuple, 0, THPVariable_Wrap(std::move(y)));
+  PyTuple_SET_ITEM(tuple, 1, THPVariable_Wrap(std::move(r)));
+  PyTuple_SET_ITEM(tuple, 2, THPVariable_Wrap(std::move(stats)));
+  return tuple;
+  END_HANDLE_TH_ERRORS
+}
+
+// norm_grads(dy, dr, r, block, post, gate, pre, lengths, scale, residual or None, wanted: five truth
+// values) -> the gradients of residual, block, post, gate and pre, None where not wanted; dy or dr
+// may be None
+PyObject* py_norm_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 15) {
+    PyErr_SetString(PyExc_TypeError, "norm_grads takes 15 arguments");
+    return nullptr;
+  }
+  NormInputs in;
+  at::Tensor dy, dr, stats, leaf;
+  const at::Tensor* const r = tensor(args[2], "r");
+  if (!r || !optional(args[0], "dy", &dy) || !optional(args[1], "dr", &dr) ||
+      !optional(args[3], "block", &in.block) || !optional(args[4], "post_weight", &in.post) ||
+      !optional(args[5], "gate", &in.gate) || !optional(args[6], "pre_weight", &in.pre) ||
+      !optional(args[7], "lengths", &stats) || !optional(args[9], "residual", &leaf))
+    return nullptr;
+  in.residual = *r;
+  const double scale = PyFloat_AsDouble(args[8]);
+  if (PyErr_Occurred()) return nullptr;
+  bool want[5];
+  for (int i = 0; i < 5; i++) {
+    const int w = PyObject_IsTrue(args[10 + i]);
+    if (w < 0) return nullptr;
+    want[i] = w;
+  }
+  if (!in.check()) return nullptr;
+  for (const at::Tensor* g : {&dy, &dr})
+    if (g->defined() && (g->sizes() != in.residual.sizes() || g->scalar_type() != in.residual.scalar_type() ||
+                         g->device() != in.residual.device())) {
+      PyErr_SetString(PyExc_ValueError, "dy and dr must be gradients of the outputs");
+      return nullptr;
+    }
+  if (!stats.defined() || stats.scalar_type() != at::kFloat || !stats.is_contiguous() || stats.numel() != 2 * in.rows ||
+      stats.device() != in.residual.device()) {
+    PyErr_SetString(PyExc_ValueError, "lengths must be those of the forward pass");
+    return nullptr;
+  }
+  const int dev = in.dev();
+  if (!check_capture({&leaf, &in.block, &in.post, &in.gate, &in.pre}, dev)) return nullptr;
+  void* const st = current_stream(dev);
+  at::Tensor out[5];
+  const at::Tensor* const like[5] = {&in.residual, &in.block, &in.post, &in.gate, &in.pre};
+  Failed failed;
+  {
+    pybind11::gil_scoped_release unlocked;
+    for (int i = 0; i < 5; i++)
+      if (want[i] && like[i]->defined()) out[i] = empty_as(*like[i], like[i]->sizes());
+    // without dy nothing comes back through the last norm
+    const bool back = in.pre.defined() && dy.defined(), any = back || dr.defined();
+    if (out[4].defined() && !back) out[4].zero_();
+    if (in.rows == 0 || !any) {
+      for (at::Tensor& g : out)
+        if (g.defined()) g.zero_();
+    } else {
+      const bool sums = out[2].defined() || out[3].defined() || (out[4].defined() && back);
+      const long long bytes = sums ? feedforward_norm_grad_bytes(in.rows, (int)in.d, (int)in.rows_per_gate, norm_code(in.residual)) : 0;
+      at::Tensor partials;
+      if (bytes > 0)
+        partials = at::empty({bytes / 4}, in.residual.options().requires_grad(false).dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+      const auto rows_of = [&](const at::Tensor& t) { return t.defined() ? Rows(t, in.rows, in.d) : Rows(); };
+      const Rows gdy = back ? rows_of(dy) : Rows(), gdr = rows_of(dr), rr = rows_of(in.residual), block = rows_of(in.block),
+                 gate = in.gate_rows();
+      const at::Tensor post = weight_of(in.post), pre = back ? weight_of(in.pre) : at::Tensor();
+      failed(feedforward_norm_grad(gdy.at(), gdy.ld, gdr.at(), gdr.ld, rr.at(), rr.ld, block.at(), block.ld, at_of(post),
+                                   gate.at(), gate.ld, (int)in.rows_per_gate, at_of(pre), (float)scale,
+                                   (const float*)stats.data_ptr(), at_of(out[0]), at_of(out[1]), at_of(out[2]),
+                                   at_of(out[3]), back ? at_of(out[4]) : nullptr, at_of(partials), bytes, in.rows,
+                                   (int)in.d, norm_code(in.residual), dev, st));
+    }
+  }
+  if (failed.raise()) return nullptr;
+  PyObject* const tuple = PyTuple_New(5);
+  if (!tuple) return nullptr;
+  for (int i = 0; i < 5; i++) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(std::move(out[i])));
+  return tuple;
+  END_HANDLE_TH_ERRORS
+}
+
 // What the conversion kernels may take: plain tensors on one GPU, 16-byte aligned,
 // without gradients.  (That nothing looks on is the caller's to know.)
 //
@@ -725,6 +953,8 @@ PyObject* py_pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {
     {"mul", (PyCFunction)(void (*)(void))py_mul, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void (*)(void))py_linear, METH_FASTCALL, nullptr},
+    {"residual_norm", (PyCFunction)(void (*)(void))py_residual_norm, METH_FASTCALL, nullptr},
+    {"norm_grads", (PyCFunction)(void (*)(void))py_norm_grads, METH_FASTCALL, nullptr},
     {"gated_dense", (PyCFunction)(void (*)(void))py_gated_dense, METH_FASTCALL, nullptr},
     {"gated_grads", (PyCFunction)(void (*)(void))py_gated_grads, METH_FASTCALL, nullptr},
     {"linear_dense", (PyCFunction)(void (*)(void))py_linear_dense, METH_FASTCALL, nullptr},

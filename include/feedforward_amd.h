@@ -46,6 +46,7 @@ int feedforward_gated_w4(const void *A, const void *B, void *C, const void *s, i
 /* types of matrices */
 #define FEEDFORWARD_FP16 0
 #define FEEDFORWARD_BF16 1
+#define FEEDFORWARD_FP32 2 /* norms only */
 
 /*
  * Matrices below are row-major in fp16 or bfloat16 (`type`), `ld...` elements from one row to
@@ -82,6 +83,36 @@ int feedforward_transpose(const void *in, void *out, int rows, int cols, long lo
 int feedforward_tile(int m, int n, int k, int gated, int cus, int *out);
 /* such tiles for every product of the calling thread (0 = by cost); for tests and tools */
 void feedforward_force_tile(int rows, int cols);
+
+/*
+ * The norm after a block, its gate, the residual's scale and the norm before the next block, row
+ * by row: p = block rstd(block) post, r = scale residual + gate p, y = r rstd(r) pre, with rstd(v)
+ * = 1 / sqrt(mean(v^2) + eps); fp32 inside, r and y rounded once, y from the unrounded r.  Every
+ * matrix is of one type (fp32 too), `rows` rows of d <= 16384 elements, `ld...` apart; r and y
+ * contiguous.  Null: post (no norm after the block, p = block), gate (1), pre (no norm before
+ * the next block, y is not written), block (r = residual, not written; then neither post nor
+ * gate).  gate has a row for every rows_per_gate rows.  stats, if not null, (rows x 2) floats:
+ * rstd(block) and rstd(r), which the backward pass takes.
+ */
+int feedforward_norm(const void *residual, long long ld_residual, const void *block,
+                     long long ld_block, const void *post, const void *gate, long long ld_gate,
+                     int rows_per_gate, const void *pre, float scale, float eps, void *r, void *y,
+                     float *stats, long long rows, int d, int type, int dev, void *stream);
+
+/* Its gradients from dy (null without pre) and dr (null: zero), r the forward pass's (the
+ * residual without a block).  Outputs that are null are not computed; dresidual and dblock
+ * (rows x d), dgate (a row per gate), dpost and dpre (d) are contiguous.  The sums over rows
+ * go through `partials`, at least feedforward_norm_grad_bytes(...) bytes of device memory, in
+ * an order that the sizes alone decide. */
+int feedforward_norm_grad(const void *dy, long long ld_dy, const void *dr, long long ld_dr,
+                          const void *r, long long ld_r, const void *block, long long ld_block,
+                          const void *post, const void *gate, long long ld_gate,
+                          int rows_per_gate, const void *pre, float scale, const float *stats,
+                          void *dresidual, void *dblock, void *dpost, void *dgate, void *dpre,
+                          void *partials, long long partial_bytes, long long rows, int d, int type,
+                          int dev, void *stream);
+/* -1 for sizes that are refused; no GPU touched */
+long long feedforward_norm_grad_bytes(long long rows, int d, int rows_per_gate, int type);
 
 const char *feedforward_last_error(void);
 
