@@ -70,8 +70,8 @@ __global__ __launch_bounds__(kThreads) void transpose_kernel(const half_t* in, l
   store_turned(lds, out + (size_t)c0 * ld_out + r0, ld_out, min(kTile, cols - c0));
 }
 
-// dg = dh u act'(g), du = dh act(g) of a gated product, in fp32 from the 16 bits that the
-// forward pass kept, rounded to 16 bits, as matrix instructions take them: as rows of
+// dg = dh u act'(g), du = dh act(g) of a gated product, in fp32 from the sums that the forward
+// pass kept in fp32, rounded to 16 bits, as matrix instructions take them: as rows of
 // [dg | du] for the product with the weights, and turned over for that with the inputs.
 template <bool BF>
 __global__ __launch_bounds__(kThreads) void gated_grad_kernel(GatedGradArgs p) {
@@ -86,18 +86,17 @@ __global__ __launch_bounds__(kThreads) void gated_grad_kernel(GatedGradArgs p) {
     dg.row[h] = du.row[h] = (i4){0, 0, 0, 0};
     if (!in || r >= p.m) continue;
     const i4 dh = *(const i4*)((const half_t*)p.dh + (size_t)r * p.lddh + c0 + 8 * c);
-    const half_t* const pre = (const half_t*)p.pre + (size_t)r * p.ldpre + c0 + 8 * c;
-    const i4 g = *(const i4*)pre, u = *(const i4*)(pre + p.n);
+    const float* const pre = p.pre + (size_t)r * p.ldpre + pre_col(c0 + 8 * c);
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
+      const f4 g = *(const f4*)(pre + 2 * i), u = *(const f4*)(pre + 2 * i + 16);
       f4 a, b;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int at = i + (e >> 1), by = 16 * (e & 1);
-        const float d = widen<BF>((unsigned)dh[at] >> by & 0xffffu);
+        const float d = widen<BF>((unsigned)dh[i + (e >> 1)] >> (16 * (e & 1)) & 0xffffu);
         float value, slope;
-        act_slope(widen<BF>((unsigned)g[at] >> by & 0xffffu), p.act, &value, &slope);
-        a[e] = d * widen<BF>((unsigned)u[at] >> by & 0xffffu) * slope;
+        act_slope(g[e], p.act, &value, &slope);
+        a[e] = d * u[e] * slope;
         b[e] = d * value;
       }
       const i2 ra = product_round<BF>(a), rb = product_round<BF>(b);

@@ -6,7 +6,7 @@ namespace w4a16 {
 
 struct GatedGradArgs {
   const void* dh;   // (m x n)
-  const void* pre;  // (m x 2n), the forward pass's sums
+  const float* pre;  // (m x ldpre), the forward pass's sums
   void* dgu;        // (m x 2n), zeros behind a row up to a multiple of 64 columns; or null
   void* dgu_t;      // (2n x m), zeros likewise; or null
   long long lddh, ldpre, lddgu, lddgu_t;

@@ -171,14 +171,14 @@ int feedforward_product(const void* A, const void* B, void* C, int m, int n, int
   return run_product(a, type == FEEDFORWARD_BF16, dev, (hipStream_t)stream);
 }
 
-int feedforward_gated(const void* x, const void* w, void* h, void* pre, int m, int n, int k, long long ldx,
+int feedforward_gated(const void* x, const void* w, void* h, float* pre, int m, int n, int k, long long ldx,
                       long long ldw, long long ldh, long long ldpre, int type, int activation, int dev,
                       void* stream) {
   int rc = check_sizes(m, n, k, type);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("x", x, ldx, k);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("w", w, ldw, k);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("h", h, ldh, n);
-  if (rc == FEEDFORWARD_OK && pre) rc = check_matrix("pre", pre, ldpre, 2LL * n);
+  if (rc == FEEDFORWARD_OK && pre) rc = check_matrix("pre", pre, ldpre, (n + 15LL) / 16 * 32);
   if (rc == FEEDFORWARD_OK && !act_known(activation))
     rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
@@ -191,12 +191,12 @@ int feedforward_gated(const void* x, const void* w, void* h, void* pre, int m, i
   return run_product(a, type == FEEDFORWARD_BF16, dev, (hipStream_t)stream);
 }
 
-int feedforward_gated_grad(const void* dh, const void* pre, void* dgu, void* dgu_t, int m, int n, long long lddh,
+int feedforward_gated_grad(const void* dh, const float* pre, void* dgu, void* dgu_t, int m, int n, long long lddh,
                            long long ldpre, long long lddgu, long long lddgu_t, int type, int activation, int dev,
                            void* stream) {
   int rc = check_sizes(m, n, 0, type);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("dh", dh, lddh, n);
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("pre", pre, ldpre, 2LL * n);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("pre", pre, ldpre, (n + 15LL) / 16 * 32);
   if (rc == FEEDFORWARD_OK && dgu) rc = check_matrix("dgu", dgu, lddgu, (2LL * n + 63) / 64 * 64);
   if (rc == FEEDFORWARD_OK && dgu_t) rc = check_matrix("dgu_t", dgu_t, lddgu_t, (m + 63LL) / 64 * 64);
   if (rc == FEEDFORWARD_OK && !act_known(activation))

@@ -16,7 +16,7 @@ struct ProductArgs {
   const void* A;
   const void* B;
   void* C;
-  void* pre;  // gated: null, or (M x 2n), both sums in 16 bits for the backward pass
+  float* pre;  // gated: null, or both sums for the backward pass, (M x ldpre) in the product's order
   int M, N, K;  // N: columns of C
   int lda, ldb, ldc, ldpre;
   int act;  // kActNone: not gated
@@ -58,6 +58,9 @@ __device__ __forceinline__ int gated_row(int first, int col, int n, int ldb) {
   if (row >= n) row = n - 1;
   return (row - (first >> 1)) * ldb + (at & 16 ? n * ldb : 0);
 }
+
+// where column `col` of C has its gate's sum in a row of `pre`; its partner's is 16 further on
+__host__ __device__ __forceinline__ int pre_col(int col) { return ((col >> 4) << 5) + (col & 15); }
 
 // Tiles of ff_tiles.hip: rows x columns of the product, 256 x 256 the big kernel's
 struct FfTile {

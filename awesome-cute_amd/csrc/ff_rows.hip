@@ -157,7 +157,7 @@ __global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(ProductArgs p
     if (row >= p.M || col >= p.N) continue;
     if constexpr (GATED) {
       if (p.pre)
-        *(i2*)((half_t*)p.pre + (size_t)row * p.ldpre + (kg >> 1 ? p.N : 0) + col) = product_round<BF>(v);
+        *(f4*)(p.pre + (size_t)row * p.ldpre + pre_col(col) + (kg >> 1 ? 16 : 0)) = v;
       if (kg < 2) *(i2*)((half_t*)p.C + (size_t)row * p.ldc + col) = product_round<BF>(act_mul4(v, up, p.act));
     } else {
       *(i2*)((half_t*)p.C + (size_t)row * p.ldc + col) = product_round<BF>(v);

@@ -7,7 +7,7 @@
 //     past the end of a row in its last 64-deep stage is requested at an offset past
 //     everything, and so reads as zeros, in A and in B,
 //   - gated, a tile's columns are gates and ups in turns of sixteen (gated_row), and its
-//     epilogue writes act(g) u, for the backward pass g and u as well.
+//     epilogue writes act(g) u, for the backward pass both sums as well.
 //
 // What bounds them: as there, the board's power for large products of 256 x 256 tiles, the way
 // into LDS for the others.
@@ -22,50 +22,49 @@ namespace {
 enum Form { kPlain, kGated, kGatedPre };
 
 // ROWS x COLS tile of 16-bit results on its way through LDS: a row holds COLS columns, or,
-// gated, COLS / 2 of C and with kGatedPre as many gates and ups behind them
+// gated, COLS / 2
 template <int COLS, Form FORM>
 constexpr int out_pitch() {
-  return (FORM == kPlain ? 2 * COLS : FORM == kGated ? COLS : 3 * COLS) + 16;
+  return (FORM == kPlain ? 2 * COLS : COLS) + 16;
 }
 
-// 16-byte pieces of ROWS rows (of the tile from `row0` on, at smem) to C and pre.  Rows are
-// stored below `rows`, columns below `cols` (of C).
+// 16-byte pieces of ROWS rows (of the tile from `row0` on, at smem) to C, rows below `rows`,
+// columns below `cols`
 template <int ROWS, int COLS, Form FORM, int THREADS, class RowOf>
 __device__ __forceinline__ void store_rows(const ProductArgs& p, const char* smem, int m0, int c0, int rows, int cols,
                                            RowOf row_of) {
   constexpr int kPitch = out_pitch<COLS, FORM>();
-  constexpr int kWidth = FORM == kPlain ? COLS : COLS / 2;
-  constexpr int kPieces = kWidth / 8, kSections = FORM == kGatedPre ? 3 : 1;
-#pragma unroll
-  for (int section = 0; section < kSections; section++) {
-    half_t* const out = section == 0 ? (half_t*)p.C + c0 : (half_t*)p.pre + c0 + (section - 1) * p.N;
-    const size_t ld = section == 0 ? p.ldc : p.ldpre;
+  constexpr int kPieces = (FORM == kPlain ? COLS : COLS / 2) / 8;
 #pragma unroll 8
-    for (int at = threadIdx.x; at < ROWS * kPieces; at += THREADS) {
-      const int r = at / kPieces, c = at % kPieces;
-      const int m = row_of(r);
-      if (m < rows && 8 * c < cols)
-        // nobody reads it again in this launch: keep it out of the way of A and B in L2
-        __builtin_nontemporal_store(*(const i4*)(smem + r * kPitch + section * (2 * kWidth) + 16 * c),
-                                    (i4*)(out + (size_t)(m0 + m) * ld + 8 * c));
-    }
+  for (int at = threadIdx.x; at < ROWS * kPieces; at += THREADS) {
+    const int r = at / kPieces, c = at % kPieces;
+    const int m = row_of(r);
+    if (m < rows && 8 * c < cols)
+      // nobody reads it again in this launch: keep it out of the way of A and B in L2
+      __builtin_nontemporal_store(*(const i4*)(smem + r * kPitch + 16 * c),
+                                  (i4*)((half_t*)p.C + (size_t)(m0 + m) * p.ldc + c0 + 8 * c));
   }
 }
 
-// what a lane puts into the tile's LDS image of operands j and (gated) j + 1 of a row block
+// What a lane puts into row `m` of the tile's LDS image, of operands j and (gated) j + 1 of a
+// row block: their sums at column `col` of the product's tile.  The sums that the backward pass
+// takes go to memory from here, in fp32 -- rounded to 16 bits they made the gradients 1.8
+// times as far off as the products' own roundings do, for 35 us less of 1030 (2048 x 2 x 10752
+// x 4096, forward and backward) -- and in the product's order, in which a gate's sixteen
+// columns and its partner's fill a cache line of a row.
 template <int COLS, Form FORM, bool BF>
-__device__ __forceinline__ void put(char* row, int col, f4 v, f4 next, int act) {
+__device__ __forceinline__ void put(const ProductArgs& p, char* image, int m0, int n0, int m, int col, int rows,
+                                    int cols, f4 v, f4 next) {
+  char* const row = image;
   if constexpr (FORM == kPlain) {
     *(i2*)(row + 2 * col) = product_round<BF>(v);
   } else {
-    // (col is that of the product; 16 of gates, 16 of ups)
-    const int at = 2 * (((col >> 5) << 4) + (col & 15));
-    *(i2*)(row + at) = product_round<BF>(act_mul4(v, next, act));
-    if constexpr (FORM == kGatedPre) {
-      // g and u are kept in 16 bits: the gradients that they meet are rounded to as many
-      // before the products of the backward pass, and in 32 they would be its largest read
-      *(i2*)(row + COLS + at) = product_round<BF>(v);
-      *(i2*)(row + 2 * COLS + at) = product_round<BF>(next);
+    const int at = ((col >> 5) << 4) + (col & 15);  // (col: 16 of gates, 16 of ups)
+    *(i2*)(row + 2 * at) = product_round<BF>(act_mul4(v, next, p.act));
+    if (FORM == kGatedPre && m < rows && at < cols) {
+      float* const pre = p.pre + (size_t)(m0 + m) * p.ldpre + n0 + col;
+      __builtin_nontemporal_store(v, (f4*)pre);
+      __builtin_nontemporal_store(next, (f4*)(pre + 16));
     }
   }
 }
@@ -250,8 +249,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
   for (int i = 0; i < RB; i++)
 #pragma unroll
     for (int j = 0; j < NJ; j += FORM == kPlain ? 1 : 2)
-      put<TN, FORM, BF>(out + 16 * i * out_pitch<TN, FORM>(), 16 * NJ * wn + 16 * j + 4 * kg, acc[i][j],
-                        acc[i][FORM == kPlain ? j : j + 1], p.act);
+      put<TN, FORM, BF>(p, out + 16 * i * out_pitch<TN, FORM>(), m0, n0, 16 * RB * wm + 16 * i + nu,
+                        16 * NJ * wn + 16 * j + 4 * kg, rows, cols, acc[i][j], acc[i][FORM == kPlain ? j : j + 1]);
   __syncthreads();
   store_rows<TM, TN, FORM, Sh::kThreads>(p, smem, m0, FORM == kPlain ? n0 : n0 >> 1, rows, cols,
                                          [](int r) { return r; });
@@ -263,7 +262,7 @@ struct BigShape {
   static constexpr int kSlabA = 256 * 128, kSlab = 2 * kSlabA;
   static constexpr int kTA = 8, kTB = 8;  // load instructions per wave and slab
   static constexpr int kLds = 2 * kSlab;  // (half a tile of results is less)
-  static_assert(128 * out_pitch<256, kGatedPre>() <= kLds && 128 * out_pitch<256, kPlain>() <= kLds, "");
+  static_assert(128 * out_pitch<256, kPlain>() <= kLds, "");
 };
 
 }  // namespace
@@ -339,8 +338,9 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int o = 0; o < 8; o += FORM == kPlain ? 1 : 2)
-        put<256, FORM, BF>(base + (64 * wm + 16 * i + nu) * kPitch, 128 * wn + 16 * o + 4 * kg, acc[4 * half + i][o],
-                           acc[4 * half + i][FORM == kPlain ? o : o + 1], p.act);
+        put<256, FORM, BF>(p, base + (64 * wm + 16 * i + nu) * kPitch, m0, n0, 128 * wm + 16 * (4 * half + i) + nu,
+                           128 * wn + 16 * o + 4 * kg, rows, cols, acc[4 * half + i][o],
+                           acc[4 * half + i][FORM == kPlain ? o : o + 1]);
     __syncthreads();
     store_rows<128, 256, FORM, 256>(p, base, m0, FORM == kPlain ? n0 : n0 >> 1, rows, cols,
                                     [&](int r) { return (r >> 6) * 128 + half * 64 + (r & 63); });

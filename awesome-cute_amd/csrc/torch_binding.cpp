@@ -13,7 +13,9 @@
 // the stream's queue, a stream's first call allocates, and an allocation may
 // wait for another thread's.
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
@@ -30,6 +32,9 @@
 #include "../../include/streamk_amd.h"
 
 namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 const at::Tensor* tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) {
@@ -308,7 +313,8 @@ PyObject* py_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 // ---- dense feed-forward products (feedforward_amd.h) with fp16 or bfloat16 tensors.  A pass that
 // takes several launches makes all of them here, its temporaries among them: they come from torch's
-// allocator on the current stream and go back to it in that stream's order.
+// allocator on the current stream and go back to it in that stream's order.  The autograd functions
+// are C++ as well: as Python's they took the host 50 us more a pass than the kernels of a small one.
 
 // a matrix as the kernels address it: rows that start on 16 bytes
 struct Matrix {
@@ -329,269 +335,312 @@ struct Matrix {
 
 long long up64(long long x) { return (x + 63) / 64 * 64; }
 
-// set by a pass that failed, raised once the interpreter lock is held again
-struct Failed {
-  int rc = 0;
-  bool operator()(int code) {
-    rc = code;
-    return code != FEEDFORWARD_OK;
-  }
-  bool raise() const {
-    if (rc == FEEDFORWARD_OK) return false;
-    PyErr_SetString(rc == FEEDFORWARD_ERR_SHAPE ? PyExc_ValueError : PyExc_RuntimeError, feedforward_last_error());
-    return true;
-  }
-};
+void feedforward_check(int rc) {
+  TORCH_CHECK_VALUE(rc != FEEDFORWARD_ERR_SHAPE, feedforward_last_error());
+  TORCH_CHECK(rc == FEEDFORWARD_OK, feedforward_last_error());
+}
 
-// x (..., k) and w (rows, k); false with an exception set
-bool check_dense(const at::Tensor& x, const at::Tensor& w, const char* x_name) {
+// x (..., k) and w (rows, k)
+void check_dense(const at::Tensor& x, const at::Tensor& w) {
   for (const at::Tensor* t : {&x, &w}) {
-    const char* const name = t == &x ? x_name : "weight";
-    if (!t->is_cuda() || (t->scalar_type() != at::kHalf && t->scalar_type() != at::kBFloat16)) {
-      PyErr_Format(PyExc_ValueError, "%s must be a torch.half or torch.bfloat16 tensor on the GPU", name);
-      return false;
-    }
-    if (t->layout() != at::kStrided || t->is_neg() || t->is_conj()) {
-      PyErr_Format(PyExc_ValueError, "%s must be a plain tensor", name);
-      return false;
-    }
+    const char* const name = t == &x ? "x" : "weight";
+    TORCH_CHECK_VALUE(t->is_cuda() && (t->scalar_type() == at::kHalf || t->scalar_type() == at::kBFloat16), name,
+                      " must be a torch.half or torch.bfloat16 tensor on the GPU");
+    TORCH_CHECK_VALUE(t->layout() == at::kStrided && !t->is_neg() && !t->is_conj(), name, " must be a plain tensor");
   }
-  if (x.scalar_type() != w.scalar_type() || x.device() != w.device()) {
-    PyErr_Format(PyExc_ValueError, "%s and weight must have one type and one device", x_name);
-    return false;
-  }
-  if (x.dim() < 1 || w.dim() != 2 || x.size(-1) != w.size(1) || w.size(1) == 0) {
-    PyErr_Format(PyExc_ValueError, "weight must have two dimensions, the second one %s's last, not 0", x_name);
-    return false;
-  }
-  if (w.size(0) > 0x7fffffff || w.size(1) > 0x7fffffff || x.numel() / w.size(1) > 0x7fffffff) {
-    PyErr_SetString(PyExc_ValueError, "a size does not fit into a C int");
-    return false;
-  }
-  return true;
+  TORCH_CHECK_VALUE(x.scalar_type() == w.scalar_type() && x.device() == w.device(),
+                    "x and weight must have one type and one device");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(1) != 0,
+                    "weight must have two dimensions, the second one x's last, not 0");
+  TORCH_CHECK_VALUE(w.size(0) <= 0x7fffffff && w.size(1) <= 0x7fffffff && x.numel() / w.size(1) <= 0x7fffffff,
+                    "a size does not fit into a C int");
 }
 
 int type_code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? FEEDFORWARD_BF16 : FEEDFORWARD_FP16; }
 
-at::Tensor empty_as(const at::Tensor& like, at::IntArrayRef shape) {
-  return at::empty(shape, like.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+at::TensorOptions options_as(const at::Tensor& like) {
+  return like.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+}
+at::Tensor empty_as(const at::Tensor& like, at::IntArrayRef shape) { return at::empty(shape, options_as(like)); }
+
+at::Tensor empty_rows(const at::Tensor& x, int64_t columns) {
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = columns;
+  return empty_as(x, shape);
 }
 
 // A backward pass that is captured into a graph while an eager graph of the same leaves is alive:
 // a leaf's accumulator lives as long as any graph that ends in it and belongs to the stream that was
 // current when it was made.  The engine would make that stream wait for the captured one, which draws
 // it into the capture without a way back, and the capture's end takes the process with it.  Refused
-// here, before the engine gets there; false with an exception set.
-bool check_capture(std::initializer_list<const at::Tensor*> inputs, int dev) {
+// here, before the engine gets there.
+void check_capture(std::initializer_list<const at::Tensor*> inputs, int dev) {
   const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev);
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return true;
+  if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
   for (const at::Tensor* t : inputs) {
     if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
     const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
     const auto stream = accumulator ? accumulator->stream() : std::nullopt;
     // (by number: torch names the device of one of them CUDA, of the other HIP)
-    if (!stream || (stream->id() == now.id() && stream->device_index() == dev)) continue;
-    PyErr_SetString(PyExc_RuntimeError,
-                    "the stream is being captured, and an eager graph of the same leaf, made on another stream, is "
-                    "alive: free what was computed from it before the capture, or compute it on this stream");
-    return false;
+    TORCH_CHECK(!stream || (stream->id() == now.id() && stream->device_index() == dev),
+                "the stream is being captured, and an eager graph of the same leaf, made on another stream, is "
+                "alive: free what was computed from it before the capture, or compute it on this stream");
   }
-  return true;
 }
 
-PyObject* pair_of(at::Tensor&& a, at::Tensor&& b) {
-  PyObject* const tuple = PyTuple_New(2);
-  if (!tuple) return nullptr;
-  PyTuple_SET_ITEM(tuple, 0, THPVariable_Wrap(std::move(a)));  // (None where undefined)
-  PyTuple_SET_ITEM(tuple, 1, THPVariable_Wrap(std::move(b)));
-  return tuple;
+// The gradients that a backward pass returns, where that is itself to be differentiated: no kernel
+// does, and whoever asks for it is told
+variable_list once_differentiable(variable_list&& grads, const char* name) {
+  if (!c10::GradMode::is_enabled()) return std::move(grads);
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once",
+                                                               (int)grads.size());
+  variable_list marked;
+  for (at::Tensor& g : grads) marked.push_back(g.defined() ? g.detach().set_requires_grad(true) : g);
+  return (*error)(std::move(marked));
 }
 
-// gated_dense(x, weight, activation, keep) -> (h, both sums or None)
-PyObject* py_gated_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  HANDLE_TH_ERRORS
-  if (nargs != 4) {
-    PyErr_SetString(PyExc_TypeError, "gated_dense takes 4 arguments");
-    return nullptr;
-  }
-  const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
-  int act;
-  if (!x || !w || !to_int(args[2], &act) || !check_dense(*x, *w, "x")) return nullptr;
-  const int keep = PyObject_IsTrue(args[3]);
-  if (keep < 0) return nullptr;
-  if (w->size(0) % 2 != 0) {
-    PyErr_SetString(PyExc_ValueError, "weight must hold the rows of gate and, behind them, as many of up");
-    return nullptr;
-  }
-  const int64_t n = w->size(0) / 2, k = w->size(1), m = x->numel() / k;
-  const int dev = x->get_device();
-  void* const st = current_stream(dev);
-  at::Tensor h, pre;
-  Failed failed;
-  {
-    pybind11::gil_scoped_release unlocked;
-    c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
-    shape.back() = n;
-    h = empty_as(*x, shape);
-    if (keep) pre = empty_as(*x, {m, 2 * n});
-    const Matrix a(x->reshape({m, k})), b(*w);
-    failed(feedforward_gated(a.at(), b.at(), h.data_ptr(), keep ? pre.data_ptr() : nullptr, (int)m, (int)n, (int)k,
-                             a.ld, b.ld, n, 2 * n, type_code(*x), act, dev, st));
-  }
-  if (failed.raise()) return nullptr;
-  return pair_of(std::move(h), std::move(pre));
-  END_HANDLE_TH_ERRORS
+// act(x G^T) * (x U^T), and with `keep` both sums (otherwise undefined)
+std::pair<at::Tensor, at::Tensor> gated_forward(const at::Tensor& x, const at::Tensor& w, int act, bool keep) {
+  check_dense(x, w);
+  TORCH_CHECK_VALUE(w.size(0) % 2 == 0, "weight must hold the rows of gate and, behind them, as many of up");
+  const int64_t n = w.size(0) / 2, k = w.size(1), m = x.numel() / k, ldpre = (n + 15) / 16 * 32;
+  const int dev = x.get_device();
+  at::Tensor h = empty_rows(x, n), pre;
+  if (keep) pre = at::empty({m, ldpre}, options_as(x).dtype(at::kFloat));
+  const Matrix a(x.reshape({m, k})), b(w);
+  feedforward_check(feedforward_gated(a.at(), b.at(), h.data_ptr(), keep ? (float*)pre.data_ptr() : nullptr, (int)m,
+                                      (int)n, (int)k, a.ld, b.ld, n, ldpre, type_code(x), act, dev,
+                                      current_stream(dev)));
+  return {h, pre};
 }
 
-// linear_dense(x, weight) -> x weight^T
-PyObject* py_linear_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  HANDLE_TH_ERRORS
-  if (nargs != 2) {
-    PyErr_SetString(PyExc_TypeError, "linear_dense takes 2 arguments");
-    return nullptr;
-  }
-  const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
-  if (!x || !w || !check_dense(*x, *w, "x")) return nullptr;
-  const int64_t n = w->size(0), k = w->size(1), m = x->numel() / k;
-  const int dev = x->get_device();
-  void* const st = current_stream(dev);
-  at::Tensor y;
-  Failed failed;
-  {
-    pybind11::gil_scoped_release unlocked;
-    c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
-    shape.back() = n;
-    y = empty_as(*x, shape);
-    const Matrix a(x->reshape({m, k})), b(*w);
-    failed(feedforward_product(a.at(), b.at(), y.data_ptr(), (int)m, (int)n, (int)k, a.ld, b.ld, n, type_code(*x),
-                               dev, st));
-  }
-  if (failed.raise()) return nullptr;
-  return THPVariable_Wrap(std::move(y));
-  END_HANDLE_TH_ERRORS
+at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w) {
+  check_dense(x, w);
+  const int64_t n = w.size(0), k = w.size(1), m = x.numel() / k;
+  const int dev = x.get_device();
+  at::Tensor y = empty_rows(x, n);
+  const Matrix a(x.reshape({m, k})), b(w);
+  feedforward_check(feedforward_product(a.at(), b.at(), y.data_ptr(), (int)m, (int)n, (int)k, a.ld, b.ld, n,
+                                        type_code(x), dev, current_stream(dev)));
+  return y;
 }
 
 // The gradients of rows x (m, k) and weights w (r, k) of a product, from its gradient as rows
 // (d, m x r, zeros behind it up to a multiple of 64 columns unless `depth` is r) and turned over
 // (d_t, r x m, zeros likewise).  dx = d w and dw = d_t x are products over r and m, of the
 // transposes of w and x.
-bool product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, int64_t depth, const at::Tensor& d_t,
-                   at::Tensor* dx, at::Tensor* dw, int dev, void* st, Failed& failed) {
+void product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, int64_t depth, const at::Tensor& d_t,
+                   at::Tensor* dx, at::Tensor* dw) {
   const int64_t m = x.size(0), k = x.size(1), r = w.size(0);
-  const int type = type_code(x);
-  if (dx) {
+  const int type = type_code(x), dev = x.get_device();
+  void* const st = current_stream(dev);
+  if (dx->defined()) {
     const Matrix b(w);
     const at::Tensor turned = empty_as(x, {k, up64(r)});
-    if (failed(feedforward_transpose(b.at(), turned.data_ptr(), (int)r, (int)k, b.ld, up64(r), dev, st))) return false;
-    if (failed(feedforward_product(d.at(), turned.data_ptr(), dx->data_ptr(), (int)m, (int)k, (int)depth, d.ld,
-                                   up64(r), k, type, dev, st)))
-      return false;
+    feedforward_check(feedforward_transpose(b.at(), turned.data_ptr(), (int)r, (int)k, b.ld, up64(r), dev, st));
+    feedforward_check(feedforward_product(d.at(), turned.data_ptr(), dx->data_ptr(), (int)m, (int)k, (int)depth, d.ld,
+                                          up64(r), k, type, dev, st));
   }
-  if (dw) {
+  if (dw->defined()) {
     const Matrix a(x);
     const at::Tensor turned = empty_as(x, {k, up64(m)});
-    if (failed(feedforward_transpose(a.at(), turned.data_ptr(), (int)m, (int)k, a.ld, up64(m), dev, st))) return false;
-    if (failed(feedforward_product(d_t.data_ptr(), turned.data_ptr(), dw->data_ptr(), (int)r, (int)k, (int)up64(m),
-                                   up64(m), up64(m), k, type, dev, st)))
-      return false;
+    feedforward_check(feedforward_transpose(a.at(), turned.data_ptr(), (int)m, (int)k, a.ld, up64(m), dev, st));
+    feedforward_check(feedforward_product(d_t.data_ptr(), turned.data_ptr(), dw->data_ptr(), (int)r, (int)k,
+                                          (int)up64(m), up64(m), up64(m), k, type, dev, st));
   }
-  return true;
 }
 
-// gated_grads(dh, sums, x, weight, activation, whether dx, whether dweight) -> (dx, dweight)
-PyObject* py_gated_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+// -> (dx, dweight), undefined where not wanted
+std::pair<at::Tensor, at::Tensor> gated_backward(const at::Tensor& dh, const at::Tensor& pre, const at::Tensor& x,
+                                                 const at::Tensor& w, int act, bool want_x, bool want_w) {
+  check_dense(x, w);
+  const int64_t n = w.size(0) / 2, k = w.size(1), m = x.numel() / k, ldpre = (n + 15) / 16 * 32;
+  TORCH_CHECK_VALUE(dh.scalar_type() == x.scalar_type() && dh.device() == x.device() && dh.dim() >= 1 &&
+                        dh.size(-1) == n && dh.numel() == m * n && pre.scalar_type() == at::kFloat &&
+                        pre.device() == x.device() && pre.numel() == m * ldpre && pre.is_contiguous(),
+                    "dh and the sums must be those of x and weight");
+  const int dev = x.get_device();
+  check_capture({&x, &w}, dev);
+  at::Tensor dx, dw, turned;
+  if (want_x) dx = empty_as(x, x.sizes());
+  if (want_w) dw = empty_as(w, w.sizes());
+  if (m == 0 || n == 0) {
+    if (want_x) dx.zero_();
+    if (want_w) dw.zero_();
+  } else if (want_x || want_w) {
+    const Matrix d(dh.reshape({m, n}));
+    Matrix dgu;
+    if (want_x) dgu = Matrix(empty_as(x, {m, up64(2 * n)}));
+    if (want_w) turned = empty_as(x, {2 * n, up64(m)});
+    feedforward_check(feedforward_gated_grad(d.at(), (const float*)pre.data_ptr(), want_x ? dgu.at() : nullptr,
+                                             want_w ? turned.data_ptr() : nullptr, (int)m, (int)n, d.ld, ldpre,
+                                             up64(2 * n), up64(m), type_code(x), act, dev, current_stream(dev)));
+    at::Tensor rows_dx = want_x ? dx.view({m, k}) : dx;
+    product_grads(x.reshape({m, k}), w, dgu, up64(2 * n), turned, &rows_dx, &dw);
+  }
+  return {dx, dw};
+}
+
+std::pair<at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w,
+                                                  bool want_x, bool want_w) {
+  check_dense(x, w);
+  const int64_t n = w.size(0), k = w.size(1), m = x.numel() / k;
+  TORCH_CHECK_VALUE(dy.scalar_type() == x.scalar_type() && dy.device() == x.device() && dy.dim() >= 1 &&
+                        dy.size(-1) == n && dy.numel() == m * n,
+                    "dy must be that of x and weight");
+  const int dev = x.get_device();
+  check_capture({&x, &w}, dev);
+  at::Tensor dx, dw, turned;
+  if (want_x) dx = empty_as(x, x.sizes());
+  if (want_w) dw = empty_as(w, w.sizes());
+  if (m == 0 || n == 0) {
+    if (want_x) dx.zero_();
+    if (want_w) dw.zero_();
+  } else if (want_x || want_w) {
+    const Matrix d(dy.reshape({m, n}));
+    if (want_w) {
+      turned = empty_as(x, {n, up64(m)});
+      feedforward_check(feedforward_transpose(d.at(), turned.data_ptr(), (int)m, (int)n, d.ld, up64(m), dev,
+                                              current_stream(dev)));
+    }
+    at::Tensor rows_dx = want_x ? dx.view({m, k}) : dx;
+    product_grads(x.reshape({m, k}), w, d, n, turned, &rows_dx, &dw);
+  }
+  return {dx, dw};
+}
+
+struct GatedFunction : torch::autograd::Function<GatedFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, int64_t act) {
+    auto [h, pre] = gated_forward(x, w, (int)act, true);
+    ctx->save_for_backward({x, w, pre});
+    ctx->saved_data["act"] = act;
+    return h;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list out(3);
+    if (grads[0].defined()) {
+      c10::AutoGradMode off(false);
+      std::tie(out[0], out[1]) = gated_backward(grads[0], saved[2], saved[0], saved[1], (int)ctx->saved_data["act"].toInt(),
+                                                ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    }
+    return once_differentiable(std::move(out), "gated");
+  }
+};
+
+struct LinearFunction : torch::autograd::Function<LinearFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w) {
+    ctx->save_for_backward({x, w});
+    return linear_forward(x, w);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list out(2);
+    if (grads[0].defined()) {
+      c10::AutoGradMode off(false);
+      std::tie(out[0], out[1]) = linear_backward(grads[0], saved[0], saved[1], ctx->needs_input_grad(0), ctx->needs_input_grad(1));
+    }
+    return once_differentiable(std::move(out), "linear");
+  }
+};
+
+PyObject* tuple_of(std::initializer_list<at::Tensor> tensors) {
+  PyObject* const tuple = PyTuple_New((Py_ssize_t)tensors.size());
+  if (!tuple) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : tensors) PyTuple_SET_ITEM(tuple, i++, THPVariable_Wrap(t));  // (None where undefined)
+  return tuple;
+}
+
+bool differentiated(std::initializer_list<const at::Tensor*> inputs) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : inputs)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+bool takes(Py_ssize_t nargs, Py_ssize_t want, const char* name) {
+  if (nargs == want) return true;
+  PyErr_Format(PyExc_TypeError, "%s takes %d arguments", name, (int)want);
+  return false;
+}
+
+// gated_dense(x, weight, activation) -> h, with what its gradients need where they are wanted
+PyObject* py_gated_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 7) {
-    PyErr_SetString(PyExc_TypeError, "gated_grads takes 7 arguments");
-    return nullptr;
-  }
-  const at::Tensor *dh = tensor(args[0], "dh"), *pre = tensor(args[1], "sums"), *x = tensor(args[2], "x"),
-                   *w = tensor(args[3], "weight");
+  if (!takes(nargs, 3, "gated_dense")) return nullptr;
+  const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
   int act;
-  if (!dh || !pre || !x || !w || !to_int(args[4], &act) || !check_dense(*x, *w, "x")) return nullptr;
-  const int want_x = PyObject_IsTrue(args[5]), want_w = PyObject_IsTrue(args[6]);
-  if (want_x < 0 || want_w < 0) return nullptr;
-  const int64_t n = w->size(0) / 2, k = w->size(1), m = x->numel() / k;
-  const auto fits = [&](const at::Tensor& t, int64_t columns) {
-    return t.scalar_type() == x->scalar_type() && t.device() == x->device() && t.dim() >= 1 &&
-           t.size(-1) == columns && t.numel() == m * columns;
-  };
-  if (!fits(*dh, n) || !fits(*pre, 2 * n) || !pre->is_contiguous()) {
-    PyErr_SetString(PyExc_ValueError, "dh and the sums must be those of x and weight");
-    return nullptr;
-  }
-  const int dev = x->get_device();
-  if (!check_capture({x, w}, dev)) return nullptr;
-  void* const st = current_stream(dev);
-  at::Tensor dx, dw;
-  Failed failed;
+  if (!x || !w || !to_int(args[2], &act)) return nullptr;
+  at::Tensor h;
   {
     pybind11::gil_scoped_release unlocked;
-    if (want_x) dx = empty_as(*x, x->sizes());
-    if (want_w) dw = empty_as(*w, w->sizes());
-    if (m == 0) {
-      if (want_w) dw.zero_();
-    } else if (want_x || want_w) {
-      const Matrix d(dh->reshape({m, n}));
-      Matrix dgu;
-      at::Tensor turned;
-      if (want_x) dgu = Matrix(empty_as(*x, {m, up64(2 * n)}));
-      if (want_w) turned = empty_as(*x, {2 * n, up64(m)});
-      at::Tensor flat_dx = want_x ? dx.view({m, k}) : dx;
-      if (!failed(feedforward_gated_grad(d.at(), pre->data_ptr(), want_x ? dgu.at() : nullptr,
-                                         want_w ? turned.data_ptr() : nullptr, (int)m, (int)n, d.ld, 2 * n,
-                                         up64(2 * n), up64(m), type_code(*x), act, dev, st)))
-        product_grads(x->reshape({m, k}), *w, dgu, up64(2 * n), turned, want_x ? &flat_dx : nullptr,
-                      want_w ? &dw : nullptr, dev, st, failed);
-    }
+    h = differentiated({x, w}) ? GatedFunction::apply(*x, *w, (int64_t)act) : gated_forward(*x, *w, act, false).first;
   }
-  if (failed.raise()) return nullptr;
-  return pair_of(std::move(dx), std::move(dw));
+  return THPVariable_Wrap(std::move(h));
   END_HANDLE_TH_ERRORS
 }
 
-// linear_grads(dy, x, weight, whether dx, whether dweight) -> (dx, dweight)
-PyObject* py_linear_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+// linear_dense(x, weight) -> x weight^T, likewise
+PyObject* py_linear_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 5) {
-    PyErr_SetString(PyExc_TypeError, "linear_grads takes 5 arguments");
-    return nullptr;
-  }
-  const at::Tensor *dy = tensor(args[0], "dy"), *x = tensor(args[1], "x"), *w = tensor(args[2], "weight");
-  if (!dy || !x || !w || !check_dense(*x, *w, "x")) return nullptr;
-  const int want_x = PyObject_IsTrue(args[3]), want_w = PyObject_IsTrue(args[4]);
-  if (want_x < 0 || want_w < 0) return nullptr;
-  const int64_t n = w->size(0), k = w->size(1), m = x->numel() / k;
-  if (dy->scalar_type() != x->scalar_type() || dy->device() != x->device() || dy->dim() < 1 || dy->size(-1) != n ||
-      dy->numel() != m * n) {
-    PyErr_SetString(PyExc_ValueError, "dy must be that of x and weight");
-    return nullptr;
-  }
-  const int dev = x->get_device();
-  if (!check_capture({x, w}, dev)) return nullptr;
-  void* const st = current_stream(dev);
-  at::Tensor dx, dw;
-  Failed failed;
+  if (!takes(nargs, 2, "linear_dense")) return nullptr;
+  const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
+  if (!x || !w) return nullptr;
+  at::Tensor y;
   {
     pybind11::gil_scoped_release unlocked;
-    if (want_x) dx = empty_as(*x, x->sizes());
-    if (want_w) dw = empty_as(*w, w->sizes());
-    if (m == 0 || n == 0) {
-      if (want_x) dx.zero_();
-      if (want_w) dw.zero_();
-    } else if (want_x || want_w) {
-      const Matrix d(dy->reshape({m, n}));
-      at::Tensor turned;
-      if (want_w) turned = empty_as(*x, {n, up64(m)});
-      at::Tensor flat_dx = want_x ? dx.view({m, k}) : dx;
-      if (!want_w || !failed(feedforward_transpose(d.at(), turned.data_ptr(), (int)m, (int)n, d.ld, up64(m), dev, st)))
-        product_grads(x->reshape({m, k}), *w, d, n, turned, want_x ? &flat_dx : nullptr, want_w ? &dw : nullptr, dev,
-                      st, failed);
-    }
+    y = differentiated({x, w}) ? LinearFunction::apply(*x, *w) : linear_forward(*x, *w);
   }
-  if (failed.raise()) return nullptr;
-  return pair_of(std::move(dx), std::move(dw));
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_sums(x, weight, activation) -> (h, both sums), gated_grads(dh, sums, x, weight, activation)
+// and linear_grads(dy, x, weight) -> (dx, dweight): the passes by themselves, for compilers
+PyObject* py_gated_sums(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (!takes(nargs, 3, "gated_sums")) return nullptr;
+  const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
+  int act;
+  if (!x || !w || !to_int(args[2], &act)) return nullptr;
+  std::pair<at::Tensor, at::Tensor> out;
+  {
+    pybind11::gil_scoped_release unlocked;
+    out = gated_forward(*x, *w, act, true);
+  }
+  return tuple_of({out.first, out.second});
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_gated_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (!takes(nargs, 5, "gated_grads")) return nullptr;
+  const at::Tensor *dh = tensor(args[0], "dh"), *pre = tensor(args[1], "sums"), *x = tensor(args[2], "x"),
+                   *w = tensor(args[3], "weight");
+  int act;
+  if (!dh || !pre || !x || !w || !to_int(args[4], &act)) return nullptr;
+  std::pair<at::Tensor, at::Tensor> out;
+  {
+    pybind11::gil_scoped_release unlocked;
+    out = gated_backward(*dh, *pre, *x, *w, act, true, true);
+  }
+  return tuple_of({out.first, out.second});
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_linear_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (!takes(nargs, 3, "linear_grads")) return nullptr;
+  const at::Tensor *dy = tensor(args[0], "dy"), *x = tensor(args[1], "x"), *w = tensor(args[2], "weight");
+  if (!dy || !x || !w) return nullptr;
+  std::pair<at::Tensor, at::Tensor> out;
+  {
+    pybind11::gil_scoped_release unlocked;
+    out = linear_backward(*dy, *x, *w, true, true);
+  }
+  return tuple_of({out.first, out.second});
   END_HANDLE_TH_ERRORS
 }
 
@@ -602,7 +651,9 @@ struct Rows {
   at::Tensor t;
   long long ld = 0;
   Rows() = default;
-  Rows(const at::Tensor& x, int64_t rows, int64_t d) : t(x.reshape({rows, d})) {
+  Rows(const at::Tensor& x, int64_t rows, int64_t d) {
+    if (!x.defined()) return;
+    t = x.reshape({rows, d});
     if (t.numel() != 0 && ((d > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < d)))
       t = t.contiguous();
     ld = rows > 1 && t.numel() != 0 ? t.stride(0) : d;
@@ -614,6 +665,154 @@ int norm_code(const at::Tensor& t) {
   return t.scalar_type() == at::kFloat ? FEEDFORWARD_FP32 : type_code(t);
 }
 
+struct NormInputs {
+  at::Tensor residual, block, post, gate, pre;  // (the last four may be undefined)
+  int64_t rows = 0, d = 0, rows_per_gate = 1;
+
+  void check() {
+    const std::pair<const char*, const at::Tensor*> all[] = {
+        {"residual", &residual}, {"block", &block}, {"post_weight", &post}, {"gate", &gate}, {"pre_weight", &pre}};
+    for (const auto& [name, t] : all) {
+      if (!t->defined()) continue;
+      const auto type = t->scalar_type();
+      TORCH_CHECK_VALUE(t->is_cuda() && (type == at::kHalf || type == at::kBFloat16 || type == at::kFloat), name,
+                        " must be a torch.half, torch.bfloat16 or torch.float tensor on the GPU");
+      TORCH_CHECK_VALUE(t->layout() == at::kStrided && !t->is_neg(), name, " must be a plain tensor");
+      TORCH_CHECK_VALUE(type == residual.scalar_type() && t->device() == residual.device(), name,
+                        " must have the residual's type and device");
+    }
+    const int64_t dims = residual.dim();
+    TORCH_CHECK_VALUE(dims >= 1 && residual.size(-1) != 0, "residual needs a last dimension, not 0");
+    d = residual.size(-1);
+    rows = residual.numel() / d;
+    TORCH_CHECK_VALUE(rows <= 0x7fffffff && d <= 0x7fffffff, "a size does not fit into a C int");
+    TORCH_CHECK_VALUE(!block.defined() || block.sizes() == residual.sizes(), "block must have the residual's shape");
+    for (const at::Tensor* w : {&post, &pre})
+      TORCH_CHECK_VALUE(!w->defined() || (w->dim() == 1 && w->size(0) == d), w == &post ? "post_weight" : "pre_weight",
+                        " must have one dimension, the residual's last");
+    TORCH_CHECK_VALUE(block.defined() || (!post.defined() && !gate.defined()), "post_weight and gate belong to a block");
+    TORCH_CHECK_VALUE(block.defined() || pre.defined(), "there is neither a block nor a pre_weight");
+    rows_per_gate = rows > 0 ? rows : 1;
+    if (!gate.defined()) return;
+    // (d), or the residual's leading dimensions, ones for the others, and d
+    bool fits = gate.dim() >= 1 && gate.size(-1) == d && (gate.dim() == 1 || gate.dim() == dims);
+    if (fits && gate.dim() > 1) {
+      int64_t ones = dims - 1, shared = 1;
+      while (ones > 0 && gate.size(ones - 1) == 1) shared *= residual.size(--ones);
+      for (int64_t i = 0; i < ones; i++) fits = fits && gate.size(i) == residual.size(i);
+      rows_per_gate = shared > 0 ? shared : 1;
+    }
+    TORCH_CHECK_VALUE(fits, "gate must have the shape (d,), or the residual's with ones for its last dimensions but d");
+  }
+  int dev() const { return residual.get_device(); }
+  Rows gate_rows() const { return gate.defined() ? Rows(gate, gate.numel() / d, d) : Rows(); }
+};
+
+at::Tensor weight_of(const at::Tensor& w) { return w.defined() ? w.contiguous() : w; }
+void* at_of(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct NormOutputs {
+  at::Tensor y, r, lengths;
+};
+
+NormOutputs norm_forward(NormInputs& in, double scale, double eps, bool keep) {
+  in.check();
+  const int dev = in.dev();
+  NormOutputs out;
+  if (in.pre.defined()) out.y = empty_as(in.residual, in.residual.sizes());
+  if (in.block.defined()) out.r = empty_as(in.residual, in.residual.sizes());
+  if (keep) out.lengths = at::empty({in.rows, 2}, options_as(in.residual).dtype(at::kFloat));
+  const Rows res(in.residual, in.rows, in.d), block(in.block, in.rows, in.d), gate = in.gate_rows();
+  const at::Tensor post = weight_of(in.post), pre = weight_of(in.pre);
+  feedforward_check(feedforward_norm(res.at(), res.ld, block.at(), block.ld, at_of(post), gate.at(), gate.ld,
+                                     (int)in.rows_per_gate, at_of(pre), (float)scale, (float)eps, at_of(out.r),
+                                     at_of(out.y), (float*)at_of(out.lengths), in.rows, (int)in.d,
+                                     norm_code(in.residual), dev, current_stream(dev)));
+  return out;
+}
+
+// The gradients of residual, block, post, gate and pre, undefined where not wanted; `in.residual` is the
+// forward pass's r.  dy or dr may be undefined; `leaf` is the residual that went in, or undefined.
+std::array<at::Tensor, 5> norm_backward(const at::Tensor& dy, const at::Tensor& dr, NormInputs& in,
+                                        const at::Tensor& lengths, double scale, const at::Tensor& leaf,
+                                        const std::array<bool, 5>& want) {
+  in.check();
+  for (const at::Tensor* g : {&dy, &dr})
+    TORCH_CHECK_VALUE(!g->defined() || (g->sizes() == in.residual.sizes() && g->scalar_type() == in.residual.scalar_type() &&
+                                        g->device() == in.residual.device()),
+                      "dy and dr must be gradients of the outputs");
+  TORCH_CHECK_VALUE(lengths.defined() && lengths.scalar_type() == at::kFloat && lengths.is_contiguous() &&
+                        lengths.numel() == 2 * in.rows && lengths.device() == in.residual.device(),
+                    "lengths must be those of the forward pass");
+  const int dev = in.dev();
+  check_capture({&leaf, &in.block, &in.post, &in.gate, &in.pre}, dev);
+  std::array<at::Tensor, 5> out;
+  const at::Tensor* const like[5] = {&in.residual, &in.block, &in.post, &in.gate, &in.pre};
+  for (int i = 0; i < 5; i++)
+    if (want[i] && like[i]->defined()) out[i] = empty_as(*like[i], like[i]->sizes());
+  // without dy nothing comes back through the last norm
+  const bool back = in.pre.defined() && dy.defined();
+  if (in.rows == 0 || (!back && !dr.defined())) {
+    for (at::Tensor& g : out)
+      if (g.defined()) g.zero_();
+    return out;
+  }
+  if (out[4].defined() && !back) out[4].zero_();
+  at::Tensor partials;
+  long long bytes = 0;
+  if (out[2].defined() || out[3].defined() || (out[4].defined() && back)) {
+    bytes = feedforward_norm_grad_bytes(in.rows, (int)in.d, (int)in.rows_per_gate, norm_code(in.residual));
+    if (bytes > 0) partials = at::empty({bytes / 4}, options_as(in.residual).dtype(at::kFloat));
+  }
+  const Rows gdy(back ? dy : at::Tensor(), in.rows, in.d), gdr(dr, in.rows, in.d), r(in.residual, in.rows, in.d),
+      block(in.block, in.rows, in.d), gate = in.gate_rows();
+  const at::Tensor post = weight_of(in.post), pre = back ? weight_of(in.pre) : at::Tensor();
+  feedforward_check(feedforward_norm_grad(
+      gdy.at(), gdy.ld, gdr.at(), gdr.ld, r.at(), r.ld, block.at(), block.ld, at_of(post), gate.at(), gate.ld,
+      (int)in.rows_per_gate, at_of(pre), (float)scale, (const float*)lengths.data_ptr(), at_of(out[0]), at_of(out[1]),
+      at_of(out[2]), at_of(out[3]), back ? at_of(out[4]) : nullptr, at_of(partials), bytes, in.rows, (int)in.d,
+      norm_code(in.residual), dev, current_stream(dev)));
+  return out;
+}
+
+// outputs y and r, those of them that there are
+struct NormFunction : torch::autograd::Function<NormFunction> {
+  using Maybe = std::optional<at::Tensor>;
+  static Maybe maybe(const at::Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& residual, const Maybe& block, const Maybe& post,
+                               const Maybe& gate, const Maybe& pre, double scale, double eps) {
+    NormInputs in{residual, block.value_or(at::Tensor()), post.value_or(at::Tensor()), gate.value_or(at::Tensor()),
+                  pre.value_or(at::Tensor())};
+    const NormOutputs out = norm_forward(in, scale, eps, true);
+    ctx->save_for_backward({residual, out.r, in.block, in.post, in.gate, in.pre, out.lengths});
+    // (without a block the residual itself is what the norm took, and it is not multiplied)
+    ctx->saved_data["scale"] = in.block.defined() ? scale : 1.0;
+    ctx->set_materialize_grads(false);
+    variable_list outputs;
+    if (out.y.defined()) outputs.push_back(out.y);
+    if (out.r.defined()) outputs.push_back(out.r);
+    return outputs;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &residual = saved[0], &r = saved[1];
+    NormInputs in{r.defined() ? r : residual, saved[2], saved[3], saved[4], saved[5]};
+    const bool norm = in.pre.defined();
+    const at::Tensor dy = norm ? grads[0] : at::Tensor(), dr = r.defined() ? grads[norm ? 1 : 0] : at::Tensor();
+    std::array<bool, 5> want;
+    // (the context counts the inputs that are there)
+    const at::Tensor* const inputs[5] = {&residual, &in.block, &in.post, &in.gate, &in.pre};
+    for (int i = 0, at = 0; i < 5; i++) want[i] = inputs[i]->defined() && ctx->needs_input_grad(at++);
+    variable_list out(7);
+    {
+      c10::AutoGradMode off(false);
+      auto g = norm_backward(dy, dr, in, saved[6], ctx->saved_data["scale"].toDouble(), residual, want);
+      for (int i = 0; i < 5; i++) out[i] = g[i];
+    }
+    return once_differentiable(std::move(out), "residual_norm");
+  }
+};
+
 // an argument that may be None; false with an exception set
 bool optional(PyObject* o, const char* name, at::Tensor* out) {
   if (o == Py_None) return true;
@@ -623,203 +822,72 @@ bool optional(PyObject* o, const char* name, at::Tensor* out) {
   return true;
 }
 
-struct NormInputs {
-  at::Tensor residual, block, post, gate, pre;
-  int64_t rows = 0, d = 0, gates = 1, rows_per_gate = 1;
+bool norm_arguments(PyObject* const* args, NormInputs* in) {
+  const at::Tensor* const residual = tensor(args[0], "residual");
+  if (!residual || !optional(args[1], "block", &in->block) || !optional(args[2], "post_weight", &in->post) ||
+      !optional(args[3], "gate", &in->gate) || !optional(args[4], "pre_weight", &in->pre))
+    return false;
+  in->residual = *residual;
+  return true;
+}
 
-  // false with an exception set
-  bool check() {
-    const struct {
-      const char* name;
-      const at::Tensor* t;
-    } all[] = {{"residual", &residual}, {"block", &block}, {"post_weight", &post}, {"gate", &gate}, {"pre_weight", &pre}};
-    for (const auto& x : all) {
-      if (!x.t->defined()) continue;
-      const auto type = x.t->scalar_type();
-      if (!x.t->is_cuda() || (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat)) {
-        PyErr_Format(PyExc_ValueError, "%s must be a torch.half, torch.bfloat16 or torch.float tensor on the GPU", x.name);
-        return false;
-      }
-      if (x.t->layout() != at::kStrided || x.t->is_neg()) {
-        PyErr_Format(PyExc_ValueError, "%s must be a plain tensor", x.name);
-        return false;
-      }
-      if (type != residual.scalar_type() || x.t->device() != residual.device()) {
-        PyErr_Format(PyExc_ValueError, "%s must have the residual's type and device", x.name);
-        return false;
-      }
-    }
-    const int64_t dims = residual.dim();
-    if (dims < 1 || residual.size(-1) == 0) {
-      PyErr_SetString(PyExc_ValueError, "residual needs a last dimension, not 0");
-      return false;
-    }
-    d = residual.size(-1);
-    rows = residual.numel() / d;
-    if (rows > 0x7fffffff || d > 0x7fffffff) {
-      PyErr_SetString(PyExc_ValueError, "a size does not fit into a C int");
-      return false;
-    }
-    if (block.defined() && block.sizes() != residual.sizes()) {
-      PyErr_SetString(PyExc_ValueError, "block must have the residual's shape");
-      return false;
-    }
-    for (const at::Tensor* w : {&post, &pre})
-      if (w->defined() && (w->dim() != 1 || w->size(0) != d)) {
-        PyErr_Format(PyExc_ValueError, "%s must have one dimension, the residual's last", w == &post ? "post_weight" : "pre_weight");
-        return false;
-      }
-    if (!block.defined() && (post.defined() || gate.defined() || !pre.defined())) {
-      PyErr_SetString(PyExc_ValueError,
-                      block.defined() || pre.defined() ? "post_weight and gate belong to a block" : "there is neither a block nor a pre_weight");
-      return false;
-    }
-    rows_per_gate = rows > 0 ? rows : 1;
-    if (gate.defined()) {
-      // (d), or the residual's leading dimensions, ones for the others, and d
-      bool fits = gate.dim() >= 1 && gate.size(-1) == d && (gate.dim() == 1 || gate.dim() == dims);
-      if (fits && gate.dim() > 1) {
-        int64_t ones = dims - 1, shared = 1;
-        while (ones > 0 && gate.size(ones - 1) == 1) shared *= residual.size(--ones);
-        for (int64_t i = 0; i < ones; i++) fits = fits && gate.size(i) == residual.size(i);
-        rows_per_gate = shared > 0 ? shared : 1;
-      }
-      if (!fits) {
-        PyErr_SetString(PyExc_ValueError,
-                        "gate must have the shape (d,), or the residual's with ones for its last dimensions but d");
-        return false;
-      }
-    }
-    gates = rows > 0 ? rows / rows_per_gate : gate.defined() ? gate.numel() / d : 1;
-    return true;
-  }
-  int dev() const { return residual.get_device(); }
-  Rows gate_rows() const { return gate.defined() ? Rows(gate, gate.numel() / d, d) : Rows(); }
-};
-
-at::Tensor weight_of(const at::Tensor& w) { return w.defined() ? w.contiguous() : w; }
-void* at_of(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
-// residual_norm(residual, block, post, gate, pre, scale, eps, keep) -> (y, r, lengths); block, post,
-// gate and pre may be None, and so are then r (without a block) and y (without pre)
+// residual_norm(residual, block, post, gate, pre, scale, eps) -> (y, r); block, post, gate and pre may
+// be None, and so are then r (without a block) and y (without pre)
 PyObject* py_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 8) {
-    PyErr_SetString(PyExc_TypeError, "residual_norm takes 8 arguments");
-    return nullptr;
-  }
   NormInputs in;
-  const at::Tensor* const residual = tensor(args[0], "residual");
-  if (!residual || !optional(args[1], "block", &in.block) || !optional(args[2], "post_weight", &in.post) ||
-      !optional(args[3], "gate", &in.gate) || !optional(args[4], "pre_weight", &in.pre))
-    return nullptr;
-  in.residual = *residual;
+  if (!takes(nargs, 7, "residual_norm") || !norm_arguments(args, &in)) return nullptr;
   const double scale = PyFloat_AsDouble(args[5]), eps = PyFloat_AsDouble(args[6]);
   if (PyErr_Occurred()) return nullptr;
-  const int keep = PyObject_IsTrue(args[7]);
-  if (keep < 0 || !in.check()) return nullptr;
-  const int dev = in.dev();
-  void* const st = current_stream(dev);
-  at::Tensor y, r, stats;
-  Failed failed;
+  NormOutputs out;
   {
     pybind11::gil_scoped_release unlocked;
-    if (in.pre.defined()) y = empty_as(in.residual, in.residual.sizes());
-    if (in.block.defined()) r = empty_as(in.residual, in.residual.sizes());
-    if (keep) stats = at::empty({in.rows, 2}, in.residual.options().requires_grad(false).dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
-    const Rows res(in.residual, in.rows, in.d), gate = in.gate_rows();
-    const Rows block = in.block.defined() ? Rows(in.block, in.rows, in.d) : Rows();
-    const at::Tensor post = weight_of(in.post), pre = weight_of(in.pre);
-    failed(feedforward_norm(res.at(), res.ld, block.at(), block.ld, at_of(post), gate.at(), gate.ld,
-                            (int)in.rows_per_gate, at_of(pre), (float)scale, (float)eps, at_of(r), at_of(y),
-                            (float*)at_of(stats), in.rows, (int)in.d, norm_code(in.residual), dev, st));
+    if (differentiated({&in.residual, &in.block, &in.post, &in.gate, &in.pre})) {
+      const variable_list v = NormFunction::apply(in.residual, NormFunction::maybe(in.block), NormFunction::maybe(in.post),
+                                                  NormFunction::maybe(in.gate), NormFunction::maybe(in.pre), scale, eps);
+      if (in.pre.defined()) out.y = v[0];
+      if (in.block.defined()) out.r = v.back();
+    } else {
+      out = norm_forward(in, scale, eps, false);
+    }
   }
-  if (failed.raise()) return nullptr;
-  PyObject* const tuple = PyTuple_New(3);
-  if (!tuple) return nullptr;
-  PyTuple_SET_ITEM(tuple, 0, THPVariable_Wrap(std::move(y)));
-  PyTuple_SET_ITEM(tuple, 1, THPVariable_Wrap(std::move(r)));
-  PyTuple_SET_ITEM(tuple, 2, THPVariable_Wrap(std::move(stats)));
-  return tuple;
+  return tuple_of({out.y, out.r});
   END_HANDLE_TH_ERRORS
 }
 
-// norm_grads(dy, dr, r, block, post, gate, pre, lengths, scale, residual or None, wanted: five truth
-// values) -> the gradients of residual, block, post, gate and pre, None where not wanted; dy or dr
-// may be None
-PyObject* py_norm_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+// norm_lengths(... as residual_norm) -> (y, r, lengths) and norm_grads(dy, dr, r, block, post, gate, pre,
+// lengths, scale) -> five gradients, None for what is: the passes by themselves, for compilers
+PyObject* py_norm_lengths(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 15) {
-    PyErr_SetString(PyExc_TypeError, "norm_grads takes 15 arguments");
-    return nullptr;
-  }
   NormInputs in;
-  at::Tensor dy, dr, stats, leaf;
-  const at::Tensor* const r = tensor(args[2], "r");
-  if (!r || !optional(args[0], "dy", &dy) || !optional(args[1], "dr", &dr) ||
-      !optional(args[3], "block", &in.block) || !optional(args[4], "post_weight", &in.post) ||
-      !optional(args[5], "gate", &in.gate) || !optional(args[6], "pre_weight", &in.pre) ||
-      !optional(args[7], "lengths", &stats) || !optional(args[9], "residual", &leaf))
-    return nullptr;
-  in.residual = *r;
-  const double scale = PyFloat_AsDouble(args[8]);
+  if (!takes(nargs, 7, "norm_lengths") || !norm_arguments(args, &in)) return nullptr;
+  const double scale = PyFloat_AsDouble(args[5]), eps = PyFloat_AsDouble(args[6]);
   if (PyErr_Occurred()) return nullptr;
-  bool want[5];
-  for (int i = 0; i < 5; i++) {
-    const int w = PyObject_IsTrue(args[10 + i]);
-    if (w < 0) return nullptr;
-    want[i] = w;
-  }
-  if (!in.check()) return nullptr;
-  for (const at::Tensor* g : {&dy, &dr})
-    if (g->defined() && (g->sizes() != in.residual.sizes() || g->scalar_type() != in.residual.scalar_type() ||
-                         g->device() != in.residual.device())) {
-      PyErr_SetString(PyExc_ValueError, "dy and dr must be gradients of the outputs");
-      return nullptr;
-    }
-  if (!stats.defined() || stats.scalar_type() != at::kFloat || !stats.is_contiguous() || stats.numel() != 2 * in.rows ||
-      stats.device() != in.residual.device()) {
-    PyErr_SetString(PyExc_ValueError, "lengths must be those of the forward pass");
-    return nullptr;
-  }
-  const int dev = in.dev();
-  if (!check_capture({&leaf, &in.block, &in.post, &in.gate, &in.pre}, dev)) return nullptr;
-  void* const st = current_stream(dev);
-  at::Tensor out[5];
-  const at::Tensor* const like[5] = {&in.residual, &in.block, &in.post, &in.gate, &in.pre};
-  Failed failed;
+  NormOutputs out;
   {
     pybind11::gil_scoped_release unlocked;
-    for (int i = 0; i < 5; i++)
-      if (want[i] && like[i]->defined()) out[i] = empty_as(*like[i], like[i]->sizes());
-    // without dy nothing comes back through the last norm
-    const bool back = in.pre.defined() && dy.defined(), any = back || dr.defined();
-    if (out[4].defined() && !back) out[4].zero_();
-    if (in.rows == 0 || !any) {
-      for (at::Tensor& g : out)
-        if (g.defined()) g.zero_();
-    } else {
-      const bool sums = out[2].defined() || out[3].defined() || (out[4].defined() && back);
-      const long long bytes = sums ? feedforward_norm_grad_bytes(in.rows, (int)in.d, (int)in.rows_per_gate, norm_code(in.residual)) : 0;
-      at::Tensor partials;
-      if (bytes > 0)
-        partials = at::empty({bytes / 4}, in.residual.options().requires_grad(false).dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
-      const auto rows_of = [&](const at::Tensor& t) { return t.defined() ? Rows(t, in.rows, in.d) : Rows(); };
-      const Rows gdy = back ? rows_of(dy) : Rows(), gdr = rows_of(dr), rr = rows_of(in.residual), block = rows_of(in.block),
-                 gate = in.gate_rows();
-      const at::Tensor post = weight_of(in.post), pre = back ? weight_of(in.pre) : at::Tensor();
-      failed(feedforward_norm_grad(gdy.at(), gdy.ld, gdr.at(), gdr.ld, rr.at(), rr.ld, block.at(), block.ld, at_of(post),
-                                   gate.at(), gate.ld, (int)in.rows_per_gate, at_of(pre), (float)scale,
-                                   (const float*)stats.data_ptr(), at_of(out[0]), at_of(out[1]), at_of(out[2]),
-                                   at_of(out[3]), back ? at_of(out[4]) : nullptr, at_of(partials), bytes, in.rows,
-                                   (int)in.d, norm_code(in.residual), dev, st));
-    }
+    out = norm_forward(in, scale, eps, true);
   }
-  if (failed.raise()) return nullptr;
-  PyObject* const tuple = PyTuple_New(5);
-  if (!tuple) return nullptr;
-  for (int i = 0; i < 5; i++) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(std::move(out[i])));
-  return tuple;
+  return tuple_of({out.y, out.r, out.lengths});
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_norm_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NormInputs in;
+  at::Tensor dy, dr;
+  if (!takes(nargs, 9, "norm_grads") || !optional(args[0], "dy", &dy) || !optional(args[1], "dr", &dr) ||
+      !norm_arguments(args + 2, &in))
+    return nullptr;
+  const at::Tensor* const lengths = tensor(args[7], "lengths");
+  const double scale = PyFloat_AsDouble(args[8]);
+  if (!lengths || PyErr_Occurred()) return nullptr;
+  std::array<at::Tensor, 5> g;
+  {
+    pybind11::gil_scoped_release unlocked;
+    g = norm_backward(dy, dr, in, *lengths, scale, at::Tensor(), {true, true, true, true, true});
+  }
+  return tuple_of({g[0], g[1], g[2], g[3], g[4]});
   END_HANDLE_TH_ERRORS
 }
 
@@ -958,6 +1026,8 @@ PyMethodDef methods[] = {
     {"gated_dense", (PyCFunction)(void (*)(void))py_gated_dense, METH_FASTCALL, nullptr},
     {"gated_grads", (PyCFunction)(void (*)(void))py_gated_grads, METH_FASTCALL, nullptr},
     {"linear_dense", (PyCFunction)(void (*)(void))py_linear_dense, METH_FASTCALL, nullptr},
+    {"gated_sums", (PyCFunction)(void (*)(void))py_gated_sums, METH_FASTCALL, nullptr},
+    {"norm_lengths", (PyCFunction)(void (*)(void))py_norm_lengths, METH_FASTCALL, nullptr},
     {"linear_grads", (PyCFunction)(void (*)(void))py_linear_grads, METH_FASTCALL, nullptr},
     {"gated_mul", (PyCFunction)(void (*)(void))py_gated_mul, METH_FASTCALL, nullptr},
     {"gated_linear", (PyCFunction)(void (*)(void))py_gated_linear, METH_FASTCALL, nullptr},

@@ -10,27 +10,6 @@ import streamk
 from native import torch_binding as _torch_binding
 
 
-class _ResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, residual, block, post, gate, pre, scale, eps):
-        y, r, lengths = _torch_binding.residual_norm(residual, block, post, gate, pre, scale, eps, True)
-        ctx.save_for_backward(residual, r, block, post, gate, pre, lengths)
-        ctx.scale = scale
-        ctx.set_materialize_grads(False)
-        return (y, r) if block is not None and pre is not None else y if block is None else r
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, *grads):
-        residual, r, block, post, gate, pre, lengths = ctx.saved_tensors
-        dy, dr = grads if len(grads) == 2 else (grads[0], None) if block is None else (None, grads[0])
-        # (without a block the residual is the saved one and not multiplied)
-        out = _torch_binding.norm_grads(dy, dr, residual if block is None else r, block, post, gate, pre, lengths,
-                                        ctx.scale if block is not None else 1.0, residual,
-                                        *ctx.needs_input_grad[:5])
-        return (*out, None, None)
-
-
 def residual_norm(residual, block=None, *, post_weight=None, gate=None, scale=1.0, pre_weight=None, eps=1e-6):
     """The norm after a block, its gate, the residual's scale and the norm before the next block in
     one launch: with rms(v) = v / sqrt(mean(v^2) + eps) over the last dimension,
@@ -50,11 +29,7 @@ def residual_norm(residual, block=None, *, post_weight=None, gate=None, scale=1.
     if torch.compiler.is_compiling():
         y, r, _ = torch.ops.marlin_amd.residual_norm(residual, block, post_weight, gate, pre_weight, scale, eps)
         return (None if pre_weight is None else y), (residual if block is None else r)
-    inputs = (residual, block, post_weight, gate, pre_weight)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
-        out = _ResidualNorm.apply(*inputs, scale, eps)
-        return (out, residual) if block is None else (None, out) if pre_weight is None else out
-    y, r, _ = _torch_binding.residual_norm(*inputs, scale, eps, False)
+    y, r = _torch_binding.residual_norm(residual, block, post_weight, gate, pre_weight, scale, eps)
     return y, residual if block is None else r
 
 
@@ -64,7 +39,7 @@ _Maybe = torch.Tensor | None
 @torch.library.custom_op("marlin_amd::residual_norm", mutates_args=())
 def _norm_op(residual: torch.Tensor, block: _Maybe, post: _Maybe, gate: _Maybe, pre: _Maybe, scale: float,
              eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    y, r, lengths = _torch_binding.residual_norm(residual, block, post, gate, pre, scale, eps, True)
+    y, r, lengths = _torch_binding.norm_lengths(residual, block, post, gate, pre, scale, eps)
     return tuple(residual.new_empty(0) if t is None else t for t in (y, r, lengths))
 
 
@@ -79,8 +54,7 @@ def _norm_fake(residual, block, post, gate, pre, scale, eps):
 @torch.library.custom_op("marlin_amd::norm_grads", mutates_args=())
 def _norm_grads_op(dy: _Maybe, dr: _Maybe, r: torch.Tensor, block: _Maybe, post: _Maybe, gate: _Maybe, pre: _Maybe,
                    lengths: torch.Tensor, scale: float) -> list[torch.Tensor]:
-    wanted = [True] + [t is not None for t in (block, post, gate, pre)]
-    out = _torch_binding.norm_grads(dy, dr, r, block, post, gate, pre, lengths, scale, None, *wanted)
+    out = _torch_binding.norm_grads(dy, dr, r, block, post, gate, pre, lengths, scale)
     return [r.new_empty(0) if g is None else g for g in out]
 
 

@@ -95,8 +95,8 @@ def gemm(A, B, C=None):
 
 # ---------------------------------------------------------------------------
 # Products with gradients.  Under a compiler each is one operator of torch's dispatcher, which
-# costs more host time than a product of a few rows takes; else an autograd function, or the call
-# itself where nothing is to be differentiated.
+# costs more host time than a product of a few rows takes; else the binding's, which is an autograd
+# function where gradients are wanted.
 
 ACTIVATIONS = {"silu": 1, "gelu": 2}  # (gelu in its tanh form)
 _lib.feedforward_tile.restype = _I
@@ -113,54 +113,19 @@ def _activation(name):
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}") from None
 
 
-class _Gated(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, act):
-        h, sums = _torch_binding.gated_dense(x, weight, act, True)
-        ctx.save_for_backward(x, weight, sums)
-        ctx.act = act
-        return h
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dh):
-        x, weight, sums = ctx.saved_tensors
-        dx, dw = _torch_binding.gated_grads(dh, sums, x, weight, ctx.act, *ctx.needs_input_grad[:2])
-        return dx, dw, None
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight):
-        ctx.save_for_backward(x, weight)
-        return _torch_binding.linear_dense(x, weight)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight = ctx.saved_tensors
-        return _torch_binding.linear_grads(dy, x, weight, *ctx.needs_input_grad)
-
-
-def _differentiated(*tensors):
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
-
-
 def gated(x, weight, activation="silu"):
     """Both projections of a gated feed-forward block, the activation and the product of the two in
     one launch: act(x @ G.T) * (x @ U.T), rounded once, for x (..., k) and weight (2n, k), the rows
     of G and behind them those of U; returns (..., n).
 
     torch.half or torch.bfloat16, n and k multiples of 8, weight at most 2 GiB; activation "silu"
-    or "gelu" (its tanh form).  Where gradients are wanted the two sums are kept in that type as
-    well, 4n bytes a row.  Rows that do not start on 16 bytes are copied.  Differentiable once, on
+    or "gelu" (its tanh form).  Where gradients are wanted the two sums are kept in fp32, 8n bytes a
+    row.  Rows that do not start on 16 bytes are copied.  Differentiable once, on
     the current stream of x's device."""
     act = _activation(activation)
     if torch.compiler.is_compiling():
         return torch.ops.marlin_amd.gated_dense(x, weight, act)[0]
-    if _differentiated(x, weight):
-        return _Gated.apply(x, weight, act)
-    return _torch_binding.gated_dense(x, weight, act, False)[0]
+    return _torch_binding.gated_dense(x, weight, act)
 
 
 def linear(x, weight):
@@ -168,26 +133,25 @@ def linear(x, weight):
     of 8; returns (..., n).  Differentiable once; streams and alignment as `gated`."""
     if torch.compiler.is_compiling():
         return torch.ops.marlin_amd.linear_dense(x, weight)
-    if _differentiated(x, weight):
-        return _Linear.apply(x, weight)
     return _torch_binding.linear_dense(x, weight)
 
 
 @torch.library.custom_op("marlin_amd::gated_dense", mutates_args=())
 def _gated_op(x: torch.Tensor, weight: torch.Tensor, act: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return _torch_binding.gated_dense(x, weight, act, True)
+    return _torch_binding.gated_sums(x, weight, act)
 
 
 @_gated_op.register_fake
 def _gated_fake(x, weight, act):
     n = weight.shape[0] // 2
-    return x.new_empty(x.shape[:-1] + (n,)), x.new_empty((x.numel() // x.shape[-1], 2 * n))
+    return (x.new_empty(x.shape[:-1] + (n,)),
+            x.new_empty((x.numel() // x.shape[-1], -(-n // 16) * 32), dtype=torch.float32))
 
 
 @torch.library.custom_op("marlin_amd::gated_grads", mutates_args=())
 def _gated_grads_op(dh: torch.Tensor, sums: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
                     act: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return _torch_binding.gated_grads(dh, sums, x, weight, act, True, True)
+    return _torch_binding.gated_grads(dh, sums, x, weight, act)
 
 
 @_gated_grads_op.register_fake
@@ -208,7 +172,7 @@ def _linear_fake(x, weight):
 @torch.library.custom_op("marlin_amd::linear_grads", mutates_args=())
 def _linear_grads_op(dy: torch.Tensor, x: torch.Tensor,
                      weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    return _torch_binding.linear_grads(dy, x, weight, True, True)
+    return _torch_binding.linear_grads(dy, x, weight)
 
 
 @_linear_grads_op.register_fake

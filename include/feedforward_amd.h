@@ -60,16 +60,17 @@ int feedforward_product(const void *A, const void *B, void *C, int m, int n, int
                         long long ldb, long long ldc, int type, int dev, void *stream);
 
 /* h (m x n) = act(x G^T) * (x U^T), element by element, x (m x k), w the n rows of G and behind
- * them the n rows of U; pre, if not null, (m x 2n): both sums in 16 bits, x G^T and beside it
- * x U^T.  w holds at most 2 GiB; k > 0. */
-int feedforward_gated(const void *x, const void *w, void *h, void *pre, int m, int n, int k,
+ * them the n rows of U.  w holds at most 2 GiB; k > 0.  pre, if not null, keeps both sums for
+ * the backward pass: m rows of floats, ldpre >= 32 ceil(n / 16) from one to the next, in which
+ * the sums of columns 16 i + c of x G^T are at 32 i + c and those of x U^T 16 further on. */
+int feedforward_gated(const void *x, const void *w, void *h, float *pre, int m, int n, int k,
                       long long ldx, long long ldw, long long ldh, long long ldpre, int type,
                       int activation, int dev, void *stream);
 
 /* The gradients of both sums from that of h: [dg | du] as rows (dgu, m x 2n) and turned over
  * (dgu_t, 2n x m), either of which may be null.  Behind a row of 2n or m columns there are
  * zeros up to the next multiple of 64, which ld has room for. */
-int feedforward_gated_grad(const void *dh, const void *pre, void *dgu, void *dgu_t, int m, int n,
+int feedforward_gated_grad(const void *dh, const float *pre, void *dgu, void *dgu_t, int m, int n,
                            long long lddh, long long ldpre, long long lddgu, long long lddgu_t,
                            int type, int activation, int dev, void *stream);
 
