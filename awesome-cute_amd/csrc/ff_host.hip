@@ -139,8 +139,9 @@ NormType norm_type(int type) {
 }
 
 int check_norm(long long rows, int d, int rows_per_gate, int type) {
-  if (rows < 0 || d < 1 || d > kNormMax)
-    return fail(FEEDFORWARD_ERR_SHAPE, "%lld rows of %d: rows must hold 1 to %d elements", rows, d, kNormMax);
+  if (rows < 0 || rows > 0x7fffffff || d < 1 || d > kNormMax)
+    return fail(FEEDFORWARD_ERR_SHAPE, "%lld rows of %d: rows must hold 1 to %d elements and fit into a C int", rows, d,
+                kNormMax);
   if (rows_per_gate < 1 || rows % rows_per_gate != 0)
     return fail(FEEDFORWARD_ERR_SHAPE, "%lld rows are no multiple of the %d of a gate", rows, rows_per_gate);
   if (type != FEEDFORWARD_FP16 && type != FEEDFORWARD_BF16 && type != FEEDFORWARD_FP32)
@@ -241,10 +242,7 @@ int feedforward_norm(const void* residual, long long ld_residual, const void* bl
 
 long long feedforward_norm_grad_bytes(long long rows, int d, int rows_per_gate, int type) {
   if (check_norm(rows, d, rows_per_gate, type) != FEEDFORWARD_OK) return -1;
-  // (whichever loads the addresses allow)
-  const size_t a = norm_parts(rows, rows_per_gate, d, type_bytes(type), true).bytes;
-  const size_t b = norm_parts(rows, rows_per_gate, d, type_bytes(type), false).bytes;
-  return (long long)(a > b ? a : b);
+  return (long long)norm_parts(rows, rows_per_gate, d, type_bytes(type)).bytes;
 }
 
 int feedforward_norm_grad(const void* dy, long long ld_dy, const void* dr, long long ld_dr, const void* r,

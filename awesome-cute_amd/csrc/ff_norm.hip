@@ -34,31 +34,65 @@ namespace w4a16 {
 namespace {
 
 typedef __bf16 bf;
+typedef int i4_anywhere __attribute__((ext_vector_type(4), aligned(2)));
 
-// VEC elements of type T as they come from memory, and as floats
-template <class T, int VEC>
+// 16 bytes of a row as they come from memory, and as floats
+template <class T>
 struct Piece {
-  T v[VEC];
+  static constexpr int kN = 16 / sizeof(T);
+  T v[kN];
   __device__ __forceinline__ float at(int i) const { return (float)v[i]; }
 };
-template <class T, int VEC>
-__device__ __forceinline__ Piece<T, VEC> load_piece(const void* p, size_t at) {
-  Piece<T, VEC> r;
-  if constexpr (VEC * sizeof(T) == 16)
-    *(i4*)&r = *(const i4*)((const T*)p + at);
-  else
-    r.v[0] = ((const T*)p)[at];
+template <class T>
+__device__ __forceinline__ Piece<T> piece_of(float x) {
+  Piece<T> r;
+#pragma unroll
+  for (int i = 0; i < Piece<T>::kN; i++) r.v[i] = (T)x;
   return r;
 }
-template <class T, int VEC>
-__device__ __forceinline__ void store_piece(void* p, size_t at, const float* f) {
-  Piece<T, VEC> r;
+// WHOLE: rows are whole pieces that start on 16 bytes.  Otherwise a piece may lie anywhere (the
+// hardware's 16-byte loads to registers take any address), and the last of a row holds `left`
+// elements, fetched one by one, zeros behind them.
+template <bool WHOLE, class T>
+__device__ __forceinline__ Piece<T> load_piece(const T* p, int left) {
+  Piece<T> r;
+  if constexpr (WHOLE) {
+    *(i4*)&r = *(const i4*)p;
+  } else if (left >= Piece<T>::kN) {
+    *(i4*)&r = *(const i4_anywhere*)p;
+  } else {
+    r = piece_of<T>(0.f);
 #pragma unroll
-  for (int i = 0; i < VEC; i++) r.v[i] = (T)f[i];
-  if constexpr (VEC * sizeof(T) == 16)
-    *(i4*)((T*)p + at) = *(const i4*)&r;
-  else
-    ((T*)p)[at] = r.v[0];
+    for (int i = 0; i < Piece<T>::kN - 1; i++)
+      if (i < left) r.v[i] = p[i];
+  }
+  return r;
+}
+template <bool WHOLE, class T>
+__device__ __forceinline__ void store_piece(T* p, int left, const float* f) {
+  Piece<T> r;
+#pragma unroll
+  for (int i = 0; i < Piece<T>::kN; i++) r.v[i] = (T)f[i];
+  if constexpr (WHOLE) {
+    *(i4*)p = *(const i4*)&r;
+  } else if (left >= Piece<T>::kN) {
+    *(i4_anywhere*)p = *(const i4*)&r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < Piece<T>::kN - 1; i++)
+      if (i < left) p[i] = r.v[i];
+  }
+}
+
+// What a lane holds over all its rows stays as it came from memory: without this the compiler
+// keeps every weight as a float from before the loop, twice the registers.
+template <class T>
+__device__ __forceinline__ void as_stored(Piece<T>& v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  i4 x = *(i4*)&v;
+  asm volatile("" : "+v"(x));
+  *(i4*)&v = x;
+#endif
 }
 
 // The sums of N values over the W waves of a row, the same in every lane.  `room` is N x waves
@@ -73,14 +107,17 @@ __device__ __forceinline__ void add_up(float (&v)[N], float* room, int wave_in_w
     float* const set = room + (turn & 1) * (N * 16);
     turn++;
     const int first = wave_in_wg / W * W;
-    if ((threadIdx.x & 63) == 0) {
+    const int l = threadIdx.x & 63;
+    if (l == 0) {
 #pragma unroll
       for (int n = 0; n < N; n++) set[n * 16 + wave_in_wg] = v[n];
     }
-    __syncthreads();
-    // (a lane a value and wave: all N sums by log W exchanges)
+#if defined(__HIP_DEVICE_COMPILE__)
+    // (only LDS is exchanged: the next row stays on its way)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#endif
+    // a lane a value and wave: all N sums by log W exchanges
     static_assert(N * W <= 64, "");
-    const int l = threadIdx.x & 63;
     float s = l < N * W ? set[l / W * 16 + first + l % W] : 0.f;
 #pragma unroll
     for (int d = W / 2; d >= 1; d >>= 1) s += __shfl_xor(s, d);
@@ -89,114 +126,138 @@ __device__ __forceinline__ void add_up(float (&v)[N], float* room, int wave_in_w
   }
 }
 
+__device__ __forceinline__ float rstd_of(float sum, float mean, float eps) {
+  return 1.f / __builtin_sqrtf(__builtin_fmaf(sum, mean, eps));
+}
+
 constexpr int wg_waves(int w) { return w < 4 ? 4 : w; }
+
+// Where a lane's pieces lie in a row
+template <class T, int NV, int W>
+struct Lane {
+  int d, lane;
+  __device__ __forceinline__ Lane(int d_) : d(d_), lane((int)threadIdx.x & (64 * W - 1)) {}
+  __device__ __forceinline__ int column(int i) const { return Piece<T>::kN * (64 * W * i + lane); }
+  __device__ __forceinline__ int left(int i) const { return d - column(i); }
+  __device__ __forceinline__ bool in(int i) const { return column(i) < d; }
+};
 
 }  // namespace
 
-// W waves a row, NV pieces a lane; a workgroup of four waves or more takes 4 / W rows at once
-template <class T, int VEC, int NV, int W>
-__global__ __launch_bounds__(64 * wg_waves(W)) void norm_kernel(NormArgs p) {
-  constexpr int kRows = wg_waves(W) / W;  // rows of a workgroup
+// W waves a row, NV pieces a lane; a workgroup of four waves or more takes 4 / W rows at once.
+// A set of W waves takes a run of rows; the next row is requested before this one's lengths are
+// known, and the weights stay in registers where a lane holds few of them.
+template <class T, bool WHOLE, int NV, int W>
+__global__ __launch_bounds__(64 * wg_waves(W)) void norm_kernel(NormArgs p, int sets) {
+  constexpr int kSets = wg_waves(W) / W, kN = Piece<T>::kN;
+  constexpr bool kKeep = NV * kN <= 8;
   __shared__ float room[2 * 16];
-  const int wave = threadIdx.x >> 6;
-  const int lane = threadIdx.x & (64 * W - 1);  // in the row
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const Lane<T, NV, W> me(p.d);
   const float mean = 1.f / (float)p.d;
-  int turn = 0;
-  // (all sets of waves of a workgroup go round equally often: they meet at barriers)
-  for (long long r0 = (long long)blockIdx.x * kRows; r0 < p.rows; r0 += (long long)gridDim.x * kRows) {
-    const long long row = r0 + wave / W;
-    const bool live = row < p.rows;
-    float r[NV][VEC];
+  const int set = (int)blockIdx.x * kSets + wave / W, rows = (int)p.rows;
+  const int longest = (rows + sets - 1) / sets;
+  const int first = (int)((long long)rows * set / sets);
+  const int last = set < sets ? (int)((long long)rows * (set + 1) / sets) : first;
+  auto load = [&](const void* base, long long at, int i) {
+    return load_piece<WHOLE>((const T*)base + at + me.column(i), me.left(i));
+  };
+  Piece<T> post[kKeep ? NV : 1], gate[kKeep ? NV : 1], pre[kKeep ? NV : 1];
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      post[i] = gate[i] = pre[i] = piece_of<T>(1.f);
+      if (p.post && me.in(i)) post[i] = load(p.post, 0, i);
+      if (p.pre && me.in(i)) pre[i] = load(p.pre, 0, i);
+    }
+  }
+  Piece<T> b[NV], x[NV];
+  auto fetch = [&](int row) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      b[i] = x[i] = piece_of<T>(0.f);
+      if (row >= last || !me.in(i)) continue;
+      if (p.block) b[i] = load(p.block, row * p.ld_block, i);
+      x[i] = load(p.residual, row * p.ld_residual, i);
+    }
+  };
+  int turn = 0, held = -1;
+  fetch(first);
+  // (all sets of a workgroup go round equally often: they meet at barriers)
+  for (int at = 0; at < longest; at++) {
+    const int row = first + at;
+    const bool live = row < last;
+    float r[NV][kN];
     if (p.block) {
-      Piece<T, VEC> b[NV], r_in[NV];
-      float sum[1] = {0.f};
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const int c = VEC * (64 * W * i + lane);
-        if (live && c < p.d) {
-          b[i] = load_piece<T, VEC>(p.block, (size_t)row * p.ld_block + c);
-          r_in[i] = load_piece<T, VEC>(p.residual, (size_t)row * p.ld_residual + c);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; e++) b[i].v[e] = r_in[i].v[e] = (T)0.f;
-        }
-      }
-      float rstd = 1.f;
+      float sum[1] = {0.f}, rstd = 1.f;
       if (p.post) {
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
-          for (int e = 0; e < VEC; e++) sum[0] = __builtin_fmaf(b[i].at(e), b[i].at(e), sum[0]);
-        add_up<W, 1>(sum, room, wave, turn);
-        rstd = 1.f / __builtin_sqrtf(__builtin_fmaf(sum[0], mean, p.eps));
-        if (p.stats && live && lane == 0) p.stats[2 * row] = rstd;
+          for (int e = 0; e < kN; e++) sum[0] = __builtin_fmaf(b[i].at(e), b[i].at(e), sum[0]);
       }
-      const size_t gate_row = p.gate && live ? (size_t)(row / p.rows_per_gate) * p.ld_gate : 0;
+      const int g = p.gate && live ? (int)((unsigned)row / (unsigned)p.rows_per_gate) : held;
+      if (kKeep && g != held) {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+          if (me.in(i)) gate[kKeep ? i : 0] = load(p.gate, g * p.ld_gate, i);
+      }
+      held = g;
+      if (p.post) {
+        add_up<W, 1>(sum, room, wave, turn);
+        rstd = rstd_of(sum[0], mean, p.eps);
+        if (p.stats && live && me.lane == 0) p.stats[2 * (size_t)row] = rstd;
+      }
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        const int c = VEC * (64 * W * i + lane);
-        if (!live || c >= p.d) {
-#pragma unroll
-          for (int e = 0; e < VEC; e++) r[i][e] = 0.f;
-          continue;
+        Piece<T> w = piece_of<T>(1.f), gt = w;
+        if constexpr (kKeep) {
+          as_stored(post[i]);
+          as_stored(gate[i]);
+          w = post[i];
+          gt = gate[i];
+        } else if (me.in(i)) {
+          if (p.post) w = load(p.post, 0, i);
+          if (p.gate && held >= 0) gt = load(p.gate, held * p.ld_gate, i);
         }
-        Piece<T, VEC> post, gate;
-        if (p.post) post = load_piece<T, VEC>(p.post, c);
-        if (p.gate) gate = load_piece<T, VEC>(p.gate, gate_row + c);
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-          float x = b[i].at(e);
-          if (p.post) x *= rstd * post.at(e);
-          if (p.gate) x *= gate.at(e);
-          r[i][e] = __builtin_fmaf(p.scale, r_in[i].at(e), x);
-        }
-        store_piece<T, VEC>(p.r, (size_t)row * p.d + c, r[i]);
+        for (int e = 0; e < kN; e++)
+          r[i][e] = __builtin_fmaf(p.scale, x[i].at(e), b[i].at(e) * (rstd * w.at(e)) * gt.at(e));
+        if (live && me.in(i))
+          store_piece<WHOLE>((T*)p.r + (long long)row * p.d + me.column(i), me.left(i), r[i]);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const int c = VEC * (64 * W * i + lane);
-        const bool in = live && c < p.d;
-        Piece<T, VEC> x;
-        if (in) x = load_piece<T, VEC>(p.residual, (size_t)row * p.ld_residual + c);
+      for (int i = 0; i < NV; i++)
 #pragma unroll
-        for (int e = 0; e < VEC; e++) r[i][e] = in ? x.at(e) : 0.f;
-      }
+        for (int e = 0; e < kN; e++) r[i][e] = x[i].at(e);
     }
+    fetch(row + 1);
     if (!p.pre) continue;
     float sum[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
-      for (int e = 0; e < VEC; e++) sum[0] = __builtin_fmaf(r[i][e], r[i][e], sum[0]);
+      for (int e = 0; e < kN; e++) sum[0] = __builtin_fmaf(r[i][e], r[i][e], sum[0]);
     add_up<W, 1>(sum, room, wave, turn);
-    const float rstd = 1.f / __builtin_sqrtf(__builtin_fmaf(sum[0], mean, p.eps));
-    if (p.stats && live && lane == 0) p.stats[2 * row + 1] = rstd;
+    const float rstd = rstd_of(sum[0], mean, p.eps);
+    if (p.stats && live && me.lane == 0) p.stats[2 * (size_t)row + 1] = rstd;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      const int c = VEC * (64 * W * i + lane);
-      if (!live || c >= p.d) continue;
-      const Piece<T, VEC> pre = load_piece<T, VEC>(p.pre, c);
-      float y[VEC];
+      if (!live || !me.in(i)) continue;
+      Piece<T> w;
+      if constexpr (kKeep) {
+        as_stored(pre[i]);
+        w = pre[i];
+      } else {
+        w = load(p.pre, 0, i);
+      }
+      float y[kN];
 #pragma unroll
-      for (int e = 0; e < VEC; e++) y[e] = r[i][e] * rstd * pre.at(e);
-      store_piece<T, VEC>(p.y, (size_t)row * p.d + c, y);
+      for (int e = 0; e < kN; e++) y[e] = r[i][e] * rstd * w.at(e);
+      store_piece<WHOLE>((T*)p.y + (long long)row * p.d + me.column(i), me.left(i), y);
     }
   }
-}
-
-// What a lane holds over all its rows stays as it came from memory: without this the compiler
-// keeps every weight as a float from before the loop, twice the registers, and with sixteen
-// waves a row the sums are then spilled.
-template <class T, int VEC>
-__device__ __forceinline__ void as_stored(Piece<T, VEC>& v) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  if constexpr (VEC * sizeof(T) == 16) {
-    i4 x = *(i4*)&v;
-    asm volatile("" : "+v"(x));
-    *(i4*)&v = x;
-  }
-#endif
 }
 
 // Sums over rows that a backward pass keeps: none; of dy rh and dt bh over a part of a gate's
@@ -204,14 +265,15 @@ __device__ __forceinline__ void as_stored(Piece<T, VEC>& v) {
 enum Sums { kNoSums, kPartSums, kGateSums };
 
 // A set of W waves takes one part.
-template <class T, int VEC, int NV, int W, Sums SUMS>
+template <class T, bool WHOLE, int NV, int W, Sums SUMS>
 __global__ __launch_bounds__(64 * wg_waves(W)) void norm_grad_kernel(NormGradArgs p, NormParts parts) {
-  constexpr int kSets = wg_waves(W) / W;
-  // (weights of more than eight elements a lane are read again for every row)
-  constexpr bool kKeep = NV * VEC <= 8;
+  constexpr int kSets = wg_waves(W) / W, kN = Piece<T>::kN;
+  // (of more than eight elements a lane the weights are read again for every row, and no row is
+  // requested ahead: sixteen waves have 128 registers each, and the sums take most of them)
+  constexpr bool kKeep = NV * kN <= 8;
   __shared__ float room[2 * 4 * 16];
-  const int wave = threadIdx.x >> 6;
-  const int lane = threadIdx.x & (64 * W - 1);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const Lane<T, NV, W> me(p.d);
   const float mean = 1.f / (float)p.d;
   const long long part = (long long)blockIdx.x * kSets + wave / W;
   // my rows
@@ -232,89 +294,90 @@ __global__ __launch_bounds__(64 * wg_waves(W)) void norm_grad_kernel(NormGradArg
       last += gate * of_gate;
     }
   }
-  auto in = [&](int i) { return VEC * (64 * W * i + lane) < p.d; };
-  auto column = [&](int i) { return VEC * (64 * W * i + lane); };
-  auto weight = [&](const void* from, int i, size_t row_at) {
-    Piece<T, VEC> v;
-#pragma unroll
-    for (int e = 0; e < VEC; e++) v.v[e] = (T)1.f;
-    if (from && in(i)) v = load_piece<T, VEC>(from, row_at + column(i));
-    return v;
+  auto load = [&](const void* base, long long at, int i) {
+    return load_piece<WHOLE>((const T*)base + at + me.column(i), me.left(i));
   };
-  Piece<T, VEC> post[kKeep ? NV : 1], pre[kKeep ? NV : 1], gate[kKeep ? NV : 1];
+  auto weight = [&](const void* from, int i, long long row_at) {
+    return from && me.in(i) ? load(from, row_at, i) : piece_of<T>(1.f);
+  };
+  Piece<T> post[kKeep ? NV : 1], pre[kKeep ? NV : 1], gate[kKeep ? NV : 1];
   if constexpr (kKeep) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       post[i] = weight(p.post, i, 0);
       pre[i] = weight(p.pre, i, 0);
-      gate[i] = weight(nullptr, i, 0);
+      gate[i] = piece_of<T>(1.f);
     }
   }
   constexpr int kHeld = SUMS == kNoSums ? 1 : NV;
-  float sum_pre[kHeld][VEC], q[kHeld][VEC], sum_post[SUMS == kGateSums ? NV : 1][VEC];
+  float sum_pre[kHeld][kN], q[kHeld][kN], sum_post[SUMS == kGateSums ? NV : 1][kN];
   if constexpr (SUMS != kNoSums) {
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
+      for (int e = 0; e < kN; e++) {
         sum_pre[i][e] = q[i][e] = 0.f;
         if constexpr (SUMS == kGateSums) sum_post[i][e] = 0.f;
       }
   }
-  long long held = -1;  // the row of `gate` that q belongs to
+  int held = -1;  // the row of `gate` that q belongs to
   // a gate's sums are complete: where parts hold whole gates, its gradient is written here
   auto close_gate = [&] {
     if constexpr (SUMS == kGateSums) {
       if (held < 0) return;
 #pragma unroll
       for (int i = 0; i < NV; i++) {
-        const Piece<T, VEC> w = weight(p.post, i, 0), g = weight(p.gate, i, (size_t)held * p.ld_gate);
-        float dgate[VEC];
+        const Piece<T> w = weight(p.post, i, 0), g = weight(p.gate, i, held * p.ld_gate);
+        float dgate[kN];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
+        for (int e = 0; e < kN; e++) {
           dgate[e] = w.at(e) * q[i][e];
           sum_post[i][e] = __builtin_fmaf(g.at(e), q[i][e], sum_post[i][e]);
           q[i][e] = 0.f;
         }
-        if (p.dgate && in(i)) store_piece<T, VEC>(p.dgate, (size_t)held * p.d + column(i), dgate);
+        if (p.dgate && me.in(i))
+          store_piece<WHOLE>((T*)p.dgate + (long long)held * p.d + me.column(i), me.left(i), dgate);
       }
     }
   };
+  Piece<T> dy[NV], dr[NV], r[NV], b[NV];
+  auto fetch = [&](long long row) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      dy[i] = dr[i] = r[i] = b[i] = piece_of<T>(0.f);
+      if (row >= last || !me.in(i)) continue;
+      if (p.pre) {
+        dy[i] = load(p.dy, row * p.ld_dy, i);
+        r[i] = load(p.r, row * p.ld_r, i);
+      }
+      if (p.dr) dr[i] = load(p.dr, row * p.ld_dr, i);
+      if (p.block) b[i] = load(p.block, row * p.ld_block, i);
+    }
+  };
   int turn = 0;
+  if (kKeep) fetch(first);
   // every set of a workgroup goes round equally often: they meet at barriers
   for (long long at = 0; at < parts.rows_per_part; at++) {
     const long long row = first + at;
     const bool live = row < last;
     if (kSets == 1 && !live) break;
-    Piece<T, VEC> dy[NV], dr[NV], r[NV], b[NV];
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-#pragma unroll
-      for (int e = 0; e < VEC; e++) dy[i].v[e] = dr[i].v[e] = r[i].v[e] = b[i].v[e] = (T)0.f;
-      if (!live || !in(i)) continue;
-      if (p.pre) {
-        dy[i] = load_piece<T, VEC>(p.dy, (size_t)row * p.ld_dy + column(i));
-        r[i] = load_piece<T, VEC>(p.r, (size_t)row * p.ld_r + column(i));
-      }
-      if (p.dr) dr[i] = load_piece<T, VEC>(p.dr, (size_t)row * p.ld_dr + column(i));
-      if (p.block) b[i] = load_piece<T, VEC>(p.block, (size_t)row * p.ld_block + column(i));
-    }
+    if (!kKeep) fetch(row);
     const float rstd1 = live && p.post ? p.stats[2 * row] : 1.f;
     const float rstd2 = live && p.pre ? p.stats[2 * row + 1] : 0.f;
     if (live && p.block) {
-      const long long g = row / p.rows_per_gate;
+      const int g = (int)((unsigned)row / (unsigned)p.rows_per_gate);
       if (g != held) {
         close_gate();
         held = g;
         if constexpr (kKeep) {
 #pragma unroll
-          for (int i = 0; i < NV; i++) gate[i] = weight(p.gate, i, (size_t)g * p.ld_gate);
+          for (int i = 0; i < NV; i++) gate[i] = weight(p.gate, i, g * p.ld_gate);
         }
       }
     }
     // this row's weights of piece i
     struct Weights {
-      Piece<T, VEC> post, pre, gate;
+      Piece<T> post, pre, gate;
     };
     auto weights = [&](int i) {
       Weights w;
@@ -324,7 +387,7 @@ __global__ __launch_bounds__(64 * wg_waves(W)) void norm_grad_kernel(NormGradArg
         as_stored(gate[i]);
         w = {post[i], pre[i], gate[i]};
       } else {
-        w = {weight(p.post, i, 0), weight(p.pre, i, 0), weight(p.gate, i, held < 0 ? 0 : (size_t)held * p.ld_gate)};
+        w = {weight(p.post, i, 0), weight(p.pre, i, 0), weight(p.gate, i, held < 0 ? 0 : held * p.ld_gate)};
       }
       return w;
     };
@@ -333,7 +396,7 @@ __global__ __launch_bounds__(64 * wg_waves(W)) void norm_grad_kernel(NormGradArg
     for (int i = 0; i < NV; i++) {
       const Weights w = weights(i);
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
+      for (int e = 0; e < kN; e++) {
         const float dyp = dy[i].at(e) * w.pre.at(e), rh = r[i].at(e) * rstd2;
         const float gpb = w.gate.at(e) * w.post.at(e) * (b[i].at(e) * rstd1);
         s[0] = __builtin_fmaf(dyp, rh, s[0]);
@@ -342,46 +405,55 @@ __global__ __launch_bounds__(64 * wg_waves(W)) void norm_grad_kernel(NormGradArg
         s[3] = __builtin_fmaf(gpb, rh, s[3]);
       }
     }
+    Piece<T> this_dy[NV], this_dr[NV], this_r[NV], this_b[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      this_dy[i] = dy[i];
+      this_dr[i] = dr[i];
+      this_r[i] = r[i];
+      this_b[i] = b[i];
+    }
+    if (kKeep) fetch(row + 1);
     add_up<W, 4>(s, room, wave, turn);
     const float m1 = s[0] * mean;
     const float m2 = p.post ? mean * (s[1] + rstd2 * (s[2] - m1 * s[3])) : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      if (!live || !in(i)) continue;
-      as_stored(dy[i]);
-      as_stored(dr[i]);
-      as_stored(r[i]);
-      as_stored(b[i]);
+      if (!live || !me.in(i)) continue;
+      as_stored(this_dy[i]);
+      as_stored(this_dr[i]);
+      as_stored(this_r[i]);
+      as_stored(this_b[i]);
       const Weights w = weights(i);
-      float d0[VEC], db[VEC];
+      float d0[kN], db[kN];
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        const float rh = r[i].at(e) * rstd2, bh = b[i].at(e) * rstd1;
-        const float dt = __builtin_fmaf(rstd2, dy[i].at(e) * w.pre.at(e) - rh * m1, dr[i].at(e));
+      for (int e = 0; e < kN; e++) {
+        const float rh = this_r[i].at(e) * rstd2, bh = this_b[i].at(e) * rstd1, dye = this_dy[i].at(e);
+        const float dt = __builtin_fmaf(rstd2, dye * w.pre.at(e) - rh * m1, this_dr[i].at(e));
         d0[e] = p.scale * dt;
         db[e] = rstd1 * (dt * w.gate.at(e) * w.post.at(e) - bh * m2);
         if constexpr (SUMS != kNoSums) {
-          sum_pre[i][e] = __builtin_fmaf(dy[i].at(e), rh, sum_pre[i][e]);
+          sum_pre[i][e] = __builtin_fmaf(dye, rh, sum_pre[i][e]);
           q[i][e] = __builtin_fmaf(dt, bh, q[i][e]);
         }
       }
-      if (p.dresidual) store_piece<T, VEC>(p.dresidual, (size_t)row * p.d + column(i), d0);
-      if (p.dblock) store_piece<T, VEC>(p.dblock, (size_t)row * p.d + column(i), db);
+      const long long at_row = row * p.d + me.column(i);
+      if (p.dresidual) store_piece<WHOLE>((T*)p.dresidual + at_row, me.left(i), d0);
+      if (p.dblock) store_piece<WHOLE>((T*)p.dblock + at_row, me.left(i), db);
     }
   }
   if constexpr (SUMS != kNoSums) {
     close_gate();
     if (part >= parts.parts) return;
-    float* const out = p.partials + (size_t)part * 2 * p.d;
+    float* const out = p.partials + part * 2 * p.d;
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      if (!in(i)) continue;
+    for (int i = 0; i < NV; i++)
 #pragma unroll
-      for (int e = 0; e < VEC; e++) {
-        out[column(i) + e] = sum_pre[i][e];
-        out[p.d + column(i) + e] = SUMS == kGateSums ? sum_post[i % (SUMS == kGateSums ? NV : 1)][e] : q[i][e];
+      for (int e = 0; e < kN; e++) {
+        if (me.left(i) <= e) continue;
+        out[me.column(i) + e] = sum_pre[i][e];
+        out[p.d + me.column(i) + e] = SUMS == kGateSums ? sum_post[i % (SUMS == kGateSums ? NV : 1)][e] : q[i][e];
       }
-    }
   }
 }
 
@@ -440,8 +512,8 @@ bool whole16(const void* p, long long ld, int per) { return ((uintptr_t)p & 15) 
 struct NormShape {
   int nv, waves;
 };
-NormShape norm_shape(int d, int vec) {
-  const int pieces = (d + vec - 1) / vec;
+NormShape norm_shape(int d, int size) {
+  const int pieces = (d * size + 15) / 16;
   int waves = 1;
   while (waves < 16 && 64 * waves < pieces) waves *= 2;
   int nv = 1;
@@ -449,9 +521,9 @@ NormShape norm_shape(int d, int vec) {
   return {nv, waves};
 }
 
-template <class T, int VEC, class F>
+template <class T, class F>
 void with_shape(int d, F f) {
-  const NormShape s = norm_shape(d, VEC);
+  const NormShape s = norm_shape(d, sizeof(T));
   using std::integral_constant;
 #define SHAPE(NV, W) \
   if (s.nv == NV && s.waves == W) return f(integral_constant<int, NV>{}, integral_constant<int, W>{});
@@ -461,17 +533,16 @@ void with_shape(int d, F f) {
   SHAPE(1, 8)
   SHAPE(1, 16)
   SHAPE(2, 16)
-  if constexpr (VEC <= 4) { SHAPE(4, 16) }
-  if constexpr (VEC == 1) { SHAPE(8, 16) SHAPE(16, 16) }
+  if constexpr (sizeof(T) == 4) { SHAPE(4, 16) }
 #undef SHAPE
 }
 
-template <class T, class F>
-void with_vectors(bool vectors, F f) {
-  if (vectors)
-    f(std::integral_constant<int, 16 / sizeof(T)>{});
+template <class F>
+void with_whole(bool whole, F f) {
+  if (whole)
+    f(std::true_type{});
   else
-    f(std::integral_constant<int, 1>{});
+    f(std::false_type{});
 }
 
 template <class F>
@@ -485,23 +556,26 @@ constexpr int kPartWaves = 4096;  // waves that the parts of a backward pass mak
 
 }  // namespace
 
-bool norm_vectors(const NormArgs& a, int size) {
+namespace {
+
+bool norm_whole(const NormArgs& a, int size) {
   const int per = 16 / size;
   return a.d % per == 0 && whole16(a.residual, a.ld_residual, per) && whole16(a.block, a.ld_block, per) &&
          whole16(a.gate, a.ld_gate, per) && whole16(a.post, 0, per) && whole16(a.pre, 0, per) &&
          whole16(a.r, 0, per) && whole16(a.y, 0, per);
 }
-bool norm_vectors(const NormGradArgs& a, int size) {
+bool norm_whole(const NormGradArgs& a, int size) {
   const int per = 16 / size;
   return a.d % per == 0 && whole16(a.dy, a.ld_dy, per) && whole16(a.dr, a.ld_dr, per) && whole16(a.r, a.ld_r, per) &&
          whole16(a.block, a.ld_block, per) && whole16(a.gate, a.ld_gate, per) && whole16(a.post, 0, per) &&
          whole16(a.pre, 0, per) && whole16(a.dresidual, 0, per) && whole16(a.dblock, 0, per) && whole16(a.dgate, 0, per);
 }
 
-NormParts norm_parts(long long rows, int rows_per_gate, int d, int size, bool vectors) {
+}  // namespace
+
+NormParts norm_parts(long long rows, int rows_per_gate, int d, int size) {
   NormParts p = {};
-  p.waves = norm_shape(d, vectors ? 16 / size : 1).waves;
-  const long long most = kPartWaves / p.waves;
+  const long long most = kPartWaves / norm_shape(d, size).waves;
   p.gates = (rows + rows_per_gate - 1) / rows_per_gate;
   p.whole = p.gates > most;
   if (p.whole) {
@@ -523,13 +597,13 @@ NormParts norm_parts(long long rows, int rows_per_gate, int d, int size, bool ve
 void launch_norm(const NormArgs& a, NormType type, int cus, hipStream_t stream) {
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
-    with_vectors<T>(norm_vectors(a, sizeof(T)), [&](auto vec) {
-      with_shape<T, decltype(vec)::value>(a.d, [&](auto nv, auto w) {
-        constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
-        constexpr int rows = wg_waves(W) / W;
-        const long long groups = (a.rows + rows - 1) / rows, most = 0x7fffffff;
-        hipLaunchKernelGGL((norm_kernel<T, VEC, NV, W>), dim3((unsigned)std::min(groups, most)),
-                           dim3(64 * wg_waves(W)), 0, stream, a);
+    with_whole(norm_whole(a, sizeof(T)), [&](auto whole) {
+      with_shape<T>(a.d, [&](auto nv, auto w) {
+        constexpr int NV = decltype(nv)::value, W = decltype(w)::value, per_wg = wg_waves(W) / W;
+        // as many sets of waves as the chip holds, 32 waves to a compute unit
+        const int sets = (int)std::min<long long>(a.rows, (long long)cus * 32 / W);
+        hipLaunchKernelGGL((norm_kernel<T, decltype(whole)::value, NV, W>), dim3((sets + per_wg - 1) / per_wg),
+                           dim3(64 * wg_waves(W)), 0, stream, a, sets);
       });
     });
   });
@@ -538,19 +612,18 @@ void launch_norm(const NormArgs& a, NormType type, int cus, hipStream_t stream) 
 void launch_norm_grad(const NormGradArgs& a, NormType type, hipStream_t stream) {
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
-    const bool vectors = norm_vectors(a, sizeof(T));
-    const NormParts parts = norm_parts(a.rows, a.rows_per_gate, a.d, sizeof(T), vectors);
-    with_vectors<T>(vectors, [&](auto vec) {
-      with_shape<T, decltype(vec)::value>(a.d, [&](auto nv, auto w) {
-        constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
-        constexpr int sets = wg_waves(W) / W;
-        const dim3 grid((unsigned)((parts.parts + sets - 1) / sets)), block(64 * wg_waves(W));
+    const NormParts parts = norm_parts(a.rows, a.rows_per_gate, a.d, sizeof(T));
+    with_whole(norm_whole(a, sizeof(T)), [&](auto whole) {
+      with_shape<T>(a.d, [&](auto nv, auto w) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        constexpr int NV = decltype(nv)::value, W = decltype(w)::value, per_wg = wg_waves(W) / W;
+        const dim3 grid((unsigned)((parts.parts + per_wg - 1) / per_wg)), block(64 * wg_waves(W));
         if (!a.partials)
-          hipLaunchKernelGGL((norm_grad_kernel<T, VEC, NV, W, kNoSums>), grid, block, 0, stream, a, parts);
+          hipLaunchKernelGGL((norm_grad_kernel<T, WHOLE, NV, W, kNoSums>), grid, block, 0, stream, a, parts);
         else if (parts.whole)
-          hipLaunchKernelGGL((norm_grad_kernel<T, VEC, NV, W, kGateSums>), grid, block, 0, stream, a, parts);
+          hipLaunchKernelGGL((norm_grad_kernel<T, WHOLE, NV, W, kGateSums>), grid, block, 0, stream, a, parts);
         else
-          hipLaunchKernelGGL((norm_grad_kernel<T, VEC, NV, W, kPartSums>), grid, block, 0, stream, a, parts);
+          hipLaunchKernelGGL((norm_grad_kernel<T, WHOLE, NV, W, kPartSums>), grid, block, 0, stream, a, parts);
       });
     });
     if (a.partials)

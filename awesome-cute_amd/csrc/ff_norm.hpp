@@ -37,7 +37,7 @@ struct NormGradArgs {
   void* dpost;
   void* dgate;
   void* dpre;
-  float* partials;    // norm_parts(...).bytes, null if none of dpost, dgate, dpre is wanted
+  float* partials;    // norm_parts(...).bytes; null if none of dpost, dgate, dpre is wanted
   long long ld_dy, ld_dr, ld_r, ld_block, ld_gate;
   long long rows;
   int rows_per_gate;
@@ -48,15 +48,11 @@ struct NormGradArgs {
 // How the rows are dealt out to parts, a part a run of rows of which one set of waves keeps the
 // sums over rows: `rows_per_part` rows of one gate's, or whole gates' where these are short.
 struct NormParts {
-  int waves;          // of a row
   bool whole;         // a part holds whole gates
   long long parts, parts_per_gate, rows_per_part, gates;
   size_t bytes;       // of partial sums: two rows of d floats per part
 };
-NormParts norm_parts(long long rows, int rows_per_gate, int d, int bytes_per_element, bool vectors);
-// whether 16-byte loads may be used: d a multiple of them, and all addresses and distances
-bool norm_vectors(const NormArgs& a, int bytes_per_element);
-bool norm_vectors(const NormGradArgs& a, int bytes_per_element);
+NormParts norm_parts(long long rows, int rows_per_gate, int d, int bytes_per_element);
 constexpr int kNormMax = 16384;  // the longest row: sixteen elements to each of a workgroup's 1024 lanes
 
 enum NormType { kNormFp16, kNormBf16, kNormFp32 };
