@@ -29,6 +29,7 @@ SOURCES = {
     "f16_streamk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "f16_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ff_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "ff_big.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ff_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ff_grads.hip": [],
     "ff_norm.hip": [],
@@ -78,7 +79,7 @@ def build_library(verbose=False):
     # the assembly statements of the four-wave kernels and of the rows kernel over 128
     # columns (prologue, main loop and accumulator hand-over with fixed registers) are
     # written by generators; the sources include them from the build directory
-    for gen in ("gen_prefill_wide.py", "gen_rows_wide.py", "gen_dense.py"):
+    for gen in ("gen_prefill_wide.py", "gen_rows_wide.py", "gen_dense.py", "gen_products.py"):
         _run([sys.executable, os.path.join(CSRC, gen), objdir], verbose)
     objs = [os.path.join(objdir, src.replace(".hip", ".o")) for src in SOURCES]
     with ThreadPoolExecutor(4) as pool:

@@ -5,15 +5,12 @@
 namespace w4a16 {
 
 struct GatedGradArgs {
-  const void* dh;   // (m x n)
+  const void* dh;    // (m x n)
   const float* pre;  // (m x ldpre), the forward pass's sums
-  void* dgu;        // (m x 2n), zeros behind a row up to a multiple of 64 columns; or null
-  void* dgu_t;      // (2n x m), zeros likewise; or null
-  long long lddh, ldpre, lddgu, lddgu_t;
+  void* dgu;         // (m x 2n), zeros behind a row up to a multiple of 64 columns
+  long long lddh, ldpre, lddgu;
   int m, n, act;
 };
 void launch_gated_grad(const GatedGradArgs& a, bool bf, hipStream_t stream);
-void launch_transpose(const void* in, long long ld_in, void* out, long long ld_out, int rows, int cols,
-                      hipStream_t stream);
 
 }  // namespace w4a16

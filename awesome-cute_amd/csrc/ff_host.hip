@@ -19,6 +19,7 @@ using namespace w4a16;
 constexpr int kMaxDevices = 16;
 thread_local char g_error[256] = "";
 thread_local FfTile t_tile = {0, 0};  // feedforward_force_tile
+thread_local int t_slices = 0;
 
 int fail(int code, const char* fmt, ...) {
   va_list args;
@@ -51,6 +52,7 @@ int on_device(int dev, F launch) {
     if (!d.configured) {
       e = hipDeviceGetAttribute(&d.cus, hipDeviceAttributeMultiprocessorCount, dev);
       if (e == hipSuccess) e = configure_product_tiles();
+      if (e == hipSuccess) e = configure_product_big();
       if (e == hipSuccess) e = configure_product_rows();
       d.configured = e == hipSuccess;
     }
@@ -76,26 +78,54 @@ constexpr TileFit kFits[] = {
     {{64, 64}, 2.32, 0.191, 0.056, 0.77, 0.179},   {{64, 128}, 3.05, 0.277, 0.088, 2.18, 0.324},
     {{96, 128}, 3.27, 0.359, 0.093, 2.04, 0.436},  {{128, 128}, 3.17, 0.424, 0.095, 2.40, 0.500},
     {{96, 256}, 4.04, 0.531, 0.205, 3.09, 0.828},  {{128, 256}, 4.46, 0.594, 0.294, 4.30, 1.020},
-    {{256, 256}, 8.30, 1.186, 0.248, 1.87, 1.92}};
+    {{160, 256}, 6.30, 0.800, 0.160, 1.30, 1.25},  {{192, 256}, 7.00, 0.930, 0.190, 1.50, 1.47},
+    {{224, 256}, 7.60, 1.060, 0.220, 1.70, 1.70},  {{256, 256}, 8.30, 1.186, 0.248, 1.87, 1.92}};
+constexpr int kSlicesMost = 8;
 
-FfTile choose_tile(int m, int columns, int k, int cus) {
-  if (t_tile.rows > 0 && (t_tile.rows < 256 || k % kDnStageK == 0)) return t_tile;
-  FfTile best = {64, 64};
+struct ProductPlan {
+  FfTile tile;
+  int slices;
+};
+
+bool tile_takes(const FfTile& t, int k, Layout layout, bool padded) {
+  // (rows end where their stages do, or have zeros behind them)
+  if (big_tile(t)) return layout == kTurnBoth || padded || k % kDnStageK == 0;
+  return layout != kTurnBoth || t.rows != 96;  // (64, 128 or 256 columns of a turned operand)
+}
+
+// room: bytes for partial sums
+ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, bool padded, int cus, long long room) {
+  const int columns = product_columns(n, gated), stages = ceil_div(k, kDnStageK);
+  ProductPlan best = {{64, 64}, 1};
   double least = 0.0;
   for (const TileFit& f : kFits) {
-    if (f.tile.rows == 256 && k % kDnStageK != 0) continue;
-    const double tiles = (double)ceil_div(m, f.tile.rows) * ceil_div(columns, f.tile.cols), r = tiles / cus;
-    const int stages = ceil_div(k, kDnStageK), rounds = (int)((tiles + cus - 1) / cus);
-    // workgroups beyond one per compute unit: half way between the rounds and their share of one
-    const double more = r > 1.0 ? 0.5 * (rounds + r) - 1.0 : 0.0;
-    const double cost =
-        f.launch + stages * (f.stage + f.fill * (r < 1.0 ? r : 1.0)) + more * (f.more + f.more_stage * stages);
-    if (least == 0.0 || cost < least) {
-      best = f.tile;
-      least = cost;
+    if (t_tile.rows > 0 && tile_takes(t_tile, k, layout, padded) && (f.tile.rows != t_tile.rows || f.tile.cols != t_tile.cols)) continue;
+    if (!tile_takes(f.tile, k, layout, padded)) continue;
+    const long long tiles = (long long)ceil_div(m, f.tile.rows) * ceil_div(columns, f.tile.cols);
+    for (int slices = 1; slices <= kSlicesMost && slices <= stages; slices++) {
+      const double bytes = 4.0 * slices * m * columns;
+      if (slices > 1 && (bytes > (double)room || (t_slices == 0 && tiles * slices > 2 * cus))) break;
+      if (t_slices > 0 && slices != t_slices && t_slices <= stages && 4.0 * t_slices * m * columns <= (double)room) continue;
+      const double r = (double)tiles * slices / cus;
+      const int rounds = (int)((tiles * slices + cus - 1) / cus), each = ceil_div(stages, slices);
+      // workgroups beyond one per compute unit: half way between the rounds and their share of one
+      const double more = r > 1.0 ? 0.5 * (rounds + r) - 1.0 : 0.0;
+      double cost = f.launch + each * (f.stage + f.fill * (r < 1.0 ? r : 1.0)) + more * (f.more + f.more_stage * each);
+      // sums written and read again, and a launch that adds them
+      if (slices > 1) cost += 4.0 + 2.0 * bytes / 4.5e6;
+      if (least == 0.0 || cost < least) {
+        best = {f.tile, slices};
+        least = cost;
+      }
     }
   }
   return best;
+}
+// bytes of partial sums that a problem's plan wants
+long long plan_bytes(int m, int n, int k, bool gated, Layout layout, bool padded, int cus) {
+  if (m == 0 || n == 0 || k == 0) return 0;
+  const ProductPlan p = choose_plan(m, n, k, gated, layout, padded, cus, 1LL << 40);
+  return p.slices > 1 ? 4LL * p.slices * m * product_columns(n, gated) : 0;
 }
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
@@ -110,27 +140,51 @@ int check_matrix(const char* name, const void* p, long long ld, long long width)
 
 int check_sizes(int m, int n, int k, int type) {
   if (m < 0 || n < 0 || k < 0) return fail(FEEDFORWARD_ERR_SHAPE, "negative size (m=%d n=%d k=%d)", m, n, k);
-  if (n % 8 != 0 || k % 8 != 0)
-    return fail(FEEDFORWARD_ERR_SHAPE, "n = %d and k = %d must be multiples of 8", n, k);
+  if (n % 8 != 0) return fail(FEEDFORWARD_ERR_SHAPE, "widths must be multiples of 8 (n = %d)", n);
   if (type != FEEDFORWARD_FP16 && type != FEEDFORWARD_BF16)
     return fail(FEEDFORWARD_ERR_SHAPE, "unknown type %d", type);
   return FEEDFORWARD_OK;
 }
 
-int run_product(ProductArgs a, bool bf, int dev, hipStream_t stream) {
-  const long long columns = a.act == kActNone ? a.N : 2LL * ((a.N + 15) / 16 * 16);
+bool layout_of(int turned, Layout* layout, bool* padded) {
+  *padded = (turned & FEEDFORWARD_PADDED) != 0;
+  turned &= ~FEEDFORWARD_PADDED;
+  *layout = (Layout)turned;
+  return turned >= FEEDFORWARD_ROWS && turned <= FEEDFORWARD_TURN_BOTH && !(*padded && turned != FEEDFORWARD_TURN_B);
+}
+
+int run_product(ProductArgs a, Layout layout, bool padded, bool bf, void* room, long long room_bytes, int dev, hipStream_t stream) {
+  const bool gated = a.act != kActNone;
+  const long long columns = product_columns(a.N, gated);
   // (a launch's grid, at the smallest tiles)
-  if (columns > 0x3fffffffLL || (columns / 64 + 1) * (a.M / 64 + 1LL) > 0x3fffffffLL)
+  if (columns > 0x3fffffffLL || (columns / 64 + 1) * (a.M / 64 + 1LL) > 0x3fffffffLL / kSlicesMost)
     return fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many tiles", a.M, a.N);
   // a gated product's rows of either half are addressed from one place
-  if (a.act != kActNone && 2LL * a.N * a.ldb * 2 > 0x7fffffffLL)
+  if (gated && 2LL * a.N * a.ldb * 2 > 0x7fffffffLL)
     return fail(FEEDFORWARD_ERR_SHAPE, "weights of more than 2 GiB (n = %d, rows of %d): split the call", a.N, a.ldb);
+  if (room && off16(room)) return fail(FEEDFORWARD_ERR_SHAPE, "scratch must start on 16 bytes");
   return on_device(dev, [&](int cus) {
-    if (a.M <= kProductRows && t_tile.rows <= 0)
-      launch_product_rows(a, bf, stream);
+    if (layout == kRows && a.M <= kProductRows && t_tile.rows <= 0) return launch_product_rows(a, bf, stream);
+    const ProductPlan p = choose_plan(a.M, a.N, a.K, gated, layout, padded, cus, room ? room_bytes : 0);
+    a.slices = p.slices;
+    a.part = p.slices > 1 ? (float*)room : nullptr;
+    a.ldpart = (int)columns;
+    if (big_tile(p.tile))
+      launch_product_big(a, p.tile.rows, layout, bf, stream);
     else
-      launch_product_tiles(a, choose_tile(a.M, (int)columns, a.K, cus), bf, stream);
+      launch_product_tiles(a, p.tile, layout, bf, stream);
+    if (a.part) launch_sum_parts(a, bf, stream);
   });
+}
+
+int device_cus(int dev) {
+  static std::mutex mu;
+  static int known[kMaxDevices] = {};
+  if (dev < 0 || dev >= kMaxDevices) return 0;
+  std::lock_guard<std::mutex> lk(mu);
+  if (known[dev] == 0 && hipDeviceGetAttribute(&known[dev], hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+    known[dev] = 0;
+  return known[dev];
 }
 
 int type_bytes(int type) { return type == FEEDFORWARD_FP32 ? 4 : 2; }
@@ -158,10 +212,18 @@ int check_rows(const char* name, const void* p, long long ld, int d) {
 extern "C" {
 
 int feedforward_product(const void* A, const void* B, void* C, int m, int n, int k, long long lda, long long ldb,
-                        long long ldc, int type, int dev, void* stream) {
+                        long long ldc, int turned, int type, void* room, long long room_bytes, int dev,
+                        void* stream) {
   int rc = check_sizes(m, n, k, type);
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("A", A, lda, k);
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("B", B, ldb, k);
+  Layout layout = kRows;
+  bool padded = false;
+  if (rc == FEEDFORWARD_OK && !layout_of(turned, &layout, &padded)) rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
+  if (rc == FEEDFORWARD_OK && layout != kTurnBoth && k % 8 != 0)
+    rc = fail(FEEDFORWARD_ERR_SHAPE, "widths must be multiples of 8 (k = %d)", k);
+  if (rc == FEEDFORWARD_OK && layout == kTurnBoth && m % 8 != 0)
+    rc = fail(FEEDFORWARD_ERR_SHAPE, "m = %d must be a multiple of 8 where A is turned over", m);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("A", A, lda, layout == kTurnBoth ? m : padded ? (k + 63LL) / 64 * 64 : k);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("B", B, ldb, layout == kRows ? k : n);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("C", C, ldc, n);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
   if (k == 0) return fail(FEEDFORWARD_ERR_SHAPE, "k = 0: an empty sum");
@@ -169,13 +231,14 @@ int feedforward_product(const void* A, const void* B, void* C, int m, int n, int
   a.A = A, a.B = B, a.C = C;
   a.M = m, a.N = n, a.K = k;
   a.lda = (int)lda, a.ldb = (int)ldb, a.ldc = (int)ldc;
-  return run_product(a, type == FEEDFORWARD_BF16, dev, (hipStream_t)stream);
+  return run_product(a, layout, padded, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
 }
 
 int feedforward_gated(const void* x, const void* w, void* h, float* pre, int m, int n, int k, long long ldx,
-                      long long ldw, long long ldh, long long ldpre, int type, int activation, int dev,
-                      void* stream) {
+                      long long ldw, long long ldh, long long ldpre, int type, int activation, void* room,
+                      long long room_bytes, int dev, void* stream) {
   int rc = check_sizes(m, n, k, type);
+  if (rc == FEEDFORWARD_OK && k % 8 != 0) rc = fail(FEEDFORWARD_ERR_SHAPE, "widths must be multiples of 8 (k = %d)", k);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("x", x, ldx, k);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("w", w, ldw, k);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("h", h, ldh, n);
@@ -189,34 +252,31 @@ int feedforward_gated(const void* x, const void* w, void* h, float* pre, int m, 
   a.M = m, a.N = n, a.K = k;
   a.lda = (int)ldx, a.ldb = (int)ldw, a.ldc = (int)ldh, a.ldpre = (int)ldpre;
   a.act = activation;
-  return run_product(a, type == FEEDFORWARD_BF16, dev, (hipStream_t)stream);
+  return run_product(a, kRows, false, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
 }
 
-int feedforward_gated_grad(const void* dh, const float* pre, void* dgu, void* dgu_t, int m, int n, long long lddh,
-                           long long ldpre, long long lddgu, long long lddgu_t, int type, int activation, int dev,
-                           void* stream) {
+long long feedforward_product_bytes(int m, int n, int k, int gated, int turned, int dev) {
+  Layout layout;
+  bool padded;
+  if (check_sizes(m, n, k, FEEDFORWARD_FP16) != FEEDFORWARD_OK || !layout_of(turned, &layout, &padded)) return -1;
+  if (layout == kRows && m <= kProductRows && t_tile.rows <= 0) return 0;
+  const int cus = device_cus(dev);
+  return cus > 0 ? plan_bytes(m, n, k, gated != 0, layout, padded, cus) : 0;
+}
+
+int feedforward_gated_grad(const void* dh, const float* pre, void* dgu, int m, int n, long long lddh, long long ldpre,
+                           long long lddgu, int type, int activation, int dev, void* stream) {
   int rc = check_sizes(m, n, 0, type);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("dh", dh, lddh, n);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("pre", pre, ldpre, (n + 15LL) / 16 * 32);
-  if (rc == FEEDFORWARD_OK && dgu) rc = check_matrix("dgu", dgu, lddgu, (2LL * n + 63) / 64 * 64);
-  if (rc == FEEDFORWARD_OK && dgu_t) rc = check_matrix("dgu_t", dgu_t, lddgu_t, (m + 63LL) / 64 * 64);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("dgu", dgu, lddgu, (2LL * n + 63) / 64 * 64);
   if (rc == FEEDFORWARD_OK && !act_known(activation))
     rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
-  if (rc == FEEDFORWARD_OK && m > 64 * 65535) rc = fail(FEEDFORWARD_ERR_SHAPE, "m = %d: too many rows", m);
+  if (rc == FEEDFORWARD_OK && (long long)m * (n / 8 + 8) > 0x7fffffffLL * 128)
+    rc = fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many", m, n);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
-  const GatedGradArgs a = {dh, pre, dgu, dgu_t, lddh, ldpre, lddgu, lddgu_t, m, n, activation};
+  const GatedGradArgs a = {dh, pre, dgu, lddh, ldpre, lddgu, m, n, activation};
   return on_device(dev, [&](int) { launch_gated_grad(a, type == FEEDFORWARD_BF16, (hipStream_t)stream); });
-}
-
-int feedforward_transpose(const void* in, void* out, int rows, int cols, long long ld_in, long long ld_out, int dev,
-                          void* stream) {
-  if (rows < 0 || cols < 0) return fail(FEEDFORWARD_ERR_SHAPE, "negative size (%d x %d)", rows, cols);
-  if (cols % 8 != 0) return fail(FEEDFORWARD_ERR_SHAPE, "columns (%d) must be a multiple of 8", cols);
-  int rc = check_matrix("in", in, ld_in, cols);
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("out", out, ld_out, (rows + 63LL) / 64 * 64);
-  if (rc == FEEDFORWARD_OK && rows > 64 * 65535) rc = fail(FEEDFORWARD_ERR_SHAPE, "%d rows: too many", rows);
-  if (rc != FEEDFORWARD_OK || rows == 0 || cols == 0) return rc;
-  return on_device(dev, [&](int) { launch_transpose(in, ld_in, out, ld_out, rows, cols, (hipStream_t)stream); });
 }
 
 int feedforward_norm(const void* residual, long long ld_residual, const void* block, long long ld_block,
@@ -278,18 +338,24 @@ int feedforward_norm_grad(const void* dy, long long ld_dy, const void* dr, long 
   return on_device(dev, [&](int) { launch_norm_grad(a, norm_type(type), (hipStream_t)stream); });
 }
 
-int feedforward_tile(int m, int n, int k, int gated, int cus, int* out) {
-  out[0] = out[1] = 0;
+int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int* out) {
+  out[0] = out[1] = out[2] = 0;
   const int rc = check_sizes(m, n, k, FEEDFORWARD_FP16);
-  if (rc != FEEDFORWARD_OK || m <= kProductRows || n == 0 || k == 0) return rc;
-  const FfTile t = choose_tile(m, gated ? 2 * ((n + 15) / 16 * 16) : n, k, cus);
-  out[0] = t.rows;
-  out[1] = t.cols;
+  if (rc != FEEDFORWARD_OK || n == 0 || k == 0 || m == 0) return rc;
+  Layout layout;
+  bool padded;
+  if (!layout_of(turned, &layout, &padded)) return fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
+  if (layout == kRows && m <= kProductRows) return rc;
+  const ProductPlan p = choose_plan(m, n, k, gated != 0, layout, padded, cus, 1LL << 40);
+  out[0] = p.tile.rows;
+  out[1] = p.tile.cols;
+  out[2] = p.slices;
   return rc;
 }
 
-void feedforward_force_tile(int rows, int cols) {
+void feedforward_force_tile(int rows, int cols, int slices) {
   t_tile = {0, 0};
+  t_slices = slices > kSlicesMost ? kSlicesMost : slices < 0 ? 0 : slices;
   for (const TileFit& f : kFits)
     if (f.tile.rows == rows && f.tile.cols == cols) t_tile = f.tile;
 }

@@ -10,17 +10,23 @@
 
 namespace w4a16 {
 
-// C (M x N) = A (M x K) B^T, B given as N rows of K, rows `lda`, `ldb`, `ldc` elements apart;
-// or, gated, C (M x n) = act(A G^T) * (A U^T), B given as the n rows of G and then the n of U.
+// How the operands of a product lie: as rows along the summed dimension, or turned over, B as K
+// rows of N and A as K rows of M (the gradients' products: dx = dy w, dw = dy^T x)
+enum Layout { kRows, kTurnB, kTurnBoth };
+
+// C (M x N) = A (M x K) B^T, rows `lda`, `ldb`, `ldc` elements apart; or, gated, C (M x n) =
+// act(A G^T) * (A U^T), B given as the n rows of G and then the n of U.
 struct ProductArgs {
   const void* A;
   const void* B;
   void* C;
-  float* pre;  // gated: null, or both sums for the backward pass, (M x ldpre) in the product's order
+  float* pre;   // gated: null, or both sums for the backward pass, (M x ldpre) in the product's order
+  float* part;  // null, or what the k range is cut into slices for: (slices x M x ldpart) partial sums
+                // in the product's order, which sum_parts turns into C
   int M, N, K;  // N: columns of C
-  int lda, ldb, ldc, ldpre;
+  int lda, ldb, ldc, ldpre, ldpart;
   int act;  // kActNone: not gated
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n, slices;
 };
 
 typedef __bf16 b4 __attribute__((ext_vector_type(4)));
@@ -62,15 +68,23 @@ __device__ __forceinline__ int gated_row(int first, int col, int n, int ldb) {
 // where column `col` of C has its gate's sum in a row of `pre`; its partner's is 16 further on
 __host__ __device__ __forceinline__ int pre_col(int col) { return ((col >> 4) << 5) + (col & 15); }
 
-// Tiles of ff_tiles.hip: rows x columns of the product, 256 x 256 the big kernel's
+// columns of the product, which are C's, or gates and ups
+__host__ __device__ __forceinline__ int product_columns(int n, bool gated) { return gated ? (n + 15) / 16 * 32 : n; }
+
+// Tiles: rows x columns of the product.  256 columns and 160, 192, 224 or 256 rows are
+// ff_big.hip's, the others ff_tiles.hip's.
 struct FfTile {
   int rows, cols;
 };
+inline bool big_tile(const FfTile& t) { return t.cols == 256 && t.rows >= 160; }
 hipError_t configure_product_tiles();
+hipError_t configure_product_big();
 hipError_t configure_product_rows();
-// launches of either kind; bf: bfloat16 operands
-void launch_product_tiles(ProductArgs a, const FfTile& t, bool bf, hipStream_t stream);
+// launches of any kind; bf: bfloat16 operands
+void launch_product_tiles(ProductArgs a, const FfTile& t, Layout layout, bool bf, hipStream_t stream);
+void launch_product_big(ProductArgs a, int rows, Layout layout, bool bf, hipStream_t stream);
 void launch_product_rows(const ProductArgs& a, bool bf, hipStream_t stream);
+void launch_sum_parts(const ProductArgs& a, bool bf, hipStream_t stream);
 constexpr int kProductRows = 64;  // rows of A that launch_product_rows takes at most
 
 }  // namespace w4a16

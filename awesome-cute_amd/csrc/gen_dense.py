@@ -1,7 +1,6 @@
 #!/usr/bin/env python3
 """Writes the main loops of the dense fp16 kernel (f16_streamk.hip) as inline
-assembly statements with fixed registers, one per tile shape, and that of the 256 x 256
-tile for bfloat16 as well (ff_tiles.hip).
+assembly statements with fixed registers, one per tile shape.
 
 A workgroup has four waves, one per SIMD, each with a 128 x 128 fp32
 accumulator (all 256 AGPRs): 256 x 256 tiles with a wave per quarter, and 128 x
@@ -147,7 +146,7 @@ def next_operands(sh, j, b):
     return ops
 
 
-def step(e, sh, mfma, slot, h, b, carry):
+def step(e, sh, slot, h, b, carry):
     """one step; carry: (slot, first load) of a request that the step before left unfinished"""
     steps = sh.steps
     outer = h == steps - 1
@@ -180,13 +179,13 @@ def step(e, sh, mfma, slot, h, b, carry):
         for o in range(8):
             e.need(AOP(i), *([BOP(b, o)] if i == 0 else []))
             acc = 32 * i + 4 * o
-            e.emit(f"{mfma} {aq(acc)}, {q(BOP(b, o))}, {q(AOP(i))}, {aq(acc)}")
+            e.emit(f"v_mfma_f32_16x16x32_f16 {aq(acc)}, {q(BOP(b, o))}, {q(AOP(i))}, {aq(acc)}")
             if 8 * i + o in at:
                 at[8 * i + o](e)
     return left
 
 
-def generate(sh, mfma):
+def generate(sh):
     e = Emitter()
     # prologue: every slot requested (the last one as far as an outer step would
     # have), the accumulators zeroed, the first step's operands read
@@ -218,7 +217,7 @@ def generate(sh, mfma):
     for turn in range(turns):
         for slot in range(sh.ring):
             for h in range(sh.steps):
-                carry = step(e, sh, mfma, slot, h, b, carry)
+                carry = step(e, sh, slot, h, b, carry)
                 b ^= 1
             e.emit(f"s_sub_u32 s{S_LEFT}, s{S_LEFT}, 1")
             e.emit(f"s_cmp_eq_u32 s{S_LEFT}, 0")
@@ -237,9 +236,9 @@ def generate(sh, mfma):
     return e.lines
 
 
-def statement(sh, mfma):
+def statement(sh):
     out = ["// generated by gen_dense.py -- do not edit", "asm volatile("]
-    out += [f'    "{l}\\n\\t"' for l in generate(sh, mfma)]
+    out += [f'    "{l}\\n\\t"' for l in generate(sh)]
     outs = [f'"={{{aq(32 * i + 4 * o)}}}"(acc[{i}][{o}])' for i in range(8) for o in range(8)]
     outs += [f'"+{{{sq(RA)}}}"(ra_words)', f'"+{{{sq(RB)}}}"(rb_words)', f'"+{{s{S_AT}}}"(s_at)']
     out.append("    : " + ",\n      ".join(outs))
@@ -261,6 +260,4 @@ if __name__ == "__main__":
     outdir = sys.argv[1] if len(sys.argv) > 1 else "."
     for sh in SHAPES:
         with open(f"{outdir}/f16_dense_{sh.name}.inc", "w") as f:
-            f.write(statement(sh, "v_mfma_f32_16x16x32_f16"))
-    with open(f"{outdir}/bf16_dense_{SHAPES[0].name}.inc", "w") as f:
-        f.write(statement(SHAPES[0], "v_mfma_f32_16x16x32_bf16"))
+            f.write(statement(sh))

@@ -1,0 +1,290 @@
+#!/usr/bin/env python3
+"""Writes the main loops of the big tiles of the feed-forward products (ff_big.hip) as inline
+assembly statements with fixed registers: for fp16 and bfloat16, for tiles of 32 rb rows (rb =
+5 ... 8) x 256 columns, and for operands by rows of the summed dimension's length or turned
+over, as rows along the output ("TurnB": B so, "TurnBoth": A too).
+
+A workgroup has four waves, one per SIMD, two by two, each with an accumulator of 16 rb x 128 in
+AGPRs; why assembly, and why that shape, says gen_dense.py, whose schedule this is with the
+number of row blocks, the reads per operand and the requests as parameters.
+
+A step is 8 rb MFMAs over 32 k-values: row blocks i = 0 ... rb - 1 of 16 rows, operands o = 0 ... 7
+of 16 columns.  A slab, 64 k-values, is two steps; two slabs are in LDS.  A operands are read
+`ahead` row blocks ahead, each row block into registers of its own; the eight B operands of the
+next step go into the other of two buffers:
+
+  inner step (the next step is in the same slab)   A and B reads dealt out evenly
+  outer step (the next step is in the next slab)
+     up to row block rb - ahead   the last A operands of this slab
+     then                         my loads of the next slab have landed, my reads of this one
+                                  too; barrier: so have everybody's
+     the rest                     B and A operands of the next step, alternating with the
+                                  request for the slab that goes where this one was; what does
+                                  not fit follows in the next step
+
+An operand by rows is one ds_read_b128; turned over it is two ds_read_b64_tr_b16, each of which
+gives sixteen lanes four k-values of their column from four rows of sixteen columns: twice the
+reads, as many bytes, and no transposed copy of the operand in memory.  More reads behind the
+barrier need it earlier, hence `ahead`.
+
+Every memory operation gets an MFMA to itself.  All s_waitcnt are computed from the order of
+issue (the counter holds 15: a wait for more becomes one for 14), and every operand is checked to
+be the one that its MFMA expects.
+
+Registers (v = VGPR, a = AGPR, s = SGPR):
+  a[32i+4o : +3]      accumulator of row block i, operand o
+  v[32b+4o : +3]      B operands, buffer b (step parity)
+  v[64+4i : +3]       A operand of row block i
+  v[96...] v[112...]  LDS addresses of the A and B reads: by rows j = slot x 2 + step; turned over
+                      8 slot + block
+  v[128+t]            byte offsets of this lane's loads, A then B
+  s[40:43] s[44:47]   buffer resources of A and B; the base moves on by a slab with every request
+  s49 s50 s51         slabs, requested, left
+  s52 s53 s59 s60     sizes of A and B for a slab, and for the last one (0 past it)
+  s54 s55 s57 s58     LDS addresses of this wave's part of the slots, A and B
+  s61 s62             bytes from one slab to the next, A and B
+"""
+import sys
+
+RA, RB = 40, 44
+S_N, S_REQ, S_LEFT, S_FULLA, S_FULLB, S_MA, S_MB = 49, 50, 51, 52, 53, 54, 57
+S_LASTA, S_LASTB, S_STEPA, S_STEPB = 59, 60, 61, 62
+V_A, V_B, V_OFF = 96, 112, 128
+ROW = 128           # bytes of a row of 64 k-values
+TURNED = 512        # bytes of a k-value's 256 columns
+RING, STEPS = 2, 2
+TYPES = {"f16": "v_mfma_f32_16x16x32_f16", "bf16": "v_mfma_f32_16x16x32_bf16"}
+
+
+class Shape:
+    def __init__(self, layout, rb):
+        self.layout, self.rb = layout, rb
+        self.turn_a, self.turn_b = layout == "both", layout in ("b", "both")
+        self.ahead = {"rows": 3, "b": 4, "both": 5}[layout]
+        if self.ahead > rb - 1:
+            self.ahead = rb - 1
+        # load instructions per wave and slab, 1 KiB each (a turned A is always 256 columns wide)
+        self.ta = 8 if self.turn_a else rb
+        self.loads = self.ta + 8
+        self.slab_a = 64 * TURNED if self.turn_a else 32 * rb * ROW
+        self.slab = self.slab_a + 256 * ROW
+        self.a_reads, self.b_reads = 1 + self.turn_a, 1 + self.turn_b
+        room = 8 * self.ahead - 8 * self.b_reads - self.ahead * self.a_reads
+        self.tail = min(self.loads, room)  # loads requested right behind the barrier
+        assert self.tail > 0
+
+
+def q(base): return f"v[{base}:{base + 3}]"
+def d(base): return f"v[{base}:{base + 1}]"
+def aq(base): return f"a[{base}:{base + 3}]"
+def sq(base): return f"s[{base}:{base + 3}]"
+def BOP(b, o): return 32 * b + 4 * o
+def AOP(i): return 64 + 4 * i
+
+
+class Emitter:
+    def __init__(self):
+        self.lines = []
+        self.lds = []       # destinations of LDS reads in flight, oldest first
+        self.content = {}   # register quad -> what was last read into it
+
+    def emit(self, text):
+        self.lines.append(text)
+
+    def read(self, dst, text, tag):
+        self.emit(text)
+        self.lds.append(dst)
+        self.content.setdefault(dst, [])
+        if not self.content[dst] or self.content[dst][0] != tag:
+            self.content[dst] = [tag, 0]
+        self.content[dst][1] += 1
+
+    def need(self, wants):
+        """wait until the reads into these registers have landed (LDS reads land in order)"""
+        for reg, tag, count in wants:
+            assert self.content.get(reg) == [tag, count], (reg, tag, self.content.get(reg))
+        regs = [reg for reg, _, _ in wants]
+        last = max([i for i, r in enumerate(self.lds) if r in regs], default=-1)
+        if last >= 0:
+            left = min(len(self.lds) - last - 1, 14)
+            self.lds = self.lds[len(self.lds) - left:]
+            self.emit(f"s_waitcnt lgkmcnt({left})")
+
+
+def request_head(e, sh, slot, first=False):
+    """what the loads of the next slab need: base, sizes (the last slab's, zero past it), m0"""
+    if not first:
+        e.emit(f"s_add_u32 s{RA}, s{RA}, s{S_STEPA}")
+        e.emit(f"s_addc_u32 s{RA + 1}, s{RA + 1}, 0")
+        e.emit(f"s_add_u32 s{RB}, s{RB}, s{S_STEPB}")
+        e.emit(f"s_addc_u32 s{RB + 1}, s{RB + 1}, 0")
+    e.emit(f"s_add_u32 s{S_REQ}, s{S_REQ}, 1")
+    e.emit(f"s_cmp_eq_u32 s{S_REQ}, s{S_N}")
+    e.emit(f"s_cselect_b32 s{RA + 2}, s{S_LASTA}, s{S_FULLA}")
+    e.emit(f"s_cselect_b32 s{RB + 2}, s{S_LASTB}, s{S_FULLB}")
+    e.emit(f"s_cmp_le_u32 s{S_REQ}, s{S_N}")
+    e.emit(f"s_cselect_b32 s{RA + 2}, s{RA + 2}, 0")
+    e.emit(f"s_cselect_b32 s{RB + 2}, s{RB + 2}, 0")
+    e.emit(f"s_mov_b32 m0, s{S_MA + slot}")
+
+
+def request(e, sh, slot, t):
+    """load t of a slab; m0 is left ready for load t + 1 (an MFMA or a nop lies between)"""
+    e.emit(f"buffer_load_dwordx4 v{V_OFF + t}, {sq(RA if t < sh.ta else RB)}, 0 offen lds")
+    if t == sh.ta - 1:
+        e.emit(f"s_mov_b32 m0, s{S_MB + slot}")
+    elif t < sh.loads - 1:
+        e.emit("s_add_u32 m0, m0, 0x400")
+
+
+def assign(ops, n):
+    """(preferred MFMA, operation) -> {MFMA: operation}, distinct, in the order of preference"""
+    at, last = {}, -1
+    for pref, fn in sorted(ops, key=lambda x: x[0]):
+        last = max(last + 1, int(pref))
+        at[last] = fn
+    assert last < n, last
+    return at
+
+
+def reads_of(sh, turned, addr, dst, slot, h, block, tag):
+    """the LDS reads of an operand, one or two functions"""
+    if not turned:
+        return [lambda e: e.read(dst, f"ds_read_b128 {q(dst)}, v{addr + 2 * slot + h} offset:{block * 16 * ROW}", tag)]
+    return [lambda e, j=j: e.read(dst, f"ds_read_b64_tr_b16 {d(dst + 2 * j)}, v{addr + 8 * slot + block} "
+                                       f"offset:{(32 * h + 4 * j) * TURNED}", tag) for j in range(2)]
+
+
+def read_a(sh, slot, h, i, tag):
+    return reads_of(sh, sh.turn_a, V_A, AOP(i), slot, h, i, ("a", tag, i))
+
+
+def read_b(sh, slot, h, b, o, tag):
+    return reads_of(sh, sh.turn_b, V_B, BOP(b, o), slot, h, o, ("b", tag, o))
+
+
+def next_operands(sh, slot, h, b, tag):
+    """the reads of the next step that an outer step issues, in order"""
+    ops = read_b(sh, slot, h, b, 0, tag) + read_a(sh, slot, h, 0, tag)
+    for o in range(1, 8):
+        ops += read_b(sh, slot, h, b, o, tag)
+    for i in range(1, sh.ahead):
+        ops += read_a(sh, slot, h, i, tag)
+    return ops
+
+
+def step(e, sh, mfma, slot, h, b, carry, tag):
+    """one step; carry: (slot, first load) of a request that the step before left unfinished"""
+    rb, ahead = sh.rb, sh.ahead
+    outer = h == STEPS - 1
+    nslot, nh = ((slot + 1) % RING, 0) if outer else (slot, h + 1)
+    ops = []
+    for i in range(rb - ahead):
+        ops += [(8 * i + x, fn) for x, fn in enumerate(read_a(sh, slot, h, i + ahead, tag))]
+    for x, t in enumerate(range(carry[1], sh.loads) if carry else ()):
+        ops.append((2 + 4 * x, lambda e, t=t: request(e, sh, carry[0], t)))
+    left = None
+    if outer:
+        bar = 8 * (rb - ahead)
+
+        def barrier(e):
+            e.emit("s_waitcnt vmcnt(0) lgkmcnt(0)")
+            e.lds = []
+            e.emit("s_barrier")
+            request_head(e, sh, slot)
+
+        ops.append((bar - 1, barrier))
+        behind = []
+        reads = next_operands(sh, nslot, nh, b ^ 1, tag + 1)
+        loads = [lambda e, t=t: request(e, sh, slot, t) for t in range(sh.tail)]
+        while reads or loads:  # in turns, and what is left of either
+            if reads:
+                behind.append(reads.pop(0))
+            if loads:
+                behind.append(loads.pop(0))
+        ops += [(bar + x * 1e-3, fn) for x, fn in enumerate(behind)]
+        left = (slot, sh.tail) if sh.tail < sh.loads else None
+    else:
+        for i in range(ahead):
+            ops += [(8 * (rb - ahead + i) + x, fn) for x, fn in enumerate(read_a(sh, nslot, nh, i, tag + 1))]
+        for o in range(8):
+            ops += [(rb * o + 2 + x, fn) for x, fn in enumerate(read_b(sh, nslot, nh, b ^ 1, o, tag + 1))]
+    at = assign(ops, 8 * rb)
+    for i in range(rb):
+        for o in range(8):
+            e.need([(AOP(i), ("a", tag, i), sh.a_reads)] + ([(BOP(b, o), ("b", tag, o), sh.b_reads)] if i == 0 else []))
+            acc = 32 * i + 4 * o
+            e.emit(f"{mfma} {aq(acc)}, {q(BOP(b, o))}, {q(AOP(i))}, {aq(acc)}")
+            if 8 * i + o in at:
+                at[8 * i + o](e)
+    return left
+
+
+def generate(sh, mfma):
+    e = Emitter()
+    # prologue: both slots requested (the second as far as an outer step would have), the
+    # accumulators zeroed, the first step's operands read
+    e.emit(f"s_mov_b32 s{S_REQ}, 0")
+    e.emit(f"s_mov_b32 s{S_LEFT}, s{S_N}")
+    e.emit(f"s_add_u32 s{S_MA + 1}, s{S_MA}, {sh.slab}")
+    e.emit(f"s_add_u32 s{S_MB + 1}, s{S_MB}, {sh.slab}")
+    for s in range(RING):
+        request_head(e, sh, s, s == 0)
+        for t in range(sh.loads if s < RING - 1 else sh.tail):
+            e.emit("s_nop 0")
+            request(e, sh, s, t)
+    for n in range(32 * sh.rb):
+        e.emit(f"v_accvgpr_write_b32 a{n}, 0")
+    e.emit(f"s_waitcnt vmcnt({sh.tail})")
+    e.emit("s_barrier")
+    for fn in next_operands(sh, 0, 0, 0, 0):
+        fn(e)
+    carry = (RING - 1, sh.tail) if sh.tail < sh.loads else None
+    first_carry, start = carry, list(e.lds)
+    e.emit(".Lff_loop_%=:")
+    tag = 0
+    for slot in range(RING):
+        for h in range(STEPS):
+            carry = step(e, sh, mfma, slot, h, tag & 1, carry, tag)
+            tag += 1
+        e.emit(f"s_sub_u32 s{S_LEFT}, s{S_LEFT}, 1")
+        e.emit(f"s_cmp_eq_u32 s{S_LEFT}, 0")
+        e.emit("s_cbranch_scc0 .Lff_loop_%=" if slot == RING - 1 else "s_cbranch_scc1 .Lff_done_%=")
+    # the loop closes: what is in flight and in the registers is what it started with
+    assert tag % 2 == 0 and e.lds == start and carry == first_carry, (e.lds, start)
+    e.emit(".Lff_done_%=:")
+    # the last MFMAs' results are not readable for 18 cycles, and the hardware does not
+    # interlock that for what follows; nothing may be on its way into LDS or registers either
+    e.emit("s_nop 15")
+    e.emit("s_nop 15")
+    e.emit("s_waitcnt vmcnt(0) lgkmcnt(0)")
+    return e.lines
+
+
+def statement(sh, mfma):
+    out = ["// generated by gen_products.py -- do not edit", "asm volatile("]
+    out += [f'    "{l}\\n\\t"' for l in generate(sh, mfma)]
+    outs = [f'"={{{aq(32 * i + 4 * o)}}}"(acc[{i}][{o}])' for i in range(sh.rb) for o in range(8)]
+    outs += [f'"+{{{sq(RA)}}}"(ra_words)', f'"+{{{sq(RB)}}}"(rb_words)']
+    out.append("    : " + ",\n      ".join(outs))
+    ins = [f'"{{s{S_N}}}"(slabs)', f'"{{s{S_MA}}}"(lds_a)', f'"{{s{S_MB}}}"(lds_b)',
+           f'"{{s{S_FULLA}}}"(full_a)', f'"{{s{S_FULLB}}}"(full_b)', f'"{{s{S_LASTA}}}"(last_a)',
+           f'"{{s{S_LASTB}}}"(last_b)', f'"{{s{S_STEPA}}}"(step_a)', f'"{{s{S_STEPB}}}"(step_b)']
+    ins += [f'"{{v{V_A + j}}}"(a_rd[{j}])' for j in range(16 if sh.turn_a else 4)]
+    ins += [f'"{{v{V_B + j}}}"(b_rd[{j}])' for j in range(16 if sh.turn_b else 4)]
+    ins += [f'"{{v{V_OFF + t}}}"(src[{t}])' for t in range(sh.loads)]
+    out.append("    : " + ",\n      ".join(ins))
+    clob = [f"v{n}" for n in range(64 + 4 * sh.rb)]
+    clob += [f"s{S_REQ}", f"s{S_LEFT}", f"s{S_MA + 1}", f"s{S_MB + 1}"]
+    clob += ["scc", "memory"]  # (m0 is the compiler's to reserve; it keeps nothing there)
+    out.append("    : " + ", ".join(f'"{c}"' for c in clob) + ");")
+    return "\n".join(out) + "\n"
+
+
+if __name__ == "__main__":
+    outdir = sys.argv[1] if len(sys.argv) > 1 else "."
+    for type, mfma in TYPES.items():
+        for layout in ("rows", "b", "both"):
+            for rb in (5, 6, 7, 8):
+                with open(f"{outdir}/ff_{type}_{layout}_{rb}.inc", "w") as f:
+                    f.write(statement(Shape(layout, rb), mfma))

@@ -400,6 +400,17 @@ variable_list once_differentiable(variable_list&& grads, const char* name) {
   return (*error)(std::move(marked));
 }
 
+// Scratch for a product's partial sums, where its plan has any
+struct Room {
+  at::Tensor t;
+  long long bytes;
+  Room(const at::Tensor& like, int64_t m, int64_t n, int64_t k, bool gated, int turned)
+      : bytes(feedforward_product_bytes((int)m, (int)n, (int)k, gated, turned, like.get_device())) {
+    if (bytes > 0) t = at::empty({bytes / 4}, options_as(like).dtype(at::kFloat));
+  }
+  void* at() const { return t.defined() ? t.data_ptr() : nullptr; }
+};
+
 // act(x G^T) * (x U^T), and with `keep` both sums (otherwise undefined)
 std::pair<at::Tensor, at::Tensor> gated_forward(const at::Tensor& x, const at::Tensor& w, int act, bool keep) {
   check_dense(x, w);
@@ -409,9 +420,10 @@ std::pair<at::Tensor, at::Tensor> gated_forward(const at::Tensor& x, const at::T
   at::Tensor h = empty_rows(x, n), pre;
   if (keep) pre = at::empty({m, ldpre}, options_as(x).dtype(at::kFloat));
   const Matrix a(x.reshape({m, k})), b(w);
+  const Room room(x, m, n, k, true, FEEDFORWARD_ROWS);
   feedforward_check(feedforward_gated(a.at(), b.at(), h.data_ptr(), keep ? (float*)pre.data_ptr() : nullptr, (int)m,
-                                      (int)n, (int)k, a.ld, b.ld, n, ldpre, type_code(x), act, dev,
-                                      current_stream(dev)));
+                                      (int)n, (int)k, a.ld, b.ld, n, ldpre, type_code(x), act, room.at(), room.bytes,
+                                      dev, current_stream(dev)));
   return {h, pre};
 }
 
@@ -421,33 +433,31 @@ at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w) {
   const int dev = x.get_device();
   at::Tensor y = empty_rows(x, n);
   const Matrix a(x.reshape({m, k})), b(w);
+  const Room room(x, m, n, k, false, FEEDFORWARD_ROWS);
   feedforward_check(feedforward_product(a.at(), b.at(), y.data_ptr(), (int)m, (int)n, (int)k, a.ld, b.ld, n,
-                                        type_code(x), dev, current_stream(dev)));
+                                        FEEDFORWARD_ROWS, type_code(x), room.at(), room.bytes, dev,
+                                        current_stream(dev)));
   return y;
 }
 
-// The gradients of rows x (m, k) and weights w (r, k) of a product, from its gradient as rows
-// (d, m x r, zeros behind it up to a multiple of 64 columns unless `depth` is r) and turned over
-// (d_t, r x m, zeros likewise).  dx = d w and dw = d_t x are products over r and m, of the
-// transposes of w and x.
-void product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, int64_t depth, const at::Tensor& d_t,
-                   at::Tensor* dx, at::Tensor* dw) {
-  const int64_t m = x.size(0), k = x.size(1), r = w.size(0);
+// The gradients of x (m, k) and w (r, k) from that of their product, d (m, r): dx = d w and
+// dw = d^T x, sums over r and over m.  padded: FEEDFORWARD_PADDED where rows of d are, or 0.
+void product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, int padded, const at::Tensor& dx,
+                   const at::Tensor& dw) {
+  const int64_t k = w.size(1), m = x.numel() / k, r = w.size(0);
   const int type = type_code(x), dev = x.get_device();
   void* const st = current_stream(dev);
-  if (dx->defined()) {
+  if (dx.defined()) {
     const Matrix b(w);
-    const at::Tensor turned = empty_as(x, {k, up64(r)});
-    feedforward_check(feedforward_transpose(b.at(), turned.data_ptr(), (int)r, (int)k, b.ld, up64(r), dev, st));
-    feedforward_check(feedforward_product(d.at(), turned.data_ptr(), dx->data_ptr(), (int)m, (int)k, (int)depth, d.ld,
-                                          up64(r), k, type, dev, st));
+    const Room room(x, m, k, r, false, FEEDFORWARD_TURN_B | padded);
+    feedforward_check(feedforward_product(d.at(), b.at(), dx.data_ptr(), (int)m, (int)k, (int)r, d.ld, b.ld, k,
+                                          FEEDFORWARD_TURN_B | padded, type, room.at(), room.bytes, dev, st));
   }
-  if (dw->defined()) {
-    const Matrix a(x);
-    const at::Tensor turned = empty_as(x, {k, up64(m)});
-    feedforward_check(feedforward_transpose(a.at(), turned.data_ptr(), (int)m, (int)k, a.ld, up64(m), dev, st));
-    feedforward_check(feedforward_product(d_t.data_ptr(), turned.data_ptr(), dw->data_ptr(), (int)r, (int)k,
-                                          (int)up64(m), up64(m), up64(m), k, type, dev, st));
+  if (dw.defined()) {
+    const Matrix a(x.reshape({m, k}));
+    const Room room(x, r, k, m, false, FEEDFORWARD_TURN_BOTH);
+    feedforward_check(feedforward_product(d.at(), a.at(), dw.data_ptr(), (int)r, (int)k, (int)m, d.ld, a.ld, k,
+                                          FEEDFORWARD_TURN_BOTH, type, room.at(), room.bytes, dev, st));
   }
 }
 
@@ -462,22 +472,17 @@ std::pair<at::Tensor, at::Tensor> gated_backward(const at::Tensor& dh, const at:
                     "dh and the sums must be those of x and weight");
   const int dev = x.get_device();
   check_capture({&x, &w}, dev);
-  at::Tensor dx, dw, turned;
+  at::Tensor dx, dw;
   if (want_x) dx = empty_as(x, x.sizes());
   if (want_w) dw = empty_as(w, w.sizes());
   if (m == 0 || n == 0) {
     if (want_x) dx.zero_();
     if (want_w) dw.zero_();
   } else if (want_x || want_w) {
-    const Matrix d(dh.reshape({m, n}));
-    Matrix dgu;
-    if (want_x) dgu = Matrix(empty_as(x, {m, up64(2 * n)}));
-    if (want_w) turned = empty_as(x, {2 * n, up64(m)});
-    feedforward_check(feedforward_gated_grad(d.at(), (const float*)pre.data_ptr(), want_x ? dgu.at() : nullptr,
-                                             want_w ? turned.data_ptr() : nullptr, (int)m, (int)n, d.ld, ldpre,
-                                             up64(2 * n), up64(m), type_code(x), act, dev, current_stream(dev)));
-    at::Tensor rows_dx = want_x ? dx.view({m, k}) : dx;
-    product_grads(x.reshape({m, k}), w, dgu, up64(2 * n), turned, &rows_dx, &dw);
+    const Matrix d(dh.reshape({m, n})), dgu(empty_as(x, {m, up64(2 * n)}));
+    feedforward_check(feedforward_gated_grad(d.at(), (const float*)pre.data_ptr(), dgu.at(), (int)m, (int)n, d.ld,
+                                             ldpre, up64(2 * n), type_code(x), act, dev, current_stream(dev)));
+    product_grads(x, w, dgu, FEEDFORWARD_PADDED, dx, dw);
   }
   return {dx, dw};
 }
@@ -491,21 +496,14 @@ std::pair<at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy, const at
                     "dy must be that of x and weight");
   const int dev = x.get_device();
   check_capture({&x, &w}, dev);
-  at::Tensor dx, dw, turned;
+  at::Tensor dx, dw;
   if (want_x) dx = empty_as(x, x.sizes());
   if (want_w) dw = empty_as(w, w.sizes());
   if (m == 0 || n == 0) {
     if (want_x) dx.zero_();
     if (want_w) dw.zero_();
   } else if (want_x || want_w) {
-    const Matrix d(dy.reshape({m, n}));
-    if (want_w) {
-      turned = empty_as(x, {n, up64(m)});
-      feedforward_check(feedforward_transpose(d.at(), turned.data_ptr(), (int)m, (int)n, d.ld, up64(m), dev,
-                                              current_stream(dev)));
-    }
-    at::Tensor rows_dx = want_x ? dx.view({m, k}) : dx;
-    product_grads(x.reshape({m, k}), w, d, n, turned, &rows_dx, &dw);
+    product_grads(x, w, Matrix(dy.reshape({m, n})), 0, dx, dw);
   }
   return {dx, dw};
 }

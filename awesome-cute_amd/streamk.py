@@ -99,10 +99,10 @@ def gemm(A, B, C=None):
 # function where gradients are wanted.
 
 ACTIVATIONS = {"silu": 1, "gelu": 2}  # (gelu in its tanh form)
-_lib.feedforward_tile.restype = _I
-_lib.feedforward_tile.argtypes = [_I, _I, _I, _I, _I, _P]
+_lib.feedforward_plan.restype = _I
+_lib.feedforward_plan.argtypes = [_I, _I, _I, _I, _I, _I, _P]
 _lib.feedforward_force_tile.restype = None
-_lib.feedforward_force_tile.argtypes = [_I, _I]
+_lib.feedforward_force_tile.argtypes = [_I, _I, _I]
 _lib.feedforward_last_error.restype = ctypes.c_char_p
 
 
@@ -203,14 +203,15 @@ _gated_op.register_autograd(_gated_backward, setup_context=_keep_gated)
 _linear_op.register_autograd(_linear_backward, setup_context=_keep_linear)
 
 
-def product_tile(m, n, k, gated=False, cus=256):
-    """(rows, columns) of the tiles that compute `linear` or `gated`, or None for few rows."""
-    out = (ctypes.c_int * 2)()
-    if _lib.feedforward_tile(m, n, k, int(gated), cus, out) != 0:
+def product_plan(m, n, k, gated=False, turned=0, cus=256):
+    """(rows, columns, slices of k) of the tiles that compute `linear` or `gated` -- turned = 1: the
+    gradient of their inputs, m rows of n over k; 2: that of their weights --, or None for few rows."""
+    out = (ctypes.c_int * 3)()
+    if _lib.feedforward_plan(m, n, k, int(gated), turned, cus, out) != 0:
         raise ValueError(_lib.feedforward_last_error().decode())
     return tuple(out) if out[0] > 0 else None
 
 
-def force_product_tile(rows, cols=0):
-    """Tiles for every product of the calling thread; 0 = by cost."""
-    _lib.feedforward_force_tile(int(rows), int(cols))
+def force_product_tile(rows, cols=0, slices=0):
+    """Tiles and slices for every product of the calling thread that they can compute; 0 = by cost."""
+    _lib.feedforward_force_tile(int(rows), int(cols), int(slices))

@@ -51,13 +51,28 @@ int feedforward_gated_w4(const void *A, const void *B, void *C, const void *s, i
 /*
  * Matrices below are row-major in fp16 or bfloat16 (`type`), `ld...` elements from one row to
  * the next; rows start on 16 bytes (addresses, and ld a multiple of 8), are at most 4 MiB
- * apart, and n and k are multiples of 8.  Sums are fp32, results rounded once.  Entries may
+ * apart, and their widths are multiples of 8.  Sums are fp32, results rounded once.  Entries may
  * be called from any thread, on any stream, and captured.
  */
 
-/* C (m x n) = A (m x k) B^T, B n rows of k; k > 0 */
+/* how the operands of a product lie: by rows, A m rows of k and B n rows of k; B turned over, k
+ * rows of n; or both, A k rows of m (a multiple of 8; k need then be none) */
+#define FEEDFORWARD_ROWS 0
+#define FEEDFORWARD_TURN_B 1
+#define FEEDFORWARD_TURN_BOTH 2
+/* added to FEEDFORWARD_TURN_B: behind a row of A's k elements there are zeros up to the next
+ * multiple of 64, which lda has room for (as feedforward_gated_grad leaves them) */
+#define FEEDFORWARD_PADDED 4
+
+/* C (m x n) = A B^T, the sum over k > 0.  With `room`, device memory of room_bytes on 16 bytes,
+ * few tiles over a deep k are computed in slices of it, whose sums are added there in a fixed
+ * order; feedforward_product_bytes says what helps (0: nothing does), less or none is correct
+ * as well, in another order of the sums. */
 int feedforward_product(const void *A, const void *B, void *C, int m, int n, int k, long long lda,
-                        long long ldb, long long ldc, int type, int dev, void *stream);
+                        long long ldb, long long ldc, int turned, int type, void *room,
+                        long long room_bytes, int dev, void *stream);
+/* -1 for sizes that are refused */
+long long feedforward_product_bytes(int m, int n, int k, int gated, int turned, int dev);
 
 /* h (m x n) = act(x G^T) * (x U^T), element by element, x (m x k), w the n rows of G and behind
  * them the n rows of U.  w holds at most 2 GiB; k > 0.  pre, if not null, keeps both sums for
@@ -65,25 +80,21 @@ int feedforward_product(const void *A, const void *B, void *C, int m, int n, int
  * the sums of columns 16 i + c of x G^T are at 32 i + c and those of x U^T 16 further on. */
 int feedforward_gated(const void *x, const void *w, void *h, float *pre, int m, int n, int k,
                       long long ldx, long long ldw, long long ldh, long long ldpre, int type,
-                      int activation, int dev, void *stream);
+                      int activation, void *room, long long room_bytes, int dev, void *stream);
 
-/* The gradients of both sums from that of h: [dg | du] as rows (dgu, m x 2n) and turned over
- * (dgu_t, 2n x m), either of which may be null.  Behind a row of 2n or m columns there are
- * zeros up to the next multiple of 64, which ld has room for. */
-int feedforward_gated_grad(const void *dh, const float *pre, void *dgu, void *dgu_t, int m, int n,
-                           long long lddh, long long ldpre, long long lddgu, long long lddgu_t,
-                           int type, int activation, int dev, void *stream);
+/* The gradients of both sums from that of h: rows of [dg | du] (m x 2n), behind each of them
+ * zeros up to the next multiple of 64 columns, which lddgu has room for. */
+int feedforward_gated_grad(const void *dh, const float *pre, void *dgu, int m, int n,
+                           long long lddh, long long ldpre, long long lddgu, int type,
+                           int activation, int dev, void *stream);
 
-/* out (cols x rows) = in^T, in (rows x cols) of either type; zeros behind a row of out up to the
- * next multiple of 64 columns, which ld_out has room for */
-int feedforward_transpose(const void *in, void *out, int rows, int cols, long long ld_in,
-                          long long ld_out, int dev, void *stream);
-
-/* out[0..1] = rows and columns of the product's tiles for a device of `cus` compute units, zeros
- * where up to 64 rows are computed by blocks of columns; no GPU touched */
-int feedforward_tile(int m, int n, int k, int gated, int cus, int *out);
-/* such tiles for every product of the calling thread (0 = by cost); for tests and tools */
-void feedforward_force_tile(int rows, int cols);
+/* out[0..2] = rows and columns of the product's tiles and the slices of k, with room for them, on
+ * a device of `cus` compute units; zeros where up to 64 rows are computed by blocks of columns; no
+ * GPU touched */
+int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int *out);
+/* such tiles (0 = by cost) and slices (0 = by cost) for every product of the calling thread that
+ * they can compute; for tests and tools */
+void feedforward_force_tile(int rows, int cols, int slices);
 
 /*
  * The norm after a block, its gate, the residual's scale and the norm before the next block, row

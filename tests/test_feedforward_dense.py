@@ -123,53 +123,73 @@ def test_refuses_host_tensors_and_unknown_activations():
 def test_codes_of_the_entries(m, n, k, lda, ldb, ldc, type, code):
     import ctypes
     lib, L = streamk._lib, ctypes.c_longlong
-    rc = lib.feedforward_product(None, None, None, m, n, k, L(lda), L(ldb), L(ldc), type, 0, None)
+    rc = lib.feedforward_product(None, None, None, m, n, k, L(lda), L(ldb), L(ldc), 0, type, None, L(0), 0, None)
     assert rc == code
-    rc = lib.feedforward_gated(None, None, None, None, m, n, k, L(lda), L(ldb), L(ldc), L(2 * ldc), type, 1, 0, None)
+    rc = lib.feedforward_gated(None, None, None, None, m, n, k, L(lda), L(ldb), L(ldc), L(2 * ldc), type, 1, None, L(0),
+                               0, None)
     assert rc == code
     assert (len(lib.feedforward_last_error()) > 0) or code == 0
 
 
-def test_codes_of_the_gradients_and_transposes():
+@pytest.mark.parametrize("m,n,k,lda,ldb,turned,code", [
+    (0, 8, 16, 16, 8, 1, 0), (0, 8, 16, 8, 8, 1, 1), (0, 16, 16, 16, 8, 1, 1),  # B: k rows of n
+    (0, 8, 13, 8, 8, 2, 0), (8, 0, 13, 8, 8, 2, 0), (8, 0, 13, 0, 8, 2, 1), (12, 0, 8, 16, 8, 2, 1),  # A: k rows of m
+    (0, 8, 40, 40, 8, 5, 1), (0, 8, 40, 64, 8, 5, 0), (0, 8, 40, 64, 40, 4, 1),  # zeros behind rows of A
+    (0, 8, 64, 64, 64, 3, 1), (0, 8, 64, 64, 64, 6, 1), (0, 8, 64, 64, 64, -1, 1)])
+def test_codes_of_the_layouts(m, n, k, lda, ldb, turned, code):
+    import ctypes
+    lib, L = streamk._lib, ctypes.c_longlong
+    rc = lib.feedforward_product(None, None, None, m, n, k, L(lda), L(ldb), L(n), turned, 0, None, L(0), 0, None)
+    assert rc == code
+    # scratch off 16 bytes
+    assert lib.feedforward_product(ctypes.c_void_p(16), ctypes.c_void_p(16), ctypes.c_void_p(16), 8, 8, 8, L(8), L(8),
+                                   L(8), 0, 0, ctypes.c_void_p(8), L(1024), 0, None) == 1
+
+
+def test_codes_of_the_gradients():
     import ctypes
     lib, L = streamk._lib, ctypes.c_longlong
 
-    def grad(m, n, lddh, ldpre, lddgu, ldt, type=0, act=1, dgu=16, dgu_t=16):
-        return lib.feedforward_gated_grad(None, None, ctypes.c_void_p(dgu), ctypes.c_void_p(dgu_t), m, n, L(lddh),
-                                          L(ldpre), L(lddgu), L(ldt), type, act, 0, None)
+    def grad(m, n, lddh, ldpre, lddgu, type=0, act=1, dgu=16):
+        return lib.feedforward_gated_grad(None, None, ctypes.c_void_p(dgu), m, n, L(lddh), L(ldpre), L(lddgu), type, act,
+                                          0, None)
 
-    assert grad(0, 40, 40, 96, 128, 64) == 0
-    assert grad(0, 40, 40, 96, 80, 64) == 1       # no room for the zeros behind 2n columns
-    assert grad(70, 0, 8, 8, 64, 64) == 1         # ... behind m columns
-    assert grad(0, 40, 32, 96, 128, 64) == 1
-    assert grad(0, 40, 40, 88, 128, 64) == 1      # 48 columns of gates and ups in turns of sixteen
-    assert grad(0, 40, 40, 96, 128, 64, act=0) == 1
-    assert grad(0, 40, 40, 96, 128, 64, type=5) == 1
-    assert grad(0, 40, 40, 96, 128, 64, dgu=8) == 1  # off 16 bytes
-    turn = lib.feedforward_transpose
-    assert turn(None, None, 0, 8, L(8), L(64), 0, None) == 0
-    assert turn(None, None, 4, 12, L(16), L(64), 0, None) == 1
-    assert turn(None, None, 65, 8, L(8), L(64), 0, None) == 1
-    assert turn(None, None, -1, 8, L(8), L(64), 0, None) == 1
+    assert grad(0, 40, 40, 96, 128) == 0
+    assert grad(0, 40, 40, 96, 80) == 1       # no room for the zeros behind 2n columns
+    assert grad(0, 40, 32, 96, 128) == 1
+    assert grad(0, 40, 40, 88, 128) == 1      # 48 columns of gates and ups in turns of sixteen
+    assert grad(0, 40, 40, 96, 128, act=0) == 1
+    assert grad(0, 40, 40, 96, 128, type=5) == 1
+    assert grad(0, 40, 40, 96, 128, dgu=8) == 1  # off 16 bytes
     # more than 2 GiB of a gated product's weights
     rc = lib.feedforward_gated(None, None, None, None, 1, 1 << 20, 1024, L(1024), L(1024), L(1 << 20), L(1 << 21), 0, 1,
-                               0, None)
+                               None, L(0), 0, None)
     assert rc == 1 and b"2 GiB" in lib.feedforward_last_error()
 
 
-def test_tiles_cover_what_they_are_asked():
+TILES = [(64, 64), (64, 128), (96, 128), (128, 128), (96, 256), (128, 256), (160, 256), (192, 256), (224, 256), (256, 256)]
+
+
+def test_plans_are_tiles_that_can_compute_the_problem():
     seen = set()
     rng = np.random.default_rng(0)
-    for _ in range(4000):
+    for _ in range(8000):
         m, n, k = (int(2 ** rng.uniform(*r)) for r in ((0, 14), (3, 14), (3, 14)))
         n, k = 8 * max(1, n // 8), 8 * max(1, k // 8)
-        for gated in (False, True):
-            t = streamk.product_tile(m, n, k, gated)
-            assert (t is None) == (m <= 64)
+        for gated, turned in ((False, 0), (True, 0), (False, 1), (False, 2), (False, 5)):
+            if turned == 2:
+                m, k = 8 * max(1, m // 8), m
+            t = streamk.product_plan(m, n, k, gated, turned)
+            assert (t is None) == (m <= 64 and turned == 0)
             if t:
-                assert k % 64 == 0 or t != (256, 256)
-                seen.add(t)
-    assert seen == {(64, 64), (64, 128), (96, 128), (128, 128), (96, 256), (128, 256), (256, 256)}
+                rows, cols, slices = t
+                assert (rows, cols) in TILES and 1 <= slices <= min(8, -(-k // 64))
+                assert k % 64 == 0 or turned in (2, 5) or rows < 160
+                assert rows != 96 or turned != 2
+                seen.add(((rows, cols), min(slices, 2)))
+            if turned == 2:
+                m, k = k, m
+    assert {t for t, _ in seen} == set(TILES)  # none that nothing reaches
 
 
 # --- on the GPU ----------------------------------------------------------------------------
@@ -190,15 +210,13 @@ def test_forward(m, n, k, type):
     check_product(streamk.linear(x, w), x, w, type)
 
 
-TILES = [(64, 64), (64, 128), (96, 128), (128, 128), (96, 256), (128, 256), (256, 256)]
-
-
 @gpu
+@pytest.mark.parametrize("slices", [1, 3])
 @pytest.mark.parametrize("tile", TILES)
-@pytest.mark.parametrize("m,n,k", [(1, 8, 64), (300, 520, 192), (257, 136, 1096), (130, 264, 128)])
-def test_every_tile(tile, m, n, k):
+@pytest.mark.parametrize("m,n,k", [(1, 8, 64), (300, 520, 192), (257, 136, 1096), (130, 264, 128), (333, 304, 640)])
+def test_every_tile(tile, m, n, k, slices):
     try:
-        streamk.force_product_tile(*tile)
+        streamk.force_product_tile(*tile, slices)
         for type in TYPES:
             x, w, dh = make(m, n, k, type, 5)
             x.requires_grad_()
@@ -208,9 +226,50 @@ def test_every_tile(tile, m, n, k):
             h = streamk.gated(x, w, "gelu")
             ref.check_forward(h.detach(), type)
             ref.check_grads(dh, *torch.autograd.grad(h, (x, w), dh), type)
-            check_product(streamk.linear(x.detach(), w.detach()), x.detach(), w.detach(), type)
+            y = streamk.linear(x, w[:n])
+            check_product(y.detach(), x.detach(), w[:n].detach(), type)
+            dx, dw = torch.autograd.grad(y, (x, w), dh)
+            check_product(dx, dh, w[:n].detach().t(), type)
+            check_product(dw[:n], dh.t(), x.detach().t(), type)
     finally:
         streamk.force_product_tile(0)
+
+
+@gpu
+@pytest.mark.parametrize("turned", [0, 1, 2, 5])
+def test_layouts_beside_rows_that_hold_nan(turned):
+    """Matrices inside larger ones: what lies beside them, and behind their last row, is NaN."""
+    import ctypes
+    lib, L, P = streamk._lib, ctypes.c_longlong, ctypes.c_void_p
+    for tile in (0, (64, 64), (128, 128), (128, 256), (160, 256), (256, 256)):
+        for m, n, k in ((72, 200, 136), (328, 264, 320), (64, 24, 56)):
+            gen = torch.Generator(device="cuda").manual_seed(m)
+            a, b = (torch.randn(r, k, device="cuda", generator=gen).half() for r in (m, n))
+
+            def inside(x, pad=0):
+                rows, cols = x.shape
+                room = torch.full((rows + 80, cols + 96), float("nan"), dtype=torch.float16, device="cuda")
+                room[8:8 + rows, 16:16 + cols] = x
+                if pad:
+                    room[8:8 + rows, 16 + cols:16 + -(-cols // 64) * 64] = 0
+                return room, room[8:8 + rows, 16:16 + cols]
+
+            ra, va = inside(a.t().contiguous() if turned == 2 else a, turned == 5)
+            rb, vb = inside(b.t().contiguous() if turned else b)
+            rc, vc = inside(torch.zeros(m, n, device="cuda").half())
+            before = rc.clone()
+            room = torch.empty(3 * m * n, device="cuda")
+            try:
+                streamk.force_product_tile(*(tile if tile else (0,)), slices=2 if m == 328 and tile else 0)
+                code = lib.feedforward_product(P(va.data_ptr()), P(vb.data_ptr()), P(vc.data_ptr()), m, n, k, L(va.stride(0)),
+                                               L(vb.stride(0)), L(vc.stride(0)), turned, 0, P(room.data_ptr()),
+                                               L(4 * room.numel()), 0, P(torch.cuda.current_stream().cuda_stream))
+            finally:
+                streamk.force_product_tile(0)
+            assert code == 0
+            check_product(vc, a, b, torch.float16)
+            vc.copy_(before[8:8 + m, 16:16 + n])
+            assert torch.equal(rc.isnan(), before.isnan()) and not rc.nan_to_num().any()  # nothing else was written
 
 
 GRADS = [(1, 8, 8), (3, 40, 72), (65, 64, 64), (64, 520, 136), (200, 1032, 264), (777, 200, 1000), (1237, 2744, 1032),
