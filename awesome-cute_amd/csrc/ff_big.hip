@@ -22,7 +22,8 @@ struct BigShape {
   // the results leave in two halves: RB / 2 (rounded up) row blocks of either wave row, and the rest
   static constexpr int kHalf = (RB + 1) / 2;
   static constexpr int kOut = 32 * kHalf * out_pitch<256, false>();
-  static constexpr int kLds = 2 * kSlab > kOut ? 2 * kSlab : kOut;
+  static constexpr int kRing = 3 * kSlab <= 160 * 1024 ? 3 : 2;
+  static constexpr int kLds = kRing * kSlab > kOut ? kRing * kSlab : kOut;
   static_assert(kLds <= 160 * 1024, "LDS of a compute unit");
 };
 
@@ -100,10 +101,10 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
   // LDS: where this wave's loads of slot 0 go, and where its operands of every slot are read
   const int lds = (int)(size_t)smem;
   const int lds_a = lds + wave * TA * 1024, lds_b = lds + Sh::kSlabA + wave * TB * 1024;
-  int a_rd[Sh::kTurnA ? 16 : 4], b_rd[Sh::kTurnedB ? 16 : 4];
+  int a_rd[(Sh::kTurnA ? 8 : 2) * Sh::kRing], b_rd[(Sh::kTurnedB ? 8 : 2) * Sh::kRing];
   const int turned_at = (8 * kg + (nu >> 2)) * 512 + 8 * (nu & 3), swizzle = turned_swizzle<256>(8 * kg + (nu >> 2));
 #pragma unroll
-  for (int slot = 0; slot < 2; slot++) {
+  for (int slot = 0; slot < Sh::kRing; slot++) {
     const int slab_a = lds + slot * Sh::kSlab, slab_b = slab_a + Sh::kSlabA;
     if constexpr (Sh::kTurnA) {
 #pragma unroll

@@ -9,7 +9,7 @@ AGPRs; why assembly, and why that shape, says gen_dense.py, whose schedule this 
 number of row blocks, the reads per operand and the requests as parameters.
 
 A step is 8 rb MFMAs over 32 k-values: row blocks i = 0 ... rb - 1 of 16 rows, operands o = 0 ... 7
-of 16 columns.  A slab, 64 k-values, is two steps; two slabs are in LDS.  A operands are read
+of 16 columns.  A slab, 64 k-values, is two steps; LDS holds a ring of two slabs, or three of 160 rows.  A operands are read
 `ahead` row blocks ahead, each row block into registers of its own; the eight B operands of the
 next step go into the other of two buffers:
 
@@ -35,24 +35,25 @@ Registers (v = VGPR, a = AGPR, s = SGPR):
   a[32i+4o : +3]      accumulator of row block i, operand o
   v[32b+4o : +3]      B operands, buffer b (step parity)
   v[64+4i : +3]       A operand of row block i
-  v[96...] v[112...]  LDS addresses of the A and B reads: by rows j = slot x 2 + step; turned over
+  v[96...] v[120...]  LDS addresses of the A and B reads: by rows j = slot x 2 + step; turned over
                       8 slot + block
-  v[128+t]            byte offsets of this lane's loads, A then B
+  v[144+t]            byte offsets of this lane's loads, A then B
   s[40:43] s[44:47]   buffer resources of A and B; the base moves on by a slab with every request
   s49 s50 s51         slabs, requested, left
-  s52 s53 s59 s60     sizes of A and B for a slab, and for the last one (0 past it)
-  s54 s55 s57 s58     LDS addresses of this wave's part of the slots, A and B
-  s61 s62             bytes from one slab to the next, A and B
+  s52 s53 s60 s61     sizes of A and B for a slab, and for the last one (0 past it)
+  s[54:56] s[57:59]   LDS addresses of this wave's part of the slots, A and B
+  s62 s63             bytes from one slab to the next, A and B
 """
 import sys
 
 RA, RB = 40, 44
 S_N, S_REQ, S_LEFT, S_FULLA, S_FULLB, S_MA, S_MB = 49, 50, 51, 52, 53, 54, 57
-S_LASTA, S_LASTB, S_STEPA, S_STEPB = 59, 60, 61, 62
-V_A, V_B, V_OFF = 96, 112, 128
+S_LASTA, S_LASTB, S_STEPA, S_STEPB = 60, 61, 62, 63
+V_A, V_B, V_OFF = 96, 120, 144
 ROW = 128           # bytes of a row of 64 k-values
 TURNED = 512        # bytes of a k-value's 256 columns
-RING, STEPS = 2, 2
+STEPS = 2           # of 32 k-values in a slab
+LDS = 160 * 1024
 TYPES = {"f16": "v_mfma_f32_16x16x32_f16", "bf16": "v_mfma_f32_16x16x32_bf16"}
 
 
@@ -68,6 +69,7 @@ class Shape:
         self.loads = self.ta + 8
         self.slab_a = 64 * TURNED if self.turn_a else 32 * rb * ROW
         self.slab = self.slab_a + 256 * ROW
+        self.ring = 3 if 3 * self.slab <= LDS else 2
         self.a_reads, self.b_reads = 1 + self.turn_a, 1 + self.turn_b
         room = 8 * self.ahead - 8 * self.b_reads - self.ahead * self.a_reads
         self.tail = min(self.loads, room)  # loads requested right behind the barrier
@@ -177,7 +179,7 @@ def step(e, sh, mfma, slot, h, b, carry, tag):
     """one step; carry: (slot, first load) of a request that the step before left unfinished"""
     rb, ahead = sh.rb, sh.ahead
     outer = h == STEPS - 1
-    nslot, nh = ((slot + 1) % RING, 0) if outer else (slot, h + 1)
+    nslot, nh = ((slot + 1) % sh.ring, 0) if outer else (slot, h + 1)
     ops = []
     for i in range(rb - ahead):
         ops += [(8 * i + x, fn) for x, fn in enumerate(read_a(sh, slot, h, i + ahead, tag))]
@@ -188,7 +190,7 @@ def step(e, sh, mfma, slot, h, b, carry, tag):
         bar = 8 * (rb - ahead)
 
         def barrier(e):
-            e.emit("s_waitcnt vmcnt(0) lgkmcnt(0)")
+            e.emit(f"s_waitcnt vmcnt({(sh.ring - 2) * sh.loads}) lgkmcnt(0)")
             e.lds = []
             e.emit("s_barrier")
             request_head(e, sh, slot)
@@ -226,30 +228,31 @@ def generate(sh, mfma):
     # accumulators zeroed, the first step's operands read
     e.emit(f"s_mov_b32 s{S_REQ}, 0")
     e.emit(f"s_mov_b32 s{S_LEFT}, s{S_N}")
-    e.emit(f"s_add_u32 s{S_MA + 1}, s{S_MA}, {sh.slab}")
-    e.emit(f"s_add_u32 s{S_MB + 1}, s{S_MB}, {sh.slab}")
-    for s in range(RING):
+    for s in range(1, sh.ring):
+        e.emit(f"s_add_u32 s{S_MA + s}, s{S_MA}, {s * sh.slab}")
+        e.emit(f"s_add_u32 s{S_MB + s}, s{S_MB}, {s * sh.slab}")
+    for s in range(sh.ring):
         request_head(e, sh, s, s == 0)
-        for t in range(sh.loads if s < RING - 1 else sh.tail):
+        for t in range(sh.loads if s < sh.ring - 1 else sh.tail):
             e.emit("s_nop 0")
             request(e, sh, s, t)
     for n in range(32 * sh.rb):
         e.emit(f"v_accvgpr_write_b32 a{n}, 0")
-    e.emit(f"s_waitcnt vmcnt({sh.tail})")
+    e.emit(f"s_waitcnt vmcnt({(sh.ring - 2) * sh.loads + sh.tail})")
     e.emit("s_barrier")
     for fn in next_operands(sh, 0, 0, 0, 0):
         fn(e)
-    carry = (RING - 1, sh.tail) if sh.tail < sh.loads else None
+    carry = (sh.ring - 1, sh.tail) if sh.tail < sh.loads else None
     first_carry, start = carry, list(e.lds)
     e.emit(".Lff_loop_%=:")
     tag = 0
-    for slot in range(RING):
+    for slot in range(sh.ring):
         for h in range(STEPS):
             carry = step(e, sh, mfma, slot, h, tag & 1, carry, tag)
             tag += 1
         e.emit(f"s_sub_u32 s{S_LEFT}, s{S_LEFT}, 1")
         e.emit(f"s_cmp_eq_u32 s{S_LEFT}, 0")
-        e.emit("s_cbranch_scc0 .Lff_loop_%=" if slot == RING - 1 else "s_cbranch_scc1 .Lff_done_%=")
+        e.emit("s_cbranch_scc0 .Lff_loop_%=" if slot == sh.ring - 1 else "s_cbranch_scc1 .Lff_done_%=")
     # the loop closes: what is in flight and in the registers is what it started with
     assert tag % 2 == 0 and e.lds == start and carry == first_carry, (e.lds, start)
     e.emit(".Lff_done_%=:")
@@ -270,12 +273,13 @@ def statement(sh, mfma):
     ins = [f'"{{s{S_N}}}"(slabs)', f'"{{s{S_MA}}}"(lds_a)', f'"{{s{S_MB}}}"(lds_b)',
            f'"{{s{S_FULLA}}}"(full_a)', f'"{{s{S_FULLB}}}"(full_b)', f'"{{s{S_LASTA}}}"(last_a)',
            f'"{{s{S_LASTB}}}"(last_b)', f'"{{s{S_STEPA}}}"(step_a)', f'"{{s{S_STEPB}}}"(step_b)']
-    ins += [f'"{{v{V_A + j}}}"(a_rd[{j}])' for j in range(16 if sh.turn_a else 4)]
-    ins += [f'"{{v{V_B + j}}}"(b_rd[{j}])' for j in range(16 if sh.turn_b else 4)]
+    ins += [f'"{{v{V_A + j}}}"(a_rd[{j}])' for j in range((8 if sh.turn_a else 2) * sh.ring)]
+    ins += [f'"{{v{V_B + j}}}"(b_rd[{j}])' for j in range((8 if sh.turn_b else 2) * sh.ring)]
     ins += [f'"{{v{V_OFF + t}}}"(src[{t}])' for t in range(sh.loads)]
     out.append("    : " + ",\n      ".join(ins))
     clob = [f"v{n}" for n in range(64 + 4 * sh.rb)]
-    clob += [f"s{S_REQ}", f"s{S_LEFT}", f"s{S_MA + 1}", f"s{S_MB + 1}"]
+    clob += [f"s{S_REQ}", f"s{S_LEFT}"]
+    clob += [f"s{S_MA + s}" for s in range(1, sh.ring)] + [f"s{S_MB + s}" for s in range(1, sh.ring)]
     clob += ["scc", "memory"]  # (m0 is the compiler's to reserve; it keeps nothing there)
     out.append("    : " + ", ".join(f'"{c}"' for c in clob) + ");")
     return "\n".join(out) + "\n"
