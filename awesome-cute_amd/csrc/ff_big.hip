@@ -18,12 +18,13 @@ struct BigShape {
   static constexpr bool kTurnA = LAYOUT == kTurnBoth, kTurnedB = LAYOUT != kRows;
   static constexpr int kTM = 32 * RB;
   static constexpr int kTA = kTurnA ? 8 : RB, kTB = 8;  // load instructions per wave and slab
-  static constexpr int kSlabA = kTA * 4 * 1024, kSlab = kSlabA + 256 * 128;
+  static constexpr int kSlabA = kTA * 4 * 1024, kSlabB = 256 * 128;
   // the results leave in two halves: RB / 2 (rounded up) row blocks of either wave row, and the rest
   static constexpr int kHalf = (RB + 1) / 2;
   static constexpr int kOut = 32 * kHalf * out_pitch<256, false>();
-  static constexpr int kRing = 3 * kSlab <= 160 * 1024 ? 3 : 2;
-  static constexpr int kLds = kRing * kSlab > kOut ? kRing * kSlab : kOut;
+  static constexpr int kRingA = 3 * (kSlabA + kSlabB) <= 160 * 1024 ? 3 : 2, kRingB = 3;  // slabs in LDS
+  static constexpr int kRings = kRingA * kSlabA + kRingB * kSlabB;
+  static constexpr int kLds = kRings > kOut ? kRings : kOut;
   static_assert(kLds <= 160 * 1024, "LDS of a compute unit");
 };
 
@@ -100,26 +101,30 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
 
   // LDS: where this wave's loads of slot 0 go, and where its operands of every slot are read
   const int lds = (int)(size_t)smem;
-  const int lds_a = lds + wave * TA * 1024, lds_b = lds + Sh::kSlabA + wave * TB * 1024;
-  int a_rd[(Sh::kTurnA ? 8 : 2) * Sh::kRing], b_rd[(Sh::kTurnedB ? 8 : 2) * Sh::kRing];
+  const int lds_a = lds + wave * TA * 1024, lds_b = lds + Sh::kRingA * Sh::kSlabA + wave * TB * 1024;
+  int a_rd[(Sh::kTurnA ? 8 : 2) * Sh::kRingA], b_rd[(Sh::kTurnedB ? 8 : 2) * Sh::kRingB];
   const int turned_at = (8 * kg + (nu >> 2)) * 512 + 8 * (nu & 3), swizzle = turned_swizzle<256>(8 * kg + (nu >> 2));
 #pragma unroll
-  for (int slot = 0; slot < Sh::kRing; slot++) {
-    const int slab_a = lds + slot * Sh::kSlab, slab_b = slab_a + Sh::kSlabA;
+  for (int slot = 0; slot < Sh::kRingA; slot++) {
+    const int slab = lds + slot * Sh::kSlabA;
     if constexpr (Sh::kTurnA) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) a_rd[8 * slot + i] = slab_a + turned_at + 32 * ((RB * wm + i) ^ swizzle);
+      for (int i = 0; i < 8; i++) a_rd[8 * slot + i] = slab + turned_at + 32 * ((RB * wm + i) ^ swizzle);
     } else {
 #pragma unroll
       for (int h = 0; h < 2; h++)
-        a_rd[2 * slot + h] = slab_a + (16 * RB * wm + nu) * 128 + 16 * ((4 * h + kg) ^ (nu & 7));
+        a_rd[2 * slot + h] = slab + (16 * RB * wm + nu) * 128 + 16 * ((4 * h + kg) ^ (nu & 7));
     }
+  }
+#pragma unroll
+  for (int slot = 0; slot < Sh::kRingB; slot++) {
+    const int slab = lds + Sh::kRingA * Sh::kSlabA + slot * Sh::kSlabB;
     if constexpr (Sh::kTurnedB) {
 #pragma unroll
-      for (int o = 0; o < 8; o++) b_rd[8 * slot + o] = slab_b + turned_at + 32 * ((8 * wn + o) ^ swizzle);
+      for (int o = 0; o < 8; o++) b_rd[8 * slot + o] = slab + turned_at + 32 * ((8 * wn + o) ^ swizzle);
     } else {
 #pragma unroll
-      for (int h = 0; h < 2; h++) b_rd[2 * slot + h] = slab_b + (128 * wn + nu) * 128 + 16 * ((4 * h + kg) ^ (nu & 7));
+      for (int h = 0; h < 2; h++) b_rd[2 * slot + h] = slab + (128 * wn + nu) * 128 + 16 * ((4 * h + kg) ^ (nu & 7));
     }
   }
 

@@ -9,7 +9,10 @@ AGPRs; why assembly, and why that shape, says gen_dense.py, whose schedule this 
 number of row blocks, the reads per operand and the requests as parameters.
 
 A step is 8 rb MFMAs over 32 k-values: row blocks i = 0 ... rb - 1 of 16 rows, operands o = 0 ... 7
-of 16 columns.  A slab, 64 k-values, is two steps; LDS holds a ring of two slabs, or three of 160 rows.  A operands are read
+of 16 columns.  A slab, 64 k-values, is two steps.  LDS holds three slabs of B and two of A (three of 160 rows): of the two it
+is B, a model's weights, that comes from memory, and a load's way from there is longer than a
+slab's MFMAs (two and two: 2048 x 10752 x 4096, B turned over, 136 us with operands in the last-level
+cache and 175 from memory).  A operands are read
 `ahead` row blocks ahead, each row block into registers of its own; the eight B operands of the
 next step go into the other of two buffers:
 
@@ -19,8 +22,8 @@ next step go into the other of two buffers:
      then                         my loads of the next slab have landed, my reads of this one
                                   too; barrier: so have everybody's
      the rest                     B and A operands of the next step, alternating with the
-                                  request for the slab that goes where this one was; what does
-                                  not fit follows in the next step
+                                  request for the slabs of A and of B that go where this one's
+                                  were (a group); what does not fit follows in the next step
 
 An operand by rows is one ds_read_b128; turned over it is two ds_read_b64_tr_b16, each of which
 gives sixteen lanes four k-values of their column from four rows of sixteen columns: twice the
@@ -35,19 +38,20 @@ Registers (v = VGPR, a = AGPR, s = SGPR):
   a[32i+4o : +3]      accumulator of row block i, operand o
   v[32b+4o : +3]      B operands, buffer b (step parity)
   v[64+4i : +3]       A operand of row block i
-  v[96...] v[120...]  LDS addresses of the A and B reads: by rows j = slot x 2 + step; turned over
+  v[96...] v[120...]  LDS addresses of the A and B reads: by rows 2 slot + step; turned over
                       8 slot + block
   v[144+t]            byte offsets of this lane's loads, A then B
   s[40:43] s[44:47]   buffer resources of A and B; the base moves on by a slab with every request
-  s49 s50 s51         slabs, requested, left
+  s49 s50 s48 s51     slabs, requested of A and of B, left
   s52 s53 s60 s61     sizes of A and B for a slab, and for the last one (0 past it)
   s[54:56] s[57:59]   LDS addresses of this wave's part of the slots, A and B
   s62 s63             bytes from one slab to the next, A and B
 """
+import math
 import sys
 
 RA, RB = 40, 44
-S_N, S_REQ, S_LEFT, S_FULLA, S_FULLB, S_MA, S_MB = 49, 50, 51, 52, 53, 54, 57
+S_REQB, S_N, S_REQA, S_LEFT, S_FULLA, S_FULLB, S_MA, S_MB = 48, 49, 50, 51, 52, 53, 54, 57
 S_LASTA, S_LASTB, S_STEPA, S_STEPB = 60, 61, 62, 63
 V_A, V_B, V_OFF = 96, 120, 144
 ROW = 128           # bytes of a row of 64 k-values
@@ -68,8 +72,11 @@ class Shape:
         self.ta = 8 if self.turn_a else rb
         self.loads = self.ta + 8
         self.slab_a = 64 * TURNED if self.turn_a else 32 * rb * ROW
-        self.slab = self.slab_a + 256 * ROW
-        self.ring = 3 if 3 * self.slab <= LDS else 2
+        self.slab_b = 256 * ROW
+        # slabs of either operand in LDS
+        self.ring_a = 3 if 3 * (self.slab_a + self.slab_b) <= LDS else 2
+        self.ring_b = 3
+        assert self.ring_a * self.slab_a + self.ring_b * self.slab_b <= LDS
         self.a_reads, self.b_reads = 1 + self.turn_a, 1 + self.turn_b
         room = 8 * self.ahead - 8 * self.b_reads - self.ahead * self.a_reads
         self.tail = min(self.loads, room)  # loads requested right behind the barrier
@@ -88,6 +95,7 @@ class Emitter:
     def __init__(self):
         self.lines = []
         self.lds = []       # destinations of LDS reads in flight, oldest first
+        self.vm = []        # slabs of the loads in flight, oldest first
         self.content = {}   # register quad -> what was last read into it
 
     def emit(self, text):
@@ -113,30 +121,45 @@ class Emitter:
             self.emit(f"s_waitcnt lgkmcnt({left})")
 
 
-def request_head(e, sh, slot, first=False):
-    """what the loads of the next slab need: base, sizes (the last slab's, zero past it), m0"""
-    if not first:
-        e.emit(f"s_add_u32 s{RA}, s{RA}, s{S_STEPA}")
-        e.emit(f"s_addc_u32 s{RA + 1}, s{RA + 1}, 0")
-        e.emit(f"s_add_u32 s{RB}, s{RB}, s{S_STEPB}")
-        e.emit(f"s_addc_u32 s{RB + 1}, s{RB + 1}, 0")
-    e.emit(f"s_add_u32 s{S_REQ}, s{S_REQ}, 1")
-    e.emit(f"s_cmp_eq_u32 s{S_REQ}, s{S_N}")
-    e.emit(f"s_cselect_b32 s{RA + 2}, s{S_LASTA}, s{S_FULLA}")
-    e.emit(f"s_cselect_b32 s{RB + 2}, s{S_LASTB}, s{S_FULLB}")
-    e.emit(f"s_cmp_le_u32 s{S_REQ}, s{S_N}")
-    e.emit(f"s_cselect_b32 s{RA + 2}, s{RA + 2}, 0")
-    e.emit(f"s_cselect_b32 s{RB + 2}, s{RB + 2}, 0")
-    e.emit(f"s_mov_b32 m0, s{S_MA + slot}")
+def request_head(e, sh, group):
+    """what the loads of a group need, A of one slab and B of another: bases, sizes (the last slab's,
+    zero past it), m0"""
+    for res, req, last, full, step, slab in ((RA, S_REQA, S_LASTA, S_FULLA, S_STEPA, group + sh.ring_a),
+                                             (RB, S_REQB, S_LASTB, S_FULLB, S_STEPB, group + sh.ring_b)):
+        if slab < 0:
+            continue
+        if slab > 0:
+            e.emit(f"s_add_u32 s{res}, s{res}, s{step}")
+            e.emit(f"s_addc_u32 s{res + 1}, s{res + 1}, 0")
+        e.emit(f"s_add_u32 s{req}, s{req}, 1")
+        e.emit(f"s_cmp_eq_u32 s{req}, s{S_N}")
+        e.emit(f"s_cselect_b32 s{res + 2}, s{last}, s{full}")
+        e.emit(f"s_cmp_le_u32 s{req}, s{S_N}")
+        e.emit(f"s_cselect_b32 s{res + 2}, s{res + 2}, 0")
+    if group + sh.ring_a >= 0:
+        e.emit(f"s_mov_b32 m0, s{S_MA + (group + sh.ring_a) % sh.ring_a}")
+    else:
+        e.emit(f"s_mov_b32 m0, s{S_MB + (group + sh.ring_b) % sh.ring_b}")
 
 
-def request(e, sh, slot, t):
-    """load t of a slab; m0 is left ready for load t + 1 (an MFMA or a nop lies between)"""
-    e.emit(f"buffer_load_dwordx4 v{V_OFF + t}, {sq(RA if t < sh.ta else RB)}, 0 offen lds")
+def request(e, sh, group, t):
+    """load t of a group, A's and then B's; m0 is left ready for load t + 1 (an MFMA or a nop lies
+    between)"""
+    of_a = t < sh.ta
+    e.emit(f"buffer_load_dwordx4 v{V_OFF + t}, {sq(RA if of_a else RB)}, 0 offen lds")
+    e.vm.append(group + (sh.ring_a if of_a else sh.ring_b))
     if t == sh.ta - 1:
-        e.emit(f"s_mov_b32 m0, s{S_MB + slot}")
+        e.emit(f"s_mov_b32 m0, s{S_MB + (group + sh.ring_b) % sh.ring_b}")
     elif t < sh.loads - 1:
         e.emit("s_add_u32 m0, m0, 0x400")
+
+
+def wait_for_slab(e, slab):
+    """... to have landed (loads complete in order)"""
+    last = max([i for i, at in enumerate(e.vm) if at <= slab], default=-1)
+    e.vm = e.vm[last + 1:]
+    assert len(e.vm) < 64
+    return f"s_waitcnt vmcnt({len(e.vm)})"
 
 
 def assign(ops, n):
@@ -149,7 +172,7 @@ def assign(ops, n):
     return at
 
 
-def reads_of(sh, turned, addr, dst, slot, h, block, tag):
+def reads_of(turned, addr, dst, slot, h, block, tag):
     """the LDS reads of an operand, one or two functions"""
     if not turned:
         return [lambda e: e.read(dst, f"ds_read_b128 {q(dst)}, v{addr + 2 * slot + h} offset:{block * 16 * ROW}", tag)]
@@ -157,64 +180,64 @@ def reads_of(sh, turned, addr, dst, slot, h, block, tag):
                                        f"offset:{(32 * h + 4 * j) * TURNED}", tag) for j in range(2)]
 
 
-def read_a(sh, slot, h, i, tag):
-    return reads_of(sh, sh.turn_a, V_A, AOP(i), slot, h, i, ("a", tag, i))
+# `at` is the step: slab 2 at, or 2 at + 1, and its half
+def read_a(sh, at, i):
+    return reads_of(sh.turn_a, V_A, AOP(i), at // 2 % sh.ring_a, at % 2, i, ("a", at, i))
 
 
-def read_b(sh, slot, h, b, o, tag):
-    return reads_of(sh, sh.turn_b, V_B, BOP(b, o), slot, h, o, ("b", tag, o))
+def read_b(sh, at, o):
+    return reads_of(sh.turn_b, V_B, BOP(at & 1, o), at // 2 % sh.ring_b, at % 2, o, ("b", at, o))
 
 
-def next_operands(sh, slot, h, b, tag):
-    """the reads of the next step that an outer step issues, in order"""
-    ops = read_b(sh, slot, h, b, 0, tag) + read_a(sh, slot, h, 0, tag)
+def next_operands(sh, at):
+    """the reads of step `at` that the outer step before it issues, in order"""
+    ops = read_b(sh, at, 0) + read_a(sh, at, 0)
     for o in range(1, 8):
-        ops += read_b(sh, slot, h, b, o, tag)
+        ops += read_b(sh, at, o)
     for i in range(1, sh.ahead):
-        ops += read_a(sh, slot, h, i, tag)
+        ops += read_a(sh, at, i)
     return ops
 
 
-def step(e, sh, mfma, slot, h, b, carry, tag):
-    """one step; carry: (slot, first load) of a request that the step before left unfinished"""
+def step(e, sh, mfma, now, carry):
+    """one step; carry: (group, first load) of a request that the step before left unfinished"""
     rb, ahead = sh.rb, sh.ahead
-    outer = h == STEPS - 1
-    nslot, nh = ((slot + 1) % sh.ring, 0) if outer else (slot, h + 1)
     ops = []
     for i in range(rb - ahead):
-        ops += [(8 * i + x, fn) for x, fn in enumerate(read_a(sh, slot, h, i + ahead, tag))]
+        ops += [(8 * i + x, fn) for x, fn in enumerate(read_a(sh, now, i + ahead))]
     for x, t in enumerate(range(carry[1], sh.loads) if carry else ()):
         ops.append((2 + 4 * x, lambda e, t=t: request(e, sh, carry[0], t)))
     left = None
-    if outer:
-        bar = 8 * (rb - ahead)
+    if now % STEPS == STEPS - 1:
+        bar, slab = 8 * (rb - ahead), now // STEPS
 
         def barrier(e):
-            e.emit(f"s_waitcnt vmcnt({(sh.ring - 2) * sh.loads}) lgkmcnt(0)")
+            e.emit(wait_for_slab(e, slab + 1) + " lgkmcnt(0)")
             e.lds = []
             e.emit("s_barrier")
-            request_head(e, sh, slot)
+            request_head(e, sh, slab)
 
         ops.append((bar - 1, barrier))
         behind = []
-        reads = next_operands(sh, nslot, nh, b ^ 1, tag + 1)
-        loads = [lambda e, t=t: request(e, sh, slot, t) for t in range(sh.tail)]
+        reads = next_operands(sh, now + 1)
+        loads = [lambda e, t=t: request(e, sh, slab, t) for t in range(sh.tail)]
         while reads or loads:  # in turns, and what is left of either
             if reads:
                 behind.append(reads.pop(0))
             if loads:
                 behind.append(loads.pop(0))
         ops += [(bar + x * 1e-3, fn) for x, fn in enumerate(behind)]
-        left = (slot, sh.tail) if sh.tail < sh.loads else None
+        left = (slab, sh.tail) if sh.tail < sh.loads else None
     else:
         for i in range(ahead):
-            ops += [(8 * (rb - ahead + i) + x, fn) for x, fn in enumerate(read_a(sh, nslot, nh, i, tag + 1))]
+            ops += [(8 * (rb - ahead + i) + x, fn) for x, fn in enumerate(read_a(sh, now + 1, i))]
         for o in range(8):
-            ops += [(rb * o + 2 + x, fn) for x, fn in enumerate(read_b(sh, nslot, nh, b ^ 1, o, tag + 1))]
+            ops += [(rb * o + 2 + x, fn) for x, fn in enumerate(read_b(sh, now + 1, o))]
     at = assign(ops, 8 * rb)
+    b = now & 1
     for i in range(rb):
         for o in range(8):
-            e.need([(AOP(i), ("a", tag, i), sh.a_reads)] + ([(BOP(b, o), ("b", tag, o), sh.b_reads)] if i == 0 else []))
+            e.need([(AOP(i), ("a", now, i), sh.a_reads)] + ([(BOP(b, o), ("b", now, o), sh.b_reads)] if i == 0 else []))
             acc = 32 * i + 4 * o
             e.emit(f"{mfma} {aq(acc)}, {q(BOP(b, o))}, {q(AOP(i))}, {aq(acc)}")
             if 8 * i + o in at:
@@ -224,37 +247,48 @@ def step(e, sh, mfma, slot, h, b, carry, tag):
 
 def generate(sh, mfma):
     e = Emitter()
-    # prologue: both slots requested (the second as far as an outer step would have), the
+    # prologue: every slot requested (the last group as far as an outer step would have), the
     # accumulators zeroed, the first step's operands read
-    e.emit(f"s_mov_b32 s{S_REQ}, 0")
+    e.emit(f"s_mov_b32 s{S_REQA}, 0")
+    e.emit(f"s_mov_b32 s{S_REQB}, 0")
     e.emit(f"s_mov_b32 s{S_LEFT}, s{S_N}")
-    for s in range(1, sh.ring):
-        e.emit(f"s_add_u32 s{S_MA + s}, s{S_MA}, {s * sh.slab}")
-        e.emit(f"s_add_u32 s{S_MB + s}, s{S_MB}, {s * sh.slab}")
-    for s in range(sh.ring):
-        request_head(e, sh, s, s == 0)
-        for t in range(sh.loads if s < sh.ring - 1 else sh.tail):
-            e.emit("s_nop 0")
-            request(e, sh, s, t)
+    for s in range(1, sh.ring_a):
+        e.emit(f"s_add_u32 s{S_MA + s}, s{S_MA}, {s * sh.slab_a}")
+    for s in range(1, sh.ring_b):
+        e.emit(f"s_add_u32 s{S_MB + s}, s{S_MB}, {s * sh.slab_b}")
+    for group in range(-max(sh.ring_a, sh.ring_b), 0):
+        request_head(e, sh, group)
+        for t in range(sh.loads if group < -1 else sh.tail):
+            if group + (sh.ring_a if t < sh.ta else sh.ring_b) >= 0:
+                e.emit("s_nop 0")
+                request(e, sh, group, t)
     for n in range(32 * sh.rb):
         e.emit(f"v_accvgpr_write_b32 a{n}, 0")
-    e.emit(f"s_waitcnt vmcnt({(sh.ring - 2) * sh.loads + sh.tail})")
+    e.emit(wait_for_slab(e, 0))
     e.emit("s_barrier")
-    for fn in next_operands(sh, 0, 0, 0, 0):
+    for fn in next_operands(sh, 0):
         fn(e)
-    carry = (sh.ring - 1, sh.tail) if sh.tail < sh.loads else None
-    first_carry, start = carry, list(e.lds)
+    carry = (-1, sh.tail) if sh.tail < sh.loads else None
+    turn = math.lcm(sh.ring_a, sh.ring_b)  # slabs after which all slots come round
+
+    def state():
+        return ([(r, e.content[r]) for r in sorted(e.content)], list(e.lds), list(e.vm), carry)
+
+    start = state()
     e.emit(".Lff_loop_%=:")
-    tag = 0
-    for slot in range(sh.ring):
-        for h in range(STEPS):
-            carry = step(e, sh, mfma, slot, h, tag & 1, carry, tag)
-            tag += 1
-        e.emit(f"s_sub_u32 s{S_LEFT}, s{S_LEFT}, 1")
-        e.emit(f"s_cmp_eq_u32 s{S_LEFT}, 0")
-        e.emit("s_cbranch_scc0 .Lff_loop_%=" if slot == sh.ring - 1 else "s_cbranch_scc1 .Lff_done_%=")
-    # the loop closes: what is in flight and in the registers is what it started with
-    assert tag % 2 == 0 and e.lds == start and carry == first_carry, (e.lds, start)
+    for now in range(2 * turn):
+        carry = step(e, sh, mfma, now, carry)
+        if now % STEPS == STEPS - 1:
+            e.emit(f"s_sub_u32 s{S_LEFT}, s{S_LEFT}, 1")
+            e.emit(f"s_cmp_eq_u32 s{S_LEFT}, 0")
+            e.emit("s_cbranch_scc0 .Lff_loop_%=" if now == 2 * turn - 1 else "s_cbranch_scc1 .Lff_done_%=")
+    # the loop closes: what is in flight, and what is ready for the first step, is what it
+    # started with, `turn` slabs on
+    end = state()
+    assert end[1] == start[1] and end[2] == [at + turn for at in start[2]]
+    assert (end[3] and (end[3][0] - turn, end[3][1])) == start[3]
+    ready = [(r, [(c[0][0], c[0][1] - 2 * turn, c[0][2]), c[1]]) for r, c in end[0] if c[0][1] == 2 * turn]
+    assert ready == [(r, c) for r, c in start[0] if c[0][1] == 0]
     e.emit(".Lff_done_%=:")
     # the last MFMAs' results are not readable for 18 cycles, and the hardware does not
     # interlock that for what follows; nothing may be on its way into LDS or registers either
@@ -273,13 +307,13 @@ def statement(sh, mfma):
     ins = [f'"{{s{S_N}}}"(slabs)', f'"{{s{S_MA}}}"(lds_a)', f'"{{s{S_MB}}}"(lds_b)',
            f'"{{s{S_FULLA}}}"(full_a)', f'"{{s{S_FULLB}}}"(full_b)', f'"{{s{S_LASTA}}}"(last_a)',
            f'"{{s{S_LASTB}}}"(last_b)', f'"{{s{S_STEPA}}}"(step_a)', f'"{{s{S_STEPB}}}"(step_b)']
-    ins += [f'"{{v{V_A + j}}}"(a_rd[{j}])' for j in range((8 if sh.turn_a else 2) * sh.ring)]
-    ins += [f'"{{v{V_B + j}}}"(b_rd[{j}])' for j in range((8 if sh.turn_b else 2) * sh.ring)]
+    ins += [f'"{{v{V_A + j}}}"(a_rd[{j}])' for j in range((8 if sh.turn_a else 2) * sh.ring_a)]
+    ins += [f'"{{v{V_B + j}}}"(b_rd[{j}])' for j in range((8 if sh.turn_b else 2) * sh.ring_b)]
     ins += [f'"{{v{V_OFF + t}}}"(src[{t}])' for t in range(sh.loads)]
     out.append("    : " + ",\n      ".join(ins))
     clob = [f"v{n}" for n in range(64 + 4 * sh.rb)]
-    clob += [f"s{S_REQ}", f"s{S_LEFT}"]
-    clob += [f"s{S_MA + s}" for s in range(1, sh.ring)] + [f"s{S_MB + s}" for s in range(1, sh.ring)]
+    clob += [f"s{S_REQA}", f"s{S_REQB}", f"s{S_LEFT}"]
+    clob += [f"s{S_MA + s}" for s in range(1, sh.ring_a)] + [f"s{S_MB + s}" for s in range(1, sh.ring_b)]
     clob += ["scc", "memory"]  # (m0 is the compiler's to reserve; it keeps nothing there)
     out.append("    : " + ", ".join(f'"{c}"' for c in clob) + ");")
     return "\n".join(out) + "\n"
