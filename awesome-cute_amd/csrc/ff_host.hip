@@ -121,11 +121,32 @@ ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, bool pad
   }
   return best;
 }
-// bytes of partial sums that a problem's plan wants
-long long plan_bytes(int m, int n, int k, bool gated, Layout layout, bool padded, int cus) {
-  if (m == 0 || n == 0 || k == 0) return 0;
-  const ProductPlan p = choose_plan(m, n, k, gated, layout, padded, cus, 1LL << 40);
-  return p.slices > 1 ? 4LL * p.slices * m * product_columns(n, gated) : 0;
+// A thread's last plans with all the room they want: planning takes the host some 3 us, asked
+// for the room and again for the launch, and a model's layers are a few sizes over and over.
+struct Planned {
+  int m = 0, n = 0, k = 0, cus = 0, form = -1;
+  ProductPlan plan = {{0, 0}, 0};
+  long long bytes = 0;  // of partial sums
+};
+constexpr int kPlansKept = 16;
+thread_local Planned t_plans[kPlansKept];
+thread_local int t_oldest = 0;
+
+Planned plan_with_room(int m, int n, int k, bool gated, Layout layout, bool padded, int cus) {
+  const int form = (gated ? 1 : 0) | (padded ? 2 : 0) | (int)layout << 2;
+  const bool forced = t_tile.rows > 0 || t_slices > 0;
+  if (!forced)
+    for (const Planned& p : t_plans)
+      if (p.m == m && p.n == n && p.k == k && p.cus == cus && p.form == form) return p;
+  Planned p;
+  p.m = m, p.n = n, p.k = k, p.cus = cus, p.form = form;
+  p.plan = choose_plan(m, n, k, gated, layout, padded, cus, 1LL << 40);
+  p.bytes = p.plan.slices > 1 ? 4LL * p.plan.slices * m * product_columns(n, gated) : 0;
+  if (!forced) {
+    t_plans[t_oldest] = p;
+    t_oldest = (t_oldest + 1) % kPlansKept;
+  }
+  return p;
 }
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
@@ -165,7 +186,10 @@ int run_product(ProductArgs a, Layout layout, bool padded, bool bf, void* room, 
   if (room && off16(room)) return fail(FEEDFORWARD_ERR_SHAPE, "scratch must start on 16 bytes");
   return on_device(dev, [&](int cus) {
     if (layout == kRows && a.M <= kProductRows && t_tile.rows <= 0) return launch_product_rows(a, bf, stream);
-    const ProductPlan p = choose_plan(a.M, a.N, a.K, gated, layout, padded, cus, room ? room_bytes : 0);
+    const Planned planned = plan_with_room(a.M, a.N, a.K, gated, layout, padded, cus);
+    const long long have = room ? room_bytes : 0;
+    const ProductPlan p =
+        planned.bytes <= have ? planned.plan : choose_plan(a.M, a.N, a.K, gated, layout, padded, cus, have);
     a.slices = p.slices;
     a.part = p.slices > 1 ? (float*)room : nullptr;
     a.ldpart = (int)columns;
@@ -261,7 +285,7 @@ long long feedforward_product_bytes(int m, int n, int k, int gated, int turned, 
   if (check_sizes(m, n, k, FEEDFORWARD_FP16) != FEEDFORWARD_OK || !layout_of(turned, &layout, &padded)) return -1;
   if (layout == kRows && m <= kProductRows && t_tile.rows <= 0) return 0;
   const int cus = device_cus(dev);
-  return cus > 0 ? plan_bytes(m, n, k, gated != 0, layout, padded, cus) : 0;
+  return cus > 0 && m > 0 && n > 0 && k > 0 ? plan_with_room(m, n, k, gated != 0, layout, padded, cus).bytes : 0;
 }
 
 int feedforward_gated_grad(const void* dh, const float* pre, void* dgu, int m, int n, long long lddh, long long ldpre,
@@ -346,7 +370,7 @@ int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int* o
   bool padded;
   if (!layout_of(turned, &layout, &padded)) return fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
   if (layout == kRows && m <= kProductRows) return rc;
-  const ProductPlan p = choose_plan(m, n, k, gated != 0, layout, padded, cus, 1LL << 40);
+  const ProductPlan p = plan_with_room(m, n, k, gated != 0, layout, padded, cus).plan;
   out[0] = p.tile.rows;
   out[1] = p.tile.cols;
   out[2] = p.slices;

@@ -457,51 +457,60 @@ __global__ __launch_bounds__(64 * wg_waves(W)) void norm_grad_kernel(NormGradArg
   }
 }
 
-// The parts' sums added in their order: 16 columns a workgroup, 16 lanes a column, lane l taking
-// every 16th part.  q of a gate's parts gives its gradient and its share of dpost.
+// The parts' sums added in their order: 64 columns and 16 waves a workgroup, a wave every
+// sixteenth part.  y = 0: of dt bh, which for a gate's parts gives its gradient and its share of
+// dpost; there `wpg` waves share a gate (few gates), or a wave takes every sixteenth gate.
+// y = 1: of dy rh.
 template <class T>
-__global__ __launch_bounds__(256) void norm_sums_kernel(NormGradArgs p, NormParts parts) {
-  __shared__ float room[2][16][17];
-  const int x = threadIdx.x & 15, l = threadIdx.x >> 4;
-  const int c = 16 * blockIdx.x + x;
+__global__ __launch_bounds__(1024) void norm_sums_kernel(NormGradArgs p, NormParts parts, int wpg) {
+  __shared__ float room[16][64];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = 64 * blockIdx.x + lane;
   const bool in = c < p.d;
-  const float post = in && p.post ? (float)((const T*)p.post)[c] : 1.f;
-  float dpost = 0.f, dpre = 0.f;
-  const long long runs = parts.whole ? 1 : parts.gates;
-  const long long run = parts.whole ? parts.parts : parts.parts_per_gate;
-  for (long long g = 0; g < runs; g++) {
-    float a = 0.f, b = 0.f;
-    if (in)
-      for (long long i = l; i < run; i += 16) {
-        const float* const from = p.partials + (size_t)(g * run + i) * 2 * p.d + c;
-        a += from[0];
-        b += from[p.d];
+  const int at = in ? c : 0;
+  // the parts first, first + step ... < last
+  auto add = [&](long long first, long long last, long long step, const float* from) {
+    float s = 0.f;
+#pragma unroll 8
+    for (long long i = first; i < last; i += step) s += from[i * 2 * p.d];
+    return s;
+  };
+  if (blockIdx.y == 1) {
+    room[wave][lane] = add(wave, parts.parts, 16, p.partials + at);
+  } else if (parts.whole) {
+    room[wave][lane] = add(wave, parts.parts, 16, p.partials + p.d + at);
+  } else {
+    const float post = in && p.post ? (float)((const T*)p.post)[c] : 1.f;
+    const long long run = parts.parts_per_gate;
+    auto gate_of = [&](long long g) { return in && p.gate ? (float)((const T*)p.gate)[g * p.ld_gate + c] : 1.f; };
+    float dpost = 0.f;
+    if (wpg == 1) {
+      for (long long g = wave; g < parts.gates; g += 16) {
+        const float q = add(0, run, 1, p.partials + g * run * 2 * p.d + p.d + at);
+        if (in && p.dgate) ((T*)p.dgate)[g * p.d + c] = (T)(post * q);
+        dpost = __builtin_fmaf(gate_of(g), q, dpost);
       }
-    __syncthreads();
-    room[0][l][x] = a;
-    room[1][l][x] = b;
-    __syncthreads();
-    if (l == 0) {
-      a = b = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        a += room[0][i][x];
-        b += room[1][i][x];
+    } else {  // (16 / wpg sets of waves, no fewer than there are gates)
+      const long long g = wave / wpg;
+      room[wave][lane] = g < parts.gates ? add(wave % wpg, run, wpg, p.partials + g * run * 2 * p.d + p.d + at) : 0.f;
+      __syncthreads();
+      if (wave % wpg == 0 && g < parts.gates) {
+        float q = 0.f;
+        for (int i = 0; i < wpg; i++) q += room[wave + i][lane];
+        if (in && p.dgate) ((T*)p.dgate)[g * p.d + c] = (T)(post * q);
+        dpost = gate_of(g) * q;
       }
-      dpre += a;
-      if (parts.whole) {
-        dpost += b;
-      } else {
-        const float gate = in && p.gate ? (float)((const T*)p.gate)[(size_t)g * p.ld_gate + c] : 1.f;
-        dpost = __builtin_fmaf(gate, b, dpost);
-        if (in && p.dgate) ((T*)p.dgate)[(size_t)g * p.d + c] = (T)(post * b);
-      }
+      __syncthreads();
     }
+    room[wave][lane] = dpost;
   }
-  if (l == 0 && in) {
-    if (p.dpre) ((T*)p.dpre)[c] = (T)dpre;
-    if (p.dpost) ((T*)p.dpost)[c] = (T)dpost;
-  }
+  __syncthreads();
+  T* const out = (T*)(blockIdx.y == 1 ? p.dpre : p.dpost);
+  if (wave != 0 || !in || !out) return;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) s += room[i][lane];
+  out[c] = (T)s;
 }
 
 namespace {
@@ -626,8 +635,11 @@ void launch_norm_grad(const NormGradArgs& a, NormType type, hipStream_t stream) 
           hipLaunchKernelGGL((norm_grad_kernel<T, WHOLE, NV, W, kPartSums>), grid, block, 0, stream, a, parts);
       });
     });
-    if (a.partials)
-      hipLaunchKernelGGL(norm_sums_kernel<T>, dim3((a.d + 15) / 16), dim3(256), 0, stream, a, parts);
+    if (a.partials) {
+      int wpg = 16;  // waves that share a gate's parts
+      while (wpg > 1 && (long long)(16 / wpg) < parts.gates) wpg /= 2;
+      hipLaunchKernelGGL(norm_sums_kernel<T>, dim3((a.d + 63) / 64, a.dpre ? 2 : 1), dim3(1024), 0, stream, a, parts, wpg);
+    }
   });
 }
 
