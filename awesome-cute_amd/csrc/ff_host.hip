@@ -85,6 +85,18 @@ constexpr TileFit kFits[] = {
     {{96, 256}, 5.28, 0.594, 0.439, 4.03, 0.838}, {{128, 256}, 5.34, 0.748, 0.456, 4.59, 1.004},
     {{160, 256}, 7.68, 0.793, 0.380, 6.47, 1.094}, {{192, 256}, 8.23, 0.911, 0.424, 7.35, 1.256},
     {{224, 256}, 9.14, 1.044, 0.434, 8.56, 1.394}, {{256, 256}, 9.25, 1.104, 0.531, 9.57, 1.483}};
+// The same of the kernel for few rows (ff_rows.hip) by its blocks of sixteen rows of A, a stage
+// being the 64 k-values of one of its four waves: one block of product columns to a workgroup, or
+// two.  Fitted to 12000 problems of 1 to 64 rows, widths of 64 to 14336, depths of 64 to 8192,
+// weights from memory.  On 8000 others the choice among these and the tiles takes 1.06, 1.07, 1.05
+// and 1.03 of the best of 25 variants measured, 1.02 to 1.07 above 16 us, much of it the measurements'
+// scatter.  Without tiles it takes 1.06, 1.08, 1.09 and 1.11; one block alone 1.07, 1.07, 1.055,
+// 1.04; four blocks, or other depths, gain less than 0.003.
+constexpr TileFit kFewFits[] = {
+    {{16, 16}, 4.36, 0.128, 0.078, 0.0, 0.335},  {{16, 32}, 4.13, 0.264, 0.231, 0.0, 0.594},
+    {{32, 16}, 4.17, 0.270, 0.084, 0.0, 0.471},  {{32, 32}, 4.06, 0.381, 0.281, 0.0, 0.822},
+    {{48, 16}, 4.12, 0.376, 0.113, 0.09, 0.677}, {{48, 32}, 4.03, 0.518, 0.349, 0.35, 0.956},
+    {{64, 16}, 4.00, 0.491, 0.147, 0.24, 0.755}, {{64, 32}, 3.98, 0.648, 0.289, 1.59, 1.293}};
 // (the sums of slices written and read again, and the launch that adds them)
 constexpr int kSlicesMost = 8;
 constexpr double kSliceLaunch = 2.96, kSliceBytes = 0.327e-6;
@@ -100,24 +112,39 @@ bool tile_takes(const FfTile& t, int k, Layout layout, bool padded) {
   return layout != kTurnBoth || t.rows != 96;  // (64, 128 or 256 columns of a turned operand)
 }
 
+double fit_cost(const TileFit& f, long long groups, int stages, int cus) {
+  const double r = (double)groups / cus;
+  const int rounds = (int)((groups + cus - 1) / cus);
+  // workgroups beyond one per compute unit: half way between the rounds and their share of one
+  const double more = r > 1.0 ? 0.5 * (rounds + r) - 1.0 : 0.0;
+  return f.launch + stages * (f.stage + f.fill * (r < 1.0 ? r : 1.0)) + more * (f.more + f.more_stage * stages);
+}
+
 // room: bytes for partial sums
 ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, bool padded, int cus, long long room) {
   const int columns = product_columns(n, gated), stages = ceil_div(k, kDnStageK);
+  const bool few = layout == kRows && m <= kProductRows;
+  const bool forced = t_tile.rows > 0 && (few_tile(t_tile) ? few : tile_takes(t_tile, k, layout, padded));
   ProductPlan best = {{64, 64}, 1};
   double least = 0.0;
+  if (few)
+    for (const TileFit& f : kFewFits) {
+      if (f.tile.rows != ceil_div(m, 16) * 16 || (forced && f.tile.cols != t_tile.cols)) continue;
+      const double cost = fit_cost(f, ceil_div(n, gated ? f.tile.cols / 2 : f.tile.cols), ceil_div(stages, 4), cus);
+      if (least == 0.0 || cost < least) {
+        best = {f.tile, 1};
+        least = cost;
+      }
+    }
   for (const TileFit& f : kFits) {
-    if (t_tile.rows > 0 && tile_takes(t_tile, k, layout, padded) && (f.tile.rows != t_tile.rows || f.tile.cols != t_tile.cols)) continue;
+    if (forced && (f.tile.rows != t_tile.rows || f.tile.cols != t_tile.cols)) continue;
     if (!tile_takes(f.tile, k, layout, padded)) continue;
     const long long tiles = (long long)ceil_div(m, f.tile.rows) * ceil_div(columns, f.tile.cols);
     for (int slices = 1; slices <= kSlicesMost && slices <= stages; slices++) {
       const double bytes = 4.0 * slices * m * columns;
       if (slices > 1 && (bytes > (double)room || (t_slices == 0 && tiles * slices > 2 * cus))) break;
       if (t_slices > 0 && slices != t_slices && t_slices <= stages && 4.0 * t_slices * m * columns <= (double)room) continue;
-      const double r = (double)tiles * slices / cus;
-      const int rounds = (int)((tiles * slices + cus - 1) / cus), each = ceil_div(stages, slices);
-      // workgroups beyond one per compute unit: half way between the rounds and their share of one
-      const double more = r > 1.0 ? 0.5 * (rounds + r) - 1.0 : 0.0;
-      double cost = f.launch + each * (f.stage + f.fill * (r < 1.0 ? r : 1.0)) + more * (f.more + f.more_stage * each);
+      double cost = fit_cost(f, tiles * slices, ceil_div(stages, slices), cus);
       if (slices > 1) cost += kSliceLaunch + kSliceBytes * bytes;
       if (least == 0.0 || cost < least) {
         best = {f.tile, slices};
@@ -191,7 +218,6 @@ int run_product(ProductArgs a, Layout layout, bool padded, bool bf, void* room, 
     return fail(FEEDFORWARD_ERR_SHAPE, "weights of more than 2 GiB (n = %d, rows of %d): split the call", a.N, a.ldb);
   if (room && off16(room)) return fail(FEEDFORWARD_ERR_SHAPE, "scratch must start on 16 bytes");
   return on_device(dev, [&](int cus) {
-    if (layout == kRows && a.M <= kProductRows && t_tile.rows <= 0) return launch_product_rows(a, bf, stream);
     const Planned planned = plan_with_room(a.M, a.N, a.K, gated, layout, padded, cus);
     const long long have = room ? room_bytes : 0;
     const ProductPlan p =
@@ -199,7 +225,9 @@ int run_product(ProductArgs a, Layout layout, bool padded, bool bf, void* room, 
     a.slices = p.slices;
     a.part = p.slices > 1 ? (float*)room : nullptr;
     a.ldpart = (int)columns;
-    if (big_tile(p.tile))
+    if (few_tile(p.tile))
+      launch_product_rows(a, p.tile.cols / 16, bf, stream);
+    else if (big_tile(p.tile))
       launch_product_big(a, p.tile.rows, layout, bf, stream);
     else
       launch_product_tiles(a, p.tile, layout, bf, stream);
@@ -289,7 +317,6 @@ long long feedforward_product_bytes(int m, int n, int k, int gated, int turned, 
   Layout layout;
   bool padded;
   if (check_sizes(m, n, k, FEEDFORWARD_FP16) != FEEDFORWARD_OK || !layout_of(turned, &layout, &padded)) return -1;
-  if (layout == kRows && m <= kProductRows && t_tile.rows <= 0) return 0;
   const int cus = device_cus(dev);
   return cus > 0 && m > 0 && n > 0 && k > 0 ? plan_with_room(m, n, k, gated != 0, layout, padded, cus).bytes : 0;
 }
@@ -375,7 +402,6 @@ int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int* o
   Layout layout;
   bool padded;
   if (!layout_of(turned, &layout, &padded)) return fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
-  if (layout == kRows && m <= kProductRows) return rc;
   const ProductPlan p = plan_with_room(m, n, k, gated != 0, layout, padded, cus).plan;
   out[0] = p.tile.rows;
   out[1] = p.tile.cols;
@@ -387,6 +413,8 @@ void feedforward_force_tile(int rows, int cols, int slices) {
   t_tile = {0, 0};
   t_slices = slices > kSlicesMost ? kSlicesMost : slices < 0 ? 0 : slices;
   for (const TileFit& f : kFits)
+    if (f.tile.rows == rows && f.tile.cols == cols) t_tile = f.tile;
+  for (const TileFit& f : kFewFits)
     if (f.tile.rows == rows && f.tile.cols == cols) t_tile = f.tile;
 }
 

@@ -72,19 +72,21 @@ __host__ __device__ __forceinline__ int pre_col(int col) { return ((col >> 4) <<
 __host__ __device__ __forceinline__ int product_columns(int n, bool gated) { return gated ? (n + 15) / 16 * 32 : n; }
 
 // Tiles: rows x columns of the product.  256 columns and 160, 192, 224 or 256 rows are
-// ff_big.hip's, the others ff_tiles.hip's.
+// ff_big.hip's, 16 and 32 columns, of up to kProductRows rows, ff_rows.hip's, the others
+// ff_tiles.hip's.
 struct FfTile {
   int rows, cols;
 };
+constexpr int kProductRows = 64;
 inline bool big_tile(const FfTile& t) { return t.cols == 256 && t.rows >= 160; }
+inline bool few_tile(const FfTile& t) { return t.cols <= 32; }
 hipError_t configure_product_tiles();
 hipError_t configure_product_big();
 hipError_t configure_product_rows();
 // launches of any kind; bf: bfloat16 operands
 void launch_product_tiles(ProductArgs a, const FfTile& t, Layout layout, bool bf, hipStream_t stream);
 void launch_product_big(ProductArgs a, int rows, Layout layout, bool bf, hipStream_t stream);
-void launch_product_rows(const ProductArgs& a, bool bf, hipStream_t stream);
+void launch_product_rows(const ProductArgs& a, int blocks, bool bf, hipStream_t stream);  // of 16 columns
 void launch_sum_parts(const ProductArgs& a, bool bf, hipStream_t stream);
-constexpr int kProductRows = 64;  // rows of A that launch_product_rows takes at most
 
 }  // namespace w4a16

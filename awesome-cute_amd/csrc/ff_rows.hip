@@ -3,8 +3,8 @@
 //
 // A workgroup owns S blocks of 16 rows of B over the whole k range -- gated, of eight gates and
 // their eight ups, so that eight columns of C are whole in it -- and all rows of A: no
-// partial sums in memory, nothing exchanged between workgroups.  Its eight waves take every
-// eighth 64-deep chunk of k by themselves, each with a ring of LDS slots of its own (no barrier
+// partial sums in memory, nothing exchanged between workgroups.  Its four waves take every
+// fourth 64-deep chunk of k by themselves, each with a ring of LDS slots of its own (no barrier
 // in the loop), and their sums meet in LDS once, at the end.
 //
 // Weights and activations go straight into LDS, eight rows of 128 bytes per instruction, whole
@@ -21,15 +21,15 @@ namespace w4a16 {
 
 namespace {
 
-constexpr int kWaves = 8;
+constexpr int kFewWaves = 4;
 
 template <int S, int MB, int DEPTH>
 struct FewShape {
   static constexpr int kLoads = 2 * (S + MB);  // of 1 KiB per wave and chunk
   static constexpr int kSlot = 1024 * kLoads;
   static constexpr int kOps = 2 * (S + MB);
-  static constexpr int kRing = kWaves * DEPTH * kSlot;
-  static constexpr int kReduce = kWaves * S * MB * 1024;
+  static constexpr int kRing = kFewWaves * DEPTH * kSlot;
+  static constexpr int kReduce = kFewWaves * S * MB * 1024;
   static constexpr int kLds = kRing > kReduce ? kRing : kReduce;
   static_assert(kLds <= 160 * 1024, "LDS of a compute unit");
 };
@@ -45,7 +45,7 @@ __device__ __forceinline__ void few_read(unsigned at, i4* v) {
 }  // namespace
 
 template <bool BF, bool GATED, int S, int MB, int DEPTH>
-__global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(ProductArgs p) {
+__global__ __launch_bounds__(64 * kFewWaves) void product_rows_kernel(ProductArgs p) {
   using Sh = FewShape<S, MB, DEPTH>;
   constexpr int kCols = GATED ? 8 : 16;  // columns of C per block
   extern __shared__ __attribute__((aligned(16))) char smem[];  // Sh::kLds
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(ProductArgs p
   const int last = p.N - 1;
 
   const int chunks = (p.K + 63) / 64;
-  const int mine = (chunks - wave + kWaves - 1) / kWaves;
+  const int mine = (chunks - wave + kFewWaves - 1) / kFewWaves;
   const __amdgpu_buffer_rsrc_t rA =
       make_rsrc(p.A, (unsigned)(p.M - 1) * (unsigned)p.lda * 2u + (unsigned)p.K * 2u);
   const int b_rows = min(S * kCols, p.N - col0) + (GATED ? p.N : 0);  // from my first row to my last
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(ProductArgs p
   char* const stage = smem + wave * (DEPTH * Sh::kSlot);
   // my i-th chunk
   auto issue = [&](int i, int slot) {
-    const int c = wave + kWaves * i;
+    const int c = wave + kFewWaves * i;
     const int inv = i >= mine ? kOob : c == chunks - 1 ? past : 0;
     char* const base = stage + slot * Sh::kSlot;
     __builtin_amdgcn_sched_barrier(0);
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(ProductArgs p
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
 
-  // ---- sum the eight waves, a block of 16 product columns x 16 rows to a wave.  A lane holds
+  // ---- sum the waves, a block of 16 product columns x 16 rows to a wave.  A lane holds
   // columns 4 kg ... 4 kg + 3 of row nu; gated, lanes 32 apart a gate and its partner.
   f4* const red = (f4*)smem;
 #pragma unroll
@@ -143,10 +143,10 @@ __global__ __launch_bounds__(64 * kWaves) void product_rows_kernel(ProductArgs p
 #pragma unroll
     for (int m = 0; m < MB; m++) red[((wave * S + s) * MB + m) * 64 + lane] = acc[s][m];
   __syncthreads();
-  for (int b = wave; b < S * MB; b += kWaves) {
+  for (int b = wave; b < S * MB; b += kFewWaves) {
     f4 v = red[b * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) v += red[(w * S * MB + b) * 64 + lane];
+    for (int w = 1; w < kFewWaves; w++) v += red[(w * S * MB + b) * 64 + lane];
     const int row = 16 * (b % MB) + nu;
     const int col = col0 + kCols * (b / MB) + 4 * (GATED ? kg & 1 : kg);
     f4 up = v;
@@ -178,16 +178,14 @@ void with_rows(int s, int mb, bool bf, bool gated, F f) {
     return f(gated ? product_rows_kernel<false, true, S, MB, DEPTH>                   \
                    : product_rows_kernel<false, false, S, MB, DEPTH>, lds);           \
   }
-  FF_ROWS(1, 1, 4)
-  FF_ROWS(2, 1, 3)
-  FF_ROWS(1, 2, 3)
+  FF_ROWS(1, 1, 3)
+  FF_ROWS(2, 1, 2)
+  FF_ROWS(1, 2, 2)
   FF_ROWS(2, 2, 2)
   FF_ROWS(1, 3, 2)
-  FF_ROWS(2, 3, 1)
-  FF_ROWS(4, 3, 1)
-  FF_ROWS(1, 4, 1)
-  FF_ROWS(2, 4, 1)
-  FF_ROWS(4, 4, 1)
+  FF_ROWS(2, 3, 2)
+  FF_ROWS(1, 4, 2)
+  FF_ROWS(2, 4, 2)
 #undef FF_ROWS
 }
 
@@ -195,7 +193,7 @@ void with_rows(int s, int mb, bool bf, bool gated, F f) {
 
 hipError_t configure_product_rows() {
   hipError_t e = hipSuccess;
-  for (const int s : {1, 2, 4})
+  for (const int s : {1, 2})
     for (const int mb : {1, 2, 3, 4})
       for (const bool bf : {false, true})
         for (const bool gated : {false, true})
@@ -206,14 +204,12 @@ hipError_t configure_product_rows() {
   return e;
 }
 
-void launch_product_rows(const ProductArgs& a, bool bf, hipStream_t stream) {
+void launch_product_rows(const ProductArgs& a, int blocks, bool bf, hipStream_t stream) {
   const bool gated = a.act != kActNone;
-  const int blocks = ceil_div(a.N, gated ? 8 : 16), mb = ceil_div(a.M, 16);
-  int s = mb >= 3 && blocks >= 4 * 256 ? 4 : blocks >= 2 * 256 ? 2 : 1;
   ProductArgs b = a;
-  b.tiles_n = ceil_div(blocks, s);
-  with_rows(s, mb, bf, gated, [&](auto kernel, int lds) {
-    hipLaunchKernelGGL(kernel, dim3(b.tiles_n), dim3(64 * kWaves), lds, stream, b);
+  b.tiles_n = ceil_div(a.N, (gated ? 8 : 16) * blocks);
+  with_rows(blocks, ceil_div(a.M, 16), bf, gated, [&](auto kernel, int lds) {
+    hipLaunchKernelGGL(kernel, dim3(b.tiles_n), dim3(64 * kFewWaves), lds, stream, b);
   });
 }
 

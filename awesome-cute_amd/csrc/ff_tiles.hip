@@ -1,5 +1,5 @@
-// Dense products in fp16 or bfloat16 by tiles, with a gated epilogue: more than kProductRows
-// rows, and what ff_rows.hip does not take.  Slabs, swizzle, order of MFMA operands and the
+// Dense products in fp16 or bfloat16 by tiles, with a gated epilogue: what
+// ff_rows.hip and ff_big.hip do not compute.  Slabs, swizzle, order of MFMA operands and the
 // loop are those of f16_tiles.hip, where they are explained and measured; here
 //   - rows of A, B and C may lie further apart than they are long,
 //   - C may have any number of columns that is a multiple of 8, and k any such depth: what is

@@ -205,7 +205,8 @@ _linear_op.register_autograd(_linear_backward, setup_context=_keep_linear)
 
 def product_plan(m, n, k, gated=False, turned=0, cus=256):
     """(rows, columns, slices of k) of the tiles that compute `linear` or `gated` -- turned = 1: the
-    gradient of their inputs, m rows of n over k; 2: that of their weights --, or None for few rows."""
+    gradient of their inputs, m rows of n over k; 2: that of their weights --, or None for empty ones.
+    16 or 32 columns: all of up to 64 rows by workgroups of whole columns."""
     out = (ctypes.c_int * 3)()
     if _lib.feedforward_plan(m, n, k, int(gated), turned, cus, out) != 0:
         raise ValueError(_lib.feedforward_last_error().decode())

@@ -89,8 +89,8 @@ int feedforward_gated_grad(const void *dh, const float *pre, void *dgu, int m, i
                            int activation, int dev, void *stream);
 
 /* out[0..2] = rows and columns of the product's tiles and the slices of k, with room for them, on
- * a device of `cus` compute units; zeros where up to 64 rows are computed by blocks of columns; no
- * GPU touched */
+ * a device of `cus` compute units (16 or 32 columns: all of up to 64 rows by workgroups of whole
+ * columns); no GPU touched */
 int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int *out);
 /* such tiles (0 = by cost) and slices (0 = by cost) for every product of the calling thread that
  * they can compute; for tests and tools */

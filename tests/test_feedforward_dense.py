@@ -169,6 +169,8 @@ def test_codes_of_the_gradients():
 
 TILES = [(64, 64), (64, 128), (96, 128), (128, 128), (96, 256), (128, 256), (160, 256), (192, 256), (224, 256), (256, 256)]
 
+FEW = [(rows, cols) for rows in (16, 32, 48, 64) for cols in (16, 32)]
+
 
 def test_plans_are_tiles_that_can_compute_the_problem():
     seen = set()
@@ -180,16 +182,18 @@ def test_plans_are_tiles_that_can_compute_the_problem():
             if turned == 2:
                 m, k = 8 * max(1, m // 8), m
             t = streamk.product_plan(m, n, k, gated, turned)
-            assert (t is None) == (m <= 64 and turned == 0)
-            if t:
-                rows, cols, slices = t
+            rows, cols, slices = t
+            if cols <= 32:  # whole columns of all rows
+                assert turned == 0 and m <= 64 and rows == -(-m // 16) * 16 and slices == 1
+                seen.add(((rows, cols), 1))
+            else:
                 assert (rows, cols) in TILES and 1 <= slices <= min(8, -(-k // 64))
                 assert k % 64 == 0 or turned in (2, 5) or rows < 160
                 assert rows != 96 or turned != 2
                 seen.add(((rows, cols), min(slices, 2)))
             if turned == 2:
                 m, k = k, m
-    assert {t for t, _ in seen} == set(TILES)  # none that nothing reaches
+    assert {t for t, _ in seen} == set(TILES + FEW)  # none that nothing reaches
 
 
 # --- on the GPU ----------------------------------------------------------------------------
@@ -236,12 +240,26 @@ def test_every_tile(tile, m, n, k, slices):
 
 
 @gpu
+@pytest.mark.parametrize("cols", [16, 32])
+@pytest.mark.parametrize("m,n,k", FORWARD[:10])
+def test_whole_columns_of_few_rows(m, n, k, cols):
+    try:
+        streamk.force_product_tile(16, cols)
+        for type in TYPES:
+            x, w, _ = make(m, n, k, type, m + n)
+            Gated64(x, w, "silu").check_forward(streamk.gated(x, w), type)
+            check_product(streamk.linear(x, w), x, w, type)
+    finally:
+        streamk.force_product_tile(0)
+
+
+@gpu
 @pytest.mark.parametrize("turned", [0, 1, 2, 5])
 def test_layouts_beside_rows_that_hold_nan(turned):
     """Matrices inside larger ones: what lies beside them, and behind their last row, is NaN."""
     import ctypes
     lib, L, P = streamk._lib, ctypes.c_longlong, ctypes.c_void_p
-    for tile in (0, (64, 64), (128, 128), (128, 256), (160, 256), (256, 256)):
+    for tile in (0, (16, 16), (16, 32), (64, 64), (128, 128), (128, 256), (160, 256), (256, 256)):
         for m, n, k in ((72, 200, 136), (328, 264, 320), (64, 24, 56)):
             gen = torch.Generator(device="cuda").manual_seed(m)
             a, b = (torch.randn(r, k, device="cuda", generator=gen).half() for r in (m, n))
