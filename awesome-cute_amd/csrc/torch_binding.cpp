@@ -316,14 +316,16 @@ PyObject* py_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // allocator on the current stream and go back to it in that stream's order.  The autograd functions
 // are C++ as well: as Python's they took the host 50 us more a pass than the kernels of a small one.
 
-// a matrix as the kernels address it: rows that start on 16 bytes
+// a matrix as the kernels address it: rows that start on 16 bytes, at most kFarthest elements apart
+constexpr int64_t kFarthest = 1 << 21;
 struct Matrix {
   at::Tensor t;
   long long ld = 0;
   Matrix() = default;
   explicit Matrix(const at::Tensor& x) : t(x) {
     const bool one = x.size(0) <= 1;
-    if (x.numel() != 0 && ((x.size(1) > 1 && x.stride(1) != 1) || (!one && (x.stride(0) % 8 != 0 || x.stride(0) < x.size(1))) ||
+    const bool apart = !one && (x.stride(0) % 8 != 0 || x.stride(0) < x.size(1) || x.stride(0) > kFarthest);
+    if (x.numel() != 0 && ((x.size(1) > 1 && x.stride(1) != 1) || apart ||
                            (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) != 0)) {
       t = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
       t.copy_(x);
@@ -782,7 +784,10 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     NormInputs in{residual, block.value_or(at::Tensor()), post.value_or(at::Tensor()), gate.value_or(at::Tensor()),
                   pre.value_or(at::Tensor())};
     const NormOutputs out = norm_forward(in, scale, eps, true);
-    ctx->save_for_backward({residual, out.r, in.block, in.post, in.gate, in.pre, out.lengths});
+    // (with a block the backward pass takes r, and of the residual, where that is a leaf, no values:
+    // it may be overwritten, and its memory go)
+    ctx->save_for_backward({in.block.defined() ? out.r : residual, in.block, in.post, in.gate, in.pre, out.lengths});
+    if (residual.is_leaf() && residual.requires_grad()) ctx->saved_data["leaf"] = residual;
     // (without a block the residual itself is what the norm took, and it is not multiplied)
     ctx->saved_data["scale"] = in.block.defined() ? scale : 1.0;
     ctx->set_materialize_grads(false);
@@ -793,18 +798,19 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &residual = saved[0], &r = saved[1];
-    NormInputs in{r.defined() ? r : residual, saved[2], saved[3], saved[4], saved[5]};
+    NormInputs in{saved[0], saved[1], saved[2], saved[3], saved[4]};
     const bool norm = in.pre.defined();
-    const at::Tensor dy = norm ? grads[0] : at::Tensor(), dr = r.defined() ? grads[norm ? 1 : 0] : at::Tensor();
+    const at::Tensor dy = norm ? grads[0] : at::Tensor(), dr = in.block.defined() ? grads[norm ? 1 : 0] : at::Tensor();
+    const auto leaf = ctx->saved_data.find("leaf");
     std::array<bool, 5> want;
     // (the context counts the inputs that are there)
-    const at::Tensor* const inputs[5] = {&residual, &in.block, &in.post, &in.gate, &in.pre};
+    const at::Tensor* const inputs[5] = {&in.residual, &in.block, &in.post, &in.gate, &in.pre};
     for (int i = 0, at = 0; i < 5; i++) want[i] = inputs[i]->defined() && ctx->needs_input_grad(at++);
     variable_list out(7);
     {
       c10::AutoGradMode off(false);
-      auto g = norm_backward(dy, dr, in, saved[6], ctx->saved_data["scale"].toDouble(), residual, want);
+      auto g = norm_backward(dy, dr, in, saved[5], ctx->saved_data["scale"].toDouble(),
+                             leaf != ctx->saved_data.end() ? leaf->second.toTensor() : at::Tensor(), want);
       for (int i = 0; i < 5; i++) out[i] = g[i];
     }
     return once_differentiable(std::move(out), "residual_norm");

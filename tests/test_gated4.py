@@ -142,7 +142,7 @@ def test_matches_the_definition(m, n, k, group):
                                    ("tile", 80), ("tile", 96), ("tile", 112), ("tile", 128)])
 @pytest.mark.parametrize("group", [128, -1])
 def test_every_kernel(force, group):
-    m, n, k = 50, 512, 5120  # (from 3072 and 5120 on eight strips take their deep loop)
+    m, n, k = 50, 512, 5120  #
     x, q, s, fake = problem(m, n, k, group, seed=3, dev="cuda")
     layer = layer_of(q, s, fake, group, "silu")
     kind, value = force

@@ -352,6 +352,45 @@ def test_strides_alignment_and_shapes(type):
 
 
 @gpu
+def test_a_residual_that_is_overwritten_before_the_backward_pass():
+    """r is what the gradients are made from: the residual itself may go."""
+    t, dy, dr = make((2, 5, 72), torch.bfloat16, "channel", 8)
+    v = leaves(t)
+    want = grads_of(v, run(v), (dy, dr))
+    v = leaves(t)
+    residual = v["residual"] * 1
+    out = run({**v, "residual": residual})
+    with torch.no_grad():
+        residual.fill_(float("nan"))
+    got = grads_of(v, out, (dy, dr))
+    assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    rows, d = 265000, 8192
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    v = {k: torch.empty(rows, d, dtype=torch.float16, device="cuda").normal_(generator=gen) for k in ("residual", "block")}
+    assert v["block"].numel() > 1 << 31
+    w = {k: torch.rand(d, device="cuda", generator=gen).half() for k in ("post_weight", "pre_weight")}
+    last = slice(rows - 20, rows)
+    dy = torch.zeros_like(v["block"])
+    dy[last].normal_(generator=gen)
+    small = {k: x[last].clone() for k, x in v.items()}
+    got, want = [], []
+    for inputs, grad, out in ((v, dy, got), (small, dy[last].clone(), want)):
+        a = {k: x.detach().requires_grad_() for k, x in {**inputs, **w}.items()}
+        y, r = residual_norm(a["residual"], a["block"], post_weight=a["post_weight"], pre_weight=a["pre_weight"])
+        out += [y.detach(), r.detach()] + list(torch.autograd.grad((y, r), list(a.values()), (grad, grad)))
+    for i, (a, b) in enumerate(zip(got, want)):
+        if a.dim() == 2:
+            assert torch.equal(a[last], b), i
+        else:  # twenty terms of about one each, added in fp32 in two orders, each sum rounded once
+            assert ((a.double() - b.double()).abs() <= half_step(torch.float16) * 2.01 * b.double().abs().clamp_min(0.1)).all()
+    assert not got[2][:rows - 20].any() and not got[3][:rows - 20].any()
+
+
+@gpu
 def test_no_rows():
     t, dy, dr = make((2, 0, 64), torch.float16, "sequence", 3)
     v = leaves(t)
