@@ -211,11 +211,12 @@ int run_product(ProductArgs a, Layout layout, bool padded, bool bf, void* room, 
   const bool gated = a.act != kActNone;
   const long long columns = product_columns(a.N, gated);
   // (a launch's grid, at the smallest tiles)
-  if (columns > 0x3fffffffLL || (columns / 64 + 1) * (a.M / 64 + 1LL) > 0x3fffffffLL / kSlicesMost)
+  if (a.M > 0x7ffffe00 || columns > 0x3fffffffLL || (columns / 64 + 1) * (a.M / 64 + 1LL) > 0x3fffffffLL / kSlicesMost)
     return fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many tiles", a.M, a.N);
   // a gated product's rows of either half are addressed from one place
   if (gated && 2LL * a.N * a.ldb * 2 > 0x7fffffffLL)
     return fail(FEEDFORWARD_ERR_SHAPE, "weights of more than 2 GiB (n = %d, rows of %d): split the call", a.N, a.ldb);
+  if (!a.A || !a.B || !a.C) return fail(FEEDFORWARD_ERR_SHAPE, "a matrix is missing");
   if (room && off16(room)) return fail(FEEDFORWARD_ERR_SHAPE, "scratch must start on 16 bytes");
   return on_device(dev, [&](int cus) {
     const Planned planned = plan_with_room(a.M, a.N, a.K, gated, layout, padded, cus);
@@ -332,6 +333,7 @@ int feedforward_gated_grad(const void* dh, const float* pre, void* dgu, int m, i
   if (rc == FEEDFORWARD_OK && (long long)m * (n / 8 + 8) > 0x7fffffffLL * 128)
     rc = fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many", m, n);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
+  if (!dh || !pre || !dgu) return fail(FEEDFORWARD_ERR_SHAPE, "a matrix is missing");
   const GatedGradArgs a = {dh, pre, dgu, lddh, ldpre, lddgu, m, n, activation};
   return on_device(dev, [&](int) { launch_gated_grad(a, type == FEEDFORWARD_BF16, (hipStream_t)stream); });
 }

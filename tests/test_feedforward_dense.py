@@ -167,6 +167,22 @@ def test_codes_of_the_gradients():
     assert rc == 1 and b"2 GiB" in lib.feedforward_last_error()
 
 
+def test_codes_of_missing_matrices_and_too_many_rows():
+    import ctypes
+    lib, L, P = streamk._lib, ctypes.c_longlong, ctypes.c_void_p
+
+    def product(a, b, c, m=4):
+        return lib.feedforward_product(a, b, c, m, 8, 8, L(8), L(8), L(8), 0, 0, None, L(0), 0, None)
+
+    there = P(16)
+    for t in ((None, there, there), (there, None, there), (there, there, None)):
+        assert product(*t) == 1 and b"missing" in lib.feedforward_last_error()
+    assert product(there, there, there, 0x7fffffff) == 1 and b"too many" in lib.feedforward_last_error()
+    for t in ((None, there, there), (there, None, there), (there, there, None)):
+        assert lib.feedforward_gated_grad(*t, 4, 16, L(16), L(32), L(64), 0, 1, 0, None) == 1
+        assert b"missing" in lib.feedforward_last_error()
+
+
 TILES = [(64, 64), (64, 128), (96, 128), (128, 128), (96, 256), (128, 256), (160, 256), (192, 256), (224, 256), (256, 256)]
 
 FEW = [(rows, cols) for rows in (16, 32, 48, 64) for cols in (16, 32)]
@@ -382,6 +398,39 @@ def test_strides_alignment_and_shapes(m):
     one = torch.autograd.grad(streamk.gated(x, w).float().sum(), (x, w))
     ones = torch.autograd.grad(streamk.gated(x, w), (x, w), torch.ones((m, n), dtype=torch.float16, device="cuda"))
     assert all(torch.equal(a, b) for a, b in zip(one, ones))
+
+
+@gpu
+def test_rows_further_apart_than_the_kernels_address():
+    x, w, _ = make(3, 16, 64, torch.float16, 4)
+    room = torch.zeros(3, (1 << 21) + 8, dtype=torch.float16, device="cuda")
+    room[:, :64] = x
+    assert torch.equal(streamk.linear(room[:, :64], w), streamk.linear(x, w))
+    assert torch.equal(streamk.gated(room[:, :64], w), streamk.gated(x, w))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements of x, of both sums and of their gradients; the last rows and the sums
+    over all of them."""
+    m, n, k = 1050000, 1024, 2064
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(m, k, dtype=torch.bfloat16, device="cuda")
+    assert x.numel() > 1 << 31 and 2 * n * m > 1 << 31
+    x.normal_(generator=gen)
+    w = torch.randn(2 * n, k, device="cuda", generator=gen).mul_(k ** -0.5).bfloat16()
+    dh = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    last = slice(m - 300, m)
+    dh[last].normal_(generator=gen)
+    x.requires_grad_()
+    w.requires_grad_()
+    h = streamk.gated(x, w)
+    ref = Gated64(x.detach()[last], w.detach(), "silu")
+    ref.check_forward(h.detach()[last], torch.bfloat16)
+    dx, dw = torch.autograd.grad(h, (x, w), dh)
+    # (only the last rows have a gradient: the others add exact zeros to that of w)
+    ref.check_grads(dh[last], dx[last], dw, torch.bfloat16)
+    assert not dx[:m - 300].any()
 
 
 @gpu
