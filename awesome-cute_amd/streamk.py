@@ -124,7 +124,9 @@ def gated(x, weight, activation="silu"):
     the current stream of x's device."""
     act = _activation(activation)
     if torch.compiler.is_compiling():
-        return torch.ops.marlin_amd.gated_dense(x, weight, act)[0]
+        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+            return torch.ops.marlin_amd.gated_dense(x, weight, act)[0]
+        return torch.ops.marlin_amd.gated_alone(x, weight, act)
     return _torch_binding.gated_dense(x, weight, act)
 
 
@@ -146,6 +148,18 @@ def _gated_fake(x, weight, act):
     n = weight.shape[0] // 2
     return (x.new_empty(x.shape[:-1] + (n,)),
             x.new_empty((x.numel() // x.shape[-1], -(-n // 16) * 32), dtype=torch.float32))
+
+
+# ... without gradients, and so without the sums
+@torch.library.custom_op("marlin_amd::gated_alone", mutates_args=())
+def _gated_alone_op(x: torch.Tensor, weight: torch.Tensor, act: int) -> torch.Tensor:
+    with torch.no_grad():
+        return _torch_binding.gated_dense(x, weight, act)
+
+
+@_gated_alone_op.register_fake
+def _gated_alone_fake(x, weight, act):
+    return x.new_empty(x.shape[:-1] + (weight.shape[0] // 2,))
 
 
 @torch.library.custom_op("marlin_amd::gated_grads", mutates_args=())

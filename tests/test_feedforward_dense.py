@@ -585,3 +585,20 @@ def test_under_a_compiler():
     got = torch.autograd.grad(compiled(*leaves)[0], leaves, dh)
     want = torch.autograd.grad(loss(*leaves)[0], leaves, dh)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        for got, want in zip(compiled(*leaves), loss(*leaves)):
+            assert torch.equal(got, want)
+    plain = [t.detach() for t in leaves]
+    for got, want in zip(compiled(*plain), loss(*plain)):
+        assert torch.equal(got, want) and not got.requires_grad
+    # the sums are kept for gradients alone
+    names = []
+
+    def record(graph, example):
+        names.append([str(node.target) for node in graph.graph.nodes])
+        return graph.forward
+
+    torch.compile(loss, backend=record, fullgraph=True)(*plain)
+    torch.compile(lambda a, b: streamk.gated(a, b), backend=record, fullgraph=True)(*leaves)
+    assert any("gated_alone" in n for n in names[0]) and not any("gated_dense" in n for n in names[0])
+    assert any("gated_dense" in n for n in names[1])
