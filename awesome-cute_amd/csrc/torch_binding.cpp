@@ -321,9 +321,16 @@ constexpr int64_t kFarthest = 1 << 21;
 struct Matrix {
   at::Tensor t;
   long long ld = 0;
-  Matrix() = default;
-  explicit Matrix(const at::Tensor& x) : t(x) {
-    const bool one = x.size(0) <= 1;
+  // y as `rows` rows of `width`.  (One that is whole is taken without a view: views of all the
+  // operands take the host 5 us of a backward pass.)
+  Matrix(const at::Tensor& y, int64_t rows, int64_t width) : t(y) {
+    if (y.is_contiguous() && (reinterpret_cast<uintptr_t>(y.data_ptr()) & 15) == 0 && width % 8 == 0) {
+      ld = width;
+      return;
+    }
+    const at::Tensor x = y.reshape({rows, width});
+    t = x;
+    const bool one = rows <= 1;
     const bool apart = !one && (x.stride(0) % 8 != 0 || x.stride(0) < x.size(1) || x.stride(0) > kFarthest);
     if (x.numel() != 0 && ((x.size(1) > 1 && x.stride(1) != 1) || apart ||
                            (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) != 0)) {
@@ -421,7 +428,7 @@ std::pair<at::Tensor, at::Tensor> gated_forward(const at::Tensor& x, const at::T
   const int dev = x.get_device();
   at::Tensor h = empty_rows(x, n), pre;
   if (keep) pre = at::empty({m, ldpre}, options_as(x).dtype(at::kFloat));
-  const Matrix a(x.reshape({m, k})), b(w);
+  const Matrix a(x, m, k), b(w, 2 * n, k);
   const Room room(x, m, n, k, true, FEEDFORWARD_ROWS);
   feedforward_check(feedforward_gated(a.at(), b.at(), h.data_ptr(), keep ? (float*)pre.data_ptr() : nullptr, (int)m,
                                       (int)n, (int)k, a.ld, b.ld, n, ldpre, type_code(x), act, room.at(), room.bytes,
@@ -434,7 +441,7 @@ at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w) {
   const int64_t n = w.size(0), k = w.size(1), m = x.numel() / k;
   const int dev = x.get_device();
   at::Tensor y = empty_rows(x, n);
-  const Matrix a(x.reshape({m, k})), b(w);
+  const Matrix a(x, m, k), b(w, n, k);
   const Room room(x, m, n, k, false, FEEDFORWARD_ROWS);
   feedforward_check(feedforward_product(a.at(), b.at(), y.data_ptr(), (int)m, (int)n, (int)k, a.ld, b.ld, n,
                                         FEEDFORWARD_ROWS, type_code(x), room.at(), room.bytes, dev,
@@ -450,13 +457,13 @@ void product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, in
   const int type = type_code(x), dev = x.get_device();
   void* const st = current_stream(dev);
   if (dx.defined()) {
-    const Matrix b(w);
+    const Matrix b(w, r, k);
     const Room room(x, m, k, r, false, FEEDFORWARD_TURN_B | padded);
     feedforward_check(feedforward_product(d.at(), b.at(), dx.data_ptr(), (int)m, (int)k, (int)r, d.ld, b.ld, k,
                                           FEEDFORWARD_TURN_B | padded, type, room.at(), room.bytes, dev, st));
   }
   if (dw.defined()) {
-    const Matrix a(x.reshape({m, k}));
+    const Matrix a(x, m, k);
     const Room room(x, r, k, m, false, FEEDFORWARD_TURN_BOTH);
     feedforward_check(feedforward_product(d.at(), a.at(), dw.data_ptr(), (int)r, (int)k, (int)m, d.ld, a.ld, k,
                                           FEEDFORWARD_TURN_BOTH, type, room.at(), room.bytes, dev, st));
@@ -481,7 +488,7 @@ std::pair<at::Tensor, at::Tensor> gated_backward(const at::Tensor& dh, const at:
     if (want_x) dx.zero_();
     if (want_w) dw.zero_();
   } else if (want_x || want_w) {
-    const Matrix d(dh.reshape({m, n})), dgu(empty_as(x, {m, up64(2 * n)}));
+    const Matrix d(dh, m, n), dgu(empty_as(x, {m, up64(2 * n)}), m, up64(2 * n));
     feedforward_check(feedforward_gated_grad(d.at(), (const float*)pre.data_ptr(), dgu.at(), (int)m, (int)n, d.ld,
                                              ldpre, up64(2 * n), type_code(x), act, dev, current_stream(dev)));
     product_grads(x, w, dgu, FEEDFORWARD_PADDED, dx, dw);
@@ -505,7 +512,7 @@ std::pair<at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy, const at
     if (want_x) dx.zero_();
     if (want_w) dw.zero_();
   } else if (want_x || want_w) {
-    product_grads(x, w, Matrix(dy.reshape({m, n})), 0, dx, dw);
+    product_grads(x, w, Matrix(dy, m, n), 0, dx, dw);
   }
   return {dx, dw};
 }
@@ -653,6 +660,11 @@ struct Rows {
   Rows() = default;
   Rows(const at::Tensor& x, int64_t rows, int64_t d) {
     if (!x.defined()) return;
+    if (x.is_contiguous()) {
+      t = x;
+      ld = d;
+      return;
+    }
     t = x.reshape({rows, d});
     if (t.numel() != 0 && ((d > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < d)))
       t = t.contiguous();
