@@ -3,7 +3,7 @@
 // kept in fp32, rounded to 16 bits, as matrix instructions take them.  Rows of [dg | du]: both
 // products of the backward pass read them as they are (ff_tile.hpp).
 //
-// Bound: HBM: 14 bytes for every element of dh.
+// Bound: HBM: 14 bytes for every element of dh.  2048 x 10752: 308 MB, 48 us, 6.4 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "ff_grads.hpp"

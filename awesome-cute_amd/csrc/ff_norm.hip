@@ -5,7 +5,10 @@
 //   r = scale r0 + gate p                                            (r = r0 without a block)
 //   y = r rstd(r) pre
 //
-// in fp32 from inputs in 16 or 32 bits, r and y rounded once (y from the unrounded r).  With
+// in fp32 from inputs in 16 or 32 bits, r and y rounded once (y from the unrounded r).  The backward
+// pass takes r as it was rounded, the value that the model goes on with: it is kept anyhow, where
+// one in fp32 would be twice the bytes; the gradients are off by 0.0023 of their length instead of
+// the 0.0017 that their own rounding makes (bfloat16).  With
 // bh = b rstd(b), rh = r rstd(r) and the gradients dy and dr of y and r
 //
 //   dt = dr + rstd(r) (dy pre - rh mean(dy pre rh))       dr0 = scale dt      dpre = sum dy rh
@@ -13,10 +16,12 @@
 //
 // the sums over the rows that share a weight or a gate.
 //
-// Bound: HBM; every row is read and written once.  A row is kept in the registers of W waves, one
-// or two 16-byte pieces a lane, so that the second pass over it that a norm needs costs nothing;
-// the waves' sums meet in LDS, two meetings a row forward.  Backward one: mean(w bh) is put
-// together from four sums, of dy pre rh, and of gate post bh times dr, dy pre and rh.
+// Bound: HBM; every row is read and written once.  8192 rows of 8192 in bfloat16 105 us, 5.1 TB/s;
+// 4096 rows of 4096 26 us and backward 45, 4.5 TB/s, and 6 for the sums over parts; one row 3.6.
+// A row is kept in the registers of W waves, one or two 16-byte pieces a lane, so that the second
+// pass over it that a norm needs costs nothing; the waves' sums meet in LDS, two meetings a row
+// forward.  Backward one: mean(w bh) is put together from four sums, of dy pre rh, and of gate post
+// bh times dr, dy pre and rh.
 //
 // Sums over rows: every part (a run of rows) adds up its own in registers, in the order of its
 // rows, and leaves them in memory; a second launch adds the parts in their order.  No atomics,

@@ -13,7 +13,11 @@
 //   - the k range may be cut into slices, whose sums meet in memory (sum_parts): problems of few
 //     tiles over a deep k.
 //
-// What bounds them: the way into LDS.
+// What bounds them: the way into LDS, and where a problem's tiles are about one to a compute unit
+// the stages' latency (eight waves hide more of it than four with twice the operands each, which
+// read a third less from LDS and take 1.0 to 1.2 of the time).  1237 x 1032 x 2744: 19 us by 117
+// tiles of 96 x 128 in two slices, and 4 for their sums; 2744 x 1237 x 1032 of its backward pass
+// 16 us, 440 TFLOP/s, 28 % of the matrix pipe's time in use.
 #include <hip/hip_runtime.h>
 
 #include "ff_tile.hpp"
