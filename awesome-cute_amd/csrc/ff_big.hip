@@ -1,7 +1,6 @@
 // Dense products in fp16 or bfloat16 by tiles of 160, 192, 224 or 256 rows x 256 columns: four
 // waves, two by two, the main loop one assembly statement (gen_products.py).  Operands by rows
-// (then k is a multiple of 64) or turned over (any k), slices and the gated epilogue as in
-// ff_tiles.hip.
+// or turned over, any depth, slices and the gated epilogue as in ff_tiles.hip.
 //
 // Bound: how evenly the tiles fill the compute units, hence the heights (777 x 2 x 5208 x 4160: 164
 // tiles of 256 rows, 205 of 160), some 12 us of a tile outside its loop (the first slabs' way, and
@@ -54,7 +53,7 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
   const int all = (p.K + kDnStageK - 1) / kDnStageK;
   const int first = at.stage(p, all, 0), end = at.stage(p, all, 1);
   const int slabs = end - first;
-  const int last_rows = end == all ? p.K - kDnStageK * (all - 1) : kDnStageK;  // of my last slab, turned over
+  const int last_k = end == all ? p.K - kDnStageK * (all - 1) : kDnStageK;  // k-values of my last slab
 
   // by rows: lane (r = lane / 8, c = lane % 8) fetches chunk c ^ r of a row; turned over: two rows
   // of 256 columns a load
@@ -62,11 +61,12 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
   i4 ra_words, rb_words;
   unsigned full_a, last_a, step_a, full_b, last_b, step_b;
   const int r8 = lane >> 3, c8 = (lane & 7) ^ r8;
+  const int past = 8 * c8 < last_k ? 0 : kOob;  // this lane's k-values of a row, in my last slab
   const int r2 = lane >> 5, piece = lane & 31;
   if constexpr (Sh::kTurnA) {
     step_a = 128u * (unsigned)p.lda;
     full_a = rows_bytes(kDnStageK, p.lda, p.M - m0);
-    last_a = rows_bytes(last_rows, p.lda, p.M - m0);
+    last_a = rows_bytes(last_k, p.lda, p.M - m0);
     ra_words = rsrc_words((const char*)p.A + ((size_t)first * kDnStageK * p.lda + m0) * 2, full_a);
 #pragma unroll
     for (int t = 0; t < TA; t++) {
@@ -75,7 +75,8 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
     }
   } else {
     step_a = kDnStageK * 2;
-    full_a = last_a = (unsigned)(rows - 1) * (unsigned)p.lda * 2u + kDnStageK * 2;
+    full_a = rows_bytes(rows, p.lda, kDnStageK);
+    last_a = rows_bytes(rows, p.lda, last_k);
     ra_words = rsrc_words((const char*)p.A + ((size_t)m0 * p.lda + (size_t)first * kDnStageK) * 2, full_a);
 #pragma unroll
     for (int t = 0; t < TA; t++) {
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
   if constexpr (Sh::kTurnedB) {
     step_b = 128u * (unsigned)p.ldb;
     full_b = rows_bytes(kDnStageK, p.ldb, p.N - n0);
-    last_b = rows_bytes(last_rows, p.ldb, p.N - n0);
+    last_b = rows_bytes(last_k, p.ldb, p.N - n0);
     rb_words = rsrc_words((const char*)p.B + ((size_t)first * kDnStageK * p.ldb + n0) * 2, full_b);
 #pragma unroll
     for (int t = 0; t < TB; t++) {
@@ -97,7 +98,8 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
     unsigned b_bytes;
     const char* const b_at = b_base<GATED>(p, n0, 256, &b_bytes, &cols);
     step_b = kDnStageK * 2;
-    full_b = last_b = b_bytes - (unsigned)p.K * 2u + kDnStageK * 2;
+    full_b = b_bytes - (unsigned)p.K * 2u + kDnStageK * 2;
+    last_b = full_b - 2u * (unsigned)(kDnStageK - last_k);
     rb_words = rsrc_words(b_at + (size_t)first * kDnStageK * 2, full_b);
 #pragma unroll
     for (int t = 0; t < TB; t++) src[TA + t] = b_offset<GATED>(p, n0, 8 * (TB * wave + t) + r8, cols) + 16 * c8;
@@ -208,7 +210,7 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
   }
 #else  // the host pass only needs the launch stub
   (void)slabs, (void)lds_a, (void)lds_b, (void)src, (void)a_rd, (void)b_rd, (void)ra_words, (void)rb_words;
-  (void)full_a, (void)last_a, (void)step_a, (void)full_b, (void)last_b, (void)step_b;
+  (void)full_a, (void)last_a, (void)step_a, (void)full_b, (void)last_b, (void)step_b, (void)past;
   for (auto& r : acc)
     for (auto& v : r) v = (f4){0.f, 0.f, 0.f, 0.f};
 #endif

@@ -107,8 +107,7 @@ struct ProductPlan {
 };
 
 bool tile_takes(const FfTile& t, int k, Layout layout, bool padded) {
-  // (rows end where their stages do, or have zeros behind them)
-  if (big_tile(t)) return layout == kTurnBoth || padded || k % kDnStageK == 0;
+  (void)k, (void)padded;
   return layout != kTurnBoth || t.rows != 96;  // (64, 128 or 256 columns of a turned operand)
 }
 

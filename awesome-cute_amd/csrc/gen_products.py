@@ -40,7 +40,9 @@ Registers (v = VGPR, a = AGPR, s = SGPR):
   v[64+4i : +3]       A operand of row block i
   v[96...] v[120...]  LDS addresses of the A and B reads: by rows 2 slot + step; turned over
                       8 slot + block
-  v[144+t]            byte offsets of this lane's loads, A then B
+  v[144+t]            byte offsets of this lane's loads, A then B; of an operand by rows past
+                      everything, by v160, for the last slab, where the lane's k-values are past the
+                      end of the rows (turned over a slab ends with the window, rows do not)
   s[40:43] s[44:47]   buffer resources of A and B; the base moves on by a slab with every request
   s49 s50 s48 s51     slabs, requested of A and of B, left
   s52 s53 s60 s61     sizes of A and B for a slab, and for the last one (0 past it)
@@ -53,7 +55,7 @@ import sys
 RA, RB = 40, 44
 S_REQB, S_N, S_REQA, S_LEFT, S_FULLA, S_FULLB, S_MA, S_MB = 48, 49, 50, 51, 52, 53, 54, 57
 S_LASTA, S_LASTB, S_STEPA, S_STEPB = 60, 61, 62, 63
-V_A, V_B, V_OFF = 96, 120, 144
+V_A, V_B, V_OFF, V_PAST = 96, 120, 144, 160
 ROW = 128           # bytes of a row of 64 k-values
 TURNED = 512        # bytes of a k-value's 256 columns
 STEPS = 2           # of 32 k-values in a slab
@@ -97,6 +99,7 @@ class Emitter:
         self.lds = []       # destinations of LDS reads in flight, oldest first
         self.vm = []        # slabs of the loads in flight, oldest first
         self.content = {}   # register quad -> what was last read into it
+        self.aside = []     # blocks that the last requests branch to
 
     def emit(self, text):
         self.lines.append(text)
@@ -122,20 +125,31 @@ class Emitter:
 
 
 def request_head(e, sh, group):
-    """what the loads of a group need, A of one slab and B of another: bases, sizes (the last slab's,
-    zero past it), m0"""
-    for res, req, last, full, step, slab in ((RA, S_REQA, S_LASTA, S_FULLA, S_STEPA, group + sh.ring_a),
-                                             (RB, S_REQB, S_LASTB, S_FULLB, S_STEPB, group + sh.ring_b)):
+    """what the loads of a group need, A of one slab and B of another: bases, m0, and aside, for the last
+    slab of either operand and those past it, sizes and offsets"""
+    n = len(e.aside)
+    block = [f".Lff_last{n}_%=:"]
+    operands = ((RA, S_REQA, S_LASTA, S_FULLA, S_STEPA, group + sh.ring_a, sh.turn_a, range(sh.ta), "a"),
+                (RB, S_REQB, S_LASTB, S_FULLB, S_STEPB, group + sh.ring_b, sh.turn_b, range(sh.ta, sh.loads), "b"))
+    for res, req, last, full, step, slab, turned, loads, name in operands:
         if slab < 0:
             continue
         if slab > 0:
             e.emit(f"s_add_u32 s{res}, s{res}, s{step}")
             e.emit(f"s_addc_u32 s{res + 1}, s{res + 1}, 0")
         e.emit(f"s_add_u32 s{req}, s{req}, 1")
-        e.emit(f"s_cmp_eq_u32 s{req}, s{S_N}")
-        e.emit(f"s_cselect_b32 s{res + 2}, s{last}, s{full}")
-        e.emit(f"s_cmp_le_u32 s{req}, s{S_N}")
-        e.emit(f"s_cselect_b32 s{res + 2}, s{res + 2}, 0")
+        block += [f"s_cmp_eq_u32 s{req}, s{S_N}", f"s_cselect_b32 s{res + 2}, s{last}, s{full}",
+                  f"s_cmp_le_u32 s{req}, s{S_N}", f"s_cselect_b32 s{res + 2}, s{res + 2}, 0"]
+        if not turned:
+            block += [f"s_cmp_lg_u32 s{req}, s{S_N}", f"s_cbranch_scc1 .Lff_not{n}{name}_%="]
+            block += [f"v_or_b32 v{V_OFF + t}, v{V_OFF + t}, v{V_PAST}" for t in loads]
+            block += [f".Lff_not{n}{name}_%=:"]
+    # (of B at least as many slabs have been requested as of A)
+    assert sh.ring_b >= sh.ring_a
+    e.emit(f"s_cmp_ge_u32 s{S_REQB}, s{S_N}")
+    e.emit(f"s_cbranch_scc1 .Lff_last{n}_%=")
+    e.emit(f".Lff_back{n}_%=:")
+    e.aside.append(block + [f"s_branch .Lff_back{n}_%="])
     if group + sh.ring_a >= 0:
         e.emit(f"s_mov_b32 m0, s{S_MA + (group + sh.ring_a) % sh.ring_a}")
     else:
@@ -295,6 +309,10 @@ def generate(sh, mfma):
     e.emit("s_nop 15")
     e.emit("s_nop 15")
     e.emit("s_waitcnt vmcnt(0) lgkmcnt(0)")
+    e.emit("s_branch .Lff_end_%=")
+    for block in e.aside:
+        e.lines += block
+    e.emit(".Lff_end_%=:")
     return e.lines
 
 
@@ -303,13 +321,17 @@ def statement(sh, mfma):
     out += [f'    "{l}\\n\\t"' for l in generate(sh, mfma)]
     outs = [f'"={{{aq(32 * i + 4 * o)}}}"(acc[{i}][{o}])' for i in range(sh.rb) for o in range(8)]
     outs += [f'"+{{{sq(RA)}}}"(ra_words)', f'"+{{{sq(RB)}}}"(rb_words)']
+    by_rows = [t for t in range(sh.loads) if not (sh.turn_a if t < sh.ta else sh.turn_b)]
+    outs += [f'"+{{v{V_OFF + t}}}"(src[{t}])' for t in by_rows]
     out.append("    : " + ",\n      ".join(outs))
     ins = [f'"{{s{S_N}}}"(slabs)', f'"{{s{S_MA}}}"(lds_a)', f'"{{s{S_MB}}}"(lds_b)',
            f'"{{s{S_FULLA}}}"(full_a)', f'"{{s{S_FULLB}}}"(full_b)', f'"{{s{S_LASTA}}}"(last_a)',
            f'"{{s{S_LASTB}}}"(last_b)', f'"{{s{S_STEPA}}}"(step_a)', f'"{{s{S_STEPB}}}"(step_b)']
     ins += [f'"{{v{V_A + j}}}"(a_rd[{j}])' for j in range((8 if sh.turn_a else 2) * sh.ring_a)]
     ins += [f'"{{v{V_B + j}}}"(b_rd[{j}])' for j in range((8 if sh.turn_b else 2) * sh.ring_b)]
-    ins += [f'"{{v{V_OFF + t}}}"(src[{t}])' for t in range(sh.loads)]
+    ins += [f'"{{v{V_OFF + t}}}"(src[{t}])' for t in range(sh.loads) if t not in by_rows]
+    if by_rows:
+        ins.append(f'"{{v{V_PAST}}}"(past)')
     out.append("    : " + ",\n      ".join(ins))
     clob = [f"v{n}" for n in range(64 + 4 * sh.rb)]
     clob += [f"s{S_REQA}", f"s{S_REQB}", f"s{S_LEFT}"]
