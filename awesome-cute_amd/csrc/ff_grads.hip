@@ -24,16 +24,11 @@ __device__ __forceinline__ float widen(unsigned bits) {
 // eight columns of a row a thread
 template <bool BF>
 __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradArgs p) {
-  // pieces of a row: n / 8, and the zeros behind its 2n columns up to a multiple of 64
-  const int pieces = p.n / 8, zeros = ((2 * p.n + 63) / 64 * 64 - 2 * p.n) / 8;
+  const int pieces = p.n / 8;
   const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int r = (int)(at / (pieces + zeros)), c = (int)(at - (long long)r * (pieces + zeros));
+  const int r = (int)(at / pieces), c = (int)(at - (long long)r * pieces);
   if (r >= p.m) return;
   half_t* const out = (half_t*)p.dgu + (size_t)r * p.lddgu;
-  if (c >= pieces) {
-    *(i4*)(out + 2 * p.n + 8 * (c - pieces)) = (i4){0, 0, 0, 0};
-    return;
-  }
   const i4 dh = *(const i4*)((const half_t*)p.dh + (size_t)r * p.lddh + 8 * c);
   const float* const pre = p.pre + (size_t)r * p.ldpre + pre_col(8 * c);
   i4 dg, du;
@@ -60,8 +55,7 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradArgs p) {
 }
 
 void launch_gated_grad(const GatedGradArgs& a, bool bf, hipStream_t stream) {
-  const int pieces = a.n / 8 + ((2 * a.n + 63) / 64 * 64 - 2 * a.n) / 8;
-  const dim3 grid((unsigned)(((long long)a.m * pieces + 255) / 256));
+  const dim3 grid((unsigned)(((long long)a.m * (a.n / 8) + 255) / 256));
   if (bf)
     hipLaunchKernelGGL(gated_grad_kernel<true>, grid, dim3(256), 0, stream, a);
   else

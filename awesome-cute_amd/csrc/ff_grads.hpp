@@ -7,7 +7,7 @@ namespace w4a16 {
 struct GatedGradArgs {
   const void* dh;    // (m x n)
   const float* pre;  // (m x ldpre), the forward pass's sums
-  void* dgu;         // (m x 2n), zeros behind a row up to a multiple of 64 columns
+  void* dgu;         // (m x 2n): [dg | du]
   long long lddh, ldpre, lddgu;
   int m, n, act;
 };

@@ -106,8 +106,7 @@ struct ProductPlan {
   int slices;
 };
 
-bool tile_takes(const FfTile& t, int k, Layout layout, bool padded) {
-  (void)k, (void)padded;
+bool tile_takes(const FfTile& t, Layout layout) {
   return layout != kTurnBoth || t.rows != 96;  // (64, 128 or 256 columns of a turned operand)
 }
 
@@ -120,10 +119,10 @@ double fit_cost(const TileFit& f, long long groups, int stages, int cus) {
 }
 
 // room: bytes for partial sums
-ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, bool padded, int cus, long long room) {
+ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, int cus, long long room) {
   const int columns = product_columns(n, gated), stages = ceil_div(k, kDnStageK);
   const bool few = layout == kRows && m <= kProductRows;
-  const bool forced = t_tile.rows > 0 && (few_tile(t_tile) ? few : tile_takes(t_tile, k, layout, padded));
+  const bool forced = t_tile.rows > 0 && (few_tile(t_tile) ? few : tile_takes(t_tile, layout));
   ProductPlan best = {{64, 64}, 1};
   double least = 0.0;
   if (few)
@@ -137,7 +136,7 @@ ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, bool pad
     }
   for (const TileFit& f : kFits) {
     if (forced && (f.tile.rows != t_tile.rows || f.tile.cols != t_tile.cols)) continue;
-    if (!tile_takes(f.tile, k, layout, padded)) continue;
+    if (!tile_takes(f.tile, layout)) continue;
     const long long tiles = (long long)ceil_div(m, f.tile.rows) * ceil_div(columns, f.tile.cols);
     for (int slices = 1; slices <= kSlicesMost && slices <= stages; slices++) {
       const double bytes = 4.0 * slices * m * columns;
@@ -164,15 +163,15 @@ constexpr int kPlansKept = 16;
 thread_local Planned t_plans[kPlansKept];
 thread_local int t_oldest = 0;
 
-Planned plan_with_room(int m, int n, int k, bool gated, Layout layout, bool padded, int cus) {
-  const int form = (gated ? 1 : 0) | (padded ? 2 : 0) | (int)layout << 2;
+Planned plan_with_room(int m, int n, int k, bool gated, Layout layout, int cus) {
+  const int form = (gated ? 1 : 0) | (int)layout << 1;
   const bool forced = t_tile.rows > 0 || t_slices > 0;
   if (!forced)
     for (const Planned& p : t_plans)
       if (p.m == m && p.n == n && p.k == k && p.cus == cus && p.form == form) return p;
   Planned p;
   p.m = m, p.n = n, p.k = k, p.cus = cus, p.form = form;
-  p.plan = choose_plan(m, n, k, gated, layout, padded, cus, 1LL << 40);
+  p.plan = choose_plan(m, n, k, gated, layout, cus, 1LL << 40);
   p.bytes = p.plan.slices > 1 ? 4LL * p.plan.slices * m * product_columns(n, gated) : 0;
   if (!forced) {
     t_plans[t_oldest] = p;
@@ -199,14 +198,12 @@ int check_sizes(int m, int n, int k, int type) {
   return FEEDFORWARD_OK;
 }
 
-bool layout_of(int turned, Layout* layout, bool* padded) {
-  *padded = (turned & FEEDFORWARD_PADDED) != 0;
-  turned &= ~FEEDFORWARD_PADDED;
+bool layout_of(int turned, Layout* layout) {
   *layout = (Layout)turned;
-  return turned >= FEEDFORWARD_ROWS && turned <= FEEDFORWARD_TURN_BOTH && !(*padded && turned != FEEDFORWARD_TURN_B);
+  return turned >= FEEDFORWARD_ROWS && turned <= FEEDFORWARD_TURN_BOTH;
 }
 
-int run_product(ProductArgs a, Layout layout, bool padded, bool bf, void* room, long long room_bytes, int dev, hipStream_t stream) {
+int run_product(ProductArgs a, Layout layout, bool bf, void* room, long long room_bytes, int dev, hipStream_t stream) {
   const bool gated = a.act != kActNone;
   const long long columns = product_columns(a.N, gated);
   // (a launch's grid, at the smallest tiles)
@@ -218,10 +215,10 @@ int run_product(ProductArgs a, Layout layout, bool padded, bool bf, void* room, 
   if (!a.A || !a.B || !a.C) return fail(FEEDFORWARD_ERR_SHAPE, "a matrix is missing");
   if (room && off16(room)) return fail(FEEDFORWARD_ERR_SHAPE, "scratch must start on 16 bytes");
   return on_device(dev, [&](int cus) {
-    const Planned planned = plan_with_room(a.M, a.N, a.K, gated, layout, padded, cus);
+    const Planned planned = plan_with_room(a.M, a.N, a.K, gated, layout, cus);
     const long long have = room ? room_bytes : 0;
     const ProductPlan p =
-        planned.bytes <= have ? planned.plan : choose_plan(a.M, a.N, a.K, gated, layout, padded, cus, have);
+        planned.bytes <= have ? planned.plan : choose_plan(a.M, a.N, a.K, gated, layout, cus, have);
     a.slices = p.slices;
     a.part = p.slices > 1 ? (float*)room : nullptr;
     a.ldpart = (int)columns;
@@ -274,13 +271,12 @@ int feedforward_product(const void* A, const void* B, void* C, int m, int n, int
                         void* stream) {
   int rc = check_sizes(m, n, k, type);
   Layout layout = kRows;
-  bool padded = false;
-  if (rc == FEEDFORWARD_OK && !layout_of(turned, &layout, &padded)) rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
+  if (rc == FEEDFORWARD_OK && !layout_of(turned, &layout)) rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
   if (rc == FEEDFORWARD_OK && layout != kTurnBoth && k % 8 != 0)
     rc = fail(FEEDFORWARD_ERR_SHAPE, "widths must be multiples of 8 (k = %d)", k);
   if (rc == FEEDFORWARD_OK && layout == kTurnBoth && m % 8 != 0)
     rc = fail(FEEDFORWARD_ERR_SHAPE, "m = %d must be a multiple of 8 where A is turned over", m);
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("A", A, lda, layout == kTurnBoth ? m : padded ? (k + 63LL) / 64 * 64 : k);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("A", A, lda, layout == kTurnBoth ? m : k);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("B", B, ldb, layout == kRows ? k : n);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("C", C, ldc, n);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
@@ -289,7 +285,7 @@ int feedforward_product(const void* A, const void* B, void* C, int m, int n, int
   a.A = A, a.B = B, a.C = C;
   a.M = m, a.N = n, a.K = k;
   a.lda = (int)lda, a.ldb = (int)ldb, a.ldc = (int)ldc;
-  return run_product(a, layout, padded, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
+  return run_product(a, layout, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
 }
 
 int feedforward_gated(const void* x, const void* w, void* h, float* pre, int m, int n, int k, long long ldx,
@@ -310,15 +306,14 @@ int feedforward_gated(const void* x, const void* w, void* h, float* pre, int m, 
   a.M = m, a.N = n, a.K = k;
   a.lda = (int)ldx, a.ldb = (int)ldw, a.ldc = (int)ldh, a.ldpre = (int)ldpre;
   a.act = activation;
-  return run_product(a, kRows, false, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
+  return run_product(a, kRows, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
 }
 
 long long feedforward_product_bytes(int m, int n, int k, int gated, int turned, int dev) {
   Layout layout;
-  bool padded;
-  if (check_sizes(m, n, k, FEEDFORWARD_FP16) != FEEDFORWARD_OK || !layout_of(turned, &layout, &padded)) return -1;
+  if (check_sizes(m, n, k, FEEDFORWARD_FP16) != FEEDFORWARD_OK || !layout_of(turned, &layout)) return -1;
   const int cus = device_cus(dev);
-  return cus > 0 && m > 0 && n > 0 && k > 0 ? plan_with_room(m, n, k, gated != 0, layout, padded, cus).bytes : 0;
+  return cus > 0 && m > 0 && n > 0 && k > 0 ? plan_with_room(m, n, k, gated != 0, layout, cus).bytes : 0;
 }
 
 int feedforward_gated_grad(const void* dh, const float* pre, void* dgu, int m, int n, long long lddh, long long ldpre,
@@ -326,10 +321,10 @@ int feedforward_gated_grad(const void* dh, const float* pre, void* dgu, int m, i
   int rc = check_sizes(m, n, 0, type);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("dh", dh, lddh, n);
   if (rc == FEEDFORWARD_OK) rc = check_matrix("pre", pre, ldpre, (n + 15LL) / 16 * 32);
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("dgu", dgu, lddgu, (2LL * n + 63) / 64 * 64);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("dgu", dgu, lddgu, 2LL * n);
   if (rc == FEEDFORWARD_OK && !act_known(activation))
     rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
-  if (rc == FEEDFORWARD_OK && (long long)m * (n / 8 + 8) > 0x7fffffffLL * 128)
+  if (rc == FEEDFORWARD_OK && (long long)m * (n / 8) > 0x7fffffffLL * 128)
     rc = fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many", m, n);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
   if (!dh || !pre || !dgu) return fail(FEEDFORWARD_ERR_SHAPE, "a matrix is missing");
@@ -401,9 +396,8 @@ int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int* o
   const int rc = check_sizes(m, n, k, FEEDFORWARD_FP16);
   if (rc != FEEDFORWARD_OK || n == 0 || k == 0 || m == 0) return rc;
   Layout layout;
-  bool padded;
-  if (!layout_of(turned, &layout, &padded)) return fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
-  const ProductPlan p = plan_with_room(m, n, k, gated != 0, layout, padded, cus).plan;
+  if (!layout_of(turned, &layout)) return fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
+  const ProductPlan p = plan_with_room(m, n, k, gated != 0, layout, cus).plan;
   out[0] = p.tile.rows;
   out[1] = p.tile.cols;
   out[2] = p.slices;

@@ -342,8 +342,6 @@ struct Matrix {
   void* at() const { return t.data_ptr(); }
 };
 
-long long up64(long long x) { return (x + 63) / 64 * 64; }
-
 void feedforward_check(int rc) {
   TORCH_CHECK_VALUE(rc != FEEDFORWARD_ERR_SHAPE, feedforward_last_error());
   TORCH_CHECK(rc == FEEDFORWARD_OK, feedforward_last_error());
@@ -450,17 +448,17 @@ at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w) {
 }
 
 // The gradients of x (m, k) and w (r, k) from that of their product, d (m, r): dx = d w and
-// dw = d^T x, sums over r and over m.  padded: FEEDFORWARD_PADDED where rows of d are, or 0.
-void product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, int padded, const at::Tensor& dx,
+// dw = d^T x, sums over r and over m.
+void product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, const at::Tensor& dx,
                    const at::Tensor& dw) {
   const int64_t k = w.size(1), m = x.numel() / k, r = w.size(0);
   const int type = type_code(x), dev = x.get_device();
   void* const st = current_stream(dev);
   if (dx.defined()) {
     const Matrix b(w, r, k);
-    const Room room(x, m, k, r, false, FEEDFORWARD_TURN_B | padded);
+    const Room room(x, m, k, r, false, FEEDFORWARD_TURN_B);
     feedforward_check(feedforward_product(d.at(), b.at(), dx.data_ptr(), (int)m, (int)k, (int)r, d.ld, b.ld, k,
-                                          FEEDFORWARD_TURN_B | padded, type, room.at(), room.bytes, dev, st));
+                                          FEEDFORWARD_TURN_B, type, room.at(), room.bytes, dev, st));
   }
   if (dw.defined()) {
     const Matrix a(x, m, k);
@@ -488,10 +486,11 @@ std::pair<at::Tensor, at::Tensor> gated_backward(const at::Tensor& dh, const at:
     if (want_x) dx.zero_();
     if (want_w) dw.zero_();
   } else if (want_x || want_w) {
-    const Matrix d(dh, m, n), dgu(empty_as(x, {m, up64(2 * n)}), m, up64(2 * n));
+    const int64_t ld = (2 * n + 63) / 64 * 64;  // rows of whole cache lines
+    const Matrix d(dh, m, n), dgu(empty_as(x, {m, ld}), m, ld);
     feedforward_check(feedforward_gated_grad(d.at(), (const float*)pre.data_ptr(), dgu.at(), (int)m, (int)n, d.ld,
-                                             ldpre, up64(2 * n), type_code(x), act, dev, current_stream(dev)));
-    product_grads(x, w, dgu, FEEDFORWARD_PADDED, dx, dw);
+                                             ldpre, ld, type_code(x), act, dev, current_stream(dev)));
+    product_grads(x, w, dgu, dx, dw);
   }
   return {dx, dw};
 }
@@ -512,7 +511,7 @@ std::pair<at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy, const at
     if (want_x) dx.zero_();
     if (want_w) dw.zero_();
   } else if (want_x || want_w) {
-    product_grads(x, w, Matrix(dy, m, n), 0, dx, dw);
+    product_grads(x, w, Matrix(dy, m, n), dx, dw);
   }
   return {dx, dw};
 }

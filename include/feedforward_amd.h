@@ -60,9 +60,6 @@ int feedforward_gated_w4(const void *A, const void *B, void *C, const void *s, i
 #define FEEDFORWARD_ROWS 0
 #define FEEDFORWARD_TURN_B 1
 #define FEEDFORWARD_TURN_BOTH 2
-/* added to FEEDFORWARD_TURN_B: behind a row of A's k elements there are zeros up to the next
- * multiple of 64, which lda has room for (as feedforward_gated_grad leaves them) */
-#define FEEDFORWARD_PADDED 4
 
 /* C (m x n) = A B^T, the sum over k > 0.  With `room`, device memory of room_bytes on 16 bytes,
  * few tiles over a deep k are computed in slices of it, whose sums are added there in a fixed
@@ -82,8 +79,7 @@ int feedforward_gated(const void *x, const void *w, void *h, float *pre, int m, 
                       long long ldx, long long ldw, long long ldh, long long ldpre, int type,
                       int activation, void *room, long long room_bytes, int dev, void *stream);
 
-/* The gradients of both sums from that of h: rows of [dg | du] (m x 2n), behind each of them
- * zeros up to the next multiple of 64 columns, which lddgu has room for. */
+/* The gradients of both sums from that of h: rows of [dg | du] (m x 2n). */
 int feedforward_gated_grad(const void *dh, const float *pre, void *dgu, int m, int n,
                            long long lddh, long long ldpre, long long lddgu, int type,
                            int activation, int dev, void *stream);
