@@ -98,7 +98,6 @@ constexpr TileFit kFewFits[] = {
     {{48, 16}, 4.12, 0.376, 0.113, 0.09, 0.677}, {{48, 32}, 4.03, 0.518, 0.349, 0.35, 0.956},
     {{64, 16}, 4.00, 0.491, 0.147, 0.24, 0.755}, {{64, 32}, 3.98, 0.648, 0.289, 1.59, 1.293}};
 // (the sums of slices written and read again, and the launch that adds them)
-constexpr int kSlicesMost = 8;
 constexpr double kSliceLaunch = 2.96, kSliceBytes = 0.327e-6;
 
 struct ProductPlan {

@@ -78,6 +78,7 @@ struct FfTile {
   int rows, cols;
 };
 constexpr int kProductRows = 64;
+constexpr int kSlicesMost = 8;  // of the k range
 inline bool big_tile(const FfTile& t) { return t.cols == 256 && t.rows >= 160; }
 inline bool few_tile(const FfTile& t) { return t.cols <= 32; }
 hipError_t configure_product_tiles();
