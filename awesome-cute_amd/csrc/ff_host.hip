@@ -181,17 +181,20 @@ Planned plan_with_room(int m, int n, int k, bool gated, Layout layout, int cus) 
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
+constexpr int kWidest = 1 << 21;  // elements from one row to the next
+
 // a matrix of 16-bit elements as the kernels address it: rows start on 16 bytes
 int check_matrix(const char* name, const void* p, long long ld, long long width) {
   if (off16(p) || ld % 8 != 0) return fail(FEEDFORWARD_ERR_SHAPE, "%s: rows must start on 16 bytes", name);
   if (ld < width) return fail(FEEDFORWARD_ERR_SHAPE, "%s: rows of %lld elements lie %lld apart", name, width, ld);
-  if (ld > (1 << 21)) return fail(FEEDFORWARD_ERR_SHAPE, "%s: rows of more than 4 MiB", name);
+  if (ld > kWidest) return fail(FEEDFORWARD_ERR_SHAPE, "%s: rows of more than 4 MiB", name);
   return FEEDFORWARD_OK;
 }
 
 int check_sizes(int m, int n, int k, int type) {
   if (m < 0 || n < 0 || k < 0) return fail(FEEDFORWARD_ERR_SHAPE, "negative size (m=%d n=%d k=%d)", m, n, k);
   if (n % 8 != 0) return fail(FEEDFORWARD_ERR_SHAPE, "widths must be multiples of 8 (n = %d)", n);
+  if (n > kWidest) return fail(FEEDFORWARD_ERR_SHAPE, "rows of more than 4 MiB (n = %d)", n);
   if (type != FEEDFORWARD_FP16 && type != FEEDFORWARD_BF16)
     return fail(FEEDFORWARD_ERR_SHAPE, "unknown type %d", type);
   return FEEDFORWARD_OK;
@@ -396,6 +399,7 @@ int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int* o
   if (rc != FEEDFORWARD_OK || n == 0 || k == 0 || m == 0) return rc;
   Layout layout;
   if (!layout_of(turned, &layout)) return fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
+  if (cus < 1) return fail(FEEDFORWARD_ERR_SHAPE, "%d compute units", cus);
   const ProductPlan p = plan_with_room(m, n, k, gated != 0, layout, cus).plan;
   out[0] = p.tile.rows;
   out[1] = p.tile.cols;

@@ -185,6 +185,17 @@ def test_codes_of_missing_matrices_and_too_many_rows():
 
 TILES = [(64, 64), (64, 128), (96, 128), (128, 128), (96, 256), (128, 256), (160, 256), (192, 256), (224, 256), (256, 256)]
 
+
+def test_plans_of_nothing():
+    with pytest.raises(ValueError, match="compute units"):
+        streamk.product_plan(8, 8, 8, cus=0)
+    with pytest.raises(ValueError, match="layout"):
+        streamk.product_plan(8, 8, 8, turned=3)
+    with pytest.raises(ValueError, match="4 MiB"):
+        streamk.product_plan(8, (1 << 21) + 8, 8, gated=True)
+    assert streamk.product_plan(0, 8, 8) is None and streamk.product_plan(8, 8, 8, cus=1) is not None
+
+
 FEW = [(rows, cols) for rows in (16, 32, 48, 64) for cols in (16, 32)]
 
 
