@@ -135,8 +135,13 @@ struct Side {
 
 }  // namespace
 
-// One barrier per 64-deep stage; the loop is dense_tile_kernel's (f16_tiles.hip).
-template <bool BF, bool GATED, Layout LAYOUT, int TM, int TN, int WM, int WN, int RING>
+// One barrier per 64-deep stage; the loop is dense_tile_kernel's (f16_tiles.hip).  ONCE: B's rows
+// are requested as read once, as the kernel for few rows requests them: where one tile is as high
+// as C.  56 problems of 9 to 64 rows that take tiles, weights from memory: 0.90 to 0.95 of the
+// time; the same weights over and over, from the last-level cache, 1.00 to 1.08, but the weights
+// of a model pass that cache.  With more tiles above each other it is slower either way (777 x 2
+// x 5208 x 4160 60 -> 69 us, 1237 x 1032 x 2744 21 -> 30).
+template <bool BF, bool GATED, Layout LAYOUT, int TM, int TN, int WM, int WN, int RING, bool ONCE>
 __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs p) {
   static_assert(!GATED || LAYOUT == kRows, "");
   using Sh = FfShape<TM, TN, WM, WN, RING, GATED>;
@@ -210,7 +215,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
     } else {
 #pragma unroll
       for (int t = 0; t < TB; t++)
-        load_to_lds16(rB, base + Sh::kSlabA + (TB * wave + t) * 1024, sb.src[t] | inv, k_at);
+        load_to_lds16<ONCE ? 2 : 0>(rB, base + Sh::kSlabA + (TB * wave + t) * 1024, sb.src[t] | inv, k_at);
     }
   };
 
@@ -345,13 +350,19 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(ProductArgs p) {
 
 namespace {
 
-// calls f(kernel, LDS bytes, threads) for a tile, a layout and a type
+// calls f(kernel, LDS bytes, threads) for a tile, a layout and a type; once: one tile is as high as C
 template <bool BF, bool GATED, Layout LAYOUT, class F>
-void with_tile(const FfTile& t, F f) {
-#define FF_TILE(TM, TN, WM, WN, RING)                                             \
-  if (t.rows == TM && t.cols == TN)                                               \
-  return f(product_tile_kernel<BF, GATED, LAYOUT, TM, TN, WM, WN, RING>,          \
+void with_tile(const FfTile& t, bool once, F f) {
+#define FF_TILE_OF(TM, TN, WM, WN, RING, ONCE)                                    \
+  if (t.rows == TM && t.cols == TN && once == ONCE)                               \
+  return f(product_tile_kernel<BF, GATED, LAYOUT, TM, TN, WM, WN, RING, ONCE>,    \
            FfShape<TM, TN, WM, WN, RING, GATED>::kLds, 64 * WM * WN)
+#define FF_TILE(TM, TN, WM, WN, RING) FF_TILE_OF(TM, TN, WM, WN, RING, false)
+  if constexpr (LAYOUT == kRows) {
+    FF_TILE_OF(64, 64, 2, 2, 4, true);
+    FF_TILE_OF(64, 128, 2, 4, 6, true);
+  }
+  once = false;
   FF_TILE(64, 64, 2, 2, 4);
   FF_TILE(64, 128, 2, 4, 6);
   FF_TILE(128, 128, 2, 4, 4);
@@ -361,13 +372,14 @@ void with_tile(const FfTile& t, F f) {
     FF_TILE(96, 256, 2, 4, 3);
   }
 #undef FF_TILE
+#undef FF_TILE_OF
 }
 template <class F>
-void with_product(const FfTile& t, bool gated, Layout layout, bool bf, F f) {
-  if (gated) return bf ? with_tile<true, true, kRows>(t, f) : with_tile<false, true, kRows>(t, f);
-  if (layout == kRows) return bf ? with_tile<true, false, kRows>(t, f) : with_tile<false, false, kRows>(t, f);
-  if (layout == kTurnB) return bf ? with_tile<true, false, kTurnB>(t, f) : with_tile<false, false, kTurnB>(t, f);
-  return bf ? with_tile<true, false, kTurnBoth>(t, f) : with_tile<false, false, kTurnBoth>(t, f);
+void with_product(const FfTile& t, bool gated, Layout layout, bool once, bool bf, F f) {
+  if (gated) return bf ? with_tile<true, true, kRows>(t, once, f) : with_tile<false, true, kRows>(t, once, f);
+  if (layout == kRows) return bf ? with_tile<true, false, kRows>(t, once, f) : with_tile<false, false, kRows>(t, once, f);
+  if (layout == kTurnB) return bf ? with_tile<true, false, kTurnB>(t, once, f) : with_tile<false, false, kTurnB>(t, once, f);
+  return bf ? with_tile<true, false, kTurnBoth>(t, once, f) : with_tile<false, false, kTurnBoth>(t, once, f);
 }
 
 }  // namespace
@@ -377,11 +389,13 @@ hipError_t configure_product_tiles() {
   for (const int rows : {64, 96, 128})
     for (const int cols : {64, 128, 256})
       for (const bool bf : {false, true})
-        for (const int form : {0, 1, 2, 3})
-          with_product({rows, cols}, form == 3, form == 3 ? kRows : (Layout)form, bf, [&](auto kernel, int lds, int) {
-            if (e == hipSuccess)
-              e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-          });
+        for (const bool once : {false, true})
+          for (const int form : {0, 1, 2, 3})
+            with_product({rows, cols}, form == 3, form == 3 ? kRows : (Layout)form, once, bf,
+                         [&](auto kernel, int lds, int) {
+                           if (e == hipSuccess)
+                             e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+                         });
   return e;
 }
 
@@ -389,7 +403,7 @@ void launch_product_tiles(ProductArgs a, const FfTile& t, Layout layout, bool bf
   const bool gated = a.act != kActNone;
   a.tiles_m = ceil_div(a.M, t.rows);
   a.tiles_n = ceil_div(product_columns(a.N, gated), t.cols);
-  with_product(t, gated, layout, bf, [&](auto kernel, int lds, int threads) {
+  with_product(t, gated, layout, a.tiles_m == 1, bf, [&](auto kernel, int lds, int threads) {
     hipLaunchKernelGGL(kernel, dim3(a.tiles_m * a.tiles_n * a.slices), dim3(threads), lds, stream, a);
   });
 }
