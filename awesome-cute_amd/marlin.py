@@ -138,6 +138,18 @@ def _gated_mul_fake(A, B, C, s, workspace, activation, max_par):
     return None
 
 
+# a layer's: rows of any shape and stride
+@torch.library.custom_op("marlin_amd::gated_linear", mutates_args=("workspace",))
+def _gated_linear_op(A: torch.Tensor, B: torch.Tensor, s: torch.Tensor, workspace: torch.Tensor,
+                     activation: int) -> torch.Tensor:
+    return _torch_binding.gated_linear(A, B, s, workspace, activation)
+
+
+@_gated_linear_op.register_fake
+def _gated_linear_fake(A, B, s, workspace, activation):
+    return A.new_empty(A.shape[:-1] + (s.shape[1] // 2,))
+
+
 # the current stream's handle, through torch's raw accessor where this torch build has it
 _get_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -362,10 +374,7 @@ class GatedLayer(Layer):
     def forward(self, A):
         if not torch.compiler.is_compiling():
             return _torch_binding.gated_linear(A, self.B, self.s, self.workspace, self._act)
-        C = torch.empty(A.shape[:-1] + (self.outfeatures,), dtype=A.dtype, device=A.device)
-        gated_mul(A.reshape((-1, A.shape[-1])), self.B, C.view((-1, self.outfeatures)), self.s,
-                  self.workspace, self.activation)
-        return C
+        return torch.ops.marlin_amd.gated_linear(A, self.B, self.s, self.workspace, self._act)
 
     def pack(self, gate, up, gate_scales, up_scales):
         """Fill B and s from two fake-quantised `torch.nn.Linear` (half weights) of (outfeatures,

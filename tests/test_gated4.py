@@ -280,3 +280,20 @@ def test_under_a_compiler():
     layer = layer_of(q, s, fake, -1, "gelu")
     compiled = torch.compile(lambda t: layer(t) * 2, backend="eager", fullgraph=True)
     assert torch.equal(compiled(x), layer(x) * 2)
+
+
+@gpu
+def test_strided_rows_under_a_compiler():
+    """What the call copies eagerly it copies there as well."""
+    n, k = 256, 256
+    x, q, s, fake = problem(6, n, k, -1, seed=9, dev="cuda")
+    layer = layer_of(q, s, fake, -1, "silu")
+    wide = torch.zeros((6, k + 40), dtype=torch.half, device="cuda")
+    wide[:, 8:8 + k] = x
+    want = layer(x)
+    for backend in ("eager", "aot_eager"):
+        compiled = torch.compile(lambda t: layer(t) * 1, backend=backend, fullgraph=True)
+        for a in (wide[:, 8:8 + k], x.t().contiguous().t(), x.reshape(2, 3, k).transpose(0, 1)):
+            assert torch.equal(compiled(a), layer(a))
+        assert torch.equal(compiled(wide[:, 8:8 + k]), want)
+    assert not layer.workspace.any()
