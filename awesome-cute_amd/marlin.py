@@ -363,18 +363,18 @@ class GatedLayer(Layer):
     Buffers as a `Layer` of 2 * outfeatures columns, gate and up in turns of eight."""
 
     def __init__(self, infeatures, outfeatures, groupsize=-1, activation="silu"):
-        self_act = _activation(activation)
+        _activation(activation)
         if outfeatures % 128 != 0:
             raise ValueError('`outfeatures` of a gated layer must be divisible by 128.')
         super().__init__(infeatures, 2 * outfeatures, groupsize)
         self.outfeatures = outfeatures
         self.activation = activation
-        self._act = self_act
 
     def forward(self, A):
+        act = _activation(self.activation)
         if not torch.compiler.is_compiling():
-            return _torch_binding.gated_linear(A, self.B, self.s, self.workspace, self._act)
-        return torch.ops.marlin_amd.gated_linear(A, self.B, self.s, self.workspace, self._act)
+            return _torch_binding.gated_linear(A, self.B, self.s, self.workspace, act)
+        return torch.ops.marlin_amd.gated_linear(A, self.B, self.s, self.workspace, act)
 
     def pack(self, gate, up, gate_scales, up_scales):
         """Fill B and s from two fake-quantised `torch.nn.Linear` (half weights) of (outfeatures,

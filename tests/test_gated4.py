@@ -297,3 +297,22 @@ def test_strided_rows_under_a_compiler():
             assert torch.equal(compiled(a), layer(a))
         assert torch.equal(compiled(wide[:, 8:8 + k]), want)
     assert not layer.workspace.any()
+
+
+def test_an_activation_is_what_the_layer_says():
+    layer = marlin.GatedLayer(256, 128)
+    layer.activation = "relu"
+    with pytest.raises(ValueError, match="activation"):
+        layer(torch.zeros(1, 256).half())
+
+
+@gpu
+def test_an_activation_that_is_changed():
+    """Eagerly and under a compiler it is the layer's attribute that counts."""
+    n, k = 128, 256
+    x, q, s, fake = problem(3, n, k, 128, seed=4, dev="cuda")
+    layer = layer_of(q, s, fake, 128, "silu")
+    want = layer_of(q, s, fake, 128, "gelu")(x)
+    layer.activation = "gelu"
+    assert torch.equal(layer(x), want)
+    assert torch.equal(torch.compile(lambda t: layer(t) * 1, backend="eager", fullgraph=True)(x), want)
