@@ -57,6 +57,25 @@ bool to_int(PyObject* o, int* v) {
 
 void* current_stream(int dev) { return (void*)c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream(); }
 
+bool differentiated(std::initializer_list<const at::Tensor*> inputs) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : inputs)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// The result of a product with 4-bit weights, which have no gradients, for inputs that want some: a
+// backward pass that gets there is told.  (The node's edges go on to the inputs, so that it is on the
+// way of every gradient that is asked for; without it a sum with the product would pass back
+// the gradient of its other terms alone.)
+at::Tensor without_gradients(const at::Tensor& out, std::initializer_list<const at::Tensor*> inputs) {
+  variable_list all = {out};
+  for (const at::Tensor* t : inputs) all.push_back(*t);
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "products with 4-bit weights have no gradients", (int64_t)all.size());
+  return (*error)(std::move(all))[0];
+}
+
 constexpr int kMulTensors = 5;
 const char* const kMulNames[kMulTensors] = {"A", "B", "C", "s", "workspace"};
 
@@ -212,6 +231,9 @@ PyObject* py_gated_mul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!(t[i] = tensor(args[i], kMulNames[i]))) return nullptr;
   int act, max_par;
   if (!to_int(args[5], &act) || !to_int(args[6], &max_par)) return nullptr;
+  // (as torch's functions with an `out` do)
+  TORCH_CHECK(!differentiated({t[0], t[2], t[3]}),
+              "gated_mul writes into C and has no gradients, but an argument requires one");
   if (!enqueue_gated(*t[0], *t[1], *t[2], *t[3], *t[4], act, max_par)) return nullptr;
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
@@ -246,7 +268,20 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     out = C.view({rows.size(0), n});
   }
   if (!enqueue_gated(rows, *B, out, *s, *workspace, act, 16)) return nullptr;
-  return THPVariable_Wrap(std::move(C));
+  return THPVariable_Wrap(differentiated({A, s}) ? without_gradients(C, {A, s}) : std::move(C));
+  END_HANDLE_TH_ERRORS
+}
+
+// without_gradients(out, A): out as the result of products of A
+PyObject* py_without_gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 2) {
+    PyErr_SetString(PyExc_TypeError, "without_gradients takes 2 arguments");
+    return nullptr;
+  }
+  const at::Tensor *out = tensor(args[0], "out"), *A = tensor(args[1], "A");
+  if (!out || !A) return nullptr;
+  return THPVariable_Wrap(differentiated({A}) ? without_gradients(*out, {A}) : *out);
   END_HANDLE_TH_ERRORS
 }
 
@@ -557,13 +592,6 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> tensors) {
   Py_ssize_t i = 0;
   for (const at::Tensor& t : tensors) PyTuple_SET_ITEM(tuple, i++, THPVariable_Wrap(t));  // (None where undefined)
   return tuple;
-}
-
-bool differentiated(std::initializer_list<const at::Tensor*> inputs) {
-  if (!c10::GradMode::is_enabled()) return false;
-  for (const at::Tensor* t : inputs)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
 }
 
 bool takes(Py_ssize_t nargs, Py_ssize_t want, const char* name) {
@@ -1046,6 +1074,7 @@ PyMethodDef methods[] = {
     {"linear_grads", (PyCFunction)(void (*)(void))py_linear_grads, METH_FASTCALL, nullptr},
     {"gated_mul", (PyCFunction)(void (*)(void))py_gated_mul, METH_FASTCALL, nullptr},
     {"gated_linear", (PyCFunction)(void (*)(void))py_gated_linear, METH_FASTCALL, nullptr},
+    {"without_gradients", (PyCFunction)(void (*)(void))py_without_gradients, METH_FASTCALL, nullptr},
     {"quantize", (PyCFunction)(void (*)(void))py_quantize, METH_FASTCALL, nullptr},
     {"pack", (PyCFunction)(void (*)(void))py_pack, METH_FASTCALL, nullptr},
     {"dense", (PyCFunction)(void (*)(void))py_dense, METH_FASTCALL, nullptr},

@@ -151,7 +151,8 @@ class FeedForward(_Half):
 
 class QuantizedFeedForward(_Half):
     """`FeedForward` with 4-bit weights, torch.half, for inference: `gate_up` a marlin.GatedLayer,
-    `down` a marlin.Layer."""
+    `down` a marlin.Layer.  The products have no gradients: a backward pass that would need them
+    raises RuntimeError, as does compiling for one."""
 
     def __init__(self, hidden, inner, activation="silu", groupsize=128, *, post_norm=True, gate=False, scale=1.0,
                  eps=1e-6, device=None):
@@ -162,4 +163,7 @@ class QuantizedFeedForward(_Half):
         self.requires_grad_(False)
 
     def _products(self, y):
-        return self.down(self.gate_up(y))
+        out = self.down(self.gate_up(y))
+        if y.requires_grad and torch.is_grad_enabled():
+            return _torch_binding.without_gradients(out, y)
+        return out

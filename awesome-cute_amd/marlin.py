@@ -113,6 +113,10 @@ def _activation(name):
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}") from None
 
 
+def _wants_gradients(t):
+    return t.requires_grad and torch.is_grad_enabled()
+
+
 def gated_mul(A, B, C, s, workspace, activation="silu", max_par=16):
     """Both projections of a gated feed-forward block, the activation and the product of the two in
     one launch: C = act(A @ G) * (A @ U), rounded once; no reference counterpart.
@@ -120,9 +124,12 @@ def gated_mul(A, B, C, s, workspace, activation="silu", max_par=16):
     A: (m, k) half.  B: (k/16, 4n) int32, s: (groups, 2n) or (1, 2n) half: G and U as
     `GatedLayer.pack` leaves them.  C: (m, n) half, overwritten.  workspace: at least n/64*max_par
     zero int32 entries; zero again afterwards.  activation: "silu" or "gelu" (its tanh form).
-    n and k are multiples of 128.  Asynchronous on the current stream of A's device."""
+    n and k are multiples of 128.  Asynchronous on the current stream of A's device.  No gradients:
+    arguments that require one are refused, unless under torch.no_grad()."""
     act = _activation(activation)
     if torch.compiler.is_compiling():
+        if any(_wants_gradients(t) for t in (A, C, s)):
+            raise RuntimeError("gated_mul writes into C and has no gradients, but an argument requires one")
         return torch.ops.marlin_amd.gated_mul(A, B, C, s, workspace, act, max_par)
     _torch_binding.gated_mul(A, B, C, s, workspace, act, max_par)
 
@@ -360,7 +367,8 @@ class _Weight:
 class GatedLayer(Layer):
     """The gate and up projections of a feed-forward block in 4 bits, with the activation and the
     product: (..., infeatures) -> (..., outfeatures) half, act(x Wg^T) * (x Wu^T) in one launch.
-    Buffers as a `Layer` of 2 * outfeatures columns, gate and up in turns of eight."""
+    Buffers as a `Layer` of 2 * outfeatures columns, gate and up in turns of eight.  For inference:
+    a backward pass that comes to it raises RuntimeError."""
 
     def __init__(self, infeatures, outfeatures, groupsize=-1, activation="silu"):
         _activation(activation)
@@ -374,6 +382,8 @@ class GatedLayer(Layer):
         act = _activation(self.activation)
         if not torch.compiler.is_compiling():
             return _torch_binding.gated_linear(A, self.B, self.s, self.workspace, act)
+        if _wants_gradients(A):
+            raise RuntimeError("products with 4-bit weights have no gradients: compile them under torch.no_grad()")
         return torch.ops.marlin_amd.gated_linear(A, self.B, self.s, self.workspace, act)
 
     def pack(self, gate, up, gate_scales, up_scales):

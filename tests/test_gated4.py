@@ -316,3 +316,43 @@ def test_an_activation_that_is_changed():
     layer.activation = "gelu"
     assert torch.equal(layer(x), want)
     assert torch.equal(torch.compile(lambda t: layer(t) * 1, backend="eager", fullgraph=True)(x), want)
+
+
+def test_what_has_no_gradients_says_so():
+    """The result of products that have none, wherever a gradient would pass through it."""
+    x, out = torch.ones(3, requires_grad=True), torch.full((3,), 2.0)
+    mark = marlin._torch_binding.without_gradients
+    y = mark(out, x)
+    assert torch.equal(y.detach(), out) and y.requires_grad
+    for backward in (lambda: (x + y).sum().backward(), lambda: torch.autograd.grad((x + y).sum(), x),
+                     lambda: torch.autograd.grad((x * 2 + mark(out, x * 3)).sum(), x)):
+        with pytest.raises(RuntimeError, match="4-bit weights have no gradients"):
+            backward()
+    with torch.no_grad():
+        assert not mark(out, x).requires_grad
+    assert not mark(out, x.detach()).requires_grad
+
+
+@gpu
+def test_gradients_are_not_lost_without_a_word():
+    n = k = 256
+    x, q, s, fake = problem(3, n, k, 128, seed=4, dev="cuda")
+    layer = layer_of(q, s, fake, 128, "silu")
+    want = layer(x)
+    x.requires_grad_()
+    y = layer(x)
+    assert torch.equal(y, want)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        (x + y).sum().backward()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        torch.autograd.grad((x + layer(x)).sum(), x)
+    C = torch.empty_like(want)
+    with pytest.raises(RuntimeError, match="gated_mul"):
+        marlin.gated_mul(x, layer.B, C, layer.s, layer.workspace)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        torch.compile(lambda t: t + layer(t), backend="aot_eager", fullgraph=True)(x)
+    with torch.no_grad():
+        assert not layer(x).requires_grad
+        marlin.gated_mul(x, layer.B, C, layer.s, layer.workspace)
+        assert torch.equal(torch.compile(lambda t: layer(t) * 1, backend="aot_eager", fullgraph=True)(x), want)
+    assert torch.equal(C, want)

@@ -618,3 +618,29 @@ def test_a_training_step_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(out, r)
         assert all(torch.equal(p.detach(), q) for p, q in zip(params, after))
+
+
+@gpu
+def test_the_block_in_four_bits_has_no_gradients_and_says_so():
+    torch.manual_seed(2)
+    four = feedforward.FeedForward(256, 256, gate=True, dtype=torch.float16, device="cuda").quantize(128)
+    x = torch.randn(5, 256, device="cuda").half()
+    with torch.no_grad():
+        want = four(x, next_weight=four.pre_weight)
+    # of the norms and the gate there are gradients, where none has to pass through the products
+    gate = torch.rand(256, device="cuda").half().requires_grad_()
+    y, r = four(x, gate, four.pre_weight)
+    assert all(torch.isfinite(g).all() and g.any() for g in torch.autograd.grad((y.float() + r.float()).sum(), gate))
+    x.requires_grad_()
+    for backward in (lambda r: r.float().sum().backward(), lambda r: torch.autograd.grad(r.float().sum(), x)):
+        y, r = four(x, next_weight=four.pre_weight)
+        assert torch.equal(r, want[1]) and torch.equal(y, want[0])
+        with pytest.raises(RuntimeError, match="4-bit weights have no gradients"):
+            backward(r)
+    normed, _ = residual_norm(x, pre_weight=four.pre_weight)
+    with pytest.raises(RuntimeError, match="4-bit weights have no gradients"):
+        torch.autograd.grad(four.after_norm(normed, x.detach())[1].float().sum(), x)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        torch.compile(lambda t: four(t)[1], backend="aot_eager", fullgraph=True)(x)
+    with torch.no_grad():
+        assert torch.equal(torch.compile(lambda t: four(t)[1], backend="aot_eager", fullgraph=True)(x), want[1])
