@@ -64,6 +64,12 @@ bool differentiated(std::initializer_list<const at::Tensor*> inputs) {
   return false;
 }
 
+// No kernel carries tangents along, and a result without one would count as a constant
+void refuse_tangents(std::initializer_list<const at::Tensor*> inputs) {
+  for (const at::Tensor* t : inputs)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "forward-mode differentiation is not supported");
+}
+
 // The result of a product with 4-bit weights, which have no gradients, for inputs that want some: a
 // backward pass that gets there is told.  (The node's edges go on to the inputs, so that it is on the
 // way of every gradient that is asked for; without it a sum with the product would pass back
@@ -231,6 +237,7 @@ PyObject* py_gated_mul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!(t[i] = tensor(args[i], kMulNames[i]))) return nullptr;
   int act, max_par;
   if (!to_int(args[5], &act) || !to_int(args[6], &max_par)) return nullptr;
+  refuse_tangents({t[0], t[2], t[3]});
   // (as torch's functions with an `out` do)
   TORCH_CHECK(!differentiated({t[0], t[2], t[3]}),
               "gated_mul writes into C and has no gradients, but an argument requires one");
@@ -251,6 +258,7 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!A || !B || !s || !workspace) return nullptr;
   int act;
   if (!to_int(args[4], &act)) return nullptr;
+  refuse_tangents({A, s});
   if (A->dim() < 1 || s->dim() != 2 || s->size(1) % 2 != 0 || A->size(-1) == 0) {
     PyErr_SetString(PyExc_ValueError, "A needs a last dimension, s two and an even number of columns");
     return nullptr;
@@ -608,6 +616,7 @@ PyObject* py_gated_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   int act;
   if (!x || !w || !to_int(args[2], &act)) return nullptr;
   at::Tensor h;
+  refuse_tangents({x, w});
   {
     pybind11::gil_scoped_release unlocked;
     h = differentiated({x, w}) ? GatedFunction::apply(*x, *w, (int64_t)act) : gated_forward(*x, *w, act, false).first;
@@ -623,6 +632,7 @@ PyObject* py_linear_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
   if (!x || !w) return nullptr;
   at::Tensor y;
+  refuse_tangents({x, w});
   {
     pybind11::gil_scoped_release unlocked;
     y = differentiated({x, w}) ? LinearFunction::apply(*x, *w) : linear_forward(*x, *w);
@@ -880,6 +890,7 @@ PyObject* py_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   NormInputs in;
   if (!takes(nargs, 7, "residual_norm") || !norm_arguments(args, &in)) return nullptr;
+  refuse_tangents({&in.residual, &in.block, &in.post, &in.gate, &in.pre});
   const double scale = PyFloat_AsDouble(args[5]), eps = PyFloat_AsDouble(args[6]);
   if (PyErr_Occurred()) return nullptr;
   NormOutputs out;

@@ -116,6 +116,16 @@ def test_refuses_host_tensors_and_unknown_activations():
         streamk.linear(None, w)
 
 
+def test_refuses_forward_mode():
+    import torch.autograd.forward_ad as forward_ad
+    x, w = torch.zeros(2, 16).half(), torch.zeros(32, 16).half()
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(x, x), w), (x, forward_ad.make_dual(w, w))):
+            for call in (streamk.gated, streamk.linear):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*args)
+
+
 @pytest.mark.parametrize("m,n,k,lda,ldb,ldc,type,code", [
     (-1, 8, 8, 8, 8, 8, 0, 1), (4, 12, 8, 8, 8, 16, 0, 1), (4, 8, 12, 16, 16, 8, 0, 1), (4, 8, 8, 8, 8, 8, 2, 1),
     (4, 8, 16, 8, 16, 8, 0, 1), (4, 8, 16, 20, 16, 8, 0, 1), (4, 8, 16, 16, 16, 4, 0, 1), (4, 8, 0, 8, 8, 8, 0, 1),
@@ -610,3 +620,19 @@ def test_under_a_compiler():
     torch.compile(lambda a, b: streamk.gated(a, b), backend=record, fullgraph=True)(*leaves)
     assert any("gated_alone" in n for n in names[0]) and not any("gated_dense" in n for n in names[0])
     assert any("gated_dense" in n for n in names[1])
+
+
+@gpu
+def test_forward_mode_is_refused_beside_tensors_without_tangents():
+    import torch.autograd.forward_ad as forward_ad
+    x, w, _ = make(20, 16, 32, torch.float16, 0)
+    want = streamk.linear(x, w)
+    with forward_ad.dual_level():
+        assert torch.equal(streamk.linear(x, w), want)
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for a in (dual, dual[:5], dual * 2):
+            for call in (streamk.gated, streamk.linear):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(a, w)
+        with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+            streamk.linear(dual, w)

@@ -356,3 +356,15 @@ def test_gradients_are_not_lost_without_a_word():
         marlin.gated_mul(x, layer.B, C, layer.s, layer.workspace)
         assert torch.equal(torch.compile(lambda t: layer(t) * 1, backend="aot_eager", fullgraph=True)(x), want)
     assert torch.equal(C, want)
+
+
+def test_refuses_forward_mode():
+    import torch.autograd.forward_ad as forward_ad
+    layer = marlin.GatedLayer(256, 128)
+    x, C = torch.zeros(1, 256).half(), torch.zeros(1, 128).half()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            layer(dual)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            marlin.gated_mul(dual, layer.B, C, layer.s, layer.workspace)

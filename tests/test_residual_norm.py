@@ -173,6 +173,19 @@ def test_refuses_host_tensors():
         feedforward.FeedForward(16, 16, "relu")
 
 
+def test_refuses_forward_mode():
+    import torch.autograd.forward_ad as forward_ad
+    x, w = torch.zeros(2, 16), torch.ones(16)
+    with forward_ad.dual_level():
+        for args in (dict(residual=forward_ad.make_dual(x, x), pre_weight=w),
+                     dict(residual=x, pre_weight=forward_ad.make_dual(w, w)),
+                     dict(residual=x, block=forward_ad.make_dual(x, x)),
+                     dict(residual=x, block=x, post_weight=forward_ad.make_dual(w, w)),
+                     dict(residual=x, block=x, gate=forward_ad.make_dual(w, w))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                residual_norm(**args)
+
+
 def test_codes_and_scratch_of_the_entries():
     import ctypes
     import marlin
