@@ -20,8 +20,10 @@
 #include <torch/csrc/autograd/variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/InferenceMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <pybind11/pybind11.h>
@@ -63,6 +65,29 @@ bool differentiated(std::initializer_list<const at::Tensor*> inputs) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+
+// Whether something records the operators of torch's dispatcher: a dispatch mode (make_fx, fake
+// tensors, a counter), torch.jit.trace, or a tensor of its own kind.  A launch behind the dispatcher
+// is nothing to them, and all that they would see of a call is its output's allocation; the caller,
+// in Python, gets NotImplemented and takes the call's operator, which comes back here with one
+// argument more (`Call::inner`) once nobody looks on.
+bool looked_on(std::initializer_list<const at::Tensor*> inputs) {
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set() || at::tracer::impl::is_dispatch_enabled()) return true;
+  for (const at::Tensor* t : inputs)
+    if (t->defined() && t->key_set().has(c10::DispatchKey::Python)) return true;
+  return false;
+}
+
+// The arguments that a call came with: `want`, or one more
+struct Call {
+  bool inner = false;
+  bool takes(Py_ssize_t nargs, Py_ssize_t want, const char* name) {
+    inner = nargs == want + 1;
+    if (nargs == want || inner) return true;
+    PyErr_Format(PyExc_TypeError, "%s takes %d arguments", name, (int)want);
+    return false;
+  }
+};
 
 // No kernel carries tangents along, and a result without one would count as a constant
 void refuse_tangents(std::initializer_list<const at::Tensor*> inputs) {
@@ -129,13 +154,12 @@ bool enqueue_mul(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C, 
 // mul(A, B, C, s, workspace, thread_k, thread_n, sms, max_par, cute_version)
 PyObject* py_mul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 10) {
-    PyErr_SetString(PyExc_TypeError, "mul takes 10 arguments");
-    return nullptr;
-  }
+  Call call;
+  if (!call.takes(nargs, 10, "mul")) return nullptr;
   const at::Tensor* t[kMulTensors];
   for (int i = 0; i < kMulTensors; i++)
     if (!(t[i] = tensor(args[i], kMulNames[i]))) return nullptr;
+  if (!call.inner && looked_on({t[0], t[1], t[2], t[3], t[4]})) Py_RETURN_NOTIMPLEMENTED;
   Hints h;
   if (!to_int(args[5], &h.thread_k) || !to_int(args[6], &h.thread_n) || !to_int(args[7], &h.sms) ||
       !to_int(args[8], &h.max_par))
@@ -152,13 +176,12 @@ PyObject* py_mul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // the weight, rows of any shape
 PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 5) {
-    PyErr_SetString(PyExc_TypeError, "linear takes 5 arguments");
-    return nullptr;
-  }
+  Call call;
+  if (!call.takes(nargs, 5, "linear")) return nullptr;
   const at::Tensor *A = tensor(args[0], "A"), *B = tensor(args[1], "B"), *s = tensor(args[2], "s"),
                    *workspace = tensor(args[3], "workspace");
   if (!A || !B || !s || !workspace) return nullptr;
+  if (!call.inner && looked_on({A, B, s, workspace})) Py_RETURN_NOTIMPLEMENTED;
   Hints h;
   h.cute = PyObject_IsTrue(args[4]);
   if (h.cute < 0) return nullptr;
@@ -228,10 +251,8 @@ bool enqueue_gated(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C
 // gated_mul(A, B, C, s, workspace, activation, max_par)
 PyObject* py_gated_mul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 7) {
-    PyErr_SetString(PyExc_TypeError, "gated_mul takes 7 arguments");
-    return nullptr;
-  }
+  Call call;
+  if (!call.takes(nargs, 7, "gated_mul")) return nullptr;
   const at::Tensor* t[kMulTensors];
   for (int i = 0; i < kMulTensors; i++)
     if (!(t[i] = tensor(args[i], kMulNames[i]))) return nullptr;
@@ -239,8 +260,9 @@ PyObject* py_gated_mul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!to_int(args[5], &act) || !to_int(args[6], &max_par)) return nullptr;
   refuse_tangents({t[0], t[2], t[3]});
   // (as torch's functions with an `out` do)
-  TORCH_CHECK(!differentiated({t[0], t[2], t[3]}),
+  TORCH_CHECK(call.inner || !differentiated({t[0], t[2], t[3]}),
               "gated_mul writes into C and has no gradients, but an argument requires one");
+  if (!call.inner && looked_on({t[0], t[1], t[2], t[3], t[4]})) Py_RETURN_NOTIMPLEMENTED;
   if (!enqueue_gated(*t[0], *t[1], *t[2], *t[3], *t[4], act, max_par)) return nullptr;
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
@@ -249,16 +271,15 @@ PyObject* py_gated_mul(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // gated_linear(A, B, s, workspace, activation) -> C, rows of any shape
 PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 5) {
-    PyErr_SetString(PyExc_TypeError, "gated_linear takes 5 arguments");
-    return nullptr;
-  }
+  Call call;
+  if (!call.takes(nargs, 5, "gated_linear")) return nullptr;
   const at::Tensor *A = tensor(args[0], "A"), *B = tensor(args[1], "B"), *s = tensor(args[2], "s"),
                    *workspace = tensor(args[3], "workspace");
   if (!A || !B || !s || !workspace) return nullptr;
   int act;
   if (!to_int(args[4], &act)) return nullptr;
   refuse_tangents({A, s});
+  if (!call.inner && looked_on({A, B, s, workspace})) Py_RETURN_NOTIMPLEMENTED;
   if (A->dim() < 1 || s->dim() != 2 || s->size(1) % 2 != 0 || A->size(-1) == 0) {
     PyErr_SetString(PyExc_ValueError, "A needs a last dimension, s two and an even number of columns");
     return nullptr;
@@ -276,7 +297,7 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     out = C.view({rows.size(0), n});
   }
   if (!enqueue_gated(rows, *B, out, *s, *workspace, act, 16)) return nullptr;
-  return THPVariable_Wrap(differentiated({A, s}) ? without_gradients(C, {A, s}) : std::move(C));
+  return THPVariable_Wrap(!call.inner && differentiated({A, s}) ? without_gradients(C, {A, s}) : std::move(C));
   END_HANDLE_TH_ERRORS
 }
 
@@ -296,14 +317,13 @@ PyObject* py_without_gradients(PyObject*, PyObject* const* args, Py_ssize_t narg
 // dense(A, B, C or None) -> C (m, n) = A (m, k) * B (n, k)^T
 PyObject* py_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 3) {
-    PyErr_SetString(PyExc_TypeError, "dense takes 3 arguments");
-    return nullptr;
-  }
+  Call call;
+  if (!call.takes(nargs, 3, "dense")) return nullptr;
   const at::Tensor* in[2];
   for (int i = 0; i < 2; i++) {
     const char* const name = i ? "B" : "A";
     if (!(in[i] = tensor(args[i], name))) return nullptr;
+    if (!call.inner && looked_on({in[i]})) Py_RETURN_NOTIMPLEMENTED;
     if (in[i]->scalar_type() != at::kHalf || !in[i]->is_cuda() || !in[i]->is_contiguous() ||
         in[i]->dim() != 2) {
       PyErr_Format(PyExc_ValueError, "%s must be a contiguous 2-d torch.half tensor on the GPU", name);
@@ -611,15 +631,17 @@ bool takes(Py_ssize_t nargs, Py_ssize_t want, const char* name) {
 // gated_dense(x, weight, activation) -> h, with what its gradients need where they are wanted
 PyObject* py_gated_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (!takes(nargs, 3, "gated_dense")) return nullptr;
+  Call call;
+  if (!call.takes(nargs, 3, "gated_dense")) return nullptr;
   const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
   int act;
   if (!x || !w || !to_int(args[2], &act)) return nullptr;
   at::Tensor h;
   refuse_tangents({x, w});
+  if (!call.inner && looked_on({x, w})) Py_RETURN_NOTIMPLEMENTED;
   {
     pybind11::gil_scoped_release unlocked;
-    h = differentiated({x, w}) ? GatedFunction::apply(*x, *w, (int64_t)act) : gated_forward(*x, *w, act, false).first;
+    h = !call.inner && differentiated({x, w}) ? GatedFunction::apply(*x, *w, (int64_t)act) : gated_forward(*x, *w, act, false).first;
   }
   return THPVariable_Wrap(std::move(h));
   END_HANDLE_TH_ERRORS
@@ -628,14 +650,16 @@ PyObject* py_gated_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // linear_dense(x, weight) -> x weight^T, likewise
 PyObject* py_linear_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (!takes(nargs, 2, "linear_dense")) return nullptr;
+  Call call;
+  if (!call.takes(nargs, 2, "linear_dense")) return nullptr;
   const at::Tensor *x = tensor(args[0], "x"), *w = tensor(args[1], "weight");
   if (!x || !w) return nullptr;
   at::Tensor y;
   refuse_tangents({x, w});
+  if (!call.inner && looked_on({x, w})) Py_RETURN_NOTIMPLEMENTED;
   {
     pybind11::gil_scoped_release unlocked;
-    y = differentiated({x, w}) ? LinearFunction::apply(*x, *w) : linear_forward(*x, *w);
+    y = !call.inner && differentiated({x, w}) ? LinearFunction::apply(*x, *w) : linear_forward(*x, *w);
   }
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
@@ -891,6 +915,7 @@ PyObject* py_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   NormInputs in;
   if (!takes(nargs, 7, "residual_norm") || !norm_arguments(args, &in)) return nullptr;
   refuse_tangents({&in.residual, &in.block, &in.post, &in.gate, &in.pre});
+  if (looked_on({&in.residual, &in.block, &in.post, &in.gate, &in.pre})) Py_RETURN_NOTIMPLEMENTED;
   const double scale = PyFloat_AsDouble(args[5]), eps = PyFloat_AsDouble(args[6]);
   if (PyErr_Occurred()) return nullptr;
   NormOutputs out;

@@ -26,11 +26,12 @@ def residual_norm(residual, block=None, *, post_weight=None, gate=None, scale=1.
     Differentiable once, on the current stream of the residual's device; sums over rows are added in
     a fixed order."""
     scale, eps = float(scale), float(eps)
-    if torch.compiler.is_compiling():
-        y, r, _ = torch.ops.marlin_amd.residual_norm(residual, block, post_weight, gate, pre_weight, scale, eps)
-        return (None if pre_weight is None else y), (residual if block is None else r)
-    y, r = _torch_binding.residual_norm(residual, block, post_weight, gate, pre_weight, scale, eps)
-    return y, residual if block is None else r
+    if not torch.compiler.is_compiling():
+        out = _torch_binding.residual_norm(residual, block, post_weight, gate, pre_weight, scale, eps)
+        if out is not NotImplemented:  # (something records the dispatcher's operators)
+            return out[0], residual if block is None else out[1]
+    y, r, _ = torch.ops.marlin_amd.residual_norm(residual, block, post_weight, gate, pre_weight, scale, eps)
+    return (None if pre_weight is None else y), (residual if block is None else r)
 
 
 _Maybe = torch.Tensor | None

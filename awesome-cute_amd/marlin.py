@@ -79,23 +79,26 @@ def mul(A, B, C, s, workspace, thread_k=-1, thread_n=-1, sms=-1, max_par=16, cut
     Asynchronous on the current stream of A's device.  Raises RuntimeError where
     the reference binding raises (marlin_gemm.cpp:27-31,48-55).
     """
-    if torch.compiler.is_compiling():
-        # under torch.compile the call is one opaque operator that mutates C and
-        # workspace (the reference advertises use within torch.compile, marlin.py:12)
-        return torch.ops.marlin_amd.mul(A, B, C, s, workspace, thread_k, thread_n, sms, max_par,
-                                        cute_version)
-    _torch_binding.mul(A, B, C, s, workspace, thread_k, thread_n, sms, max_par, cute_version)
+    if not torch.compiler.is_compiling():
+        if _torch_binding.mul(A, B, C, s, workspace, thread_k, thread_n, sms, max_par,
+                              cute_version) is not NotImplemented:
+            return
+    # under torch.compile the call is one opaque operator that mutates C and
+    # workspace (the reference advertises use within torch.compile, marlin.py:12)
+    torch.ops.marlin_amd.mul(A, B, C, s, workspace, thread_k, thread_n, sms, max_par, cute_version)
 
 
-# The same call as an operator of torch's dispatcher, for compilers that trace
-# Python: `mul` routes through it while torch.compile is tracing and calls the
+# The same call as an operator of torch's dispatcher, for compilers and tracers:
+# `mul` routes through it while torch.compile is tracing, or where something
+# records the dispatcher's operators and the binding says NotImplemented, and calls the
 # library directly otherwise (the dispatcher costs more host time than the
-# one-row kernel takes).  It returns nothing; C and workspace are mutated.
+# one-row kernel takes).  It returns nothing; C and workspace are mutated.  (The
+# argument more says that the call is the operator's own.)
 @torch.library.custom_op("marlin_amd::mul", mutates_args=("C", "workspace"))
 def _mul_op(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, s: torch.Tensor,
             workspace: torch.Tensor, thread_k: int, thread_n: int, sms: int, max_par: int,
             cute_version: bool) -> None:
-    _torch_binding.mul(A, B, C, s, workspace, thread_k, thread_n, sms, max_par, cute_version)
+    _torch_binding.mul(A, B, C, s, workspace, thread_k, thread_n, sms, max_par, cute_version, True)
 
 
 @_mul_op.register_fake
@@ -127,17 +130,18 @@ def gated_mul(A, B, C, s, workspace, activation="silu", max_par=16):
     n and k are multiples of 128.  Asynchronous on the current stream of A's device.  No gradients:
     arguments that require one are refused, unless under torch.no_grad()."""
     act = _activation(activation)
-    if torch.compiler.is_compiling():
-        if any(_wants_gradients(t) for t in (A, C, s)):
-            raise RuntimeError("gated_mul writes into C and has no gradients, but an argument requires one")
-        return torch.ops.marlin_amd.gated_mul(A, B, C, s, workspace, act, max_par)
-    _torch_binding.gated_mul(A, B, C, s, workspace, act, max_par)
+    if not torch.compiler.is_compiling():
+        if _torch_binding.gated_mul(A, B, C, s, workspace, act, max_par) is not NotImplemented:
+            return
+    if any(_wants_gradients(t) for t in (A, C, s)):
+        raise RuntimeError("gated_mul writes into C and has no gradients, but an argument requires one")
+    torch.ops.marlin_amd.gated_mul(A, B, C, s, workspace, act, max_par)
 
 
 @torch.library.custom_op("marlin_amd::gated_mul", mutates_args=("C", "workspace"))
 def _gated_mul_op(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, s: torch.Tensor,
                   workspace: torch.Tensor, activation: int, max_par: int) -> None:
-    _torch_binding.gated_mul(A, B, C, s, workspace, activation, max_par)
+    _torch_binding.gated_mul(A, B, C, s, workspace, activation, max_par, True)
 
 
 @_gated_mul_op.register_fake
@@ -149,7 +153,7 @@ def _gated_mul_fake(A, B, C, s, workspace, activation, max_par):
 @torch.library.custom_op("marlin_amd::gated_linear", mutates_args=("workspace",))
 def _gated_linear_op(A: torch.Tensor, B: torch.Tensor, s: torch.Tensor, workspace: torch.Tensor,
                      activation: int) -> torch.Tensor:
-    return _torch_binding.gated_linear(A, B, s, workspace, activation)
+    return _torch_binding.gated_linear(A, B, s, workspace, activation, True)
 
 
 @_gated_linear_op.register_fake
@@ -329,7 +333,9 @@ class Layer(nn.Module):
                 B, s, workspace = held['B'], held['s'], held['workspace']
             except KeyError:  # made a parameter, or computed by a parametrisation
                 B, s, workspace = self.B, self.s, self.workspace
-            return _torch_binding.linear(A, B, s, workspace, self.cute_version)
+            C = _torch_binding.linear(A, B, s, workspace, self.cute_version)
+            if C is not NotImplemented:
+                return C
         C = torch.empty(A.shape[:-1] + (self.s.shape[1],), dtype=A.dtype, device=A.device)
         mul(A.reshape((-1, A.shape[-1])), self.B, C.view((-1, C.shape[-1])), self.s,
             self.workspace, cute_version=self.cute_version)
@@ -381,9 +387,11 @@ class GatedLayer(Layer):
     def forward(self, A):
         act = _activation(self.activation)
         if not torch.compiler.is_compiling():
-            return _torch_binding.gated_linear(A, self.B, self.s, self.workspace, act)
+            C = _torch_binding.gated_linear(A, self.B, self.s, self.workspace, act)
+            if C is not NotImplemented:
+                return C
         if _wants_gradients(A):
-            raise RuntimeError("products with 4-bit weights have no gradients: compile them under torch.no_grad()")
+            raise RuntimeError("products with 4-bit weights have no gradients: compile or trace them under torch.no_grad()")
         return torch.ops.marlin_amd.gated_linear(A, self.B, self.s, self.workspace, act)
 
     def pack(self, gate, up, gate_scales, up_scales):

@@ -90,13 +90,31 @@ def force_finish_polls(polls):
 
 def gemm(A, B, C=None):
     """C (m, n) = A (m, k) @ B (n, k).T on the current stream; returns C."""
-    return _torch_binding.dense(A, B, C)
+    if not torch.compiler.is_compiling():
+        out = _torch_binding.dense(A, B, C)
+        if out is not NotImplemented:
+            return out
+    if C is None:
+        C = A.new_empty((A.shape[0], B.shape[0]))
+    torch.ops.marlin_amd.gemm(A, B, C)
+    return C
+
+
+@torch.library.custom_op("marlin_amd::gemm", mutates_args=("C",))
+def _gemm_op(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor) -> None:
+    _torch_binding.dense(A, B, C, True)
+
+
+@_gemm_op.register_fake
+def _gemm_fake(A, B, C):
+    return None
 
 
 # ---------------------------------------------------------------------------
-# Products with gradients.  Under a compiler each is one operator of torch's dispatcher, which
+# Products with gradients.  Under a compiler, or where something records the dispatcher's operators
+# (the binding says NotImplemented), each is one operator of torch's dispatcher, which
 # costs more host time than a product of a few rows takes; else the binding's, which is an autograd
-# function where gradients are wanted.
+# function where gradients are wanted.  (An argument more: the call is an operator's own.)
 
 ACTIVATIONS = {"silu": 1, "gelu": 2}  # (gelu in its tanh form)
 _lib.feedforward_plan.restype = _I
@@ -123,19 +141,23 @@ def gated(x, weight, activation="silu"):
     row.  Rows that do not start on 16 bytes are copied.  Differentiable once, on
     the current stream of x's device."""
     act = _activation(activation)
-    if torch.compiler.is_compiling():
-        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-            return torch.ops.marlin_amd.gated_dense(x, weight, act)[0]
-        return torch.ops.marlin_amd.gated_alone(x, weight, act)
-    return _torch_binding.gated_dense(x, weight, act)
+    if not torch.compiler.is_compiling():
+        h = _torch_binding.gated_dense(x, weight, act)
+        if h is not NotImplemented:
+            return h
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return torch.ops.marlin_amd.gated_dense(x, weight, act)[0]
+    return torch.ops.marlin_amd.gated_alone(x, weight, act)
 
 
 def linear(x, weight):
     """x @ weight.T for x (..., k) and weight (n, k), torch.half or torch.bfloat16, n and k multiples
     of 8; returns (..., n).  Differentiable once; streams and alignment as `gated`."""
-    if torch.compiler.is_compiling():
-        return torch.ops.marlin_amd.linear_dense(x, weight)
-    return _torch_binding.linear_dense(x, weight)
+    if not torch.compiler.is_compiling():
+        y = _torch_binding.linear_dense(x, weight)
+        if y is not NotImplemented:
+            return y
+    return torch.ops.marlin_amd.linear_dense(x, weight)
 
 
 @torch.library.custom_op("marlin_amd::gated_dense", mutates_args=())
@@ -153,8 +175,7 @@ def _gated_fake(x, weight, act):
 # ... without gradients, and so without the sums
 @torch.library.custom_op("marlin_amd::gated_alone", mutates_args=())
 def _gated_alone_op(x: torch.Tensor, weight: torch.Tensor, act: int) -> torch.Tensor:
-    with torch.no_grad():
-        return _torch_binding.gated_dense(x, weight, act)
+    return _torch_binding.gated_dense(x, weight, act, True)
 
 
 @_gated_alone_op.register_fake
@@ -175,7 +196,7 @@ def _gated_grads_fake(dh, sums, x, weight, act):
 
 @torch.library.custom_op("marlin_amd::linear_dense", mutates_args=())
 def _linear_op(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
-    return _torch_binding.linear_dense(x, weight)
+    return _torch_binding.linear_dense(x, weight, True)
 
 
 @_linear_op.register_fake
