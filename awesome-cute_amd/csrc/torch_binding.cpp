@@ -460,14 +460,20 @@ void check_capture(std::initializer_list<const at::Tensor*> inputs, int dev) {
 }
 
 // The gradients that a backward pass returns, where that is itself to be differentiated: no kernel
-// does, and whoever asks for it is told
-variable_list once_differentiable(variable_list&& grads, const char* name) {
+// does, and whoever asks for it is told.  `from`: what they are made of, to which the edges of the
+// node that tells go on -- without these it is on the way to no input, and a second derivative
+// that has another path to its input would be that path's alone.
+variable_list once_differentiable(variable_list&& grads, const char* name, std::initializer_list<const variable_list*> from) {
   if (!c10::GradMode::is_enabled()) return std::move(grads);
+  const size_t count = grads.size();
+  variable_list all;
+  for (at::Tensor& g : grads) all.push_back(g.defined() ? g.detach().set_requires_grad(true) : g);
+  for (const variable_list* list : from) all.insert(all.end(), list->begin(), list->end());
   auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once",
-                                                               (int)grads.size());
-  variable_list marked;
-  for (at::Tensor& g : grads) marked.push_back(g.defined() ? g.detach().set_requires_grad(true) : g);
-  return (*error)(std::move(marked));
+                                                               (int64_t)all.size());
+  variable_list marked = (*error)(std::move(all));
+  marked.resize(count);
+  return marked;
 }
 
 // Scratch for a product's partial sums, where its plan has any
@@ -594,7 +600,7 @@ struct GatedFunction : torch::autograd::Function<GatedFunction> {
       std::tie(out[0], out[1]) = gated_backward(grads[0], saved[2], saved[0], saved[1], (int)ctx->saved_data["act"].toInt(),
                                                 ctx->needs_input_grad(0), ctx->needs_input_grad(1));
     }
-    return once_differentiable(std::move(out), "gated");
+    return once_differentiable(std::move(out), "gated", {&grads, &saved});
   }
 };
 
@@ -610,7 +616,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       c10::AutoGradMode off(false);
       std::tie(out[0], out[1]) = linear_backward(grads[0], saved[0], saved[1], ctx->needs_input_grad(0), ctx->needs_input_grad(1));
     }
-    return once_differentiable(std::move(out), "linear");
+    return once_differentiable(std::move(out), "linear", {&grads, &saved});
   }
 };
 
@@ -886,7 +892,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
                              leaf != ctx->saved_data.end() ? leaf->second.toTensor() : at::Tensor(), want);
       for (int i = 0; i < 5; i++) out[i] = g[i];
     }
-    return once_differentiable(std::move(out), "residual_norm");
+    return once_differentiable(std::move(out), "residual_norm", {&grads, &saved});
   }
 };
 

@@ -636,3 +636,20 @@ def test_forward_mode_is_refused_beside_tensors_without_tangents():
                     call(a, w)
         with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
             streamk.linear(dual, w)
+
+
+@gpu
+def test_second_derivatives_beside_another_path_to_the_same_input():
+    """Asked for by inputs, where no node that is on no way to them would be run."""
+    for call in (streamk.gated, streamk.linear):
+        x, w, dh = make(20, 16, 32, torch.float16, 0)
+        dh = call(x, w).clone()
+        leaves = [t.requires_grad_() for t in (x, w, dh)]
+        for i in (0, 1):
+            g, = torch.autograd.grad(call(x, w), leaves[i], dh, create_graph=True)
+            for leaf in leaves:
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    torch.autograd.grad(g.float().sum() + leaf.float().sum(), leaf, retain_graph=True)
+            # what has nothing to do with them is none of theirs
+            z = torch.ones(3, device="cuda", requires_grad=True)
+            assert torch.autograd.grad(g.float().sum() + (2 * z).sum(), z)[0].eq(2).all()

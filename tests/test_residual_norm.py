@@ -657,3 +657,19 @@ def test_the_block_in_four_bits_has_no_gradients_and_says_so():
         torch.compile(lambda t: four(t)[1], backend="aot_eager", fullgraph=True)(x)
     with torch.no_grad():
         assert torch.equal(torch.compile(lambda t: four(t)[1], backend="aot_eager", fullgraph=True)(x), want[1])
+
+
+@gpu
+def test_second_derivatives_beside_another_path_to_the_same_input():
+    t, dy, dr = make((2, 5, 72), torch.float32, "channel", 8)
+    v = leaves(t)
+    dy.requires_grad_()
+    for name in NAMES:
+        g, = torch.autograd.grad(run(v), v[name], (dy, dr), create_graph=True)
+        for leaf in (*v.values(), dy):
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                torch.autograd.grad(g.sum() + leaf.sum(), leaf, retain_graph=True)
+    x, w = v["residual"], v["pre_weight"]
+    g, = torch.autograd.grad(residual_norm(x, pre_weight=w)[0], w, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(g.sum() + x.sum(), x)
