@@ -436,7 +436,8 @@ __global__ __launch_bounds__(64 * wg_waves(W)) void norm_grad_kernel(NormGradArg
         const float rh = this_r[i].at(e) * rstd2, bh = this_b[i].at(e) * rstd1, dye = this_dy[i].at(e);
         const float dt = __builtin_fmaf(rstd2, dye * w.pre.at(e) - rh * m1, this_dr[i].at(e));
         d0[e] = p.scale * dt;
-        db[e] = rstd1 * (dt * w.gate.at(e) * w.post.at(e) - bh * m2);
+        // (without a norm after the block its values, infinite ones too, are no part of its gradient)
+        db[e] = rstd1 * (dt * w.gate.at(e) * w.post.at(e) - (p.post ? bh : 0.f) * m2);
         if constexpr (SUMS != kNoSums) {
           sum_pre[i][e] = __builtin_fmaf(dye, rh, sum_pre[i][e]);
           q[i][e] = __builtin_fmaf(dt, bh, q[i][e]);

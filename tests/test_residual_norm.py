@@ -673,3 +673,22 @@ def test_second_derivatives_beside_another_path_to_the_same_input():
     g, = torch.autograd.grad(residual_norm(x, pre_weight=w)[0], w, dy, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(g.sum() + x.sum(), x)
+
+
+@gpu
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("d", [72, 1001, 16384])
+def test_infinities_of_a_block_without_a_norm_are_no_part_of_its_gradient(d, type):
+    """r = scale residual + gate block is linear in the block: its gradient is gate dr, whatever is in it."""
+    for gate in ("none", "channel", "sequence"):
+        t, _, dr = make((2, 9, d), type, gate, 5, post=False, pre=False)
+        v = leaves(t)
+        want = torch.autograd.grad(run(v)[1], (v["residual"], v["block"]), dr)
+        gp = 1.0 if t["gate"] is None else t["gate"].double()
+        assert ((want[1].double() - gp * dr.double()).abs() <= half_step(type) * (gp * dr.double()).abs() + least(type)).all()
+        t["block"][0, 3, 5] = float("inf")
+        t["block"][1, 0, 70] = float("-inf")
+        t["block"][1, 4] = float("nan")
+        v = leaves(t)
+        got = torch.autograd.grad(run(v)[1], (v["residual"], v["block"]), dr)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
