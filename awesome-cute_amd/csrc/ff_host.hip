@@ -389,7 +389,7 @@ int feedforward_norm_grad(const void* dy, long long ld_dy, const void* dr, long 
   a.partials = sums ? (float*)partials : nullptr;
   a.ld_dy = ld_dy, a.ld_dr = ld_dr, a.ld_r = ld_r, a.ld_block = ld_block, a.ld_gate = ld_gate;
   a.rows = rows, a.rows_per_gate = rows_per_gate, a.d = d;
-  a.scale = scale;
+  a.scale = block ? scale : 1.f;  // (without a block r is the residual, whatever the scale)
   return on_device(dev, [&](int) { launch_norm_grad(a, norm_type(type), (hipStream_t)stream); });
 }
 

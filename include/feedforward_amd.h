@@ -98,19 +98,19 @@ void feedforward_force_tile(int rows, int cols, int slices);
  * = 1 / sqrt(mean(v^2) + eps); fp32 inside, r and y rounded once, y from the unrounded r.  Every
  * matrix is of one type (fp32 too), `rows` rows of d <= 16384 elements, `ld...` apart; r and y
  * contiguous.  Null: post (no norm after the block, p = block), gate (1), pre (no norm before
- * the next block, y is not written), block (r = residual, not written; then neither post nor
- * gate).  gate has a row for every rows_per_gate rows.  stats, if not null, (rows x 2) floats:
- * rstd(block) and rstd(r), which the backward pass takes.
+ * the next block, y is not written), block (r = residual whatever the scale, not written; then
+ * neither post nor gate).  gate has a row for every rows_per_gate rows.  stats, if not null,
+ * (rows x 2) floats: rstd(block) and rstd(r), which the backward pass takes.
  */
 int feedforward_norm(const void *residual, long long ld_residual, const void *block,
                      long long ld_block, const void *post, const void *gate, long long ld_gate,
                      int rows_per_gate, const void *pre, float scale, float eps, void *r, void *y,
                      float *stats, long long rows, int d, int type, int dev, void *stream);
 
-/* Its gradients from dy (null without pre) and dr (null: zero), r the forward pass's (the
- * residual without a block).  Outputs that are null are not computed; dresidual and dblock
- * (rows x d), dgate (a row per gate), dpost and dpre (d) are contiguous.  The sums over rows
- * go through `partials`, at least feedforward_norm_grad_bytes(...) bytes of device memory, in
+/* Its gradients from dy (null without pre) and dr (null: zero), r the forward pass's (without a
+ * block the residual, whatever the scale).  Outputs that are null are not computed, and of no
+ * rows none is written, dpost and dpre neither; dresidual and dblock (rows x d), dgate (a row
+ * per gate), dpost and dpre (d) are contiguous.  The sums over rows go through `partials`, at least feedforward_norm_grad_bytes(...) bytes of device memory, in
  * an order that the sizes alone decide. */
 int feedforward_norm_grad(const void *dy, long long ld_dy, const void *dr, long long ld_dr,
                           const void *r, long long ld_r, const void *block, long long ld_block,

@@ -692,3 +692,33 @@ def test_infinities_of_a_block_without_a_norm_are_no_part_of_its_gradient(d, typ
         v = leaves(t)
         got = torch.autograd.grad(run(v)[1], (v["residual"], v["block"]), dr)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_the_entries_take_one_scale_for_both_passes():
+    """Without a block r is the residual itself, and its gradient is that of the norm alone, whatever
+    the scale."""
+    import ctypes
+    import marlin
+    lib, L, I, D, P = marlin._lib, ctypes.c_longlong, ctypes.c_int, ctypes.c_float, ctypes.c_void_p
+    rows, d = 6, 136
+    t, dy, _ = make((rows, d), torch.float32, "none", 4, block=False, post=False)
+    v = leaves(t)
+    want_y = run(v)[0]
+    want, = torch.autograd.grad(want_y, v["residual"], dy)
+    x, w = t["residual"], t["pre_weight"]
+    y, dx, stats = torch.empty_like(x), torch.empty_like(x), torch.empty(rows, 2, device="cuda")
+
+    def at(t):
+        return P(t.data_ptr())
+
+    torch.cuda.synchronize()
+    for scale in (1.0, 0.5):
+        dx.fill_(float("nan"))
+        stream = P(torch.cuda.current_stream().cuda_stream)
+        assert lib.feedforward_norm(at(x), L(d), None, L(d), None, None, L(d), I(rows), at(w), D(scale), D(EPS), None,
+                                    at(y), at(stats), L(rows), I(d), I(2), I(0), stream) == 0
+        assert lib.feedforward_norm_grad(at(dy), L(d), None, L(d), at(x), L(d), None, L(d), None, None, L(d), I(rows),
+                                         at(w), D(scale), at(stats), at(dx), None, None, None, None, None, L(0), L(rows),
+                                         I(d), I(2), I(0), stream) == 0
+        assert torch.equal(y, want_y) and torch.equal(dx, want), scale
