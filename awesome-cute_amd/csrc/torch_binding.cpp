@@ -671,8 +671,15 @@ PyObject* py_linear_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// gated_sums(x, weight, activation) -> (h, both sums), gated_grads(dh, sums, x, weight, activation)
-// and linear_grads(dy, x, weight) -> (dx, dweight): the passes by themselves, for compilers
+// gated_sums(x, weight, activation) -> (h, both sums), gated_grads(dh, sums, x, weight, activation, want_x,
+// want_weight) and linear_grads(dy, x, weight, want_x, want_weight) -> (dx, dweight), None where not
+// wanted: the passes by themselves, for compilers
+bool to_bool(PyObject* o, bool* v) {
+  const int is = PyObject_IsTrue(o);
+  *v = is > 0;
+  return is >= 0;
+}
+
 PyObject* py_gated_sums(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   if (!takes(nargs, 3, "gated_sums")) return nullptr;
@@ -690,15 +697,17 @@ PyObject* py_gated_sums(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 PyObject* py_gated_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (!takes(nargs, 5, "gated_grads")) return nullptr;
+  if (!takes(nargs, 7, "gated_grads")) return nullptr;
   const at::Tensor *dh = tensor(args[0], "dh"), *pre = tensor(args[1], "sums"), *x = tensor(args[2], "x"),
                    *w = tensor(args[3], "weight");
   int act;
-  if (!dh || !pre || !x || !w || !to_int(args[4], &act)) return nullptr;
+  bool want_x, want_w;
+  if (!dh || !pre || !x || !w || !to_int(args[4], &act) || !to_bool(args[5], &want_x) || !to_bool(args[6], &want_w))
+    return nullptr;
   std::pair<at::Tensor, at::Tensor> out;
   {
     pybind11::gil_scoped_release unlocked;
-    out = gated_backward(*dh, *pre, *x, *w, act, true, true);
+    out = gated_backward(*dh, *pre, *x, *w, act, want_x, want_w);
   }
   return tuple_of({out.first, out.second});
   END_HANDLE_TH_ERRORS
@@ -706,13 +715,14 @@ PyObject* py_gated_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 PyObject* py_linear_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (!takes(nargs, 3, "linear_grads")) return nullptr;
+  if (!takes(nargs, 5, "linear_grads")) return nullptr;
   const at::Tensor *dy = tensor(args[0], "dy"), *x = tensor(args[1], "x"), *w = tensor(args[2], "weight");
-  if (!dy || !x || !w) return nullptr;
+  bool want_x, want_w;
+  if (!dy || !x || !w || !to_bool(args[3], &want_x) || !to_bool(args[4], &want_w)) return nullptr;
   std::pair<at::Tensor, at::Tensor> out;
   {
     pybind11::gil_scoped_release unlocked;
-    out = linear_backward(*dy, *x, *w, true, true);
+    out = linear_backward(*dy, *x, *w, want_x, want_w);
   }
   return tuple_of({out.first, out.second});
   END_HANDLE_TH_ERRORS
@@ -941,7 +951,8 @@ PyObject* py_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // norm_lengths(... as residual_norm) -> (y, r, lengths) and norm_grads(dy, dr, r, block, post, gate, pre,
-// lengths, scale) -> five gradients, None for what is: the passes by themselves, for compilers
+// lengths, scale, and which of the five are wanted) -> five gradients, None where not wanted and for what
+// is None: the passes by themselves, for compilers
 PyObject* py_norm_lengths(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   NormInputs in;
@@ -961,16 +972,19 @@ PyObject* py_norm_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   NormInputs in;
   at::Tensor dy, dr;
-  if (!takes(nargs, 9, "norm_grads") || !optional(args[0], "dy", &dy) || !optional(args[1], "dr", &dr) ||
+  if (!takes(nargs, 14, "norm_grads") || !optional(args[0], "dy", &dy) || !optional(args[1], "dr", &dr) ||
       !norm_arguments(args + 2, &in))
     return nullptr;
   const at::Tensor* const lengths = tensor(args[7], "lengths");
   const double scale = PyFloat_AsDouble(args[8]);
   if (!lengths || PyErr_Occurred()) return nullptr;
+  std::array<bool, 5> want;
+  for (int i = 0; i < 5; i++)
+    if (!to_bool(args[9 + i], &want[i])) return nullptr;
   std::array<at::Tensor, 5> g;
   {
     pybind11::gil_scoped_release unlocked;
-    g = norm_backward(dy, dr, in, *lengths, scale, at::Tensor(), {true, true, true, true, true});
+    g = norm_backward(dy, dr, in, *lengths, scale, at::Tensor(), want);
   }
   return tuple_of({g[0], g[1], g[2], g[3], g[4]});
   END_HANDLE_TH_ERRORS

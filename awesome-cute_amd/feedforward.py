@@ -54,14 +54,14 @@ def _norm_fake(residual, block, post, gate, pre, scale, eps):
 
 @torch.library.custom_op("marlin_amd::norm_grads", mutates_args=())
 def _norm_grads_op(dy: _Maybe, dr: _Maybe, r: torch.Tensor, block: _Maybe, post: _Maybe, gate: _Maybe, pre: _Maybe,
-                   lengths: torch.Tensor, scale: float) -> list[torch.Tensor]:
-    out = _torch_binding.norm_grads(dy, dr, r, block, post, gate, pre, lengths, scale)
+                   lengths: torch.Tensor, scale: float, want: list[bool]) -> list[torch.Tensor]:
+    out = _torch_binding.norm_grads(dy, dr, r, block, post, gate, pre, lengths, scale, *want)
     return [r.new_empty(0) if g is None else g for g in out]
 
 
 @_norm_grads_op.register_fake
-def _norm_grads_fake(dy, dr, r, block, post, gate, pre, lengths, scale):
-    return [r.new_empty(0 if t is None else t.shape) for t in (r, block, post, gate, pre)]
+def _norm_grads_fake(dy, dr, r, block, post, gate, pre, lengths, scale, want):
+    return [r.new_empty(0 if t is None or not w else t.shape) for t, w in zip((r, block, post, gate, pre), want)]
 
 
 def _keep_norm(ctx, inputs, output):
@@ -72,9 +72,10 @@ def _keep_norm(ctx, inputs, output):
 
 def _norm_backward(ctx, dy, dr, _):
     r, block, post, gate, pre, lengths = ctx.saved_tensors
+    want = list(ctx.needs_input_grad[:5])  # (False of what is None)
     out = torch.ops.marlin_amd.norm_grads(dy if pre is not None else None, dr if block is not None else None, r, block,
-                                          post, gate, pre, lengths, ctx.scale)
-    return (out[0], *(None if t is None else g for t, g in zip((block, post, gate, pre), out[1:])), None, None)
+                                          post, gate, pre, lengths, ctx.scale, want)
+    return (*(g if w else None for g, w in zip(out, want)), None, None)
 
 
 _norm_op.register_autograd(_norm_backward, setup_context=_keep_norm)

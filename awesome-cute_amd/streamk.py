@@ -183,15 +183,24 @@ def _gated_alone_fake(x, weight, act):
     return x.new_empty(x.shape[:-1] + (weight.shape[0] // 2,))
 
 
+# (of gradients that are not wanted an operator, which has to return tensors, returns empty ones)
+def _wanted(x, dx, dw):
+    return tuple(x.new_empty(0) if g is None else g for g in (dx, dw))
+
+
+def _grads_fake(x, weight, want_x, want_weight):
+    return x.new_empty(x.shape if want_x else 0), weight.new_empty(weight.shape if want_weight else 0)
+
+
 @torch.library.custom_op("marlin_amd::gated_grads", mutates_args=())
-def _gated_grads_op(dh: torch.Tensor, sums: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
-                    act: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return _torch_binding.gated_grads(dh, sums, x, weight, act)
+def _gated_grads_op(dh: torch.Tensor, sums: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act: int,
+                    want_x: bool, want_weight: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return _wanted(x, *_torch_binding.gated_grads(dh, sums, x, weight, act, want_x, want_weight))
 
 
 @_gated_grads_op.register_fake
-def _gated_grads_fake(dh, sums, x, weight, act):
-    return x.new_empty(x.shape), weight.new_empty(weight.shape)
+def _gated_grads_fake(dh, sums, x, weight, act, want_x, want_weight):
+    return _grads_fake(x, weight, want_x, want_weight)
 
 
 @torch.library.custom_op("marlin_amd::linear_dense", mutates_args=())
@@ -205,14 +214,14 @@ def _linear_fake(x, weight):
 
 
 @torch.library.custom_op("marlin_amd::linear_grads", mutates_args=())
-def _linear_grads_op(dy: torch.Tensor, x: torch.Tensor,
-                     weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    return _torch_binding.linear_grads(dy, x, weight)
+def _linear_grads_op(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, want_x: bool,
+                     want_weight: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return _wanted(x, *_torch_binding.linear_grads(dy, x, weight, want_x, want_weight))
 
 
 @_linear_grads_op.register_fake
-def _linear_grads_fake(dy, x, weight):
-    return x.new_empty(x.shape), weight.new_empty(weight.shape)
+def _linear_grads_fake(dy, x, weight, want_x, want_weight):
+    return _grads_fake(x, weight, want_x, want_weight)
 
 
 def _keep_gated(ctx, inputs, output):
@@ -222,8 +231,9 @@ def _keep_gated(ctx, inputs, output):
 
 def _gated_backward(ctx, dh, _):
     x, weight, sums = ctx.saved_tensors
-    dx, dw = torch.ops.marlin_amd.gated_grads(dh, sums, x, weight, ctx.act)
-    return dx, dw, None
+    want = ctx.needs_input_grad
+    dx, dw = torch.ops.marlin_amd.gated_grads(dh, sums, x, weight, ctx.act, want[0], want[1])
+    return dx if want[0] else None, dw if want[1] else None, None
 
 
 def _keep_linear(ctx, inputs, output):
@@ -231,7 +241,9 @@ def _keep_linear(ctx, inputs, output):
 
 
 def _linear_backward(ctx, dy):
-    return torch.ops.marlin_amd.linear_grads(dy, *ctx.saved_tensors)
+    want = ctx.needs_input_grad
+    dx, dw = torch.ops.marlin_amd.linear_grads(dy, *ctx.saved_tensors, want[0], want[1])
+    return dx if want[0] else None, dw if want[1] else None
 
 
 _gated_op.register_autograd(_gated_backward, setup_context=_keep_gated)

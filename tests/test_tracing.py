@@ -141,3 +141,50 @@ def test_gradients_under_a_mode():
     with Record() as record:
         got = torch.autograd.grad(streamk.linear(x, w), (x, w), dy)
     assert same(got, want) and record.seen[0] == "linear_dense"
+
+
+def backward_calls(call, inputs):
+    """The backward operators' nodes of a compiled call, and the gradients that it gives."""
+    from torch._dynamo.backends.common import aot_autograd
+    from functorch.compile import make_boxed_func
+    nodes = []
+
+    def backward(graph, example):
+        nodes.extend(n for n in graph.graph.nodes if "_grads" in str(n.target))
+        return make_boxed_func(graph.forward)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(call, backend=aot_autograd(fw_compiler=lambda g, e: make_boxed_func(g.forward),
+                                                        bw_compiler=backward), fullgraph=True)
+    wanted = [t for t in inputs if t.requires_grad]
+    outs = compiled(*inputs)
+    outs = outs if isinstance(outs, tuple) else (outs,)
+    return nodes, torch.autograd.grad(outs, wanted, [o.detach() for o in outs])
+
+
+@gpu
+@pytest.mark.parametrize("frozen", [0, 1])
+@pytest.mark.parametrize("name", ["gated", "linear"])
+def test_compiled_backward_passes_compute_what_is_wanted(name, frozen):
+    call, shapes, _ = calls("cuda")[name]
+    inputs = make(shapes, 4)
+    inputs[1 - frozen].requires_grad_()
+    nodes, got = backward_calls(call, inputs)
+    out = call(*inputs)
+    assert same(got, torch.autograd.grad(out, inputs[1 - frozen], out.detach()))
+    assert [n.args[-2:] for n in nodes] == [(frozen == 1, frozen == 0)]
+
+
+@gpu
+def test_compiled_backward_passes_of_norms_compute_what_is_wanted():
+    shapes = ((20, 64), (20, 64), (64,), (64,), (64,))
+
+    def call(x, b, post, gate, pre):
+        return feedforward.residual_norm(x, b, post_weight=post, gate=gate, pre_weight=pre)
+
+    for wanted in ((0, 1), (2, 4), (3,), (0, 1, 2, 3, 4)):
+        inputs = [t.requires_grad_(i in wanted) for i, t in enumerate(make(shapes, 5))]
+        nodes, got = backward_calls(call, inputs)
+        outs = call(*inputs)
+        assert same(got, torch.autograd.grad(outs, [inputs[i] for i in wanted], [o.detach() for o in outs]))
+        assert [n.args[-1] for n in nodes] == [[i in wanted for i in range(5)]]
