@@ -1018,9 +1018,10 @@ int run(const void* A, const void* B, void* C, const void* s, int m, int n, int 
   }
   // the kernels address A, B and C with 32-bit byte offsets
   const long long lim = 0x7fffffffLL;
-  if ((long long)k * n / 2 > lim || (long long)m * k * 2 > lim || (long long)m * n * 2 > lim) {
+  const int c_cols = act ? n / 2 : n;
+  if ((long long)k * n / 2 > lim || (long long)m * k * 2 > lim || (long long)m * c_cols * 2 > lim) {
     snprintf(g_last_error, sizeof(g_last_error),
-             "operand of more than 2 GiB (m=%d n=%d k=%d): split the call", m, n, k);
+             "operand of more than 2 GiB (m=%d n=%d k=%d): split the call", m, c_cols, k);
     return MARLIN_ERR_RUNTIME;
   }
   if (dev < 0 || dev >= kMaxDevices) {

@@ -368,3 +368,24 @@ def test_refuses_forward_mode():
             layer(dual)
         with pytest.raises(RuntimeError, match="forward-mode"):
             marlin.gated_mul(dual, layer.B, C, layer.s, layer.workspace)
+
+
+@pytest.mark.parametrize("m,n,k,code", [(80000, 14336, 128, 3), (8192, 128, 1 << 17, 3), (1, 1 << 17, 1 << 14, 3)])
+def test_operands_of_more_than_two_gib_are_refused(m, n, k, code):
+    import ctypes
+    err = ctypes.create_string_buffer(256)
+    rc = marlin._lib.feedforward_gated_w4(None, None, None, None, m, n, k, 1, None, ctypes.c_longlong(1 << 30), 1, 0,
+                                          None, 16, err, 256)
+    assert rc == code and b"2 GiB" in err.value and f"m={m} n={n} k={k}".encode() in err.value
+
+
+@gpu
+def test_as_many_rows_as_make_two_gib_of_results():
+    """The product has twice C's columns, and would be more; the first rows, the last and some between."""
+    n, k, m = 14336, 128, 74880
+    assert 1.99 * 2 ** 30 < 2 * m * n < 2 ** 31
+    x, q, s, fake = problem(m, n, k, -1, seed=1, dev="cuda")
+    layer = layer_of(q, s, fake, -1, "silu")
+    y = layer(x)
+    for first in (0, 37440, m - 200):
+        check(y[first:first + 200], x[first:first + 200], q, s, "silu")
