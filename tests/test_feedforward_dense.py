@@ -653,3 +653,78 @@ def test_second_derivatives_beside_another_path_to_the_same_input():
             # what has nothing to do with them is none of theirs
             z = torch.ones(3, device="cuda", requires_grad=True)
             assert torch.autograd.grad(g.float().sum() + (2 * z).sum(), z)[0].eq(2).all()
+
+
+# A forced tile is the calling thread's, and the autograd engine's threads are others: what follows
+# makes the backward passes' calls on this thread, and asks it for the plan that they take.
+
+def forced_plan(tile, slices, m, n, k, turned):
+    """The plan is the forced one: its tile, unless that layout has no such height, and its slices,
+    unless there are not as many stages of 64."""
+    rows, cols, got = streamk.product_plan(m, n, k, False, turned)
+    if tile[0] != 96 or turned != 2:
+        assert (rows, cols) == tile
+        assert got == slices or -(-k // 64) < slices
+    return True
+
+
+@gpu
+@pytest.mark.parametrize("slices", [1, 3])
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("m,n,k", [(1, 8, 64), (300, 520, 192), (257, 136, 1096), (130, 264, 128), (333, 304, 640)])
+def test_gradients_by_every_tile(tile, m, n, k, slices):
+    binding = streamk._torch_binding
+    for type in TYPES:
+        x, w, dh = make(m, n, k, type, 5)
+        ref = Gated64(x, w, "gelu")
+        try:
+            streamk.force_product_tile(*tile, slices)
+            assert forced_plan(tile, slices, m, k, 2 * n, 1) and forced_plan(tile, slices, 2 * n, k, m, 2)
+            assert forced_plan(tile, slices, m, k, n, 1) and forced_plan(tile, slices, n, k, m, 2)
+            h, sums = binding.gated_sums(x, w, 2)
+            dx, dw = binding.gated_grads(dh, sums, x, w, 2, True, True)
+            lx, lw = binding.linear_grads(dh, x, w[:n], True, True)
+        finally:
+            streamk.force_product_tile(0)
+        ref.check_forward(h, type)
+        ref.check_grads(dh, dx, dw, type)
+        check_product(lx, dh, w[:n].t(), type)
+        check_product(lw, dh.t(), x.t(), type)
+
+
+@gpu
+@pytest.mark.parametrize("slices", [1, 3])
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("tile,turned", [(t, turned) for t in TILES for turned in (0, 1, 2) if t[0] != 96 or turned != 2])
+def test_every_tile_beside_rows_that_hold_nan(tile, turned, type, slices):
+    """Matrices inside larger ones, as above, by every tile, in both types, whole and in slices."""
+    import ctypes
+    lib, L, P = streamk._lib, ctypes.c_longlong, ctypes.c_void_p
+    for m, n, k in ((72, 200, 136), (328, 264, 320), (264, 520, 456)):
+        gen = torch.Generator(device="cuda").manual_seed(m)
+        a, b = (torch.randn(r, k, device="cuda", generator=gen).to(type) for r in (m, n))
+
+        def inside(x):
+            rows, cols = x.shape
+            room = torch.full((rows + 80, cols + 96), float("nan"), dtype=type, device="cuda")
+            room[8:8 + rows, 16:16 + cols] = x
+            return room, room[8:8 + rows, 16:16 + cols]
+
+        ra, va = inside(a.t().contiguous() if turned == 2 else a)
+        rb, vb = inside(b.t().contiguous() if turned else b)
+        rc, vc = inside(torch.zeros(m, n, device="cuda").to(type))
+        before = rc.clone()
+        room = torch.empty(3 * m * n, device="cuda")
+        try:
+            streamk.force_product_tile(*tile, slices)
+            assert forced_plan(tile, slices, m, n, k, turned)
+            code = lib.feedforward_product(P(va.data_ptr()), P(vb.data_ptr()), P(vc.data_ptr()), m, n, k, L(va.stride(0)),
+                                           L(vb.stride(0)), L(vc.stride(0)), turned, int(type == torch.bfloat16),
+                                           P(room.data_ptr()), L(4 * room.numel()), 0,
+                                           P(torch.cuda.current_stream().cuda_stream))
+        finally:
+            streamk.force_product_tile(0)
+        assert code == 0
+        check_product(vc, a, b, type)
+        vc.copy_(before[8:8 + m, 16:16 + n])
+        assert torch.equal(rc.isnan(), before.isnan()) and not rc.nan_to_num().any()  # nothing else was written
