@@ -219,8 +219,8 @@ bool enqueue_gated(const at::Tensor& A, const at::Tensor& B, const at::Tensor& C
       PyErr_Format(PyExc_ValueError, "%s must be of type torch.%s", kMulNames[i], whole ? "int32" : "half");
       return false;
     }
-    if (t[i]->device() != A.device()) {
-      PyErr_Format(PyExc_ValueError, "%s must be on A's device", kMulNames[i]);
+    if (t[i]->device() != A.device() || t[i]->is_neg()) {
+      PyErr_Format(PyExc_ValueError, "%s must be a plain tensor on A's device", kMulNames[i]);
       return false;
     }
   }
@@ -405,6 +405,9 @@ struct Matrix {
   void* at() const { return t.data_ptr(); }
 };
 
+// a gradient whose memory holds its values: autograd may hand over a view that is to be read negated
+at::Tensor plain_values(const at::Tensor& grad) { return grad.defined() ? grad.resolve_neg() : grad; }
+
 void feedforward_check(int rc) {
   TORCH_CHECK_VALUE(rc != FEEDFORWARD_ERR_SHAPE, feedforward_last_error());
   TORCH_CHECK(rc == FEEDFORWARD_OK, feedforward_last_error());
@@ -556,7 +559,7 @@ std::pair<at::Tensor, at::Tensor> gated_backward(const at::Tensor& dh, const at:
     if (want_w) dw.zero_();
   } else if (want_x || want_w) {
     const int64_t ld = (2 * n + 63) / 64 * 64;  // rows of whole cache lines
-    const Matrix d(dh, m, n), dgu(empty_as(x, {m, ld}), m, ld);
+    const Matrix d(plain_values(dh), m, n), dgu(empty_as(x, {m, ld}), m, ld);
     feedforward_check(feedforward_gated_grad(d.at(), (const float*)pre.data_ptr(), dgu.at(), (int)m, (int)n, d.ld,
                                              ldpre, ld, type_code(x), act, dev, current_stream(dev)));
     product_grads(x, w, dgu, dx, dw);
@@ -580,7 +583,7 @@ std::pair<at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy, const at
     if (want_x) dx.zero_();
     if (want_w) dw.zero_();
   } else if (want_x || want_w) {
-    product_grads(x, w, Matrix(dy, m, n), dx, dw);
+    product_grads(x, w, Matrix(plain_values(dy), m, n), dx, dw);
   }
   return {dx, dw};
 }
@@ -853,7 +856,7 @@ std::array<at::Tensor, 5> norm_backward(const at::Tensor& dy, const at::Tensor& 
     bytes = feedforward_norm_grad_bytes(in.rows, (int)in.d, (int)in.rows_per_gate, norm_code(in.residual));
     if (bytes > 0) partials = at::empty({bytes / 4}, options_as(in.residual).dtype(at::kFloat));
   }
-  const Rows gdy(back ? dy : at::Tensor(), in.rows, in.d), gdr(dr, in.rows, in.d), r(in.residual, in.rows, in.d),
+  const Rows gdy(back ? plain_values(dy) : at::Tensor(), in.rows, in.d), gdr(plain_values(dr), in.rows, in.d), r(in.residual, in.rows, in.d),
       block(in.block, in.rows, in.d), gate = in.gate_rows();
   const at::Tensor post = weight_of(in.post), pre = back ? weight_of(in.pre) : at::Tensor();
   feedforward_check(feedforward_norm_grad(

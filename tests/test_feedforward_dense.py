@@ -728,3 +728,15 @@ def test_every_tile_beside_rows_that_hold_nan(tile, turned, type, slices):
         check_product(vc, a, b, type)
         vc.copy_(before[8:8 + m, 16:16 + n])
         assert torch.equal(rc.isnan(), before.isnan()) and not rc.nan_to_num().any()  # nothing else was written
+
+
+@gpu
+def test_gradients_that_are_views_to_be_read_negated():
+    x, w, dh = make(20, 16, 32, torch.float16, 0)
+    leaves = [t.requires_grad_() for t in (x, w)]
+    for call in (streamk.gated, streamk.linear):
+        h = call(x, w)
+        dh = torch.randn_like(h)
+        want = torch.autograd.grad(h, leaves, dh, retain_graph=True)
+        got = torch.autograd.grad(h, leaves, torch._neg_view(-dh))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

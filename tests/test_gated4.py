@@ -389,3 +389,13 @@ def test_as_many_rows_as_make_two_gib_of_results():
     y = layer(x)
     for first in (0, 37440, m - 200):
         check(y[first:first + 200], x[first:first + 200], q, s, "silu")
+
+
+@gpu
+def test_views_to_be_read_negated():
+    x, q, s, fake = problem(2, 128, 256, -1, dev="cuda")
+    layer = layer_of(q, s, fake, -1, "silu")
+    C = torch.empty((2, 128), dtype=torch.half, device="cuda")
+    for call in (layer, lambda a: marlin.gated_mul(a, layer.B, C, layer.s, layer.workspace)):
+        with pytest.raises(ValueError, match="plain tensor"):
+            call(torch._neg_view(x))

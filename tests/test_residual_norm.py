@@ -722,3 +722,18 @@ def test_the_entries_take_one_scale_for_both_passes():
                                          at(w), D(scale), at(stats), at(dx), None, None, None, None, None, L(0), L(rows),
                                          I(d), I(2), I(0), stream) == 0
         assert torch.equal(y, want_y) and torch.equal(dx, want), scale
+
+
+@gpu
+def test_gradients_that_are_views_to_be_read_negated():
+    """As the imaginary part of a conjugate is, and what autograd makes of one."""
+    for d in (1, 64):
+        t, dy, dr = make((5, d), torch.float32, "channel", 4)
+        v = leaves(t)
+        outs = run(v)
+        negated = [torch.imag(torch.complex(torch.zeros_like(g), -g).conj()) for g in (dy, dr)]
+        assert all(n.is_neg() and torch.equal(n, g) for n, g in zip(negated, (dy, dr)))
+        want = torch.autograd.grad(outs, list(v.values()), (dy, dr), retain_graph=True)
+        for grads in (negated, [torch._neg_view(-g) for g in (dy, dr)]):
+            got = torch.autograd.grad(outs, list(v.values()), grads, retain_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
