@@ -221,7 +221,7 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
     for (int i = 0; i < RB; i++)
 #pragma unroll
       for (int o = 0; o < 8; o++)
-        put_part<GATED>(p, at.slice, m0 + 16 * RB * wm + 16 * i + nu, n0 + 128 * wn + 16 * o + 4 * kg, p.M, columns,
+        put_part(p, at.slice, m0 + 16 * RB * wm + 16 * i + nu, n0 + 128 * wn + 16 * o + 4 * kg, p.M, columns,
                         acc[i][o]);
     return;
   }

@@ -18,10 +18,10 @@
 //
 // Bound: HBM; every row is read and written once.  8192 rows of 8192 in bfloat16 105 us, 5.1 TB/s;
 // 4096 rows of 4096 26 us and backward 45, 4.5 TB/s, and 6 for the sums over parts; one row 3.6.
-// A row is kept in the registers of W waves, one or two 16-byte pieces a lane, so that the second
-// pass over it that a norm needs costs nothing; the waves' sums meet in LDS, two meetings a row
-// forward.  Backward one: mean(w bh) is put together from four sums, of dy pre rh, and of gate post
-// bh times dr, dy pre and rh.
+// A row is kept in the registers of W waves, a 16-byte piece a lane, of the longest rows two or (fp32)
+// four, so that the second pass over it that a norm needs costs nothing; the waves' sums meet in
+// LDS, two meetings a row forward.  Backward one: mean(w bh) is put together from four sums, of dy
+// pre rh, and of gate post bh times dr, dy pre and rh.
 //
 // Sums over rows: every part (a run of rows) adds up its own in registers, in the order of its
 // rows, and leaves them in memory; a second launch adds the parts in their order.  No atomics,

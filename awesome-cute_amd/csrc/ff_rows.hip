@@ -32,7 +32,6 @@ template <int S, int MB, int DEPTH>
 struct FewShape {
   static constexpr int kLoads = 2 * (S + MB);  // of 1 KiB per wave and chunk
   static constexpr int kSlot = 1024 * kLoads;
-  static constexpr int kOps = 2 * (S + MB);
   static constexpr int kRing = kFewWaves * DEPTH * kSlot;
   static constexpr int kReduce = kFewWaves * S * MB * 1024;
   static constexpr int kLds = kRing > kReduce ? kRing : kReduce;

@@ -90,7 +90,6 @@ __device__ __forceinline__ void put(const ProductArgs& p, char* row, int m0, int
   }
 }
 // ... and of a slice: the sums as they are (columns in the product's order)
-template <bool GATED>
 __device__ __forceinline__ void put_part(const ProductArgs& p, int slice, int m, int col, int rows_end, int cols_end,
                                          f4 v) {
   if (m < rows_end && col < cols_end)

@@ -31,7 +31,6 @@ template <int TM, int TN, int WM, int WN, int RING, bool GATED>
 struct FfShape {
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
   static constexpr int kRB = TM / 16 / WM, kNJ = TN / 16 / WN;  // operands of a wave per k step
-  static constexpr int kOps = 2 * (kRB + kNJ);                  // ... per stage
   static constexpr int kTA = (TM / 8 + kWaves - 1) / kWaves, kTB = TN / 8 / kWaves;  // loads per wave and slab
   static constexpr int kSlabA = kTA * kWaves * 1024, kSlab = kSlabA + TN * 128;
   static constexpr int kLoads = kTA + kTB;
@@ -299,7 +298,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
     for (int i = 0; i < RB; i++)
 #pragma unroll
       for (int j = 0; j < NJ; j++)
-        put_part<GATED>(p, at.slice, m0 + 16 * RB * wm + 16 * i + nu, n0 + 16 * NJ * wn + 16 * j + 4 * kg, p.M, columns,
+        put_part(p, at.slice, m0 + 16 * RB * wm + 16 * i + nu, n0 + 16 * NJ * wn + 16 * j + 4 * kg, p.M, columns,
                         acc[i][j]);
     return;
   }

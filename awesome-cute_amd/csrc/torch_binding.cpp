@@ -876,8 +876,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     NormInputs in{residual, block.value_or(at::Tensor()), post.value_or(at::Tensor()), gate.value_or(at::Tensor()),
                   pre.value_or(at::Tensor())};
     const NormOutputs out = norm_forward(in, scale, eps, true);
-    // (with a block the backward pass takes r, and of the residual, where that is a leaf, no values:
-    // it may be overwritten, and its memory go)
+    // (with a block the backward pass takes r and no values of the residual: it may be overwritten, and
+    // where it is no leaf -- a leaf's accumulator, which the graph holds, holds the leaf --, go)
     ctx->save_for_backward({in.block.defined() ? out.r : residual, in.block, in.post, in.gate, in.pre, out.lengths});
     if (residual.is_leaf() && residual.requires_grad()) ctx->saved_data["leaf"] = residual;
     // (without a block the residual itself is what the norm took, and it is not multiplied)

@@ -10,7 +10,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-from native import lib as _lib, torch_binding as _torch_binding
+from native import ACTIVATIONS, activation as _activation, lib as _lib, torch_binding as _torch_binding  # noqa: F401
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -104,16 +104,6 @@ def _mul_op(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, s: torch.Tensor,
 @_mul_op.register_fake
 def _mul_fake(A, B, C, s, workspace, thread_k, thread_n, sms, max_par, cute_version):
     return None
-
-
-ACTIVATIONS = {"silu": 1, "gelu": 2}  # (gelu in its tanh form)
-
-
-def _activation(name):
-    try:
-        return ACTIVATIONS[name]
-    except (KeyError, TypeError):
-        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}") from None
 
 
 def _wants_gradients(t):

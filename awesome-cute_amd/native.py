@@ -30,3 +30,13 @@ def _binding():
 
 lib = ctypes.CDLL(_path("libmarlin_amd.so"))
 torch_binding = _binding()
+
+ACTIVATIONS = {"silu": 1, "gelu": 2}  # of gated projections (gelu in its tanh form)
+
+
+def activation(name):
+    """The library's number of an activation."""
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}") from None

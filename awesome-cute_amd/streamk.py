@@ -10,7 +10,7 @@ import ctypes
 
 import torch
 
-from native import lib as _lib, torch_binding as _torch_binding
+from native import ACTIVATIONS, activation as _activation, lib as _lib, torch_binding as _torch_binding  # noqa: F401
 
 _P, _I = ctypes.c_void_p, ctypes.c_int
 _lib.streamk_amd_check.restype = _I
@@ -116,19 +116,11 @@ def _gemm_fake(A, B, C):
 # costs more host time than a product of a few rows takes; else the binding's, which is an autograd
 # function where gradients are wanted.  (An argument more: the call is an operator's own.)
 
-ACTIVATIONS = {"silu": 1, "gelu": 2}  # (gelu in its tanh form)
 _lib.feedforward_plan.restype = _I
 _lib.feedforward_plan.argtypes = [_I, _I, _I, _I, _I, _I, _P]
 _lib.feedforward_force_tile.restype = None
 _lib.feedforward_force_tile.argtypes = [_I, _I, _I]
 _lib.feedforward_last_error.restype = ctypes.c_char_p
-
-
-def _activation(name):
-    try:
-        return ACTIVATIONS[name]
-    except (KeyError, TypeError):
-        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}") from None
 
 
 def gated(x, weight, activation="silu"):
