@@ -4,10 +4,11 @@
 //
 // Bound: how evenly the tiles fill the compute units, hence the heights (777 x 2 x 5208 x 4160: 164
 // tiles of 256 rows, 205 of 160), some 12 us of a tile outside its loop (the first slabs' way, and
-// results that all compute units write at once), and in the loop the board's power.  bfloat16, us
-// and TFLOP/s: 2048 x 2 x 10752 x 4096 284, 1270 (with the sums kept 314); its backward pass 2048 x
-// 4096 x 21504 272, 1320 and 21504 x 4096 x 2048 310, 1160; 8192 x 4096 x 4096 204, 1350.  The matrix
-// pipe is in use for 58 to 72 % of these.  Results past the caches or through them: level.
+// results that all compute units write at once), and in the loop the board's power.  bfloat16, operands
+// from memory, us and TFLOP/s: 2048 x 2 x 10752 x 4096 296, 1220 (with the sums kept 313); its backward
+// pass 2048 x 4096 x 21504 277, 1300, of which 14 the slices' sums, and 21504 x 4096 x 2048 307, 1170;
+// 8192 x 4096 x 4096 205, 1340.  The matrix pipe is in use for 57 to 72 % of these.  Results past the
+// caches or through them: level.
 #include <hip/hip_runtime.h>
 
 #include "ff_tile.hpp"

@@ -71,10 +71,11 @@ int on_device(int dev, F launch) {
 // Costs of the tiles in us, as in f16_tiles.hip: a launch, a stage of 64 k-values (dearer the
 // fuller the chip), and workgroups beyond one per compute unit.  Fitted to every tile that can
 // compute them on 9000 problems, m = 16 ... 8192, widths of 64 to 22016, forward and of the
-// backward pass, operands from memory; 5 to 12 % rms.  On 5000 others the choice takes 1.014 of the
-// best tile and slices measured, 1.19 at the 99th percentile and 1.5 at worst.  Without any one
-// of the tiles it would be 1.015 to 1.025, without that of 64 x 64 1.107; without slices 1.140.
-// Sixteen slices gain 0.15 % where known, and lose as much by the fit.
+// backward pass, operands from memory; 5 to 12 % rms (before big tiles took every depth, and before
+// one tile's weights were requested as read once).  On 8600 others, with the kernels as they are, the
+// choice takes 1.012 of the best tile and slices measured, 1.20 at the 99th percentile and 1.85 at
+// worst.  Without any one of the tiles it would be 1.014 to 1.023, without that of 64 x 64 1.116;
+// without slices 1.147.  Sixteen slices gain 0.15 % where known, and lose as much by the fit.
 struct TileFit {
   FfTile tile;
   double launch, stage, fill, more, more_stage;
@@ -88,10 +89,11 @@ constexpr TileFit kFits[] = {
 // The same of the kernel for few rows (ff_rows.hip) by its blocks of sixteen rows of A, a stage
 // being the 64 k-values of one of its four waves: one block of product columns to a workgroup, or
 // two.  Fitted to 12000 problems of 1 to 64 rows, widths of 64 to 14336, depths of 64 to 8192,
-// weights from memory.  On 8000 others the choice among these and the tiles takes 1.06, 1.07, 1.05
-// and 1.03 of the best of 25 variants measured, 1.02 to 1.07 above 16 us, much of it the measurements'
-// scatter.  Without tiles it takes 1.06, 1.08, 1.09 and 1.11; one block alone 1.07, 1.07, 1.055,
-// 1.04; four blocks, or other depths, gain less than 0.003.
+// weights from memory.  On 22000 others, with the kernels as they are, the choice among these and the
+// tiles takes by blocks of rows 1.020, 1.022, 1.017 and 1.012 of the best measured (the better of two
+// timings each), 1.18 at the 99th percentile and 1.5 at worst.  Without tiles it takes 1.019, 1.054,
+// 1.098 and 1.169; one block alone 1.033, 1.032, 1.028 and 1.021; four blocks, or other depths, gain
+// less than 0.003.
 constexpr TileFit kFewFits[] = {
     {{16, 16}, 4.36, 0.128, 0.078, 0.0, 0.335},  {{16, 32}, 4.13, 0.264, 0.231, 0.0, 0.594},
     {{32, 16}, 4.17, 0.270, 0.084, 0.0, 0.471},  {{32, 32}, 4.06, 0.381, 0.281, 0.0, 0.822},

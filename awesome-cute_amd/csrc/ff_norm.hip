@@ -16,8 +16,10 @@
 //
 // the sums over the rows that share a weight or a gate.
 //
-// Bound: HBM; every row is read and written once.  8192 rows of 8192 in bfloat16 105 us, 5.1 TB/s;
-// 4096 rows of 4096 26 us and backward 45, 4.5 TB/s, and 6 for the sums over parts; one row 3.6.
+// Bound: HBM; every row is read and written once.  8192 rows of 8192 in bfloat16 110 us, 4.9 TB/s, by
+// one norm alone 48, 5.6; 4096 rows of 4096 26 us and backward 45, 4.5 TB/s, and 6 for the sums over
+// parts; one row 3.7.  A wave is the least that takes a row: of 64 elements in 16 bits eight lanes
+// hold some, and 262144 such rows take 99 us, 1.4 TB/s.
 // A row is kept in the registers of W waves, a 16-byte piece a lane, of the longest rows two or (fp32)
 // four, so that the second pass over it that a norm needs costs nothing; the waves' sums meet in
 // LDS, two meetings a row forward.  Backward one: mean(w bh) is put together from four sums, of dy

@@ -71,9 +71,9 @@ __device__ __forceinline__ void store_rows(const ProductArgs& p, const char* sme
 // What a lane puts into row `m` of the tile's LDS image, of operands j and (gated) j + 1 of a
 // row block: their sums at column `col` of the product's tile.  The sums that the backward pass
 // takes go to memory from here, in fp32 -- rounded to 16 bits they made the gradients 1.8
-// times as far off as the products' own roundings do; they cost 30 us of a forward pass of 314
-// (2048 x 2 x 10752 x 4096) and some 15 of a backward pass -- and in the product's order, in which a gate's sixteen
-// columns and its partner's fill a cache line of a row.
+// times as far off as the products' own roundings do; they cost 17 us of a forward pass of 313 (2048
+// x 2 x 10752 x 4096) and some 15 of a backward pass -- and in the product's order, in which a
+// gate's sixteen columns and its partner's fill a cache line of a row.
 template <int COLS, bool GATED, bool BF>
 __device__ __forceinline__ void put(const ProductArgs& p, char* row, int m0, int n0, int m, int col, int rows, int cols,
                                     f4 v, f4 next) {
