@@ -32,6 +32,7 @@ SOURCES = {
     "ff_big.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ff_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "ff_grads.hip": [],
+    "ff_dropout.hip": [],
     "ff_norm.hip": [],
     "ff_host.hip": [],
 }

@@ -34,8 +34,9 @@ struct BigShape {
 
 }  // namespace
 
-template <bool BF, bool GATED, Layout LAYOUT, int RB>
+template <bool BF, Finish FINISH, Layout LAYOUT, int RB>
 __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
+  constexpr bool GATED = FINISH == kGated;
   using Sh = BigShape<RB, LAYOUT>;
   extern __shared__ __attribute__((aligned(16))) char smem[];  // Sh::kLds
   constexpr int TA = Sh::kTA, TB = Sh::kTB, TM = Sh::kTM;
@@ -230,18 +231,46 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
   // LDS while the first is on its way to memory.
   constexpr int kPitch = out_pitch<256, GATED>(), kHalf = Sh::kHalf;
   constexpr bool kBoth = 64 * kHalf * kPitch <= Sh::kLds;
+  const DropKey key(p.drop);
+  const int col0 = 128 * wn + 4 * kg;
+  i2 bias[8];
+  if (FINISH == kFull && p.bias)
+#pragma unroll
+    for (int o = 0; o < 8; o++) bias[o] = full_bias(p, n0, col0 + 16 * o, cols);
 #pragma unroll
   for (int half = 0; half < 2; half++) {
     char* const base = smem + (kBoth ? half * 32 * kHalf * kPitch : 0);
     if (half == 0 || !kBoth) __syncthreads();  // (nothing is on its way into LDS, and nobody reads it)
+    if constexpr (FINISH == kFull) {
+      i2 residual[kHalf][8];
+      if (p.residual)
 #pragma unroll
-    for (int i = 0; i < kHalf; i++) {
-      if (kHalf * half + i >= RB) continue;
+        for (int i = 0; i < kHalf; i++)
 #pragma unroll
-      for (int o = 0; o < 8; o += GATED ? 2 : 1)
-        put<256, GATED, BF>(p, base + (16 * kHalf * wm + 16 * i + nu) * kPitch, m0, n0,
-                            16 * RB * wm + 16 * (kHalf * half + i) + nu, 128 * wn + 16 * o + 4 * kg, rows, cols,
-                            acc[(kHalf * half + i) % RB][o], acc[(kHalf * half + i) % RB][GATED ? o + 1 : o]);
+          for (int o = 0; o < 8; o++)
+            if (kHalf * half + i < RB)
+              residual[i][o] =
+                  full_residual(p, m0, n0, 16 * RB * wm + 16 * (kHalf * half + i) + nu, col0 + 16 * o, rows, cols);
+#pragma unroll
+      for (int i = 0; i < kHalf; i++) {
+        if (kHalf * half + i >= RB) continue;
+#pragma unroll
+        for (int o = 0; o < 8; o += 2)
+          put_full<BF>(p, key, base + (16 * kHalf * wm + 16 * i + nu) * kPitch, m0, n0,
+                       16 * RB * wm + 16 * (kHalf * half + i) + nu, col0 + 16 * o, kg, rows, cols, bias + o,
+                       residual[i] + o, acc[(kHalf * half + i) % RB][o], acc[(kHalf * half + i) % RB][o + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kHalf; i++) {
+        if (kHalf * half + i >= RB) continue;
+#pragma unroll
+        for (int o = 0; o < 8; o += GATED ? 2 : 1)
+          put<256, GATED, BF>(p, base + (16 * kHalf * wm + 16 * i + nu) * kPitch, m0, n0,
+                              16 * RB * wm + 16 * (kHalf * half + i) + nu, 128 * wn + 16 * o + 4 * kg, rows, cols,
+                              acc[(kHalf * half + i) % RB][o],
+                              acc[(kHalf * half + i) % RB][GATED ? o + 1 : o]);
+      }
     }
     __syncthreads();
     store_rows<32 * kHalf, 256, GATED, 256>(p, base, m0, GATED ? n0 >> 1 : n0, rows, cols, [&](int r) {
@@ -254,19 +283,24 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
 namespace {
 
 // calls f(kernel, LDS bytes) for a height, a layout and a type
-template <bool BF, bool GATED, Layout LAYOUT, class F>
+template <bool BF, Finish FINISH, Layout LAYOUT, class F>
 void with_height(int rows, F f) {
-  if (rows == 256) f(product_big_kernel<BF, GATED, LAYOUT, 8>, BigShape<8, LAYOUT>::kLds);
-  if (rows == 224) f(product_big_kernel<BF, GATED, LAYOUT, 7>, BigShape<7, LAYOUT>::kLds);
-  if (rows == 192) f(product_big_kernel<BF, GATED, LAYOUT, 6>, BigShape<6, LAYOUT>::kLds);
-  if (rows == 160) f(product_big_kernel<BF, GATED, LAYOUT, 5>, BigShape<5, LAYOUT>::kLds);
+  if (rows == 256) f(product_big_kernel<BF, FINISH, LAYOUT, 8>, BigShape<8, LAYOUT>::kLds);
+  if (rows == 224) f(product_big_kernel<BF, FINISH, LAYOUT, 7>, BigShape<7, LAYOUT>::kLds);
+  if (rows == 192) f(product_big_kernel<BF, FINISH, LAYOUT, 6>, BigShape<6, LAYOUT>::kLds);
+  if (rows == 160) f(product_big_kernel<BF, FINISH, LAYOUT, 5>, BigShape<5, LAYOUT>::kLds);
+}
+template <bool BF, class F>
+void with_finish(int rows, Finish finish, Layout layout, F f) {
+  if (finish == kGated) return with_height<BF, kGated, kRows>(rows, f);
+  if (finish == kFull) return with_height<BF, kFull, kRows>(rows, f);
+  if (layout == kRows) return with_height<BF, kPlain, kRows>(rows, f);
+  if (layout == kTurnB) return with_height<BF, kPlain, kTurnB>(rows, f);
+  return with_height<BF, kPlain, kTurnBoth>(rows, f);
 }
 template <class F>
-void with_big(int rows, bool gated, Layout layout, bool bf, F f) {
-  if (gated) return bf ? with_height<true, true, kRows>(rows, f) : with_height<false, true, kRows>(rows, f);
-  if (layout == kRows) return bf ? with_height<true, false, kRows>(rows, f) : with_height<false, false, kRows>(rows, f);
-  if (layout == kTurnB) return bf ? with_height<true, false, kTurnB>(rows, f) : with_height<false, false, kTurnB>(rows, f);
-  return bf ? with_height<true, false, kTurnBoth>(rows, f) : with_height<false, false, kTurnBoth>(rows, f);
+void with_big(int rows, Finish finish, Layout layout, bool bf, F f) {
+  bf ? with_finish<true>(rows, finish, layout, f) : with_finish<false>(rows, finish, layout, f);
 }
 
 }  // namespace
@@ -275,8 +309,8 @@ hipError_t configure_product_big() {
   hipError_t e = hipSuccess;
   for (const int rows : {160, 192, 224, 256})
     for (const bool bf : {false, true})
-      for (const int form : {0, 1, 2, 3})
-        with_big(rows, form == 3, form == 3 ? kRows : (Layout)form, bf, [&](auto kernel, int lds) {
+      for (const int form : {0, 1, 2, 3, 4})
+        with_big(rows, form > 2 ? (Finish)(form - 2) : kPlain, form > 2 ? kRows : (Layout)form, bf, [&](auto kernel, int lds) {
           if (e == hipSuccess)
             e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         });
@@ -284,10 +318,9 @@ hipError_t configure_product_big() {
 }
 
 void launch_product_big(ProductArgs a, int rows, Layout layout, bool bf, hipStream_t stream) {
-  const bool gated = a.act != kActNone;
   a.tiles_m = ceil_div(a.M, rows);
-  a.tiles_n = ceil_div(product_columns(a.N, gated), 256);
-  with_big(rows, gated, layout, bf, [&](auto kernel, int lds) {
+  a.tiles_n = ceil_div(product_columns(a.N, a.finish == kGated), 256);
+  with_big(rows, a.finish, layout, bf, [&](auto kernel, int lds) {
     hipLaunchKernelGGL(kernel, dim3(a.tiles_m * a.tiles_n * a.slices), dim3(256), lds, stream, a);
   });
 }

@@ -1,25 +1,23 @@
-// What stands between the products of a gated projection's backward pass: the gradients of its
+// What stands between the products of a backward pass.
+//
+// Of a gated projection: the gradients of its
 // two sums, dg = dh u act'(g) and du = dh act(g), in fp32 from the sums that the forward pass
 // kept in fp32, rounded to 16 bits, as matrix instructions take them.  Rows of [dg | du]: both
-// products of the backward pass read them as they are (ff_tile.hpp).
+// products of the backward pass read them as they are (ff_tile.hpp).  Bound: HBM: 14 bytes for every element of dh.  2048 x 10752: 308 MB, 48 us, 6.4 TB/s.
 //
-// Bound: HBM: 14 bytes for every element of dh.  2048 x 10752: 308 MB, 48 us, 6.4 TB/s.
+// Of a full product, y = residual + drop(act(z)) with z = x W^T + bias: dz = drop(dy) act'(z), rounded to
+// 16 bits for the products, and the bias's gradient, its sum over rows, of the unrounded values in
+// fp32.  A workgroup takes 256 columns (fewer where there are fewer) of a run of rows, 16 bytes a
+// thread; its column sums meet in LDS and go to `partials`, and a second launch adds the runs' in their
+// order.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "ff_grads.hpp"
 #include "ff_products.hpp"
 
 namespace w4a16 {
-
-namespace {
-
-template <bool BF>
-__device__ __forceinline__ float widen(unsigned bits) {
-  if constexpr (BF) return __builtin_bit_cast(float, bits << 16);
-  return (float)__builtin_bit_cast(half_t, (unsigned short)bits);
-}
-
-}  // namespace
 
 // eight columns of a row a thread
 template <bool BF>
@@ -35,14 +33,14 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradArgs p) {
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
     const f4 g = *(const f4*)(pre + 2 * i), u = *(const f4*)(pre + 2 * i + 16);
+    const f4 d = widen4<BF>((i2){dh[i], dh[i + 1]});
     f4 a, b;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float d = widen<BF>((unsigned)dh[i + (e >> 1)] >> (16 * (e & 1)) & 0xffffu);
       float value, slope;
       act_slope(g[e], p.act, &value, &slope);
-      a[e] = d * u[e] * slope;
-      b[e] = d * value;
+      a[e] = d[e] * u[e] * slope;
+      b[e] = d[e] * value;
     }
     const i2 ra = product_round<BF>(a), rb = product_round<BF>(b);
     dg[i] = ra[0];
@@ -60,6 +58,125 @@ void launch_gated_grad(const GatedGradArgs& a, bool bf, hipStream_t stream) {
     hipLaunchKernelGGL(gated_grad_kernel<true>, grid, dim3(256), 0, stream, a);
   else
     hipLaunchKernelGGL(gated_grad_kernel<false>, grid, dim3(256), 0, stream, a);
+}
+
+namespace {
+
+constexpr int kRunThreads = 256;
+constexpr int kRunGroups = 2048;  // workgroups that the runs make up, eight to a compute unit
+constexpr int kRunRows = 4;       // ... rows that a thread has at least
+
+// threads beside each other along a row, eight columns each
+__host__ __device__ __forceinline__ int run_width(int n) {
+  int width = 32;
+  while (width > 1 && 4 * width >= n) width /= 2;
+  return width;
+}
+
+}  // namespace
+
+template <bool BF>
+__global__ __launch_bounds__(kRunThreads) void linear_grad_kernel(LinearGradArgs p) {
+  __shared__ float room[kRunThreads][8 + 1];
+  const int width = run_width(p.n), high = kRunThreads / width;
+  const int c = threadIdx.x % width, r0 = threadIdx.x / width;
+  const int col = 8 * ((int)blockIdx.x * width + c);
+  const bool in = col < p.n;
+  const int part = blockIdx.y;
+  const long long first = (long long)part * p.rows_per_part;
+  const long long end = min(first + p.rows_per_part, (long long)p.m);
+  const DropKey key(p.drop);
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (in) {
+#pragma unroll 2
+    for (long long r = first + r0; r < end; r += high) {
+      const i4 dy = *(const i4*)((const half_t*)p.dy + (size_t)r * p.lddy + col);
+      f4 z[2];
+      if (p.pre) {
+        z[0] = *(const f4*)(p.pre + (size_t)r * p.ldpre + col);
+        z[1] = *(const f4*)(p.pre + (size_t)r * p.ldpre + col + 4);
+      }
+      i4 bits;
+      if (p.drop.below) bits = drop_bits((unsigned long long)r * (unsigned)(p.n >> 3) + (unsigned)(col >> 3), key);
+      i4 dz;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        f4 d = widen4<BF>((i2){dy[2 * h], dy[2 * h + 1]});
+        if (p.pre)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            float value, slope;
+            act_slope(z[h][e], p.act, &value, &slope);
+            d[e] *= slope;
+          }
+        // (last: what is dropped has no gradient, whatever its slope)
+        if (p.drop.below) d = drop4(d, (i2){bits[2 * h], bits[2 * h + 1]}, p.drop);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[4 * h + e] += d[e];
+        const i2 rounded = product_round<BF>(d);
+        dz[2 * h] = rounded[0];
+        dz[2 * h + 1] = rounded[1];
+      }
+      if (p.dz) *(i4*)((half_t*)p.dz + (size_t)r * p.lddz + col) = dz;
+    }
+  }
+  if (!p.partials) return;
+#pragma unroll
+  for (int e = 0; e < 8; e++) room[threadIdx.x][e] = sum[e];
+  __syncthreads();
+  // a thread a column, the rows' sums in their order
+  for (int at = threadIdx.x; at < 8 * width; at += kRunThreads) {
+    const int column = 8 * (int)blockIdx.x * width + at;
+    if (column >= p.n) continue;
+    float s = room[at / 8][at % 8];
+    for (int r = 1; r < high; r++) s += room[r * width + at / 8][at % 8];
+    p.partials[(size_t)part * p.n + column] = s;
+  }
+}
+
+// the runs' sums: 64 columns and 16 waves a workgroup, a wave every sixteenth run
+template <bool BF>
+__global__ __launch_bounds__(1024) void bias_sums_kernel(LinearGradArgs p, int parts) {
+  __shared__ float room[16][64];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = 64 * blockIdx.x + lane;
+  const float* const from = p.partials + (c < p.n ? c : 0);
+  float s = 0.f;
+#pragma unroll 8
+  for (int i = wave; i < parts; i += 16) s += from[(size_t)i * p.n];
+  room[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || c >= p.n) return;
+  s = room[0][lane];
+#pragma unroll
+  for (int i = 1; i < 16; i++) s += room[i][lane];
+  if constexpr (BF)
+    ((__bf16*)p.dbias)[c] = (__bf16)s;
+  else
+    ((half_t*)p.dbias)[c] = (half_t)s;
+}
+
+int linear_grad_parts(int m, int n) {
+  const int width = run_width(n), across = ceil_div(n, 8 * width), high = kRunThreads / width;
+  const int most = std::max(1, kRunGroups / across);
+  return std::max(1, std::min(most, ceil_div(m, kRunRows * high)));
+}
+
+void launch_linear_grad(LinearGradArgs a, bool bf, hipStream_t stream) {
+  const int width = run_width(a.n);
+  int parts = linear_grad_parts(a.m, a.n);
+  a.rows_per_part = ceil_div(a.m, parts);
+  parts = ceil_div(a.m, a.rows_per_part);
+  const dim3 grid(ceil_div(a.n, 8 * width), parts), sums(ceil_div(a.n, 64));
+  if (bf)
+    hipLaunchKernelGGL(linear_grad_kernel<true>, grid, dim3(kRunThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL(linear_grad_kernel<false>, grid, dim3(kRunThreads), 0, stream, a);
+  if (!a.partials) return;
+  if (bf)
+    hipLaunchKernelGGL(bias_sums_kernel<true>, sums, dim3(1024), 0, stream, a, parts);
+  else
+    hipLaunchKernelGGL(bias_sums_kernel<false>, sums, dim3(1024), 0, stream, a, parts);
 }
 
 }  // namespace w4a16

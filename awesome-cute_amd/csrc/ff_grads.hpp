@@ -2,6 +2,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include "dropout.hpp"
+
 namespace w4a16 {
 
 struct GatedGradArgs {
@@ -12,5 +14,28 @@ struct GatedGradArgs {
   int m, n, act;
 };
 void launch_gated_grad(const GatedGradArgs& a, bool bf, hipStream_t stream);
+
+struct LinearGradArgs {
+  const void* dy;    // (m x n)
+  const float* pre;  // null (no activation), or the forward pass's sums (m x ldpre)
+  void* dz;          // null, or (m x n)
+  void* dbias;       // n elements, with partials
+  float* partials;   // null, or linear_grad_parts(m, n) rows of n
+  long long lddy, ldpre, lddz;
+  int m, n, act, rows_per_part;
+  DropArgs drop;
+};
+int linear_grad_parts(int m, int n);
+void launch_linear_grad(LinearGradArgs a, bool bf, hipStream_t stream);
+
+// y = residual (or null) + drop(x), `count` elements that lie as one row
+struct DropoutArgs {
+  const void* x;
+  const void* residual;
+  void* y;
+  long long count;
+  DropArgs drop;
+};
+void launch_dropout(const DropoutArgs& a, int type, hipStream_t stream);  // FEEDFORWARD_FP16 ...
 
 }  // namespace w4a16

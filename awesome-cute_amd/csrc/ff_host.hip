@@ -2,6 +2,7 @@
 // choice of kernel, launches.  Nothing here allocates, waits or keeps anything of a call.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -183,6 +184,7 @@ Planned plan_with_room(int m, int n, int k, bool gated, Layout layout, int cus) 
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
+constexpr long long kMostDropped = 1LL << 40;  // elements of a call (a launch's grid)
 constexpr int kWidest = 1 << 21;  // elements from one row to the next
 
 // a matrix of 16-bit elements as the kernels address it: rows start on 16 bytes
@@ -202,13 +204,31 @@ int check_sizes(int m, int n, int k, int type) {
   return FEEDFORWARD_OK;
 }
 
+// the mask's arguments as the kernels take them: nothing below zero, and no seed in memory, where
+// nothing is dropped
+int drop_args(const feedforward_drop* d, DropArgs* out) {
+  *out = {};
+  out->factor = 1.f;
+  if (!d) return FEEDFORWARD_OK;
+  if (!(d->p >= 0.0 && d->p <= 1.0)) return fail(FEEDFORWARD_ERR_SHAPE, "p = %g is no probability", d->p);
+  const int below = (int)std::nearbyint(65536.0 * d->p);
+  if (below == 0) return FEEDFORWARD_OK;
+  if ((uintptr_t)d->seed_at & 7) return fail(FEEDFORWARD_ERR_SHAPE, "the seed must start on 8 bytes");
+  out->seed_at = d->seed_at;
+  out->seed = (unsigned long long)d->seed;
+  out->site = d->site;
+  out->below = (unsigned)below;
+  out->factor = below == 65536 ? 0.f : (float)(65536.0 / (65536 - below));
+  return FEEDFORWARD_OK;
+}
+
 bool layout_of(int turned, Layout* layout) {
   *layout = (Layout)turned;
   return turned >= FEEDFORWARD_ROWS && turned <= FEEDFORWARD_TURN_BOTH;
 }
 
 int run_product(ProductArgs a, Layout layout, bool bf, void* room, long long room_bytes, int dev, hipStream_t stream) {
-  const bool gated = a.act != kActNone;
+  const bool gated = a.finish == kGated;
   const long long columns = product_columns(a.N, gated);
   // (a launch's grid, at the smallest tiles)
   if (a.M > 0x7ffffe00 || columns > 0x3fffffffLL || (columns / 64 + 1) * (a.M / 64 + 1LL) > 0x3fffffffLL / kSlicesMost)
@@ -309,8 +329,78 @@ int feedforward_gated(const void* x, const void* w, void* h, float* pre, int m, 
   a.A = x, a.B = w, a.C = h, a.pre = pre;
   a.M = m, a.N = n, a.K = k;
   a.lda = (int)ldx, a.ldb = (int)ldw, a.ldc = (int)ldh, a.ldpre = (int)ldpre;
+  a.finish = kGated;
   a.act = activation;
   return run_product(a, kRows, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
+}
+
+int feedforward_linear(const void* x, const void* w, void* y, const void* bias, const void* residual, float* pre, int m,
+                       int n, int k, long long ldx, long long ldw, long long ldy, long long ldr, long long ldpre,
+                       int type, int activation, const feedforward_drop* drop, void* room, long long room_bytes,
+                       int dev, void* stream) {
+  int rc = check_sizes(m, n, k, type);
+  ProductArgs a = {};
+  if (rc == FEEDFORWARD_OK && k % 8 != 0) rc = fail(FEEDFORWARD_ERR_SHAPE, "widths must be multiples of 8 (k = %d)", k);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("x", x, ldx, k);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("w", w, ldw, k);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("y", y, ldy, n);
+  if (rc == FEEDFORWARD_OK && bias) rc = check_matrix("bias", bias, n, n);
+  if (rc == FEEDFORWARD_OK && residual) rc = check_matrix("residual", residual, ldr, n);
+  if (rc == FEEDFORWARD_OK && pre) rc = check_matrix("pre", pre, ldpre, n);
+  if (rc == FEEDFORWARD_OK && activation != kActNone && !act_known(activation))
+    rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
+  if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
+  if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
+  if (k == 0) return fail(FEEDFORWARD_ERR_SHAPE, "k = 0: an empty sum");
+  a.A = x, a.B = w, a.C = y, a.pre = pre, a.bias = bias, a.residual = residual;
+  a.M = m, a.N = n, a.K = k;
+  a.lda = (int)ldx, a.ldb = (int)ldw, a.ldc = (int)ldy, a.ldr = residual ? (int)ldr : 0, a.ldpre = pre ? (int)ldpre : 0;
+  a.finish = kFull;
+  a.act = activation;
+  return run_product(a, kRows, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
+}
+
+long long feedforward_linear_grad_bytes(int m, int n) {
+  if (check_sizes(m, n, 0, FEEDFORWARD_FP16) != FEEDFORWARD_OK) return -1;
+  return m > 0 && n > 0 ? 4LL * n * linear_grad_parts(m, n) : 0;
+}
+
+int feedforward_linear_grad(const void* dy, const float* pre, void* dz, void* dbias, int m, int n, long long lddy,
+                            long long ldpre, long long lddz, int type, int activation, const feedforward_drop* drop,
+                            void* partials, long long partial_bytes, int dev, void* stream) {
+  int rc = check_sizes(m, n, 0, type);
+  LinearGradArgs a = {};
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("dy", dy, lddy, n);
+  if (rc == FEEDFORWARD_OK && pre) rc = check_matrix("pre", pre, ldpre, n);
+  if (rc == FEEDFORWARD_OK && dz) rc = check_matrix("dz", dz, lddz, n);
+  if (rc == FEEDFORWARD_OK && activation != kActNone && !act_known(activation))
+    rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
+  if (rc == FEEDFORWARD_OK && (activation == kActNone) != !pre)
+    rc = fail(FEEDFORWARD_ERR_SHAPE, "the sums belong to an activation");
+  if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
+  if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
+  if (!dy || (!dz && !dbias)) return fail(FEEDFORWARD_ERR_SHAPE, "dy, or every output, is missing");
+  if (dbias && (!partials || ((uintptr_t)partials & 3) || partial_bytes < feedforward_linear_grad_bytes(m, n)))
+    return fail(FEEDFORWARD_ERR_SHAPE, "the sums over rows need %lld bytes of scratch", feedforward_linear_grad_bytes(m, n));
+  a.dy = dy, a.pre = pre, a.dz = dz, a.dbias = dbias, a.partials = dbias ? (float*)partials : nullptr;
+  a.lddy = lddy, a.ldpre = ldpre, a.lddz = lddz;
+  a.m = m, a.n = n, a.act = activation;
+  return on_device(dev, [&](int) { launch_linear_grad(a, type == FEEDFORWARD_BF16, (hipStream_t)stream); });
+}
+
+int feedforward_dropout(const void* x, const void* residual, void* y, long long count, int type,
+                        const feedforward_drop* drop, int dev, void* stream) {
+  if (count < 0 || count > kMostDropped) return fail(FEEDFORWARD_ERR_SHAPE, "%lld elements", count);
+  if (type != FEEDFORWARD_FP16 && type != FEEDFORWARD_BF16 && type != FEEDFORWARD_FP32)
+    return fail(FEEDFORWARD_ERR_SHAPE, "unknown type %d", type);
+  const uintptr_t off = type_bytes(type) - 1;
+  if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y) & off)
+    return fail(FEEDFORWARD_ERR_SHAPE, "elements must lie on whole addresses");
+  DropoutArgs a = {x, residual, y, count, {}};
+  const int rc = drop_args(drop, &a.drop);
+  if (rc != FEEDFORWARD_OK || count == 0) return rc;
+  if (!x || !y) return fail(FEEDFORWARD_ERR_SHAPE, "a matrix is missing");
+  return on_device(dev, [&](int) { launch_dropout(a, type, (hipStream_t)stream); });
 }
 
 long long feedforward_product_bytes(int m, int n, int k, int gated, int turned, int dev) {

@@ -1,9 +1,10 @@
 // What the dense products of the feed-forward block share: their arguments, the two 16-bit
-// types, and the gated column order.
+// types, the gated column order, and what becomes of a product's sums.
 #pragma once
 #include <hip/hip_runtime.h>
 
 #include "buffer_loads.hpp"
+#include "dropout.hpp"
 #include "f16_dense.hpp"
 #include "gated_act.hpp"
 #include "w4a16_common.hpp"
@@ -14,19 +15,29 @@ namespace w4a16 {
 // rows of N and A as K rows of M (the gradients' products: dx = dy w, dw = dy^T x)
 enum Layout { kRows, kTurnB, kTurnBoth };
 
-// C (M x N) = A (M x K) B^T, rows `lda`, `ldb`, `ldc` elements apart; or, gated, C (M x n) =
-// act(A G^T) * (A U^T), B given as the n rows of G and then the n of U.
+// What becomes of the sums: they are C; or, gated, C (M x n) = act(A G^T) * (A U^T), B given as the n
+// rows of G and then the n of U; or C = residual + drop(act(A B^T + bias)), whatever of these there is
+enum Finish { kPlain, kGated, kFull };
+
+// C (M x N) = A (M x K) B^T, rows `lda`, `ldb`, `ldc` elements apart, finished one way or another
 struct ProductArgs {
   const void* A;
   const void* B;
   void* C;
-  float* pre;   // gated: null, or both sums for the backward pass, (M x ldpre) in the product's order
+  float* pre;   // null, or what the backward pass takes, rows of ldpre floats: gated both sums in the
+                // product's order, full the sums with the bias
   float* part;  // null, or what the k range is cut into slices for: (slices x M x ldpart) partial sums
                 // in the product's order, which sum_parts turns into C
   int M, N, K;  // N: columns of C
   int lda, ldb, ldc, ldpre, ldpart;
-  int act;  // kActNone: not gated
+  Finish finish;
+  int act;
   int tiles_m, tiles_n, slices;
+  // full alone
+  const void* bias;      // null, or N elements
+  const void* residual;  // null, or rows ldr elements apart
+  int ldr;
+  DropArgs drop;
 };
 
 typedef __bf16 b4 __attribute__((ext_vector_type(4)));
@@ -47,6 +58,42 @@ __device__ __forceinline__ i2 product_round(f4 v) {
     return __builtin_bit_cast(i2, (b4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]});
   else
     return __builtin_bit_cast(i2, (h4){(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]});
+}
+
+// four elements of memory
+template <bool BF>
+__device__ __forceinline__ f4 widen4(i2 v) {
+  if constexpr (BF) {
+    const unsigned lo = (unsigned)v[0], hi = (unsigned)v[1];
+    return (f4){__builtin_bit_cast(float, lo << 16), __builtin_bit_cast(float, lo & 0xffff0000u),
+                __builtin_bit_cast(float, hi << 16), __builtin_bit_cast(float, hi & 0xffff0000u)};
+  } else {
+    const h4 h = __builtin_bit_cast(h4, v);
+    return (f4){(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+  }
+}
+
+__device__ __forceinline__ f4 act4(f4 v, int act) {
+  return (f4){act_value(v[0], act), act_value(v[1], act), act_value(v[2], act), act_value(v[3], act)};
+}
+__device__ __forceinline__ f4 drop4(f4 v, i2 bits, const DropArgs& a) {
+  return (f4){drop_one(v[0], bits, 0, a), drop_one(v[1], bits, 1, a), drop_one(v[2], bits, 2, a),
+              drop_one(v[3], bits, 3, a)};
+}
+
+// kFull, four columns of a row of C by themselves: where a lane has no others of their group of
+// eight, and makes its bits alone
+template <bool BF>
+__device__ __forceinline__ void finish_full(const ProductArgs& p, int row, int col, f4 v) {
+  if (p.bias) v += widen4<BF>(*(const i2*)((const half_t*)p.bias + col));
+  if (p.pre) *(f4*)(p.pre + (size_t)row * p.ldpre + col) = v;
+  if (p.act != kActNone) v = act4(v, p.act);
+  if (p.drop.below) {
+    const i4 bits = drop_bits((unsigned long long)row * (unsigned)(p.N >> 3) + (unsigned)(col >> 3), DropKey(p.drop));
+    v = drop4(v, col & 4 ? (i2){bits[2], bits[3]} : (i2){bits[0], bits[1]}, p.drop);
+  }
+  if (p.residual) v += widen4<BF>(*(const i2*)((const half_t*)p.residual + (size_t)row * p.ldr + col));
+  *(i2*)((half_t*)p.C + (size_t)row * p.ldc + col) = product_round<BF>(v);
 }
 
 __device__ __forceinline__ f4 act_mul4(f4 g, f4 u, int act) {

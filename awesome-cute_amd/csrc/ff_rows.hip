@@ -48,8 +48,9 @@ __device__ __forceinline__ void few_read(unsigned at, i4* v) {
 
 }  // namespace
 
-template <bool BF, bool GATED, int S, int MB, int DEPTH>
+template <bool BF, Finish FINISH, int S, int MB, int DEPTH>
 __global__ __launch_bounds__(64 * kFewWaves) void product_rows_kernel(ProductArgs p) {
+  constexpr bool GATED = FINISH == kGated;
   using Sh = FewShape<S, MB, DEPTH>;
   constexpr int kCols = GATED ? 8 : 16;  // columns of C per block
   extern __shared__ __attribute__((aligned(16))) char smem[];  // Sh::kLds
@@ -163,6 +164,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_rows_kernel(ProductArg
       if (p.pre)
         *(f4*)(p.pre + (size_t)row * p.ldpre + pre_col(col) + (kg >> 1 ? 16 : 0)) = v;
       if (kg < 2) *(i2*)((half_t*)p.C + (size_t)row * p.ldc + col) = product_round<BF>(act_mul4(v, up, p.act));
+    } else if constexpr (FINISH == kFull) {
+      finish_full<BF>(p, row, col, v);
     } else {
       *(i2*)((half_t*)p.C + (size_t)row * p.ldc + col) = product_round<BF>(v);
     }
@@ -171,17 +174,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_rows_kernel(ProductArg
 
 namespace {
 
-template <class F>
-void with_rows(int s, int mb, bool bf, bool gated, F f) {
-#define FF_ROWS(S, MB, DEPTH)                                                         \
-  if (s == S && mb == MB) {                                                           \
-    constexpr int lds = FewShape<S, MB, DEPTH>::kLds;                                 \
-    if (bf)                                                                           \
-      return f(gated ? product_rows_kernel<true, true, S, MB, DEPTH>                  \
-                     : product_rows_kernel<true, false, S, MB, DEPTH>, lds);          \
-    return f(gated ? product_rows_kernel<false, true, S, MB, DEPTH>                   \
-                   : product_rows_kernel<false, false, S, MB, DEPTH>, lds);           \
-  }
+template <bool BF, Finish FINISH, class F>
+void with_blocks(int s, int mb, F f) {
+#define FF_ROWS(S, MB, DEPTH) \
+  if (s == S && mb == MB) return f(product_rows_kernel<BF, FINISH, S, MB, DEPTH>, FewShape<S, MB, DEPTH>::kLds);
   FF_ROWS(1, 1, 3)
   FF_ROWS(2, 1, 2)
   FF_ROWS(1, 2, 2)
@@ -192,6 +188,16 @@ void with_rows(int s, int mb, bool bf, bool gated, F f) {
   FF_ROWS(2, 4, 2)
 #undef FF_ROWS
 }
+template <bool BF, class F>
+void with_finish(int s, int mb, Finish finish, F f) {
+  if (finish == kGated) return with_blocks<BF, kGated>(s, mb, f);
+  if (finish == kFull) return with_blocks<BF, kFull>(s, mb, f);
+  with_blocks<BF, kPlain>(s, mb, f);
+}
+template <class F>
+void with_rows(int s, int mb, bool bf, Finish finish, F f) {
+  bf ? with_finish<true>(s, mb, finish, f) : with_finish<false>(s, mb, finish, f);
+}
 
 }  // namespace
 
@@ -200,8 +206,8 @@ hipError_t configure_product_rows() {
   for (const int s : {1, 2})
     for (const int mb : {1, 2, 3, 4})
       for (const bool bf : {false, true})
-        for (const bool gated : {false, true})
-          with_rows(s, mb, bf, gated, [&](auto kernel, int lds) {
+        for (const Finish finish : {kPlain, kGated, kFull})
+          with_rows(s, mb, bf, finish, [&](auto kernel, int lds) {
             if (e == hipSuccess)
               e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
           });
@@ -209,10 +215,9 @@ hipError_t configure_product_rows() {
 }
 
 void launch_product_rows(const ProductArgs& a, int blocks, bool bf, hipStream_t stream) {
-  const bool gated = a.act != kActNone;
   ProductArgs b = a;
-  b.tiles_n = ceil_div(a.N, (gated ? 8 : 16) * blocks);
-  with_rows(blocks, ceil_div(a.M, 16), bf, gated, [&](auto kernel, int lds) {
+  b.tiles_n = ceil_div(a.N, (a.finish == kGated ? 8 : 16) * blocks);
+  with_rows(blocks, ceil_div(a.M, 16), bf, a.finish, [&](auto kernel, int lds) {
     hipLaunchKernelGGL(kernel, dim3(b.tiles_n), dim3(64 * kFewWaves), lds, stream, b);
   });
 }

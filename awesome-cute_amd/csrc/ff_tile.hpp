@@ -89,6 +89,64 @@ __device__ __forceinline__ void put(const ProductArgs& p, char* row, int m0, int
     }
   }
 }
+
+// kFull: what a lane brings to row `m` of the tile's LDS image, of a pair of operands j and j + 1, the
+// first at column `col` of the tile.  Bias and residual are fetched ahead; rows and columns
+// past the last repeat it, and are not stored.
+__device__ __forceinline__ i2 full_bias(const ProductArgs& p, int n0, int col, int cols) {
+  return *(const i2*)((const half_t*)p.bias + n0 + min(col, cols - 4));
+}
+__device__ __forceinline__ i2 full_residual(const ProductArgs& p, int m0, int n0, int m, int col, int rows, int cols) {
+  return *(const i2*)((const half_t*)p.residual + (size_t)(m0 + min(m, rows - 1)) * p.ldr + n0 + min(col, cols - 4));
+}
+// The 128 bits of a group of eight columns are those of two lanes sixteen apart, each with four of
+// them.  Of the pair's two groups the even lane group makes the first operand's, the odd one the
+// second's, and they swap what is the other's: one generator's run for eight elements.
+__device__ __forceinline__ void full_bits(const ProductArgs& p, const DropKey& key, int m0, int n0, int m, int col,
+                                          int kg, i2* first, i2* second) {
+  const int at = n0 + col - 4 * kg + (kg & 1 ? 16 : 0) + 8 * (kg >> 1);
+  const i4 w = drop_bits((unsigned long long)(unsigned)(m0 + m) * (unsigned)(p.N >> 3) + (unsigned)(at >> 3), key);
+#if defined(__HIP_DEVICE_COMPILE__)
+  // (the odd rows of sixteen lanes of one with the even rows of the other)
+  const auto a = __builtin_amdgcn_permlane16_swap((unsigned)w[0], (unsigned)w[2], false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap((unsigned)w[1], (unsigned)w[3], false, false);
+  *first = (i2){(int)a[0], (int)b[0]};
+  *second = (i2){(int)a[1], (int)b[1]};
+#else
+  *first = *second = (i2){w[0], w[1]};
+#endif
+}
+template <bool BF>
+__device__ __forceinline__ void put_full(const ProductArgs& p, const DropKey& key, char* row, int m0, int n0, int m,
+                                         int col, int kg, int rows, int cols, const i2* bias, const i2* residual,
+                                         f4 v, f4 next) {
+  if (p.bias) {
+    v += widen4<BF>(bias[0]);
+    next += widen4<BF>(bias[1]);
+  }
+  if (p.pre && m < rows) {
+    float* const pre = p.pre + (size_t)(m0 + m) * p.ldpre + n0 + col;
+    if (col < cols) __builtin_nontemporal_store(v, (f4*)pre);
+    if (col + 16 < cols) __builtin_nontemporal_store(next, (f4*)(pre + 16));
+  }
+  if (p.act != kActNone) {
+    v = act4(v, p.act);
+    next = act4(next, p.act);
+  }
+  if (p.drop.below) {
+    i2 first, second;
+    full_bits(p, key, m0, n0, m, col, kg, &first, &second);
+    v = drop4(v, first, p.drop);
+    next = drop4(next, second, p.drop);
+  }
+  if (p.residual) {
+    v += widen4<BF>(residual[0]);
+    next += widen4<BF>(residual[1]);
+  }
+  *(i2*)(row + 2 * col) = product_round<BF>(v);
+  *(i2*)(row + 2 * (col + 16)) = product_round<BF>(next);
+}
+
 // ... and of a slice: the sums as they are (columns in the product's order)
 __device__ __forceinline__ void put_part(const ProductArgs& p, int slice, int m, int col, int rows_end, int cols_end,
                                          f4 v) {

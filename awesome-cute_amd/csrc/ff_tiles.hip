@@ -10,6 +10,7 @@
 //     those took 75 us of 1060 of a forward and backward pass of 2048 x 2 x 10752 x 4096,
 //   - gated, a tile's columns are gates and ups in turns of sixteen (gated_row), and its
 //     epilogue writes act(g) u, for the backward pass both sums as well,
+//   - full (kFull), it adds a bias, applies an activation, drops and adds a residual,
 //   - the k range may be cut into slices, whose sums meet in memory (sum_parts): problems of few
 //     tiles over a deep k.
 //
@@ -140,9 +141,10 @@ struct Side {
 // time; the same weights over and over, from the last-level cache, 1.00 to 1.08, but the weights
 // of a model pass that cache.  With more tiles above each other it is slower either way (777 x 2
 // x 5208 x 4160 60 -> 69 us, 1237 x 1032 x 2744 21 -> 30).
-template <bool BF, bool GATED, Layout LAYOUT, int TM, int TN, int WM, int WN, int RING, bool ONCE>
+template <bool BF, Finish FINISH, Layout LAYOUT, int TM, int TN, int WM, int WN, int RING, bool ONCE>
 __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs p) {
-  static_assert(!GATED || LAYOUT == kRows, "");
+  static_assert(FINISH == kPlain || LAYOUT == kRows, "");
+  constexpr bool GATED = FINISH == kGated;
   using Sh = FfShape<TM, TN, WM, WN, RING, GATED>;
   constexpr int RB = Sh::kRB, NJ = Sh::kNJ, TA = Sh::kTA, TB = Sh::kTB;
   constexpr bool kTurnA = LAYOUT == kTurnBoth, kTurnedB = LAYOUT != kRows;
@@ -303,12 +305,34 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
     return;
   }
   char* const out = smem + (16 * RB * wm + nu) * out_pitch<TN, GATED>();
+  if constexpr (FINISH == kFull) {
+    static_assert(NJ % 2 == 0, "pairs of operands");
+    const DropKey key(p.drop);
+    const int col0 = 16 * NJ * wn + 4 * kg;
+    i2 bias[NJ], residual[RB][NJ];
+    if (p.residual)
 #pragma unroll
-  for (int i = 0; i < RB; i++)
+      for (int i = 0; i < RB; i++)
 #pragma unroll
-    for (int j = 0; j < NJ; j += GATED ? 2 : 1)
-      put<TN, GATED, BF>(p, out + 16 * i * out_pitch<TN, GATED>(), m0, n0, 16 * RB * wm + 16 * i + nu,
-                         16 * NJ * wn + 16 * j + 4 * kg, rows, cols, acc[i][j], acc[i][GATED ? j + 1 : j]);
+        for (int j = 0; j < NJ; j++)
+          residual[i][j] = full_residual(p, m0, n0, 16 * RB * wm + 16 * i + nu, col0 + 16 * j, rows, cols);
+    if (p.bias)
+#pragma unroll
+      for (int j = 0; j < NJ; j++) bias[j] = full_bias(p, n0, col0 + 16 * j, cols);
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+      for (int j = 0; j < NJ; j += 2)
+        put_full<BF>(p, key, out + 16 * i * out_pitch<TN, false>(), m0, n0, 16 * RB * wm + 16 * i + nu, col0 + 16 * j,
+                     kg, rows, cols, bias + j, residual[i] + j, acc[i][j], acc[i][j + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+      for (int j = 0; j < NJ; j += GATED ? 2 : 1)
+        put<TN, GATED, BF>(p, out + 16 * i * out_pitch<TN, GATED>(), m0, n0, 16 * RB * wm + 16 * i + nu,
+                           16 * NJ * wn + 16 * j + 4 * kg, rows, cols, acc[i][j], acc[i][GATED ? j + 1 : j]);
+  }
   __syncthreads();
   store_rows<TM, TN, GATED, Sh::kThreads>(p, smem, m0, GATED ? n0 >> 1 : n0, rows, cols, [](int r) { return r; });
 }
@@ -316,8 +340,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
 // The slices' sums in their order, and what a tile's epilogue does with them; four columns of C
 // a thread.  All SLICES are on their way together: fetched one after the other, eight cost 1.2 us
 // of 13.5 where C is small (64 x 2048 x 8192).
-template <bool BF, bool GATED, int SLICES>
+template <bool BF, Finish FINISH, int SLICES>
 __global__ __launch_bounds__(256) void sum_parts_kernel(ProductArgs p) {
+  constexpr bool GATED = FINISH == kGated;
   const int quads = p.N / 4;
   const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
   const int m = (int)(at / quads), col = 4 * (int)(at - (long long)m * quads);
@@ -344,18 +369,21 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(ProductArgs p) {
     }
     v = act_mul4(v, up, p.act);
   }
-  *(i2*)((half_t*)p.C + (size_t)m * p.ldc + col) = product_round<BF>(v);
+  if constexpr (FINISH == kFull)
+    finish_full<BF>(p, m, col, v);
+  else
+    *(i2*)((half_t*)p.C + (size_t)m * p.ldc + col) = product_round<BF>(v);
 }
 
 namespace {
 
 // calls f(kernel, LDS bytes, threads) for a tile, a layout and a type; once: one tile is as high as C
-template <bool BF, bool GATED, Layout LAYOUT, class F>
+template <bool BF, Finish FINISH, Layout LAYOUT, class F>
 void with_tile(const FfTile& t, bool once, F f) {
 #define FF_TILE_OF(TM, TN, WM, WN, RING, ONCE)                                    \
   if (t.rows == TM && t.cols == TN && once == ONCE)                               \
-  return f(product_tile_kernel<BF, GATED, LAYOUT, TM, TN, WM, WN, RING, ONCE>,    \
-           FfShape<TM, TN, WM, WN, RING, GATED>::kLds, 64 * WM * WN)
+  return f(product_tile_kernel<BF, FINISH, LAYOUT, TM, TN, WM, WN, RING, ONCE>,   \
+           FfShape<TM, TN, WM, WN, RING, FINISH == kGated>::kLds, 64 * WM * WN)
 #define FF_TILE(TM, TN, WM, WN, RING) FF_TILE_OF(TM, TN, WM, WN, RING, false)
   if constexpr (LAYOUT == kRows) {
     FF_TILE_OF(64, 64, 2, 2, 4, true);
@@ -373,12 +401,17 @@ void with_tile(const FfTile& t, bool once, F f) {
 #undef FF_TILE
 #undef FF_TILE_OF
 }
+template <bool BF, class F>
+void with_finish(const FfTile& t, Finish finish, Layout layout, bool once, F f) {
+  if (finish == kGated) return with_tile<BF, kGated, kRows>(t, once, f);
+  if (finish == kFull) return with_tile<BF, kFull, kRows>(t, once, f);
+  if (layout == kRows) return with_tile<BF, kPlain, kRows>(t, once, f);
+  if (layout == kTurnB) return with_tile<BF, kPlain, kTurnB>(t, once, f);
+  return with_tile<BF, kPlain, kTurnBoth>(t, once, f);
+}
 template <class F>
-void with_product(const FfTile& t, bool gated, Layout layout, bool once, bool bf, F f) {
-  if (gated) return bf ? with_tile<true, true, kRows>(t, once, f) : with_tile<false, true, kRows>(t, once, f);
-  if (layout == kRows) return bf ? with_tile<true, false, kRows>(t, once, f) : with_tile<false, false, kRows>(t, once, f);
-  if (layout == kTurnB) return bf ? with_tile<true, false, kTurnB>(t, once, f) : with_tile<false, false, kTurnB>(t, once, f);
-  return bf ? with_tile<true, false, kTurnBoth>(t, once, f) : with_tile<false, false, kTurnBoth>(t, once, f);
+void with_product(const FfTile& t, Finish finish, Layout layout, bool once, bool bf, F f) {
+  bf ? with_finish<true>(t, finish, layout, once, f) : with_finish<false>(t, finish, layout, once, f);
 }
 
 }  // namespace
@@ -389,8 +422,8 @@ hipError_t configure_product_tiles() {
     for (const int cols : {64, 128, 256})
       for (const bool bf : {false, true})
         for (const bool once : {false, true})
-          for (const int form : {0, 1, 2, 3})
-            with_product({rows, cols}, form == 3, form == 3 ? kRows : (Layout)form, once, bf,
+          for (const int form : {0, 1, 2, 3, 4})
+            with_product({rows, cols}, form > 2 ? (Finish)(form - 2) : kPlain, form > 2 ? kRows : (Layout)form, once, bf,
                          [&](auto kernel, int lds, int) {
                            if (e == hipSuccess)
                              e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -399,10 +432,9 @@ hipError_t configure_product_tiles() {
 }
 
 void launch_product_tiles(ProductArgs a, const FfTile& t, Layout layout, bool bf, hipStream_t stream) {
-  const bool gated = a.act != kActNone;
   a.tiles_m = ceil_div(a.M, t.rows);
-  a.tiles_n = ceil_div(product_columns(a.N, gated), t.cols);
-  with_product(t, gated, layout, a.tiles_m == 1, bf, [&](auto kernel, int lds, int threads) {
+  a.tiles_n = ceil_div(product_columns(a.N, a.finish == kGated), t.cols);
+  with_product(t, a.finish, layout, a.tiles_m == 1, bf, [&](auto kernel, int lds, int threads) {
     hipLaunchKernelGGL(kernel, dim3(a.tiles_m * a.tiles_n * a.slices), dim3(threads), lds, stream, a);
   });
 }
@@ -411,13 +443,15 @@ template <int SLICES>
 static void launch_sum_of(const ProductArgs& a, bool bf, hipStream_t stream) {
   if constexpr (SLICES > 1) {
     if (a.slices != SLICES) return launch_sum_of<SLICES - 1>(a, bf, stream);
-    const bool gated = a.act != kActNone;
     const dim3 grid((unsigned)(((long long)a.M * (a.N / 4) + 255) / 256)), block(256);
     const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
-    if (bf)
-      gated ? launch(sum_parts_kernel<true, true, SLICES>) : launch(sum_parts_kernel<true, false, SLICES>);
-    else
-      gated ? launch(sum_parts_kernel<false, true, SLICES>) : launch(sum_parts_kernel<false, false, SLICES>);
+    const auto finished = [&](auto type) {
+      constexpr bool BF = decltype(type)::value;
+      if (a.finish == kGated) return launch(sum_parts_kernel<BF, kGated, SLICES>);
+      if (a.finish == kFull) return launch(sum_parts_kernel<BF, kFull, SLICES>);
+      launch(sum_parts_kernel<BF, kPlain, SLICES>);
+    };
+    bf ? finished(std::true_type{}) : finished(std::false_type{});
   }
 }
 void launch_sum_parts(const ProductArgs& a, bool bf, hipStream_t stream) { launch_sum_of<kSlicesMost>(a, bf, stream); }

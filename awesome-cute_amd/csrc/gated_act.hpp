@@ -1,4 +1,4 @@
-// The activations of the gated projections: act(g) = g sigma(t), with t = g for silu and
+// The activations of the products: act(g) = g sigma(t), with t = g for silu and
 // t = sqrt(8 / pi) (g + 0.044715 g^3) for gelu in its tanh form (g / 2 (1 + tanh(t / 2))).
 // All in fp32: an exponential and a reciprocal, each good to some 1e-7 of its argument's
 // size, far below the half steps of the 16 bits that the results are rounded to.
@@ -18,6 +18,8 @@ __device__ __forceinline__ float act_sigma(float g, int act) {
   // (exp(-t) beyond the largest float is infinity, and its reciprocal zero)
   return __builtin_amdgcn_rcpf(1.f + __expf(-t));
 }
+
+__device__ __forceinline__ float act_value(float g, int act) { return g * act_sigma(g, act); }
 
 // act(g) u
 __device__ __forceinline__ float act_mul(float g, float u, int act) { return g * act_sigma(g, act) * u; }

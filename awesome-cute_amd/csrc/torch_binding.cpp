@@ -46,6 +46,15 @@ const at::Tensor* tensor(PyObject* o, const char* name) {
   return &THPVariable_Unpack(o);
 }
 
+// an argument that may be None; false with an exception set
+bool optional(PyObject* o, const char* name, at::Tensor* out) {
+  if (o == Py_None) return true;
+  const at::Tensor* const t = tensor(o, name);
+  if (!t) return false;
+  *out = *t;
+  return true;
+}
+
 bool to_int(PyObject* o, int* v) {
   const long x = PyLong_AsLong(o);
   if (x == -1 && PyErr_Occurred()) return false;
@@ -429,7 +438,13 @@ void check_dense(const at::Tensor& x, const at::Tensor& w) {
                     "a size does not fit into a C int");
 }
 
-int type_code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? FEEDFORWARD_BF16 : FEEDFORWARD_FP16; }
+int type_code(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat ? FEEDFORWARD_FP32 : t.scalar_type() == at::kBFloat16 ? FEEDFORWARD_BF16 : FEEDFORWARD_FP16;
+}
+void* at_of(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+using Maybe = std::optional<at::Tensor>;
+Maybe maybe(const at::Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 
 at::TensorOptions options_as(const at::Tensor& like) {
   return like.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
@@ -731,6 +746,359 @@ PyObject* py_linear_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- dropout, and products with an epilogue
+
+// What makes a mask: with p = 0 there is none, and whatever seed was given is let go.
+struct Drop {
+  double p = 0.0;
+  int64_t seed = 0, site = 0;
+  at::Tensor seed_at;  // or undefined
+
+  bool on() const { return p != 0.0; }
+  void check(const at::Tensor& x) const {
+    TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "the probability of dropout must be 0 to 1, not ", p);
+    TORCH_CHECK_VALUE(site >= 0 && site <= 0xffffffffLL, "site must be 0 to 2^32 - 1, not ", site);
+    TORCH_CHECK_VALUE(!seed_at.defined() || (seed_at.scalar_type() == at::kLong && seed_at.numel() == 1 &&
+                                             seed_at.layout() == at::kStrided && seed_at.device() == x.device()),
+                      "a seed that is a tensor must be one torch.int64 on the device of x");
+  }
+  feedforward_drop plain() const {
+    return {p, (long long)seed, seed_at.defined() ? (const long long*)seed_at.data_ptr() : nullptr, (unsigned)site};
+  }
+};
+
+bool to_int64(PyObject* o, const char* name, int64_t* v) {
+  int past = 0;
+  const long long x = PyLong_AsLongLongAndOverflow(o, &past);
+  if (x == -1 && PyErr_Occurred()) return false;
+  if (past != 0) {
+    PyErr_Format(PyExc_ValueError, "%s does not fit into 64 bits", name);
+    return false;
+  }
+  *v = x;
+  return true;
+}
+
+// p, seed (an int, a tensor or None) and site
+bool drop_arguments(PyObject* const* args, Drop* out) {
+  out->p = PyFloat_AsDouble(args[0]);
+  if (PyErr_Occurred()) return false;
+  if (!to_int64(args[2], "site", &out->site)) return false;
+  if (!out->on()) return true;
+  if (args[1] == Py_None) {
+    PyErr_SetString(PyExc_ValueError, "dropout needs a seed");
+    return false;
+  }
+  if (THPVariable_Check(args[1])) {
+    out->seed_at = THPVariable_Unpack(args[1]);
+    return true;
+  }
+  return to_int64(args[1], "seed", &out->seed);
+}
+
+// The leaf that a gradient goes to, where the backward pass has no other use for the input
+// (check_capture wants it, and a leaf's accumulator, which the graph holds, holds the leaf)
+void keep_leaf(AutogradContext* ctx, const char* name, const at::Tensor& t) {
+  if (t.defined() && t.is_leaf() && t.requires_grad()) ctx->saved_data[name] = t;
+}
+at::Tensor kept_leaf(AutogradContext* ctx, const char* name) {
+  const auto at = ctx->saved_data.find(name);
+  return at == ctx->saved_data.end() ? at::Tensor() : at->second.toTensor();
+}
+void keep_drop(AutogradContext* ctx, const Drop& drop) {
+  ctx->saved_data["p"] = drop.p;
+  ctx->saved_data["seed"] = drop.seed;
+  ctx->saved_data["site"] = drop.site;
+}
+Drop kept_drop(AutogradContext* ctx, const at::Tensor& seed_at) {
+  return {ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), ctx->saved_data["site"].toInt(), seed_at};
+}
+
+struct FullInputs {
+  at::Tensor x, w, bias, residual;  // (the last two may be undefined)
+  int act = 0;
+  Drop drop;
+  int64_t m = 0, n = 0, k = 0;
+
+  void check() {
+    check_dense(x, w);
+    n = w.size(0), k = w.size(1), m = x.numel() / k;
+    for (const at::Tensor* t : {&bias, &residual}) {
+      if (!t->defined()) continue;
+      const char* const name = t == &bias ? "bias" : "residual";
+      TORCH_CHECK_VALUE(t->scalar_type() == x.scalar_type() && t->device() == x.device(), name,
+                        " must have the type and the device of x");
+      TORCH_CHECK_VALUE(t->layout() == at::kStrided && !t->is_neg(), name, " must be a plain tensor");
+    }
+    TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == n), "bias must have one dimension, the rows of weight");
+    if (residual.defined()) {
+      bool fits = residual.dim() == x.dim() && residual.size(-1) == n;
+      for (int64_t i = 0; fits && i + 1 < x.dim(); i++) fits = residual.size(i) == x.size(i);
+      TORCH_CHECK_VALUE(fits, "residual must have the result's shape");
+    }
+    drop.check(x);
+  }
+};
+
+// residual + drop(act(x w^T + bias)), and, with `keep` and an activation, the sums that the backward
+// pass takes (otherwise undefined)
+std::pair<at::Tensor, at::Tensor> full_forward(FullInputs& in, bool keep) {
+  in.check();
+  const int dev = in.x.get_device();
+  at::Tensor y = empty_rows(in.x, in.n), pre;
+  if (keep && in.act != 0) pre = at::empty({in.m, in.n}, options_as(in.x).dtype(at::kFloat));
+  const Matrix a(in.x, in.m, in.k), b(in.w, in.n, in.k);
+  std::optional<Matrix> bias, residual;
+  if (in.bias.defined()) bias.emplace(in.bias, 1, in.n);
+  if (in.residual.defined()) residual.emplace(in.residual, in.m, in.n);
+  const Room room(in.x, in.m, in.n, in.k, false, FEEDFORWARD_ROWS);
+  const feedforward_drop drop = in.drop.plain();
+  feedforward_check(feedforward_linear(a.at(), b.at(), y.data_ptr(), bias ? bias->at() : nullptr,
+                                       residual ? residual->at() : nullptr, (float*)at_of(pre), (int)in.m, (int)in.n,
+                                       (int)in.k, a.ld, b.ld, in.n, residual ? residual->ld : 0, in.n, type_code(in.x),
+                                       in.act, &drop, room.at(), room.bytes, dev, current_stream(dev)));
+  return {y, pre};
+}
+
+// -> (dx, dweight, dbias), undefined where not wanted.  (The residual's gradient is dy.)
+std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& pre, FullInputs& in,
+                                        const std::array<bool, 3>& want, std::initializer_list<const at::Tensor*> leaves) {
+  in.check();
+  const int64_t m = in.m, n = in.n;
+  TORCH_CHECK_VALUE(dy.scalar_type() == in.x.scalar_type() && dy.device() == in.x.device() && dy.dim() >= 1 &&
+                        dy.size(-1) == n && dy.numel() == m * n,
+                    "dy must be that of x and weight");
+  TORCH_CHECK_VALUE(pre.defined() == (in.act != 0) &&
+                        (!pre.defined() || (pre.scalar_type() == at::kFloat && pre.device() == in.x.device() &&
+                                            pre.numel() == m * n && pre.is_contiguous())),
+                    "the sums must be those of x and weight");
+  const int dev = in.x.get_device();
+  check_capture(leaves, dev);
+  std::array<at::Tensor, 3> out;
+  if (want[0]) out[0] = empty_as(in.x, in.x.sizes());
+  if (want[1]) out[1] = empty_as(in.w, in.w.sizes());
+  if (want[2]) out[2] = empty_as(in.x, {n});
+  if (m == 0 || n == 0) {
+    for (at::Tensor& g : out)
+      if (g.defined()) g.zero_();
+    return out;
+  }
+  const bool products = want[0] || want[1];
+  if (!products && !want[2]) return out;
+  const Matrix d(plain_values(dy), m, n);
+  // without an activation and a mask the sums' gradient is dy
+  std::optional<Matrix> dz;
+  if (products && (in.act != 0 || in.drop.on())) {
+    const int64_t ld = (n + 63) / 64 * 64;  // rows of whole cache lines
+    dz.emplace(empty_as(in.x, {m, ld}), m, ld);
+  }
+  if (dz || want[2]) {
+    at::Tensor partials;
+    long long bytes = 0;
+    if (want[2]) {
+      bytes = feedforward_linear_grad_bytes((int)m, (int)n);
+      if (bytes > 0) partials = at::empty({bytes / 4}, options_as(in.x).dtype(at::kFloat));
+    }
+    const feedforward_drop drop = in.drop.plain();
+    feedforward_check(feedforward_linear_grad(d.at(), (const float*)at_of(pre), dz ? dz->at() : nullptr, at_of(out[2]),
+                                              (int)m, (int)n, d.ld, n, dz ? dz->ld : 0, type_code(in.x), in.act, &drop,
+                                              at_of(partials), bytes, dev, current_stream(dev)));
+  }
+  if (products) product_grads(in.x, in.w, dz ? *dz : d, out[0], out[1]);
+  return out;
+}
+
+struct FullFunction : torch::autograd::Function<FullFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const Maybe& bias,
+                            const Maybe& residual, int64_t act, double p, int64_t seed, int64_t site,
+                            const Maybe& seed_at) {
+    FullInputs in{x, w, bias.value_or(at::Tensor()), residual.value_or(at::Tensor()), (int)act,
+                  Drop{p, seed, site, seed_at.value_or(at::Tensor())}};
+    auto [y, pre] = full_forward(in, true);
+    // (a seed in memory that has been written since raises)
+    ctx->save_for_backward({x, w, pre, in.drop.seed_at});
+    ctx->saved_data["act"] = act;
+    keep_drop(ctx, in.drop);
+    keep_leaf(ctx, "bias", in.bias);
+    keep_leaf(ctx, "residual", in.residual);
+    ctx->saved_data["inputs"] = (int64_t)(in.bias.defined() | in.residual.defined() << 1);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list out(9);
+    if (grads[0].defined()) {
+      c10::AutoGradMode off(false);
+      const int64_t inputs = ctx->saved_data["inputs"].toInt();
+      const bool has_bias = inputs & 1, has_residual = inputs & 2;
+      FullInputs in{saved[0], saved[1], at::Tensor(), at::Tensor(), (int)ctx->saved_data["act"].toInt(),
+                    kept_drop(ctx, saved[3])};
+      const at::Tensor bias = kept_leaf(ctx, "bias"), residual = kept_leaf(ctx, "residual");
+      // (the context counts the inputs that are there)
+      const std::array<bool, 3> want = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                        has_bias && ctx->needs_input_grad(2)};
+      auto g = full_backward(grads[0], saved[2], in, want, {&in.x, &in.w, &bias, &residual});
+      for (int i = 0; i < 3; i++) out[i] = g[i];
+      if (has_residual && ctx->needs_input_grad(2 + has_bias)) out[3] = grads[0];
+    }
+    return once_differentiable(std::move(out), "linear", {&grads, &saved});
+  }
+};
+
+struct DropoutInputs {
+  at::Tensor x, residual;  // (the latter may be undefined)
+  Drop drop;
+
+  void check() const {
+    for (const at::Tensor* t : {&x, &residual}) {
+      if (!t->defined()) continue;
+      const char* const name = t == &x ? "x" : "residual";
+      const auto type = t->scalar_type();
+      TORCH_CHECK_VALUE(t->is_cuda() && (type == at::kHalf || type == at::kBFloat16 || type == at::kFloat), name,
+                        " must be a torch.half, torch.bfloat16 or torch.float tensor on the GPU");
+      TORCH_CHECK_VALUE(t->layout() == at::kStrided && !t->is_neg(), name, " must be a plain tensor");
+    }
+    TORCH_CHECK_VALUE(!residual.defined() || (residual.scalar_type() == x.scalar_type() &&
+                                              residual.device() == x.device() && residual.sizes() == x.sizes()),
+                      "residual must have the type, the device and the shape of x");
+    drop.check(x);
+  }
+};
+
+at::Tensor dropout_forward(const DropoutInputs& in) {
+  in.check();
+  const int dev = in.x.get_device();
+  at::Tensor y = empty_as(in.x, in.x.sizes());
+  const at::Tensor x = in.x.contiguous(), residual = in.residual.defined() ? in.residual.contiguous() : in.residual;
+  const feedforward_drop drop = in.drop.plain();
+  feedforward_check(feedforward_dropout(x.data_ptr(), at_of(residual), y.data_ptr(), x.numel(), type_code(x), &drop, dev,
+                                        current_stream(dev)));
+  return y;
+}
+
+// the gradient of x
+at::Tensor dropout_backward(const at::Tensor& dy, const Drop& drop, std::initializer_list<const at::Tensor*> leaves) {
+  check_capture(leaves, dy.get_device());
+  return dropout_forward({plain_values(dy), at::Tensor(), drop});
+}
+
+struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const Maybe& residual, double p, int64_t seed,
+                            int64_t site, const Maybe& seed_at) {
+    const DropoutInputs in{x, residual.value_or(at::Tensor()), Drop{p, seed, site, seed_at.value_or(at::Tensor())}};
+    at::Tensor y = dropout_forward(in);
+    ctx->save_for_backward({in.drop.seed_at});
+    keep_drop(ctx, in.drop);
+    keep_leaf(ctx, "x", x);
+    keep_leaf(ctx, "residual", in.residual);
+    ctx->saved_data["added"] = in.residual.defined();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list out(6);
+    if (grads[0].defined()) {
+      c10::AutoGradMode off(false);
+      const at::Tensor x = kept_leaf(ctx, "x"), residual = kept_leaf(ctx, "residual");
+      if (ctx->needs_input_grad(0)) out[0] = dropout_backward(grads[0], kept_drop(ctx, saved[0]), {&x, &residual});
+      if (ctx->saved_data["added"].toBool() && ctx->needs_input_grad(1)) out[1] = grads[0];
+    }
+    return once_differentiable(std::move(out), "dropout", {&grads, &saved});
+  }
+};
+
+// x, weight, bias, residual (the last two may be None), activation, p, seed and site
+bool full_arguments(PyObject* const* args, FullInputs* in) {
+  const at::Tensor *x = tensor(args[0], "x"), *w = x ? tensor(args[1], "weight") : nullptr;
+  if (!x || !w || !optional(args[2], "bias", &in->bias) || !optional(args[3], "residual", &in->residual) ||
+      !to_int(args[4], &in->act) || !drop_arguments(args + 5, &in->drop))
+    return false;
+  in->x = *x;
+  in->w = *w;
+  return true;
+}
+
+// linear_full(x, weight, bias, residual, activation, p, seed, site) -> y, with what its gradients need where
+// they are wanted
+PyObject* py_linear_full(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Call call;
+  FullInputs in;
+  if (!call.takes(nargs, 8, "linear_full") || !full_arguments(args, &in)) return nullptr;
+  refuse_tangents({&in.x, &in.w, &in.bias, &in.residual});
+  if (!call.inner && looked_on({&in.x, &in.w, &in.bias, &in.residual, &in.drop.seed_at})) Py_RETURN_NOTIMPLEMENTED;
+  at::Tensor y;
+  {
+    pybind11::gil_scoped_release unlocked;
+    y = !call.inner && differentiated({&in.x, &in.w, &in.bias, &in.residual})
+            ? FullFunction::apply(in.x, in.w, maybe(in.bias), maybe(in.residual), (int64_t)in.act, in.drop.p,
+                                  in.drop.seed, in.drop.site, maybe(in.drop.seed_at))
+            : full_forward(in, false).first;
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// dropout(x, residual, p, seed, site) -> y, likewise
+PyObject* py_dropout(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Call call;
+  DropoutInputs in;
+  if (!call.takes(nargs, 5, "dropout")) return nullptr;
+  const at::Tensor* const x = tensor(args[0], "x");
+  if (!x || !optional(args[1], "residual", &in.residual) || !drop_arguments(args + 2, &in.drop)) return nullptr;
+  in.x = *x;
+  refuse_tangents({&in.x, &in.residual});
+  if (!call.inner && looked_on({&in.x, &in.residual, &in.drop.seed_at})) Py_RETURN_NOTIMPLEMENTED;
+  at::Tensor y;
+  {
+    pybind11::gil_scoped_release unlocked;
+    y = !call.inner && differentiated({&in.x, &in.residual})
+            ? DropoutFunction::apply(in.x, maybe(in.residual), in.drop.p, in.drop.seed, in.drop.site, maybe(in.drop.seed_at))
+            : dropout_forward(in);
+  }
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_full_sums(... as linear_full) -> (y, the sums or None) and linear_full_grads(dy, sums, x, weight,
+// activation, p, seed, site, want_x, want_weight, want_bias) -> (dx, dweight, dbias), None where not wanted: the
+// passes by themselves, for compilers
+PyObject* py_linear_full_sums(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  FullInputs in;
+  if (!takes(nargs, 8, "linear_full_sums") || !full_arguments(args, &in)) return nullptr;
+  std::pair<at::Tensor, at::Tensor> out;
+  {
+    pybind11::gil_scoped_release unlocked;
+    out = full_forward(in, true);
+  }
+  return tuple_of({out.first, out.second});
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_linear_full_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (!takes(nargs, 11, "linear_full_grads")) return nullptr;
+  const at::Tensor *dy = tensor(args[0], "dy"), *x = dy ? tensor(args[2], "x") : nullptr,
+                   *w = x ? tensor(args[3], "weight") : nullptr;
+  FullInputs in;
+  at::Tensor pre;
+  std::array<bool, 3> want;
+  if (!w || !optional(args[1], "sums", &pre) || !to_int(args[4], &in.act) || !drop_arguments(args + 5, &in.drop)) return nullptr;
+  for (int i = 0; i < 3; i++)
+    if (!to_bool(args[8 + i], &want[i])) return nullptr;
+  in.x = *x;
+  in.w = *w;
+  std::array<at::Tensor, 3> g;
+  {
+    pybind11::gil_scoped_release unlocked;
+    g = full_backward(*dy, pre, in, want, {&in.x, &in.w});
+  }
+  return tuple_of({g[0], g[1], g[2]});
+  END_HANDLE_TH_ERRORS
+}
+
 // ---- the norms around a block, fp16, bfloat16 or fp32
 
 // rows of d neighbouring elements, any distance apart that is not less
@@ -752,10 +1120,6 @@ struct Rows {
   }
   void* at() const { return t.defined() ? t.data_ptr() : nullptr; }
 };
-
-int norm_code(const at::Tensor& t) {
-  return t.scalar_type() == at::kFloat ? FEEDFORWARD_FP32 : type_code(t);
-}
 
 struct NormInputs {
   at::Tensor residual, block, post, gate, pre;  // (the last four may be undefined)
@@ -801,7 +1165,6 @@ struct NormInputs {
 };
 
 at::Tensor weight_of(const at::Tensor& w) { return w.defined() ? w.contiguous() : w; }
-void* at_of(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 struct NormOutputs {
   at::Tensor y, r, lengths;
@@ -819,7 +1182,7 @@ NormOutputs norm_forward(NormInputs& in, double scale, double eps, bool keep) {
   feedforward_check(feedforward_norm(res.at(), res.ld, block.at(), block.ld, at_of(post), gate.at(), gate.ld,
                                      (int)in.rows_per_gate, at_of(pre), (float)scale, (float)eps, at_of(out.r),
                                      at_of(out.y), (float*)at_of(out.lengths), in.rows, (int)in.d,
-                                     norm_code(in.residual), dev, current_stream(dev)));
+                                     type_code(in.residual), dev, current_stream(dev)));
   return out;
 }
 
@@ -853,7 +1216,7 @@ std::array<at::Tensor, 5> norm_backward(const at::Tensor& dy, const at::Tensor& 
   at::Tensor partials;
   long long bytes = 0;
   if (out[2].defined() || out[3].defined() || (out[4].defined() && back)) {
-    bytes = feedforward_norm_grad_bytes(in.rows, (int)in.d, (int)in.rows_per_gate, norm_code(in.residual));
+    bytes = feedforward_norm_grad_bytes(in.rows, (int)in.d, (int)in.rows_per_gate, type_code(in.residual));
     if (bytes > 0) partials = at::empty({bytes / 4}, options_as(in.residual).dtype(at::kFloat));
   }
   const Rows gdy(back ? plain_values(dy) : at::Tensor(), in.rows, in.d), gdr(plain_values(dr), in.rows, in.d), r(in.residual, in.rows, in.d),
@@ -863,14 +1226,12 @@ std::array<at::Tensor, 5> norm_backward(const at::Tensor& dy, const at::Tensor& 
       gdy.at(), gdy.ld, gdr.at(), gdr.ld, r.at(), r.ld, block.at(), block.ld, at_of(post), gate.at(), gate.ld,
       (int)in.rows_per_gate, at_of(pre), (float)scale, (const float*)lengths.data_ptr(), at_of(out[0]), at_of(out[1]),
       at_of(out[2]), at_of(out[3]), back ? at_of(out[4]) : nullptr, at_of(partials), bytes, in.rows, (int)in.d,
-      norm_code(in.residual), dev, current_stream(dev)));
+      type_code(in.residual), dev, current_stream(dev)));
   return out;
 }
 
 // outputs y and r, those of them that there are
 struct NormFunction : torch::autograd::Function<NormFunction> {
-  using Maybe = std::optional<at::Tensor>;
-  static Maybe maybe(const at::Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
   static variable_list forward(AutogradContext* ctx, const at::Tensor& residual, const Maybe& block, const Maybe& post,
                                const Maybe& gate, const Maybe& pre, double scale, double eps) {
     NormInputs in{residual, block.value_or(at::Tensor()), post.value_or(at::Tensor()), gate.value_or(at::Tensor()),
@@ -909,15 +1270,6 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
   }
 };
 
-// an argument that may be None; false with an exception set
-bool optional(PyObject* o, const char* name, at::Tensor* out) {
-  if (o == Py_None) return true;
-  const at::Tensor* const t = tensor(o, name);
-  if (!t) return false;
-  *out = *t;
-  return true;
-}
-
 bool norm_arguments(PyObject* const* args, NormInputs* in) {
   const at::Tensor* const residual = tensor(args[0], "residual");
   if (!residual || !optional(args[1], "block", &in->block) || !optional(args[2], "post_weight", &in->post) ||
@@ -941,8 +1293,8 @@ PyObject* py_residual_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   {
     pybind11::gil_scoped_release unlocked;
     if (differentiated({&in.residual, &in.block, &in.post, &in.gate, &in.pre})) {
-      const variable_list v = NormFunction::apply(in.residual, NormFunction::maybe(in.block), NormFunction::maybe(in.post),
-                                                  NormFunction::maybe(in.gate), NormFunction::maybe(in.pre), scale, eps);
+      const variable_list v = NormFunction::apply(in.residual, maybe(in.block), maybe(in.post),
+                                                  maybe(in.gate), maybe(in.pre), scale, eps);
       if (in.pre.defined()) out.y = v[0];
       if (in.block.defined()) out.r = v.back();
     } else {
@@ -1128,6 +1480,10 @@ PyMethodDef methods[] = {
     {"gated_dense", (PyCFunction)(void (*)(void))py_gated_dense, METH_FASTCALL, nullptr},
     {"gated_grads", (PyCFunction)(void (*)(void))py_gated_grads, METH_FASTCALL, nullptr},
     {"linear_dense", (PyCFunction)(void (*)(void))py_linear_dense, METH_FASTCALL, nullptr},
+    {"linear_full", (PyCFunction)(void (*)(void))py_linear_full, METH_FASTCALL, nullptr},
+    {"linear_full_sums", (PyCFunction)(void (*)(void))py_linear_full_sums, METH_FASTCALL, nullptr},
+    {"linear_full_grads", (PyCFunction)(void (*)(void))py_linear_full_grads, METH_FASTCALL, nullptr},
+    {"dropout", (PyCFunction)(void (*)(void))py_dropout, METH_FASTCALL, nullptr},
     {"gated_sums", (PyCFunction)(void (*)(void))py_gated_sums, METH_FASTCALL, nullptr},
     {"norm_lengths", (PyCFunction)(void (*)(void))py_norm_lengths, METH_FASTCALL, nullptr},
     {"linear_grads", (PyCFunction)(void (*)(void))py_linear_grads, METH_FASTCALL, nullptr},

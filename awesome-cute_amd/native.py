@@ -6,7 +6,7 @@ import importlib.machinery
 import importlib.util
 import os
 
-import torch  # noqa: F401  (its libraries have to be loaded before the binding)
+import torch  # (its libraries have to be loaded before the binding)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -31,7 +31,7 @@ def _binding():
 lib = ctypes.CDLL(_path("libmarlin_amd.so"))
 torch_binding = _binding()
 
-ACTIVATIONS = {"silu": 1, "gelu": 2}  # of gated projections (gelu in its tanh form)
+ACTIVATIONS = {"silu": 1, "gelu": 2}  # of products (gelu in its tanh form)
 
 
 def activation(name):
@@ -40,3 +40,12 @@ def activation(name):
         return ACTIVATIONS[name]
     except (KeyError, TypeError):
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {name!r}") from None
+
+
+def seed_parts(p, seed):
+    """A mask's seed as the operators of torch's dispatcher take it: (number, tensor or None)."""
+    if not p:
+        return 0, None
+    if seed is None:
+        raise ValueError("dropout needs a seed")
+    return (0, seed) if isinstance(seed, torch.Tensor) else (seed, None)

@@ -10,7 +10,7 @@ import ctypes
 
 import torch
 
-from native import ACTIVATIONS, activation as _activation, lib as _lib, torch_binding as _torch_binding  # noqa: F401
+from native import ACTIVATIONS, activation as _activation, lib as _lib, seed_parts as _seed_parts, torch_binding as _torch_binding  # noqa: F401,E501
 
 _P, _I = ctypes.c_void_p, ctypes.c_int
 _lib.streamk_amd_check.restype = _I
@@ -142,14 +142,37 @@ def gated(x, weight, activation="silu"):
     return torch.ops.marlin_amd.gated_alone(x, weight, act)
 
 
-def linear(x, weight):
+def linear(x, weight, bias=None, activation=None, residual=None, *, dropout=0.0, seed=None, site=0):
     """x @ weight.T for x (..., k) and weight (n, k), torch.half or torch.bfloat16, n and k multiples
-    of 8; returns (..., n).  Differentiable once; streams and alignment as `gated`."""
+    of 8; returns (..., n).  With what else is given, in the product's epilogue and rounded once,
+
+        residual + drop(activation(x @ weight.T + bias))
+
+    bias: (n,).  activation: "silu" or "gelu" (its tanh form).  residual: the result's shape.
+    dropout: the probability with which an element is dropped; `seed`, an int or one torch.int64 on x's
+    device, and `site`, 0 to 2^32 - 1, which distinguishes masks of one seed, make the mask, that of
+    `feedforward.dropout`, which is not stored: the backward pass makes it again, and a seed that is
+    a tensor must not have been written until then.
+
+    Where gradients are wanted, those of the bias and of the residual are there too, and with an
+    activation the sums are kept in fp32, 4n bytes a row.  Differentiable once; streams and alignment as
+    `gated`."""
+    if bias is None and activation is None and residual is None and not dropout:
+        if not torch.compiler.is_compiling():
+            y = _torch_binding.linear_dense(x, weight)
+            if y is not NotImplemented:
+                return y
+        return torch.ops.marlin_amd.linear_dense(x, weight)
+    act = 0 if activation is None else _activation(activation)
     if not torch.compiler.is_compiling():
-        y = _torch_binding.linear_dense(x, weight)
+        y = _torch_binding.linear_full(x, weight, bias, residual, act, dropout, seed, site)
         if y is not NotImplemented:
             return y
-    return torch.ops.marlin_amd.linear_dense(x, weight)
+    number, tensor = _seed_parts(dropout, seed)
+    args = (x, weight, bias, residual, act, float(dropout), number, tensor, site)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        return torch.ops.marlin_amd.linear_full(*args)[0]
+    return torch.ops.marlin_amd.linear_alone(*args)
 
 
 @torch.library.custom_op("marlin_amd::gated_dense", mutates_args=())
@@ -214,6 +237,70 @@ def _linear_grads_op(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, wa
 @_linear_grads_op.register_fake
 def _linear_grads_fake(dy, x, weight, want_x, want_weight):
     return _grads_fake(x, weight, want_x, want_weight)
+
+
+_Maybe = torch.Tensor | None
+
+
+# (a seed is a number, or a tensor that takes its place)
+@torch.library.custom_op("marlin_amd::linear_full", mutates_args=())
+def _full_op(x: torch.Tensor, weight: torch.Tensor, bias: _Maybe, residual: _Maybe, act: int, p: float, seed: int,
+             seed_at: _Maybe, site: int) -> tuple[torch.Tensor, torch.Tensor]:
+    y, sums = _torch_binding.linear_full_sums(x, weight, bias, residual, act, p, seed if seed_at is None else seed_at,
+                                              site)
+    return y, x.new_empty(0, dtype=torch.float32) if sums is None else sums
+
+
+@_full_op.register_fake
+def _full_fake(x, weight, bias, residual, act, p, seed, seed_at, site):
+    n = weight.shape[0]
+    return (x.new_empty(x.shape[:-1] + (n,)),
+            x.new_empty((x.numel() // x.shape[-1], n) if act else 0, dtype=torch.float32))
+
+
+# ... without gradients, and so without the sums
+@torch.library.custom_op("marlin_amd::linear_alone", mutates_args=())
+def _alone_op(x: torch.Tensor, weight: torch.Tensor, bias: _Maybe, residual: _Maybe, act: int, p: float, seed: int,
+              seed_at: _Maybe, site: int) -> torch.Tensor:
+    return _torch_binding.linear_full(x, weight, bias, residual, act, p, seed if seed_at is None else seed_at, site,
+                                      True)
+
+
+@_alone_op.register_fake
+def _alone_fake(x, weight, bias, residual, act, p, seed, seed_at, site):
+    return x.new_empty(x.shape[:-1] + (weight.shape[0],))
+
+
+@torch.library.custom_op("marlin_amd::linear_full_grads", mutates_args=())
+def _full_grads_op(dy: torch.Tensor, sums: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act: int, p: float,
+                   seed: int, seed_at: _Maybe, site: int,
+                   want: list[bool]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    out = _torch_binding.linear_full_grads(dy, sums if act else None, x, weight, act, p,
+                                           seed if seed_at is None else seed_at, site, *want)
+    return tuple(x.new_empty(0) if g is None else g for g in out)
+
+
+@_full_grads_op.register_fake
+def _full_grads_fake(dy, sums, x, weight, act, p, seed, seed_at, site, want):
+    return (*_grads_fake(x, weight, want[0], want[1]), x.new_empty(weight.shape[0] if want[2] else 0))
+
+
+def _keep_full(ctx, inputs, output):
+    x, weight, _, _, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site = inputs
+    ctx.save_for_backward(x, weight, output[1], seed_at)
+
+
+def _full_backward(ctx, dy, _):
+    x, weight, sums, seed_at = ctx.saved_tensors
+    want = list(ctx.needs_input_grad[:4])  # (False of what is None)
+    grads = (None,) * 3
+    if any(want[:3]):
+        grads = torch.ops.marlin_amd.linear_full_grads(dy, sums, x, weight, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site,
+                                                       want[:3])
+    return (*(g if w else None for g, w in zip(grads, want)), dy if want[3] else None, None, None, None, None, None)
+
+
+_full_op.register_autograd(_full_backward, setup_context=_keep_full)
 
 
 def _keep_gated(ctx, inputs, output):

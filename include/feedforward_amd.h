@@ -46,7 +46,7 @@ int feedforward_gated_w4(const void *A, const void *B, void *C, const void *s, i
 /* types of matrices */
 #define FEEDFORWARD_FP16 0
 #define FEEDFORWARD_BF16 1
-#define FEEDFORWARD_FP32 2 /* norms only */
+#define FEEDFORWARD_FP32 2 /* norms and dropout only */
 
 /*
  * Matrices below are row-major in fp16 or bfloat16 (`type`), `ld...` elements from one row to
@@ -83,6 +83,46 @@ int feedforward_gated(const void *x, const void *w, void *h, float *pre, int m, 
 int feedforward_gated_grad(const void *dh, const float *pre, void *dgu, int m, int n,
                            long long lddh, long long ldpre, long long lddgu, int type,
                            int activation, int dev, void *stream);
+
+/*
+ * Dropout: an element is dropped (zero, whatever its value) with probability p and multiplied by
+ * 1 / (1 - p) otherwise.  p is rounded to a multiple of 2^-16, T of them, and 1 / (1 - p) with it.
+ * Element i of the result, row by row, is dropped where its 16 random bits are below T: half i % 2
+ * (the low one first) of word i % 8 / 2 of the Philox4x32 generator's seven rounds (Salmon, Moraes,
+ * Dror, Shaw, SC 2011), key the seed's low and high words, counter the low and high words of i / 8, the
+ * site, 0.  Nothing is stored: the backward pass makes the mask again.
+ */
+typedef struct feedforward_drop {
+  double p;                 /* 0 to 1; 0 is no dropout */
+  long long seed;           /* any */
+  const long long *seed_at; /* null, or device memory that holds the seed in its place */
+  unsigned site;            /* distinguishes masks that share a seed */
+} feedforward_drop;
+
+/* y (m x n) = residual + drop(act(x w^T + bias)), x (m x k), w (n x k), k > 0.  Null: bias (n
+ * elements), residual (m x n), drop, and pre, which keeps x w^T + bias for the backward pass (m rows of
+ * floats).  activation 0: none. */
+int feedforward_linear(const void *x, const void *w, void *y, const void *bias, const void *residual,
+                       float *pre, int m, int n, int k, long long ldx, long long ldw, long long ldy,
+                       long long ldr, long long ldpre, int type, int activation,
+                       const feedforward_drop *drop, void *room, long long room_bytes, int dev,
+                       void *stream);
+
+/* dz = drop(dy) act'(pre) (m x n), the gradient of x w^T + bias, and dbias (n), its sum over rows;
+ * either may be null.  pre is there if and only if there is an activation.  dbias needs `partials`, at
+ * least feedforward_linear_grad_bytes(m, n) bytes of device memory, and is not written of no rows; the
+ * order of its sums goes by the sizes alone. */
+int feedforward_linear_grad(const void *dy, const float *pre, void *dz, void *dbias, int m, int n,
+                            long long lddy, long long ldpre, long long lddz, int type, int activation,
+                            const feedforward_drop *drop, void *partials, long long partial_bytes,
+                            int dev, void *stream);
+/* -1 for sizes that are refused; no GPU touched */
+long long feedforward_linear_grad_bytes(int m, int n);
+
+/* y = residual + drop(x), or drop(x) without one; `count` elements (at most 2^40) of any type, each
+ * matrix one contiguous row.  y may be x or the residual itself.  The gradient of x is drop(dy). */
+int feedforward_dropout(const void *x, const void *residual, void *y, long long count, int type,
+                        const feedforward_drop *drop, int dev, void *stream);
 
 /* out[0..2] = rows and columns of the product's tiles and the slices of k, with room for them, on
  * a device of `cus` compute units (16 or 32 columns: all of up to 64 rows by workgroups of whole
