@@ -1,8 +1,16 @@
 // Dropout, with the residual's addition or without, and its gradient, which is the same of dy: the
 // mask is made from the seed both times (dropout.hpp) and never stored.
 //
-// A thread has one group of eight elements: 16 bytes of 16-bit elements, one run of the generator.
-// Inside fp32, rounded once.
+// A lane has eight elements: a group of 16-bit ones, 16 bytes and one run of the generator; of 32-bit
+// ones four of one group and four of another, so that a wave's loads are of neighbouring bytes.  Inside
+// fp32, rounded once.
+//
+// Bound: HBM, or the last-level cache, which holds up to 256 MB of a call.  Results are stored as not
+// read again here (nontemporal).  Operands are requested so where a call moves more than that cache holds: 16384 x 4096
+// bfloat16 with a residual, 403 MB, 61.7 us, 6.5 TB/s (otherwise 67.7, and 69.1 with plain stores).  Where it
+// moves less they are mostly there, just written by what came before, and such requests would pass it by:
+// 2048 x 10752 12.0 us, 7.4 TB/s (15.0).  The generator costs nothing visible; two or four groups
+// a lane, or a grid of eight workgroups a compute unit, 2 to 10 % more.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -16,58 +24,92 @@ namespace w4a16 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr long long kLastLevel = 256LL << 20;  // bytes of the last-level cache
 
 template <class T>
-struct Eight {
-  T v[8];
-};
+using Piece16 = T __attribute__((ext_vector_type(16 / sizeof(T))));
+
+// 16 bytes of elements at `at`, of which `left` are there
+template <bool WHOLE, bool ONCE, class T>
+__device__ __forceinline__ Piece16<T> load_piece(const T* at, long long left) {
+  constexpr int kN = 16 / sizeof(T);
+  if (WHOLE && left >= kN) {
+    const i4* const p = (const i4*)at;
+    return __builtin_bit_cast(Piece16<T>, ONCE ? __builtin_nontemporal_load(p) : *p);
+  }
+  Piece16<T> out = {};
+#pragma unroll
+  for (int e = 0; e < kN; e++)
+    if (e < left) out[e] = at[e];
+  return out;
+}
+template <bool WHOLE, class T>
+__device__ __forceinline__ void store_piece16(T* at, long long left, Piece16<T> v) {
+  constexpr int kN = 16 / sizeof(T);
+  if (WHOLE && left >= kN) {
+    __builtin_nontemporal_store(__builtin_bit_cast(i4, v), (i4*)at);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < kN; e++)
+    if (e < left) at[e] = v[e];
+}
 
 }  // namespace
 
-// WHOLE: every matrix starts on 16 bytes, the count is a multiple of eight
-template <class T, bool WHOLE>
+// WHOLE: every matrix starts on 16 bytes; ONCE: operands are requested as read once
+template <class T, bool WHOLE, bool ONCE>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(DropoutArgs p) {
-  const unsigned long long group = (unsigned long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long left = p.count - (long long)(8 * group);
-  if (left <= 0) return;
-  const T* const x = (const T*)p.x + 8 * group;
-  const T* const residual = (const T*)p.residual + 8 * group;
-  T* const y = (T*)p.y + 8 * group;
-  __attribute__((aligned(16))) Eight<T> a, r;
-  if constexpr (WHOLE) {
-    a = *(const Eight<T>*)__builtin_assume_aligned(x, 16);
-    if (p.residual) r = *(const Eight<T>*)__builtin_assume_aligned(residual, 16);
-  } else {
+  constexpr int kN = 16 / sizeof(T), kPieces = 8 / kN;
+  const int lane = threadIdx.x & 63;
+  const unsigned long long wave = (unsigned long long)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  Piece16<T> x[kPieces], residual[kPieces];
+  long long at[kPieces];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      a.v[e] = e < left ? x[e] : (T)0.f;
-      if (p.residual) r.v[e] = e < left ? residual[e] : (T)0.f;
+  for (int i = 0; i < kPieces; i++) {
+    at[i] = (long long)(512 * wave) + 64 * kN * i + kN * lane;
+    x[i] = load_piece<WHOLE, ONCE>((const T*)p.x + at[i], p.count - at[i]);
+    if (p.residual) residual[i] = load_piece<WHOLE, ONCE>((const T*)p.residual + at[i], p.count - at[i]);
+  }
+  i4 bits;
+  if constexpr (kPieces == 1) {
+    bits = drop_bits(64 * wave + lane, DropKey(p.drop));
+  } else {
+    // lanes 2 i and 2 i + 1 have group i of the first piece and group 32 + i of the second, a half each: the
+    // even one makes the bits of the first, the odd one of the second, and they exchange halves
+    const i4 w = drop_bits(64 * wave + (lane >> 1) + (lane & 1 ? 32 : 0), DropKey(p.drop));
+    const bool odd = lane & 1;
+    int mine[2], other[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      mine[h] = odd ? w[2 + h] : w[h];
+      other[h] = __builtin_amdgcn_mov_dpp(odd ? w[h] : w[2 + h], 0xb1 /* quads 1, 0, 3, 2 */, 0xf, 0xf, true);
     }
+    bits = odd ? (i4){other[0], other[1], mine[0], mine[1]} : (i4){mine[0], mine[1], other[0], other[1]};
   }
-  const i4 bits = drop_bits(group, DropKey(p.drop));
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
-    const float v = drop_one((float)a.v[e], bits, e, p.drop);
-    a.v[e] = (T)(p.residual ? (float)r.v[e] + v : v);
-  }
-  if constexpr (WHOLE) {
-    *(Eight<T>*)__builtin_assume_aligned(y, 16) = a;
-  } else {
+  for (int i = 0; i < kPieces; i++) {
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (e < left) y[e] = a.v[e];
+    for (int e = 0; e < kN; e++) {
+      const float v = drop_one((float)x[i][e], bits, kN * i + e, p.drop);
+      x[i][e] = (T)(p.residual ? (float)residual[i][e] + v : v);
+    }
+    store_piece16<WHOLE, T>((T*)p.y + at[i], p.count - at[i], x[i]);
   }
 }
 
 template <class T>
 static void launch_of(const DropoutArgs& a, hipStream_t stream) {
-  const bool whole = a.count % 8 == 0 && ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.residual & 15) == 0 &&
-                     ((uintptr_t)a.y & 15) == 0;
+  const bool whole = (((uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.y) & 15) == 0;
+  const bool once = a.count * (long long)sizeof(T) * (a.residual ? 3 : 2) > kLastLevel;
   const dim3 grid((unsigned)((a.count + 8 * kThreads - 1) / (8 * kThreads)));
-  if (whole)
-    hipLaunchKernelGGL((dropout_kernel<T, true>), grid, dim3(kThreads), 0, stream, a);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a); };
+  if (!whole)
+    launch(dropout_kernel<T, false, false>);
+  else if (once)
+    launch(dropout_kernel<T, true, true>);
   else
-    hipLaunchKernelGGL((dropout_kernel<T, false>), grid, dim3(kThreads), 0, stream, a);
+    launch(dropout_kernel<T, true, false>);
 }
 
 void launch_dropout(const DropoutArgs& a, int type, hipStream_t stream) {
