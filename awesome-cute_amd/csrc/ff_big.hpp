@@ -9,6 +9,9 @@
 // pass 2048 x 4096 x 21504 277, 1300, of which 14 the slices' sums, and 21504 x 4096 x 2048 307, 1170;
 // 8192 x 4096 x 4096 205, 1340.  The matrix pipe is in use for 57 to 72 % of these.  Results past the
 // caches or through them: level.
+//
+// A source for each type includes this: the kernels of one take the compiler a minute and more.
+#pragma once
 #include <hip/hip_runtime.h>
 
 #include "ff_tile.hpp"
@@ -25,16 +28,58 @@ struct BigShape {
   static constexpr int kSlabA = kTA * 4 * 1024, kSlabB = 256 * 128;
   // the results leave in two halves: RB / 2 (rounded up) row blocks of either wave row, and the rest
   static constexpr int kHalf = (RB + 1) / 2;
-  static constexpr int kOut = 32 * kHalf * out_pitch<256, false>();
+  static constexpr int kOut = 2 * 32 * kHalf * out_pitch<256, false>();  // (a half of the results, and of the slopes)
   static constexpr int kRingA = 3 * (kSlabA + kSlabB) <= 160 * 1024 ? 3 : 2, kRingB = 3;  // slabs in LDS
   static constexpr int kRings = kRingA * kSlabA + kRingB * kSlabB;
   static constexpr int kLds = kRings > kOut ? kRings : kOut;
   static_assert(kLds <= 160 * 1024, "LDS of a compute unit");
 };
 
+// How two slices of a tile meet, at a word of which nothing is known but that it is not this launch's: it
+// counts as empty unless it holds the launch's token, a number of 61 bits that no other launch of the
+// process has, and it is left as zero, so that a captured launch, whose token is always the same, finds
+// none of its own either.  (What memory held before could be the token by chance, once in 2^61
+// tiles.  Zeros ahead of the launch, from a kernel of their own, took 2 to 4 us.)
+//
+// Bits 0 and 1 of the word: slice 0, 1 has arrived; bit 2: it has left.  Thread 0 calls meet_arrive once the
+// workgroup's sums of the other's half have been acknowledged: the halves to finish as a bit mask, or 0 if the
+// other has not come within some 50 us -- the slices are equally long and start together, but nothing
+// promises that they run at the same time --, and then meet_abandon, once those of its own half are out as well:
+// the same, 0 meaning that the other finishes both.
+__device__ __forceinline__ bool meet_swap(unsigned long long* word, unsigned long long* seen, unsigned long long next) {
+  return __hip_atomic_compare_exchange_strong(word, seen, next, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                              __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ int meet_arrive(unsigned long long* word, unsigned long long token, int slice, int max_polls) {
+  const unsigned long long other = token | (2 >> slice), both = token | 3;
+  unsigned long long v = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (;;) {  // (the other slice alone writes the word, twice at most)
+    const unsigned long long next = v == other ? both : v == (other | 4) ? 0 : token | (1 << slice);
+    if (!meet_swap(word, &v, next)) continue;
+    if (v == other) return 1 << slice;
+    if (v == (other | 4)) return 3;
+    break;
+  }
+  for (int polls = 0; polls < max_polls; polls++) {
+    __builtin_amdgcn_s_sleep(2);
+    v = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (v != both) continue;
+    __hip_atomic_store(word, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return 1 << slice;
+  }
+  return 0;
+}
+__device__ __forceinline__ int meet_abandon(unsigned long long* word, unsigned long long token, int slice) {
+  unsigned long long v = token | (1 << slice);
+  if (meet_swap(word, &v, v | 4)) return 0;
+  __hip_atomic_store(word, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // (it is `both`)
+  return 1 << slice;
+}
+
 }  // namespace
 
-template <bool BF, Finish FINISH, Layout LAYOUT, int RB>
+// MEET: two slices of a tile finish it together
+template <bool BF, Finish FINISH, Layout LAYOUT, int RB, bool MEET>
 __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
   constexpr bool GATED = FINISH == kGated;
   using Sh = BigShape<RB, LAYOUT>;
@@ -136,6 +181,11 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
     }
   }
 
+  const int m_at = 16 * RB * wm + nu, col = 128 * wn + 4 * kg;
+  i2 bias[8];
+  // (where two slices meet their meeting hides its way, and in registers for the loop's length it spills)
+  if constexpr (FINISH == kFull && !MEET) fetch_bias(p, n0, col, cols, bias);
+
   f4 acc[RB][8];
 #if defined(__HIP_DEVICE_COMPILE__)
   if constexpr (BF == false && LAYOUT == kRows && RB == 5) {
@@ -217,7 +267,44 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
     for (auto& v : r) v = (f4){0.f, 0.f, 0.f, 0.f};
 #endif
   // a lane holds, per (i, o), row 16i + nu and four consecutive columns
-  if (p.part) {
+  constexpr int kHalf = Sh::kHalf;
+  int halves = 3;  // of the tile's row blocks that this workgroup finishes, kHalf and the rest
+  const __amdgpu_buffer_rsrc_t rP = make_rsrc(p.part, 0x7fffffffu);
+  const int lane_at = wave * (RB * 8 * 1024) + lane * 16;
+  const auto part = [&](int slice) { return (2 * at.tile + slice) * (int)big_sums(TM); };
+  if constexpr (MEET) {
+    if constexpr (FINISH == kFull) fetch_bias(p, n0, col, cols, bias);
+    // Two slices that finish their tile together (meet_arrive): each writes its sums of the other's
+    // half through to memory, waits for the acknowledgement and arrives, and adds the other's sums to its
+    // own, in whichever order the same bits as sum_parts.  (Nobody waits for long, whatever runs when.)  A
+    // launch that adds up both slices' sums of everything takes 14 us of 145 (2048 x 4096 x 10752, B turned
+    // over), and 21 of 165 with a residual.
+    unsigned long long* const word = p.words + at.tile * kWordStride;
+    const auto write_out = [&](int which) {
+      for_each<RB>([&](auto I) {
+        constexpr int i = decltype(I)::value;
+        if (which >> (i >= kHalf) & 1)
+          for_each<8>([&](auto O) {
+            constexpr int o = decltype(O)::value;
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, acc[i][o]), rP, lane_at + (8 * i + o) * 1024,
+                                                   part(at.slice), 16 /* sc1 */);
+          });
+      });
+      __builtin_amdgcn_s_waitcnt(vmcnt(0));  // my stores have been acknowledged
+      __syncthreads();                       // so have everybody's, and LDS is free
+    };
+    volatile int* const shares = (volatile int*)smem;
+    write_out(2 >> at.slice);
+    if (tid == 0) *shares = meet_arrive(word, p.token, at.slice, p.polls);
+    __syncthreads();
+    halves = __builtin_amdgcn_readfirstlane(*shares);
+    if (halves == 0) {
+      write_out(1 << at.slice);
+      if (tid == 0) *shares = meet_abandon(word, p.token, at.slice);
+      __syncthreads();
+      halves = __builtin_amdgcn_readfirstlane(*shares);
+    }
+  } else if (p.part) {
     const int columns = product_columns(p.N, GATED);
 #pragma unroll
     for (int i = 0; i < RB; i++)
@@ -228,99 +315,105 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
     return;
   }
   // The tile leaves through LDS in two halves; where both have room, the second is written to
-  // LDS while the first is on its way to memory.
-  constexpr int kPitch = out_pitch<256, GATED>(), kHalf = Sh::kHalf;
-  constexpr bool kBoth = 64 * kHalf * kPitch <= Sh::kLds;
-  const DropKey key(p.drop);
-  const int col0 = 128 * wn + 4 * kg;
-  i2 bias[8];
-  if (FINISH == kFull && p.bias)
-#pragma unroll
-    for (int o = 0; o < 8; o++) bias[o] = full_bias(p, n0, col0 + 16 * o, cols);
-#pragma unroll
-  for (int half = 0; half < 2; half++) {
-    char* const base = smem + (kBoth ? half * 32 * kHalf * kPitch : 0);
-    if (half == 0 || !kBoth) __syncthreads();  // (nothing is on its way into LDS, and nobody reads it)
-    if constexpr (FINISH == kFull) {
-      i2 residual[kHalf][8];
-      if (p.residual)
-#pragma unroll
-        for (int i = 0; i < kHalf; i++)
-#pragma unroll
-          for (int o = 0; o < 8; o++)
-            if (kHalf * half + i < RB)
-              residual[i][o] =
-                  full_residual(p, m0, n0, 16 * RB * wm + 16 * (kHalf * half + i) + nu, col0 + 16 * o, rows, cols);
-#pragma unroll
-      for (int i = 0; i < kHalf; i++) {
-        if (kHalf * half + i >= RB) continue;
-#pragma unroll
-        for (int o = 0; o < 8; o += 2)
-          put_full<BF>(p, key, base + (16 * kHalf * wm + 16 * i + nu) * kPitch, m0, n0,
-                       16 * RB * wm + 16 * (kHalf * half + i) + nu, col0 + 16 * o, kg, rows, cols, bias + o,
-                       residual[i] + o, acc[(kHalf * half + i) % RB][o], acc[(kHalf * half + i) % RB][o + 1]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kHalf; i++) {
-        if (kHalf * half + i >= RB) continue;
-#pragma unroll
-        for (int o = 0; o < 8; o += GATED ? 2 : 1)
-          put<256, GATED, BF>(p, base + (16 * kHalf * wm + 16 * i + nu) * kPitch, m0, n0,
-                              16 * RB * wm + 16 * (kHalf * half + i) + nu, 128 * wn + 16 * o + 4 * kg, rows, cols,
-                              acc[(kHalf * half + i) % RB][o],
-                              acc[(kHalf * half + i) % RB][GATED ? o + 1 : o]);
-      }
-    }
+  // LDS while the first is on its way to memory.  (Full, the slopes' image is the second half's.)
+  constexpr int kPitch = out_pitch<256, GATED>(), kImage = 32 * kHalf * kPitch;
+  const bool both = !MEET && 2 * kImage <= Sh::kLds && !(FINISH == kFull && p.slopes);
+  for_each<2>([&](auto Half) {
+    constexpr int half = decltype(Half)::value, first_block = half * kHalf, kBlocks = half ? RB - kHalf : kHalf;
+    if (MEET && !(halves >> half & 1)) return;
+    char* const base = smem + (both ? half * kImage : 0);
+    if (half == 0 || !both) __syncthreads();  // (nothing is on its way into LDS, and nobody reads it)
+    char* const out = base + (16 * kHalf * wm + nu) * kPitch;
+    // four row blocks two at a time: with the residual, or the other slice's sums, registers spill otherwise
+    constexpr int kChunk = kHalf > 3 ? 2 : kHalf;
+    for_each<(kBlocks + kChunk - 1) / kChunk>([&](auto At) {
+      constexpr int i0 = kChunk * decltype(At)::value, block = first_block + i0;
+      constexpr int count = kBlocks - i0 < kChunk ? kBlocks - i0 : kChunk;
+      const int m = m_at + 16 * block;
+      f4 v[count][8];
+      for_each<count * 8>([&](auto At) {
+        constexpr int i = decltype(At)::value / 8, o = decltype(At)::value % 8;
+        if constexpr (MEET)
+          v[i][o] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rP, lane_at + (8 * (block + i) + o) * 1024,
+                                                                                 part(1 - at.slice), 16 /* sc1 */));
+        else
+          v[i][o] = acc[block + i][o];
+      });
+      i2 residual[count][8];
+      if constexpr (FINISH == kFull) fetch_residual(p, m0, n0, m, col, rows, cols, residual);
+      if constexpr (MEET)
+        for_each<count * 8>([&](auto At) {
+          constexpr int i = decltype(At)::value / 8, o = decltype(At)::value % 8;
+          v[i][o] += acc[block + i][o];
+        });
+      if constexpr (FINISH == kFull)
+        put_full<BF, count, 8, kPitch>(p, out + 16 * i0 * kPitch, kImage, m0, n0, m, col, kg, bias, residual, v);
+      else
+        for_each<count>([&](auto I) {
+          constexpr int i = decltype(I)::value, step = GATED ? 2 : 1;
+          for_each<8 / step>([&](auto O) {
+            constexpr int o = step * decltype(O)::value;
+            put<256, GATED, BF>(p, out + 16 * (i0 + i) * kPitch, m0, n0, m + 16 * i, col + 16 * o, rows, cols, v[i][o],
+                                v[i][GATED ? o + 1 : o]);
+          });
+        });
+    });
     __syncthreads();
-    store_rows<32 * kHalf, 256, GATED, 256>(p, base, m0, GATED ? n0 >> 1 : n0, rows, cols, [&](int r) {
+    const auto row_of = [&](int r) {
       const int up = r / (16 * kHalf), at_row = 16 * kHalf * half + r % (16 * kHalf);
       return at_row < 16 * RB ? 16 * RB * up + at_row : TM;  // (an odd number of row blocks: the second half has one fewer)
-    });
-  }
+    };
+    store_rows<32 * kHalf, 256, GATED, 256>(p.C, p.ldc, base, m0, GATED ? n0 >> 1 : n0, rows, cols, row_of);
+    if constexpr (FINISH == kFull)
+      if (p.slopes)
+        store_rows<32 * kHalf, 256, false, 256>(p.slopes, p.ldslopes, base + kImage, m0, n0, rows, cols, row_of);
+  });
 }
 
 namespace {
 
-// calls f(kernel, LDS bytes) for a height, a layout and a type
-template <bool BF, Finish FINISH, Layout LAYOUT, class F>
+// calls f(kernel, LDS bytes) for a height, a layout, a type and whether two slices meet
+template <bool BF, Finish FINISH, Layout LAYOUT, bool MEET, class F>
 void with_height(int rows, F f) {
-  if (rows == 256) f(product_big_kernel<BF, FINISH, LAYOUT, 8>, BigShape<8, LAYOUT>::kLds);
-  if (rows == 224) f(product_big_kernel<BF, FINISH, LAYOUT, 7>, BigShape<7, LAYOUT>::kLds);
-  if (rows == 192) f(product_big_kernel<BF, FINISH, LAYOUT, 6>, BigShape<6, LAYOUT>::kLds);
-  if (rows == 160) f(product_big_kernel<BF, FINISH, LAYOUT, 5>, BigShape<5, LAYOUT>::kLds);
+  if (rows == 256) f(product_big_kernel<BF, FINISH, LAYOUT, 8, MEET>, BigShape<8, LAYOUT>::kLds);
+  if (rows == 224) f(product_big_kernel<BF, FINISH, LAYOUT, 7, MEET>, BigShape<7, LAYOUT>::kLds);
+  if (rows == 192) f(product_big_kernel<BF, FINISH, LAYOUT, 6, MEET>, BigShape<6, LAYOUT>::kLds);
+  if (rows == 160) f(product_big_kernel<BF, FINISH, LAYOUT, 5, MEET>, BigShape<5, LAYOUT>::kLds);
+}
+template <bool BF, bool MEET, class F>
+void with_finish(int rows, Finish finish, Layout layout, F f) {
+  if (finish == kGated) return with_height<BF, kGated, kRows, MEET>(rows, f);
+  if (finish == kFull) return with_height<BF, kFull, kRows, MEET>(rows, f);
+  if (layout == kRows) return with_height<BF, kPlain, kRows, MEET>(rows, f);
+  if (layout == kTurnB) return with_height<BF, kPlain, kTurnB, MEET>(rows, f);
+  return with_height<BF, kPlain, kTurnBoth, MEET>(rows, f);
 }
 template <bool BF, class F>
-void with_finish(int rows, Finish finish, Layout layout, F f) {
-  if (finish == kGated) return with_height<BF, kGated, kRows>(rows, f);
-  if (finish == kFull) return with_height<BF, kFull, kRows>(rows, f);
-  if (layout == kRows) return with_height<BF, kPlain, kRows>(rows, f);
-  if (layout == kTurnB) return with_height<BF, kPlain, kTurnB>(rows, f);
-  return with_height<BF, kPlain, kTurnBoth>(rows, f);
-}
-template <class F>
-void with_big(int rows, Finish finish, Layout layout, bool bf, F f) {
-  bf ? with_finish<true>(rows, finish, layout, f) : with_finish<false>(rows, finish, layout, f);
+void with_big(int rows, Finish finish, Layout layout, bool meet, F f) {
+  meet ? with_finish<BF, true>(rows, finish, layout, f) : with_finish<BF, false>(rows, finish, layout, f);
 }
 
 }  // namespace
 
-hipError_t configure_product_big() {
+template <bool BF>
+hipError_t configure_big() {
   hipError_t e = hipSuccess;
   for (const int rows : {160, 192, 224, 256})
-    for (const bool bf : {false, true})
+    for (const bool meet : {false, true})
       for (const int form : {0, 1, 2, 3, 4})
-        with_big(rows, form > 2 ? (Finish)(form - 2) : kPlain, form > 2 ? kRows : (Layout)form, bf, [&](auto kernel, int lds) {
-          if (e == hipSuccess)
-            e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        });
+        with_big<BF>(rows, form > 2 ? (Finish)(form - 2) : kPlain, form > 2 ? kRows : (Layout)form, meet,
+                     [&](auto kernel, int lds) {
+                       if (e == hipSuccess)
+                         e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+                     });
   return e;
 }
 
-void launch_product_big(ProductArgs a, int rows, Layout layout, bool bf, hipStream_t stream) {
+template <bool BF>
+void launch_big(ProductArgs a, int rows, Layout layout, hipStream_t stream) {
   a.tiles_m = ceil_div(a.M, rows);
   a.tiles_n = ceil_div(product_columns(a.N, a.finish == kGated), 256);
-  with_big(rows, a.finish, layout, bf, [&](auto kernel, int lds) {
+  with_big<BF>(rows, a.finish, layout, a.words != nullptr, [&](auto kernel, int lds) {
     hipLaunchKernelGGL(kernel, dim3(a.tiles_m * a.tiles_n * a.slices), dim3(256), lds, stream, a);
   });
 }

@@ -91,24 +91,16 @@ __global__ __launch_bounds__(kRunThreads) void linear_grad_kernel(LinearGradArgs
 #pragma unroll 2
     for (long long r = first + r0; r < end; r += high) {
       const i4 dy = *(const i4*)((const half_t*)p.dy + (size_t)r * p.lddy + col);
-      f4 z[2];
-      if (p.pre) {
-        z[0] = *(const f4*)(p.pre + (size_t)r * p.ldpre + col);
-        z[1] = *(const f4*)(p.pre + (size_t)r * p.ldpre + col + 4);
-      }
-      i4 bits;
+      i4 slopes, bits;
+      if (p.slopes) slopes = *(const i4*)(p.slopes + (size_t)r * p.ldslopes + col);
       if (p.drop.below) bits = drop_bits((unsigned long long)r * (unsigned)(p.n >> 3) + (unsigned)(col >> 3), key);
       i4 dz;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         f4 d = widen4<BF>((i2){dy[2 * h], dy[2 * h + 1]});
-        if (p.pre)
+        if (p.slopes)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            float value, slope;
-            act_slope(z[h][e], p.act, &value, &slope);
-            d[e] *= slope;
-          }
+          for (int e = 0; e < 4; e++) d[e] *= slope_of((unsigned)slopes[2 * h + (e >> 1)] >> (16 * (e & 1)) & 0xffffu);
         // (last: what is dropped has no gradient, whatever its slope)
         if (p.drop.below) d = drop4(d, (i2){bits[2 * h], bits[2 * h + 1]}, p.drop);
 #pragma unroll

@@ -17,12 +17,12 @@ void launch_gated_grad(const GatedGradArgs& a, bool bf, hipStream_t stream);
 
 struct LinearGradArgs {
   const void* dy;    // (m x n)
-  const float* pre;  // null (no activation), or the forward pass's sums (m x ldpre)
+  const unsigned short* slopes;  // null (no activation), or the forward pass's (m x n)
   void* dz;          // null, or (m x n)
   void* dbias;       // n elements, with partials
   float* partials;   // null, or linear_grad_parts(m, n) rows of n
-  long long lddy, ldpre, lddz;
-  int m, n, act, rows_per_part;
+  long long lddy, ldslopes, lddz;
+  int m, n, rows_per_part;
   DropArgs drop;
 };
 int linear_grad_parts(int m, int n);

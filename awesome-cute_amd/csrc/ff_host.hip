@@ -2,11 +2,14 @@
 // choice of kernel, launches.  Nothing here allocates, waits or keeps anything of a call.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
 #include <mutex>
+#include <random>
 
 #include "../../include/feedforward_amd.h"
 #include "ff_grads.hpp"
@@ -21,6 +24,7 @@ constexpr int kMaxDevices = 16;
 thread_local char g_error[256] = "";
 thread_local FfTile t_tile = {0, 0};  // feedforward_force_tile
 thread_local int t_slices = 0;
+thread_local int t_polls = -1;  // feedforward_force_polls
 
 int fail(int code, const char* fmt, ...) {
   va_list args;
@@ -53,7 +57,8 @@ int on_device(int dev, F launch) {
     if (!d.configured) {
       e = hipDeviceGetAttribute(&d.cus, hipDeviceAttributeMultiprocessorCount, dev);
       if (e == hipSuccess) e = configure_product_tiles();
-      if (e == hipSuccess) e = configure_product_big();
+      if (e == hipSuccess) e = configure_product_big_f16();
+      if (e == hipSuccess) e = configure_product_big_bf16();
       if (e == hipSuccess) e = configure_product_rows();
       d.configured = e == hipSuccess;
     }
@@ -154,12 +159,36 @@ ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, int cus,
   }
   return best;
 }
+// Two slices of big tiles finish them together: their sums, and behind these the words at which
+// they meet.  More, and those of other tiles, are added up by a launch of their own.
+struct Meeting {
+  int tiles;        // 0: they do not
+  long long words;  // bytes ahead of the words
+  long long bytes;
+};
+Meeting meeting(const ProductPlan& p, int m, int columns) {
+  const long long tiles = (long long)ceil_div(m, p.tile.rows) * ceil_div(columns, p.tile.cols);
+  const long long sums = 2 * tiles * (long long)big_sums(p.tile.rows);
+  // (the sums' offsets are ints)
+  if (p.slices != 2 || !big_tile(p.tile) || sums > 0x7fffffffLL) return {0, 0, 0};
+  return {(int)tiles, sums, sums + tiles * kWordStride * 8};
+}
+
+// a launch's own: products with an odd number do not repeat within 2^61, nor look like data
+unsigned long long next_token() {
+  static std::atomic<unsigned long long> launches{std::random_device{}()};
+  unsigned long long token;
+  do token = ++launches * 0x9E3779B97F4A7C15ull << 3;
+  while (token == 0);
+  return token;
+}
+
 // A thread's last plans with all the room they want: planning takes the host some 3 us, asked
 // for the room and again for the launch, and a model's layers are a few sizes over and over.
 struct Planned {
   int m = 0, n = 0, k = 0, cus = 0, form = -1;
   ProductPlan plan = {{0, 0}, 0};
-  long long bytes = 0;  // of partial sums
+  long long bytes = 0;  // of partial sums, and where slices meet in their tiles of the words
 };
 constexpr int kPlansKept = 16;
 thread_local Planned t_plans[kPlansKept];
@@ -175,6 +204,7 @@ Planned plan_with_room(int m, int n, int k, bool gated, Layout layout, int cus) 
   p.m = m, p.n = n, p.k = k, p.cus = cus, p.form = form;
   p.plan = choose_plan(m, n, k, gated, layout, cus, 1LL << 40);
   p.bytes = p.plan.slices > 1 ? 4LL * p.plan.slices * m * product_columns(n, gated) : 0;
+  p.bytes = std::max(p.bytes, meeting(p.plan, m, product_columns(n, gated)).bytes);
   if (!forced) {
     t_plans[t_oldest] = p;
     t_oldest = (t_oldest + 1) % kPlansKept;
@@ -246,13 +276,19 @@ int run_product(ProductArgs a, Layout layout, bool bf, void* room, long long roo
     a.slices = p.slices;
     a.part = p.slices > 1 ? (float*)room : nullptr;
     a.ldpart = (int)columns;
+    a.polls = t_polls < 0 ? kFinishPolls : t_polls;
+    const Meeting meet = meeting(p, a.M, (int)columns);
+    if (meet.tiles > 0 && meet.bytes <= have) {
+      a.words = (unsigned long long*)((char*)room + meet.words);
+      a.token = next_token();
+    }
     if (few_tile(p.tile))
       launch_product_rows(a, p.tile.cols / 16, bf, stream);
     else if (big_tile(p.tile))
-      launch_product_big(a, p.tile.rows, layout, bf, stream);
+      (bf ? launch_product_big_bf16 : launch_product_big_f16)(a, p.tile.rows, layout, stream);
     else
       launch_product_tiles(a, p.tile, layout, bf, stream);
-    if (a.part) launch_sum_parts(a, bf, stream);
+    if (a.part && !a.words) launch_sum_parts(a, bf, stream);
   });
 }
 
@@ -334,8 +370,8 @@ int feedforward_gated(const void* x, const void* w, void* h, float* pre, int m, 
   return run_product(a, kRows, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
 }
 
-int feedforward_linear(const void* x, const void* w, void* y, const void* bias, const void* residual, float* pre, int m,
-                       int n, int k, long long ldx, long long ldw, long long ldy, long long ldr, long long ldpre,
+int feedforward_linear(const void* x, const void* w, void* y, const void* bias, const void* residual, void* slopes, int m,
+                       int n, int k, long long ldx, long long ldw, long long ldy, long long ldr, long long ldslopes,
                        int type, int activation, const feedforward_drop* drop, void* room, long long room_bytes,
                        int dev, void* stream) {
   int rc = check_sizes(m, n, k, type);
@@ -346,15 +382,18 @@ int feedforward_linear(const void* x, const void* w, void* y, const void* bias, 
   if (rc == FEEDFORWARD_OK) rc = check_matrix("y", y, ldy, n);
   if (rc == FEEDFORWARD_OK && bias) rc = check_matrix("bias", bias, n, n);
   if (rc == FEEDFORWARD_OK && residual) rc = check_matrix("residual", residual, ldr, n);
-  if (rc == FEEDFORWARD_OK && pre) rc = check_matrix("pre", pre, ldpre, n);
+  if (rc == FEEDFORWARD_OK && slopes) rc = check_matrix("slopes", slopes, ldslopes, n);
   if (rc == FEEDFORWARD_OK && activation != kActNone && !act_known(activation))
     rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
+  if (rc == FEEDFORWARD_OK && activation == kActNone && slopes)
+    rc = fail(FEEDFORWARD_ERR_SHAPE, "slopes belong to an activation");
   if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
   if (k == 0) return fail(FEEDFORWARD_ERR_SHAPE, "k = 0: an empty sum");
-  a.A = x, a.B = w, a.C = y, a.pre = pre, a.bias = bias, a.residual = residual;
+  a.A = x, a.B = w, a.C = y, a.bias = bias, a.residual = residual, a.slopes = (unsigned short*)slopes;
   a.M = m, a.N = n, a.K = k;
-  a.lda = (int)ldx, a.ldb = (int)ldw, a.ldc = (int)ldy, a.ldr = residual ? (int)ldr : 0, a.ldpre = pre ? (int)ldpre : 0;
+  a.lda = (int)ldx, a.ldb = (int)ldw, a.ldc = (int)ldy;
+  a.ldr = residual ? (int)ldr : 0, a.ldslopes = slopes ? (int)ldslopes : 0;
   a.finish = kFull;
   a.act = activation;
   return run_product(a, kRows, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
@@ -365,26 +404,23 @@ long long feedforward_linear_grad_bytes(int m, int n) {
   return m > 0 && n > 0 ? 4LL * n * linear_grad_parts(m, n) : 0;
 }
 
-int feedforward_linear_grad(const void* dy, const float* pre, void* dz, void* dbias, int m, int n, long long lddy,
-                            long long ldpre, long long lddz, int type, int activation, const feedforward_drop* drop,
+int feedforward_linear_grad(const void* dy, const void* slopes, void* dz, void* dbias, int m, int n, long long lddy,
+                            long long ldslopes, long long lddz, int type, const feedforward_drop* drop,
                             void* partials, long long partial_bytes, int dev, void* stream) {
   int rc = check_sizes(m, n, 0, type);
   LinearGradArgs a = {};
   if (rc == FEEDFORWARD_OK) rc = check_matrix("dy", dy, lddy, n);
-  if (rc == FEEDFORWARD_OK && pre) rc = check_matrix("pre", pre, ldpre, n);
+  if (rc == FEEDFORWARD_OK && slopes) rc = check_matrix("slopes", slopes, ldslopes, n);
   if (rc == FEEDFORWARD_OK && dz) rc = check_matrix("dz", dz, lddz, n);
-  if (rc == FEEDFORWARD_OK && activation != kActNone && !act_known(activation))
-    rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
-  if (rc == FEEDFORWARD_OK && (activation == kActNone) != !pre)
-    rc = fail(FEEDFORWARD_ERR_SHAPE, "the sums belong to an activation");
   if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
   if (!dy || (!dz && !dbias)) return fail(FEEDFORWARD_ERR_SHAPE, "dy, or every output, is missing");
   if (dbias && (!partials || ((uintptr_t)partials & 3) || partial_bytes < feedforward_linear_grad_bytes(m, n)))
     return fail(FEEDFORWARD_ERR_SHAPE, "the sums over rows need %lld bytes of scratch", feedforward_linear_grad_bytes(m, n));
-  a.dy = dy, a.pre = pre, a.dz = dz, a.dbias = dbias, a.partials = dbias ? (float*)partials : nullptr;
-  a.lddy = lddy, a.ldpre = ldpre, a.lddz = lddz;
-  a.m = m, a.n = n, a.act = activation;
+  a.dy = dy, a.slopes = (const unsigned short*)slopes, a.dz = dz, a.dbias = dbias;
+  a.partials = dbias ? (float*)partials : nullptr;
+  a.lddy = lddy, a.ldslopes = ldslopes, a.lddz = lddz;
+  a.m = m, a.n = n;
   return on_device(dev, [&](int) { launch_linear_grad(a, type == FEEDFORWARD_BF16, (hipStream_t)stream); });
 }
 
@@ -507,6 +543,8 @@ void feedforward_force_tile(int rows, int cols, int slices) {
   for (const TileFit& f : kFewFits)
     if (f.tile.rows == rows && f.tile.cols == cols) t_tile = f.tile;
 }
+
+void feedforward_force_polls(int polls) { t_polls = polls < 0 || polls > kFinishPolls ? -1 : polls; }
 
 const char* feedforward_last_error(void) { return g_error; }
 

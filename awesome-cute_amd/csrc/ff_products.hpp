@@ -24,19 +24,22 @@ struct ProductArgs {
   const void* A;
   const void* B;
   void* C;
-  float* pre;   // null, or what the backward pass takes, rows of ldpre floats: gated both sums in the
-                // product's order, full the sums with the bias
+  float* pre;   // gated: null, or both sums for the backward pass, (M x ldpre) in the product's order
   float* part;  // null, or what the k range is cut into slices for: (slices x M x ldpart) partial sums
-                // in the product's order, which sum_parts turns into C
+                // in the product's order, which sum_parts turns into C; or, with words, a tile of
+                // sums as the waves hold them for every workgroup, which finish it together
+  unsigned long long* words;  // big tiles: null, or one for every tile, kWordStride apart, whatever is in them
+  unsigned long long token;   // this launch's, a multiple of eight (meet_arrive)
   int M, N, K;  // N: columns of C
   int lda, ldb, ldc, ldpre, ldpart;
   Finish finish;
   int act;
-  int tiles_m, tiles_n, slices;
+  int tiles_m, tiles_n, slices, polls;  // polls: looks at a tile's other slice before leaving it a share
   // full alone
   const void* bias;      // null, or N elements
   const void* residual;  // null, or rows ldr elements apart
-  int ldr;
+  unsigned short* slopes;  // null, or act' of the sums for the backward pass, rows ldslopes apart
+  int ldr, ldslopes;
   DropArgs drop;
 };
 
@@ -73,8 +76,18 @@ __device__ __forceinline__ f4 widen4(i2 v) {
   }
 }
 
-__device__ __forceinline__ f4 act4(f4 v, int act) {
-  return (f4){act_value(v[0], act), act_value(v[1], act), act_value(v[2], act), act_value(v[3], act)};
+template <int ACT>
+__device__ __forceinline__ f4 act4(f4 v) {
+  return (f4){act_value<ACT>(v[0]), act_value<ACT>(v[1]), act_value<ACT>(v[2]), act_value<ACT>(v[3])};
+}
+// ... and their slopes as the backward pass takes them
+template <int ACT>
+__device__ __forceinline__ f4 act4(f4 v, i2* slopes) {
+  unsigned code[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = act_coded<ACT>(v[e], &code[e]);
+  *slopes = (i2){(int)__builtin_amdgcn_perm(code[1], code[0], 0x05040100), (int)__builtin_amdgcn_perm(code[3], code[2], 0x05040100)};
+  return v;
 }
 __device__ __forceinline__ f4 drop4(f4 v, i2 bits, const DropArgs& a) {
   return (f4){drop_one(v[0], bits, 0, a), drop_one(v[1], bits, 1, a), drop_one(v[2], bits, 2, a),
@@ -86,8 +99,11 @@ __device__ __forceinline__ f4 drop4(f4 v, i2 bits, const DropArgs& a) {
 template <bool BF>
 __device__ __forceinline__ void finish_full(const ProductArgs& p, int row, int col, f4 v) {
   if (p.bias) v += widen4<BF>(*(const i2*)((const half_t*)p.bias + col));
-  if (p.pre) *(f4*)(p.pre + (size_t)row * p.ldpre + col) = v;
-  if (p.act != kActNone) v = act4(v, p.act);
+  if (p.act != kActNone) {
+    i2 slopes;
+    v = p.act == kActGelu ? act4<kActGelu>(v, &slopes) : act4<kActSilu>(v, &slopes);
+    if (p.slopes) *(i2*)(p.slopes + (size_t)row * p.ldslopes + col) = slopes;
+  }
   if (p.drop.below) {
     const i4 bits = drop_bits((unsigned long long)row * (unsigned)(p.N >> 3) + (unsigned)(col >> 3), DropKey(p.drop));
     v = drop4(v, col & 4 ? (i2){bits[2], bits[3]} : (i2){bits[0], bits[1]}, p.drop);
@@ -119,21 +135,26 @@ __host__ __device__ __forceinline__ int pre_col(int col) { return ((col >> 4) <<
 __host__ __device__ __forceinline__ int product_columns(int n, bool gated) { return gated ? (n + 15) / 16 * 32 : n; }
 
 // Tiles: rows x columns of the product.  256 columns and 160, 192, 224 or 256 rows are
-// ff_big.hip's, 16 and 32 columns, of up to kProductRows rows, ff_rows.hip's, the others
+// ff_big.hpp's, 16 and 32 columns, of up to kProductRows rows, ff_rows.hip's, the others
 // ff_tiles.hip's.
 struct FfTile {
   int rows, cols;
 };
 constexpr int kProductRows = 64;
 constexpr int kSlicesMost = 8;  // of the k range
+constexpr int kWordStride = 8;  // a tile's slices meet in a cache line of their own
+// bytes of a big tile's sums
+constexpr size_t big_sums(int rows) { return (size_t)rows * 256 * 4; }
 inline bool big_tile(const FfTile& t) { return t.cols == 256 && t.rows >= 160; }
 inline bool few_tile(const FfTile& t) { return t.cols <= 32; }
 hipError_t configure_product_tiles();
-hipError_t configure_product_big();
+hipError_t configure_product_big_f16();
+hipError_t configure_product_big_bf16();
 hipError_t configure_product_rows();
 // launches of any kind; bf: bfloat16 operands
 void launch_product_tiles(ProductArgs a, const FfTile& t, Layout layout, bool bf, hipStream_t stream);
-void launch_product_big(ProductArgs a, int rows, Layout layout, bool bf, hipStream_t stream);
+void launch_product_big_f16(const ProductArgs& a, int rows, Layout layout, hipStream_t stream);
+void launch_product_big_bf16(const ProductArgs& a, int rows, Layout layout, hipStream_t stream);
 void launch_product_rows(const ProductArgs& a, int blocks, bool bf, hipStream_t stream);  // of 16 columns
 void launch_sum_parts(const ProductArgs& a, bool bf, hipStream_t stream);
 

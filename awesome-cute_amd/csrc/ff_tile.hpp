@@ -1,4 +1,4 @@
-// What the product tiles of ff_tiles.hip and ff_big.hip share: where a tile's operands lie and
+// What the product tiles of ff_tiles.hip and ff_big.hpp share: where a tile's operands lie and
 // how its results leave.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -14,13 +14,14 @@ namespace w4a16 {
 
 // The tile of a workgroup: (tile, slice), the slices of one k range neighbours
 struct TileAt {
-  int m0, n0, slice;
+  int m0, n0, slice, tile;
   __device__ __forceinline__ TileAt(const ProductArgs& p, int tm_rows, int tn_cols) {
     const int tiles = p.tiles_m * p.tiles_n;
     const int work = xcd_work_index((int)blockIdx.x, tiles * p.slices);
     slice = work / tiles;
+    tile = work - slice * tiles;
     int tm, tn;
-    dn_tile_coord(work - slice * tiles, p.tiles_m, p.tiles_n, &tm, &tn);
+    dn_tile_coord(tile, p.tiles_m, p.tiles_n, &tm, &tn);
     m0 = tm_rows * tm;
     n0 = tn_cols * tn;
   }
@@ -51,9 +52,10 @@ constexpr int out_pitch() {
   return (GATED ? COLS : 2 * COLS) + 16;
 }
 
-// 16-byte pieces of ROWS rows (at smem) to C, rows below `rows`, columns below `cols`
+// 16-byte pieces of ROWS rows (at smem) to `to`, which is C or of its shape, rows below `rows`, columns
+// below `cols`
 template <int ROWS, int COLS, bool GATED, int THREADS, class RowOf>
-__device__ __forceinline__ void store_rows(const ProductArgs& p, const char* smem, int m0, int c0, int rows, int cols,
+__device__ __forceinline__ void store_rows(void* to, int ld, const char* smem, int m0, int c0, int rows, int cols,
                                            RowOf row_of) {
   constexpr int kPitch = out_pitch<COLS, GATED>();
   constexpr int kPieces = (GATED ? COLS / 2 : COLS) / 8;
@@ -64,7 +66,7 @@ __device__ __forceinline__ void store_rows(const ProductArgs& p, const char* sme
     if (m < rows && 8 * c < cols)
       // nobody reads it again in this launch: keep it out of the way of A and B in L2
       __builtin_nontemporal_store(*(const i4*)(smem + r * kPitch + 16 * c),
-                                  (i4*)((half_t*)p.C + (size_t)(m0 + m) * p.ldc + c0 + 8 * c));
+                                  (i4*)((half_t*)to + (size_t)(m0 + m) * ld + c0 + 8 * c));
   }
 }
 
@@ -90,22 +92,14 @@ __device__ __forceinline__ void put(const ProductArgs& p, char* row, int m0, int
   }
 }
 
-// kFull: what a lane brings to row `m` of the tile's LDS image, of a pair of operands j and j + 1, the
-// first at column `col` of the tile.  Bias and residual are fetched ahead; rows and columns
-// past the last repeat it, and are not stored.
-__device__ __forceinline__ i2 full_bias(const ProductArgs& p, int n0, int col, int cols) {
-  return *(const i2*)((const half_t*)p.bias + n0 + min(col, cols - 4));
-}
-__device__ __forceinline__ i2 full_residual(const ProductArgs& p, int m0, int n0, int m, int col, int rows, int cols) {
-  return *(const i2*)((const half_t*)p.residual + (size_t)(m0 + min(m, rows - 1)) * p.ldr + n0 + min(col, cols - 4));
-}
 // The 128 bits of a group of eight columns are those of two lanes sixteen apart, each with four of
-// them.  Of the pair's two groups the even lane group makes the first operand's, the odd one the
-// second's, and they swap what is the other's: one generator's run for eight elements.
-__device__ __forceinline__ void full_bits(const ProductArgs& p, const DropKey& key, int m0, int n0, int m, int col,
-                                          int kg, i2* first, i2* second) {
-  const int at = n0 + col - 4 * kg + (kg & 1 ? 16 : 0) + 8 * (kg >> 1);
-  const i4 w = drop_bits((unsigned long long)(unsigned)(m0 + m) * (unsigned)(p.N >> 3) + (unsigned)(at >> 3), key);
+// them.  Of a pair of operands' two groups the even lane group makes the first one's, the odd one the
+// second's, and they swap what is the other's: one generator's run for eight elements.  `row`, `col`: of C
+// and the first operand's.
+__device__ __forceinline__ void full_bits(const ProductArgs& p, const DropKey& key, int row, int col, int kg, i2* first,
+                                          i2* second) {
+  const int at = col - 4 * kg + (kg & 1 ? 16 : 0) + 8 * (kg >> 1);
+  const i4 w = drop_bits((unsigned long long)(unsigned)row * (unsigned)(p.N >> 3) + (unsigned)(at >> 3), key);
 #if defined(__HIP_DEVICE_COMPILE__)
   // (the odd rows of sixteen lanes of one with the even rows of the other)
   const auto a = __builtin_amdgcn_permlane16_swap((unsigned)w[0], (unsigned)w[2], false, false);
@@ -116,35 +110,93 @@ __device__ __forceinline__ void full_bits(const ProductArgs& p, const DropKey& k
   *first = *second = (i2){w[0], w[1]};
 #endif
 }
-template <bool BF>
-__device__ __forceinline__ void put_full(const ProductArgs& p, const DropKey& key, char* row, int m0, int n0, int m,
-                                         int col, int kg, int rows, int cols, const i2* bias, const i2* residual,
-                                         f4 v, f4 next) {
-  if (p.bias) {
-    v += widen4<BF>(bias[0]);
-    next += widen4<BF>(bias[1]);
-  }
-  if (p.pre && m < rows) {
-    float* const pre = p.pre + (size_t)(m0 + m) * p.ldpre + n0 + col;
-    if (col < cols) __builtin_nontemporal_store(v, (f4*)pre);
-    if (col + 16 < cols) __builtin_nontemporal_store(next, (f4*)(pre + 16));
-  }
-  if (p.act != kActNone) {
-    v = act4(v, p.act);
-    next = act4(next, p.act);
-  }
+
+// kFull: what a wave brings to the tile's LDS image, of NI row blocks and NJ operands, from their sums v.
+// `out`: this lane's row of the image in the first block, `slopes_at` bytes further on that of the slopes
+// (stored from the registers, 8 bytes of a row a lane, they took 19 us of 174, 2048 x 10752 x 4096); m, col:
+// its row and first column of the tile, of which rows x cols are there.  Bias and residual, fetched ahead,
+// are past them the last ones, and are not stored.  (The bias ahead of the residual, and of the main loop: loads come
+// back in order, and what waits for a bias behind a residual waits for both.)
+//
+// One pass over the registers for each of what there may be: a branch for each of them at every
+// operand spreads what a call executes over 127 KB of instructions, twice the cache that two compute
+// units share, and took 8192 x 4096 x 4096 with a bias from 212 us to 232.
+template <int NJ>
+__device__ __forceinline__ void fetch_bias(const ProductArgs& p, int n0, int col, int cols, i2 (&bias)[NJ]) {
+  if (p.bias)
+    for_each<NJ>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      bias[j] = *(const i2*)((const half_t*)p.bias + n0 + min(col + 16 * j, cols - 4));
+    });
+}
+template <int NI, int NJ>
+__device__ __forceinline__ void fetch_residual(const ProductArgs& p, int m0, int n0, int m, int col, int rows, int cols,
+                                               i2 (&residual)[NI][NJ]) {
+  if (p.residual)
+    for_each<NI>([&](auto I) {
+      constexpr int i = decltype(I)::value;
+      const half_t* const row = (const half_t*)p.residual + (size_t)(m0 + min(m + 16 * i, rows - 1)) * p.ldr + n0;
+      for_each<NJ>([&](auto J) {
+        constexpr int j = decltype(J)::value;
+        residual[i][j] = *(const i2*)(row + min(col + 16 * j, cols - 4));
+      });
+    });
+}
+template <bool BF, int NI, int NJ, int PITCH>
+__device__ __forceinline__ void put_full(const ProductArgs& p, char* out, int slopes_at, int m0, int n0, int m, int col,
+                                         int kg, const i2 (&bias)[NJ], const i2 (&residual)[NI][NJ], f4 (&v)[NI][NJ]) {
+  static_assert(NJ % 2 == 0, "pairs of operands");
+  if (p.bias)
+    for_each<NJ>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      const f4 add = widen4<BF>(bias[j]);
+      for_each<NI>([&](auto I) { v[decltype(I)::value][j] += add; });
+    });
+  const auto activate = [&](auto Act) {
+    constexpr int act = decltype(Act)::value;
+    for_each<NI>([&](auto I) {
+      for_each<NJ>([&](auto J) {
+        constexpr int i = decltype(I)::value, j = decltype(J)::value;
+        v[i][j] = act4<act>(v[i][j]);
+      });
+    });
+  };
+  const auto activate_slopes = [&](auto Act) {
+    constexpr int act = decltype(Act)::value;
+    for_each<NI>([&](auto I) {
+      for_each<NJ>([&](auto J) {
+        constexpr int i = decltype(I)::value, j = decltype(J)::value;
+        i2 slopes;
+        v[i][j] = act4<act>(v[i][j], &slopes);
+        *(i2*)(out + slopes_at + 16 * i * PITCH + 2 * (col + 16 * j)) = slopes;
+      });
+    });
+  };
+  if (p.act == kActGelu)
+    p.slopes ? activate_slopes(std::integral_constant<int, kActGelu>{}) : activate(std::integral_constant<int, kActGelu>{});
+  else if (p.act == kActSilu)
+    p.slopes ? activate_slopes(std::integral_constant<int, kActSilu>{}) : activate(std::integral_constant<int, kActSilu>{});
   if (p.drop.below) {
-    i2 first, second;
-    full_bits(p, key, m0, n0, m, col, kg, &first, &second);
-    v = drop4(v, first, p.drop);
-    next = drop4(next, second, p.drop);
+    const DropKey key(p.drop);
+    for_each<NI>([&](auto I) {
+      for_each<NJ / 2>([&](auto J) {
+        constexpr int i = decltype(I)::value, j = 2 * decltype(J)::value;
+        i2 first, second;
+        full_bits(p, key, m0 + m + 16 * i, n0 + col + 16 * j, kg, &first, &second);
+        v[i][j] = drop4(v[i][j], first, p.drop);
+        v[i][j + 1] = drop4(v[i][j + 1], second, p.drop);
+      });
+    });
   }
-  if (p.residual) {
-    v += widen4<BF>(residual[0]);
-    next += widen4<BF>(residual[1]);
-  }
-  *(i2*)(row + 2 * col) = product_round<BF>(v);
-  *(i2*)(row + 2 * (col + 16)) = product_round<BF>(next);
+  if (p.residual)
+    for_each<NI * NJ>([&](auto At) {
+      constexpr int i = decltype(At)::value / NJ, j = decltype(At)::value % NJ;
+      v[i][j] += widen4<BF>(residual[i][j]);
+    });
+  for_each<NI * NJ>([&](auto At) {
+    constexpr int i = decltype(At)::value / NJ, j = decltype(At)::value % NJ;
+    *(i2*)(out + 16 * i * PITCH + 2 * (col + 16 * j)) = product_round<BF>(v[i][j]);
+  });
 }
 
 // ... and of a slice: the sums as they are (columns in the product's order)

@@ -1,5 +1,5 @@
 // Dense products in fp16 or bfloat16 by tiles, with a gated epilogue: what
-// ff_rows.hip and ff_big.hip do not compute.  Slabs, swizzle, order of MFMA operands and the
+// ff_rows.hip and ff_big.hpp do not compute.  Slabs, swizzle, order of MFMA operands and the
 // loop are those of f16_tiles.hip, where they are explained and measured; here
 //   - rows of A, B and C may lie further apart than they are long,
 //   - C may have any number of columns that is a multiple of 8, and k any such depth: what is
@@ -28,14 +28,17 @@ namespace w4a16 {
 namespace {
 
 // TM x TN tiles, WM x WN waves
-template <int TM, int TN, int WM, int WN, int RING, bool GATED>
+template <int TM, int TN, int WM, int WN, int RING, Finish FINISH>
 struct FfShape {
+  static constexpr bool GATED = FINISH == kGated;
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
   static constexpr int kRB = TM / 16 / WM, kNJ = TN / 16 / WN;  // operands of a wave per k step
   static constexpr int kTA = (TM / 8 + kWaves - 1) / kWaves, kTB = TN / 8 / kWaves;  // loads per wave and slab
   static constexpr int kSlabA = kTA * kWaves * 1024, kSlab = kSlabA + TN * 128;
   static constexpr int kLoads = kTA + kTB;
-  static constexpr int kRingBytes = RING * kSlab, kTileBytes = TM * out_pitch<TN, GATED>();
+  static constexpr int kRingBytes = RING * kSlab;
+  static constexpr int kImage = TM * out_pitch<TN, GATED>();            // of the results
+  static constexpr int kTileBytes = (FINISH == kFull ? 2 : 1) * kImage;  // ... and of the slopes
   static constexpr int kLds = kRingBytes > kTileBytes ? kRingBytes : kTileBytes;
   static_assert(kTB * 8 * kWaves == TN && TM % (16 * WM) == 0 && TN % (16 * WN) == 0, "whole blocks");
   static_assert(!GATED || kNJ % 2 == 0, "a gate's operand and its partner's in one wave");
@@ -145,7 +148,7 @@ template <bool BF, Finish FINISH, Layout LAYOUT, int TM, int TN, int WM, int WN,
 __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs p) {
   static_assert(FINISH == kPlain || LAYOUT == kRows, "");
   constexpr bool GATED = FINISH == kGated;
-  using Sh = FfShape<TM, TN, WM, WN, RING, GATED>;
+  using Sh = FfShape<TM, TN, WM, WN, RING, FINISH>;
   constexpr int RB = Sh::kRB, NJ = Sh::kNJ, TA = Sh::kTA, TB = Sh::kTB;
   constexpr bool kTurnA = LAYOUT == kTurnBoth, kTurnedB = LAYOUT != kRows;
   using SideA = Side<kTurnA, TM, Sh::kWaves, TA, RB>;
@@ -243,6 +246,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
     ff_landed(o.a);
   };
 
+  const int col_at = 16 * NJ * wn + 4 * kg;  // (full)
+  i2 bias[NJ];
+  if constexpr (FINISH == kFull) fetch_bias(p, n0, col_at, cols, bias);
   f4 acc[RB][NJ];
 #pragma unroll
   for (int i = 0; i < RB; i++)
@@ -306,25 +312,10 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
   }
   char* const out = smem + (16 * RB * wm + nu) * out_pitch<TN, GATED>();
   if constexpr (FINISH == kFull) {
-    static_assert(NJ % 2 == 0, "pairs of operands");
-    const DropKey key(p.drop);
-    const int col0 = 16 * NJ * wn + 4 * kg;
-    i2 bias[NJ], residual[RB][NJ];
-    if (p.residual)
-#pragma unroll
-      for (int i = 0; i < RB; i++)
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-          residual[i][j] = full_residual(p, m0, n0, 16 * RB * wm + 16 * i + nu, col0 + 16 * j, rows, cols);
-    if (p.bias)
-#pragma unroll
-      for (int j = 0; j < NJ; j++) bias[j] = full_bias(p, n0, col0 + 16 * j, cols);
-#pragma unroll
-    for (int i = 0; i < RB; i++)
-#pragma unroll
-      for (int j = 0; j < NJ; j += 2)
-        put_full<BF>(p, key, out + 16 * i * out_pitch<TN, false>(), m0, n0, 16 * RB * wm + 16 * i + nu, col0 + 16 * j,
-                     kg, rows, cols, bias + j, residual[i] + j, acc[i][j], acc[i][j + 1]);
+    const int m = 16 * RB * wm + nu;
+    i2 residual[RB][NJ];
+    fetch_residual(p, m0, n0, m, col_at, rows, cols, residual);
+    put_full<BF, RB, NJ, out_pitch<TN, false>()>(p, out, Sh::kImage, m0, n0, m, col_at, kg, bias, residual, acc);
   } else {
 #pragma unroll
     for (int i = 0; i < RB; i++)
@@ -334,7 +325,11 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
                            16 * NJ * wn + 16 * j + 4 * kg, rows, cols, acc[i][j], acc[i][GATED ? j + 1 : j]);
   }
   __syncthreads();
-  store_rows<TM, TN, GATED, Sh::kThreads>(p, smem, m0, GATED ? n0 >> 1 : n0, rows, cols, [](int r) { return r; });
+  const auto same = [](int r) { return r; };
+  store_rows<TM, TN, GATED, Sh::kThreads>(p.C, p.ldc, smem, m0, GATED ? n0 >> 1 : n0, rows, cols, same);
+  if constexpr (FINISH == kFull)
+    if (p.slopes)
+      store_rows<TM, TN, false, Sh::kThreads>(p.slopes, p.ldslopes, smem + Sh::kImage, m0, n0, rows, cols, same);
 }
 
 // The slices' sums in their order, and what a tile's epilogue does with them; four columns of C
@@ -383,7 +378,7 @@ void with_tile(const FfTile& t, bool once, F f) {
 #define FF_TILE_OF(TM, TN, WM, WN, RING, ONCE)                                    \
   if (t.rows == TM && t.cols == TN && once == ONCE)                               \
   return f(product_tile_kernel<BF, FINISH, LAYOUT, TM, TN, WM, WN, RING, ONCE>,   \
-           FfShape<TM, TN, WM, WN, RING, FINISH == kGated>::kLds, 64 * WM * WN)
+           FfShape<TM, TN, WM, WN, RING, FINISH>::kLds, 64 * WM * WN)
 #define FF_TILE(TM, TN, WM, WN, RING) FF_TILE_OF(TM, TN, WM, WN, RING, false)
   if constexpr (LAYOUT == kRows) {
     FF_TILE_OF(64, 64, 2, 2, 4, true);

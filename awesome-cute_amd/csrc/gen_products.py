@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""Writes the main loops of the big tiles of the feed-forward products (ff_big.hip) as inline
+"""Writes the main loops of the big tiles of the feed-forward products (ff_big.hpp) as inline
 assembly statements with fixed registers: for fp16 and bfloat16, for tiles of 32 rb rows (rb =
 5 ... 8) x 256 columns, and for operands by rows of the summed dimension's length or turned
 over, as rows along the output ("TurnB": B so, "TurnBoth": A too).

@@ -840,13 +840,13 @@ struct FullInputs {
   }
 };
 
-// residual + drop(act(x w^T + bias)), and, with `keep` and an activation, the sums that the backward
-// pass takes (otherwise undefined)
+// residual + drop(act(x w^T + bias)), and, with `keep` and an activation, the slopes that the backward
+// pass takes, 16 bits each (otherwise undefined)
 std::pair<at::Tensor, at::Tensor> full_forward(FullInputs& in, bool keep) {
   in.check();
   const int dev = in.x.get_device();
-  at::Tensor y = empty_rows(in.x, in.n), pre;
-  if (keep && in.act != 0) pre = at::empty({in.m, in.n}, options_as(in.x).dtype(at::kFloat));
+  at::Tensor y = empty_rows(in.x, in.n), slopes;
+  if (keep && in.act != 0) slopes = at::empty({in.m, in.n}, options_as(in.x).dtype(at::kShort));
   const Matrix a(in.x, in.m, in.k), b(in.w, in.n, in.k);
   std::optional<Matrix> bias, residual;
   if (in.bias.defined()) bias.emplace(in.bias, 1, in.n);
@@ -854,24 +854,24 @@ std::pair<at::Tensor, at::Tensor> full_forward(FullInputs& in, bool keep) {
   const Room room(in.x, in.m, in.n, in.k, false, FEEDFORWARD_ROWS);
   const feedforward_drop drop = in.drop.plain();
   feedforward_check(feedforward_linear(a.at(), b.at(), y.data_ptr(), bias ? bias->at() : nullptr,
-                                       residual ? residual->at() : nullptr, (float*)at_of(pre), (int)in.m, (int)in.n,
+                                       residual ? residual->at() : nullptr, at_of(slopes), (int)in.m, (int)in.n,
                                        (int)in.k, a.ld, b.ld, in.n, residual ? residual->ld : 0, in.n, type_code(in.x),
                                        in.act, &drop, room.at(), room.bytes, dev, current_stream(dev)));
-  return {y, pre};
+  return {y, slopes};
 }
 
 // -> (dx, dweight, dbias), undefined where not wanted.  (The residual's gradient is dy.)
-std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& pre, FullInputs& in,
+std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& slopes, FullInputs& in,
                                         const std::array<bool, 3>& want, std::initializer_list<const at::Tensor*> leaves) {
   in.check();
   const int64_t m = in.m, n = in.n;
   TORCH_CHECK_VALUE(dy.scalar_type() == in.x.scalar_type() && dy.device() == in.x.device() && dy.dim() >= 1 &&
                         dy.size(-1) == n && dy.numel() == m * n,
                     "dy must be that of x and weight");
-  TORCH_CHECK_VALUE(pre.defined() == (in.act != 0) &&
-                        (!pre.defined() || (pre.scalar_type() == at::kFloat && pre.device() == in.x.device() &&
-                                            pre.numel() == m * n && pre.is_contiguous())),
-                    "the sums must be those of x and weight");
+  TORCH_CHECK_VALUE(slopes.defined() == (in.act != 0) &&
+                        (!slopes.defined() || (slopes.scalar_type() == at::kShort && slopes.device() == in.x.device() &&
+                                            slopes.numel() == m * n && slopes.is_contiguous())),
+                    "the slopes must be those of x and weight");
   const int dev = in.x.get_device();
   check_capture(leaves, dev);
   std::array<at::Tensor, 3> out;
@@ -900,9 +900,8 @@ std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& 
       if (bytes > 0) partials = at::empty({bytes / 4}, options_as(in.x).dtype(at::kFloat));
     }
     const feedforward_drop drop = in.drop.plain();
-    feedforward_check(feedforward_linear_grad(d.at(), (const float*)at_of(pre), dz ? dz->at() : nullptr, at_of(out[2]),
-                                              (int)m, (int)n, d.ld, n, dz ? dz->ld : 0, type_code(in.x), in.act, &drop,
-                                              at_of(partials), bytes, dev, current_stream(dev)));
+    feedforward_check(feedforward_linear_grad(d.at(), at_of(slopes), dz ? dz->at() : nullptr, at_of(out[2]),
+                                              (int)m, (int)n, d.ld, n, dz ? dz->ld : 0, type_code(in.x), &drop, at_of(partials), bytes, dev, current_stream(dev)));
   }
   if (products) product_grads(in.x, in.w, dz ? *dz : d, out[0], out[1]);
   return out;
@@ -914,9 +913,9 @@ struct FullFunction : torch::autograd::Function<FullFunction> {
                             const Maybe& seed_at) {
     FullInputs in{x, w, bias.value_or(at::Tensor()), residual.value_or(at::Tensor()), (int)act,
                   Drop{p, seed, site, seed_at.value_or(at::Tensor())}};
-    auto [y, pre] = full_forward(in, true);
+    auto [y, slopes] = full_forward(in, true);
     // (a seed in memory that has been written since raises)
-    ctx->save_for_backward({x, w, pre, in.drop.seed_at});
+    ctx->save_for_backward({x, w, slopes, in.drop.seed_at});
     ctx->saved_data["act"] = act;
     keep_drop(ctx, in.drop);
     keep_leaf(ctx, "bias", in.bias);
@@ -1061,13 +1060,13 @@ PyObject* py_dropout(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// linear_full_sums(... as linear_full) -> (y, the sums or None) and linear_full_grads(dy, sums, x, weight,
+// linear_full_slopes(... as linear_full) -> (y, the slopes or None) and linear_full_grads(dy, slopes, x, weight,
 // activation, p, seed, site, want_x, want_weight, want_bias) -> (dx, dweight, dbias), None where not wanted: the
 // passes by themselves, for compilers
-PyObject* py_linear_full_sums(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+PyObject* py_linear_full_slopes(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   FullInputs in;
-  if (!takes(nargs, 8, "linear_full_sums") || !full_arguments(args, &in)) return nullptr;
+  if (!takes(nargs, 8, "linear_full_slopes") || !full_arguments(args, &in)) return nullptr;
   std::pair<at::Tensor, at::Tensor> out;
   {
     pybind11::gil_scoped_release unlocked;
@@ -1083,9 +1082,9 @@ PyObject* py_linear_full_grads(PyObject*, PyObject* const* args, Py_ssize_t narg
   const at::Tensor *dy = tensor(args[0], "dy"), *x = dy ? tensor(args[2], "x") : nullptr,
                    *w = x ? tensor(args[3], "weight") : nullptr;
   FullInputs in;
-  at::Tensor pre;
+  at::Tensor slopes;
   std::array<bool, 3> want;
-  if (!w || !optional(args[1], "sums", &pre) || !to_int(args[4], &in.act) || !drop_arguments(args + 5, &in.drop)) return nullptr;
+  if (!w || !optional(args[1], "slopes", &slopes) || !to_int(args[4], &in.act) || !drop_arguments(args + 5, &in.drop)) return nullptr;
   for (int i = 0; i < 3; i++)
     if (!to_bool(args[8 + i], &want[i])) return nullptr;
   in.x = *x;
@@ -1093,7 +1092,7 @@ PyObject* py_linear_full_grads(PyObject*, PyObject* const* args, Py_ssize_t narg
   std::array<at::Tensor, 3> g;
   {
     pybind11::gil_scoped_release unlocked;
-    g = full_backward(*dy, pre, in, want, {&in.x, &in.w});
+    g = full_backward(*dy, slopes, in, want, {&in.x, &in.w});
   }
   return tuple_of({g[0], g[1], g[2]});
   END_HANDLE_TH_ERRORS
@@ -1481,7 +1480,7 @@ PyMethodDef methods[] = {
     {"gated_grads", (PyCFunction)(void (*)(void))py_gated_grads, METH_FASTCALL, nullptr},
     {"linear_dense", (PyCFunction)(void (*)(void))py_linear_dense, METH_FASTCALL, nullptr},
     {"linear_full", (PyCFunction)(void (*)(void))py_linear_full, METH_FASTCALL, nullptr},
-    {"linear_full_sums", (PyCFunction)(void (*)(void))py_linear_full_sums, METH_FASTCALL, nullptr},
+    {"linear_full_slopes", (PyCFunction)(void (*)(void))py_linear_full_slopes, METH_FASTCALL, nullptr},
     {"linear_full_grads", (PyCFunction)(void (*)(void))py_linear_full_grads, METH_FASTCALL, nullptr},
     {"dropout", (PyCFunction)(void (*)(void))py_dropout, METH_FASTCALL, nullptr},
     {"gated_sums", (PyCFunction)(void (*)(void))py_gated_sums, METH_FASTCALL, nullptr},

@@ -155,7 +155,7 @@ def linear(x, weight, bias=None, activation=None, residual=None, *, dropout=0.0,
     a tensor must not have been written until then.
 
     Where gradients are wanted, those of the bias and of the residual are there too, and with an
-    activation the sums are kept in fp32, 4n bytes a row.  Differentiable once; streams and alignment as
+    activation its slopes are kept, 2n bytes a row.  Differentiable once; streams and alignment as
     `gated`."""
     if bias is None and activation is None and residual is None and not dropout:
         if not torch.compiler.is_compiling():
@@ -246,19 +246,19 @@ _Maybe = torch.Tensor | None
 @torch.library.custom_op("marlin_amd::linear_full", mutates_args=())
 def _full_op(x: torch.Tensor, weight: torch.Tensor, bias: _Maybe, residual: _Maybe, act: int, p: float, seed: int,
              seed_at: _Maybe, site: int) -> tuple[torch.Tensor, torch.Tensor]:
-    y, sums = _torch_binding.linear_full_sums(x, weight, bias, residual, act, p, seed if seed_at is None else seed_at,
+    y, slopes = _torch_binding.linear_full_slopes(x, weight, bias, residual, act, p, seed if seed_at is None else seed_at,
                                               site)
-    return y, x.new_empty(0, dtype=torch.float32) if sums is None else sums
+    return y, x.new_empty(0, dtype=torch.int16) if slopes is None else slopes
 
 
 @_full_op.register_fake
 def _full_fake(x, weight, bias, residual, act, p, seed, seed_at, site):
     n = weight.shape[0]
     return (x.new_empty(x.shape[:-1] + (n,)),
-            x.new_empty((x.numel() // x.shape[-1], n) if act else 0, dtype=torch.float32))
+            x.new_empty((x.numel() // x.shape[-1], n) if act else 0, dtype=torch.int16))
 
 
-# ... without gradients, and so without the sums
+# ... without gradients, and so without the slopes
 @torch.library.custom_op("marlin_amd::linear_alone", mutates_args=())
 def _alone_op(x: torch.Tensor, weight: torch.Tensor, bias: _Maybe, residual: _Maybe, act: int, p: float, seed: int,
               seed_at: _Maybe, site: int) -> torch.Tensor:
@@ -272,16 +272,16 @@ def _alone_fake(x, weight, bias, residual, act, p, seed, seed_at, site):
 
 
 @torch.library.custom_op("marlin_amd::linear_full_grads", mutates_args=())
-def _full_grads_op(dy: torch.Tensor, sums: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act: int, p: float,
+def _full_grads_op(dy: torch.Tensor, slopes: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act: int, p: float,
                    seed: int, seed_at: _Maybe, site: int,
                    want: list[bool]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    out = _torch_binding.linear_full_grads(dy, sums if act else None, x, weight, act, p,
+    out = _torch_binding.linear_full_grads(dy, slopes if act else None, x, weight, act, p,
                                            seed if seed_at is None else seed_at, site, *want)
     return tuple(x.new_empty(0) if g is None else g for g in out)
 
 
 @_full_grads_op.register_fake
-def _full_grads_fake(dy, sums, x, weight, act, p, seed, seed_at, site, want):
+def _full_grads_fake(dy, slopes, x, weight, act, p, seed, seed_at, site, want):
     return (*_grads_fake(x, weight, want[0], want[1]), x.new_empty(weight.shape[0] if want[2] else 0))
 
 
@@ -291,11 +291,11 @@ def _keep_full(ctx, inputs, output):
 
 
 def _full_backward(ctx, dy, _):
-    x, weight, sums, seed_at = ctx.saved_tensors
+    x, weight, slopes, seed_at = ctx.saved_tensors
     want = list(ctx.needs_input_grad[:4])  # (False of what is None)
     grads = (None,) * 3
     if any(want[:3]):
-        grads = torch.ops.marlin_amd.linear_full_grads(dy, sums, x, weight, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site,
+        grads = torch.ops.marlin_amd.linear_full_grads(dy, slopes, x, weight, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site,
                                                        want[:3])
     return (*(g if w else None for g, w in zip(grads, want)), dy if want[3] else None, None, None, None, None, None)
 

@@ -100,20 +100,20 @@ typedef struct feedforward_drop {
 } feedforward_drop;
 
 /* y (m x n) = residual + drop(act(x w^T + bias)), x (m x k), w (n x k), k > 0.  Null: bias (n
- * elements), residual (m x n), drop, and pre, which keeps x w^T + bias for the backward pass (m rows of
- * floats).  activation 0: none. */
+ * elements), residual (m x n), drop, and slopes, which keeps act' of x w^T + bias for the backward pass
+ * (m x n numbers of 16 bits in the library's own form).  activation 0: none, and no slopes. */
 int feedforward_linear(const void *x, const void *w, void *y, const void *bias, const void *residual,
-                       float *pre, int m, int n, int k, long long ldx, long long ldw, long long ldy,
-                       long long ldr, long long ldpre, int type, int activation,
+                       void *slopes, int m, int n, int k, long long ldx, long long ldw, long long ldy,
+                       long long ldr, long long ldslopes, int type, int activation,
                        const feedforward_drop *drop, void *room, long long room_bytes, int dev,
                        void *stream);
 
-/* dz = drop(dy) act'(pre) (m x n), the gradient of x w^T + bias, and dbias (n), its sum over rows;
- * either may be null.  pre is there if and only if there is an activation.  dbias needs `partials`, at
- * least feedforward_linear_grad_bytes(m, n) bytes of device memory, and is not written of no rows; the
- * order of its sums goes by the sizes alone. */
-int feedforward_linear_grad(const void *dy, const float *pre, void *dz, void *dbias, int m, int n,
-                            long long lddy, long long ldpre, long long lddz, int type, int activation,
+/* dz (m x n) = drop(dy) times the slopes (null: ones), the gradient of x w^T + bias, and dbias (n), its
+ * sum over rows; either may be null.  dbias needs `partials`, at least feedforward_linear_grad_bytes(m, n)
+ * bytes of device memory, and is not written of no rows; the order of its sums goes by the sizes
+ * alone. */
+int feedforward_linear_grad(const void *dy, const void *slopes, void *dz, void *dbias, int m, int n,
+                            long long lddy, long long ldslopes, long long lddz, int type,
                             const feedforward_drop *drop, void *partials, long long partial_bytes,
                             int dev, void *stream);
 /* -1 for sizes that are refused; no GPU touched */
@@ -131,6 +131,9 @@ int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int *o
 /* such tiles (0 = by cost) and slices (0 = by cost) for every product of the calling thread that
  * they can compute; for tests and tools */
 void feedforward_force_tile(int rows, int cols, int slices);
+/* how often one of two slices of a tile looks for the other before it leaves it its share of the sums,
+ * at most and by default 64 times (-1); calling thread only, for tests */
+void feedforward_force_polls(int polls);
 
 /*
  * The norm after a block, its gate, the residual's scale and the norm before the next block, row

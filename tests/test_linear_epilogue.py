@@ -7,7 +7,8 @@ element by element, with e half a step of the type (2^-11 fp16, 2^-8 bf16):
   sum S of its terms' magnitudes;
   the activations' slopes stay below 1.13, their second derivatives below 1, and in fp32 values and
   slopes are off by less than 2^-18 of their size (an exponential whose argument is good to 2^-24 of
-  itself), slopes near zero by 2^-18 altogether;
+  itself), slopes near zero by 2^-18 altogether; for the backward pass slopes are kept in steps of 2^-15,
+  half a step of which they are off by;
   the mask's factor and the residual's addition round three times more, 2^-22 of the terms together;
   a result is rounded once, e of it, and for the products of the backward pass so is dz.
 """
@@ -28,7 +29,7 @@ import streamk  # noqa: E402
 
 gpu = pytest.mark.gpu
 TYPES = [torch.float16, torch.bfloat16]
-FP32, FEW, ACT = 2.0 ** -24, 2.0 ** -22, 2.0 ** -18
+FP32, FEW, ACT, SLOPE = 2.0 ** -24, 2.0 ** -22, 2.0 ** -18, 2.0 ** -16
 TILES = [(64, 64), (64, 128), (96, 128), (128, 128), (96, 256), (128, 256), (160, 256), (192, 256), (224, 256),
          (256, 256)]
 
@@ -90,11 +91,16 @@ class Full64:
         dropped = self.factor == 0
         assert torch.equal(y.reshape(want.shape)[dropped].double(), r[dropped])
 
+    def check_slopes(self, codes):
+        """Steps of 2^-15 from -1/4 on, a number of 16 bits each."""
+        got = ((codes.long() & 0xffff) - 8192).double() / 32768
+        assert codes.dtype == torch.int16 and ((got - self.slope).abs() <= self.off_z + ACT + SLOPE).all()
+
     def check_grads(self, dy, dx=None, dw=None, dbias=None, dresidual=None):
         d, e, type = dy.double().reshape(self.factor.shape) * self.factor, half_step(self.type), self.type
         m, n = d.shape
         dz = d * self.slope
-        off = FEW * dz.abs() + (d.abs() * (self.off_z + ACT) if self.act else 0)
+        off = FEW * dz.abs() + (d.abs() * (self.off_z + ACT + SLOPE) if self.act else 0)
         if dbias is not None:
             want = dz.sum(0)
             within(dbias, want, off.sum(0) + m * FP32 * dz.abs().sum(0) + e * want.abs(), type, 1.5)
@@ -171,17 +177,17 @@ class DropArgs(ctypes.Structure):
 def test_codes_of_the_entries():
     lib, L, P = streamk._lib, ctypes.c_longlong, ctypes.c_void_p
 
-    def linear(m=0, n=8, k=8, x=16, w=16, y=16, bias=None, residual=None, pre=None, ldx=8, ldw=8, ldy=8, ldr=8, ldpre=8,
+    def linear(m=0, n=8, k=8, x=16, w=16, y=16, bias=None, residual=None, slopes=None, ldx=8, ldw=8, ldy=8, ldr=8, lds=8,
                type=0, act=0, p=None, room=None):
         drop = None if p is None else ctypes.byref(DropArgs(p, 0, None, 0))
-        return lib.feedforward_linear(P(x), P(w), P(y), P(bias), P(residual), P(pre), m, n, k, L(ldx), L(ldw), L(ldy),
-                                      L(ldr), L(ldpre), type, act, drop, P(room), L(0), 0, None)
+        return lib.feedforward_linear(P(x), P(w), P(y), P(bias), P(residual), P(slopes), m, n, k, L(ldx), L(ldw), L(ldy),
+                                      L(ldr), L(lds), type, act, drop, P(room), L(0), 0, None)
 
     assert linear() == 0 and linear(x=None, w=None, y=None) == 0
-    assert linear(bias=16, residual=16, pre=16, act=2, p=0.5) == 0
+    assert linear(bias=16, residual=16, slopes=16, act=2, p=0.5) == 0
     for bad in (dict(m=-1), dict(n=12), dict(k=12, ldx=16, ldw=16), dict(ldx=4), dict(ldw=0), dict(ldy=12), dict(type=2),
-                dict(act=3), dict(act=-1), dict(x=8), dict(bias=8), dict(residual=8), dict(pre=8), dict(residual=16, ldr=0),
-                dict(pre=16, ldpre=4), dict(p=2.0), dict(p=float("nan")), dict(residual=16, ldr=1 << 22),
+                dict(act=3), dict(act=-1), dict(x=8), dict(bias=8), dict(residual=8), dict(slopes=8, act=1), dict(residual=16, ldr=0),
+                dict(slopes=16, act=1, lds=4), dict(slopes=16), dict(p=2.0), dict(p=float("nan")), dict(residual=16, ldr=1 << 22),
                 dict(m=4, k=0, ldx=0, ldw=0), dict(m=4, x=None), dict(m=4, w=None), dict(m=4, y=None),
                 dict(m=4, room=8), dict(m=0x7fffffff)):
         assert linear(**bad) == 1, bad
@@ -190,15 +196,15 @@ def test_codes_of_the_entries():
     lib.feedforward_linear_grad_bytes.restype = L
     many = lib.feedforward_linear_grad_bytes
 
-    def grad(m=4, n=8, dy=16, pre=None, dz=16, dbias=None, lddy=8, ldpre=8, lddz=8, type=0, act=0, p=None, partials=None,
+    def grad(m=4, n=8, dy=16, slopes=None, dz=16, dbias=None, lddy=8, lds=8, lddz=8, type=0, p=None, partials=None,
              count=0):
         drop = None if p is None else ctypes.byref(DropArgs(p, 0, None, 0))
-        return lib.feedforward_linear_grad(P(dy), P(pre), P(dz), P(dbias), m, n, L(lddy), L(ldpre), L(lddz), type, act,
+        return lib.feedforward_linear_grad(P(dy), P(slopes), P(dz), P(dbias), m, n, L(lddy), L(lds), L(lddz), type,
                                            drop, P(partials), L(count), 0, None)
 
     assert grad(m=0) == 0 and grad(n=0) == 0 and grad(m=0, dy=None, dz=None) == 0
-    for bad in (dict(m=-1), dict(n=12), dict(lddy=4), dict(dz=8), dict(lddz=0), dict(act=1), dict(pre=16),
-                dict(pre=8, act=1), dict(pre=16, act=1, ldpre=4), dict(act=5, pre=16), dict(type=2), dict(p=-1.0),
+    for bad in (dict(m=-1), dict(n=12), dict(lddy=4), dict(dz=8), dict(lddz=0), dict(slopes=8),
+                dict(slopes=16, lds=4), dict(type=2), dict(p=-1.0),
                 dict(dy=None), dict(dz=None), dict(dbias=16), dict(dbias=16, partials=16, count=many(4, 8) - 1),
                 dict(dbias=16, partials=18, count=many(4, 8))):
         assert grad(**bad) == 1, bad
@@ -258,9 +264,8 @@ def test_every_tile(tile, m, n, k, slices):
             for i, form in enumerate(FORMS):
                 oracle(x, w, bias, residual, form, 9, i).check_forward(call(x, w, bias, residual, form, 9, i))
             # what the backward pass takes
-            sums = streamk._torch_binding.linear_full_sums(x, w, bias, None, 1, 0.0, None, 0)[1]
-            ref = Full64(x, w, bias, None, None)
-            assert sums.dtype == torch.float32 and ((sums.double() - ref.value).abs() <= ref.off_z).all()
+            slopes = streamk._torch_binding.linear_full_slopes(x, w, bias, None, 1, 0.0, None, 0)[1]
+            Full64(x, w, bias, "silu", None).check_slopes(slopes)
     finally:
         streamk.force_product_tile(0)
 
@@ -275,9 +280,8 @@ def test_whole_columns_of_few_rows(m, n, k, cols):
             x, w, bias, residual, _ = make(m, n, k, type, m + n)
             for i, form in enumerate(FORMS):
                 oracle(x, w, bias, residual, form, 1, i).check_forward(call(x, w, bias, residual, form, 1, i))
-            sums = streamk._torch_binding.linear_full_sums(x, w, bias, None, 1, 0.0, None, 0)[1]
-            ref = Full64(x, w, bias, None, None)
-            assert ((sums.double() - ref.value).abs() <= ref.off_z).all()
+            slopes = streamk._torch_binding.linear_full_slopes(x, w, bias, None, 1, 0.0, None, 0)[1]
+            Full64(x, w, bias, "silu", None).check_slopes(slopes)
     finally:
         streamk.force_product_tile(0)
 
@@ -294,33 +298,32 @@ def test_inside_rows_that_hold_nan(tile, slices):
 
             def inside(t, dtype=None):
                 rows, cols = t.shape
-                room = torch.full((rows + 80, cols + 96), float("nan"), dtype=dtype or type, device="cuda")
+                room = torch.full((rows + 80, cols + 96), -7 if dtype else float("nan"), dtype=dtype or type, device="cuda")
                 room[8:8 + rows, 16:16 + cols] = t
                 return room, room[8:8 + rows, 16:16 + cols]
 
             (_, vx), (_, vw), (_, vr) = inside(x), inside(w), inside(residual)
-            (ry, vy), (rp, vp) = inside(torch.zeros_like(residual)), inside(torch.zeros_like(residual), torch.float32)
+            (ry, vy), (rs, vs) = inside(torch.zeros_like(residual)), inside(torch.zeros_like(residual), torch.int16)
             vb = inside(bias[None])[1]
-            before, before_pre = ry.clone(), rp.clone()
+            before, before_slopes = ry.clone(), rs.clone()
             room = torch.empty(3 * m * n, device="cuda")
             drop = DropArgs(0.3, 77, None, 2)
             try:
                 streamk.force_product_tile(*tile, slices)
                 code = lib.feedforward_linear(
                     P(vx.data_ptr()), P(vw.data_ptr()), P(vy.data_ptr()), P(vb.data_ptr()), P(vr.data_ptr()),
-                    P(vp.data_ptr()), m, n, k, L(vx.stride(0)), L(vw.stride(0)), L(vy.stride(0)), L(vr.stride(0)),
-                    L(vp.stride(0)), int(type == torch.bfloat16), 2, ctypes.byref(drop), P(room.data_ptr()),
+                    P(vs.data_ptr()), m, n, k, L(vx.stride(0)), L(vw.stride(0)), L(vy.stride(0)), L(vr.stride(0)),
+                    L(vs.stride(0)), int(type == torch.bfloat16), 2, ctypes.byref(drop), P(room.data_ptr()),
                     L(4 * room.numel()), 0, P(torch.cuda.current_stream().cuda_stream))
             finally:
                 streamk.force_product_tile(0)
             assert code == 0
             Full64(x, w, bias, "gelu", residual, 0.3, 77, 2).check_forward(vy)
-            ref = Full64(x, w, bias, None, None)
-            assert ((vp.double() - ref.value).abs() <= ref.off_z).all()
+            Full64(x, w, bias, "gelu", None).check_slopes(vs)
             vy.copy_(before[8:8 + m, 16:16 + n])
-            vp.copy_(before_pre[8:8 + m, 16:16 + n])
+            vs.copy_(before_slopes[8:8 + m, 16:16 + n])
             assert torch.equal(ry.isnan(), before.isnan()) and not ry.nan_to_num().any()
-            assert torch.equal(rp.isnan(), before_pre.isnan()) and not rp.nan_to_num().any()
+            assert torch.equal(rs, before_slopes)
 
 
 GRADS = [(1, 8, 8), (3, 40, 72), (65, 64, 64), (64, 520, 136), (200, 1032, 264), (777, 200, 1000), (1237, 2744, 1032),
@@ -710,3 +713,125 @@ def test_the_operators_as_they_are_used_together():
         torch.cuda.synchronize()
         assert torch.equal(out, want[step][0])
         assert all(torch.equal(a, b) for a, b in zip(grads, want[step][1]))
+
+
+# --- two slices of a big tile, which finish it together -------------------------------------
+
+@pytest.fixture
+def polls():
+    lib = streamk._lib
+    lib.feedforward_force_polls.argtypes = [ctypes.c_int]
+    lib.feedforward_force_polls.restype = None
+    yield lib.feedforward_force_polls
+    lib.feedforward_force_polls(-1)
+
+
+def product(a, b, m, n, k, turned, room, garbage=0):
+    """The C entry, with that many bytes of room, filled with the byte `garbage`."""
+    lib, L, P = streamk._lib, ctypes.c_longlong, ctypes.c_void_p
+    c = torch.full((m, n), float("nan"), dtype=a.dtype, device="cuda")
+    at = torch.full((max(room, 16),), garbage, dtype=torch.uint8, device="cuda")
+    assert lib.feedforward_product(P(a.data_ptr()), P(b.data_ptr()), P(c.data_ptr()), m, n, k, L(a.stride(0)),
+                                   L(b.stride(0)), L(n), turned, int(a.dtype == torch.bfloat16), P(at.data_ptr()),
+                                   L(room), 0, P(torch.cuda.current_stream().cuda_stream)) == 0
+    return c, at
+
+
+@gpu
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("tile", TILES[6:])
+@pytest.mark.parametrize("m,n,k", [(328, 264, 320), (8, 8, 72), (1000, 1544, 200)])
+def test_slices_that_meet_are_their_sum(m, n, k, tile, type, polls):
+    """To the bit, whether they wait for each other or not, whatever was in the room, and with room that
+    does for the sums alone, which a launch of its own adds up."""
+    lib = streamk._lib
+    lib.feedforward_product_bytes.restype = ctypes.c_longlong
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    a, b = (torch.randn(r, k, device="cuda", generator=gen).to(type) for r in (m, n))
+    for turned in (0, 1, 2):
+        va, vb = a.t().contiguous() if turned == 2 else a, b.t().contiguous() if turned else b
+        try:
+            streamk.force_product_tile(*tile, 2)
+            assert streamk.product_plan(m, n, k, False, turned) == (*tile, 2)
+            room = lib.feedforward_product_bytes(m, n, k, 0, turned, 0)
+            assert room > 8 * m * n
+            want, _ = product(va, vb, m, n, k, turned, 8 * m * n)
+            for count in (-1, 0, 1, 64):
+                polls(count)
+                for garbage in (0, 255, 37):
+                    got, at = product(va, vb, m, n, k, turned, room, garbage)
+                    assert torch.equal(got, want)
+                # once more in what the last call left there
+                lib, L, P = streamk._lib, ctypes.c_longlong, ctypes.c_void_p
+                again = torch.full_like(got, float("nan"))
+                assert lib.feedforward_product(
+                    P(va.data_ptr()), P(vb.data_ptr()), P(again.data_ptr()), m, n, k, L(va.stride(0)), L(vb.stride(0)),
+                    L(n), turned, int(type == torch.bfloat16), P(at.data_ptr()), L(room), 0,
+                    P(torch.cuda.current_stream().cuda_stream)) == 0
+                assert torch.equal(again, want)
+        finally:
+            streamk.force_product_tile(0)
+        exact = a.double() @ b.double().t()
+        bound = k * FP32 * (a.double().abs() @ b.double().abs().t()) + half_step(type) * exact.abs()
+        within(want, exact, bound, type, 1.01)
+
+
+@gpu
+@pytest.mark.parametrize("tile", TILES[6:])
+def test_epilogues_of_slices_that_meet(tile, polls):
+    for type in TYPES:
+        for m, n, k in ((333, 528, 640), (100, 144, 1096)):
+            x, w, bias, residual, _ = make(m, n, k, type, 5)
+            for count in (-1, 0):
+                polls(count)
+                try:
+                    streamk.force_product_tile(*tile, 2)
+                    for i, form in enumerate(FORMS):
+                        oracle(x, w, bias, residual, form, 9, i).check_forward(call(x, w, bias, residual, form, 9, i))
+                    slopes = streamk._torch_binding.linear_full_slopes(x, w, bias, None, 2, 0.0, None, 0)[1]
+                    Full64(x, w, bias, "gelu", None).check_slopes(slopes)
+                    # the gated epilogue, and what it keeps, against its form in one slice
+                    h, sums = streamk._torch_binding.gated_sums(x, w, 1)
+                    streamk.force_product_tile(*tile, 1)
+                    h1, sums1 = streamk._torch_binding.gated_sums(x, w, 1)
+                finally:
+                    streamk.force_product_tile(0)
+                size = x.double().abs() @ w.double().abs().t()
+                off = 2 * k * FP32 * size.max() + 2.0 ** -22
+                half = n // 2
+                for c in range(0, half, 16):
+                    wide = min(16, half - c)
+                    for at in (2 * c, 2 * c + 16):
+                        assert ((sums[:, at:at + wide] - sums1[:, at:at + wide]).abs() <= off).all()
+                assert ((h.double() - h1.double()).abs() <= 4 * half_step(type) * h1.double().abs() + 8 * off * (1 + size.max())).all()
+
+
+@gpu
+def test_slices_that_meet_captured_and_on_two_streams():
+    a, b = (torch.randn(r, 4096, device="cuda").bfloat16() for r in (512, 1024))
+    try:
+        streamk.force_product_tile(256, 256, 2)
+        want = streamk.linear(a, b)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(3)]
+        graphs, outs = [], []
+        for stream in streams:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                outs.append([streamk.linear(a, b) for _ in range(3)])
+            graphs.append(graph)
+        for _ in range(4):
+            for out in outs:
+                for o in out:
+                    o.zero_()
+            torch.cuda.synchronize()
+            eager = []
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+                    eager.append(streamk.linear(a, b))
+            torch.cuda.synchronize()
+            assert all(torch.equal(o, want) for out in outs for o in out)
+            assert all(torch.equal(o, want) for o in eager)
+    finally:
+        streamk.force_product_tile(0)
