@@ -63,8 +63,8 @@ void launch_gated_grad(const GatedGradArgs& a, bool bf, hipStream_t stream) {
 namespace {
 
 constexpr int kRunThreads = 256;
-constexpr int kRunGroups = 2048;  // workgroups that the runs make up, eight to a compute unit
-constexpr int kRunRows = 4;       // ... rows that a thread has at least
+constexpr int kRunGroups = 4096;  // workgroups that the runs make up, at most
+constexpr int kRunRows = 2;       // rows that a thread has, at least
 
 // threads beside each other along a row, eight columns each
 __host__ __device__ __forceinline__ int run_width(int n) {
@@ -92,7 +92,8 @@ __global__ __launch_bounds__(kRunThreads) void linear_grad_kernel(LinearGradArgs
     for (long long r = first + r0; r < end; r += high) {
       const i4 dy = *(const i4*)((const half_t*)p.dy + (size_t)r * p.lddy + col);
       i4 slopes, bits;
-      if (p.slopes) slopes = *(const i4*)(p.slopes + (size_t)r * p.ldslopes + col);
+      // (read this once, and written a forward pass ago)
+      if (p.slopes) slopes = __builtin_nontemporal_load((const i4*)(p.slopes + (size_t)r * p.ldslopes + col));
       if (p.drop.below) bits = drop_bits((unsigned long long)r * (unsigned)(p.n >> 3) + (unsigned)(col >> 3), key);
       i4 dz;
 #pragma unroll

@@ -95,10 +95,17 @@ __device__ __forceinline__ f4 drop4(f4 v, i2 bits, const DropArgs& a) {
 }
 
 // kFull, four columns of a row of C by themselves: where a lane has no others of their group of
-// eight, and makes its bits alone
+// eight, and makes its bits alone.  Bias and residual are fetched ahead of the sums.
+struct FullOperands {
+  i2 bias, residual;
+  __device__ __forceinline__ void fetch(const ProductArgs& p, int row, int col) {
+    if (p.bias) bias = *(const i2*)((const half_t*)p.bias + col);
+    if (p.residual) residual = *(const i2*)((const half_t*)p.residual + (size_t)row * p.ldr + col);
+  }
+};
 template <bool BF>
-__device__ __forceinline__ void finish_full(const ProductArgs& p, int row, int col, f4 v) {
-  if (p.bias) v += widen4<BF>(*(const i2*)((const half_t*)p.bias + col));
+__device__ __forceinline__ void finish_full(const ProductArgs& p, int row, int col, f4 v, const FullOperands& o) {
+  if (p.bias) v += widen4<BF>(o.bias);
   if (p.act != kActNone) {
     i2 slopes;
     v = p.act == kActGelu ? act4<kActGelu>(v, &slopes) : act4<kActSilu>(v, &slopes);
@@ -108,7 +115,7 @@ __device__ __forceinline__ void finish_full(const ProductArgs& p, int row, int c
     const i4 bits = drop_bits((unsigned long long)row * (unsigned)(p.N >> 3) + (unsigned)(col >> 3), DropKey(p.drop));
     v = drop4(v, col & 4 ? (i2){bits[2], bits[3]} : (i2){bits[0], bits[1]}, p.drop);
   }
-  if (p.residual) v += widen4<BF>(*(const i2*)((const half_t*)p.residual + (size_t)row * p.ldr + col));
+  if (p.residual) v += widen4<BF>(o.residual);
   *(i2*)((half_t*)p.C + (size_t)row * p.ldc + col) = product_round<BF>(v);
 }
 

@@ -343,6 +343,8 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(ProductArgs p) {
   const int m = (int)(at / quads), col = 4 * (int)(at - (long long)m * quads);
   if (m >= p.M) return;
   const float* const from = p.part + (size_t)m * p.ldpart + (GATED ? pre_col(col) : col);
+  FullOperands full;
+  if constexpr (FINISH == kFull) full.fetch(p, m, col);
   f4 part[SLICES], part_up[GATED ? SLICES : 1];
 #pragma unroll
   for (int s = 0; s < SLICES; s++) {
@@ -365,7 +367,7 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(ProductArgs p) {
     v = act_mul4(v, up, p.act);
   }
   if constexpr (FINISH == kFull)
-    finish_full<BF>(p, m, col, v);
+    finish_full<BF>(p, m, col, v, full);
   else
     *(i2*)((half_t*)p.C + (size_t)m * p.ldc + col) = product_round<BF>(v);
 }
