@@ -9,7 +9,7 @@
 // 16 bits for the products, and the bias's gradient, its sum over rows, of the unrounded values in
 // fp32.  A workgroup takes 256 columns (fewer where there are fewer) of a run of rows, 16 bytes a
 // thread; its column sums meet in LDS and go to `partials`, and a second launch adds the runs' in their
-// order.
+// order, unless there is one.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -73,6 +73,14 @@ __host__ __device__ __forceinline__ int run_width(int n) {
   return width;
 }
 
+template <bool BF>
+__device__ __forceinline__ void store_bias(void* dbias, int column, float sum) {
+  if constexpr (BF)
+    ((__bf16*)dbias)[column] = (__bf16)sum;
+  else
+    ((half_t*)dbias)[column] = (half_t)sum;
+}
+
 }  // namespace
 
 template <bool BF>
@@ -113,7 +121,7 @@ __global__ __launch_bounds__(kRunThreads) void linear_grad_kernel(LinearGradArgs
       if (p.dz) *(i4*)((half_t*)p.dz + (size_t)r * p.lddz + col) = dz;
     }
   }
-  if (!p.partials) return;
+  if (!p.dbias) return;
 #pragma unroll
   for (int e = 0; e < 8; e++) room[threadIdx.x][e] = sum[e];
   __syncthreads();
@@ -123,7 +131,10 @@ __global__ __launch_bounds__(kRunThreads) void linear_grad_kernel(LinearGradArgs
     if (column >= p.n) continue;
     float s = room[at / 8][at % 8];
     for (int r = 1; r < high; r++) s += room[r * width + at / 8][at % 8];
-    p.partials[(size_t)part * p.n + column] = s;
+    if (p.partials)
+      p.partials[(size_t)part * p.n + column] = s;
+    else
+      store_bias<BF>(p.dbias, column, s);
   }
 }
 
@@ -143,10 +154,7 @@ __global__ __launch_bounds__(1024) void bias_sums_kernel(LinearGradArgs p, int p
   s = room[0][lane];
 #pragma unroll
   for (int i = 1; i < 16; i++) s += room[i][lane];
-  if constexpr (BF)
-    ((__bf16*)p.dbias)[c] = (__bf16)s;
-  else
-    ((half_t*)p.dbias)[c] = (half_t)s;
+  store_bias<BF>(p.dbias, c, s);
 }
 
 int linear_grad_parts(int m, int n) {
@@ -160,6 +168,7 @@ void launch_linear_grad(LinearGradArgs a, bool bf, hipStream_t stream) {
   int parts = linear_grad_parts(a.m, a.n);
   a.rows_per_part = ceil_div(a.m, parts);
   parts = ceil_div(a.m, a.rows_per_part);
+  if (parts == 1) a.partials = nullptr;  // (its sums are the bias's)
   const dim3 grid(ceil_div(a.n, 8 * width), parts), sums(ceil_div(a.n, 64));
   if (bf)
     hipLaunchKernelGGL(linear_grad_kernel<true>, grid, dim3(kRunThreads), 0, stream, a);

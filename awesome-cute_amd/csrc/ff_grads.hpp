@@ -19,8 +19,8 @@ struct LinearGradArgs {
   const void* dy;    // (m x n)
   const unsigned short* slopes;  // null (no activation), or the forward pass's (m x n)
   void* dz;          // null, or (m x n)
-  void* dbias;       // n elements, with partials
-  float* partials;   // null, or linear_grad_parts(m, n) rows of n
+  void* dbias;       // null, or n elements
+  float* partials;   // linear_grad_parts(m, n) rows of n, where dbias is wanted and these are more than one
   long long lddy, ldslopes, lddz;
   int m, n, rows_per_part;
   DropArgs drop;

@@ -401,7 +401,8 @@ int feedforward_linear(const void* x, const void* w, void* y, const void* bias, 
 
 long long feedforward_linear_grad_bytes(int m, int n) {
   if (check_sizes(m, n, 0, FEEDFORWARD_FP16) != FEEDFORWARD_OK) return -1;
-  return m > 0 && n > 0 ? 4LL * n * linear_grad_parts(m, n) : 0;
+  const int parts = m > 0 && n > 0 ? linear_grad_parts(m, n) : 0;
+  return parts > 1 ? 4LL * n * parts : 0;
 }
 
 int feedforward_linear_grad(const void* dy, const void* slopes, void* dz, void* dbias, int m, int n, long long lddy,
@@ -415,10 +416,11 @@ int feedforward_linear_grad(const void* dy, const void* slopes, void* dz, void* 
   if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
   if (!dy || (!dz && !dbias)) return fail(FEEDFORWARD_ERR_SHAPE, "dy, or every output, is missing");
-  if (dbias && (!partials || ((uintptr_t)partials & 3) || partial_bytes < feedforward_linear_grad_bytes(m, n)))
-    return fail(FEEDFORWARD_ERR_SHAPE, "the sums over rows need %lld bytes of scratch", feedforward_linear_grad_bytes(m, n));
+  const long long sums = dbias ? feedforward_linear_grad_bytes(m, n) : 0;
+  if (sums > 0 && (!partials || ((uintptr_t)partials & 3) || partial_bytes < sums))
+    return fail(FEEDFORWARD_ERR_SHAPE, "the sums over rows need %lld bytes of scratch", sums);
   a.dy = dy, a.slopes = (const unsigned short*)slopes, a.dz = dz, a.dbias = dbias;
-  a.partials = dbias ? (float*)partials : nullptr;
+  a.partials = sums > 0 ? (float*)partials : nullptr;
   a.lddy = lddy, a.ldslopes = ldslopes, a.lddz = lddz;
   a.m = m, a.n = n;
   return on_device(dev, [&](int) { launch_linear_grad(a, type == FEEDFORWARD_BF16, (hipStream_t)stream); });

@@ -392,7 +392,9 @@ PyObject* py_dense(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 constexpr int64_t kFarthest = 1 << 21;
 struct Matrix {
   at::Tensor t;
+  void* there = nullptr;  // (without a tensor)
   long long ld = 0;
+  Matrix(void* at, long long ld) : there(at), ld(ld) {}
   // y as `rows` rows of `width`.  (One that is whole is taken without a view: views of all the
   // operands take the host 5 us of a backward pass.)
   Matrix(const at::Tensor& y, int64_t rows, int64_t width) : t(y) {
@@ -411,7 +413,7 @@ struct Matrix {
     }
     ld = t.size(0) <= 1 || t.numel() == 0 ? (t.size(1) + 7) / 8 * 8 : t.stride(0);
   }
-  void* at() const { return t.data_ptr(); }
+  void* at() const { return t.defined() ? t.data_ptr() : there; }
 };
 
 // a gradient whose memory holds its values: autograd may hand over a view that is to be read negated
@@ -494,15 +496,17 @@ variable_list once_differentiable(variable_list&& grads, const char* name, std::
   return marked;
 }
 
-// Scratch for a product's partial sums, where its plan has any
+// Scratch for a product's partial sums, where its plan has any: its own, or memory that is there
 struct Room {
   at::Tensor t;
+  void* there = nullptr;
   long long bytes;
+  Room(void* at, long long bytes) : there(at), bytes(bytes) {}
   Room(const at::Tensor& like, int64_t m, int64_t n, int64_t k, bool gated, int turned)
       : bytes(feedforward_product_bytes((int)m, (int)n, (int)k, gated, turned, like.get_device())) {
     if (bytes > 0) t = at::empty({bytes / 4}, options_as(like).dtype(at::kFloat));
   }
-  void* at() const { return t.defined() ? t.data_ptr() : nullptr; }
+  void* at() const { return t.defined() ? t.data_ptr() : there; }
 };
 
 // act(x G^T) * (x U^T), and with `keep` both sums (otherwise undefined)
@@ -535,21 +539,21 @@ at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w) {
 }
 
 // The gradients of x (m, k) and w (r, k) from that of their product, d (m, r): dx = d w and
-// dw = d^T x, sums over r and over m.
+// dw = d^T x, sums over r and over m.  `shared`, if there: room for one of the two at a time.
 void product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, const at::Tensor& dx,
-                   const at::Tensor& dw) {
+                   const at::Tensor& dw, const Room* shared = nullptr) {
   const int64_t k = w.size(1), m = x.numel() / k, r = w.size(0);
   const int type = type_code(x), dev = x.get_device();
   void* const st = current_stream(dev);
   if (dx.defined()) {
     const Matrix b(w, r, k);
-    const Room room(x, m, k, r, false, FEEDFORWARD_TURN_B);
+    const Room room = shared ? *shared : Room(x, m, k, r, false, FEEDFORWARD_TURN_B);
     feedforward_check(feedforward_product(d.at(), b.at(), dx.data_ptr(), (int)m, (int)k, (int)r, d.ld, b.ld, k,
                                           FEEDFORWARD_TURN_B, type, room.at(), room.bytes, dev, st));
   }
   if (dw.defined()) {
     const Matrix a(x, m, k);
-    const Room room(x, r, k, m, false, FEEDFORWARD_TURN_BOTH);
+    const Room room = shared ? *shared : Room(x, r, k, m, false, FEEDFORWARD_TURN_BOTH);
     feedforward_check(feedforward_product(d.at(), a.at(), dw.data_ptr(), (int)r, (int)k, (int)m, d.ld, a.ld, k,
                                           FEEDFORWARD_TURN_BOTH, type, room.at(), room.bytes, dev, st));
   }
@@ -796,22 +800,26 @@ bool drop_arguments(PyObject* const* args, Drop* out) {
   return to_int64(args[1], "seed", &out->seed);
 }
 
-// The leaf that a gradient goes to, where the backward pass has no other use for the input
-// (check_capture wants it, and a leaf's accumulator, which the graph holds, holds the leaf)
-void keep_leaf(AutogradContext* ctx, const char* name, const at::Tensor& t) {
-  if (t.defined() && t.is_leaf() && t.requires_grad()) ctx->saved_data[name] = t;
+// What a forward pass keeps besides the tensors that it saves, as one object (an entry of the context's
+// dictionary for each takes the host 0.1 to 0.2 us, both ways).  The leaves are what gradients go to that the
+// backward pass has no other use for: check_capture wants them, and a leaf's accumulator, which the
+// graph holds, holds the leaf.
+struct Kept : torch::CustomClassHolder {
+  int act = 0;
+  Drop drop;  // (its seed in memory is saved: if that has been written since, asking for it raises)
+  at::Tensor leaves[2];
+  bool there[2] = {};
+  void input(int i, const at::Tensor& t) {
+    there[i] = t.defined();
+    if (t.defined() && t.is_leaf() && t.requires_grad()) leaves[i] = t;
+  }
+};
+void keep(AutogradContext* ctx, c10::intrusive_ptr<Kept> kept) {
+  kept->drop.seed_at = at::Tensor();
+  ctx->saved_data["kept"] = c10::IValue::make_capsule(std::move(kept));
 }
-at::Tensor kept_leaf(AutogradContext* ctx, const char* name) {
-  const auto at = ctx->saved_data.find(name);
-  return at == ctx->saved_data.end() ? at::Tensor() : at->second.toTensor();
-}
-void keep_drop(AutogradContext* ctx, const Drop& drop) {
-  ctx->saved_data["p"] = drop.p;
-  ctx->saved_data["seed"] = drop.seed;
-  ctx->saved_data["site"] = drop.site;
-}
-Drop kept_drop(AutogradContext* ctx, const at::Tensor& seed_at) {
-  return {ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), ctx->saved_data["site"].toInt(), seed_at};
+c10::intrusive_ptr<Kept> kept_by(AutogradContext* ctx) {
+  return c10::static_intrusive_pointer_cast<Kept>(ctx->saved_data.at("kept").toCapsule());
 }
 
 struct FullInputs {
@@ -886,24 +894,31 @@ std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& 
   const bool products = want[0] || want[1];
   if (!products && !want[2]) return out;
   const Matrix d(plain_values(dy), m, n);
-  // without an activation and a mask the sums' gradient is dy
-  std::optional<Matrix> dz;
-  if (products && (in.act != 0 || in.drop.on())) {
-    const int64_t ld = (n + 63) / 64 * 64;  // rows of whole cache lines
-    dz.emplace(empty_as(in.x, {m, ld}), m, ld);
-  }
-  if (dz || want[2]) {
-    at::Tensor partials;
-    long long bytes = 0;
-    if (want[2]) {
-      bytes = feedforward_linear_grad_bytes((int)m, (int)n);
-      if (bytes > 0) partials = at::empty({bytes / 4}, options_as(in.x).dtype(at::kFloat));
-    }
+  // One allocation holds what lives no longer than this call: the sums' gradient, which without an
+  // activation and a mask is dy, the bias's partial sums, and room for the products, one after the other.
+  // (Each of its own takes the host 1.2 us of a pass that on small problems is the host's.)
+  const bool other = products && (in.act != 0 || in.drop.on());
+  const int64_t ld = (n + 63) / 64 * 64;  // rows of whole cache lines
+  const long long dz_bytes = other ? 2 * m * ld : 0;
+  const long long sum_bytes = want[2] ? (feedforward_linear_grad_bytes((int)m, (int)n) + 255) / 256 * 256 : 0;
+  const auto product_bytes = [&](int64_t rows, int64_t sum, int turned) {
+    return feedforward_product_bytes((int)rows, (int)in.k, (int)sum, 0, turned, dev);
+  };
+  const long long room_bytes = std::max(want[0] ? product_bytes(m, n, FEEDFORWARD_TURN_B) : 0,
+                                        want[1] ? product_bytes(n, m, FEEDFORWARD_TURN_BOTH) : 0);
+  at::Tensor scratch;
+  if (dz_bytes + sum_bytes + room_bytes > 0)
+    scratch = at::empty({dz_bytes + sum_bytes + room_bytes}, options_as(in.x).dtype(at::kByte));
+  char* const base = (char*)at_of(scratch);
+  const Matrix dz = other ? Matrix(base, ld) : d;
+  if (other || want[2]) {
     const feedforward_drop drop = in.drop.plain();
-    feedforward_check(feedforward_linear_grad(d.at(), at_of(slopes), dz ? dz->at() : nullptr, at_of(out[2]),
-                                              (int)m, (int)n, d.ld, n, dz ? dz->ld : 0, type_code(in.x), &drop, at_of(partials), bytes, dev, current_stream(dev)));
+    feedforward_check(feedforward_linear_grad(d.at(), at_of(slopes), other ? base : nullptr, at_of(out[2]), (int)m, (int)n,
+                                              d.ld, n, ld, type_code(in.x), &drop, sum_bytes ? base + dz_bytes : nullptr,
+                                              sum_bytes, dev, current_stream(dev)));
   }
-  if (products) product_grads(in.x, in.w, dz ? *dz : d, out[0], out[1]);
+  const Room room(room_bytes > 0 ? base + dz_bytes + sum_bytes : nullptr, room_bytes);
+  if (products) product_grads(in.x, in.w, dz, out[0], out[1], &room);
   return out;
 }
 
@@ -914,13 +929,13 @@ struct FullFunction : torch::autograd::Function<FullFunction> {
     FullInputs in{x, w, bias.value_or(at::Tensor()), residual.value_or(at::Tensor()), (int)act,
                   Drop{p, seed, site, seed_at.value_or(at::Tensor())}};
     auto [y, slopes] = full_forward(in, true);
-    // (a seed in memory that has been written since raises)
     ctx->save_for_backward({x, w, slopes, in.drop.seed_at});
-    ctx->saved_data["act"] = act;
-    keep_drop(ctx, in.drop);
-    keep_leaf(ctx, "bias", in.bias);
-    keep_leaf(ctx, "residual", in.residual);
-    ctx->saved_data["inputs"] = (int64_t)(in.bias.defined() | in.residual.defined() << 1);
+    auto kept = c10::make_intrusive<Kept>();
+    kept->act = in.act;
+    kept->drop = in.drop;
+    kept->input(0, in.bias);
+    kept->input(1, in.residual);
+    keep(ctx, std::move(kept));
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -928,17 +943,15 @@ struct FullFunction : torch::autograd::Function<FullFunction> {
     variable_list out(9);
     if (grads[0].defined()) {
       c10::AutoGradMode off(false);
-      const int64_t inputs = ctx->saved_data["inputs"].toInt();
-      const bool has_bias = inputs & 1, has_residual = inputs & 2;
-      FullInputs in{saved[0], saved[1], at::Tensor(), at::Tensor(), (int)ctx->saved_data["act"].toInt(),
-                    kept_drop(ctx, saved[3])};
-      const at::Tensor bias = kept_leaf(ctx, "bias"), residual = kept_leaf(ctx, "residual");
+      const auto kept = kept_by(ctx);
+      FullInputs in{saved[0], saved[1], at::Tensor(), at::Tensor(), kept->act, kept->drop};
+      in.drop.seed_at = saved[3];
       // (the context counts the inputs that are there)
       const std::array<bool, 3> want = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
-                                        has_bias && ctx->needs_input_grad(2)};
-      auto g = full_backward(grads[0], saved[2], in, want, {&in.x, &in.w, &bias, &residual});
+                                        kept->there[0] && ctx->needs_input_grad(2)};
+      auto g = full_backward(grads[0], saved[2], in, want, {&in.x, &in.w, &kept->leaves[0], &kept->leaves[1]});
       for (int i = 0; i < 3; i++) out[i] = g[i];
-      if (has_residual && ctx->needs_input_grad(2 + has_bias)) out[3] = grads[0];
+      if (kept->there[1] && ctx->needs_input_grad(2 + kept->there[0])) out[3] = grads[0];
     }
     return once_differentiable(std::move(out), "linear", {&grads, &saved});
   }
@@ -987,10 +1000,11 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
     const DropoutInputs in{x, residual.value_or(at::Tensor()), Drop{p, seed, site, seed_at.value_or(at::Tensor())}};
     at::Tensor y = dropout_forward(in);
     ctx->save_for_backward({in.drop.seed_at});
-    keep_drop(ctx, in.drop);
-    keep_leaf(ctx, "x", x);
-    keep_leaf(ctx, "residual", in.residual);
-    ctx->saved_data["added"] = in.residual.defined();
+    auto kept = c10::make_intrusive<Kept>();
+    kept->drop = in.drop;
+    kept->input(0, x);
+    kept->input(1, in.residual);
+    keep(ctx, std::move(kept));
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -998,9 +1012,11 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
     variable_list out(6);
     if (grads[0].defined()) {
       c10::AutoGradMode off(false);
-      const at::Tensor x = kept_leaf(ctx, "x"), residual = kept_leaf(ctx, "residual");
-      if (ctx->needs_input_grad(0)) out[0] = dropout_backward(grads[0], kept_drop(ctx, saved[0]), {&x, &residual});
-      if (ctx->saved_data["added"].toBool() && ctx->needs_input_grad(1)) out[1] = grads[0];
+      const auto kept = kept_by(ctx);
+      Drop drop = kept->drop;
+      drop.seed_at = saved[0];
+      if (ctx->needs_input_grad(0)) out[0] = dropout_backward(grads[0], drop, {&kept->leaves[0], &kept->leaves[1]});
+      if (kept->there[1] && ctx->needs_input_grad(1)) out[1] = grads[0];
     }
     return once_differentiable(std::move(out), "dropout", {&grads, &saved});
   }

@@ -116,7 +116,7 @@ int feedforward_linear_grad(const void *dy, const void *slopes, void *dz, void *
                             long long lddy, long long ldslopes, long long lddz, int type,
                             const feedforward_drop *drop, void *partials, long long partial_bytes,
                             int dev, void *stream);
-/* -1 for sizes that are refused; no GPU touched */
+/* -1 for sizes that are refused, 0 where few rows need none; no GPU touched */
 long long feedforward_linear_grad_bytes(int m, int n);
 
 /* y = residual + drop(x), or drop(x) without one; `count` elements (at most 2^40) of any type, each

@@ -205,12 +205,14 @@ def test_codes_of_the_entries():
     assert grad(m=0) == 0 and grad(n=0) == 0 and grad(m=0, dy=None, dz=None) == 0
     for bad in (dict(m=-1), dict(n=12), dict(lddy=4), dict(dz=8), dict(lddz=0), dict(slopes=8),
                 dict(slopes=16, lds=4), dict(type=2), dict(p=-1.0),
-                dict(dy=None), dict(dz=None), dict(dbias=16), dict(dbias=16, partials=16, count=many(4, 8) - 1),
-                dict(dbias=16, partials=18, count=many(4, 8))):
+                dict(dy=None), dict(dz=None), dict(m=4096, dbias=16),
+                dict(m=4096, dbias=16, partials=16, count=many(4096, 8) - 1),
+                dict(m=4096, dbias=16, partials=18, count=many(4096, 8))):
         assert grad(**bad) == 1, bad
     assert many(-1, 8) == -1 and many(4, 12) == -1 and many(0, 8) == 0 and many(4, 0) == 0
-    for m, n in ((1, 8), (1 << 20, 8), (2048, 10752), (7, 1 << 21), (0x7fffffff, 8)):
-        assert 4 * n <= many(m, n) <= 4 * n * 4096
+    assert many(1, 8) == 0 and many(7, 1 << 21) == 0
+    for m, n in ((1 << 20, 8), (2048, 10752), (300, 1 << 14), (0x7fffffff, 8)):
+        assert 4 * n < many(m, n) <= 4 * n * 4096
 
 
 def test_fake_tensors_record_the_operators():
