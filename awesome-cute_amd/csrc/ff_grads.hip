@@ -157,17 +157,17 @@ __global__ __launch_bounds__(1024) void bias_sums_kernel(LinearGradArgs p, int p
   store_bias<BF>(p.dbias, c, s);
 }
 
+// (rows count in 64 bits: with what rounds them up they may pass an int)
+static int runs_of(int m, long long rows) { return (int)((m + rows - 1) / rows); }
 int linear_grad_parts(int m, int n) {
   const int width = run_width(n), across = ceil_div(n, 8 * width), high = kRunThreads / width;
-  const int most = std::max(1, kRunGroups / across);
-  return std::max(1, std::min(most, ceil_div(m, kRunRows * high)));
+  return std::max(1, std::min(kRunGroups / across, runs_of(m, kRunRows * high)));
 }
 
 void launch_linear_grad(LinearGradArgs a, bool bf, hipStream_t stream) {
   const int width = run_width(a.n);
-  int parts = linear_grad_parts(a.m, a.n);
-  a.rows_per_part = ceil_div(a.m, parts);
-  parts = ceil_div(a.m, a.rows_per_part);
+  a.rows_per_part = runs_of(a.m, linear_grad_parts(a.m, a.n));
+  const int parts = runs_of(a.m, a.rows_per_part);
   if (parts == 1) a.partials = nullptr;  // (its sums are the bias's)
   const dim3 grid(ceil_div(a.n, 8 * width), parts), sums(ceil_div(a.n, 64));
   if (bf)
