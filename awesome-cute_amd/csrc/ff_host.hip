@@ -214,7 +214,7 @@ Planned plan_with_room(int m, int n, int k, bool gated, Layout layout, int cus) 
 
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
-constexpr long long kMostDropped = 1LL << 40;  // elements of a call (a launch's grid)
+constexpr long long kMostDropped = 1LL << 34;  // elements of a call: a launch has fewer than 2^32 threads
 constexpr int kWidest = 1 << 21;  // elements from one row to the next
 
 // a matrix of 16-bit elements as the kernels address it: rows start on 16 bytes

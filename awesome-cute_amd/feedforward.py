@@ -85,7 +85,7 @@ def dropout(x, p, seed, *, site=0, residual=None):
     """Every element of x zero with probability p (whatever its value), multiplied by 1 / (1 - p)
     otherwise, and added to `residual`, if that is given; rounded once.
 
-    x: torch.half, torch.bfloat16 or torch.float, any shape; residual of x's shape and type.  Strided
+    x: torch.half, torch.bfloat16 or torch.float, any shape of up to 2^34 elements; residual of x's shape and type.  Strided
     tensors are copied.  p is rounded to a multiple of 2^-16.  The mask is a function of `seed`, an int of
     64 bits with its sign or one torch.int64 on x's device (which a captured graph can advance),
     of `site`, 0 to 2^32 - 1, which distinguishes masks of one seed, and of the elements' places; include/

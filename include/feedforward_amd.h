@@ -99,7 +99,8 @@ typedef struct feedforward_drop {
   unsigned site;            /* distinguishes masks that share a seed */
 } feedforward_drop;
 
-/* y (m x n) = residual + drop(act(x w^T + bias)), x (m x k), w (n x k), k > 0.  Null: bias (n
+/* y (m x n) = residual + drop(act(x w^T + bias)), x (m x k), w (n x k), k > 0; y overlaps none of
+ * them.  Null: bias (n
  * elements), residual (m x n), drop, and slopes, which keeps act' of x w^T + bias for the backward pass
  * (m x n numbers of 16 bits in the library's own form).  activation 0: none, and no slopes. */
 int feedforward_linear(const void *x, const void *w, void *y, const void *bias, const void *residual,
@@ -119,7 +120,7 @@ int feedforward_linear_grad(const void *dy, const void *slopes, void *dz, void *
 /* -1 for sizes that are refused, 0 where few rows need none; no GPU touched */
 long long feedforward_linear_grad_bytes(int m, int n);
 
-/* y = residual + drop(x), or drop(x) without one; `count` elements (at most 2^40) of any type, each
+/* y = residual + drop(x), or drop(x) without one; `count` elements (at most 2^34) of any type, each
  * matrix one contiguous row.  y may be x or the residual itself.  The gradient of x is drop(dy). */
 int feedforward_dropout(const void *x, const void *residual, void *y, long long count, int type,
                         const feedforward_drop *drop, int dev, void *stream);

@@ -113,7 +113,7 @@ def test_codes_of_the_entry():
         return lib.feedforward_dropout(P(x), P(residual), P(y), L(count), type, ctypes.byref(drop), 0, None)
 
     assert call(0) == 0 and call(0, x=None, y=None) == 0
-    assert call(-1) == 1 and call(2 ** 40 + 1) == 1 and call(8, type=3) == 1
+    assert call(-1) == 1 and call(2 ** 34 + 1) == 1 and call(8, type=3) == 1
     for p in (-0.1, 1.1, float("nan"), float("inf")):
         assert call(0, p=p) == 1 and b"probability" in lib.feedforward_last_error()
     assert call(8, x=17) == 1 and call(8, residual=17) == 1 and call(8, y=18, type=2) == 1

@@ -518,6 +518,14 @@ def test_infinities_and_nan(m):
         got = torch.autograd.grad(call(*leaves, residual, form), leaves, ndy)
         want = torch.autograd.grad(call(*leaves, residual, form), leaves, dy)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # NaN in a row of x is in that row's gradients, where they are kept, and in no other's
+    for act in ("silu", "gelu"):
+        dirty = x.clone()
+        dirty[m // 2, 5] = float("nan")
+        dirty.requires_grad_()
+        g, = torch.autograd.grad(streamk.linear(dirty, w, bias, act), dirty, dy)
+        rows = torch.arange(m, device="cuda") != m // 2
+        assert torch.isfinite(g[rows]).all() and g[m // 2].isnan().all()
     # far out the activations are their arguments and zero, their slopes one and zero
     far = torch.full((1, 8), 200.0, device="cuda").half().requires_grad_()
     eye = torch.eye(8, device="cuda").half()
