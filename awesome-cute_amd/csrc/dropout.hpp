@@ -9,7 +9,7 @@
 // of 2^-16, and the mean is kept exactly.  A select, no product: what is dropped is zero, infinite
 // and undefined values as well.
 //
-// Seven rounds, the fewest that pass the paper's tests (its table 2).  Sixteen bits an element and
+// Seven rounds, the fewest with which the paper finds it to pass its tests.  Sixteen bits an element and
 // eight to a group: a group is 16 bytes of 16-bit elements, a lane's piece of memory.
 #pragma once
 #include <hip/hip_runtime.h>

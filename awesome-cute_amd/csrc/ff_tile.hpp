@@ -113,7 +113,7 @@ __device__ __forceinline__ void full_bits(const ProductArgs& p, const DropKey& k
 
 // kFull: what a wave brings to the tile's LDS image, of NI row blocks and NJ operands, from their sums v.
 // `out`: this lane's row of the image in the first block, `slopes_at` bytes further on that of the slopes
-// (stored from the registers, 8 bytes of a row a lane, they took 19 us of 174, 2048 x 10752 x 4096); m, col:
+// (stored from the registers, 8 bytes of a row a lane: 2048 x 10752 x 4096 174 us, so 169); m, col:
 // its row and first column of the tile, of which rows x cols are there.  Bias and residual, fetched ahead,
 // are past them the last ones, and are not stored.  (The bias ahead of the residual, and of the main loop: loads come
 // back in order, and what waits for a bias behind a residual waits for both.)

@@ -845,3 +845,110 @@ def test_slices_that_meet_captured_and_on_two_streams():
             assert all(torch.equal(o, want) for o in eager)
     finally:
         streamk.force_product_tile(0)
+
+
+# --- sizes and ways of calling at the ends ---------------------------------------------------
+
+@gpu
+def test_results_of_more_than_32_bits():
+    """2^31 elements and more, 4 GiB each of result, residual and gradient: the last rows, their mask and their
+    gradients."""
+    m, n, k = (1 << 16) + 40, (1 << 15) + 8, 64
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x, w, bias = (torch.randn(s, device="cuda", generator=gen).bfloat16() for s in ((m, k), (n, k), (n,)))
+    residual = torch.empty((m, n), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    for t in (x, w, bias):
+        t.requires_grad_()
+    y = streamk.linear(x, w, bias, "silu", residual, dropout=0.5, seed=77, site=3)
+    grads = torch.autograd.grad(y, (x, w, bias), residual)
+    y = y.detach()
+    last = slice(m - 16, m)
+    with torch.no_grad():
+        ref = Full64(x[last], w, bias, "silu", residual[last])
+        # the mask of these rows, element by element of the generator
+        first = (m - 16) * n
+        assert first % 8 == 0
+        group = np.arange(first // 8, m * n // 8, dtype=np.uint64)
+        c = [group & _masks.LOW, group >> np.uint64(32), np.full_like(group, 3), np.zeros_like(group)]
+        for r in range(7):
+            k0, k1 = np.uint64((77 + r * _masks.W0) % 2 ** 32), np.uint64(r * _masks.W1 % 2 ** 32)
+            a, b = c[0] * np.uint64(_masks.M0), c[2] * np.uint64(_masks.M1)
+            c = [b >> np.uint64(32) ^ c[1] ^ k0, b & _masks.LOW, a >> np.uint64(32) ^ c[3] ^ k1, a & _masks.LOW]
+        words = np.stack(c, axis=1)
+        bits = np.stack([words & np.uint64(0xffff), words >> np.uint64(16)], axis=2).reshape(16, n)
+        ref.factor = torch.from_numpy((bits >= 32768).astype(np.float64) * 2).cuda()
+        ref.check_forward(y[last])
+        ref.check_grads(residual[last], dx=grads[0][last])
+    assert all(torch.isfinite(g).all() for g in grads)
+
+
+@gpu
+def test_only_the_residual_wants_a_gradient():
+    x, w, bias, residual, dy = make(20, 24, 16, torch.float16, 1)
+    residual.requires_grad_()
+    y = streamk.linear(x, w, bias, "silu", residual, dropout=0.5, seed=1)
+    assert torch.equal(torch.autograd.grad(y, residual, dy)[0], dy)
+    y = feedforward.dropout(dy, 0.5, 1, residual=residual)
+    assert torch.equal(torch.autograd.grad(y, residual, dy)[0], dy)
+
+
+@gpu
+def test_backward_twice_and_accumulated():
+    x, w, bias, residual, dy = make(70, 72, 136, torch.bfloat16, 1)
+    leaves = [t.requires_grad_() for t in (x, w, bias, residual)]
+    y = streamk.linear(x, w, bias, "gelu", residual, dropout=0.25, seed=3)
+    want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    y.backward(dy, retain_graph=True)
+    assert all(torch.equal(t.grad, g) for t, g in zip(leaves, want))
+    kept = dy.clone()
+    y.backward(dy)
+    assert all(torch.equal(t.grad, g + g) for t, g in zip(leaves, want))
+    assert torch.equal(dy, kept)  # the residual's gradient is dy, and accumulating does not write to it
+
+
+@gpu
+def test_threads_at_once():
+    import threading
+    cases = [make(m, 264, 4160, torch.bfloat16, m) for m in (1, 70, 300, 600)]
+    form = (True, "gelu", True, 0.25)
+
+    def step(c):
+        leaves = [t.detach().requires_grad_() for t in c[:4]]
+        y = call(*leaves, form)
+        return (y.detach(), *torch.autograd.grad(y, leaves, c[4]))
+
+    want = [step(c) for c in cases]
+    torch.cuda.synchronize()
+    got = [None] * len(cases)
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i] = step(cases[i])
+        torch.cuda.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+@gpu
+def test_a_compiled_block_and_a_checkpointed_one():
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(0)
+    mlp = feedforward.Mlp(64, 136, dropout=0.2, device="cuda")
+    x = torch.randn((3, 37, 64), device="cuda").bfloat16().requires_grad_()
+    params = [x, *mlp.parameters()]
+
+    def loss(f):
+        return torch.autograd.grad(f(x)[1].float().square().sum(), params)
+
+    want = loss(lambda t: mlp(t, seed=5))
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda t: mlp(t, seed=5), backend="aot_eager", fullgraph=True)
+    assert all(torch.equal(a, b) for a, b in zip(loss(compiled), want))
+    again = loss(lambda t: checkpoint(lambda u: mlp(u, seed=5), t, use_reentrant=False))
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
