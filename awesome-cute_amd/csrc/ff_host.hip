@@ -92,6 +92,12 @@ constexpr TileFit kFits[] = {
     {{96, 256}, 5.28, 0.594, 0.439, 4.03, 0.838}, {{128, 256}, 5.34, 0.748, 0.456, 4.59, 1.004},
     {{160, 256}, 7.68, 0.793, 0.380, 6.47, 1.094}, {{192, 256}, 8.23, 0.911, 0.424, 7.35, 1.256},
     {{224, 256}, 9.14, 1.044, 0.434, 8.56, 1.394}, {{256, 256}, 9.25, 1.104, 0.531, 9.57, 1.483}};
+// Tiles of full products (feedforward_linear) alone, beside those above: problems of a few 64 x 64 tiles.
+// Fitted to 400 problems of 23 to 4096 rows, widths of 64 to 11585 and depths of 64 to 8192, operands from
+// memory, and brought to the others' level by what these cost there.  On 500 more problems, drawn alike, 196 take
+// them, and 0.836 of the time (at best 0.60: 200 x 1024 x 2048 9.2 -> 6.1 us; at worst 1.12).
+// (Other products' plans, and with them their results' last bits, are as they were.)
+constexpr TileFit kSmallFits[] = {{{32, 32}, 4.05, 0.129, 0.031, 1.09, 0.138}, {{32, 64}, 4.18, 0.183, 0.088, 1.17, 0.214}};
 // The same of the kernel for few rows (ff_rows.hip) by its blocks of sixteen rows of A, a stage
 // being the 64 k-values of one of its four waves: one block of product columns to a workgroup, or
 // two.  Fitted to 12000 problems of 1 to 64 rows, widths of 64 to 14336, depths of 64 to 8192,
@@ -114,7 +120,10 @@ struct ProductPlan {
   int slices;
 };
 
-bool tile_takes(const FfTile& t, Layout layout) {
+bool tile_takes(const FfTile& t, Layout layout, Finish finish, int m) {
+  // (of 32 columns: where the kernel for few rows, whose tiles are named so too, does not compute)
+  if (t.rows == 32) return finish == kFull && (t.cols == 64 || (t.cols == 32 && m > kProductRows));
+  if (few_tile(t)) return false;
   return layout != kTurnBoth || t.rows != 96;  // (64, 128 or 256 columns of a turned operand)
 }
 
@@ -127,10 +136,11 @@ double fit_cost(const TileFit& f, long long groups, int stages, int cus) {
 }
 
 // room: bytes for partial sums
-ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, int cus, long long room) {
+ProductPlan choose_plan(int m, int n, int k, Finish finish, Layout layout, int cus, long long room) {
+  const bool gated = finish == kGated;
   const int columns = product_columns(n, gated), stages = ceil_div(k, kDnStageK);
   const bool few = layout == kRows && m <= kProductRows;
-  const bool forced = t_tile.rows > 0 && (few_tile(t_tile) ? few : tile_takes(t_tile, layout));
+  const bool forced = t_tile.rows > 0 && ((few && few_tile(t_tile)) || tile_takes(t_tile, layout, finish, m));
   ProductPlan best = {{64, 64}, 1};
   double least = 0.0;
   if (few)
@@ -142,9 +152,9 @@ ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, int cus,
         least = cost;
       }
     }
-  for (const TileFit& f : kFits) {
-    if (forced && (f.tile.rows != t_tile.rows || f.tile.cols != t_tile.cols)) continue;
-    if (!tile_takes(f.tile, layout)) continue;
+  const auto consider = [&](const TileFit& f) {
+    if (forced && (f.tile.rows != t_tile.rows || f.tile.cols != t_tile.cols)) return;
+    if (!tile_takes(f.tile, layout, finish, m)) return;
     const long long tiles = (long long)ceil_div(m, f.tile.rows) * ceil_div(columns, f.tile.cols);
     for (int slices = 1; slices <= kSlicesMost && slices <= stages; slices++) {
       const double bytes = 4.0 * slices * m * columns;
@@ -157,7 +167,9 @@ ProductPlan choose_plan(int m, int n, int k, bool gated, Layout layout, int cus,
         least = cost;
       }
     }
-  }
+  };
+  for (const TileFit& f : kFits) consider(f);
+  for (const TileFit& f : kSmallFits) consider(f);
   return best;
 }
 // Two slices of big tiles finish them together: their sums, and behind these the words at which
@@ -195,15 +207,16 @@ constexpr int kPlansKept = 16;
 thread_local Planned t_plans[kPlansKept];
 thread_local int t_oldest = 0;
 
-Planned plan_with_room(int m, int n, int k, bool gated, Layout layout, int cus) {
-  const int form = (gated ? 1 : 0) | (int)layout << 1;
+Planned plan_with_room(int m, int n, int k, Finish finish, Layout layout, int cus) {
+  const bool gated = finish == kGated;
+  const int form = (int)finish | (int)layout << 2;
   const bool forced = t_tile.rows > 0 || t_slices > 0;
   if (!forced)
     for (const Planned& p : t_plans)
       if (p.m == m && p.n == n && p.k == k && p.cus == cus && p.form == form) return p;
   Planned p;
   p.m = m, p.n = n, p.k = k, p.cus = cus, p.form = form;
-  p.plan = choose_plan(m, n, k, gated, layout, cus, 1LL << 40);
+  p.plan = choose_plan(m, n, k, finish, layout, cus, 1LL << 40);
   p.bytes = p.plan.slices > 1 ? 4LL * p.plan.slices * m * product_columns(n, gated) : 0;
   p.bytes = std::max(p.bytes, meeting(p.plan, m, product_columns(n, gated)).bytes);
   if (!forced) {
@@ -253,6 +266,8 @@ int drop_args(const feedforward_drop* d, DropArgs* out) {
   return FEEDFORWARD_OK;
 }
 
+Finish finish_of(int gated) { return gated == FEEDFORWARD_FULL ? kFull : gated ? kGated : kPlain; }
+
 bool layout_of(int turned, Layout* layout) {
   *layout = (Layout)turned;
   return turned >= FEEDFORWARD_ROWS && turned <= FEEDFORWARD_TURN_BOTH;
@@ -270,10 +285,10 @@ int run_product(ProductArgs a, Layout layout, bool bf, void* room, long long roo
   if (!a.A || !a.B || !a.C) return fail(FEEDFORWARD_ERR_SHAPE, "a matrix is missing");
   if (room && off16(room)) return fail(FEEDFORWARD_ERR_SHAPE, "scratch must start on 16 bytes");
   return on_device(dev, [&](int cus) {
-    const Planned planned = plan_with_room(a.M, a.N, a.K, gated, layout, cus);
+    const Planned planned = plan_with_room(a.M, a.N, a.K, a.finish, layout, cus);
     const long long have = room ? room_bytes : 0;
     const ProductPlan p =
-        planned.bytes <= have ? planned.plan : choose_plan(a.M, a.N, a.K, gated, layout, cus, have);
+        planned.bytes <= have ? planned.plan : choose_plan(a.M, a.N, a.K, a.finish, layout, cus, have);
     a.slices = p.slices;
     a.part = p.slices > 1 ? (float*)room : nullptr;
     a.ldpart = (int)columns;
@@ -283,7 +298,7 @@ int run_product(ProductArgs a, Layout layout, bool bf, void* room, long long roo
       a.words = (unsigned long long*)((char*)room + meet.words);
       a.token = next_token();
     }
-    if (few_tile(p.tile))
+    if (few_tile(p.tile) && a.M <= kProductRows)
       launch_product_rows(a, p.tile.cols / 16, bf, stream);
     else if (big_tile(p.tile))
       (bf ? launch_product_big_bf16 : launch_product_big_f16)(a, p.tile.rows, layout, stream);
@@ -446,7 +461,7 @@ long long feedforward_product_bytes(int m, int n, int k, int gated, int turned, 
   Layout layout;
   if (check_sizes(m, n, k, FEEDFORWARD_FP16) != FEEDFORWARD_OK || !layout_of(turned, &layout)) return -1;
   const int cus = device_cus(dev);
-  return cus > 0 && m > 0 && n > 0 && k > 0 ? plan_with_room(m, n, k, gated != 0, layout, cus).bytes : 0;
+  return cus > 0 && m > 0 && n > 0 && k > 0 ? plan_with_room(m, n, k, finish_of(gated), layout, cus).bytes : 0;
 }
 
 int feedforward_gated_grad(const void* dh, const float* pre, void* dgu, int m, int n, long long lddh, long long ldpre,
@@ -531,7 +546,7 @@ int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int* o
   Layout layout;
   if (!layout_of(turned, &layout)) return fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
   if (cus < 1) return fail(FEEDFORWARD_ERR_SHAPE, "%d compute units", cus);
-  const ProductPlan p = plan_with_room(m, n, k, gated != 0, layout, cus).plan;
+  const ProductPlan p = plan_with_room(m, n, k, finish_of(gated), layout, cus).plan;
   out[0] = p.tile.rows;
   out[1] = p.tile.cols;
   out[2] = p.slices;
@@ -542,6 +557,8 @@ void feedforward_force_tile(int rows, int cols, int slices) {
   t_tile = {0, 0};
   t_slices = slices > kSlicesMost ? kSlicesMost : slices < 0 ? 0 : slices;
   for (const TileFit& f : kFits)
+    if (f.tile.rows == rows && f.tile.cols == cols) t_tile = f.tile;
+  for (const TileFit& f : kSmallFits)
     if (f.tile.rows == rows && f.tile.cols == cols) t_tile = f.tile;
   for (const TileFit& f : kFewFits)
     if (f.tile.rows == rows && f.tile.cols == cols) t_tile = f.tile;

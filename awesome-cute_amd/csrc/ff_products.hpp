@@ -94,6 +94,12 @@ __device__ __forceinline__ f4 drop4(f4 v, i2 bits, const DropArgs& a) {
               drop_one(v[3], bits, 3, a)};
 }
 
+// the random bits of four columns of a row of C, of which their group of eight has as many again
+__device__ __forceinline__ i2 own_bits(const ProductArgs& p, const DropKey& key, int row, int col) {
+  const i4 w = drop_bits((unsigned long long)(unsigned)row * (unsigned)(p.N >> 3) + (unsigned)(col >> 3), key);
+  return col & 4 ? (i2){w[2], w[3]} : (i2){w[0], w[1]};
+}
+
 // kFull, four columns of a row of C by themselves: where a lane has no others of their group of
 // eight, and makes its bits alone.  Bias and residual are fetched ahead of the sums.
 struct FullOperands {
@@ -111,10 +117,7 @@ __device__ __forceinline__ void finish_full(const ProductArgs& p, int row, int c
     v = p.act == kActGelu ? act4<kActGelu>(v, &slopes) : act4<kActSilu>(v, &slopes);
     if (p.slopes) *(i2*)(p.slopes + (size_t)row * p.ldslopes + col) = slopes;
   }
-  if (p.drop.below) {
-    const i4 bits = drop_bits((unsigned long long)row * (unsigned)(p.N >> 3) + (unsigned)(col >> 3), DropKey(p.drop));
-    v = drop4(v, col & 4 ? (i2){bits[2], bits[3]} : (i2){bits[0], bits[1]}, p.drop);
-  }
+  if (p.drop.below) v = drop4(v, own_bits(p, DropKey(p.drop), row, col), p.drop);
   if (p.residual) v += widen4<BF>(o.residual);
   *(i2*)((half_t*)p.C + (size_t)row * p.ldc + col) = product_round<BF>(v);
 }
@@ -142,7 +145,7 @@ __host__ __device__ __forceinline__ int pre_col(int col) { return ((col >> 4) <<
 __host__ __device__ __forceinline__ int product_columns(int n, bool gated) { return gated ? (n + 15) / 16 * 32 : n; }
 
 // Tiles: rows x columns of the product.  256 columns and 160, 192, 224 or 256 rows are
-// ff_big.hpp's, 16 and 32 columns, of up to kProductRows rows, ff_rows.hip's, the others
+// ff_big.hpp's, 16 and 32 columns of products of up to kProductRows rows ff_rows.hip's, the others
 // ff_tiles.hip's.
 struct FfTile {
   int rows, cols;

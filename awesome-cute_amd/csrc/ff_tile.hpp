@@ -145,7 +145,6 @@ __device__ __forceinline__ void fetch_residual(const ProductArgs& p, int m0, int
 template <bool BF, int NI, int NJ, int PITCH>
 __device__ __forceinline__ void put_full(const ProductArgs& p, char* out, int slopes_at, int m0, int n0, int m, int col,
                                          int kg, const i2 (&bias)[NJ], const i2 (&residual)[NI][NJ], f4 (&v)[NI][NJ]) {
-  static_assert(NJ % 2 == 0, "pairs of operands");
   if (p.bias)
     for_each<NJ>([&](auto J) {
       constexpr int j = decltype(J)::value;
@@ -179,13 +178,17 @@ __device__ __forceinline__ void put_full(const ProductArgs& p, char* out, int sl
   if (p.drop.below) {
     const DropKey key(p.drop);
     for_each<NI>([&](auto I) {
+      constexpr int i = decltype(I)::value;
+      const int row = m0 + m + 16 * i;
       for_each<NJ / 2>([&](auto J) {
-        constexpr int i = decltype(I)::value, j = 2 * decltype(J)::value;
+        constexpr int j = 2 * decltype(J)::value;
         i2 first, second;
-        full_bits(p, key, m0 + m + 16 * i, n0 + col + 16 * j, kg, &first, &second);
+        full_bits(p, key, row, n0 + col + 16 * j, kg, &first, &second);
         v[i][j] = drop4(v[i][j], first, p.drop);
         v[i][j + 1] = drop4(v[i][j + 1], second, p.drop);
       });
+      if constexpr (NJ % 2)  // (one without a partner)
+        v[i][NJ - 1] = drop4(v[i][NJ - 1], own_bits(p, key, row, n0 + col + 16 * (NJ - 1)), p.drop);
     });
   }
   if (p.residual)

@@ -387,6 +387,10 @@ void with_tile(const FfTile& t, bool once, F f) {
     FF_TILE_OF(64, 128, 2, 4, 6, true);
   }
   once = false;
+  if constexpr (FINISH == kFull) {
+    FF_TILE(32, 32, 2, 2, 8);
+    FF_TILE(32, 64, 2, 2, 6);
+  }
   FF_TILE(64, 64, 2, 2, 4);
   FF_TILE(64, 128, 2, 4, 6);
   FF_TILE(128, 128, 2, 4, 4);
@@ -415,8 +419,8 @@ void with_product(const FfTile& t, Finish finish, Layout layout, bool once, bool
 
 hipError_t configure_product_tiles() {
   hipError_t e = hipSuccess;
-  for (const int rows : {64, 96, 128})
-    for (const int cols : {64, 128, 256})
+  for (const int rows : {32, 64, 96, 128})
+    for (const int cols : {32, 64, 128, 256})
       for (const bool bf : {false, true})
         for (const bool once : {false, true})
           for (const int form : {0, 1, 2, 3, 4})

@@ -502,7 +502,7 @@ struct Room {
   void* there = nullptr;
   long long bytes;
   Room(void* at, long long bytes) : there(at), bytes(bytes) {}
-  Room(const at::Tensor& like, int64_t m, int64_t n, int64_t k, bool gated, int turned)
+  Room(const at::Tensor& like, int64_t m, int64_t n, int64_t k, int gated, int turned)
       : bytes(feedforward_product_bytes((int)m, (int)n, (int)k, gated, turned, like.get_device())) {
     if (bytes > 0) t = at::empty({bytes / 4}, options_as(like).dtype(at::kFloat));
   }
@@ -859,7 +859,7 @@ std::pair<at::Tensor, at::Tensor> full_forward(FullInputs& in, bool keep) {
   std::optional<Matrix> bias, residual;
   if (in.bias.defined()) bias.emplace(in.bias, 1, in.n);
   if (in.residual.defined()) residual.emplace(in.residual, in.m, in.n);
-  const Room room(in.x, in.m, in.n, in.k, false, FEEDFORWARD_ROWS);
+  const Room room(in.x, in.m, in.n, in.k, FEEDFORWARD_FULL, FEEDFORWARD_ROWS);
   const feedforward_drop drop = in.drop.plain();
   feedforward_check(feedforward_linear(a.at(), b.at(), y.data_ptr(), bias ? bias->at() : nullptr,
                                        residual ? residual->at() : nullptr, at_of(slopes), (int)in.m, (int)in.n,

@@ -68,7 +68,8 @@ int feedforward_gated_w4(const void *A, const void *B, void *C, const void *s, i
 int feedforward_product(const void *A, const void *B, void *C, int m, int n, int k, long long lda,
                         long long ldb, long long ldc, int turned, int type, void *room,
                         long long room_bytes, int dev, void *stream);
-/* -1 for sizes that are refused */
+/* `gated`: 0, 1, or FEEDFORWARD_FULL for feedforward_linear; -1 for sizes that are refused */
+#define FEEDFORWARD_FULL 2
 long long feedforward_product_bytes(int m, int n, int k, int gated, int turned, int dev);
 
 /* h (m x n) = act(x G^T) * (x U^T), element by element, x (m x k), w the n rows of G and behind

@@ -254,10 +254,46 @@ def test_forward(m, n, k, type):
         oracle(x, w, bias, residual, form, m, i).check_forward(call(x, w, bias, residual, form, m, i))
 
 
+SMALL = [(32, 32), (32, 64)]  # with an epilogue alone
+
+
+def test_plans_with_an_epilogue():
+    """The small tiles are reached, and are no other products'; where they are not taken the plan is the
+    product's without an epilogue."""
+    seen, rng = set(), np.random.default_rng(0)
+    for _ in range(4000):
+        m, n, k = (int(2 ** rng.uniform(*r)) for r in ((0, 13), (3, 13), (3, 13)))
+        n, k = 8 * max(1, n // 8), 8 * max(1, k // 8)
+        rows, cols, slices = plan = streamk.product_plan(m, n, k, 2)
+        bare = streamk.product_plan(m, n, k)
+        if cols <= 32 and m <= 64:
+            assert plan == bare and slices == 1 and rows == -(-m // 16) * 16
+        elif (rows, cols) in SMALL:
+            assert cols == 64 or m > 64
+            assert 1 <= slices <= min(8, -(-k // 64))
+            seen.add((rows, cols))
+        else:
+            assert plan == bare and (rows, cols) in TILES
+        assert bare[:2] not in SMALL or m <= 64
+    assert seen == set(SMALL)
+    try:
+        streamk.force_product_tile(32, 64, 2)
+        assert streamk.product_plan(300, 520, 192, 2) == (32, 64, 2)
+        assert streamk.product_plan(300, 520, 192) != (32, 64, 2) and streamk.product_plan(20, 520, 192, 2) == (32, 64, 2)
+        streamk.force_product_tile(32, 32)
+        assert streamk.product_plan(300, 520, 192, 2)[:2] == (32, 32)
+        assert streamk.product_plan(300, 520, 192)[:2] != (32, 32)
+        assert streamk.product_plan(20, 520, 192, 2) == streamk.product_plan(20, 520, 192) == (32, 32, 1)
+        streamk.force_product_tile(16, 16)
+        assert streamk.product_plan(300, 520, 192, 2)[1] != 16
+    finally:
+        streamk.force_product_tile(0)
+
+
 @gpu
 @pytest.mark.parametrize("slices", [1, 3])
-@pytest.mark.parametrize("tile", TILES)
-@pytest.mark.parametrize("m,n,k", [(1, 8, 64), (300, 520, 192), (257, 136, 1096), (333, 304, 640)])
+@pytest.mark.parametrize("tile", SMALL + TILES)
+@pytest.mark.parametrize("m,n,k", [(1, 8, 64), (300, 520, 192), (257, 136, 1096), (333, 304, 640), (65, 40, 72)])
 def test_every_tile(tile, m, n, k, slices):
     try:
         streamk.force_product_tile(*tile, slices)
@@ -290,7 +326,7 @@ def test_whole_columns_of_few_rows(m, n, k, cols):
 
 @gpu
 @pytest.mark.parametrize("slices", [1, 2])
-@pytest.mark.parametrize("tile", [(16, 16), (16, 32)] + TILES)
+@pytest.mark.parametrize("tile", [(16, 16), (16, 32)] + SMALL + TILES)
 def test_inside_rows_that_hold_nan(tile, slices):
     """Matrices inside larger ones: what lies beside them, and behind their last row, is NaN, and stays."""
     lib, L, P = streamk._lib, ctypes.c_longlong, ctypes.c_void_p
