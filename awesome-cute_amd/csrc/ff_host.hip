@@ -4,12 +4,12 @@
 
 #include <algorithm>
 #include <atomic>
+#include <chrono>
 #include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
 #include <mutex>
-#include <random>
 
 #include "../../include/feedforward_amd.h"
 #include "ff_grads.hpp"
@@ -187,9 +187,11 @@ Meeting meeting(const ProductPlan& p, int m, int columns) {
   return {(int)tiles, sums, sums + tiles * kWordStride * 8};
 }
 
-// a launch's own: products with an odd number do not repeat within 2^61, nor look like data
+// a launch's own: products with an odd number do not repeat within 2^61, nor look like data.  (From the
+// clock: std::random_device may throw, and the entries are C's.)
 unsigned long long next_token() {
-  static std::atomic<unsigned long long> launches{std::random_device{}()};
+  static std::atomic<unsigned long long> launches{
+      (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
   unsigned long long token;
   do token = ++launches * 0x9E3779B97F4A7C15ull << 3;
   while (token == 0);

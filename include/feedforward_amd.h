@@ -127,8 +127,8 @@ int feedforward_dropout(const void *x, const void *residual, void *y, long long 
                         const feedforward_drop *drop, int dev, void *stream);
 
 /* out[0..2] = rows and columns of the product's tiles and the slices of k, with room for them, on
- * a device of `cus` compute units (16 or 32 columns: all of up to 64 rows by workgroups of whole
- * columns); no GPU touched */
+ * a device of `cus` compute units (16 or 32 columns, up to 64 rows: all of them by workgroups of whole
+ * columns); `gated` as above; no GPU touched */
 int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int *out);
 /* such tiles (0 = by cost) and slices (0 = by cost) for every product of the calling thread that
  * they can compute; for tests and tools */
