@@ -84,7 +84,8 @@ __device__ __forceinline__ void store_bias(void* dbias, int column, float sum) {
 
 }  // namespace
 
-template <bool BF>
+// STEPS: slopes in steps alone
+template <bool BF, bool STEPS>
 __global__ __launch_bounds__(kRunThreads) void linear_grad_kernel(LinearGradArgs p) {
   __shared__ float room[kRunThreads][8 + 1];
   const int width = run_width(p.n), high = kRunThreads / width;
@@ -110,7 +111,10 @@ __global__ __launch_bounds__(kRunThreads) void linear_grad_kernel(LinearGradArgs
         f4 d = widen4<BF>((i2){dy[2 * h], dy[2 * h + 1]});
         if (p.slopes)
 #pragma unroll
-          for (int e = 0; e < 4; e++) d[e] *= slope_of((unsigned)slopes[2 * h + (e >> 1)] >> (16 * (e & 1)) & 0xffffu);
+          for (int e = 0; e < 4; e++) {
+            const unsigned code = (unsigned)slopes[2 * h + (e >> 1)] >> (16 * (e & 1)) & 0xffffu;
+            d[e] *= STEPS ? slope_of_steps(code) : slope_of<BF>(code);
+          }
         // (last: what is dropped has no gradient, whatever its slope)
         if (p.drop.below) d = drop4(d, (i2){bits[2 * h], bits[2 * h + 1]}, p.drop);
 #pragma unroll
@@ -171,10 +175,11 @@ void launch_linear_grad(LinearGradArgs a, bool bf, hipStream_t stream) {
   const int parts = runs_of(a.m, a.rows_per_part);
   if (parts == 1) a.partials = nullptr;  // (its sums are the bias's)
   const dim3 grid(ceil_div(a.n, 8 * width), parts), sums(ceil_div(a.n, 64));
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kRunThreads), 0, stream, a); };
   if (bf)
-    hipLaunchKernelGGL(linear_grad_kernel<true>, grid, dim3(kRunThreads), 0, stream, a);
+    a.slope_steps ? launch(linear_grad_kernel<true, true>) : launch(linear_grad_kernel<true, false>);
   else
-    hipLaunchKernelGGL(linear_grad_kernel<false>, grid, dim3(kRunThreads), 0, stream, a);
+    a.slope_steps ? launch(linear_grad_kernel<false, true>) : launch(linear_grad_kernel<false, false>);
   if (!a.partials) return;
   if (bf)
     hipLaunchKernelGGL(bias_sums_kernel<true>, sums, dim3(1024), 0, stream, a, parts);

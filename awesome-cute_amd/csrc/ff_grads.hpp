@@ -23,6 +23,7 @@ struct LinearGradArgs {
   float* partials;   // linear_grad_parts(m, n) rows of n, where dbias is wanted and these are more than one
   long long lddy, ldslopes, lddz;
   int m, n, rows_per_part;
+  bool slope_steps;  // their form (gated_act.hpp)
   DropArgs drop;
 };
 int linear_grad_parts(int m, int n);

@@ -340,6 +340,65 @@ int check_rows(const char* name, const void* p, long long ld, int d) {
   return FEEDFORWARD_OK;
 }
 
+// feedforward_linear and feedforward_linear_train, which differ in the form of the slopes
+int run_linear(bool steps, const void* x, const void* w, void* y, const void* bias, const void* residual, void* slopes, int m,
+               int n, int k, long long ldx, long long ldw, long long ldy, long long ldr, long long ldslopes,
+               int type, int activation, const feedforward_drop* drop, void* room, long long room_bytes,
+               int dev, void* stream) {
+  int rc = check_sizes(m, n, k, type);
+  ProductArgs a = {};
+  if (rc == FEEDFORWARD_OK && k % 8 != 0) rc = fail(FEEDFORWARD_ERR_SHAPE, "widths must be multiples of 8 (k = %d)", k);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("x", x, ldx, k);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("w", w, ldw, k);
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("y", y, ldy, n);
+  if (rc == FEEDFORWARD_OK && bias) rc = check_matrix("bias", bias, n, n);
+  if (rc == FEEDFORWARD_OK && residual) rc = check_matrix("residual", residual, ldr, n);
+  if (rc == FEEDFORWARD_OK && slopes) rc = check_matrix("slopes", slopes, ldslopes, n);
+  if (rc == FEEDFORWARD_OK && activation != kActNone && !act_known(activation))
+    rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
+  if (rc == FEEDFORWARD_OK && activation == kActNone && slopes)
+    rc = fail(FEEDFORWARD_ERR_SHAPE, "slopes belong to an activation");
+  if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
+  if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
+  if (k == 0) return fail(FEEDFORWARD_ERR_SHAPE, "k = 0: an empty sum");
+  a.A = x, a.B = w, a.C = y, a.bias = bias, a.residual = residual, a.slopes = (unsigned short*)slopes;
+  a.M = m, a.N = n, a.K = k;
+  a.lda = (int)ldx, a.ldb = (int)ldw, a.ldc = (int)ldy;
+  a.ldr = residual ? (int)ldr : 0, a.ldslopes = slopes ? (int)ldslopes : 0;
+  a.slope_steps = steps;
+  a.finish = kFull;
+  a.act = activation;
+  return run_product(a, kRows, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
+}
+
+// of the sums over rows
+long long linear_sums_bytes(int m, int n) {
+  const int parts = m > 0 && n > 0 ? linear_grad_parts(m, n) : 0;
+  return parts > 1 ? 4LL * n * parts : 0;
+}
+
+int run_linear_grad(bool steps, const void* dy, const void* slopes, void* dz, void* dbias, int m, int n, long long lddy,
+                    long long ldslopes, long long lddz, int type, const feedforward_drop* drop,
+                    void* partials, long long partial_bytes, int dev, void* stream) {
+  int rc = check_sizes(m, n, 0, type);
+  LinearGradArgs a = {};
+  if (rc == FEEDFORWARD_OK) rc = check_matrix("dy", dy, lddy, n);
+  if (rc == FEEDFORWARD_OK && slopes) rc = check_matrix("slopes", slopes, ldslopes, n);
+  if (rc == FEEDFORWARD_OK && dz) rc = check_matrix("dz", dz, lddz, n);
+  if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
+  if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
+  if (!dy || (!dz && !dbias)) return fail(FEEDFORWARD_ERR_SHAPE, "dy, or every output, is missing");
+  const long long sums = dbias ? linear_sums_bytes(m, n) : 0;
+  if (sums > 0 && (!partials || ((uintptr_t)partials & 3) || partial_bytes < sums))
+    return fail(FEEDFORWARD_ERR_SHAPE, "the sums over rows need %lld bytes of scratch", sums);
+  a.dy = dy, a.slopes = (const unsigned short*)slopes, a.dz = dz, a.dbias = dbias;
+  a.partials = sums > 0 ? (float*)partials : nullptr;
+  a.lddy = lddy, a.ldslopes = ldslopes, a.lddz = lddz;
+  a.m = m, a.n = n;
+  a.slope_steps = steps;
+  return on_device(dev, [&](int) { launch_linear_grad(a, type == FEEDFORWARD_BF16, (hipStream_t)stream); });
+}
+
 }  // namespace
 
 extern "C" {
@@ -392,56 +451,34 @@ int feedforward_linear(const void* x, const void* w, void* y, const void* bias, 
                        int n, int k, long long ldx, long long ldw, long long ldy, long long ldr, long long ldslopes,
                        int type, int activation, const feedforward_drop* drop, void* room, long long room_bytes,
                        int dev, void* stream) {
-  int rc = check_sizes(m, n, k, type);
-  ProductArgs a = {};
-  if (rc == FEEDFORWARD_OK && k % 8 != 0) rc = fail(FEEDFORWARD_ERR_SHAPE, "widths must be multiples of 8 (k = %d)", k);
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("x", x, ldx, k);
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("w", w, ldw, k);
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("y", y, ldy, n);
-  if (rc == FEEDFORWARD_OK && bias) rc = check_matrix("bias", bias, n, n);
-  if (rc == FEEDFORWARD_OK && residual) rc = check_matrix("residual", residual, ldr, n);
-  if (rc == FEEDFORWARD_OK && slopes) rc = check_matrix("slopes", slopes, ldslopes, n);
-  if (rc == FEEDFORWARD_OK && activation != kActNone && !act_known(activation))
-    rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
-  if (rc == FEEDFORWARD_OK && activation == kActNone && slopes)
-    rc = fail(FEEDFORWARD_ERR_SHAPE, "slopes belong to an activation");
-  if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
-  if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
-  if (k == 0) return fail(FEEDFORWARD_ERR_SHAPE, "k = 0: an empty sum");
-  a.A = x, a.B = w, a.C = y, a.bias = bias, a.residual = residual, a.slopes = (unsigned short*)slopes;
-  a.M = m, a.N = n, a.K = k;
-  a.lda = (int)ldx, a.ldb = (int)ldw, a.ldc = (int)ldy;
-  a.ldr = residual ? (int)ldr : 0, a.ldslopes = slopes ? (int)ldslopes : 0;
-  a.finish = kFull;
-  a.act = activation;
-  return run_product(a, kRows, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
+  return run_linear(true, x, w, y, bias, residual, slopes, m, n, k, ldx, ldw, ldy, ldr, ldslopes, type, activation, drop,
+                    room, room_bytes, dev, stream);
+}
+
+int feedforward_linear_train(const void* x, const void* w, void* y, const void* bias, const void* residual, void* slopes, int m,
+                             int n, int k, long long ldx, long long ldw, long long ldy, long long ldr, long long ldslopes,
+                             int type, int activation, const feedforward_drop* drop, void* room, long long room_bytes,
+                             int dev, void* stream) {
+  return run_linear(false, x, w, y, bias, residual, slopes, m, n, k, ldx, ldw, ldy, ldr, ldslopes, type, activation, drop,
+                    room, room_bytes, dev, stream);
 }
 
 long long feedforward_linear_grad_bytes(int m, int n) {
-  if (check_sizes(m, n, 0, FEEDFORWARD_FP16) != FEEDFORWARD_OK) return -1;
-  const int parts = m > 0 && n > 0 ? linear_grad_parts(m, n) : 0;
-  return parts > 1 ? 4LL * n * parts : 0;
+  return check_sizes(m, n, 0, FEEDFORWARD_FP16) == FEEDFORWARD_OK ? linear_sums_bytes(m, n) : -1;
 }
 
 int feedforward_linear_grad(const void* dy, const void* slopes, void* dz, void* dbias, int m, int n, long long lddy,
                             long long ldslopes, long long lddz, int type, const feedforward_drop* drop,
                             void* partials, long long partial_bytes, int dev, void* stream) {
-  int rc = check_sizes(m, n, 0, type);
-  LinearGradArgs a = {};
-  if (rc == FEEDFORWARD_OK) rc = check_matrix("dy", dy, lddy, n);
-  if (rc == FEEDFORWARD_OK && slopes) rc = check_matrix("slopes", slopes, ldslopes, n);
-  if (rc == FEEDFORWARD_OK && dz) rc = check_matrix("dz", dz, lddz, n);
-  if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
-  if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
-  if (!dy || (!dz && !dbias)) return fail(FEEDFORWARD_ERR_SHAPE, "dy, or every output, is missing");
-  const long long sums = dbias ? feedforward_linear_grad_bytes(m, n) : 0;
-  if (sums > 0 && (!partials || ((uintptr_t)partials & 3) || partial_bytes < sums))
-    return fail(FEEDFORWARD_ERR_SHAPE, "the sums over rows need %lld bytes of scratch", sums);
-  a.dy = dy, a.slopes = (const unsigned short*)slopes, a.dz = dz, a.dbias = dbias;
-  a.partials = sums > 0 ? (float*)partials : nullptr;
-  a.lddy = lddy, a.ldslopes = ldslopes, a.lddz = lddz;
-  a.m = m, a.n = n;
-  return on_device(dev, [&](int) { launch_linear_grad(a, type == FEEDFORWARD_BF16, (hipStream_t)stream); });
+  return run_linear_grad(true, dy, slopes, dz, dbias, m, n, lddy, ldslopes, lddz, type, drop, partials, partial_bytes,
+                         dev, stream);
+}
+
+int feedforward_linear_backward(const void* dy, const void* slopes, void* dz, void* dbias, int m, int n, long long lddy,
+                                long long ldslopes, long long lddz, int type, const feedforward_drop* drop,
+                                void* partials, long long partial_bytes, int dev, void* stream) {
+  return run_linear_grad(false, dy, slopes, dz, dbias, m, n, lddy, ldslopes, lddz, type, drop, partials, partial_bytes,
+                         dev, stream);
 }
 
 int feedforward_dropout(const void* x, const void* residual, void* y, long long count, int type,

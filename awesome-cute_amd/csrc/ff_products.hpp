@@ -40,6 +40,7 @@ struct ProductArgs {
   const void* residual;  // null, or rows ldr elements apart
   unsigned short* slopes;  // null, or act' of the sums for the backward pass, rows ldslopes apart
   int ldr, ldslopes;
+  bool slope_steps;      // their form (gated_act.hpp)
   DropArgs drop;
 };
 
@@ -80,13 +81,19 @@ template <int ACT>
 __device__ __forceinline__ f4 act4(f4 v) {
   return (f4){act_value<ACT>(v[0]), act_value<ACT>(v[1]), act_value<ACT>(v[2]), act_value<ACT>(v[3])};
 }
-// ... and their slopes as the backward pass takes them
-template <int ACT>
+// ... and their slopes as the backward pass takes them; STEPS: in steps alone
+template <bool BF, int ACT, bool STEPS>
 __device__ __forceinline__ f4 act4(f4 v, i2* slopes) {
-  unsigned code[4];
+  f4 s;
 #pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = act_coded<ACT>(v[e], &code[e]);
-  *slopes = (i2){(int)__builtin_amdgcn_perm(code[1], code[0], 0x05040100), (int)__builtin_amdgcn_perm(code[3], code[2], 0x05040100)};
+  for (int e = 0; e < 4; e++) {
+    float slope;
+    v[e] = act_value_slope<ACT>(v[e], &slope);
+    s[e] = slope;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+    (*slopes)[h] = (int)(STEPS ? slope_step_codes(s[2 * h], s[2 * h + 1]) : slope_codes<BF>(s[2 * h], s[2 * h + 1]));
   return v;
 }
 __device__ __forceinline__ f4 drop4(f4 v, i2 bits, const DropArgs& a) {
@@ -114,7 +121,10 @@ __device__ __forceinline__ void finish_full(const ProductArgs& p, int row, int c
   if (p.bias) v += widen4<BF>(o.bias);
   if (p.act != kActNone) {
     i2 slopes;
-    v = p.act == kActGelu ? act4<kActGelu>(v, &slopes) : act4<kActSilu>(v, &slopes);
+    if (p.slope_steps)
+      v = p.act == kActGelu ? act4<BF, kActGelu, true>(v, &slopes) : act4<BF, kActSilu, true>(v, &slopes);
+    else
+      v = p.act == kActGelu ? act4<BF, kActGelu, false>(v, &slopes) : act4<BF, kActSilu, false>(v, &slopes);
     if (p.slopes) *(i2*)(p.slopes + (size_t)row * p.ldslopes + col) = slopes;
   }
   if (p.drop.below) v = drop4(v, own_bits(p, DropKey(p.drop), row, col), p.drop);

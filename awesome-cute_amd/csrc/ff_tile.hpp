@@ -160,21 +160,35 @@ __device__ __forceinline__ void put_full(const ProductArgs& p, char* out, int sl
       });
     });
   };
-  const auto activate_slopes = [&](auto Act) {
+  const auto activate_slopes = [&](auto Act, auto Steps) {
     constexpr int act = decltype(Act)::value;
     for_each<NI>([&](auto I) {
       for_each<NJ>([&](auto J) {
         constexpr int i = decltype(I)::value, j = decltype(J)::value;
         i2 slopes;
-        v[i][j] = act4<act>(v[i][j], &slopes);
+#if defined(__HIP_DEVICE_COMPILE__)
+        // (what both forms have in common stays behind the branch to either: ahead of it, it spills)
+        if constexpr (decltype(Steps)::value) asm("" : "+v"(v[i][j]));
+#endif
+        v[i][j] = act4<BF, act, decltype(Steps)::value>(v[i][j], &slopes);
         *(i2*)(out + slopes_at + 16 * i * PITCH + 2 * (col + 16 * j)) = slopes;
+        // (four operands by themselves: more at once take registers that the big tiles do not have)
+        if constexpr (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       });
     });
   };
+  const auto activated = [&](auto Act) {
+    if (!p.slopes)
+      activate(Act);
+    else if (p.slope_steps)
+      activate_slopes(Act, std::true_type{});
+    else
+      activate_slopes(Act, std::false_type{});
+  };
   if (p.act == kActGelu)
-    p.slopes ? activate_slopes(std::integral_constant<int, kActGelu>{}) : activate(std::integral_constant<int, kActGelu>{});
+    activated(std::integral_constant<int, kActGelu>{});
   else if (p.act == kActSilu)
-    p.slopes ? activate_slopes(std::integral_constant<int, kActSilu>{}) : activate(std::integral_constant<int, kActSilu>{});
+    activated(std::integral_constant<int, kActSilu>{});
   if (p.drop.below) {
     const DropKey key(p.drop);
     for_each<NI>([&](auto I) {

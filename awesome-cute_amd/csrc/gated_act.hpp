@@ -5,6 +5,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 namespace w4a16 {
 
 constexpr int kActNone = 0, kActSilu = 1, kActGelu = 2;
@@ -43,25 +45,83 @@ __device__ __forceinline__ float act_sigma_of(float g, float g2) {
 template <int ACT>
 __device__ __forceinline__ float act_value(float g) { return g * act_sigma_of<ACT>(g, g * g); }
 
-// Where such a product keeps anything for its backward pass, it is the slope, in 16 bits: slopes
-// lie between -0.13 and 1.13, and a step of 2^-15 leaves them off by at most 2^-16, a thirtieth of what the
-// rounding of dy act' to 16 bits adds where slopes are near one, and zero and one are exact.  The sums
-// in 32 bits would take twice the bytes: 2048 x 10752 x 4096 12 us of 168 forward, and 14 of 40 backward.
-// A slope's code is 8192 more than its steps, a NaN's zero.
+// Where such a product keeps anything for its backward pass, it is the slope, in 16 bits.  Slopes lie between
+// -0.13 and 1.13, so that a step of 2^-15 leaves them off by at most 2^-16, a thirtieth of what the rounding
+// of dy act' to fp16 adds where slopes are near one; but of a unit that is far on the negative side,
+// where slopes are 2^-14 and less, such steps leave little or nothing.  So slopes below a border B in size,
+// 2^-5 in fp16 and 2^-7 in bfloat16, are numbers of the type itself, brought by a power of two to where its
+// exponents begin, and steps of 2^-15 go on from there, as fine as these are at the border:
+//   code = the number's bits of min(s, B)  +  (s - B) 2^15, if that is positive,
+// of a slope's size; 65535 less this for negative ones, and 49151, between the two, for NaN.  bfloat16: good to 2^-8
+// of a slope, what dy act' is rounded to, down to 2^-102.  fp16: to 2^-11 down to 2^-16, from there in
+// steps of 2^-26, no coarser than fp16 holds dy act' where dy is up to 4.  Nowhere off by more than 2^-16; zero and one
+// are exact.  The sums in 32 bits would take twice the bytes: 2048 x 10752 x 4096 12 us of 168 forward, and 14
+// of 40 backward.
 constexpr float kSlopeSteps = 32768.f;
+constexpr unsigned kSlopeBorder = 12288, kSlopeNan = 49151;  // codes
+template <bool BF>
+struct SlopeForm {
+  static constexpr float kBorder = BF ? 0x1p-7f : 0x1p-5f;
+  static constexpr float kUnit = BF ? 0x1p-24f : 4.f;  // (brings the border to the number whose bits are kSlopeBorder)
+};
+
+// Steps of 2^-15 alone (feedforward_linear's form): a code is 8192 more than a slope's steps, a NaN's is zero.
 constexpr int kSlopeZero = 8192;
+
+// act(g), and the slope
 template <int ACT>
-__device__ __forceinline__ float act_coded(float g, unsigned* code) {
+__device__ __forceinline__ float act_value_slope(float g, float* slope) {
   const float g2 = g * g, s = act_sigma_of<ACT>(g, g2);
   // sigma + g t' sigma (1 - sigma); far out, where the last factor is 0, g t' must not be infinite
   const float gt = ACT == kActGelu ? g * __builtin_fmaf(3.f * kGeluB, g2, kGeluA) : g;
-  const float slope = __builtin_fmaf(__builtin_amdgcn_fmed3f(gt, -3e38f, 3e38f), __builtin_fmaf(-s, s, s), s);
-  // the steps, rounded, are the low bits of a number as large as this (NaN: the maximum's other operand)
-  constexpr float kLarge = 8388608.f;  // 2^23
-  *code = __builtin_bit_cast(unsigned, __builtin_fmaxf(__builtin_fmaf(slope, kSlopeSteps, kLarge + kSlopeZero), kLarge));
+  *slope = __builtin_fmaf(__builtin_amdgcn_fmed3f(gt, -3e38f, 3e38f), __builtin_fmaf(-s, s, s), s);
   return g * s;
 }
+
+// the low halves of two numbers
+__device__ __forceinline__ unsigned low_halves(float first, float second) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, second), __builtin_bit_cast(unsigned, first), 0x05040100);
+}
+
+// the codes of two slopes
+template <bool BF>
+__device__ __forceinline__ unsigned slope_codes(float a, float b) {
+  typedef short S2 __attribute__((ext_vector_type(2)));
+  typedef unsigned short U2 __attribute__((ext_vector_type(2)));
+  using Number = std::conditional_t<BF, __bf16, _Float16>;
+  typedef Number N2 __attribute__((ext_vector_type(2)));
+  using Form = SlopeForm<BF>;
+  const auto inside = [](float s) { return __builtin_amdgcn_fmed3f(s, -Form::kBorder, Form::kBorder); };
+  const float ia = inside(a), ib = inside(b);
+  unsigned number = __builtin_bit_cast(unsigned, (N2){(Number)(ia * Form::kUnit), (Number)(ib * Form::kUnit)});
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("" : "+v"(number));  // (one register: otherwise each half is converted once more for its sign)
+#endif
+  const unsigned negative = __builtin_bit_cast(unsigned, __builtin_bit_cast(S2, number) >> 15);
+  // What is left in steps of 2^-15, rounded, a negative slope's negative: the low bits of a number as large as 384.  (NaN:
+  // the maximum's other operand, and its inside is -B, the least of the median's others: their sum is kSlopeNan.)
+  const auto steps = [](float left) { return __builtin_fmaxf(left + 384.f, 384.f - 4096.f / kSlopeSteps); };
+  static_assert((0xffffu - kSlopeBorder) - 4096 == kSlopeNan, "");
+  return __builtin_bit_cast(unsigned, (U2)(__builtin_bit_cast(U2, (number & 0x7fff7fffu) ^ negative) +
+                                           __builtin_bit_cast(U2, low_halves(steps(a - ia), steps(b - ib)))));
+}
+template <bool BF>
 __device__ __forceinline__ float slope_of(unsigned code) {
+  using Number = std::conditional_t<BF, __bf16, _Float16>;
+  const bool negative = code > kSlopeNan;
+  const unsigned size = negative ? 0xffffu - code : code, number = size < kSlopeBorder ? size : kSlopeBorder;
+  const float inside = (float)__builtin_bit_cast(Number, (unsigned short)number) * (1.f / SlopeForm<BF>::kUnit);
+  const float s = __builtin_fmaf((float)(size - number), 1.f / kSlopeSteps, inside);
+  return code == kSlopeNan ? __builtin_nanf("") : negative ? -s : s;
+}
+
+// ... and in steps alone
+__device__ __forceinline__ unsigned slope_step_codes(float a, float b) {
+  // (likewise; NaN: the maximum's other operand)
+  const auto steps = [](float s) { return __builtin_fmaxf(s + (256.f + kSlopeZero / kSlopeSteps), 256.f); };
+  return low_halves(steps(a), steps(b));
+}
+__device__ __forceinline__ float slope_of_steps(unsigned code) {
   return code == 0 ? __builtin_nanf("") : (float)((int)code - kSlopeZero) * (1.f / kSlopeSteps);
 }
 

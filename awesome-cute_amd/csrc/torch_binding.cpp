@@ -848,23 +848,24 @@ struct FullInputs {
   }
 };
 
-// residual + drop(act(x w^T + bias)), and, with `keep` and an activation, the slopes that the backward
-// pass takes, 16 bits each (otherwise undefined)
-std::pair<at::Tensor, at::Tensor> full_forward(FullInputs& in, bool keep) {
+// residual + drop(act(x w^T + bias)), and, with an activation and anything to keep, the slopes that a backward
+// pass takes, 16 bits each (otherwise undefined): those of feedforward_linear_train, or of feedforward_linear
+enum class Keep { kNothing, kSlopes, kSteps };
+std::pair<at::Tensor, at::Tensor> full_forward(FullInputs& in, Keep keep) {
   in.check();
   const int dev = in.x.get_device();
   at::Tensor y = empty_rows(in.x, in.n), slopes;
-  if (keep && in.act != 0) slopes = at::empty({in.m, in.n}, options_as(in.x).dtype(at::kShort));
+  if (keep != Keep::kNothing && in.act != 0) slopes = at::empty({in.m, in.n}, options_as(in.x).dtype(at::kShort));
   const Matrix a(in.x, in.m, in.k), b(in.w, in.n, in.k);
   std::optional<Matrix> bias, residual;
   if (in.bias.defined()) bias.emplace(in.bias, 1, in.n);
   if (in.residual.defined()) residual.emplace(in.residual, in.m, in.n);
   const Room room(in.x, in.m, in.n, in.k, FEEDFORWARD_FULL, FEEDFORWARD_ROWS);
   const feedforward_drop drop = in.drop.plain();
-  feedforward_check(feedforward_linear(a.at(), b.at(), y.data_ptr(), bias ? bias->at() : nullptr,
-                                       residual ? residual->at() : nullptr, at_of(slopes), (int)in.m, (int)in.n,
-                                       (int)in.k, a.ld, b.ld, in.n, residual ? residual->ld : 0, in.n, type_code(in.x),
-                                       in.act, &drop, room.at(), room.bytes, dev, current_stream(dev)));
+  const auto linear = keep == Keep::kSteps ? feedforward_linear : feedforward_linear_train;
+  feedforward_check(linear(a.at(), b.at(), y.data_ptr(), bias ? bias->at() : nullptr, residual ? residual->at() : nullptr,
+                           at_of(slopes), (int)in.m, (int)in.n, (int)in.k, a.ld, b.ld, in.n, residual ? residual->ld : 0,
+                           in.n, type_code(in.x), in.act, &drop, room.at(), room.bytes, dev, current_stream(dev)));
   return {y, slopes};
 }
 
@@ -913,9 +914,10 @@ std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& 
   const Matrix dz = other ? Matrix(base, ld) : d;
   if (other || want[2]) {
     const feedforward_drop drop = in.drop.plain();
-    feedforward_check(feedforward_linear_grad(d.at(), at_of(slopes), other ? base : nullptr, at_of(out[2]), (int)m, (int)n,
-                                              d.ld, n, ld, type_code(in.x), &drop, sum_bytes ? base + dz_bytes : nullptr,
-                                              sum_bytes, dev, current_stream(dev)));
+    feedforward_check(feedforward_linear_backward(d.at(), at_of(slopes), other ? base : nullptr, at_of(out[2]), (int)m,
+                                                  (int)n, d.ld, n, ld, type_code(in.x), &drop,
+                                                  sum_bytes ? base + dz_bytes : nullptr, sum_bytes, dev,
+                                                  current_stream(dev)));
   }
   const Room room(room_bytes > 0 ? base + dz_bytes + sum_bytes : nullptr, room_bytes);
   if (products) product_grads(in.x, in.w, dz, out[0], out[1], &room);
@@ -928,7 +930,7 @@ struct FullFunction : torch::autograd::Function<FullFunction> {
                             const Maybe& seed_at) {
     FullInputs in{x, w, bias.value_or(at::Tensor()), residual.value_or(at::Tensor()), (int)act,
                   Drop{p, seed, site, seed_at.value_or(at::Tensor())}};
-    auto [y, slopes] = full_forward(in, true);
+    auto [y, slopes] = full_forward(in, Keep::kSlopes);
     ctx->save_for_backward({x, w, slopes, in.drop.seed_at});
     auto kept = c10::make_intrusive<Kept>();
     kept->act = in.act;
@@ -1048,7 +1050,7 @@ PyObject* py_linear_full(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     y = !call.inner && differentiated({&in.x, &in.w, &in.bias, &in.residual})
             ? FullFunction::apply(in.x, in.w, maybe(in.bias), maybe(in.residual), (int64_t)in.act, in.drop.p,
                                   in.drop.seed, in.drop.site, maybe(in.drop.seed_at))
-            : full_forward(in, false).first;
+            : full_forward(in, Keep::kNothing).first;
   }
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
@@ -1076,17 +1078,20 @@ PyObject* py_dropout(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// linear_full_slopes(... as linear_full) -> (y, the slopes or None) and linear_full_grads(dy, slopes, x, weight,
+// linear_full_kept(... as linear_full) -> (y, the slopes or None) and linear_full_grads(dy, slopes, x, weight,
 // activation, p, seed, site, want_x, want_weight, want_bias) -> (dx, dweight, dbias), None where not wanted: the
-// passes by themselves, for compilers
-PyObject* py_linear_full_slopes(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+// passes by themselves, for compilers.  linear_full_slopes: linear_full_kept with slopes in the form of the C
+// entry feedforward_linear.
+template <Keep KEEP>
+PyObject* py_linear_full_kept(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   FullInputs in;
-  if (!takes(nargs, 8, "linear_full_slopes") || !full_arguments(args, &in)) return nullptr;
+  if (!takes(nargs, 8, KEEP == Keep::kSteps ? "linear_full_slopes" : "linear_full_kept") || !full_arguments(args, &in))
+    return nullptr;
   std::pair<at::Tensor, at::Tensor> out;
   {
     pybind11::gil_scoped_release unlocked;
-    out = full_forward(in, true);
+    out = full_forward(in, KEEP);
   }
   return tuple_of({out.first, out.second});
   END_HANDLE_TH_ERRORS
@@ -1496,7 +1501,8 @@ PyMethodDef methods[] = {
     {"gated_grads", (PyCFunction)(void (*)(void))py_gated_grads, METH_FASTCALL, nullptr},
     {"linear_dense", (PyCFunction)(void (*)(void))py_linear_dense, METH_FASTCALL, nullptr},
     {"linear_full", (PyCFunction)(void (*)(void))py_linear_full, METH_FASTCALL, nullptr},
-    {"linear_full_slopes", (PyCFunction)(void (*)(void))py_linear_full_slopes, METH_FASTCALL, nullptr},
+    {"linear_full_kept", (PyCFunction)(void (*)(void))py_linear_full_kept<Keep::kSlopes>, METH_FASTCALL, nullptr},
+    {"linear_full_slopes", (PyCFunction)(void (*)(void))py_linear_full_kept<Keep::kSteps>, METH_FASTCALL, nullptr},
     {"linear_full_grads", (PyCFunction)(void (*)(void))py_linear_full_grads, METH_FASTCALL, nullptr},
     {"dropout", (PyCFunction)(void (*)(void))py_dropout, METH_FASTCALL, nullptr},
     {"gated_sums", (PyCFunction)(void (*)(void))py_gated_sums, METH_FASTCALL, nullptr},

@@ -103,7 +103,8 @@ typedef struct feedforward_drop {
 /* y (m x n) = residual + drop(act(x w^T + bias)), x (m x k), w (n x k), k > 0; y overlaps none of
  * them.  Null: bias (n
  * elements), residual (m x n), drop, and slopes, which keeps act' of x w^T + bias for the backward pass
- * (m x n numbers of 16 bits in the library's own form).  activation 0: none, and no slopes. */
+ * (m x n numbers of 16 bits, 8192 more than the slope's steps of 2^-15).  activation 0: none, and no slopes.
+ * Slopes below 2^-16 in size are kept as zero: silu's from -13.6 down and gelu's from -4.6 down. */
 int feedforward_linear(const void *x, const void *w, void *y, const void *bias, const void *residual,
                        void *slopes, int m, int n, int k, long long ldx, long long ldw, long long ldy,
                        long long ldr, long long ldslopes, int type, int activation,
@@ -120,6 +121,19 @@ int feedforward_linear_grad(const void *dy, const void *slopes, void *dz, void *
                             int dev, void *stream);
 /* -1 for sizes that are refused, 0 where few rows need none; no GPU touched */
 long long feedforward_linear_grad_bytes(int m, int n);
+
+/* The same two for training, with slopes that are good relative to their size as well, 16 bits each in the
+ * library's own form: off by at most 2^-16, and in bfloat16 by at most 2^-8 of themselves down to 2^-102, in
+ * fp16 by 2^-11 of themselves or 2^-27, whichever is more.  One's slopes are the other's alone. */
+int feedforward_linear_train(const void *x, const void *w, void *y, const void *bias, const void *residual,
+                             void *slopes, int m, int n, int k, long long ldx, long long ldw, long long ldy,
+                             long long ldr, long long ldslopes, int type, int activation,
+                             const feedforward_drop *drop, void *room, long long room_bytes, int dev,
+                             void *stream);
+int feedforward_linear_backward(const void *dy, const void *slopes, void *dz, void *dbias, int m, int n,
+                                long long lddy, long long ldslopes, long long lddz, int type,
+                                const feedforward_drop *drop, void *partials, long long partial_bytes,
+                                int dev, void *stream);
 
 /* y = residual + drop(x), or drop(x) without one; `count` elements (at most 2^34) of any type, each
  * matrix one contiguous row.  y may be x or the residual itself.  The gradient of x is drop(dy). */
