@@ -346,6 +346,9 @@ __global__ __launch_bounds__(256) void product_big_kernel(ProductArgs p) {
           constexpr int i = decltype(At)::value / 8, o = decltype(At)::value % 8;
           v[i][o] += acc[block + i][o];
         });
+      if constexpr (FINISH == kPlain)
+        if (p.scale != 1.f)
+          for_each<count * 8>([&](auto At) { v[decltype(At)::value / 8][decltype(At)::value % 8] *= p.scale; });
       if constexpr (FINISH == kFull)
         put_full<BF, count, 8, kPitch>(p, out + 16 * i0 * kPitch, kImage, m0, n0, m, col, kg, bias, residual, v);
       else

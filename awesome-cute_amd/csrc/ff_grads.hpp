@@ -25,6 +25,7 @@ struct LinearGradArgs {
   int m, n, rows_per_part;
   bool slope_steps;  // their form (gated_act.hpp)
   DropArgs drop;
+  float bias_factor;  // of dbias (of what is kept, where dz is without it)
 };
 int linear_grad_parts(int m, int n);
 void launch_linear_grad(LinearGradArgs a, bool bf, hipStream_t stream);

@@ -379,13 +379,14 @@ long long linear_sums_bytes(int m, int n) {
 
 int run_linear_grad(bool steps, const void* dy, const void* slopes, void* dz, void* dbias, int m, int n, long long lddy,
                     long long ldslopes, long long lddz, int type, const feedforward_drop* drop,
-                    void* partials, long long partial_bytes, int dev, void* stream) {
+                    void* partials, long long partial_bytes, float* factor, int dev, void* stream) {
   int rc = check_sizes(m, n, 0, type);
   LinearGradArgs a = {};
   if (rc == FEEDFORWARD_OK) rc = check_matrix("dy", dy, lddy, n);
   if (rc == FEEDFORWARD_OK && slopes) rc = check_matrix("slopes", slopes, ldslopes, n);
   if (rc == FEEDFORWARD_OK && dz) rc = check_matrix("dz", dz, lddz, n);
   if (rc == FEEDFORWARD_OK) rc = drop_args(drop, &a.drop);
+  if (factor) *factor = 1.f;
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
   if (!dy || (!dz && !dbias)) return fail(FEEDFORWARD_ERR_SHAPE, "dy, or every output, is missing");
   const long long sums = dbias ? linear_sums_bytes(m, n) : 0;
@@ -396,6 +397,11 @@ int run_linear_grad(bool steps, const void* dy, const void* slopes, void* dz, vo
   a.lddy = lddy, a.ldslopes = ldslopes, a.lddz = lddz;
   a.m = m, a.n = n;
   a.slope_steps = steps;
+  a.bias_factor = 1.f;
+  if (factor && !slopes) {
+    *factor = a.bias_factor = a.drop.factor;
+    a.drop.factor = 1.f;
+  }
   return on_device(dev, [&](int) { launch_linear_grad(a, type == FEEDFORWARD_BF16, (hipStream_t)stream); });
 }
 
@@ -406,6 +412,12 @@ extern "C" {
 int feedforward_product(const void* A, const void* B, void* C, int m, int n, int k, long long lda, long long ldb,
                         long long ldc, int turned, int type, void* room, long long room_bytes, int dev,
                         void* stream) {
+  return feedforward_product_scaled(A, B, C, m, n, k, lda, ldb, ldc, turned, type, 1.f, room, room_bytes, dev, stream);
+}
+
+int feedforward_product_scaled(const void* A, const void* B, void* C, int m, int n, int k, long long lda, long long ldb,
+                               long long ldc, int turned, int type, float scale, void* room, long long room_bytes,
+                               int dev, void* stream) {
   int rc = check_sizes(m, n, k, type);
   Layout layout = kRows;
   if (rc == FEEDFORWARD_OK && !layout_of(turned, &layout)) rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
@@ -422,6 +434,7 @@ int feedforward_product(const void* A, const void* B, void* C, int m, int n, int
   a.A = A, a.B = B, a.C = C;
   a.M = m, a.N = n, a.K = k;
   a.lda = (int)lda, a.ldb = (int)ldb, a.ldc = (int)ldc;
+  a.scale = scale;
   return run_product(a, layout, type == FEEDFORWARD_BF16, room, room_bytes, dev, (hipStream_t)stream);
 }
 
@@ -471,14 +484,14 @@ int feedforward_linear_grad(const void* dy, const void* slopes, void* dz, void* 
                             long long ldslopes, long long lddz, int type, const feedforward_drop* drop,
                             void* partials, long long partial_bytes, int dev, void* stream) {
   return run_linear_grad(true, dy, slopes, dz, dbias, m, n, lddy, ldslopes, lddz, type, drop, partials, partial_bytes,
-                         dev, stream);
+                         nullptr, dev, stream);
 }
 
 int feedforward_linear_backward(const void* dy, const void* slopes, void* dz, void* dbias, int m, int n, long long lddy,
                                 long long ldslopes, long long lddz, int type, const feedforward_drop* drop,
-                                void* partials, long long partial_bytes, int dev, void* stream) {
+                                void* partials, long long partial_bytes, float* factor, int dev, void* stream) {
   return run_linear_grad(false, dy, slopes, dz, dbias, m, n, lddy, ldslopes, lddz, type, drop, partials, partial_bytes,
-                         dev, stream);
+                         factor, dev, stream);
 }
 
 int feedforward_dropout(const void* x, const void* residual, void* y, long long count, int type,

@@ -15,7 +15,7 @@ namespace w4a16 {
 // rows of N and A as K rows of M (the gradients' products: dx = dy w, dw = dy^T x)
 enum Layout { kRows, kTurnB, kTurnBoth };
 
-// What becomes of the sums: they are C; or, gated, C (M x n) = act(A G^T) * (A U^T), B given as the n
+// What becomes of the sums: times a number, they are C; or, gated, C (M x n) = act(A G^T) * (A U^T), B given as the n
 // rows of G and then the n of U; or C = residual + drop(act(A B^T + bias)), whatever of these there is
 enum Finish { kPlain, kGated, kFull };
 
@@ -33,6 +33,7 @@ struct ProductArgs {
   int M, N, K;  // N: columns of C
   int lda, ldb, ldc, ldpre, ldpart;
   Finish finish;
+  float scale;  // plain: of the sums
   int act;
   int tiles_m, tiles_n, slices, polls;  // polls: looks at a tile's other slice before leaving it a share
   // full alone

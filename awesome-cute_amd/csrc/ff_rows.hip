@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_rows_kernel(ProductArg
     } else if constexpr (FINISH == kFull) {
       finish_full<BF>(p, row, col, v, full[i]);
     } else {
-      *(i2*)((half_t*)p.C + (size_t)row * p.ldc + col) = product_round<BF>(v);
+      *(i2*)((half_t*)p.C + (size_t)row * p.ldc + col) = product_round<BF>(v * p.scale);
     }
   }
 }

@@ -317,6 +317,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(ProductArgs 
     fetch_residual(p, m0, n0, m, col_at, rows, cols, residual);
     put_full<BF, RB, NJ, out_pitch<TN, false>()>(p, out, Sh::kImage, m0, n0, m, col_at, kg, bias, residual, acc);
   } else {
+    if constexpr (FINISH == kPlain)
+      if (p.scale != 1.f)
+        for_each<RB * NJ>([&](auto At) { acc[decltype(At)::value / NJ][decltype(At)::value % NJ] *= p.scale; });
 #pragma unroll
     for (int i = 0; i < RB; i++)
 #pragma unroll
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(ProductArgs p) {
   if constexpr (FINISH == kFull)
     finish_full<BF>(p, m, col, v, full);
   else
-    *(i2*)((half_t*)p.C + (size_t)m * p.ldc + col) = product_round<BF>(v);
+    *(i2*)((half_t*)p.C + (size_t)m * p.ldc + col) = product_round<BF>(GATED ? v : v * p.scale);
 }
 
 namespace {

@@ -539,23 +539,23 @@ at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w) {
 }
 
 // The gradients of x (m, k) and w (r, k) from that of their product, d (m, r): dx = d w and
-// dw = d^T x, sums over r and over m.  `shared`, if there: room for one of the two at a time.
+// dw = d^T x, sums over r and over m, times `scale`.  `shared`, if there: room for one of the two at a time.
 void product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, const at::Tensor& dx,
-                   const at::Tensor& dw, const Room* shared = nullptr) {
+                   const at::Tensor& dw, float scale = 1.f, const Room* shared = nullptr) {
   const int64_t k = w.size(1), m = x.numel() / k, r = w.size(0);
   const int type = type_code(x), dev = x.get_device();
   void* const st = current_stream(dev);
   if (dx.defined()) {
     const Matrix b(w, r, k);
     const Room room = shared ? *shared : Room(x, m, k, r, false, FEEDFORWARD_TURN_B);
-    feedforward_check(feedforward_product(d.at(), b.at(), dx.data_ptr(), (int)m, (int)k, (int)r, d.ld, b.ld, k,
-                                          FEEDFORWARD_TURN_B, type, room.at(), room.bytes, dev, st));
+    feedforward_check(feedforward_product_scaled(d.at(), b.at(), dx.data_ptr(), (int)m, (int)k, (int)r, d.ld, b.ld, k,
+                                                 FEEDFORWARD_TURN_B, type, scale, room.at(), room.bytes, dev, st));
   }
   if (dw.defined()) {
     const Matrix a(x, m, k);
     const Room room = shared ? *shared : Room(x, r, k, m, false, FEEDFORWARD_TURN_BOTH);
-    feedforward_check(feedforward_product(d.at(), a.at(), dw.data_ptr(), (int)r, (int)k, (int)m, d.ld, a.ld, k,
-                                          FEEDFORWARD_TURN_BOTH, type, room.at(), room.bytes, dev, st));
+    feedforward_check(feedforward_product_scaled(d.at(), a.at(), dw.data_ptr(), (int)r, (int)k, (int)m, d.ld, a.ld, k,
+                                                 FEEDFORWARD_TURN_BOTH, type, scale, room.at(), room.bytes, dev, st));
   }
 }
 
@@ -912,15 +912,16 @@ std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& 
     scratch = at::empty({dz_bytes + sum_bytes + room_bytes}, options_as(in.x).dtype(at::kByte));
   char* const base = (char*)at_of(scratch);
   const Matrix dz = other ? Matrix(base, ld) : d;
+  float factor = 1.f;
   if (other || want[2]) {
     const feedforward_drop drop = in.drop.plain();
     feedforward_check(feedforward_linear_backward(d.at(), at_of(slopes), other ? base : nullptr, at_of(out[2]), (int)m,
                                                   (int)n, d.ld, n, ld, type_code(in.x), &drop,
-                                                  sum_bytes ? base + dz_bytes : nullptr, sum_bytes, dev,
+                                                  sum_bytes ? base + dz_bytes : nullptr, sum_bytes, &factor, dev,
                                                   current_stream(dev)));
   }
   const Room room(room_bytes > 0 ? base + dz_bytes + sum_bytes : nullptr, room_bytes);
-  if (products) product_grads(in.x, in.w, dz, out[0], out[1], &room);
+  if (products) product_grads(in.x, in.w, dz, out[0], out[1], factor, &room);
   return out;
 }
 

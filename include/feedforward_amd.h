@@ -68,6 +68,10 @@ int feedforward_gated_w4(const void *A, const void *B, void *C, const void *s, i
 int feedforward_product(const void *A, const void *B, void *C, int m, int n, int k, long long lda,
                         long long ldb, long long ldc, int turned, int type, void *room,
                         long long room_bytes, int dev, void *stream);
+/* C = scale A B^T, rounded once */
+int feedforward_product_scaled(const void *A, const void *B, void *C, int m, int n, int k, long long lda,
+                               long long ldb, long long ldc, int turned, int type, float scale, void *room,
+                               long long room_bytes, int dev, void *stream);
 /* `gated`: 0, 1, or FEEDFORWARD_FULL for feedforward_linear; -1 for sizes that are refused */
 #define FEEDFORWARD_FULL 2
 long long feedforward_product_bytes(int m, int n, int k, int gated, int turned, int dev);
@@ -124,7 +128,10 @@ long long feedforward_linear_grad_bytes(int m, int n);
 
 /* The same two for training, with slopes that are good relative to their size as well, 16 bits each in the
  * library's own form: off by at most 2^-16, and in bfloat16 by at most 2^-8 of themselves down to 2^-102, in
- * fp16 by 2^-11 of themselves or 2^-27, whichever is more.  One's slopes are the other's alone. */
+ * fp16 by 2^-11 of themselves or 2^-27, whichever is more.  One's slopes are the other's alone.
+ * With `factor`, a float in host memory, dz without slopes is dy or zero, exactly, and dz times *factor, the
+ * mask's 1 / (1 - p), the gradient: for feedforward_product_scaled.  (*factor is 1 where there are slopes or no
+ * mask; dbias is whole either way.) */
 int feedforward_linear_train(const void *x, const void *w, void *y, const void *bias, const void *residual,
                              void *slopes, int m, int n, int k, long long ldx, long long ldw, long long ldy,
                              long long ldr, long long ldslopes, int type, int activation,
@@ -133,7 +140,7 @@ int feedforward_linear_train(const void *x, const void *w, void *y, const void *
 int feedforward_linear_backward(const void *dy, const void *slopes, void *dz, void *dbias, int m, int n,
                                 long long lddy, long long ldslopes, long long lddz, int type,
                                 const feedforward_drop *drop, void *partials, long long partial_bytes,
-                                int dev, void *stream);
+                                float *factor, int dev, void *stream);
 
 /* y = residual + drop(x), or drop(x) without one; `count` elements (at most 2^34) of any type, each
  * matrix one contiguous row.  y may be x or the residual itself.  The gradient of x is drop(dy). */

@@ -212,7 +212,9 @@ def test_codes_of_the_entries():
 
     def grad(entry, m=0, n=8, dy=16, slopes=None, dz=16, dbias=None, lds=8, type=0, p=None, partials=None, count=0):
         drop = None if p is None else ctypes.byref(DropArgs(p, 0, None, 0))
-        return entry(P(dy), P(slopes), P(dz), P(dbias), m, n, L(8), L(lds), L(8), type, drop, P(partials), L(count), 0, None)
+        factor = [None] if entry == lib.feedforward_linear_backward else []
+        return entry(P(dy), P(slopes), P(dz), P(dbias), m, n, L(8), L(lds), L(8), type, drop, P(partials), L(count), *factor,
+                     0, None)
 
     for entry in (lib.feedforward_linear, lib.feedforward_linear_train):
         assert linear(entry) == 0 and linear(entry, slopes=16, act=2, p=0.5) == 0
@@ -237,8 +239,9 @@ def by_entries(forward, backward, x, w, bias, act, dy):
     sums = torch.empty(max(lib.feedforward_linear_grad_bytes(m, n), 4), dtype=torch.uint8, device=dev)
     assert forward(P(x.data_ptr()), P(w.data_ptr()), P(y.data_ptr()), P(bias.data_ptr()), None, P(slopes.data_ptr()), m, n, k,
                    L(k), L(k), L(n), L(0), L(n), code, {"silu": 1, "gelu": 2}[act], None, None, L(0), 0, stream) == 0
+    factor = [None] if backward == lib.feedforward_linear_backward else []
     assert backward(P(dy.data_ptr()), P(slopes.data_ptr()), P(dz.data_ptr()), P(db.data_ptr()), m, n, L(n), L(n), L(n), code,
-                    None, P(sums.data_ptr()), L(sums.numel()), 0, stream) == 0
+                    None, P(sums.data_ptr()), L(sums.numel()), *factor, 0, stream) == 0
     return y, dz, db
 
 
