@@ -424,14 +424,16 @@ void feedforward_check(int rc) {
   TORCH_CHECK(rc == FEEDFORWARD_OK, feedforward_last_error());
 }
 
+void check_operand(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.is_cuda() && (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16), name,
+                    " must be a torch.half or torch.bfloat16 tensor on the GPU");
+  TORCH_CHECK_VALUE(t.layout() == at::kStrided && !t.is_neg() && !t.is_conj(), name, " must be a plain tensor");
+}
+
 // x (..., k) and w (rows, k)
 void check_dense(const at::Tensor& x, const at::Tensor& w) {
-  for (const at::Tensor* t : {&x, &w}) {
-    const char* const name = t == &x ? "x" : "weight";
-    TORCH_CHECK_VALUE(t->is_cuda() && (t->scalar_type() == at::kHalf || t->scalar_type() == at::kBFloat16), name,
-                      " must be a torch.half or torch.bfloat16 tensor on the GPU");
-    TORCH_CHECK_VALUE(t->layout() == at::kStrided && !t->is_neg() && !t->is_conj(), name, " must be a plain tensor");
-  }
+  check_operand(x, "x");
+  check_operand(w, "weight");
   TORCH_CHECK_VALUE(x.scalar_type() == w.scalar_type() && x.device() == w.device(),
                     "x and weight must have one type and one device");
   TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(1) != 0,
@@ -464,13 +466,13 @@ at::Tensor empty_rows(const at::Tensor& x, int64_t columns) {
 // current when it was made.  The engine would make that stream wait for the captured one, which draws
 // it into the capture without a way back, and the capture's end takes the process with it.  Refused
 // here, before the engine gets there.
-void check_capture(std::initializer_list<const at::Tensor*> inputs, int dev) {
+void check_capture(at::ArrayRef<at::Tensor> inputs, int dev) {
   const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev);
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
-  for (const at::Tensor* t : inputs) {
-    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+  for (const at::Tensor& t : inputs) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
     const auto stream = accumulator ? accumulator->stream() : std::nullopt;
     // (by number: torch names the device of one of them CUDA, of the other HIP)
     TORCH_CHECK(!stream || (stream->id() == now.id() && stream->device_index() == dev),
@@ -539,21 +541,24 @@ at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w) {
 }
 
 // The gradients of x (m, k) and w (r, k) from that of their product, d (m, r): dx = d w and
-// dw = d^T x, sums over r and over m, times `scale`.  `shared`, if there: room for one of the two at a time.
+// dw = d^T x, sums over r and over m, times `scale`.  x and w need be there for the other's gradient alone.
+// `shared`, if there: room for one of the two at a time.
 void product_grads(const at::Tensor& x, const at::Tensor& w, const Matrix& d, const at::Tensor& dx,
                    const at::Tensor& dw, float scale = 1.f, const Room* shared = nullptr) {
-  const int64_t k = w.size(1), m = x.numel() / k, r = w.size(0);
-  const int type = type_code(x), dev = x.get_device();
+  const at::Tensor &as_x = x.defined() ? x : dx, &as_w = w.defined() ? w : dw, &like = dx.defined() ? dx : dw;
+  if (!like.defined()) return;
+  const int64_t k = like.size(-1), m = as_x.defined() ? as_x.numel() / k : 0, r = as_w.defined() ? as_w.size(0) : 0;
+  const int type = type_code(like), dev = like.get_device();
   void* const st = current_stream(dev);
   if (dx.defined()) {
     const Matrix b(w, r, k);
-    const Room room = shared ? *shared : Room(x, m, k, r, false, FEEDFORWARD_TURN_B);
+    const Room room = shared ? *shared : Room(like, m, k, r, false, FEEDFORWARD_TURN_B);
     feedforward_check(feedforward_product_scaled(d.at(), b.at(), dx.data_ptr(), (int)m, (int)k, (int)r, d.ld, b.ld, k,
                                                  FEEDFORWARD_TURN_B, type, scale, room.at(), room.bytes, dev, st));
   }
   if (dw.defined()) {
     const Matrix a(x, m, k);
-    const Room room = shared ? *shared : Room(x, r, k, m, false, FEEDFORWARD_TURN_BOTH);
+    const Room room = shared ? *shared : Room(like, r, k, m, false, FEEDFORWARD_TURN_BOTH);
     feedforward_check(feedforward_product_scaled(d.at(), a.at(), dw.data_ptr(), (int)r, (int)k, (int)m, d.ld, a.ld, k,
                                                  FEEDFORWARD_TURN_BOTH, type, scale, room.at(), room.bytes, dev, st));
   }
@@ -569,7 +574,7 @@ std::pair<at::Tensor, at::Tensor> gated_backward(const at::Tensor& dh, const at:
                         pre.device() == x.device() && pre.numel() == m * ldpre && pre.is_contiguous(),
                     "dh and the sums must be those of x and weight");
   const int dev = x.get_device();
-  check_capture({&x, &w}, dev);
+  check_capture({x, w}, dev);
   at::Tensor dx, dw;
   if (want_x) dx = empty_as(x, x.sizes());
   if (want_w) dw = empty_as(w, w.sizes());
@@ -594,7 +599,7 @@ std::pair<at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy, const at
                         dy.size(-1) == n && dy.numel() == m * n,
                     "dy must be that of x and weight");
   const int dev = x.get_device();
-  check_capture({&x, &w}, dev);
+  check_capture({x, w}, dev);
   at::Tensor dx, dw;
   if (want_x) dx = empty_as(x, x.sizes());
   if (want_w) dw = empty_as(w, w.sizes());
@@ -806,12 +811,16 @@ bool drop_arguments(PyObject* const* args, Drop* out) {
 // graph holds, holds the leaf.
 struct Kept : torch::CustomClassHolder {
   int act = 0;
+  int64_t k = 0;
   Drop drop;  // (its seed in memory is saved: if that has been written since, asking for it raises)
-  at::Tensor leaves[2];
-  bool there[2] = {};
+  std::vector<at::Tensor> leaves;
+  bool there[2] = {};  // of a product the bias and the residual, of dropout the input and the residual
+  void leaf(const at::Tensor& t) {
+    if (t.defined() && t.is_leaf() && t.requires_grad()) leaves.push_back(t);
+  }
   void input(int i, const at::Tensor& t) {
     there[i] = t.defined();
-    if (t.defined() && t.is_leaf() && t.requires_grad()) leaves[i] = t;
+    leaf(t);
   }
 };
 void keep(AutogradContext* ctx, c10::intrusive_ptr<Kept> kept) {
@@ -869,24 +878,25 @@ std::pair<at::Tensor, at::Tensor> full_forward(FullInputs& in, Keep keep) {
   return {y, slopes};
 }
 
+// What a backward pass takes of a product: x (m, k) where its weight's gradient is wanted, w (n, k) where x's is
+struct FullGrads {
+  at::Tensor slopes, x, w;
+  int act = 0;
+  Drop drop;
+  int64_t k = 0;
+};
+
 // -> (dx, dweight, dbias), undefined where not wanted.  (The residual's gradient is dy.)
-std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& slopes, FullInputs& in,
-                                        const std::array<bool, 3>& want, std::initializer_list<const at::Tensor*> leaves) {
-  in.check();
-  const int64_t m = in.m, n = in.n;
-  TORCH_CHECK_VALUE(dy.scalar_type() == in.x.scalar_type() && dy.device() == in.x.device() && dy.dim() >= 1 &&
-                        dy.size(-1) == n && dy.numel() == m * n,
-                    "dy must be that of x and weight");
-  TORCH_CHECK_VALUE(slopes.defined() == (in.act != 0) &&
-                        (!slopes.defined() || (slopes.scalar_type() == at::kShort && slopes.device() == in.x.device() &&
-                                            slopes.numel() == m * n && slopes.is_contiguous())),
-                    "the slopes must be those of x and weight");
-  const int dev = in.x.get_device();
+std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const FullGrads& in, const std::array<bool, 3>& want,
+                                        at::ArrayRef<at::Tensor> leaves) {
+  const int64_t n = dy.size(-1), m = n > 0 ? dy.numel() / n : 0, k = in.k;
+  const at::Tensor& slopes = in.slopes;
+  const int dev = dy.get_device();
   check_capture(leaves, dev);
   std::array<at::Tensor, 3> out;
-  if (want[0]) out[0] = empty_as(in.x, in.x.sizes());
-  if (want[1]) out[1] = empty_as(in.w, in.w.sizes());
-  if (want[2]) out[2] = empty_as(in.x, {n});
+  if (want[0]) out[0] = empty_rows(dy, k);
+  if (want[1]) out[1] = empty_as(dy, {n, k});
+  if (want[2]) out[2] = empty_as(dy, {n});
   if (m == 0 || n == 0) {
     for (at::Tensor& g : out)
       if (g.defined()) g.zero_();
@@ -903,20 +913,20 @@ std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& 
   const long long dz_bytes = other ? 2 * m * ld : 0;
   const long long sum_bytes = want[2] ? (feedforward_linear_grad_bytes((int)m, (int)n) + 255) / 256 * 256 : 0;
   const auto product_bytes = [&](int64_t rows, int64_t sum, int turned) {
-    return feedforward_product_bytes((int)rows, (int)in.k, (int)sum, 0, turned, dev);
+    return feedforward_product_bytes((int)rows, (int)k, (int)sum, 0, turned, dev);
   };
   const long long room_bytes = std::max(want[0] ? product_bytes(m, n, FEEDFORWARD_TURN_B) : 0,
                                         want[1] ? product_bytes(n, m, FEEDFORWARD_TURN_BOTH) : 0);
   at::Tensor scratch;
   if (dz_bytes + sum_bytes + room_bytes > 0)
-    scratch = at::empty({dz_bytes + sum_bytes + room_bytes}, options_as(in.x).dtype(at::kByte));
+    scratch = at::empty({dz_bytes + sum_bytes + room_bytes}, options_as(dy).dtype(at::kByte));
   char* const base = (char*)at_of(scratch);
   const Matrix dz = other ? Matrix(base, ld) : d;
   float factor = 1.f;
   if (other || want[2]) {
     const feedforward_drop drop = in.drop.plain();
     feedforward_check(feedforward_linear_backward(d.at(), at_of(slopes), other ? base : nullptr, at_of(out[2]), (int)m,
-                                                  (int)n, d.ld, n, ld, type_code(in.x), &drop,
+                                                  (int)n, d.ld, n, ld, type_code(dy), &drop,
                                                   sum_bytes ? base + dz_bytes : nullptr, sum_bytes, &factor, dev,
                                                   current_stream(dev)));
   }
@@ -925,17 +935,50 @@ std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const at::Tensor& 
   return out;
 }
 
+// ... as they come from elsewhere than a forward pass that has checked them
+void check_full_grads(const at::Tensor& dy, FullGrads* in, const std::array<bool, 3>& want) {
+  check_operand(dy.resolve_neg(), "dy");
+  TORCH_CHECK_VALUE(dy.dim() >= 1, "dy must have a dimension");
+  const int64_t n = dy.size(-1);
+  TORCH_CHECK_VALUE((in->w.defined() || !want[0]) && (in->x.defined() || !want[1]),
+                    "the gradients of x and weight need each the other");
+  for (const at::Tensor* t : {&in->x, &in->w}) {
+    if (!t->defined()) continue;
+    const bool is_x = t == &in->x;
+    check_operand(*t, is_x ? "x" : "weight");
+    TORCH_CHECK_VALUE(t->scalar_type() == dy.scalar_type() && t->device() == dy.device() && t->dim() >= 1 &&
+                          (is_x || t->dim() == 2) && t->size(-1) != 0 && (in->k == 0 || in->k == t->size(-1)) &&
+                          (is_x ? t->numel() / t->size(-1) * n == dy.numel() : t->size(0) == n),
+                      "dy must be that of x and weight");
+    in->k = t->size(-1);
+  }
+  TORCH_CHECK_VALUE(n <= 0x7fffffff && in->k <= 0x7fffffff && (n == 0 || dy.numel() / n <= 0x7fffffff),
+                    "a size does not fit into a C int");
+  const at::Tensor& slopes = in->slopes;
+  TORCH_CHECK_VALUE(slopes.defined() == (in->act != 0) &&
+                        (!slopes.defined() || (slopes.scalar_type() == at::kShort && slopes.device() == dy.device() &&
+                                            slopes.numel() == dy.numel() && slopes.is_contiguous())),
+                    "the slopes must be those of x and weight");
+  in->drop.check(dy);
+}
+
 struct FullFunction : torch::autograd::Function<FullFunction> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const Maybe& bias,
                             const Maybe& residual, int64_t act, double p, int64_t seed, int64_t site,
                             const Maybe& seed_at) {
     FullInputs in{x, w, bias.value_or(at::Tensor()), residual.value_or(at::Tensor()), (int)act,
                   Drop{p, seed, site, seed_at.value_or(at::Tensor())}};
-    auto [y, slopes] = full_forward(in, Keep::kSlopes);
-    ctx->save_for_backward({x, w, slopes, in.drop.seed_at});
+    // Each operand is saved for the other's gradient, and the slopes for those of what they belong to: the residual's is
+    // dy whatever they are.  (Operands of a frozen layer need not live until the backward pass.)
+    const bool dx = x.requires_grad(), dw = w.requires_grad();
+    auto [y, slopes] = full_forward(in, dx || dw || (in.bias.defined() && in.bias.requires_grad()) ? Keep::kSlopes : Keep::kNothing);
+    ctx->save_for_backward({dw ? x : at::Tensor(), dx ? w : at::Tensor(), slopes, in.drop.seed_at});
     auto kept = c10::make_intrusive<Kept>();
     kept->act = in.act;
+    kept->k = in.k;
     kept->drop = in.drop;
+    kept->leaf(x);
+    kept->leaf(w);
     kept->input(0, in.bias);
     kept->input(1, in.residual);
     keep(ctx, std::move(kept));
@@ -947,12 +990,12 @@ struct FullFunction : torch::autograd::Function<FullFunction> {
     if (grads[0].defined()) {
       c10::AutoGradMode off(false);
       const auto kept = kept_by(ctx);
-      FullInputs in{saved[0], saved[1], at::Tensor(), at::Tensor(), kept->act, kept->drop};
+      FullGrads in{saved[2], saved[0], saved[1], kept->act, kept->drop, kept->k};
       in.drop.seed_at = saved[3];
       // (the context counts the inputs that are there)
       const std::array<bool, 3> want = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                                         kept->there[0] && ctx->needs_input_grad(2)};
-      auto g = full_backward(grads[0], saved[2], in, want, {&in.x, &in.w, &kept->leaves[0], &kept->leaves[1]});
+      auto g = full_backward(grads[0], in, want, kept->leaves);
       for (int i = 0; i < 3; i++) out[i] = g[i];
       if (kept->there[1] && ctx->needs_input_grad(2 + kept->there[0])) out[3] = grads[0];
     }
@@ -992,7 +1035,7 @@ at::Tensor dropout_forward(const DropoutInputs& in) {
 }
 
 // the gradient of x
-at::Tensor dropout_backward(const at::Tensor& dy, const Drop& drop, std::initializer_list<const at::Tensor*> leaves) {
+at::Tensor dropout_backward(const at::Tensor& dy, const Drop& drop, at::ArrayRef<at::Tensor> leaves) {
   check_capture(leaves, dy.get_device());
   return dropout_forward({plain_values(dy), at::Tensor(), drop});
 }
@@ -1018,7 +1061,7 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
       const auto kept = kept_by(ctx);
       Drop drop = kept->drop;
       drop.seed_at = saved[0];
-      if (ctx->needs_input_grad(0)) out[0] = dropout_backward(grads[0], drop, {&kept->leaves[0], &kept->leaves[1]});
+      if (ctx->needs_input_grad(0)) out[0] = dropout_backward(grads[0], drop, kept->leaves);
       if (kept->there[1] && ctx->needs_input_grad(1)) out[1] = grads[0];
     }
     return once_differentiable(std::move(out), "dropout", {&grads, &saved});
@@ -1101,20 +1144,19 @@ PyObject* py_linear_full_kept(PyObject*, PyObject* const* args, Py_ssize_t nargs
 PyObject* py_linear_full_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   if (!takes(nargs, 11, "linear_full_grads")) return nullptr;
-  const at::Tensor *dy = tensor(args[0], "dy"), *x = dy ? tensor(args[2], "x") : nullptr,
-                   *w = x ? tensor(args[3], "weight") : nullptr;
-  FullInputs in;
-  at::Tensor slopes;
+  const at::Tensor* const dy = tensor(args[0], "dy");
+  FullGrads in;
   std::array<bool, 3> want;
-  if (!w || !optional(args[1], "slopes", &slopes) || !to_int(args[4], &in.act) || !drop_arguments(args + 5, &in.drop)) return nullptr;
+  if (!dy || !optional(args[1], "slopes", &in.slopes) || !optional(args[2], "x", &in.x) ||
+      !optional(args[3], "weight", &in.w) || !to_int(args[4], &in.act) || !drop_arguments(args + 5, &in.drop))
+    return nullptr;
   for (int i = 0; i < 3; i++)
     if (!to_bool(args[8 + i], &want[i])) return nullptr;
-  in.x = *x;
-  in.w = *w;
   std::array<at::Tensor, 3> g;
   {
     pybind11::gil_scoped_release unlocked;
-    g = full_backward(*dy, slopes, in, want, {&in.x, &in.w});
+    check_full_grads(*dy, &in, want);
+    g = full_backward(*dy, in, want, {in.x, in.w});
   }
   return tuple_of({g[0], g[1], g[2]});
   END_HANDLE_TH_ERRORS
@@ -1221,7 +1263,7 @@ std::array<at::Tensor, 5> norm_backward(const at::Tensor& dy, const at::Tensor& 
                         lengths.numel() == 2 * in.rows && lengths.device() == in.residual.device(),
                     "lengths must be those of the forward pass");
   const int dev = in.dev();
-  check_capture({&leaf, &in.block, &in.post, &in.gate, &in.pre}, dev);
+  check_capture({leaf, in.block, in.post, in.gate, in.pre}, dev);
   std::array<at::Tensor, 5> out;
   const at::Tensor* const like[5] = {&in.residual, &in.block, &in.post, &in.gate, &in.pre};
   for (int i = 0; i < 5; i++)

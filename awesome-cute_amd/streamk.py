@@ -171,8 +171,9 @@ def linear(x, weight, bias=None, activation=None, residual=None, *, dropout=0.0,
             return y
     number, tensor = _seed_parts(dropout, seed)
     args = (x, weight, bias, residual, act, float(dropout), number, tensor, site)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
-        return torch.ops.marlin_amd.linear_full(*args)[0]
+    wants = [torch.is_grad_enabled() and t is not None and t.requires_grad for t in args[:4]]
+    if any(wants):
+        return torch.ops.marlin_amd.linear_full(*args, any(wants[:3]))[0]
     return torch.ops.marlin_amd.linear_alone(*args)
 
 
@@ -243,20 +244,21 @@ def _linear_grads_fake(dy, x, weight, want_x, want_weight):
 _Maybe = torch.Tensor | None
 
 
-# (a seed is a number, or a tensor that takes its place)
+# (a seed is a number, or a tensor that takes its place; keep: the slopes, which the residual's gradient alone does
+# not take)
 @torch.library.custom_op("marlin_amd::linear_full", mutates_args=())
 def _full_op(x: torch.Tensor, weight: torch.Tensor, bias: _Maybe, residual: _Maybe, act: int, p: float, seed: int,
-             seed_at: _Maybe, site: int) -> tuple[torch.Tensor, torch.Tensor]:
-    y, slopes = _torch_binding.linear_full_kept(x, weight, bias, residual, act, p, seed if seed_at is None else seed_at,
-                                                site)
+             seed_at: _Maybe, site: int, keep: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    args = (x, weight, bias, residual, act, p, seed if seed_at is None else seed_at, site)
+    y, slopes = _torch_binding.linear_full_kept(*args) if keep else (_torch_binding.linear_full(*args, True), None)
     return y, x.new_empty(0, dtype=torch.int16) if slopes is None else slopes
 
 
 @_full_op.register_fake
-def _full_fake(x, weight, bias, residual, act, p, seed, seed_at, site):
+def _full_fake(x, weight, bias, residual, act, p, seed, seed_at, site, keep):
     n = weight.shape[0]
     return (x.new_empty(x.shape[:-1] + (n,)),
-            x.new_empty((x.numel() // x.shape[-1], n) if act else 0, dtype=torch.int16))
+            x.new_empty((x.numel() // x.shape[-1], n) if act and keep else 0, dtype=torch.int16))
 
 
 # ... without gradients, and so without the slopes
@@ -273,22 +275,26 @@ def _alone_fake(x, weight, bias, residual, act, p, seed, seed_at, site):
 
 
 @torch.library.custom_op("marlin_amd::linear_full_grads", mutates_args=())
-def _full_grads_op(dy: torch.Tensor, slopes: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act: int, p: float,
-                   seed: int, seed_at: _Maybe, site: int,
+def _full_grads_op(dy: torch.Tensor, slopes: torch.Tensor, x: _Maybe, weight: _Maybe, act: int, p: float, seed: int,
+                   seed_at: _Maybe, site: int,
                    want: list[bool]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     out = _torch_binding.linear_full_grads(dy, slopes if act else None, x, weight, act, p,
                                            seed if seed_at is None else seed_at, site, *want)
-    return tuple(x.new_empty(0) if g is None else g for g in out)
+    return tuple(dy.new_empty(0) if g is None else g for g in out)
 
 
 @_full_grads_op.register_fake
 def _full_grads_fake(dy, slopes, x, weight, act, p, seed, seed_at, site, want):
-    return (*_grads_fake(x, weight, want[0], want[1]), x.new_empty(weight.shape[0] if want[2] else 0))
+    n = dy.shape[-1]
+    return (dy.new_empty(dy.shape[:-1] + weight.shape[1:] if want[0] else 0),
+            dy.new_empty((n,) + x.shape[-1:] if want[1] else 0), dy.new_empty(n if want[2] else 0))
 
 
 def _keep_full(ctx, inputs, output):
-    x, weight, _, _, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site = inputs
-    ctx.save_for_backward(x, weight, output[1], seed_at)
+    x, weight, _, _, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site, _ = inputs
+    # (each operand for the other's gradient)
+    want_x, want_weight = ctx.needs_input_grad[:2]
+    ctx.save_for_backward(x if want_weight else None, weight if want_x else None, output[1], seed_at)
 
 
 def _full_backward(ctx, dy, _):
@@ -298,7 +304,7 @@ def _full_backward(ctx, dy, _):
     if any(want[:3]):
         grads = torch.ops.marlin_amd.linear_full_grads(dy, slopes, x, weight, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site,
                                                        want[:3])
-    return (*(g if w else None for g, w in zip(grads, want)), dy if want[3] else None, None, None, None, None, None)
+    return (*(g if w else None for g, w in zip(grads, want)), dy if want[3] else None, *(None,) * 6)
 
 
 _full_op.register_autograd(_full_backward, setup_context=_keep_full)

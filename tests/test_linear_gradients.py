@@ -160,3 +160,117 @@ def test_the_factor_of_the_entry():
     for slopes in (None, 16):
         factor.value = 7.0
         assert call(0.5, slopes) == 0 and factor.value == 1.0  # (of no rows)
+
+
+# --- what is kept between the passes ---------------------------------------------------------
+
+def kept_bytes(call):
+    """(what lives after `call` beyond what it was given and what it returns, its result)"""
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = call()
+    return torch.cuda.memory_allocated() - before - y.numel() * y.element_size(), y
+
+
+@gpu
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("dropout", [0, 0.5])
+def test_slopes_are_kept_for_the_gradients_that_take_them(act, dropout):
+    m, n, k = 1024, 2048, 512
+    for wanted in range(4):
+        inputs = list(make(m, n, k, torch.bfloat16, 1))
+        dy = inputs.pop()
+        inputs[wanted].requires_grad_()
+        bytes, y = kept_bytes(lambda: streamk.linear(*inputs[:3], act, inputs[3], dropout=dropout, seed=3))
+        assert bytes == (2 * m * n if act and wanted < 3 else 0)
+        g, = torch.autograd.grad(y, inputs[wanted], dy)
+        assert g.shape == inputs[wanted].shape and torch.isfinite(g).all() and g.any()
+        if wanted == 3:
+            assert torch.equal(g, dy)
+
+
+@gpu
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_operands_are_kept_for_each_others_gradients(act):
+    """A frozen layer's input, and a weight whose input wants nothing, need not live until the backward pass, and
+    what is written to them then does not matter."""
+    m, n, k = 1024, 2048, 512
+    x, w, bias, residual, dy = make(m, n, k, torch.bfloat16, 1)
+    leaf = x.clone().requires_grad_()
+    want, = torch.autograd.grad(streamk.linear(leaf, w, bias, act, residual), leaf, dy)
+    inner = leaf * 1
+    bytes, y = kept_bytes(lambda: streamk.linear(inner, w, bias, act, residual))
+    assert bytes == (2 * m * n if act else 0)
+    before = torch.cuda.memory_allocated()
+    del inner
+    assert before - torch.cuda.memory_allocated() == 2 * m * k
+    assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], want)
+    inner = leaf * 1
+    y = streamk.linear(inner, w, bias, act, residual)
+    inner.detach().zero_()
+    assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], want)
+    # the weight alone, and the bias alone
+    weight = w.clone().requires_grad_()
+    want, = torch.autograd.grad(streamk.linear(x, weight, bias, act, residual), weight, dy)
+    inner = weight * 1
+    y = streamk.linear(x, inner, bias, act, residual)
+    before = torch.cuda.memory_allocated()
+    del inner
+    assert before - torch.cuda.memory_allocated() == 2 * n * k
+    assert torch.equal(torch.autograd.grad(y, weight, dy)[0], want)
+    b = bias.clone().requires_grad_()
+    want, = torch.autograd.grad(streamk.linear(x, w, b, act, residual), b, dy)
+    copies = [x.clone(), w.clone()]
+    y = streamk.linear(*copies, b, act, residual)
+    before = torch.cuda.memory_allocated()
+    del copies
+    assert before - torch.cuda.memory_allocated() == 2 * (m + n) * k
+    assert torch.equal(torch.autograd.grad(y, b, dy)[0], want)
+    # what is needed is still looked at
+    inner = x * 1
+    y = streamk.linear(inner, weight, bias, act, residual)
+    inner.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, weight, dy)
+
+
+@gpu
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_compiled_passes_with_some_of_the_gradients(act):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    m, n, k = 70, 72, 136
+    for wanted in range(4):
+        inputs = list(make(m, n, k, torch.bfloat16, 1))
+        dy = inputs.pop()
+        inputs[wanted].requires_grad_()
+
+        def f(x, w, b, r):
+            return streamk.linear(x, w, b, act, r, dropout=0.25, seed=7)
+
+        want, = torch.autograd.grad(f(*inputs), inputs[wanted], dy)
+        torch._dynamo.reset()
+        compiled = torch.compile(f, backend="aot_eager", fullgraph=True)
+        assert torch.equal(torch.autograd.grad(compiled(*inputs), inputs[wanted], dy)[0], want)
+
+        def step(x, w, b, r, dy):
+            return torch.autograd.grad(f(x, w, b, r), (x, w, b, r)[wanted], dy)[0]
+
+        assert torch.equal(make_fx(step)(*inputs, dy)(*inputs, dy), want)
+
+
+@gpu
+def test_refusals_of_the_gradients_by_themselves():
+    x, w, bias, residual, dy = make(20, 24, 16, torch.float16, 1)
+    grads = streamk._torch_binding.linear_full_grads
+    slopes = torch.zeros(20, 24, dtype=torch.int16, device="cuda")
+    assert grads(dy, None, None, w, 0, 0.0, None, 0, True, False, True)[0].shape == (20, 16)
+    assert grads(dy, None, x, None, 0, 0.0, None, 0, False, True, False)[1].shape == (24, 16)
+    assert grads(dy, slopes, None, None, 1, 0.0, None, 0, False, False, True)[2].shape == (24,)
+    for args in ((dy, None, x, None, 0, 0.0, None, 0, True, False, False), (dy, None, None, w, 0, 0.0, None, 0, False, True, False),
+                 (dy, None, x, w[:16], 0, 0.0, None, 0, True, False, False), (dy[:10], None, x, w, 0, 0.0, None, 0, True, True, False),
+                 (dy.bfloat16(), None, x, w, 0, 0.0, None, 0, True, True, False), (dy.cpu(), None, x, w, 0, 0.0, None, 0, True, True, False),
+                 (dy, None, x, w[:, :8], 0, 0.0, None, 0, True, True, False), (dy, None, x, w, 1, 0.0, None, 0, True, True, False),
+                 (dy, slopes, x, w, 0, 0.0, None, 0, True, True, False), (dy, slopes[:10], x, w, 1, 0.0, None, 0, True, True, False),
+                 (dy, None, x, w, 0, 1.5, 1, 0, True, True, False)):
+        with pytest.raises(ValueError):
+            grads(*args)
