@@ -117,13 +117,15 @@ constexpr double kSliceLaunch = 2.96, kSliceBytes = 0.327e-6;
 
 struct ProductPlan {
   FfTile tile;
-  int slices;
+  int slices;  // 0: no tile computes the product in one launch
+  bool few;    // by the kernel for few rows, whose tiles are one of kFewFits
 };
 
+// whether a tile of kFits or kSmallFits computes a product
 bool tile_takes(const FfTile& t, Layout layout, Finish finish, int m) {
   // (of 32 columns: where the kernel for few rows, whose tiles are named so too, does not compute)
   if (t.rows == 32) return finish == kFull && (t.cols == 64 || (t.cols == 32 && m > kProductRows));
-  if (few_tile(t)) return false;
+  if (t.cols < 64) return false;  // (one of that kernel's alone)
   return layout != kTurnBoth || t.rows != 96;  // (64, 128 or 256 columns of a turned operand)
 }
 
@@ -140,15 +142,15 @@ ProductPlan choose_plan(int m, int n, int k, Finish finish, Layout layout, int c
   const bool gated = finish == kGated;
   const int columns = product_columns(n, gated), stages = ceil_div(k, kDnStageK);
   const bool few = layout == kRows && m <= kProductRows;
-  const bool forced = t_tile.rows > 0 && ((few && few_tile(t_tile)) || tile_takes(t_tile, layout, finish, m));
-  ProductPlan best = {{64, 64}, 1};
+  const bool forced = t_tile.rows > 0 && ((few && t_tile.cols <= 32) || tile_takes(t_tile, layout, finish, m));
+  ProductPlan best = {{64, 64}, 0, false};
   double least = 0.0;
   if (few)
     for (const TileFit& f : kFewFits) {
       if (f.tile.rows != ceil_div(m, 16) * 16 || (forced && f.tile.cols != t_tile.cols)) continue;
       const double cost = fit_cost(f, ceil_div(n, gated ? f.tile.cols / 2 : f.tile.cols), ceil_div(stages, 4), cus);
       if (least == 0.0 || cost < least) {
-        best = {f.tile, 1};
+        best = {f.tile, 1, true};
         least = cost;
       }
     }
@@ -159,11 +161,12 @@ ProductPlan choose_plan(int m, int n, int k, Finish finish, Layout layout, int c
     for (int slices = 1; slices <= kSlicesMost && slices <= stages; slices++) {
       const double bytes = 4.0 * slices * m * columns;
       if (slices > 1 && (bytes > (double)room || (t_slices == 0 && tiles * slices > 2 * cus))) break;
+      if (tiles * slices * tile_threads(f.tile) > kLaunchThreads || (slices > 1 && (long long)m * n / 4 > kLaunchThreads)) break;
       if (t_slices > 0 && slices != t_slices && t_slices <= stages && 4.0 * t_slices * m * columns <= (double)room) continue;
       double cost = fit_cost(f, tiles * slices, ceil_div(stages, slices), cus);
       if (slices > 1) cost += kSliceLaunch + kSliceBytes * bytes;
       if (least == 0.0 || cost < least) {
-        best = {f.tile, slices};
+        best = {f.tile, slices, false};
         least = cost;
       }
     }
@@ -183,7 +186,7 @@ Meeting meeting(const ProductPlan& p, int m, int columns) {
   const long long tiles = (long long)ceil_div(m, p.tile.rows) * ceil_div(columns, p.tile.cols);
   const long long sums = 2 * tiles * (long long)big_sums(p.tile.rows);
   // (the sums' offsets are ints)
-  if (p.slices != 2 || !big_tile(p.tile) || sums > 0x7fffffffLL) return {0, 0, 0};
+  if (p.few || p.slices != 2 || !big_tile(p.tile) || sums > 0x7fffffffLL) return {0, 0, 0};
   return {(int)tiles, sums, sums + tiles * kWordStride * 8};
 }
 
@@ -202,7 +205,7 @@ unsigned long long next_token() {
 // for the room and again for the launch, and a model's layers are a few sizes over and over.
 struct Planned {
   int m = 0, n = 0, k = 0, cus = 0, form = -1;
-  ProductPlan plan = {{0, 0}, 0};
+  ProductPlan plan = {{0, 0}, 0, false};
   long long bytes = 0;  // of partial sums, and where slices meet in their tiles of the words
 };
 constexpr int kPlansKept = 16;
@@ -278,19 +281,22 @@ bool layout_of(int turned, Layout* layout) {
 int run_product(ProductArgs a, Layout layout, bool bf, void* room, long long room_bytes, int dev, hipStream_t stream) {
   const bool gated = a.finish == kGated;
   const long long columns = product_columns(a.N, gated);
-  // (a launch's grid, at the smallest tiles)
-  if (a.M > 0x7ffffe00 || columns > 0x3fffffffLL || (columns / 64 + 1) * (a.M / 64 + 1LL) > 0x3fffffffLL / kSlicesMost)
+  // (rows rounded up to tiles are an int, and the highest and widest tiles a launch: a plan takes such as are)
+  if (a.M > 0x7ffffe00 || (columns + 255) / 256 * ((a.M + 255) / 256) * 256 > kLaunchThreads)
     return fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many tiles", a.M, a.N);
   // a gated product's rows of either half are addressed from one place
   if (gated && 2LL * a.N * a.ldb * 2 > 0x7fffffffLL)
     return fail(FEEDFORWARD_ERR_SHAPE, "weights of more than 2 GiB (n = %d, rows of %d): split the call", a.N, a.ldb);
   if (!a.A || !a.B || !a.C) return fail(FEEDFORWARD_ERR_SHAPE, "a matrix is missing");
   if (room && off16(room)) return fail(FEEDFORWARD_ERR_SHAPE, "scratch must start on 16 bytes");
-  return on_device(dev, [&](int cus) {
+  bool fits = true;
+  const int rc = on_device(dev, [&](int cus) {
     const Planned planned = plan_with_room(a.M, a.N, a.K, a.finish, layout, cus);
     const long long have = room ? room_bytes : 0;
     const ProductPlan p =
         planned.bytes <= have ? planned.plan : choose_plan(a.M, a.N, a.K, a.finish, layout, cus, have);
+    fits = p.slices > 0;
+    if (!fits) return;  // (where a tile is forced)
     a.slices = p.slices;
     a.part = p.slices > 1 ? (float*)room : nullptr;
     a.ldpart = (int)columns;
@@ -300,7 +306,7 @@ int run_product(ProductArgs a, Layout layout, bool bf, void* room, long long roo
       a.words = (unsigned long long*)((char*)room + meet.words);
       a.token = next_token();
     }
-    if (few_tile(p.tile) && a.M <= kProductRows)
+    if (p.few)
       launch_product_rows(a, p.tile.cols / 16, bf, stream);
     else if (big_tile(p.tile))
       (bf ? launch_product_big_bf16 : launch_product_big_f16)(a, p.tile.rows, layout, stream);
@@ -308,6 +314,9 @@ int run_product(ProductArgs a, Layout layout, bool bf, void* room, long long roo
       launch_product_tiles(a, p.tile, layout, bf, stream);
     if (a.part && !a.words) launch_sum_parts(a, bf, stream);
   });
+  if (rc == FEEDFORWARD_OK && !fits)
+    return fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many tiles", a.M, a.N);
+  return rc;
 }
 
 int device_cus(int dev) {
@@ -524,7 +533,7 @@ int feedforward_gated_grad(const void* dh, const float* pre, void* dgu, int m, i
   if (rc == FEEDFORWARD_OK) rc = check_matrix("dgu", dgu, lddgu, 2LL * n);
   if (rc == FEEDFORWARD_OK && !act_known(activation))
     rc = fail(FEEDFORWARD_ERR_SHAPE, "unknown activation %d", activation);
-  if (rc == FEEDFORWARD_OK && (long long)m * (n / 8) > 0x7fffffffLL * 128)
+  if (rc == FEEDFORWARD_OK && (long long)m * (n / 8) > kLaunchThreads - 255)
     rc = fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many", m, n);
   if (rc != FEEDFORWARD_OK || m == 0 || n == 0) return rc;
   if (!dh || !pre || !dgu) return fail(FEEDFORWARD_ERR_SHAPE, "a matrix is missing");
@@ -599,6 +608,7 @@ int feedforward_plan(int m, int n, int k, int gated, int turned, int cus, int* o
   if (!layout_of(turned, &layout)) return fail(FEEDFORWARD_ERR_SHAPE, "unknown layout %d", turned);
   if (cus < 1) return fail(FEEDFORWARD_ERR_SHAPE, "%d compute units", cus);
   const ProductPlan p = plan_with_room(m, n, k, finish_of(gated), layout, cus).plan;
+  if (p.slices == 0) return fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many tiles", m, n);
   out[0] = p.tile.rows;
   out[1] = p.tile.cols;
   out[2] = p.slices;

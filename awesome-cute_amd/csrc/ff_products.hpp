@@ -166,8 +166,10 @@ constexpr int kSlicesMost = 8;  // of the k range
 constexpr int kWordStride = 8;  // a tile's slices meet in a cache line of their own
 // bytes of a big tile's sums
 constexpr size_t big_sums(int rows) { return (size_t)rows * 256 * 4; }
-inline bool big_tile(const FfTile& t) { return t.cols == 256 && t.rows >= 160; }
-inline bool few_tile(const FfTile& t) { return t.cols <= 32; }
+constexpr bool big_tile(const FfTile& t) { return t.cols == 256 && t.rows >= 160; }
+// a tile's workgroup
+constexpr int tile_threads(const FfTile& t) { return t.cols <= 64 || big_tile(t) ? 256 : 512; }
+constexpr long long kLaunchThreads = 0xffffffffLL;  // of all workgroups of a launch
 hipError_t configure_product_tiles();
 hipError_t configure_product_big_f16();
 hipError_t configure_product_big_bf16();

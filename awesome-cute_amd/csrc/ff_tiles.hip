@@ -42,6 +42,7 @@ struct FfShape {
   static constexpr int kLds = kRingBytes > kTileBytes ? kRingBytes : kTileBytes;
   static_assert(kTB * 8 * kWaves == TN && TM % (16 * WM) == 0 && TN % (16 * WN) == 0, "whole blocks");
   static_assert(!GATED || kNJ % 2 == 0, "a gate's operand and its partner's in one wave");
+  static_assert(kThreads == tile_threads({TM, TN}), "");
   static_assert(kLds <= 160 * 1024 - 256, "LDS of a compute unit");
 };
 
