@@ -40,8 +40,9 @@ SOURCES = {
     "ff_host.hip": [],
 }
 # Kernels whose main loop is one assembly statement with fixed registers: what the compiler spills, it
-# spills around that statement, and results have been wrong where it did (tiles of 256 rows).  The build
-# fails instead.
+# spills around that statement, and results have been wrong where it did (tiles of 256 rows).  Why is not
+# known: gen_products.py checks that the statement tells of every register that it writes, and waits for all that it
+# issues.  The build fails instead.
 WITHOUT_SCRATCH = {"ff_big_f16.hip", "ff_big_bf16.hip"}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

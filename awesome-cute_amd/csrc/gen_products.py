@@ -50,6 +50,7 @@ Registers (v = VGPR, a = AGPR, s = SGPR):
   s62 s63             bytes from one slab to the next, A and B
 """
 import math
+import re
 import sys
 
 RA, RB = 40, 44
@@ -316,9 +317,46 @@ def generate(sh, mfma):
     return e.lines
 
 
+def registers(operand):
+    """the registers that an operand names, one by one"""
+    match = re.fullmatch(r"([sva])(?:(\d+)|\[(\d+):(\d+)\])", operand)
+    if not match:
+        return {"m0"} if operand == "m0" else set()
+    kind, one, lo, hi = match.groups()
+    return {f"{kind}{n}" for n in range(int(one or lo), int(one or hi) + 1)}
+
+
+WRITES = re.compile(r"v_(mfma_\w+|accvgpr_write_b32|or_b32)|ds_read_\w+|s_(mov_b32|add_u32|addc_u32|sub_u32|cselect_b32)")
+WRITES_NOTHING = re.compile(r"buffer_load_dwordx4|s_(cmp_\w+|c?branch\w*|waitcnt|barrier|nop)")
+
+
+def check_operands(lines, outs, ties, ins, clobbers):
+    """What a statement does to registers is what it says: what it writes is an output, tied or clobbered (m0 apart, which is
+    reserved: the compiler sets it ahead of each use of its own, and would only warn), what it reads it was
+    given or has written, and none of the four lists shares a register with another."""
+    groups = [set().union(*map(registers, g)) for g in (outs, ties, ins, clobbers)]
+    assert sum(map(len, groups)) == len(set().union(*groups)), "a register in two lists"
+    outs, ties, ins, clobbers = groups
+    written, known = set(), ties | ins
+    for line in lines:
+        if line.endswith(":"):
+            continue
+        name, _, rest = line.partition(" ")
+        operands = [registers(o) for o in re.split(r",? +|,", rest)]
+        assert WRITES.fullmatch(name) or WRITES_NOTHING.fullmatch(name), line
+        if WRITES.fullmatch(name):
+            written |= operands[0]
+            known |= operands.pop(0)
+        missing = set().union(*operands) - known if operands else set()
+        assert not missing, (line, missing)
+    assert written <= outs | ties | clobbers | {"m0"}, written - outs - ties - clobbers
+    assert not written & ins and outs <= written
+
+
 def statement(sh, mfma):
+    lines = generate(sh, mfma)
     out = ["// generated by gen_products.py -- do not edit", "asm volatile("]
-    out += [f'    "{l}\\n\\t"' for l in generate(sh, mfma)]
+    out += [f'    "{l}\\n\\t"' for l in lines]
     outs = [f'"={{{aq(32 * i + 4 * o)}}}"(acc[{i}][{o}])' for i in range(sh.rb) for o in range(8)]
     outs += [f'"+{{{sq(RA)}}}"(ra_words)', f'"+{{{sq(RB)}}}"(rb_words)']
     by_rows = [t for t in range(sh.loads) if not (sh.turn_a if t < sh.ta else sh.turn_b)]
@@ -336,7 +374,10 @@ def statement(sh, mfma):
     clob = [f"v{n}" for n in range(64 + 4 * sh.rb)]
     clob += [f"s{S_REQA}", f"s{S_REQB}", f"s{S_LEFT}"]
     clob += [f"s{S_MA + s}" for s in range(1, sh.ring_a)] + [f"s{S_MB + s}" for s in range(1, sh.ring_b)]
-    clob += ["scc", "memory"]  # (m0 is the compiler's to reserve; it keeps nothing there)
+    named = [re.findall(r"\{([^}]*)\}", " ".join(c)) for c in
+             ([o for o in outs if o[1] == "="], [o for o in outs if o[1] == "+"], ins)]
+    check_operands(lines, *named, clob)
+    clob += ["scc", "memory"]
     out.append("    : " + ", ".join(f'"{c}"' for c in clob) + ");")
     return "\n".join(out) + "\n"
 
