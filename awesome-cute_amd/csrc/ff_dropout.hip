@@ -5,11 +5,14 @@
 // ones four of one group and four of another, so that a wave's loads are of neighbouring bytes.  Inside
 // fp32, rounded once.
 //
-// Bound: HBM, or the last-level cache, which holds up to 256 MB of a call.  Results are stored as not
-// read again here (nontemporal).  Operands are requested so where a call moves more than that cache holds: 16384 x 4096
-// bfloat16 with a residual, 403 MB, 61.7 us, 6.5 TB/s (otherwise 67.7, and 69.1 with plain stores).  Where it
-// moves less they are mostly there, just written by what came before, and such requests would pass it by:
-// 2048 x 10752 12.0 us, 7.4 TB/s (15.0).  The generator costs nothing visible; two or four groups
+// Bound: HBM, or the last-level cache, which holds up to 256 MB of a call.  Operands are requested as read once
+// (nontemporal) where a call moves more than that cache holds: 16384 x 4096 bfloat16 with a residual, 403 MB, 61.2 us,
+// 6.6 TB/s (otherwise 70.3).  Where it moves less they are mostly there, just written by what came before, and such
+// requests would pass it by: 2048 x 10752 12.0 us (15.0), with operands that take turns 13.9.  Results are
+// stored past the caches where they alone are more than the last one holds: 65536 x 4096 with a residual 249 us (261), and the norm that
+// reads it 222 (227).  Smaller ones are read from there next, and stored past it cost their reader more than they save
+// here: 2048 x 10752 13.6 us in place of 13.9, but with a product behind it 162 in place of 151, 16384 x 4096
+// 44.0 in place of 41.0, and 480 in place of 442.  The generator costs nothing visible; two or four groups
 // a lane, or a grid of eight workgroups a compute unit, 2 to 10 % more.
 #include <hip/hip_runtime.h>
 
@@ -43,11 +46,14 @@ __device__ __forceinline__ Piece16<T> load_piece(const T* at, long long left) {
     if (e < left) out[e] = at[e];
   return out;
 }
-template <bool WHOLE, class T>
+template <bool WHOLE, bool PAST, class T>
 __device__ __forceinline__ void store_piece16(T* at, long long left, Piece16<T> v) {
   constexpr int kN = 16 / sizeof(T);
   if (WHOLE && left >= kN) {
-    __builtin_nontemporal_store(__builtin_bit_cast(i4, v), (i4*)at);
+    if constexpr (PAST)
+      __builtin_nontemporal_store(__builtin_bit_cast(i4, v), (i4*)at);
+    else
+      *(i4*)at = __builtin_bit_cast(i4, v);
     return;
   }
 #pragma unroll
@@ -57,8 +63,8 @@ __device__ __forceinline__ void store_piece16(T* at, long long left, Piece16<T> 
 
 }  // namespace
 
-// WHOLE: every matrix starts on 16 bytes; ONCE: operands are requested as read once
-template <class T, bool WHOLE, bool ONCE>
+// WHOLE: every matrix starts on 16 bytes; ONCE: operands are requested as read once; PAST: results are stored past the caches
+template <class T, bool WHOLE, bool ONCE, bool PAST>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(DropoutArgs p) {
   constexpr int kN = 16 / sizeof(T), kPieces = 8 / kN;
   const int lane = threadIdx.x & 63;
@@ -94,22 +100,24 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(DropoutArgs p) {
       const float v = drop_one((float)x[i][e], bits, kN * i + e, p.drop);
       x[i][e] = (T)(p.residual ? (float)residual[i][e] + v : v);
     }
-    store_piece16<WHOLE, T>((T*)p.y + at[i], p.count - at[i], x[i]);
+    store_piece16<WHOLE, PAST, T>((T*)p.y + at[i], p.count - at[i], x[i]);
   }
 }
 
 template <class T>
 static void launch_of(const DropoutArgs& a, hipStream_t stream) {
   const bool whole = (((uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.y) & 15) == 0;
-  const bool once = a.count * (long long)sizeof(T) * (a.residual ? 3 : 2) > kLastLevel;
+  const long long bytes = a.count * (long long)sizeof(T);
   const dim3 grid((unsigned)((a.count + 8 * kThreads - 1) / (8 * kThreads)));
   const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a); };
   if (!whole)
-    launch(dropout_kernel<T, false, false>);
-  else if (once)
-    launch(dropout_kernel<T, true, true>);
+    launch(dropout_kernel<T, false, false, false>);
+  else if (bytes > kLastLevel)
+    launch(dropout_kernel<T, true, true, true>);
+  else if (bytes * (a.residual ? 3 : 2) > kLastLevel)
+    launch(dropout_kernel<T, true, true, false>);
   else
-    launch(dropout_kernel<T, true, false>);
+    launch(dropout_kernel<T, true, false, false>);
 }
 
 void launch_dropout(const DropoutArgs& a, int type, hipStream_t stream) {
