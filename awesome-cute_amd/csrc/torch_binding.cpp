@@ -424,16 +424,14 @@ void feedforward_check(int rc) {
   TORCH_CHECK(rc == FEEDFORWARD_OK, feedforward_last_error());
 }
 
-void check_operand(const at::Tensor& t, const char* name) {
-  TORCH_CHECK_VALUE(t.is_cuda() && (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16), name,
-                    " must be a torch.half or torch.bfloat16 tensor on the GPU");
-  TORCH_CHECK_VALUE(t.layout() == at::kStrided && !t.is_neg() && !t.is_conj(), name, " must be a plain tensor");
-}
-
 // x (..., k) and w (rows, k)
 void check_dense(const at::Tensor& x, const at::Tensor& w) {
-  check_operand(x, "x");
-  check_operand(w, "weight");
+  for (const at::Tensor* t : {&x, &w}) {
+    const char* const name = t == &x ? "x" : "weight";
+    TORCH_CHECK_VALUE(t->is_cuda() && (t->scalar_type() == at::kHalf || t->scalar_type() == at::kBFloat16), name,
+                      " must be a torch.half or torch.bfloat16 tensor on the GPU");
+    TORCH_CHECK_VALUE(t->layout() == at::kStrided && !t->is_neg() && !t->is_conj(), name, " must be a plain tensor");
+  }
   TORCH_CHECK_VALUE(x.scalar_type() == w.scalar_type() && x.device() == w.device(),
                     "x and weight must have one type and one device");
   TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(1) != 0,
@@ -936,24 +934,13 @@ std::array<at::Tensor, 3> full_backward(const at::Tensor& dy, const FullGrads& i
 }
 
 // ... as they come from elsewhere than a forward pass that has checked them
-void check_full_grads(const at::Tensor& dy, FullGrads* in, const std::array<bool, 3>& want) {
-  check_operand(dy.resolve_neg(), "dy");
-  TORCH_CHECK_VALUE(dy.dim() >= 1, "dy must have a dimension");
-  const int64_t n = dy.size(-1);
-  TORCH_CHECK_VALUE((in->w.defined() || !want[0]) && (in->x.defined() || !want[1]),
-                    "the gradients of x and weight need each the other");
-  for (const at::Tensor* t : {&in->x, &in->w}) {
-    if (!t->defined()) continue;
-    const bool is_x = t == &in->x;
-    check_operand(*t, is_x ? "x" : "weight");
-    TORCH_CHECK_VALUE(t->scalar_type() == dy.scalar_type() && t->device() == dy.device() && t->dim() >= 1 &&
-                          (is_x || t->dim() == 2) && t->size(-1) != 0 && (in->k == 0 || in->k == t->size(-1)) &&
-                          (is_x ? t->numel() / t->size(-1) * n == dy.numel() : t->size(0) == n),
-                      "dy must be that of x and weight");
-    in->k = t->size(-1);
-  }
-  TORCH_CHECK_VALUE(n <= 0x7fffffff && in->k <= 0x7fffffff && (n == 0 || dy.numel() / n <= 0x7fffffff),
-                    "a size does not fit into a C int");
+void check_full_grads(const at::Tensor& dy, FullGrads* in) {
+  check_dense(in->x, in->w);
+  in->k = in->w.size(1);
+  TORCH_CHECK_VALUE(dy.scalar_type() == in->x.scalar_type() && dy.device() == in->x.device() &&
+                        dy.layout() == at::kStrided && dy.dim() >= 1 && dy.size(-1) == in->w.size(0) &&
+                        dy.numel() == in->x.numel() / in->k * in->w.size(0),
+                    "dy must be that of x and weight");
   const at::Tensor& slopes = in->slopes;
   TORCH_CHECK_VALUE(slopes.defined() == (in->act != 0) &&
                         (!slopes.defined() || (slopes.scalar_type() == at::kShort && slopes.device() == dy.device() &&
@@ -1144,18 +1131,20 @@ PyObject* py_linear_full_kept(PyObject*, PyObject* const* args, Py_ssize_t nargs
 PyObject* py_linear_full_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   if (!takes(nargs, 11, "linear_full_grads")) return nullptr;
-  const at::Tensor* const dy = tensor(args[0], "dy");
+  const at::Tensor *dy = tensor(args[0], "dy"), *x = dy ? tensor(args[2], "x") : nullptr,
+                   *w = x ? tensor(args[3], "weight") : nullptr;
   FullGrads in;
   std::array<bool, 3> want;
-  if (!dy || !optional(args[1], "slopes", &in.slopes) || !optional(args[2], "x", &in.x) ||
-      !optional(args[3], "weight", &in.w) || !to_int(args[4], &in.act) || !drop_arguments(args + 5, &in.drop))
+  if (!w || !optional(args[1], "slopes", &in.slopes) || !to_int(args[4], &in.act) || !drop_arguments(args + 5, &in.drop))
     return nullptr;
+  in.x = *x;
+  in.w = *w;
   for (int i = 0; i < 3; i++)
     if (!to_bool(args[8 + i], &want[i])) return nullptr;
   std::array<at::Tensor, 3> g;
   {
     pybind11::gil_scoped_release unlocked;
-    check_full_grads(*dy, &in, want);
+    check_full_grads(*dy, &in);
     g = full_backward(*dy, in, want, {in.x, in.w});
   }
   return tuple_of({g[0], g[1], g[2]});

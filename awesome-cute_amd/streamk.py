@@ -275,26 +275,23 @@ def _alone_fake(x, weight, bias, residual, act, p, seed, seed_at, site):
 
 
 @torch.library.custom_op("marlin_amd::linear_full_grads", mutates_args=())
-def _full_grads_op(dy: torch.Tensor, slopes: torch.Tensor, x: _Maybe, weight: _Maybe, act: int, p: float, seed: int,
-                   seed_at: _Maybe, site: int,
+def _full_grads_op(dy: torch.Tensor, slopes: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act: int, p: float,
+                   seed: int, seed_at: _Maybe, site: int,
                    want: list[bool]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     out = _torch_binding.linear_full_grads(dy, slopes if act else None, x, weight, act, p,
                                            seed if seed_at is None else seed_at, site, *want)
-    return tuple(dy.new_empty(0) if g is None else g for g in out)
+    return tuple(x.new_empty(0) if g is None else g for g in out)
 
 
 @_full_grads_op.register_fake
 def _full_grads_fake(dy, slopes, x, weight, act, p, seed, seed_at, site, want):
-    n = dy.shape[-1]
-    return (dy.new_empty(dy.shape[:-1] + weight.shape[1:] if want[0] else 0),
-            dy.new_empty((n,) + x.shape[-1:] if want[1] else 0), dy.new_empty(n if want[2] else 0))
+    return (*_grads_fake(x, weight, want[0], want[1]), x.new_empty(weight.shape[0] if want[2] else 0))
 
 
 def _keep_full(ctx, inputs, output):
     x, weight, _, _, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site, _ = inputs
-    # (each operand for the other's gradient)
-    want_x, want_weight = ctx.needs_input_grad[:2]
-    ctx.save_for_backward(x if want_weight else None, weight if want_x else None, output[1], seed_at)
+    # (both, whichever is needed: they are also the leaves that a captured backward pass looks at)
+    ctx.save_for_backward(x, weight, output[1], seed_at)
 
 
 def _full_backward(ctx, dy, _):

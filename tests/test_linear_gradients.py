@@ -263,14 +263,33 @@ def test_refusals_of_the_gradients_by_themselves():
     x, w, bias, residual, dy = make(20, 24, 16, torch.float16, 1)
     grads = streamk._torch_binding.linear_full_grads
     slopes = torch.zeros(20, 24, dtype=torch.int16, device="cuda")
-    assert grads(dy, None, None, w, 0, 0.0, None, 0, True, False, True)[0].shape == (20, 16)
-    assert grads(dy, None, x, None, 0, 0.0, None, 0, False, True, False)[1].shape == (24, 16)
-    assert grads(dy, slopes, None, None, 1, 0.0, None, 0, False, False, True)[2].shape == (24,)
-    for args in ((dy, None, x, None, 0, 0.0, None, 0, True, False, False), (dy, None, None, w, 0, 0.0, None, 0, False, True, False),
-                 (dy, None, x, w[:16], 0, 0.0, None, 0, True, False, False), (dy[:10], None, x, w, 0, 0.0, None, 0, True, True, False),
-                 (dy.bfloat16(), None, x, w, 0, 0.0, None, 0, True, True, False), (dy.cpu(), None, x, w, 0, 0.0, None, 0, True, True, False),
-                 (dy, None, x, w[:, :8], 0, 0.0, None, 0, True, True, False), (dy, None, x, w, 1, 0.0, None, 0, True, True, False),
-                 (dy, slopes, x, w, 0, 0.0, None, 0, True, True, False), (dy, slopes[:10], x, w, 1, 0.0, None, 0, True, True, False),
-                 (dy, None, x, w, 0, 1.5, 1, 0, True, True, False)):
+    want = (True, False, True)
+    dx, dw, db = grads(dy, slopes, x, w, 1, 0.0, None, 0, *want)
+    assert dx.shape == (20, 16) and dw is None and db.shape == (24,)
+    for args in ((dy, None, x, w[:16], 0), (dy[:10], None, x, w, 0), (dy.bfloat16(), None, x, w, 0), (dy.cpu(), None, x, w, 0),
+                 (dy, None, x, w[:, :8], 0), (dy, None, x, w, 1), (dy, slopes, x, w, 0), (dy, slopes[:10], x, w, 1)):
         with pytest.raises(ValueError):
-            grads(*args)
+            grads(*args, 0.0, None, 0, *want)
+    with pytest.raises(ValueError):
+        grads(dy, None, x, w, 0, 1.5, 1, 0, *want)
+
+
+@gpu
+def test_a_captured_pass_of_an_operator_beside_an_eager_graph_of_its_leaves():
+    """The operator that compilers see looks at its operands, also at one that no gradient takes."""
+    x, w, bias, residual, dy = make(70, 72, 136, torch.float16, 6)
+    side = torch.cuda.Stream()
+    for i in range(2):
+        inputs = [x, w]
+        inputs[i] = inputs[i].clone().requires_grad_()
+
+        def forward():
+            return torch.ops.marlin_amd.linear_full(*inputs, bias, None, 1, 0.0, 0, None, 0, True)[0]
+
+        alive = forward()
+        with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                torch.autograd.grad(forward(), inputs[i], dy)
+        torch.cuda.synchronize()
+        assert torch.isfinite(torch.autograd.grad(alive, inputs[i], dy)[0]).all()
+        del alive
