@@ -803,6 +803,17 @@ bool drop_arguments(PyObject* const* args, Drop* out) {
   return to_int64(args[1], "seed", &out->seed);
 }
 
+// the tensors behind the first `want` arguments
+bool leaves_behind(PyObject* const* args, Py_ssize_t nargs, Py_ssize_t want, const char* name, std::vector<at::Tensor>* out) {
+  if (nargs < want) return takes(nargs, want, name);
+  for (Py_ssize_t i = want; i < nargs; i++) {
+    const at::Tensor* const t = tensor(args[i], "leaves");
+    if (!t) return false;
+    out->push_back(*t);
+  }
+  return true;
+}
+
 // What a forward pass keeps besides the tensors that it saves, as one object (an entry of the context's
 // dictionary for each takes the host 0.1 to 0.2 us, both ways).  The leaves are what gradients go to that the
 // backward pass has no other use for: check_capture wants them, and a leaf's accumulator, which the
@@ -1109,9 +1120,26 @@ PyObject* py_dropout(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// dropout_grad(dy, p, seed, site, leaves) -> dx, for compilers
+PyObject* py_dropout_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Drop drop;
+  std::vector<at::Tensor> leaves;
+  if (!leaves_behind(args, nargs, 4, "dropout_grad", &leaves)) return nullptr;
+  const at::Tensor* const dy = tensor(args[0], "dy");
+  if (!dy || !drop_arguments(args + 1, &drop)) return nullptr;
+  at::Tensor dx;
+  {
+    pybind11::gil_scoped_release unlocked;
+    dx = dropout_backward(*dy, drop, leaves);
+  }
+  return THPVariable_Wrap(std::move(dx));
+  END_HANDLE_TH_ERRORS
+}
+
 // linear_full_kept(... as linear_full) -> (y, the slopes or None) and linear_full_grads(dy, slopes, x, weight,
-// activation, p, seed, site, want_x, want_weight, want_bias) -> (dx, dweight, dbias), None where not wanted: the
-// passes by themselves, for compilers.  linear_full_slopes: linear_full_kept with slopes in the form of the C
+// activation, p, seed, site, want_x, want_weight, want_bias, more leaves) -> (dx, dweight, dbias), None where not
+// wanted: the passes by themselves, for compilers.  linear_full_slopes: linear_full_kept with slopes in the form of the C
 // entry feedforward_linear.
 template <Keep KEEP>
 PyObject* py_linear_full_kept(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -1130,7 +1158,8 @@ PyObject* py_linear_full_kept(PyObject*, PyObject* const* args, Py_ssize_t nargs
 
 PyObject* py_linear_full_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (!takes(nargs, 11, "linear_full_grads")) return nullptr;
+  std::vector<at::Tensor> leaves;
+  if (!leaves_behind(args, nargs, 11, "linear_full_grads", &leaves)) return nullptr;
   const at::Tensor *dy = tensor(args[0], "dy"), *x = dy ? tensor(args[2], "x") : nullptr,
                    *w = x ? tensor(args[3], "weight") : nullptr;
   FullGrads in;
@@ -1141,11 +1170,13 @@ PyObject* py_linear_full_grads(PyObject*, PyObject* const* args, Py_ssize_t narg
   in.w = *w;
   for (int i = 0; i < 3; i++)
     if (!to_bool(args[8 + i], &want[i])) return nullptr;
+  leaves.push_back(in.x);
+  leaves.push_back(in.w);
   std::array<at::Tensor, 3> g;
   {
     pybind11::gil_scoped_release unlocked;
     check_full_grads(*dy, &in);
-    g = full_backward(*dy, in, want, {in.x, in.w});
+    g = full_backward(*dy, in, want, leaves);
   }
   return tuple_of({g[0], g[1], g[2]});
   END_HANDLE_TH_ERRORS
@@ -1537,6 +1568,7 @@ PyMethodDef methods[] = {
     {"linear_full_slopes", (PyCFunction)(void (*)(void))py_linear_full_kept<Keep::kSteps>, METH_FASTCALL, nullptr},
     {"linear_full_grads", (PyCFunction)(void (*)(void))py_linear_full_grads, METH_FASTCALL, nullptr},
     {"dropout", (PyCFunction)(void (*)(void))py_dropout, METH_FASTCALL, nullptr},
+    {"dropout_grad", (PyCFunction)(void (*)(void))py_dropout_grad, METH_FASTCALL, nullptr},
     {"gated_sums", (PyCFunction)(void (*)(void))py_gated_sums, METH_FASTCALL, nullptr},
     {"norm_lengths", (PyCFunction)(void (*)(void))py_norm_lengths, METH_FASTCALL, nullptr},
     {"linear_grads", (PyCFunction)(void (*)(void))py_linear_grads, METH_FASTCALL, nullptr},

@@ -106,8 +106,9 @@ def _dropout_op(x: torch.Tensor, residual: _Maybe, p: float, seed: int, seed_at:
 
 
 @torch.library.custom_op("marlin_amd::dropout_grad", mutates_args=())
-def _dropout_grad_op(dy: torch.Tensor, p: float, seed: int, seed_at: _Maybe, site: int) -> torch.Tensor:
-    return _torch_binding.dropout(dy.resolve_neg(), None, p, seed if seed_at is None else seed_at, site, True)
+def _dropout_grad_op(dy: torch.Tensor, p: float, seed: int, seed_at: _Maybe, site: int,
+                     leaves: list[torch.Tensor]) -> torch.Tensor:
+    return _torch_binding.dropout_grad(dy, p, seed if seed_at is None else seed_at, site, *leaves)
 
 
 @_dropout_op.register_fake
@@ -116,18 +117,20 @@ def _dropout_fake(x, residual, p, seed, seed_at, site):
 
 
 @_dropout_grad_op.register_fake
-def _dropout_grad_fake(dy, p, seed, seed_at, site):
+def _dropout_grad_fake(dy, p, seed, seed_at, site, leaves):
     return dy.new_empty(dy.shape)
 
 
 def _keep_dropout(ctx, inputs, output):
-    _, _, ctx.p, ctx.seed, seed_at, ctx.site = inputs
-    ctx.save_for_backward(seed_at)
+    x, residual, ctx.p, ctx.seed, seed_at, ctx.site = inputs
+    ctx.save_for_backward(seed_at, *streamk._leaves(x, residual))
 
 
 def _dropout_backward(ctx, dy):
-    seed_at, = ctx.saved_tensors
-    dx = torch.ops.marlin_amd.dropout_grad(dy, ctx.p, ctx.seed, seed_at, ctx.site) if ctx.needs_input_grad[0] else None
+    seed_at, *leaves = ctx.saved_tensors
+    dx = None
+    if ctx.needs_input_grad[0]:
+        dx = torch.ops.marlin_amd.dropout_grad(dy, ctx.p, ctx.seed, seed_at, ctx.site, leaves)
     return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
 
 

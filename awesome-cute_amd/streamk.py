@@ -276,31 +276,36 @@ def _alone_fake(x, weight, bias, residual, act, p, seed, seed_at, site):
 
 @torch.library.custom_op("marlin_amd::linear_full_grads", mutates_args=())
 def _full_grads_op(dy: torch.Tensor, slopes: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act: int, p: float,
-                   seed: int, seed_at: _Maybe, site: int,
-                   want: list[bool]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                   seed: int, seed_at: _Maybe, site: int, want: list[bool],
+                   leaves: list[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     out = _torch_binding.linear_full_grads(dy, slopes if act else None, x, weight, act, p,
-                                           seed if seed_at is None else seed_at, site, *want)
+                                           seed if seed_at is None else seed_at, site, *want, *leaves)
     return tuple(x.new_empty(0) if g is None else g for g in out)
 
 
 @_full_grads_op.register_fake
-def _full_grads_fake(dy, slopes, x, weight, act, p, seed, seed_at, site, want):
+def _full_grads_fake(dy, slopes, x, weight, act, p, seed, seed_at, site, want, leaves):
     return (*_grads_fake(x, weight, want[0], want[1]), x.new_empty(weight.shape[0] if want[2] else 0))
 
 
 def _keep_full(ctx, inputs, output):
-    x, weight, _, _, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site, _ = inputs
-    # (both, whichever is needed: they are also the leaves that a captured backward pass looks at)
-    ctx.save_for_backward(x, weight, output[1], seed_at)
+    x, weight, bias, residual, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site, _ = inputs
+    # (both operands, whichever is needed: they are also among the leaves that a captured backward pass looks at)
+    ctx.save_for_backward(x, weight, output[1], seed_at, *_leaves(bias, residual))
+
+
+def _leaves(*tensors):
+    """Those that gradients are accumulated to."""
+    return [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
 
 
 def _full_backward(ctx, dy, _):
-    x, weight, slopes, seed_at = ctx.saved_tensors
+    x, weight, slopes, seed_at, *leaves = ctx.saved_tensors
     want = list(ctx.needs_input_grad[:4])  # (False of what is None)
     grads = (None,) * 3
     if any(want[:3]):
         grads = torch.ops.marlin_amd.linear_full_grads(dy, slopes, x, weight, ctx.act, ctx.p, ctx.seed, seed_at, ctx.site,
-                                                       want[:3])
+                                                       want[:3], leaves)
     return (*(g if w else None for g, w in zip(grads, want)), dy if want[3] else None, *(None,) * 6)
 
 

@@ -16,6 +16,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "awesome-cute_amd"))
 sys.path.insert(0, os.path.join(ROOT, "tests"))
 import _masks  # noqa: E402
+import feedforward  # noqa: E402,F401  (its operators)
 import streamk  # noqa: E402
 
 gpu = pytest.mark.gpu
@@ -276,20 +277,30 @@ def test_refusals_of_the_gradients_by_themselves():
 
 @gpu
 def test_a_captured_pass_of_an_operator_beside_an_eager_graph_of_its_leaves():
-    """The operator that compilers see looks at its operands, also at one that no gradient takes."""
+    """The operators that compilers see look at all that gradients go to, as the eager functions do."""
     x, w, bias, residual, dy = make(70, 72, 136, torch.float16, 6)
     side = torch.cuda.Stream()
-    for i in range(2):
-        inputs = [x, w]
-        inputs[i] = inputs[i].clone().requires_grad_()
+    full, dropout = torch.ops.marlin_amd.linear_full, torch.ops.marlin_amd.dropout
 
-        def forward():
-            return torch.ops.marlin_amd.linear_full(*inputs, bias, None, 1, 0.0, 0, None, 0, True)[0]
-
+    def beside(leaf, forward, others):
         alive = forward()
         with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
             with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
-                torch.autograd.grad(forward(), inputs[i], dy)
+                torch.autograd.grad(forward(), [leaf, *others], dy)
         torch.cuda.synchronize()
-        assert torch.isfinite(torch.autograd.grad(alive, inputs[i], dy)[0]).all()
-        del alive
+        assert torch.isfinite(torch.autograd.grad(alive, leaf, dy)[0]).all()
+
+    for i in range(4):
+        inputs = [x, w, bias, residual]
+        inputs[i] = inputs[i].clone().requires_grad_()
+        # (the residual's gradient alone takes no kernel: beside one that does, whose own graph is on the side stream)
+        with torch.cuda.stream(side):
+            other = bias.clone().requires_grad_()
+        torch.cuda.synchronize()
+        if i == 3:
+            beside(inputs[3], lambda: full(x, w, other if torch.cuda.current_stream() == side else bias, inputs[3], 1, 0.0, 0,
+                                           None, 0, True)[0], [other])
+        else:
+            beside(inputs[i], lambda: full(*inputs, 1, 0.0, 0, None, 0, True)[0], [])
+    leaf = dy.clone().requires_grad_()
+    beside(leaf, lambda: dropout(leaf, None, 0.5, 1, None, 0), [])
