@@ -7,8 +7,9 @@
 // results that all compute units write at once), and in the loop the board's power.  bfloat16, operands
 // from memory, us and TFLOP/s: 2048 x 2 x 10752 x 4096 296, 1220 (with the sums kept 313); its backward
 // pass 2048 x 4096 x 21504 267, 1350, in two slices that meet, and 21504 x 4096 x 2048 307, 1170;
-// 8192 x 4096 x 4096 205, 1340, with bias and residual 218.  The matrix pipe is in use for 57 to 72 % of these.  Results past the
-// caches or through them: level.
+// 8192 x 4096 x 4096 205, 1340, with bias and residual 226 to 230.  The matrix pipe is in use for 53 to 72 % of these.  Results
+// past the caches or through them: level, with what reads them next too (two products one after the other, an Mlp's
+// training step: 2 % to either side).
 //
 // A source for each type includes this: the kernels of one take the compiler a minute and more.
 #pragma once

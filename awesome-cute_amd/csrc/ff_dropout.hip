@@ -7,8 +7,8 @@
 //
 // Bound: HBM, or the last-level cache, which holds up to 256 MB of a call.  Operands are requested as read once
 // (nontemporal) where a call moves more than that cache holds: 16384 x 4096 bfloat16 with a residual, 403 MB, 61.2 us,
-// 6.6 TB/s (otherwise 70.3).  Where it moves less they are mostly there, just written by what came before, and such
-// requests would pass it by: 2048 x 10752 12.0 us (15.0), with operands that take turns 13.9.  Results are
+// 6.6 TB/s (otherwise 70.3).  Where it moves less they are mostly there, and such requests would pass it by: 2048 x 10752 13.8 us, 6.4
+// TB/s (16.2; of an operand that the call before has just written 13.9 and 14.2).  Results are
 // stored past the caches where they alone are more than the last one holds: 65536 x 4096 with a residual 249 us (261), and the norm that
 // reads it 222 (227).  Smaller ones are read from there next, and stored past it cost their reader more than they save
 // here: 2048 x 10752 13.6 us in place of 13.9, but with a product behind it 162 in place of 151, 16384 x 4096

@@ -10,7 +10,7 @@
 // factor of what is kept (rounded with it, gradients were 1.4 times as far off as their own rounding makes them) --, and the bias's gradient, its sum over rows, of the unrounded values in
 // fp32.  A workgroup takes 256 columns (fewer where there are fewer) of a run of rows, 16 bytes a
 // thread; its column sums meet in LDS and go to `partials`, and a second launch adds the runs' in their
-// order, unless there is one.  Bound: HBM, of small ones the launches: 2048 x 10752 with slopes 132 MB, 23 us,
+// order, unless there is one.  Bound: HBM, of small ones the launches: 2048 x 10752 with slopes 132 MB, 23.4 us,
 // 5.8 TB/s, and 4 us for the sums; four rows a thread at least and half the workgroups 25, eight rows 30.
 #include <hip/hip_runtime.h>
 

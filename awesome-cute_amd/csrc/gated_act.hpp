@@ -55,8 +55,8 @@ __device__ __forceinline__ float act_value(float g) { return g * act_sigma_of<AC
 // of a slope's size; 65535 less this for negative ones, and 49151, between the two, for NaN.  bfloat16: good to 2^-8
 // of a slope, what dy act' is rounded to, down to 2^-102.  fp16: to 2^-11 down to 2^-16, from there in
 // steps of 2^-26, no coarser than fp16 holds dy act' where dy is up to 4.  Nowhere off by more than 2^-16; zero and one
-// are exact.  The sums in 32 bits would take twice the bytes: 2048 x 10752 x 4096 12 us of 168 forward, and 14
-// of 40 backward.
+// are exact.  Both passes of 2048 x 10752 x 4096 take 477 us, with steps alone 473; the sums in 32 bits, twice the
+// bytes, took 12 more forward and 14 more backward.
 constexpr float kSlopeSteps = 32768.f;
 constexpr unsigned kSlopeBorder = 12288, kSlopeNan = 49151;  // codes
 template <bool BF>
