@@ -496,6 +496,16 @@ variable_list once_differentiable(variable_list&& grads, const char* name, std::
   return marked;
 }
 
+// What stands for the inputs of the node that runs, where the backward pass has not kept them: nothing but their edges
+variable_list inputs_of_the_node() {
+  variable_list out;
+  if (!c10::GradMode::is_enabled()) return out;
+  if (const auto node = torch::autograd::get_current_node())
+    for (const torch::autograd::Edge& edge : node->next_edges())
+      if (edge.is_valid()) torch::autograd::impl::set_gradient_edge(out.emplace_back(at::empty({0})), edge);
+  return out;
+}
+
 // Scratch for a product's partial sums, where its plan has any: its own, or memory that is there
 struct Room {
   at::Tensor t;
@@ -997,7 +1007,8 @@ struct FullFunction : torch::autograd::Function<FullFunction> {
       for (int i = 0; i < 3; i++) out[i] = g[i];
       if (kept->there[1] && ctx->needs_input_grad(2 + kept->there[0])) out[3] = grads[0];
     }
-    return once_differentiable(std::move(out), "linear", {&grads, &saved});
+    const variable_list inputs = inputs_of_the_node();
+    return once_differentiable(std::move(out), "linear", {&grads, &saved, &inputs});
   }
 };
 

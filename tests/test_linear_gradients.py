@@ -304,3 +304,23 @@ def test_a_captured_pass_of_an_operator_beside_an_eager_graph_of_its_leaves():
             beside(inputs[i], lambda: full(*inputs, 1, 0.0, 0, None, 0, True)[0], [])
     leaf = dy.clone().requires_grad_()
     beside(leaf, lambda: dropout(leaf, None, 0.5, 1, None, 0), [])
+
+
+@gpu
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_second_derivatives_raise_where_an_operand_is_not_kept(act):
+    """Also where another path leads to the input that the backward pass has not kept."""
+    m, n, k = 20, 24, 16
+    for wanted in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        for leaf in (True, False):
+            inputs = list(make(m, n, k, torch.float16, 1))
+            dy = inputs.pop()
+            roots = {i: inputs[i].requires_grad_() for i in wanted}
+            if not leaf:
+                for i in wanted:
+                    inputs[i] = roots[i] * 1
+            y = streamk.linear(*inputs[:3], act, inputs[3], dropout=0.25, seed=3)
+            for i in wanted:
+                g, = torch.autograd.grad(y, roots[i], dy, create_graph=True)
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    torch.autograd.grad(g.float().sum() + roots[i].float().sum(), roots[i], retain_graph=True)

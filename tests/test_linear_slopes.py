@@ -125,15 +125,15 @@ def test_slopes_of_every_size_by_every_tile(tile, slices):
             check_units(z, act, dy, torch.autograd.grad(y, leaf, dy)[0])
 
 
+FAR = [("silu", -4, 0.3), ("silu", -8, 1), ("silu", -12, 1), ("silu", -14, 1), ("gelu", -3.5, 0.2), ("gelu", -4.5, 0.3),
+       ("gelu", -5, 0.25)]
+FARTHER = [("silu", -16, 0.5), ("gelu", -7, 0.3)]  # (of these dz is below fp16's range)
+
+
 @gpu
-@pytest.mark.parametrize("type", TYPES)
-@pytest.mark.parametrize("act,mean,width", [("silu", -4, 0.3), ("silu", -8, 1), ("silu", -12, 1), ("silu", -14, 1),
-                                            ("silu", -16, 0.5), ("gelu", -3.5, 0.2), ("gelu", -4.5, 0.3), ("gelu", -5, 0.25),
-                                            ("gelu", -7, 0.3)])
 @pytest.mark.parametrize("m", [40, 300])
+@pytest.mark.parametrize("act,mean,width,type", [(*unit, type) for type in TYPES for unit in FAR + FARTHER * (type == torch.bfloat16)])
 def test_gradients_of_units_far_on_the_negative_side(m, act, mean, width, type):
-    if type == torch.float16 and (act, mean) in (("silu", -16), ("gelu", -7)):
-        pytest.skip("dz is below fp16's range")
     n, k = 72, 64
     gen = torch.Generator(device="cuda").manual_seed(m)
     x = torch.randn((m, k), device="cuda", generator=gen).to(type)
