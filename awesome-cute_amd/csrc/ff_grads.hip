@@ -6,8 +6,9 @@
 // products of the backward pass read them as they are (ff_tile.hpp).  Bound: HBM: 14 bytes for every element of dh.  2048 x 10752: 308 MB, 48 us, 6.4 TB/s.
 //
 // Of a full product, y = residual + drop(act(z)) with z = x W^T + bias: dz = drop(dy) act'(z), rounded to
-// 16 bits for the products -- without an activation dy or zero, exactly, where the products multiply by the
-// factor of what is kept (rounded with it, gradients were 1.4 times as far off as their own rounding makes them) --, and the bias's gradient, its sum over rows, of the unrounded values in
+// 16 bits for the products, without the factor of what is kept, by which these multiply their sums in fp32: so it is,
+// without an activation, dy or zero, exactly (rounded with the factor, gradients were 1.4 times as far off as their
+// own rounding makes them), and stays in fp16's range whatever the factor, and the bias's gradient, its sum over rows, of the unrounded values in
 // fp32.  A workgroup takes 256 columns (fewer where there are fewer) of a run of rows, 16 bytes a
 // thread; its column sums meet in LDS and go to `partials`, and a second launch adds the runs' in their
 // order, unless there is one.  Bound: HBM, of small ones the launches: 2048 x 10752 with slopes 132 MB, 23.4 us,

@@ -407,7 +407,7 @@ int run_linear_grad(bool steps, const void* dy, const void* slopes, void* dz, vo
   a.m = m, a.n = n;
   a.slope_steps = steps;
   a.bias_factor = 1.f;
-  if (factor && !slopes) {
+  if (factor) {
     *factor = a.bias_factor = a.drop.factor;
     a.drop.factor = 1.f;
   }

@@ -129,8 +129,8 @@ long long feedforward_linear_grad_bytes(int m, int n);
 /* The same two for training, with slopes that are good relative to their size as well, 16 bits each in the
  * library's own form: off by at most 2^-16, and in bfloat16 by at most 2^-8 of themselves down to 2^-102, in
  * fp16 by 2^-11 of themselves or 2^-27, whichever is more.  One's slopes are the other's alone.
- * With `factor`, a float in host memory, dz without slopes is dy or zero, exactly, and dz times *factor, the
- * mask's 1 / (1 - p), the gradient: for feedforward_product_scaled.  (*factor is 1 where there are slopes or no
+ * With `factor`, a float in host memory, what is kept enters dz as it is, without slopes exactly, and dz times
+ * *factor, the mask's 1 / (1 - p), is the gradient: for feedforward_product_scaled.  (*factor is 1 without a
  * mask; dbias is whole either way.) */
 int feedforward_linear_train(const void *x, const void *w, void *y, const void *bias, const void *residual,
                              void *slopes, int m, int n, int k, long long ldx, long long ldw, long long ldy,

@@ -72,12 +72,15 @@ def test_masked_gradients_are_not_rounded(m, n, k, p, type):
 
 
 @gpu
+@pytest.mark.parametrize("act", [None, "silu", "gelu"])
 @pytest.mark.parametrize("m", [4, 300])
-def test_a_factor_past_the_range_of_fp16(m):
-    """p = 1 - 2^-16: what is kept is multiplied by 65536, which dz in 16 bits would not hold."""
+def test_a_factor_past_the_range_of_fp16(m, act):
+    """p = 1 - 2^-16: what is kept is multiplied by 65536, which dz in 16 bits would not hold.  (Activations of arguments
+    above 30, whose slopes are one.)"""
     n, k, p = 4096, 64, 1 - 2.0 ** -16
     x = torch.ones((m, k), dtype=torch.float16, device="cuda")
     w = torch.full((n, k), 2.0 ** -12, dtype=torch.float16, device="cuda")
+    bias = torch.full((n,), 32.0, dtype=torch.float16, device="cuda")
     dy = torch.full((m, n), 4.0, dtype=torch.float16, device="cuda")
     dy[:, 1::2] = -2.0
     for seed in range(64):  # (one in 65536 is kept)
@@ -85,13 +88,13 @@ def test_a_factor_past_the_range_of_fp16(m):
         if keep.any():
             break
     assert keep.any()
-    leaves = [t.requires_grad_() for t in (x, w)]
-    dx, dw = torch.autograd.grad(streamk.linear(x, w, dropout=p, seed=seed), leaves, dy)
+    leaves = [t.requires_grad_() for t in (x, w, bias)]
+    dx, dw, db = torch.autograd.grad(streamk.linear(x, w, bias, act, dropout=p, seed=seed), leaves, dy)
     dz = dy.double() * keep * 65536
     # exact: powers of two, and few of them
     assert torch.equal(dx.double(), dz @ w.detach().double())
-    want = dz.t() @ x.detach().double()
-    assert torch.equal(dw.isinf(), want.abs() > 65504) and not dw.isnan().any()
+    for got, want in ((dw, dz.t() @ x.detach().double()), (db, dz.sum(0))):
+        assert torch.equal(got.isinf(), want.abs() > 65504) and not got.isnan().any()
 
 
 def product(a, b, m, n, k, turned, scale, room):
