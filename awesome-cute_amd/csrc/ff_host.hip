@@ -115,6 +115,8 @@ constexpr TileFit kFewFits[] = {
 // meet, cost some 10 us of 14 less where C is large, but the choice, and with it results' last bits, is as it was)
 constexpr double kSliceLaunch = 2.96, kSliceBytes = 0.327e-6;
 
+constexpr int kMostRows = 0x7ffffe00;  // of a product: rounded up to tiles they are an int
+
 struct ProductPlan {
   FfTile tile;
   int slices;  // 0: no tile computes the product in one launch
@@ -221,6 +223,7 @@ Planned plan_with_room(int m, int n, int k, Finish finish, Layout layout, int cu
       if (p.m == m && p.n == n && p.k == k && p.cus == cus && p.form == form) return p;
   Planned p;
   p.m = m, p.n = n, p.k = k, p.cus = cus, p.form = form;
+  if (m > kMostRows) return p;
   p.plan = choose_plan(m, n, k, finish, layout, cus, 1LL << 40);
   p.bytes = p.plan.slices > 1 ? 4LL * p.plan.slices * m * product_columns(n, gated) : 0;
   p.bytes = std::max(p.bytes, meeting(p.plan, m, product_columns(n, gated)).bytes);
@@ -281,8 +284,8 @@ bool layout_of(int turned, Layout* layout) {
 int run_product(ProductArgs a, Layout layout, bool bf, void* room, long long room_bytes, int dev, hipStream_t stream) {
   const bool gated = a.finish == kGated;
   const long long columns = product_columns(a.N, gated);
-  // (rows rounded up to tiles are an int, and the highest and widest tiles a launch: a plan takes such as are)
-  if (a.M > 0x7ffffe00 || (columns + 255) / 256 * ((a.M + 255) / 256) * 256 > kLaunchThreads)
+  // (the highest and widest tiles have to be a launch: a plan takes such as are)
+  if (a.M > kMostRows || (columns + 255) / 256 * ((a.M + 255) / 256) * 256 > kLaunchThreads)
     return fail(FEEDFORWARD_ERR_SHAPE, "m = %d and n = %d are too many tiles", a.M, a.N);
   // a gated product's rows of either half are addressed from one place
   if (gated && 2LL * a.N * a.ldb * 2 > 0x7fffffffLL)

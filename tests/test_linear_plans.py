@@ -51,6 +51,8 @@ def test_launches_at_the_limit():
     for gated in (0, 2):
         with pytest.raises(ValueError, match="too many"):
             streamk.product_plan(0x7ffffe00, 1024, 64, gated)
+        with pytest.raises(ValueError, match="too many"):
+            streamk.product_plan(0x7fffffff, 8, 64, gated)
     try:
         streamk.force_product_tile(64, 64)
         with pytest.raises(ValueError, match="too many"):
